@@ -186,6 +186,71 @@ int  lmrs_b200_weights_upload(int q_type, const void* wq, const float* ws, int n
 int  lmrs_b200_matmul_w(float* xout, const void* xq, const float* xs, const lmrs_b200_weights_t* w, int rows);
 void lmrs_b200_weights_free(lmrs_b200_weights_t* w);
 
+/* ---- many sequences at once (no reference counterpart: src/bin/backend.rs:87-110 keeps one Transformer, and one cache, per connection) ----------
+ * Keys and values of any number of sequences in pages of one pool, rows of a call appended to them with their rotary positions (one axis or
+ * several: time, height, width of image and video rows) applied on the way, and attention over them in which a prefix that all sequences share is
+ * read and computed once for all.  DEVICE pointers, on the caller's stream (a cudaStream_t; NULL: the legacy default stream) and the current
+ * device; nothing is allocated, kept or synchronised, so calls on several streams, and calls captured into CUDA graphs, do not meet anywhere but in the
+ * caller's own arrays.  dtype: 0 bfloat16, 1 float32, 2 float16, the same for all arrays of a call; angles, scores, softmax and sums are 32-bit or
+ * wider.  Strides count elements; the elements of a head lie next to each other.
+ *
+ * rope: pair j (of `pairs` <= 128) turns by positions[axis[j]] * freq[j] radians, whatever the position's size (positions are int32; the
+ * product is kept modulo a turn in 64 bits).  layout 0: pair j is elements j and j + pairs of a head; 1: elements 2j and 2j + 1.  Elements from
+ * 2 * pairs on pass unchanged.  rope_init fills the caller's struct (plain data, no ownership); axis NULL: one axis. */
+typedef struct lmrs_b200_rope {
+    uint64_t turns[128];   /* freq / 2 pi modulo 1, in 2^-64 */
+    uint8_t  axis[128];
+    int32_t  pairs, axes, layout;
+} lmrs_b200_rope_t;
+int lmrs_b200_rope_init(lmrs_b200_rope_t* out, const double* freq, const uint8_t* axis, int pairs, int layout);
+
+/* rows x heads x head_size elements, `row` and `head` elements from one row or head to the next */
+typedef struct lmrs_b200_rows {
+    void*   data;
+    int64_t row, head;
+} lmrs_b200_rows_t;
+/* int32 positions: axis a of row r at data[a * axis + r * row] */
+typedef struct lmrs_b200_positions {
+    const int32_t* data;
+    int64_t axis, row;
+} lmrs_b200_positions_t;
+/* out = x turned by its rows' positions; out may be x itself */
+int lmrs_b200_rope_axes(const lmrs_b200_rope_t* rope, int dtype, const lmrs_b200_rows_t* x, const lmrs_b200_rows_t* out, int64_t n_rows, int heads, int head_size,
+                        const lmrs_b200_positions_t* pos, void* stream);
+
+/* the pool: keys k[page][slot][head][head_size] and values v, strides k_page, k_slot, k_head and v_... in elements */
+typedef struct lmrs_b200_pages {
+    void *  k, *v;
+    int64_t k_page, k_slot, k_head, v_page, v_slot, v_head;
+    int32_t pages, page_size, kv_heads, head_size, dtype;
+} lmrs_b200_pages_t;
+/* the sequences of a call.  Sequence b holds lens[b] tokens, those of the call included, which are its last: rows rows[b] .. rows[b + 1] of the call's
+ * arrays (rows NULL: row b alone), so that row i of its c has index lens[b] - c + i.  Token x lies in slot x % page_size of page
+ * tables[b * table_stride + x / page_size].  A row whose index is negative is padding; rows from rows[seqs] on are not touched.
+ * The prefix_len tokens of the pages that `prefix` lists come before every sequence's own (prefix NULL: none).
+ * lens, rows, tables and prefix are int32 in device memory and read by the kernels, so a captured call follows what is written there.  An entry of
+ * tables or prefix outside 0 .. pages - 1 is no page: what would lie there is neither written nor seen, nor is what lies beyond table_len pages.
+ * max_rows: most rows of one sequence (it chooses the kernels, no result depends on it). */
+typedef struct lmrs_b200_batch {
+    const int32_t *lens, *rows, *tables, *prefix;
+    int64_t table_stride;
+    int32_t seqs, table_len, max_rows, prefix_len;
+} lmrs_b200_batch_t;
+/* Writes the rows k and v [n_rows][kv_heads][head_size] to their places in the pages, k turned; with q, also q_out = q turned ([n_rows][q_heads]
+ * [head_size]; q_out may be q).  rope NULL: nothing is turned (then q is refused).  pos NULL: the position of a row is prefix_len + its index on every axis.
+ * Padding rows are turned in q_out and written nowhere else.  Two rows with one place: either's elements. */
+int lmrs_b200_paged_append(const lmrs_b200_pages_t* pages, const lmrs_b200_batch_t* batch, int64_t n_rows, const lmrs_b200_rows_t* k, const lmrs_b200_rows_t* v,
+                           const lmrs_b200_rope_t* rope, const lmrs_b200_positions_t* pos, const lmrs_b200_rows_t* q, const lmrs_b200_rows_t* q_out, int q_heads, void* stream);
+/* out = softmax(scale * q . keys) . values for every row: the prefix, and the row's own sequence up to the row's index.  q head h reads KV head
+ * h / (q_heads / kv_heads).  softcap > 0: scores become softcap * tanh(score / softcap).  lse (NULL, or f32 [n_rows][q_heads]): the logarithm of the sum
+ * of the exponentials.  A row that sees nothing (padding rows see no prefix either): out 0, lse -infinity.  head_size: a multiple of 8, at most 256;
+ * k, v and their strides on 16-byte boundaries.  workspace: device memory of the size that paged_attention_workspace gives for
+ * the same pages, batch (its host fields), n_rows and q_heads, on a 256-byte boundary; its contents do not matter before the call and mean nothing after it.  Calls
+ * that may run at the same time need one each. */
+int lmrs_b200_paged_attention_workspace(const lmrs_b200_pages_t* pages, const lmrs_b200_batch_t* batch, int64_t n_rows, int q_heads, size_t* bytes);
+int lmrs_b200_paged_attention(const lmrs_b200_pages_t* pages, const lmrs_b200_batch_t* batch, int64_t n_rows, const lmrs_b200_rows_t* q, const lmrs_b200_rows_t* out,
+                              int q_heads, float scale, float softcap, float* lse, void* workspace, size_t workspace_bytes, void* stream);
+
 const char* lmrs_b200_last_error(void);
 /* "lmrs_b200 <version> sm_100a" */
 const char* lmrs_b200_version(void);

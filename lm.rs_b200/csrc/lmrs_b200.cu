@@ -45,6 +45,7 @@ static thread_local std::string g_err;
 extern "C" const char* lmrs_b200_last_error(void) { return g_err.c_str(); }
 extern "C" const char* lmrs_b200_version(void) { return "lmrs_b200 0.1 sm_100a"; }
 static int fail(const std::string& m) { g_err = m; return 1; }
+namespace lmrs { int set_error(const std::string& m) { return fail(m); } }   // (declared in paged.h)
 
 #define CK(call)                                                                                   \
     do {                                                                                           \

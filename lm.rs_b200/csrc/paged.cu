@@ -1,0 +1,255 @@
+// paged.cu -- entry points of include/lmrs_b200.h for many sequences at once: checks of the arguments, choice of the kernels, launches.
+// Device pointers, the caller's stream; nothing here allocates, synchronises or remembers anything from one call to the next.
+#include <math.h>
+
+#include <string>
+
+#include "paged_attn.cuh"
+#include "paged_rows.cuh"
+
+using namespace lmrs;
+using namespace lmrs::paged;
+
+namespace {
+
+int refuse(const char* where, const std::string& why) { return set_error(std::string("lmrs_b200_") + where + ": " + why); }
+
+int launched(const char* where) {
+    const cudaError_t e = cudaGetLastError();
+    return e == cudaSuccess ? 0 : refuse(where, std::string("launch failed: ") + cudaGetErrorString(e));
+}
+
+// the current device: its number of SMs, or 0 with an error set
+int device_sms(const char* where, int* device) {
+    int n = 0, major = 0, sms = 0;
+    if (cudaGetDeviceCount(&n) != cudaSuccess || n == 0) {
+        cudaGetLastError();
+        refuse(where, "no CUDA device available (this library has no CPU fallback)");
+        return 0;
+    }
+    if (cudaGetDevice(device) != cudaSuccess || cudaDeviceGetAttribute(&major, cudaDevAttrComputeCapabilityMajor, *device) != cudaSuccess ||
+        cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, *device) != cudaSuccess || major != 10) {
+        cudaGetLastError();
+        refuse(where, "the current device is not sm_100; this library contains sm_100a code only");
+        return 0;
+    }
+    return sms;
+}
+// a pointer that kernels on the current device may follow
+bool on_device(const void* p, int device) {
+    cudaPointerAttributes a;
+    if (cudaPointerGetAttributes(&a, p) != cudaSuccess) { cudaGetLastError(); return false; }
+    return (a.type == cudaMemoryTypeDevice && a.device == device) || a.type == cudaMemoryTypeManaged;
+}
+bool aligned(const void* p, size_t n) { return (uintptr_t)p % n == 0; }
+size_t size_of(int dtype) { return dtype == 1 ? 4 : 2; }
+template <typename F> int by_type(int dtype, F f) {
+    return dtype == 0 ? f(__nv_bfloat16()) : dtype == 1 ? f(float()) : f(__half());
+}
+template <typename T> Rows<T> rows_as(const lmrs_b200_rows_t* r) { return Rows<T>{(T*)r->data, r->row, r->head}; }
+Positions pos_as(const lmrs_b200_positions_t* p) { return p ? Positions{p->data, p->axis, p->row} : Positions{nullptr, 0, 0}; }
+
+std::string bad_dtype(int dtype) { return dtype < 0 || dtype > 2 ? "dtype must be 0 (bfloat16), 1 (float32) or 2 (float16)" : ""; }
+std::string bad_rows(const lmrs_b200_rows_t* r, const char* name, int dtype, int device) {
+    if (!r || !r->data) return std::string("null ") + name;
+    if (!aligned(r->data, size_of(dtype))) return std::string(name) + " does not lie on a boundary of its elements";
+    if (r->row < 0 || r->head < 0) return std::string("negative stride of ") + name;
+    if (!on_device(r->data, device)) return std::string(name) + " is not memory of the current device";
+    return "";
+}
+std::string bad_ints(const int32_t* p, const char* name, int device) {
+    if (!aligned(p, 4)) return std::string(name) + " does not lie on a boundary of its elements";
+    return on_device(p, device) ? "" : std::string(name) + " is not memory of the current device";
+}
+std::string bad_rope(const lmrs_b200_rope_t* r, int head_size) {
+    if (r->pairs < 1 || r->pairs > 128 || r->axes < 1 || (r->layout != 0 && r->layout != 1)) return "rope was not filled by lmrs_b200_rope_init";
+    return 2 * r->pairs > head_size ? "rope turns " + std::to_string(2 * r->pairs) + " elements, head_size is " + std::to_string(head_size) : "";
+}
+std::string bad_pages(const lmrs_b200_pages_t* p) {
+    if (!p || !p->k || !p->v) return "null pages";
+    const std::string why = bad_dtype(p->dtype);
+    if (!why.empty()) return why;
+    if (p->pages < 1 || p->page_size < 1 || p->kv_heads < 1) return "pages, page_size and kv_heads must be positive";
+    if (p->head_size < 1 || p->head_size > 256) return "head_size must be 1 .. 256";
+    if (p->k_page < 0 || p->k_slot < 0 || p->k_head < 0 || p->v_page < 0 || p->v_slot < 0 || p->v_head < 0) return "negative stride of pages";
+    return "";
+}
+std::string bad_batch(const lmrs_b200_batch_t* b, int64_t n_rows, int page_size) {
+    if (!b) return "null batch";
+    if (b->seqs < 0 || n_rows < 0 || n_rows > 0x7fffffff) return "seqs and n_rows must be 0 .. 2^31 - 1";
+    if (b->table_len < 0 || b->table_stride < 0) return "negative table_len or table_stride";
+    if (b->prefix_len < 0 || (b->prefix_len > 0 && !b->prefix)) return "prefix_len without prefix";
+    if ((int64_t)b->table_len * page_size + b->prefix_len > 0x7fffffff) return "prefix_len + table_len * page_size is beyond 2^31 - 1";
+    if (b->seqs > 0 && (!b->lens || (b->table_len > 0 && !b->tables))) return "null lens or tables";
+    if (b->max_rows < 1 && n_rows > 0) return "max_rows must be positive";
+    if (!b->rows && n_rows != b->seqs) return "without rows, n_rows must be seqs (one row each)";
+    return "";
+}
+std::string bad_batch_memory(const lmrs_b200_batch_t* b, int device) {
+    std::string why = bad_ints(b->lens, "lens", device);
+    if (why.empty() && b->rows) why = bad_ints(b->rows, "rows", device);
+    if (why.empty() && b->table_len) why = bad_ints(b->tables, "tables", device);
+    if (why.empty() && b->prefix_len) why = bad_ints(b->prefix, "prefix", device);
+    return why;
+}
+Batch batch_as(const lmrs_b200_batch_t* b, const lmrs_b200_pages_t* p, int64_t n_rows) {
+    return Batch{b->lens, b->rows, b->tables, b->prefix, b->table_stride, b->seqs, b->table_len, b->prefix_len, p->pages, p->page_size, n_rows};
+}
+template <typename F> int guarded(const char* where, F f) {   // no exception leaves a C entry point
+    try {
+        return f();
+    } catch (...) {
+        try { return refuse(where, "out of host memory"); } catch (...) { return 1; }
+    }
+}
+unsigned row_grid(int64_t n_rows) { return (unsigned)n_rows; }
+
+}  // namespace
+
+extern "C" int lmrs_b200_rope_init(lmrs_b200_rope_t* out, const double* freq, const uint8_t* axis, int pairs, int layout) {
+    return guarded("rope_init", [&]() -> int {
+        if (!out || !freq) return refuse("rope_init", "null argument");
+        if (pairs < 1 || pairs > 128) return refuse("rope_init", "pairs must be 1 .. 128");
+        if (layout != 0 && layout != 1) return refuse("rope_init", "layout must be 0 (halves) or 1 (neighbours)");
+        lmrs_b200_rope_t r = {};
+        r.pairs = pairs;
+        r.layout = layout;
+        for (int j = 0; j < pairs; j++) {
+            if (!isfinite(freq[j])) return refuse("rope_init", "a frequency is not finite");
+            const long double turns = (long double)freq[j] / 6.283185307179586476925286766559005768L, part = turns - floorl(turns);
+            const long double scaled = floorl(ldexpl(part, 64) + 0.5L);
+            r.turns[j] = scaled >= ldexpl(1.0L, 64) ? 0 : (uint64_t)scaled;   // (a whole turn is none)
+            r.axis[j] = axis ? axis[j] : 0;
+            if (r.axis[j] >= r.axes) r.axes = r.axis[j] + 1;
+        }
+        *out = r;
+        return 0;
+    });
+}
+
+extern "C" int lmrs_b200_rope_axes(const lmrs_b200_rope_t* rope, int dtype, const lmrs_b200_rows_t* x, const lmrs_b200_rows_t* out, int64_t n_rows, int heads,
+                                   int head_size, const lmrs_b200_positions_t* pos, void* stream) {
+    static const char* me = "rope_axes";
+    return guarded(me, [&]() -> int {
+        if (!rope || !x || !out || !pos) return refuse(me, "null argument");
+        std::string why = bad_dtype(dtype);
+        if (!why.empty()) return refuse(me, why);
+        if (n_rows < 0 || n_rows > 0x7fffffff || heads < 0 || head_size < 1 || head_size > 256) return refuse(me, "n_rows and heads must be 0 .. 2^31 - 1, head_size 1 .. 256");
+        why = bad_rope(rope, head_size);
+        if (!why.empty()) return refuse(me, why);
+        int device = 0;
+        if (!device_sms(me, &device)) return 1;
+        if (n_rows == 0 || heads == 0) return 0;
+        why = bad_rows(x, "x", dtype, device);
+        if (why.empty()) why = bad_rows(out, "out", dtype, device);
+        if (why.empty()) why = !pos->data ? "null positions" : bad_ints(pos->data, "positions", device);
+        if (!why.empty()) return refuse(me, why);
+        return by_type(dtype, [&](auto t) {
+            using T = decltype(t);
+            rope_axes_kernel<T><<<row_grid(n_rows), 256, 0, (cudaStream_t)stream>>>(*rope, rows_as<const T>(x), rows_as<T>(out), n_rows, heads, head_size, pos_as(pos));
+            return launched(me);
+        });
+    });
+}
+
+extern "C" int lmrs_b200_paged_append(const lmrs_b200_pages_t* pages, const lmrs_b200_batch_t* batch, int64_t n_rows, const lmrs_b200_rows_t* k, const lmrs_b200_rows_t* v,
+                                      const lmrs_b200_rope_t* rope, const lmrs_b200_positions_t* pos, const lmrs_b200_rows_t* q, const lmrs_b200_rows_t* q_out, int q_heads,
+                                      void* stream) {
+    static const char* me = "paged_append";
+    return guarded(me, [&]() -> int {
+        std::string why = bad_pages(pages);
+        if (why.empty()) why = bad_batch(batch, n_rows, pages->page_size);
+        if (why.empty() && (q || q_out) && (!q || !q_out)) why = "q and q_out come together";
+        if (why.empty() && q && !rope) why = "q without rope";
+        if (why.empty() && q && q_heads < 1) why = "q_heads must be positive";
+        if (why.empty() && rope) why = bad_rope(rope, pages->head_size);
+        if (!why.empty()) return refuse(me, why);
+        int device = 0;
+        if (!device_sms(me, &device)) return 1;
+        if (n_rows == 0 || batch->seqs == 0) return 0;
+        const int dtype = pages->dtype;
+        why = bad_batch_memory(batch, device);
+        if (why.empty()) why = bad_rows(k, "k", dtype, device);
+        if (why.empty()) why = bad_rows(v, "v", dtype, device);
+        if (why.empty() && q) why = bad_rows(q, "q", dtype, device);
+        if (why.empty() && q) why = bad_rows(q_out, "q_out", dtype, device);
+        if (why.empty() && pos) why = !pos->data ? "null positions" : bad_ints(pos->data, "positions", device);
+        if (why.empty() && (!on_device(pages->k, device) || !on_device(pages->v, device))) why = "the pages are not memory of the current device";
+        if (!why.empty()) return refuse(me, why);
+        return by_type(dtype, [&](auto t) {
+            using T = decltype(t);
+            AppendParams<T> p = {};
+            if (rope) p.rope = *rope;
+            p.batch = batch_as(batch, pages, n_rows);
+            p.pos = pos_as(rope ? pos : nullptr);
+            p.k = rows_as<const T>(k);
+            p.v = rows_as<const T>(v);
+            if (q) { p.q = rows_as<const T>(q); p.q_out = rows_as<T>(q_out); p.q_heads = q_heads; }
+            p.k_pages = (T*)pages->k; p.v_pages = (T*)pages->v;
+            p.k_page = pages->k_page; p.k_slot = pages->k_slot; p.k_head = pages->k_head;
+            p.v_page = pages->v_page; p.v_slot = pages->v_slot; p.v_head = pages->v_head;
+            p.kv_heads = pages->kv_heads; p.head_size = pages->head_size;
+            paged_append_kernel<T><<<row_grid(n_rows), 256, 0, (cudaStream_t)stream>>>(p);
+            return launched(me);
+        });
+    });
+}
+
+static std::string bad_attention(const lmrs_b200_pages_t* pages, const lmrs_b200_batch_t* batch, int64_t n_rows, int q_heads) {
+    std::string why = bad_pages(pages);
+    if (why.empty()) why = bad_batch(batch, n_rows, pages->page_size);
+    if (!why.empty()) return why;
+    const int64_t vec = 16 / (int64_t)size_of(pages->dtype);
+    if (pages->head_size % 8) return "head_size must be a multiple of 8";
+    if (q_heads < 1 || q_heads % pages->kv_heads) return "q_heads must be a positive multiple of kv_heads";
+    if (!aligned(pages->k, 16) || !aligned(pages->v, 16) || pages->k_page % vec || pages->k_slot % vec || pages->k_head % vec || pages->v_page % vec || pages->v_slot % vec ||
+        pages->v_head % vec)
+        return "the pages' rows must lie on 16-byte boundaries";
+    return "";
+}
+
+extern "C" int lmrs_b200_paged_attention_workspace(const lmrs_b200_pages_t* pages, const lmrs_b200_batch_t* batch, int64_t n_rows, int q_heads, size_t* bytes) {
+    static const char* me = "paged_attention_workspace";
+    return guarded(me, [&]() -> int {
+        if (!bytes) return refuse(me, "null argument");
+        const std::string why = bad_attention(pages, batch, n_rows, q_heads);
+        if (!why.empty()) return refuse(me, why);
+        *bytes = 0;
+        return 0;
+    });
+}
+
+extern "C" int lmrs_b200_paged_attention(const lmrs_b200_pages_t* pages, const lmrs_b200_batch_t* batch, int64_t n_rows, const lmrs_b200_rows_t* q, const lmrs_b200_rows_t* out,
+                                         int q_heads, float scale, float softcap, float* lse, void* workspace, size_t workspace_bytes, void* stream) {
+    static const char* me = "paged_attention";
+    return guarded(me, [&]() -> int {
+        std::string why = bad_attention(pages, batch, n_rows, q_heads);
+        if (why.empty() && !isfinite(scale)) why = "scale is not finite";
+        if (why.empty() && !(softcap >= 0.0f && isfinite(softcap))) why = "softcap must be 0 (none) or positive";
+        if (!why.empty()) return refuse(me, why);
+        int device = 0;
+        if (!device_sms(me, &device)) return 1;
+        if (n_rows == 0 || batch->seqs == 0) return 0;
+        const int dtype = pages->dtype;
+        why = bad_batch_memory(batch, device);
+        if (why.empty()) why = bad_rows(q, "q", dtype, device);
+        if (why.empty()) why = bad_rows(out, "out", dtype, device);
+        if (why.empty() && lse && (!aligned(lse, 4) || !on_device(lse, device))) why = "lse is not memory of the current device";
+        if (why.empty() && (!on_device(pages->k, device) || !on_device(pages->v, device))) why = "the pages are not memory of the current device";
+        if (!why.empty()) return refuse(me, why);
+        return by_type(dtype, [&](auto t) {
+            using T = decltype(t);
+            AttnParams<T> p = {};
+            p.batch = batch_as(batch, pages, n_rows);
+            p.q = rows_as<const T>(q);
+            p.out = rows_as<T>(out);
+            p.k = (const T*)pages->k; p.v = (const T*)pages->v;
+            p.k_page = pages->k_page; p.k_slot = pages->k_slot; p.k_head = pages->k_head;
+            p.v_page = pages->v_page; p.v_slot = pages->v_slot; p.v_head = pages->v_head;
+            p.kv_heads = pages->kv_heads; p.q_heads = q_heads; p.head_size = pages->head_size;
+            p.scale = scale; p.softcap = softcap; p.lse = lse;
+            paged_attention_kernel<T><<<dim3(row_grid(n_rows), (unsigned)q_heads), 128, 0, (cudaStream_t)stream>>>(p);
+            return launched(me);
+        });
+    });
+}

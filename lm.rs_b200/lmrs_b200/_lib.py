@@ -17,6 +17,7 @@ ABI_SYMBOLS = [
     "lmrs_b200_quantize_q8", "lmrs_b200_quantize_q4", "lmrs_b200_rmsnorm", "lmrs_b200_softmax", "lmrs_b200_layernorm",
     "lmrs_b200_weights_upload", "lmrs_b200_matmul_w", "lmrs_b200_weights_free",
     "lmrs_b200_open", "lmrs_b200_forward_tokens", "lmrs_b200_set_option",
+    "lmrs_b200_rope_init", "lmrs_b200_rope_axes", "lmrs_b200_paged_append", "lmrs_b200_paged_attention", "lmrs_b200_paged_attention_workspace",
     "lmrs_b200_last_error", "lmrs_b200_version",
 ]
 
@@ -87,6 +88,12 @@ def lib():
     L.lmrs_b200_matmul_w.argtypes = [vp, vp, vp, vp, i]
     L.lmrs_b200_weights_free.argtypes = [vp]
     L.lmrs_b200_weights_free.restype = None
+    i64 = C.c_int64
+    L.lmrs_b200_rope_init.argtypes = [vp, vp, vp, i, i]
+    L.lmrs_b200_rope_axes.argtypes = [vp, i, vp, vp, i64, i, i, vp, vp]
+    L.lmrs_b200_paged_append.argtypes = [vp, vp, i64] + [vp] * 6 + [i, vp]
+    L.lmrs_b200_paged_attention_workspace.argtypes = [vp, vp, i64, i, C.POINTER(sz)]
+    L.lmrs_b200_paged_attention.argtypes = [vp, vp, i64, vp, vp, i, C.c_float, C.c_float, vp, vp, sz, vp]
     L.lmrs_b200_open.argtypes = [C.c_char_p, i, i, u32, C.POINTER(vp)]
     L.lmrs_b200_forward_tokens.argtypes = [vp, vp, sz, u32, vp, sz, vp]
     L.lmrs_b200_set_option.argtypes = [vp, C.c_char_p, i]

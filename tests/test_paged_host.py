@@ -1,0 +1,144 @@
+"""Many sequences at once: what needs no GPU -- the rotary tables, and every call that the library has to refuse (nothing is launched)."""
+import ctypes as C
+import math
+
+import pytest
+
+torch = pytest.importorskip("torch")
+
+
+@pytest.fixture(scope="module")
+def paged(gpu_lib):
+    from lmrs_b200 import paged
+    return paged
+
+
+def test_turns_are_the_frequencies_modulo_a_turn(paged):
+    freq = [1.0, 0.5, 1e-6, 0.0, 7.0, -0.25, 2 * math.pi]
+    r = paged.RopeAxes(freq, [0, 1, 2, 0, 1, 2, 0], layout="pairs")
+    assert (r.pairs, r.axes, r._c.pairs, r._c.axes, r._c.layout) == (7, 3, 7, 3, 1)
+    for j, f in enumerate(freq):
+        turns = r._c.turns[j] / 2.0 ** 64
+        want = (f / (2 * math.pi)) % 1.0
+        assert min(abs(turns - want), 1 - abs(turns - want)) < 2.0 ** -52
+    assert list(r._c.axis[:7]) == [0, 1, 2, 0, 1, 2, 0]
+
+
+def test_sections(paged):
+    assert list(paged.RopeAxes.sections(16, 1e4, [2, 3, 3])._c.axis[:8]) == [0, 0, 1, 1, 1, 2, 2, 2]
+    assert list(paged.RopeAxes.sections(16, 1e4, [1, 3, 4], order="cycle")._c.axis[:8]) == [0, 1, 2, 1, 2, 1, 2, 2]
+    assert paged.RopeAxes.sections(64, 1e4).axes == 1
+    for bad in (dict(rot=15), dict(rot=16, sections=[4, 5]), dict(rot=16, sections=[9, -1]), dict(rot=16, order="x"), dict(rot=0), dict(rot=258)):
+        with pytest.raises(paged.LmrsError):
+            paged.RopeAxes.sections(**{"theta": 1e4, **bad})
+    for freq, axis, layout in (([], None, "halves"), ([1.0] * 129, None, "halves"), ([math.inf], None, "halves"), ([math.nan], None, "pairs"), ([1.0], [256], "halves"),
+                               ([1.0], [-1], "halves"), ([1.0], [0, 0], "halves"), ([1.0], None, "thirds")):
+        with pytest.raises(paged.LmrsError):
+            paged.RopeAxes(freq, axis, layout)
+
+
+def test_host_tensors_are_refused(paged):
+    x, pos = torch.zeros(2, 3, 8), torch.zeros(2, dtype=torch.int32)
+    rope = paged.RopeAxes([1.0])
+    with pytest.raises(paged.LmrsError, match="GPU"):
+        paged.rope_axes(x, pos, rope)
+    with pytest.raises(paged.LmrsError, match="GPU"):
+        paged.KVPages(torch.zeros(1, 1, 1, 8), torch.zeros(1, 1, 1, 8))
+    with pytest.raises(paged.LmrsError, match="GPU"):
+        paged.Batch(pos, pos[:, None])
+    for bad in (lambda: paged.rope_axes(x.numpy(), pos, rope), lambda: paged.rope_axes(x, pos, None), lambda: paged.KVPages(None, None), lambda: paged.Batch(None, None)):
+        with pytest.raises(paged.LmrsError):
+            bad()
+
+
+def test_disjoint(paged):
+    t = torch.zeros(4, 6, 8)
+    assert paged._disjoint(t) and paged._disjoint(t.transpose(0, 1)) and paged._disjoint(t[:, ::2]) and paged._disjoint(t[:1].expand(1, 6, 8)) and paged._disjoint(t[:0])
+    assert not paged._disjoint(t[:1].expand(4, 6, 8)) and not paged._disjoint(torch.zeros(100).as_strided((4, 6, 8), (4, 8, 1)))
+
+
+# ---- the C entry points: pointers that nothing may follow, because every one of these calls is refused before a launch ----
+P = 4096   # an aligned address
+
+
+def _pages(paged, **kw):
+    p = paged._Pages(P, P, 16 * 2 * 64, 2 * 64, 64, 16 * 2 * 64, 2 * 64, 64, 8, 16, 2, 64, 0)
+    for k, v in kw.items():
+        setattr(p, k, v)
+    return p
+
+
+def _batch(paged, **kw):
+    b = paged._Batch(P, None, P, None, 4, 3, 4, 1, 0)
+    for k, v in kw.items():
+        setattr(b, k, v)
+    return b
+
+
+BAD_PAGES = [dict(k=None), dict(v=None), dict(dtype=3), dict(dtype=-1), dict(pages=0), dict(page_size=0), dict(kv_heads=0), dict(head_size=0), dict(head_size=257), dict(k_slot=-1), dict(v_head=-64)]
+BAD_BATCH = [dict(seqs=-1), dict(lens=None), dict(tables=None), dict(table_len=-1), dict(table_stride=-1), dict(prefix_len=-1), dict(prefix_len=1), dict(table_len=1 << 30),
+             dict(prefix_len=2 ** 31 - 1, prefix=P), dict(max_rows=0), dict(seqs=2), dict(seqs=4)]
+
+
+@pytest.mark.parametrize("pages, batch", [(p, {}) for p in BAD_PAGES] + [({}, b) for b in BAD_BATCH], ids=str)
+def test_bad_pages_and_batches(paged, gpu_lib, pages, batch):
+    L = gpu_lib.lib()
+    pg, bt, rows = _pages(paged, **pages), _batch(paged, **batch), paged._Rows(P, 256, 64)
+    r, size = C.byref(rows), C.c_size_t()
+    assert L.lmrs_b200_paged_append(C.byref(pg), C.byref(bt), 3, r, r, None, None, None, None, 0, None)
+    assert b"no CUDA device" not in L.lmrs_b200_last_error()
+    assert L.lmrs_b200_paged_attention(C.byref(pg), C.byref(bt), 3, r, r, 4, 0.125, 0.0, None, P, 1 << 30, None)
+    assert b"no CUDA device" not in L.lmrs_b200_last_error()
+    assert L.lmrs_b200_paged_attention_workspace(C.byref(pg), C.byref(bt), 3, 4, C.byref(size))
+
+
+def test_bad_attention(paged, gpu_lib):
+    L = gpu_lib.lib()
+    rows, size = paged._Rows(P, 256, 64), C.c_size_t()
+    r = C.byref(rows)
+
+    def attend(heads=4, scale=0.125, cap=0.0, n=3, **pages):
+        pg, bt = _pages(paged, **pages), _batch(paged)
+        assert L.lmrs_b200_paged_attention(C.byref(pg), C.byref(bt), n, r, r, heads, scale, cap, None, P, 1 << 30, None)
+        return L.lmrs_b200_last_error()
+
+    for kw in (dict(heads=0), dict(heads=3), dict(heads=-2), dict(scale=math.inf), dict(scale=math.nan), dict(cap=-1.0), dict(cap=math.nan), dict(cap=math.inf), dict(head_size=60), dict(k=P + 2),
+               dict(v=P + 8), dict(k_slot=132), dict(v_head=4), dict(v_page=2049), dict(n=-1), dict(n=2 ** 31)):
+        assert b"no CUDA device" not in attend(**kw), kw
+    assert L.lmrs_b200_paged_attention_workspace(None, None, 3, 4, C.byref(size)) and L.lmrs_b200_paged_attention(None, None, 3, r, r, 4, 1.0, 0.0, None, None, 0, None)
+    pg, bt = _pages(paged), _batch(paged)
+    assert L.lmrs_b200_paged_attention_workspace(C.byref(pg), C.byref(bt), 3, 4, None)
+    assert L.lmrs_b200_paged_attention_workspace(C.byref(pg), C.byref(bt), 3, 4, C.byref(size)) == 0   # needs no GPU
+
+
+def test_bad_appends_and_rotations(paged, gpu_lib):
+    L = gpu_lib.lib()
+    rope, wide = paged.RopeAxes([1.0] * 32)._c, paged.RopeAxes([1.0] * 33)._c
+    pg, bt, rows, pos = _pages(paged), _batch(paged), paged._Rows(P, 256, 64), paged._Positions(P, 3, 1)
+    r, empty = C.byref(rows), paged._Rope()
+
+    def append(rope, q, q_out, heads):
+        assert L.lmrs_b200_paged_append(C.byref(pg), C.byref(bt), 3, r, r, rope, None, q, q_out, heads, None)
+        return L.lmrs_b200_last_error()
+
+    for args in ((C.byref(rope), r, None, 4), (C.byref(rope), None, r, 4), (None, r, r, 4), (C.byref(rope), r, r, 0), (C.byref(wide), None, None, 0), (C.byref(empty), None, None, 0)):
+        assert b"no CUDA device" not in append(*args)
+
+    def turn(rope=C.byref(rope), dtype=0, x=r, out=r, n=3, heads=4, size=64, pos=C.byref(pos)):
+        assert L.lmrs_b200_rope_axes(rope, dtype, x, out, n, heads, size, pos, None)
+        return L.lmrs_b200_last_error()
+
+    for kw in (dict(rope=None), dict(rope=C.byref(wide)), dict(rope=C.byref(empty)), dict(dtype=3), dict(x=None), dict(out=None), dict(pos=None), dict(n=-1), dict(heads=-1), dict(size=0), dict(size=257),
+               dict(size=63)):
+        assert b"no CUDA device" not in turn(**kw), kw
+
+
+def test_every_refusal_without_a_gpu_says_so(paged, gpu_lib):
+    if torch.cuda.is_available():
+        pytest.skip("a GPU is there")
+    L = gpu_lib.lib()
+    pg, bt, rows, pos, rope = _pages(paged), _batch(paged), paged._Rows(P, 256, 64), paged._Positions(P, 3, 1), paged.RopeAxes([1.0] * 32)._c
+    r = C.byref(rows)
+    assert L.lmrs_b200_paged_attention(C.byref(pg), C.byref(bt), 3, r, r, 4, 0.125, 0.0, None, P, 1 << 30, None) and b"no CUDA device" in L.lmrs_b200_last_error()
+    assert L.lmrs_b200_paged_append(C.byref(pg), C.byref(bt), 3, r, r, C.byref(rope), None, None, None, 0, None) and b"no CUDA device" in L.lmrs_b200_last_error()
+    assert L.lmrs_b200_rope_axes(C.byref(rope), 0, r, r, 3, 4, 64, C.byref(pos), None) and b"no CUDA device" in L.lmrs_b200_last_error()
