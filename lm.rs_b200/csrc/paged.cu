@@ -2,6 +2,7 @@
 // Device pointers, the caller's stream; nothing here allocates, synchronises or remembers anything from one call to the next.
 #include <math.h>
 
+#include <algorithm>
 #include <string>
 
 #include "paged_attn.cuh"
@@ -69,7 +70,7 @@ std::string bad_pages(const lmrs_b200_pages_t* p) {
     if (!p || !p->k || !p->v) return "null pages";
     const std::string why = bad_dtype(p->dtype);
     if (!why.empty()) return why;
-    if (p->pages < 1 || p->page_size < 1 || p->kv_heads < 1) return "pages, page_size and kv_heads must be positive";
+    if (p->pages < 1 || p->page_size < 1 || p->kv_heads < 1 || p->kv_heads > MAX_HEADS) return "pages, page_size and kv_heads must be positive, kv_heads at most 65535";
     if (p->head_size < 1 || p->head_size > 256) return "head_size must be 1 .. 256";
     if (p->k_page < 0 || p->k_slot < 0 || p->k_head < 0 || p->v_page < 0 || p->v_slot < 0 || p->v_head < 0) return "negative stride of pages";
     return "";
@@ -104,6 +105,19 @@ template <typename F> int guarded(const char* where, F f) {   // no exception le
 }
 unsigned row_grid(int64_t n_rows) { return (unsigned)n_rows; }
 
+// do an array's heads all begin on 16-byte boundaries?
+bool vectors(const void* p, int64_t row, int64_t head, int dtype) {
+    const int64_t vec = 16 / (int64_t)size_of(dtype);
+    return aligned(p, 16) && row % vec == 0 && head % vec == 0;
+}
+bool vectors(const lmrs_b200_rows_t* r, int dtype) { return vectors(r->data, r->row, r->head, dtype); }
+// Warps for a row's pieces: one, or more where the rows alone would not give every SM's schedulers a few each; a warp keeps at least one piece a lane
+int parts_of(int64_t n_rows, int64_t pieces, int sms) {
+    const int64_t want = ((int64_t)sms * 16 + n_rows - 1) / n_rows, most = (pieces + 31) / 32;
+    return (int)std::max<int64_t>(1, std::min(want, most));
+}
+unsigned warps_grid(int64_t warps, int sms) { return (unsigned)std::min<int64_t>((warps + ROW_WARPS - 1) / ROW_WARPS, (int64_t)sms * ROW_CTAS); }
+
 }  // namespace
 
 extern "C" int lmrs_b200_rope_init(lmrs_b200_rope_t* out, const double* freq, const uint8_t* axis, int pairs, int layout) {
@@ -134,11 +148,13 @@ extern "C" int lmrs_b200_rope_axes(const lmrs_b200_rope_t* rope, int dtype, cons
         if (!rope || !x || !out || !pos) return refuse(me, "null argument");
         std::string why = bad_dtype(dtype);
         if (!why.empty()) return refuse(me, why);
-        if (n_rows < 0 || n_rows > 0x7fffffff || heads < 0 || head_size < 1 || head_size > 256) return refuse(me, "n_rows and heads must be 0 .. 2^31 - 1, head_size 1 .. 256");
+        if (n_rows < 0 || n_rows > 0x7fffffff || heads < 0 || heads > MAX_HEADS || head_size < 1 || head_size > 256)
+            return refuse(me, "n_rows must be 0 .. 2^31 - 1, heads 0 .. 65535, head_size 1 .. 256");
         why = bad_rope(rope, head_size);
         if (!why.empty()) return refuse(me, why);
         int device = 0;
-        if (!device_sms(me, &device)) return 1;
+        const int sms = device_sms(me, &device);
+        if (!sms) return 1;
         if (n_rows == 0 || heads == 0) return 0;
         why = bad_rows(x, "x", dtype, device);
         if (why.empty()) why = bad_rows(out, "out", dtype, device);
@@ -146,7 +162,12 @@ extern "C" int lmrs_b200_rope_axes(const lmrs_b200_rope_t* rope, int dtype, cons
         if (!why.empty()) return refuse(me, why);
         return by_type(dtype, [&](auto t) {
             using T = decltype(t);
-            rope_axes_kernel<T><<<row_grid(n_rows), 256, 0, (cudaStream_t)stream>>>(*rope, rows_as<const T>(x), rows_as<T>(out), n_rows, heads, head_size, pos_as(pos));
+            constexpr int VEC = 16 / sizeof(T);
+            const bool wide = vectors(x, dtype) && vectors(out, dtype) && rope->pairs % VEC == 0 && head_size % VEC == 0;
+            const Cut cut = cut_of(rope->pairs, rope->layout, head_size, wide ? VEC : 1);
+            const int parts = parts_of(n_rows, (int64_t)heads * (cut.turning + cut.passing), sms);
+            (wide ? rope_axes_kernel<T, VEC> : rope_axes_kernel<T, 1>)<<<warps_grid(n_rows * parts, sms), 32 * ROW_WARPS, 0, (cudaStream_t)stream>>>(
+                *rope, rows_as<const T>(x), rows_as<T>(out), n_rows, heads, cut, pos_as(pos), parts);
             return launched(me);
         });
     });
@@ -161,11 +182,12 @@ extern "C" int lmrs_b200_paged_append(const lmrs_b200_pages_t* pages, const lmrs
         if (why.empty()) why = bad_batch(batch, n_rows, pages->page_size);
         if (why.empty() && (q || q_out) && (!q || !q_out)) why = "q and q_out come together";
         if (why.empty() && q && !rope) why = "q without rope";
-        if (why.empty() && q && q_heads < 1) why = "q_heads must be positive";
+        if (why.empty() && q && (q_heads < 1 || q_heads > MAX_HEADS)) why = "q_heads must be 1 .. 65535";
         if (why.empty() && rope) why = bad_rope(rope, pages->head_size);
         if (!why.empty()) return refuse(me, why);
         int device = 0;
-        if (!device_sms(me, &device)) return 1;
+        const int sms = device_sms(me, &device);
+        if (!sms) return 1;
         if (n_rows == 0 || batch->seqs == 0) return 0;
         const int dtype = pages->dtype;
         why = bad_batch_memory(batch, device);
@@ -188,8 +210,15 @@ extern "C" int lmrs_b200_paged_append(const lmrs_b200_pages_t* pages, const lmrs
             p.k_pages = (T*)pages->k; p.v_pages = (T*)pages->v;
             p.k_page = pages->k_page; p.k_slot = pages->k_slot; p.k_head = pages->k_head;
             p.v_page = pages->v_page; p.v_slot = pages->v_slot; p.v_head = pages->v_head;
-            p.kv_heads = pages->kv_heads; p.head_size = pages->head_size;
-            paged_append_kernel<T><<<row_grid(n_rows), 256, 0, (cudaStream_t)stream>>>(p);
+            p.kv_heads = pages->kv_heads;
+            constexpr int VEC = 16 / sizeof(T);
+            const int pairs = rope ? rope->pairs : 0, size = pages->head_size;
+            const bool wide = vectors(k, dtype) && vectors(v, dtype) && (!q || (vectors(q, dtype) && vectors(q_out, dtype))) && vectors(pages->k, pages->k_page, pages->k_head, dtype) &&
+                              vectors(pages->v, pages->v_page, pages->v_head, dtype) && pages->k_slot % VEC == 0 && pages->v_slot % VEC == 0 && pairs % VEC == 0 && size % VEC == 0;
+            p.turn = cut_of(pairs, rope ? rope->layout : 0, size, wide ? VEC : 1);
+            p.pass = cut_of(0, 0, size, wide ? VEC : 1);
+            p.parts = parts_of(n_rows, (int64_t)(p.kv_heads + p.q_heads) * (p.turn.turning + p.turn.passing) + (int64_t)p.kv_heads * p.pass.passing, sms);
+            (wide ? paged_append_kernel<T, VEC> : paged_append_kernel<T, 1>)<<<warps_grid(n_rows * p.parts, sms), 32 * ROW_WARPS, 0, (cudaStream_t)stream>>>(p);
             return launched(me);
         });
     });

@@ -56,36 +56,52 @@ def _disjoint(t):
 
 
 def _gpu(t, name, device):
-    _need(isinstance(t, torch.Tensor) and t.is_cuda, f"{name} must be a tensor on a GPU (this library has no CPU fallback)")
-    _need(t.device == device, f"{name} lies on {t.device}, other arrays of the call on {device}")
+    if not isinstance(t, torch.Tensor) or not t.is_cuda:
+        raise LmrsError(f"{name} must be a tensor on a GPU (this library has no CPU fallback)")
+    if t.device != device:
+        raise LmrsError(f"{name} lies on {t.device}, other arrays of the call on {device}")
 
 
+# (these run in every call: messages are made only where one is raised)
 def _heads(t, name, device, dtype, rows, heads, size, out=False):
+    """t as the library takes it, checked: [rows, heads, size]"""
     _gpu(t, name, device)
-    _need(t.dtype == dtype, f"{name} is {t.dtype}, other arrays of the call {dtype}")
-    _need(t.dim() == 3 and t.shape[2] == size and (rows is None or t.shape[0] == rows) and (heads is None or t.shape[1] == heads),
-          f"{name} must be [{'rows' if rows is None else rows}, {'heads' if heads is None else heads}, {size}], not {list(t.shape)}")
-    _need(t.stride(2) == 1 or size == 1, f"the elements of a head of {name} must lie next to each other")
-    _need(not out or _disjoint(t), f"elements of {name} share their places")
-    return _Rows(t.data_ptr(), t.stride(0), t.stride(1))
+    if t.dtype != dtype:
+        raise LmrsError(f"{name} is {t.dtype}, other arrays of the call {dtype}")
+    if t.shape != (rows, heads, size):
+        raise LmrsError(f"{name} must be [{rows}, {heads}, {size}], not {list(t.shape)}")
+    stride = t.stride()
+    if stride[2] != 1 and size != 1:
+        raise LmrsError(f"the elements of a head of {name} must lie next to each other")
+    if out and not t.is_contiguous() and not _disjoint(t):
+        raise LmrsError(f"elements of {name} share their places")
+    return _Rows(t.data_ptr(), stride[0], stride[1])
 
 
 def _ints(t, name, device):
     _gpu(t, name, device)
-    _need(t.dtype == torch.int32, f"{name} must be int32, not {t.dtype}")
+    if t.dtype != torch.int32:
+        raise LmrsError(f"{name} must be int32, not {t.dtype}")
 
 
 def _positions(pos, axes, rows, device):
     _ints(pos, "pos", device)
-    if pos.dim() == 1:
-        _need(axes == 1 and pos.shape[0] == rows, f"pos must be [{axes}, {rows}], not {list(pos.shape)}")
+    if pos.dim() == 1 and axes == 1 and pos.shape[0] == rows:
         return _Positions(pos.data_ptr(), 0, pos.stride(0))
-    _need(pos.dim() == 2 and pos.shape[0] >= axes and pos.shape[1] == rows, f"pos must be [{axes}, {rows}], not {list(pos.shape)}")
-    return _Positions(pos.data_ptr(), pos.stride(0), pos.stride(1))
+    if pos.dim() != 2 or pos.shape[0] < axes or pos.shape[1] != rows:
+        raise LmrsError(f"pos must be [{axes}, {rows}], not {list(pos.shape)}")
+    return _Positions(pos.data_ptr(), *pos.stride())
 
 
 def _on(device):
-    return contextlib.nullcontext() if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+    return _HERE if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+
+
+def _stream(device):
+    return torch._C._cuda_getCurrentRawStream(device.index)   # torch.cuda.current_stream(device).cuda_stream without the objects (2 us of a call's 10)
+
+
+_HERE = contextlib.nullcontext()
 
 
 class RopeAxes:
@@ -100,7 +116,7 @@ class RopeAxes:
         _need(layout in ("halves", "pairs"), f"layout must be 'halves' or 'pairs', not {layout!r}")
         self._c = _Rope()
         check(lib().lmrs_b200_rope_init(C.byref(self._c), (C.c_double * max(1, len(freq)))(*freq), (C.c_uint8 * max(1, len(axis)))(*axis), len(freq), int(layout == "pairs")))
-        self.pairs, self.axes, self.layout = len(freq), self._c.axes, layout
+        self.pairs, self.axes, self.layout, self._ref = len(freq), self._c.axes, layout, C.byref(self._c)
 
     @classmethod
     def sections(cls, rot, theta, sections=None, order="blocks", layout="halves"):
@@ -168,54 +184,66 @@ class Batch:
         self._ref = C.byref(self._c)
 
     def _for(self, pages, n_rows):
-        _need(isinstance(pages, KVPages), "pages must be KVPages")
-        _need(self.device == pages.device, f"the batch lies on {self.device}, the pages on {pages.device}")
-        _need(self.prefix_len == 0 or self.prefix.shape[0] * pages.page_size >= self.prefix_len, f"prefix lists too few pages for {self.prefix_len} tokens")
-        _need(self.rows is not None or n_rows == self.seqs, f"{n_rows} rows for {self.seqs} sequences of one row each")
+        if not isinstance(pages, KVPages):
+            raise LmrsError("pages must be KVPages")
+        if self.device != pages.device:
+            raise LmrsError(f"the batch lies on {self.device}, the pages on {pages.device}")
+        if self.prefix_len and self.prefix.shape[0] * pages.page_size < self.prefix_len:
+            raise LmrsError(f"prefix lists too few pages for {self.prefix_len} tokens")
+        if self.rows is None and n_rows != self.seqs:
+            raise LmrsError(f"{n_rows} rows for {self.seqs} sequences of one row each")
 
 
 def rope_axes(x, pos, rope, out=None):
     """x [rows, heads, head_size] turned by pos [axes, rows] (or [rows] for one axis); out may be x."""
-    _need(isinstance(rope, RopeAxes), "rope must be RopeAxes")
-    _need(isinstance(x, torch.Tensor) and x.dim() == 3 and x.dtype in _DTYPES, "x must be a [rows, heads, head_size] tensor of bfloat16, float16 or float32")
+    if not isinstance(rope, RopeAxes):
+        raise LmrsError("rope must be RopeAxes")
+    if not isinstance(x, torch.Tensor) or x.dim() != 3 or x.dtype not in _DTYPES:
+        raise LmrsError("x must be a [rows, heads, head_size] tensor of bfloat16, float16 or float32")
     n, heads, size = x.shape
-    device = x.device
-    xr = _heads(x, "x", device, x.dtype, n, heads, size)
+    device, dtype = x.device, x.dtype
+    xr = _heads(x, "x", device, dtype, n, heads, size)
     p = _positions(pos, rope.axes, n, device)
     with _on(device):
         if out is None:
-            out = torch.empty(x.shape, dtype=x.dtype, device=device)
-        o = _heads(out, "out", device, x.dtype, n, heads, size, out=True)
-        check(lib().lmrs_b200_rope_axes(C.byref(rope._c), _DTYPES[x.dtype], C.byref(xr), C.byref(o), n, heads, size, C.byref(p), torch.cuda.current_stream(device).cuda_stream))
+            out = torch.empty_like(x)
+        o = _heads(out, "out", device, dtype, n, heads, size, out=True)
+        check(lib().lmrs_b200_rope_axes(rope._ref, _DTYPES[dtype], C.byref(xr), C.byref(o), n, heads, size, C.byref(p), _stream(device)))
     return out
 
 
 def append(pages, batch, k, v, rope=None, pos=None, q=None, q_out=None):
     """Writes k and v [rows, kv_heads, head_size] to the places in the pages that the batch gives their rows, k turned by pos [axes, rows] (None: by its
     place, the prefix included, on every axis); rope None: k as it is.  Returns q [rows, heads, head_size] turned alike (q_out may be q), or None."""
-    _need(isinstance(batch, Batch), "batch must be a Batch")
-    _need(isinstance(k, torch.Tensor) and k.dim() == 3, "k must be a [rows, kv_heads, head_size] tensor")
+    if not isinstance(batch, Batch):
+        raise LmrsError("batch must be a Batch")
+    if not isinstance(k, torch.Tensor) or k.dim() != 3:
+        raise LmrsError("k must be a [rows, kv_heads, head_size] tensor")
     n = k.shape[0]
     batch._for(pages, n)
     device, dtype, size = pages.device, pages.dtype, pages.head_size
     kr = _heads(k, "k", device, dtype, n, pages.kv_heads, size)
     vr = _heads(v, "v", device, dtype, n, pages.kv_heads, size)
-    _need(rope is None or isinstance(rope, RopeAxes), "rope must be RopeAxes")
-    _need(rope is not None or (pos is None and q is None), "pos and q go with rope")
-    _need(q is not None or q_out is None, "q_out without q")
+    if rope is None:
+        if pos is not None or q is not None or q_out is not None:
+            raise LmrsError("pos and q go with rope")
+    elif not isinstance(rope, RopeAxes):
+        raise LmrsError("rope must be RopeAxes")
     p = None if pos is None else C.byref(_positions(pos, rope.axes, n, device))
     with _on(device):
         qr = qo = None
         heads = 0
         if q is not None:
-            qr = _heads(q, "q", device, dtype, n, None, size)
+            if not isinstance(q, torch.Tensor) or q.dim() != 3:
+                raise LmrsError("q must be a [rows, heads, head_size] tensor")
             heads = q.shape[1]
+            qr = C.byref(_heads(q, "q", device, dtype, n, heads, size))
             if q_out is None:
-                q_out = torch.empty(q.shape, dtype=dtype, device=device)
-            qo = C.byref(_heads(q_out, "q_out", device, dtype, n, heads, size, out=True)) if heads else None
-            qr = C.byref(qr) if heads else None
-        check(lib().lmrs_b200_paged_append(pages._ref, batch._ref, n, C.byref(kr), C.byref(vr), None if rope is None else C.byref(rope._c), p, qr, qo, heads,
-                                           torch.cuda.current_stream(device).cuda_stream))
+                q_out = torch.empty_like(q)
+            qo = C.byref(_heads(q_out, "q_out", device, dtype, n, heads, size, out=True))
+        elif q_out is not None:
+            raise LmrsError("q_out without q")
+        check(lib().lmrs_b200_paged_append(pages._ref, batch._ref, n, C.byref(kr), C.byref(vr), None if rope is None else rope._ref, p, qr, qo, heads, _stream(device)))
     return q_out
 
 
@@ -223,21 +251,23 @@ def attention(pages, batch, q, out=None, scale=None, softcap=0.0, return_lse=Fal
     """softmax(scale * q . keys) . values for q [rows, heads, head_size]: every row over the prefix and over its own sequence up to its own place.
     heads: a multiple of kv_heads, neighbours share one.  scale None: head_size ** -0.5.  softcap > 0: scores s become softcap * tanh(s / softcap).  A row
     that sees nothing is 0.  return_lse: also the logarithms of the sums of exponentials, float32 [rows, heads] (-inf for a row that sees nothing)."""
-    _need(isinstance(batch, Batch), "batch must be a Batch")
-    _need(isinstance(q, torch.Tensor) and q.dim() == 3, "q must be a [rows, heads, head_size] tensor")
-    n, heads = q.shape[:2]
+    if not isinstance(batch, Batch):
+        raise LmrsError("batch must be a Batch")
+    if not isinstance(q, torch.Tensor) or q.dim() != 3:
+        raise LmrsError("q must be a [rows, heads, head_size] tensor")
+    n, heads, size = q.shape
     batch._for(pages, n)
-    device, dtype, size = pages.device, pages.dtype, pages.head_size
-    qr = _heads(q, "q", device, dtype, n, heads, size)
+    device, dtype = pages.device, pages.dtype
+    qr = _heads(q, "q", device, dtype, n, heads, pages.head_size)
     with _on(device):
         if out is None:
-            out = torch.empty(q.shape, dtype=dtype, device=device)
+            out = torch.empty_like(q)
         o = _heads(out, "out", device, dtype, n, heads, size, out=True)
         lse = torch.empty((n, heads), dtype=torch.float32, device=device) if return_lse else None
-        need = C.c_size_t()
-        check(lib().lmrs_b200_paged_attention_workspace(pages._ref, batch._ref, n, heads, C.byref(need)))
-        work = torch.empty(need.value, dtype=torch.uint8, device=device) if need.value else None
-        check(lib().lmrs_b200_paged_attention(pages._ref, batch._ref, n, C.byref(qr), C.byref(o), heads, size ** -0.5 if scale is None else scale, softcap,
-                                              lse.data_ptr() if return_lse and lse.numel() else None, None if work is None else work.data_ptr(), need.value,
-                                              torch.cuda.current_stream(device).cuda_stream))
+        L, need = lib(), C.c_size_t()
+        check(L.lmrs_b200_paged_attention_workspace(pages._ref, batch._ref, n, heads, C.byref(need)))
+        bytes = need.value
+        work = torch.empty(bytes, dtype=torch.uint8, device=device) if bytes else None
+        check(L.lmrs_b200_paged_attention(pages._ref, batch._ref, n, C.byref(qr), C.byref(o), heads, size ** -0.5 if scale is None else scale, softcap,
+                                          lse.data_ptr() if return_lse and n and heads else None, work.data_ptr() if bytes else None, bytes, _stream(device)))
     return (out, lse) if return_lse else out
