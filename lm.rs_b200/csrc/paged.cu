@@ -3,7 +3,9 @@
 #include <math.h>
 
 #include <algorithm>
+#include <atomic>
 #include <string>
+#include <type_traits>
 
 #include "paged_attn.cuh"
 #include "paged_rows.cuh"
@@ -103,8 +105,6 @@ template <typename F> int guarded(const char* where, F f) {   // no exception le
         try { return refuse(where, "out of host memory"); } catch (...) { return 1; }
     }
 }
-unsigned row_grid(int64_t n_rows) { return (unsigned)n_rows; }
-
 // do an array's heads all begin on 16-byte boundaries?
 bool vectors(const void* p, int64_t row, int64_t head, int dtype) {
     const int64_t vec = 16 / (int64_t)size_of(dtype);
@@ -230,12 +230,69 @@ static std::string bad_attention(const lmrs_b200_pages_t* pages, const lmrs_b200
     if (!why.empty()) return why;
     const int64_t vec = 16 / (int64_t)size_of(pages->dtype);
     if (pages->head_size % 8) return "head_size must be a multiple of 8";
-    if (q_heads < 1 || q_heads % pages->kv_heads) return "q_heads must be a positive multiple of kv_heads";
+    if (q_heads < 1 || q_heads > MAX_HEADS || q_heads % pages->kv_heads) return "q_heads must be a positive multiple of kv_heads, at most 65535";
+    if (n_rows * (q_heads / pages->kv_heads) > 0x7fffffff) return "n_rows * q_heads / kv_heads is beyond 2^31 - 1";
     if (!aligned(pages->k, 16) || !aligned(pages->v, 16) || pages->k_page % vec || pages->k_slot % vec || pages->k_head % vec || pages->v_page % vec || pages->v_slot % vec ||
         pages->v_head % vec)
         return "the pages' rows must lie on 16-byte boundaries";
     return "";
 }
+
+namespace {
+
+// How a call is cut, from what the host knows of it.  The number of CTAs counts a B200's SMs: it is part of the cut, and the workspace's size goes by it
+constexpr int SMS = 148;
+struct Cutting {
+    int tile_rows, tile_keys, ctas, front_tiles;
+    int64_t front_units, slots;
+    size_t plan_at, ml_at, o_at, bytes;
+};
+template <typename T, int DP> Cutting cutting(const lmrs_b200_pages_t* pages, const lmrs_b200_batch_t* batch, int64_t n_rows, int q_heads) {
+    using S = TileShape<T, DP>;
+    const int64_t rows = n_rows * (q_heads / pages->kv_heads);
+    Cutting c = {};
+    c.tile_rows = S::ROWS;
+    c.tile_keys = S::KEYS;
+    c.ctas = SMS * S::CTAS;
+    c.front_tiles = (int)(((int64_t)batch->prefix_len + S::KEYS - 1) / S::KEYS);
+    c.front_units = c.front_tiles ? (rows + S::ROWS - 1) / S::ROWS * pages->kv_heads : 0;
+    c.slots = c.front_units + (rows / S::ROWS + batch->seqs) * pages->kv_heads + c.ctas;   // (a sequence's last unit may be a part of one)
+    auto take = [&](size_t n) { const size_t at = c.bytes; c.bytes += (n + 255) / 256 * 256; return at; };
+    c.plan_at = take(sizeof(Plan) * ((size_t)batch->seqs + 1));
+    c.ml_at = take(sizeof(float2) * (size_t)c.slots * S::ROWS);
+    c.o_at = take(sizeof(float) * (size_t)c.slots * S::ROWS * pages->head_size);
+    return c;
+}
+template <typename F> int by_shape(const lmrs_b200_pages_t* pages, F f) {
+    return by_type(pages->dtype, [&](auto t) {
+        using T = decltype(t);
+        return pages->head_size <= 64 ? f(T(), std::integral_constant<int, 64>()) : pages->head_size <= 128 ? f(T(), std::integral_constant<int, 128>()) : f(T(), std::integral_constant<int, 256>());
+    });
+}
+// lets a kernel use more than 48 KB of shared memory: once a device
+template <typename K> cudaError_t allow_smem(K kernel, int device, int bytes, std::atomic<uint64_t>& done) {
+    const uint64_t bit = 1ull << (device & 63);
+    if (device < 64 && (done.load(std::memory_order_acquire) & bit)) return cudaSuccess;
+    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    if (e == cudaSuccess && device < 64) done.fetch_or(bit, std::memory_order_release);
+    return e;
+}
+// a kernel that may be set up while the one before it still runs, and waits for its results by itself
+template <typename K, typename P> cudaError_t launch_after(K kernel, unsigned grid, unsigned threads, size_t smem, cudaStream_t stream, const P& p) {
+    cudaLaunchConfig_t c = {};
+    c.gridDim = dim3(grid);
+    c.blockDim = dim3(threads);
+    c.dynamicSmemBytes = smem;
+    c.stream = stream;
+    cudaLaunchAttribute a = {};
+    a.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    a.val.programmaticStreamSerializationAllowed = 1;
+    c.attrs = &a;
+    c.numAttrs = 1;
+    return cudaLaunchKernelEx(&c, kernel, p);
+}
+
+}  // namespace
 
 extern "C" int lmrs_b200_paged_attention_workspace(const lmrs_b200_pages_t* pages, const lmrs_b200_batch_t* batch, int64_t n_rows, int q_heads, size_t* bytes) {
     static const char* me = "paged_attention_workspace";
@@ -244,7 +301,11 @@ extern "C" int lmrs_b200_paged_attention_workspace(const lmrs_b200_pages_t* page
         const std::string why = bad_attention(pages, batch, n_rows, q_heads);
         if (!why.empty()) return refuse(me, why);
         *bytes = 0;
-        return 0;
+        if (n_rows == 0 || batch->seqs == 0) return 0;
+        return by_shape(pages, [&](auto t, auto d) {
+            *bytes = cutting<decltype(t), decltype(d)::value>(pages, batch, n_rows, q_heads).bytes;
+            return 0;
+        });
     });
 }
 
@@ -265,9 +326,13 @@ extern "C" int lmrs_b200_paged_attention(const lmrs_b200_pages_t* pages, const l
         if (why.empty()) why = bad_rows(out, "out", dtype, device);
         if (why.empty() && lse && (!aligned(lse, 4) || !on_device(lse, device))) why = "lse is not memory of the current device";
         if (why.empty() && (!on_device(pages->k, device) || !on_device(pages->v, device))) why = "the pages are not memory of the current device";
+        if (why.empty() && (!workspace || !aligned(workspace, 256) || !on_device(workspace, device))) why = "workspace is not memory of the current device on a 256-byte boundary";
         if (!why.empty()) return refuse(me, why);
-        return by_type(dtype, [&](auto t) {
+        return by_shape(pages, [&](auto t, auto d) {
             using T = decltype(t);
+            using S = TileShape<T, decltype(d)::value>;
+            const Cutting c = cutting<T, decltype(d)::value>(pages, batch, n_rows, q_heads);
+            if (workspace_bytes < c.bytes) return refuse(me, "workspace has " + std::to_string(workspace_bytes) + " bytes, the call needs " + std::to_string(c.bytes));
             AttnParams<T> p = {};
             p.batch = batch_as(batch, pages, n_rows);
             p.q = rows_as<const T>(q);
@@ -275,10 +340,26 @@ extern "C" int lmrs_b200_paged_attention(const lmrs_b200_pages_t* pages, const l
             p.k = (const T*)pages->k; p.v = (const T*)pages->v;
             p.k_page = pages->k_page; p.k_slot = pages->k_slot; p.k_head = pages->k_head;
             p.v_page = pages->v_page; p.v_slot = pages->v_slot; p.v_head = pages->v_head;
-            p.kv_heads = pages->kv_heads; p.q_heads = q_heads; p.head_size = pages->head_size;
-            p.scale = scale; p.softcap = softcap; p.lse = lse;
-            paged_attention_kernel<T><<<dim3(row_grid(n_rows), (unsigned)q_heads), 128, 0, (cudaStream_t)stream>>>(p);
-            return launched(me);
+            p.kv_heads = pages->kv_heads; p.q_heads = q_heads; p.head_size = pages->head_size; p.group = q_heads / pages->kv_heads;
+            p.scale2 = scale * LOG2E; p.softcap = softcap; p.cap_in = softcap > 0.0f ? scale / softcap : 0.0f; p.lse = lse;
+            p.q_wide = vectors(q, dtype);
+            p.out_wide = aligned(out->data, 4 * sizeof(T)) && out->row % 4 == 0 && out->head % 4 == 0;
+            p.tile_rows = c.tile_rows; p.tile_keys = c.tile_keys; p.ctas = c.ctas; p.front_units = c.front_units; p.front_tiles = c.front_tiles;
+            p.plan = (Plan*)((char*)workspace + c.plan_at);
+            p.part_ml = (float2*)((char*)workspace + c.ml_at);
+            p.part_o = (float*)((char*)workspace + c.o_at);
+            p.slots = c.slots;
+            static std::atomic<uint64_t> allowed{0};
+            auto kernel = rows16_kernel<T, decltype(d)::value>;
+            cudaError_t e = allow_smem(kernel, device, S::SMEM, allowed);
+            if (e != cudaSuccess) return refuse(me, cudaGetErrorString(e));
+            kernel<<<(unsigned)c.ctas, S::THREADS, S::SMEM, (cudaStream_t)stream>>>(p);
+            if (launched(me)) return 1;
+            // a warp a row and head, or 8 while that leaves warps on the GPU idle
+            const int64_t items = n_rows * q_heads;
+            e = items <= SMS * 16 ? launch_after(join_kernel<T, 8>, (unsigned)items, 256, 0, (cudaStream_t)stream, p)
+                                  : launch_after(join_kernel<T, 1>, (unsigned)std::min<int64_t>((items + 7) / 8, SMS * 16), 256, 0, (cudaStream_t)stream, p);
+            return e == cudaSuccess ? 0 : refuse(me, std::string("launch failed: ") + cudaGetErrorString(e));
         });
     });
 }

@@ -1,4 +1,15 @@
 // paged_attn.cuh -- attention of the rows of many sequences over their pages and over a prefix that all of them share.
+//
+// For one row: out = sum_j e^(s_j) v_j / sum_j e^(s_j) over the keys that it sees.  The keys are cut into parts that are worked on apart; a part leaves
+// (m, l, o): the largest score, l = sum e^(s_j - m), o = sum e^(s_j - m) v_j, and parts are joined by rescaling to the largest m.  Scores are kept in
+// powers of two (s log2 e).  What is cut, and how, is the same for all kernels here:
+//   unit    16 (TILE_ROWS) rows of one KV head against one list of keys: the rows of one sequence, a row being a token and one of the query heads that share the
+//           KV head, against the sequence's own tokens; or any rows of the call against the prefix, which is so read once for 16 rows, whoever they belong to
+//   tile    TILE_KEYS keys of a unit
+//   part    the tiles of a unit that one CTA takes.  All tiles of all units stand in one line, and CTA i of n takes those from T i / n to T (i + 1) / n,
+//           whatever the sequences' lengths, which are read on the device: one long sequence spreads over the whole GPU, many short ones are packed.
+// A unit that one CTA takes whole, with no prefix to join, is finished where it is computed; for the others join_kernel reads the parts from the workspace, in
+// the order of their keys, so that a result depends on nothing but the call.
 #pragma once
 #include "paged.h"
 #include "paged_rows.cuh"
@@ -6,74 +17,799 @@
 namespace lmrs {
 namespace paged {
 
+PG_DEVINL uint32_t smem_at(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
+PG_DEVINL float ex2(float v) { float r; asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v)); return r; }
+// 16 bytes to shared memory, zeros where there is nothing to copy
+PG_DEVINL void copy16(uint32_t to, const void* from, bool there) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(there ? 16 : 0) : "memory");
+}
+PG_DEVINL void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N> PG_DEVINL void copy_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+PG_DEVINL void grid_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+PG_DEVINL void grid_launch() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+
+constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
+
+struct Plan {          // of sequence b, in the workspace: what stands before it in the line
+    int64_t tiles;
+    int64_t units;
+};
 template <typename T> struct AttnParams {
     Batch batch;
     Rows<const T> q;
     Rows<T> out;
     const T *k, *v;
     int64_t k_page, k_slot, k_head, v_page, v_slot, v_head;
-    int kv_heads, q_heads, head_size;
-    float scale, softcap;
+    int kv_heads, q_heads, head_size, group;   // group: query heads that share a KV head
+    float scale2, softcap, cap_in;             // scores: scale2 = scale * log2 e; or softcap * log2 e * tanh(dot * cap_in), cap_in = scale / softcap
     float* lse;
+    bool q_wide, out_wide;                     // rows on 16-byte boundaries
+    // the line: units of the prefix stand before those of the sequences
+    int tile_rows, tile_keys, ctas;
+    int64_t front_units;                       // kv_heads * tiles of rows
+    int front_tiles;                           // of each
+    // workspace
+    Plan* plan;        // [seqs + 1]
+    float2* part_ml;   // [slots][tile_rows]
+    float* part_o;     // [slots][tile_rows][head_size]
+    int64_t slots;     // part of unit u by CTA c: u + c (each step along the line goes on to another unit, another CTA or both)
 };
 
-// CTA = a row and a head, its keys 128 at a time with the running maximum and sum: the plainest form
-template <typename T>
-__global__ void __launch_bounds__(128) paged_attention_kernel(const __grid_constant__ AttnParams<T> p) {
-    __shared__ int found;
-    __shared__ float q[256], w[128], red[4];
-    __shared__ int64_t at[128];
-    const int64_t r = blockIdx.x;
-    const int h = blockIdx.y, g = h / (p.q_heads / p.kv_heads), D = p.head_size, t = threadIdx.x;
-    const int b = seq_of_row(p.batch, r, &found);
-    if (b < 0) return;
-    const Span s = span_of(p.batch, b);
-    const int64_t index = (int64_t)s.len - s.count + (r - s.first);
-    const int prefix = index < 0 ? 0 : p.batch.prefix_len;
-    const int64_t n_own = index < 0 ? 0 : min((int64_t)p.batch.table_len * p.batch.page_size, index + 1);
-    const int ps = p.batch.page_size, prefix_pages = (p.batch.prefix_len + ps - 1) / ps;
-    for (int e = t; e < D; e += 128) q[e] = to_f(p.q.data[r * p.q.row + h * p.q.head + e]);
-    float m = -INFINITY, l = 0.0f, acc[2] = {0.0f, 0.0f};
-    bool any = false;
-    for (int64_t x0 = 0; x0 < prefix + n_own; x0 += 128) {
-        __syncthreads();
-        const int64_t x = x0 + t;
-        const int64_t slot = x < prefix            ? slot_of(p.batch.prefix, prefix_pages, ps, p.batch.pages, (int)x)
-                             : x < prefix + n_own ? slot_of(p.batch.tables + b * p.batch.table_stride, p.batch.table_len, ps, p.batch.pages, (int)(x - prefix))
-                                                  : -1;
-        const int64_t page = slot / ps, place = slot - page * ps;
-        float a = -INFINITY;
-        if (slot >= 0) {
-            const T* k = p.k + page * p.k_page + place * p.k_slot + g * p.k_head;
-            a = 0.0f;
-            for (int e = 0; e < D; e++) a = fmaf(q[e], to_f(k[e]), a);
-            a *= p.scale;
-            if (p.softcap > 0.0f) a = p.softcap * tanhf(a / p.softcap);
+// (no more CTAs than tiles, so that each that takes part has some, and the parts of a unit are those of neighbours)
+PG_DEVINL int64_t cta_begin(int64_t total, int ctas, int i) {
+    const int64_t n = min((int64_t)ctas, total);
+    return i < n ? total * i / n : total;
+}
+PG_DEVINL int cta_of(int64_t total, int ctas, int64_t tile) { return (int)((min((int64_t)ctas, total) * (tile + 1) + total - 1) / total) - 1; }
+
+// rows of a sequence's unit and the keys it goes through
+// (a call's rows times the group stay below 2^31)
+PG_DEVINL int unit_rows(const Span& s, int group, int tile_rows) { return (s.count * group + tile_rows - 1) / tile_rows; }
+template <typename T> PG_DEVINL int keys_upto(const AttnParams<T>& p, int64_t index) {   // keys of its own that a row of this index sees
+    const int64_t most = (int64_t)p.batch.table_len * p.batch.page_size, n = index + 1;
+    return n <= 0 ? 0 : (int)(n < most ? n : most);
+}
+template <typename T> PG_DEVINL int unit_keys(const AttnParams<T>& p, const Span& s, int tile) {
+    const int last = min(s.count * p.group, (tile + 1) * p.tile_rows) - 1;
+    return keys_upto(p, (int64_t)s.len - s.count + last / p.group);
+}
+template <typename T> PG_DEVINL int unit_tiles(const AttnParams<T>& p, const Span& s, int tile) { return (unit_keys(p, s, tile) + p.tile_keys - 1) / p.tile_keys; }
+template <typename T> PG_DEVINL int64_t seq_tiles(const AttnParams<T>& p, const Span& s) {
+    int64_t n = 0;
+    for (int t = unit_rows(s, p.group, p.tile_rows) - 1; t >= 0; t--) n += unit_tiles(p, s, t);
+    return n * p.kv_heads;
+}
+
+// Where a CTA is in the line
+struct Walk {
+    int64_t unit;              // number of the unit
+    int b, head, row_tile;     // sequence (-1: the prefix), KV head, tile of rows
+    int tile, tiles, keys;     // tile of keys, how many the unit has, its keys
+    Span s;
+};
+template <typename T> PG_DEVINL void walk_unit(const AttnParams<T>& p, Walk& w) {   // fills in the keys of the unit that b, head and row_tile name
+    w.keys = w.b < 0 ? p.batch.prefix_len : unit_keys(p, w.s, w.row_tile);
+    w.tiles = (w.keys + p.tile_keys - 1) / p.tile_keys;
+}
+// the next unit that has tiles; KV heads lie innermost
+template <typename T> PG_DEVINL void walk_next_unit(const AttnParams<T>& p, Walk& w) {
+    do {
+        w.unit++;
+        if (++w.head == p.kv_heads) {
+            w.head = 0;
+            w.row_tile++;
+            if (w.b < 0 ? w.unit >= p.front_units : w.row_tile >= unit_rows(w.s, p.group, p.tile_rows)) {
+                w.row_tile = 0;
+                do {
+                    w.b++;
+                    if (w.b >= p.batch.seqs) { w.tiles = w.keys = 0; return; }   // the end of the line
+                    w.s = span_of(p.batch, w.b);
+                } while (w.s.count == 0);
+            }
         }
-        at[t] = slot < 0 ? -1 : page * p.v_page + place * p.v_slot + g * p.v_head;
-        any |= slot >= 0;
+        walk_unit(p, w);
+    } while (w.tiles == 0);
+    w.tile = 0;
+}
+// All threads: the whole line's length, and the CTA's place where it begins (`from` is that tile's number).  CTA 0 leaves the plan for join_kernel
+template <typename T, int THREADS>
+PG_DEVINL int64_t walk_begin(const AttnParams<T>& p, Walk& w, int64_t& from, int64_t& to) {
+    __shared__ int64_t warp_tiles[THREADS / 32], warp_units[THREADS / 32], found[3];
+    const int t = threadIdx.x, lane = t & 31, each = (p.batch.seqs + THREADS - 1) / THREADS, b0 = min(p.batch.seqs, t * each), b1 = min(p.batch.seqs, b0 + each);
+    int64_t tiles = 0, units = 0;
+    for (int b = b0; b < b1; b++) {
+        const Span s = span_of(p.batch, b);
+        tiles += seq_tiles(p, s);
+        units += (int64_t)unit_rows(s, p.group, p.tile_rows) * p.kv_heads;
+    }
+    int64_t tiles_to = tiles, units_to = units;   // up to and with this thread's
+    for (int o = 1; o < 32; o <<= 1) {
+        const int64_t a = __shfl_up_sync(~0u, tiles_to, o), c = __shfl_up_sync(~0u, units_to, o);
+        if (lane >= o) { tiles_to += a; units_to += c; }
+    }
+    if (lane == 31) { warp_tiles[t >> 5] = tiles_to; warp_units[t >> 5] = units_to; }
+    if (t == 0) found[0] = found[1] = found[2] = 0;
+    __syncthreads();
+    const int64_t front = p.front_units * p.front_tiles;
+    int64_t total = front;
+    tiles_to += front;
+    units_to += p.front_units;
+    for (int i = 0; i < THREADS / 32; i++) {
+        if (i < t >> 5) { tiles_to += warp_tiles[i]; units_to += warp_units[i]; }
+        total += warp_tiles[i];
+    }
+    from = cta_begin(total, p.ctas, blockIdx.x);
+    to = cta_begin(total, p.ctas, blockIdx.x + 1);
+    if (blockIdx.x == 0) {
+        int64_t at = tiles_to - tiles, u = units_to - units;
+        for (int b = b0; b < b1; b++) {
+            const Span s = span_of(p.batch, b);
+            p.plan[b] = Plan{at, u};
+            at += seq_tiles(p, s);
+            u += (int64_t)unit_rows(s, p.group, p.tile_rows) * p.kv_heads;
+        }
+        if (t == 0) p.plan[p.batch.seqs] = Plan{total, 0};
+    }
+    if (from >= front && from < to && tiles_to - tiles <= from && from < tiles_to) {   // one thread's sequences hold it
+        int64_t at = tiles_to - tiles, u = units_to - units;
+        for (int b = b0; b < b1; b++) {
+            const Span s = span_of(p.batch, b);
+            const int64_t n = seq_tiles(p, s);
+            if (from < at + n) {
+                found[0] = b;
+                found[1] = at;
+                found[2] = u;
+                break;
+            }
+            at += n;
+            u += (int64_t)unit_rows(s, p.group, p.tile_rows) * p.kv_heads;
+        }
+    }
+    __syncthreads();
+    if (from >= to) return total;
+    if (from < front) {
+        w.unit = from / p.front_tiles;
+        w.b = -1;
+        w.row_tile = (int)(w.unit / p.kv_heads);
+        w.head = (int)(w.unit - (int64_t)w.row_tile * p.kv_heads);
+        w.tile = (int)(from - w.unit * p.front_tiles);
+    } else {
+        w.b = (int)found[0];
+        w.s = span_of(p.batch, w.b);
+        int64_t left = from - found[1];
+        int n = unit_tiles(p, w.s, 0);
+        w.row_tile = 0;
+        for (const int rows = unit_rows(w.s, p.group, p.tile_rows); w.row_tile + 1 < rows && left >= (int64_t)n * p.kv_heads; n = unit_tiles(p, w.s, ++w.row_tile)) left -= (int64_t)n * p.kv_heads;
+        n = max(n, 1);   // (it is; lengths that change under the kernel may make it otherwise)
+        w.head = min((int)(left / n), p.kv_heads - 1);
+        w.tile = (int)(left - (int64_t)w.head * n);
+        w.unit = found[2] + (int64_t)w.row_tile * p.kv_heads + w.head;
+    }
+    walk_unit(p, w);
+    return total;
+}
+
+// What row `x` of a unit is: its row of the call's arrays (-1: none), its query head, and how many of the unit's keys it sees
+struct UnitRow { int64_t row; int head, keys; };
+template <typename T> PG_DEVINL UnitRow unit_row(const AttnParams<T>& p, const Walk& w, int x) {
+    const int i = w.row_tile * p.tile_rows + x, token = i / p.group;
+    UnitRow r = {-1, w.head * p.group + (i - token * p.group), w.keys};   // (rows that are not there see all, so that they need no mask)
+    if (w.b < 0) {
+        if (token < p.batch.n_rows) r.row = token;
+    } else if (token < w.s.count) {
+        r.row = w.s.first + token;
+        r.keys = min(w.keys, keys_upto(p, (int64_t)w.s.len - w.s.count + token));
+    }
+    return r;
+}
+// where key x of a unit lies: page (-1: nowhere) and place in it
+struct Place { int page, place; };
+template <typename T> PG_DEVINL Place unit_place(const AttnParams<T>& p, const Walk& w, int x) {
+    Place r = {-1, 0};
+    if (x < w.keys) {   // (so the table reaches it)
+        const int i = x / p.batch.page_size, page = (w.b < 0 ? p.batch.prefix : p.batch.tables + w.b * p.batch.table_stride)[i];
+        r.page = page < 0 || page >= p.batch.pages ? -1 : page;
+        r.place = x - i * p.batch.page_size;
+    }
+    return r;
+}
+template <typename T> PG_DEVINL float score2(const AttnParams<T>& p, float dot) {   // in powers of two
+    return p.softcap > 0.0f ? p.softcap * LOG2E * tanhf(dot * p.cap_in) : dot * p.scale2;
+}
+
+template <typename T> PG_DEVINL void store_row(const AttnParams<T>& p, const UnitRow& r, int e, float4 v) {   // 4 elements of a result
+    T* to = p.out.data + r.row * p.out.row + r.head * p.out.head + e;
+    if (p.out_wide) {
+        Piece<T, 4> x;
+        x.v[0] = from_f<T>(v.x); x.v[1] = from_f<T>(v.y); x.v[2] = from_f<T>(v.z); x.v[3] = from_f<T>(v.w);
+        *reinterpret_cast<Piece<T, 4>*>(to) = x;
+    } else {
+        to[0] = from_f<T>(v.x); to[1] = from_f<T>(v.y); to[2] = from_f<T>(v.z); to[3] = from_f<T>(v.w);
+    }
+}
+
+// A row of a unit once more, keys `from` to `to` - 1 of the unit, by all threads of the CTA: only keys that the row sees are touched.  In the matrix products a
+// value that is not finite spoils, through its weight 0, also the rows of the tile that do not see it.  acc[i]: column threadIdx.x + i * THREADS, unnormalised.
+// Rows that come out finite never come here.
+template <typename T, int THREADS>
+static __device__ __noinline__ void row_again(const AttnParams<T>& p, const Walk& w, const UnitRow& r, int from, int to, float& m, float& l, float (&acc)[256 / THREADS]) {
+    __shared__ float weight[THREADS], most[THREADS / 32];
+    __shared__ int64_t at[THREADS];
+    const int t = threadIdx.x, D = p.head_size;
+    const T* q = p.q.data + r.row * p.q.row + r.head * p.q.head;
+    m = -INFINITY;
+    l = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 256 / THREADS; i++) acc[i] = 0.0f;
+    to = min(to, r.keys);
+    for (int x0 = from; x0 < to; x0 += THREADS) {
+        Place at_x = {-1, 0};
+        if (x0 + t < to) at_x = unit_place(p, w, x0 + t);
+        const bool there = at_x.page >= 0;
+        float a = -INFINITY;
+        if (there) {
+            const T* k = p.k + at_x.page * p.k_page + at_x.place * p.k_slot + w.head * p.k_head;
+            a = 0.0f;
+            for (int e = 0; e < D; e++) a = fmaf(to_f(q[e]), to_f(k[e]), a);
+            a = score2(p, a);
+        }
         float top = a;
         for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(~0u, top, o));
-        if ((t & 31) == 0) red[t >> 5] = top;
         __syncthreads();
-        const float mn = fmaxf(fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3])), m), base = mn == -INFINITY ? 0.0f : mn;
-        const float corr = expf(m - base);   // (m -infinity: 0)
-        w[t] = slot < 0 ? 0.0f : expf(a - base);
-        m = mn;
+        at[t] = there ? at_x.page * p.v_page + at_x.place * p.v_slot + w.head * p.v_head : -1;
+        if ((t & 31) == 0) most[t >> 5] = top;
+        __syncthreads();
+        float now = m;
+        for (int i = 0; i < THREADS / 32; i++) now = fmaxf(now, most[i]);
+        const float base = now == -INFINITY ? 0.0f : now, corr = ex2(m - base);
+        weight[t] = there ? ex2(a - base) : 0.0f;
+        m = now;
         __syncthreads();
         l *= corr;
-        for (int i = 0; i < 128; i++) l += w[i];
-        for (int c = 0; c < 2; c++)
-            if (t + 128 * c < D) {
+        for (int i = 0; i < THREADS; i++) l += weight[i];
+#pragma unroll
+        for (int c = 0; c < 256 / THREADS; c++)
+            if (t + c * THREADS < D) {
                 acc[c] *= corr;
-                for (int i = 0; i < 128; i++)
-                    if (at[i] >= 0) acc[c] = fmaf(w[i], to_f(p.v[at[i] + t + 128 * c]), acc[c]);
+                for (int i = 0; i < THREADS; i++)
+                    if (at[i] >= 0) acc[c] = fmaf(weight[i], to_f(p.v[at[i] + t + c * THREADS]), acc[c]);
             }
     }
-    any = __syncthreads_or(any);
-    for (int c = 0; c < 2; c++)
-        if (t + 128 * c < D) p.out.data[r * p.out.row + h * p.out.head + t + 128 * c] = from_f<T>(any ? acc[c] / l : 0.0f);
-    if (t == 0 && p.lse) p.lse[r * p.q_heads + h] = any ? logf(l) + (m == -INFINITY ? 0.0f : m) : -INFINITY;
+    __syncthreads();
+}
+
+// A part's row leaves as (m, l) and o in the workspace, or as a result.  l = -1: the part holds no key that the row sees
+PG_DEVINL float lse_of(float m, float l) { return ((m == -INFINITY ? 0.0f : m) + log2f(l)) * LN2; }
+template <typename T> PG_DEVINL bool whole_unit(const AttnParams<T>& p, const Walk& w, int first, int last) { return w.b >= 0 && p.front_tiles == 0 && first == 0 && last == w.tiles - 1; }
+
+// ---- 16 rows a unit ------------------------------------------------------------------------------------------------------------------------
+// CTA = 4 warps that share a tile's keys, each with the running (m, l, o) of all 16 rows over its keys; they meet when a part ends.  What bounds it is the
+// bytes of the pages.  Copies to shared memory (16 bytes a thread, zeros for keys that are not there) run two or three tiles ahead of the products, on into
+// the units that follow, with the places of the keys one tile further ahead; rows are 16-byte pieces rotated by the row's number, which keeps all reads
+// free of bank conflicts.  A page may end anywhere in a tile.
+template <typename T, int DP> struct TileShape {
+    static constexpr int ROWS = 16, THREADS = 128, ROW = DP * (int)sizeof(T), PIECES = ROW / 16, KEYS = ROW > 512 ? 32 : 64, STAGES = ROW > 512 ? 2 : 3;
+    static constexpr int WARP_KEYS = KEYS / 4, COPY_KEYS = KEYS / 32;   // keys a warp works on; keys a thread copies a quarter of
+    static constexpr int KV = KEYS * ROW, Q = ROWS * ROW, SMEM = STAGES * (2 * KV + Q);   // (queries: one set for each unit that copies can have got to)
+    static constexpr int CTAS = ROW <= 128 ? 3 : ROW <= 256 ? 2 : 1;
+    static_assert(4 * ROWS * DP * 4 <= 2 * KV, "the four warps' rows fit where a tile's keys and values were");
+};
+PG_DEVINL uint32_t piece_at(int row, int piece, int row_bytes) { return (uint32_t)(row * row_bytes + ((piece ^ (row & 7)) << 4)); }
+
+// where the warps' sums meet: float c of row r, rotated so that the rows that a store touches lie in different banks
+template <int DP> PG_DEVINL int sum_at(int r, int c) { return r * DP + (c ^ ((r & 3) << 3)); }
+
+PG_DEVINL void ldmatrix4(uint32_t (&r)[4], uint32_t at) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(at) : "memory");
+}
+PG_DEVINL void ldmatrix4t(uint32_t (&r)[4], uint32_t at) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(at) : "memory");
+}
+PG_DEVINL void mma16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1, __nv_bfloat16) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+PG_DEVINL void mma16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1, __half) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+// Weights are rounded to the type of the values for the products (half a step of a weight that is at most 1 to 2^-9 of the row's sum, of either sign; the sums that
+// they are divided by are of the unrounded ones).  float16 keeps fewer small numbers: its weights are 2^7 times as large (m is 7 less), so that what a
+// weight loses below 2^-14 is 2^-32 of the largest at most.
+template <typename T> constexpr float WEIGHT_SHIFT = 0.0f;
+template <> constexpr float WEIGHT_SHIFT<__half> = 7.0f;
+
+// the products of one warp, 16-bit types: mma.sync, 16 rows x 16 keys at a time
+template <typename T, int DP> struct WarpTile {
+    using S = TileShape<T, DP>;
+    uint32_t q[DP / 16][4];
+    float o[DP / 8][4], m[2], l[2];   // rows lane / 4 and lane / 4 + 8
+    bool seen[2];
+    PG_DEVINL void begin(uint32_t q_at, int head_size) {
+        const int lane = threadIdx.x & 31;
+#pragma unroll
+        for (int k = 0; k < DP / 16; k++)
+            if (16 * k < head_size) ldmatrix4(q[k], q_at + piece_at(lane & 15, 2 * k + (lane >> 4), S::ROW));
+#pragma unroll
+        for (int n = 0; n < DP / 8; n++) o[n][0] = o[n][1] = o[n][2] = o[n][3] = 0.0f;
+        m[0] = m[1] = -INFINITY;
+        l[0] = l[1] = 0.0f;
+        seen[0] = seen[1] = false;
+    }
+    // there: bit j: key j of the warp's is there; first: number of its first key; row_keys: how many keys each row sees
+    PG_DEVINL void tile(const AttnParams<T>& p, uint32_t, uint32_t k_at, uint32_t v_at, uint32_t there, int first, const int* row_keys, int, float*) {
+        const int lane = threadIdx.x & 31, key0 = 16 * (threadIdx.x >> 5);
+        const int limit[2] = {row_keys[lane / 4] - first, row_keys[lane / 4 + 8] - first};
+        float s[2][4] = {};
+#pragma unroll
+        for (int k = 0; k < DP / 16; k++)
+            if (16 * k < p.head_size) {
+                uint32_t b[4];
+                ldmatrix4(b, k_at + piece_at(key0 + (lane & 7) + ((lane >> 4) << 3), 2 * k + ((lane >> 3) & 1), S::ROW));
+                mma16816(s[0], q[k], b[0], b[1], T());
+                mma16816(s[1], q[k], b[2], b[3], T());
+            }
+        const bool all = there == 0xffffu && limit[0] >= 16 && limit[1] >= 16;
+#pragma unroll
+        for (int h = 0; h < 2; h++)
+#pragma unroll
+            for (int c = 0; c < 4; c++) {
+                const int j = 8 * h + 2 * (lane & 3) + (c & 1);
+                float a = score2(p, s[h][c]);
+                s[h][c] = all || ((there >> j & 1) && j < limit[c >> 1]) ? a : -INFINITY;
+            }
+        uint32_t a[4];
+#pragma unroll
+        for (int i = 0; i < 2; i++) {
+            float top = fmaxf(fmaxf(s[0][2 * i], s[0][2 * i + 1]), fmaxf(s[1][2 * i], s[1][2 * i + 1]));
+            top = fmaxf(top, __shfl_xor_sync(~0u, top, 1));
+            top = fmaxf(top, __shfl_xor_sync(~0u, top, 2));
+            const float now = fmaxf(m[i], top - WEIGHT_SHIFT<T>), base = now == -INFINITY ? 0.0f : now, corr = ex2(m[i] - base);
+            m[i] = now;
+            seen[i] = seen[i] || all || (there & (limit[i] >= 16 ? 0xffffu : limit[i] <= 0 ? 0u : (1u << limit[i]) - 1)) != 0;
+            float w[4];
+#pragma unroll
+            for (int h = 0; h < 2; h++) {
+                w[2 * h] = ex2(s[h][2 * i] - base);
+                w[2 * h + 1] = ex2(s[h][2 * i + 1] - base);
+                a[2 * h + i] = close_word(make_float2(w[2 * h], w[2 * h + 1]), T());
+            }
+            l[i] = l[i] * corr + ((w[0] + w[1]) + (w[2] + w[3]));   // (of this lane's keys: the four lanes of a row meet at the end)
+            if (__any_sync(~0u, corr != 1.0f)) {
+#pragma unroll
+                for (int n = 0; n < DP / 8; n++) { o[n][2 * i] *= corr; o[n][2 * i + 1] *= corr; }
+            }
+        }
+#pragma unroll
+        for (int n = 0; n < DP / 16; n++)
+            if (16 * n < p.head_size) {
+                uint32_t b[4];
+                ldmatrix4t(b, v_at + piece_at(key0 + (lane & 15), 2 * n + (lane >> 4), S::ROW));
+                mma16816(o[2 * n], a, b[0], b[1], T());
+                mma16816(o[2 * n + 1], a, b[2], b[3], T());
+            }
+    }
+    PG_DEVINL void put_ml(float2* ml) {   // [16]
+        const int lane = threadIdx.x & 31;
+#pragma unroll
+        for (int i = 0; i < 2; i++) {
+            l[i] += __shfl_xor_sync(~0u, l[i], 1);
+            l[i] += __shfl_xor_sync(~0u, l[i], 2);
+            if ((lane & 3) == 0) ml[lane / 4 + 8 * i] = make_float2(m[i], seen[i] ? l[i] : -1.0f);
+        }
+    }
+    PG_DEVINL void put_o(float* to, const float* factor) {   // [16][DP] as sum_at has them, times the rows' factors
+        const int lane = threadIdx.x & 31;
+#pragma unroll
+        for (int i = 0; i < 2; i++) {
+            const int r = lane / 4 + 8 * i;
+            const float f = factor[r];
+#pragma unroll
+            for (int n = 0; n < DP / 8; n++) *reinterpret_cast<float2*>(to + sum_at<DP>(r, 8 * n + 2 * (lane & 3))) = make_float2(o[n][2 * i] * f, o[n][2 * i + 1] * f);
+        }
+    }
+};
+
+// the same in float32: multiply-adds.  Scores: a lane takes one of the warp's keys and some of the rows; values: all rows, DP / 32 columns.  Rows that the unit
+// does not have (it has `used`) cost nothing.
+template <int DP> struct WarpTile<float, DP> {
+    using S = TileShape<float, DP>;
+    static constexpr int KEYS = S::WARP_KEYS, TEAMS = 32 / KEYS, SHARE = 16 / TEAMS, COLS = DP / 32;   // lanes KEYS * i .. are team i: rows i, i + TEAMS, ...
+    float o[16][COLS], m[SHARE], l[SHARE];
+    bool seen[SHARE];
+    PG_DEVINL void begin(uint32_t, int) {
+#pragma unroll
+        for (int r = 0; r < 16; r++)
+#pragma unroll
+            for (int c = 0; c < COLS; c++) o[r][c] = 0.0f;
+#pragma unroll
+        for (int i = 0; i < SHARE; i++) { m[i] = -INFINITY; l[i] = 0.0f; seen[i] = false; }
+    }
+    PG_DEVINL static float4 load4(uint32_t at) {
+        float4 v;
+        asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(at));
+        return v;
+    }
+    PG_DEVINL static float2 load2(uint32_t at) {
+        float2 v;
+        asm volatile("ld.shared.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(at));
+        return v;
+    }
+    // scratch: the warp's own [KEYS + 1][16] floats: weights, and what the rows' sums are rescaled by
+    PG_DEVINL void tile(const AttnParams<float>& p, uint32_t q_at, uint32_t k_at, uint32_t v_at, uint32_t there, int first, const int* row_keys, int used, float* scratch) {
+        const int lane = threadIdx.x & 31, key0 = KEYS * (threadIdx.x >> 5), key = lane % KEYS, team = lane / KEYS;
+        float s[SHARE] = {};
+#pragma unroll 4
+        for (int c = 0; c < p.head_size / 4; c++) {
+            const float4 k = load4(k_at + piece_at(key0 + key, c, S::ROW));
+#pragma unroll
+            for (int i = 0; i < SHARE; i++)
+                if (i * TEAMS < used) {
+                    const float4 q = load4(q_at + piece_at(i * TEAMS + team, c, S::ROW));
+                    s[i] = fmaf(q.x, k.x, fmaf(q.y, k.y, fmaf(q.z, k.z, fmaf(q.w, k.w, s[i]))));
+                }
+        }
+        __syncwarp();   // (the weights of the tile before have been read)
+#pragma unroll
+        for (int i = 0; i < SHARE; i++)
+            if (i * TEAMS < used) {
+                const int row = i * TEAMS + team;
+                const bool sees = (there >> key & 1) && first + key < row_keys[row];
+                const float a = sees ? score2(p, s[i]) : -INFINITY;
+                float top = a;
+#pragma unroll
+                for (int d = KEYS / 2; d; d >>= 1) top = fmaxf(top, __shfl_xor_sync(~0u, top, d));
+                const float now = fmaxf(m[i], top), base = now == -INFINITY ? 0.0f : now, corr = ex2(m[i] - base), w = ex2(a - base);
+                m[i] = now;
+                l[i] = l[i] * corr + w;   // (this lane's keys)
+                seen[i] = seen[i] || sees;
+                scratch[key * 16 + row] = w;
+                if (key == 0) scratch[KEYS * 16 + row] = corr;
+            }
+        __syncwarp();
+#pragma unroll
+        for (int r = 0; r < 16; r++)
+            if ((r & ~3) < used) {
+                const float corr = scratch[KEYS * 16 + r];
+#pragma unroll
+                for (int c = 0; c < COLS; c++) o[r][c] *= corr;
+            }
+#pragma unroll 2
+        for (int j = 0; j < KEYS; j++) {
+            float v[COLS];
+            if constexpr (COLS == 2) {
+                const float2 x = load2(v_at + piece_at(key0 + j, lane >> 1, S::ROW) + 8 * (lane & 1));
+                v[0] = x.x; v[1] = x.y;
+            } else {
+#pragma unroll
+                for (int c = 0; c < COLS; c += 4) {
+                    const float4 x = load4(v_at + piece_at(key0 + j, lane + 8 * c, S::ROW));
+                    v[c] = x.x; v[c + 1] = x.y; v[c + 2] = x.z; v[c + 3] = x.w;
+                }
+            }
+#pragma unroll
+            for (int r = 0; r < 16; r += 4)
+                if (r < used) {
+                    const float4 w = *reinterpret_cast<const float4*>(scratch + j * 16 + r);
+#pragma unroll
+                    for (int c = 0; c < COLS; c++) {
+                        o[r][c] = fmaf(w.x, v[c], o[r][c]);
+                        o[r + 1][c] = fmaf(w.y, v[c], o[r + 1][c]);
+                        o[r + 2][c] = fmaf(w.z, v[c], o[r + 2][c]);
+                        o[r + 3][c] = fmaf(w.w, v[c], o[r + 3][c]);
+                    }
+                }
+        }
+    }
+    PG_DEVINL void put_ml(float2* ml) {
+        const int lane = threadIdx.x & 31, team = lane / KEYS;
+#pragma unroll
+        for (int i = 0; i < SHARE; i++) {
+            const unsigned any = __ballot_sync(~0u, seen[i]);
+#pragma unroll
+            for (int d = KEYS / 2; d; d >>= 1) l[i] += __shfl_xor_sync(~0u, l[i], d);
+            if (lane % KEYS == 0) ml[i * TEAMS + team] = make_float2(m[i], any >> (KEYS * team) & (KEYS == 16 ? 0xffffu : 0xffu) ? l[i] : -1.0f);
+        }
+    }
+    PG_DEVINL void put_o(float* to, const float* factor) {
+        const int lane = threadIdx.x & 31;
+#pragma unroll
+        for (int r = 0; r < 16; r++) {
+            const float f = factor[r];
+            if constexpr (COLS == 2) {
+                *reinterpret_cast<float2*>(to + sum_at<DP>(r, 2 * lane)) = make_float2(o[r][0] * f, o[r][1] * f);
+            } else {
+#pragma unroll
+                for (int c = 0; c < COLS; c += 4)
+                    *reinterpret_cast<float4*>(to + sum_at<DP>(r, 4 * lane + 32 * c)) = make_float4(o[r][c] * f, o[r][c + 1] * f, o[r][c + 2] * f, o[r][c + 3] * f);
+            }
+        }
+    }
+};
+
+// (the f32 sums' 128 registers for heads of 256 leave no room for more than one CTA anyway)
+template <typename T, int DP>
+__global__ void __launch_bounds__(TileShape<T, DP>::THREADS, TileShape<T, DP>::CTAS) rows16_kernel(const __grid_constant__ AttnParams<T> p) {
+    using S = TileShape<T, DP>;
+    extern __shared__ __align__(1024) uint8_t smem[];
+    __shared__ Walk walks[S::STAGES];             // of the units that copies have got to, by their number in this CTA modulo STAGES
+    __shared__ int row_keys[S::STAGES][S::ROWS];
+    __shared__ __align__(8) uint8_t there[S::STAGES][S::KEYS / 8];
+    __shared__ float2 ml[4][S::ROWS];
+    __shared__ __align__(16) float factor[4][S::ROWS], weights[sizeof(T) == 4 ? 4 : 1][sizeof(T) == 4 ? (S::WARP_KEYS + 1) * 16 : 1];
+    __shared__ unsigned again;
+    const int t = threadIdx.x, lane = t & 31, warp = t >> 5, D = p.head_size;
+    const uint32_t kv = smem_at(smem), queries = kv + S::STAGES * 2 * S::KV;
+
+    Walk ahead;   // where copies are
+    int64_t from, to;
+    walk_begin<T, S::THREADS>(p, ahead, from, to);
+    grid_launch();
+    if (from >= to) return;
+
+    // copies of a thread: keys t / 4 (and t / 4 + 32) of the tile, every fourth 16 bytes
+    Place place[S::COPY_KEYS];
+    int64_t line = from, unit_no = 0;   // the tile that `ahead` stands at, and which unit of this CTA that is
+    bool first = true;
+    auto look = [&]() {
+#pragma unroll
+        for (int i = 0; i < S::COPY_KEYS; i++) place[i] = unit_place(p, ahead, ahead.tile * S::KEYS + t / 4 + 32 * i);
+    };
+    auto copy_tile = [&]() {   // the tile at `line`, whose places are known; then on to the next one
+        if (line < to) {
+            const int stage = (int)((line - from) % S::STAGES);
+            const uint32_t k_at = kv + stage * 2 * S::KV, v_at = k_at + S::KV;
+            const int pieces = 2 * ((D * (int)sizeof(T) + 31) / 32), whole = D * (int)sizeof(T) / 16;   // (an odd last piece is paired with zeros)
+#pragma unroll
+            for (int i = 0; i < S::COPY_KEYS; i++) {
+                const bool is = place[i].page >= 0;
+                const int row = t / 4 + 32 * i;
+                const T* k = p.k + (is ? place[i].page * p.k_page + place[i].place * p.k_slot + ahead.head * p.k_head : 0);
+                const T* v = p.v + (is ? place[i].page * p.v_page + place[i].place * p.v_slot + ahead.head * p.v_head : 0);
+#pragma unroll
+                for (int c0 = 0; c0 < S::PIECES; c0 += 4) {
+                    const int c = c0 + (t & 3);
+                    if (c < pieces) {
+                        const bool in = is && c < whole;
+                        copy16(k_at + piece_at(row, c, S::ROW), in ? k + c * (16 / sizeof(T)) : p.k, in);
+                        copy16(v_at + piece_at(row, c, S::ROW), in ? v + c * (16 / sizeof(T)) : p.v, in);
+                    }
+                }
+                const unsigned bits = __ballot_sync(~0u, __shfl_sync(~0u, is, (4 * lane) & 31)) & 0xff;
+                if (lane == 0) there[stage][warp + 4 * i] = (uint8_t)bits;
+            }
+            if (first) {
+                const int set = (int)(unit_no % S::STAGES);
+                if (t == 0) walks[set] = ahead;
+                if (t < S::ROWS) row_keys[set][t] = unit_row(p, ahead, t).keys;
+                const uint32_t q_at = queries + set * S::Q;
+                for (int e = t; e < S::ROWS * S::PIECES; e += S::THREADS) {
+                    const int x = e / S::PIECES, c = e % S::PIECES;
+                    if (c >= pieces) continue;
+                    const UnitRow r = unit_row(p, ahead, x);
+                    const bool in = r.row >= 0 && c < whole;
+                    const T* q = in ? p.q.data + r.row * p.q.row + r.head * p.q.head + c * (16 / sizeof(T)) : p.q.data;
+                    const uint32_t at = q_at + piece_at(x, c, S::ROW);
+                    if (p.q_wide) {
+                        copy16(at, q, in);
+                    } else {
+                        Piece<T, 16 / sizeof(T)> v;
+#pragma unroll
+                        for (int i = 0; i < 16 / (int)sizeof(T); i++) v.v[i] = in ? q[i] : from_f<T>(0.0f);
+                        *reinterpret_cast<Piece<T, 16 / sizeof(T)>*>(smem + (at - kv)) = v;
+                    }
+                }
+                first = false;
+            }
+            line++;
+            if (line < to) {
+                if (++ahead.tile == ahead.tiles) {
+                    walk_next_unit(p, ahead);
+                    unit_no++;
+                    first = true;
+                }
+                look();
+            }
+        }
+        copy_commit();
+    };
+    look();
+#pragma unroll
+    for (int i = 0; i < S::STAGES - 1; i++) copy_tile();
+
+    WarpTile<T, DP> tile;
+    Walk w;
+    int set = S::STAGES - 1, begun = 0, used = 0;
+    bool start = true;
+    for (int64_t at = from; at < to; at++) {
+        copy_wait<S::STAGES - 2>();
+        __syncthreads();   // the tile has landed for all threads, and the one before has been worked on by all
+        copy_tile();
+        const int stage = (int)((at - from) % S::STAGES);
+        const uint32_t k_at = kv + stage * 2 * S::KV, v_at = k_at + S::KV;
+        if (start) {
+            set = set + 1 == S::STAGES ? 0 : set + 1;
+            w = walks[set];
+            begun = w.tile;
+            tile.begin(queries + set * S::Q, D);
+            used = w.b < 0 ? (int)min((int64_t)S::ROWS, p.batch.n_rows * p.group - (int64_t)w.row_tile * S::ROWS) : min(S::ROWS, w.s.count * p.group - w.row_tile * S::ROWS);
+            start = false;
+        }
+        const uint32_t bits = S::WARP_KEYS == 16 ? *reinterpret_cast<const uint16_t*>(&there[stage][2 * warp]) : there[stage][warp];
+        tile.tile(p, queries + set * S::Q, k_at, v_at, bits, w.tile * S::KEYS + warp * S::WARP_KEYS, row_keys[set], used, weights[sizeof(T) == 4 ? warp : 0]);
+        const bool last = w.tile + 1 == w.tiles;
+        if (last || at + 1 == to) {   // the part ends: the warps' rows meet in the tile's place
+            tile.put_ml(ml[warp]);
+            if (t == 0) again = 0;
+            __syncthreads();
+            if (t < S::ROWS) {
+                float m = -INFINITY, l = 0.0f;
+                bool any = false;
+                for (int i = 0; i < 4; i++)
+                    if (ml[i][t].y >= 0.0f || ml[i][t].y != ml[i][t].y) { m = fmaxf(m, ml[i][t].x); any = true; }
+                const float base = m == -INFINITY ? 0.0f : m;
+                for (int i = 0; i < 4; i++) {
+                    const bool has = !(ml[i][t].y < 0.0f);
+                    factor[i][t] = has ? ex2(ml[i][t].x - base) : 0.0f;
+                    if (has) l += ml[i][t].y * factor[i][t];
+                }
+                ml[0][t] = make_float2(m, any ? l : -1.0f);
+            }
+            __syncthreads();
+            float* rows = reinterpret_cast<float*>(smem + stage * 2 * S::KV);
+            tile.put_o(rows + warp * S::ROWS * DP, factor[warp]);
+            __syncthreads();
+            const bool whole = whole_unit(p, w, begun, w.tile);
+            const int64_t slot = w.unit + blockIdx.x;
+            const int quads = D / 4;
+            for (int e = t; e < used * quads; e += S::THREADS) {
+                const int x = e / quads, c = 4 * (e - x * quads);
+                const float2 s = ml[0][x];
+                float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                if (!(s.y < 0.0f)) {
+#pragma unroll
+                    for (int i = 0; i < 4; i++) {
+                        const float4 a = *reinterpret_cast<const float4*>(rows + sum_at<DP>(i * S::ROWS + x, c));
+                        v.x += a.x; v.y += a.y; v.z += a.z; v.w += a.w;
+                    }
+                }
+                if (!isfinite(v.x + v.y + v.z + v.w) && w.b >= 0 && w.s.count > 1) atomicOr(&again, 1u << x);
+                if (whole) {
+                    const UnitRow r = unit_row(p, w, x);
+                    if (!(s.y < 0.0f)) { v.x /= s.y; v.y /= s.y; v.z /= s.y; v.w /= s.y; }
+                    store_row(p, r, c, v);
+                    if (c == 0 && p.lse) p.lse[r.row * p.q_heads + r.head] = s.y < 0.0f ? -INFINITY : lse_of(s.x, s.y);
+                } else if (slot < p.slots) {
+                    *reinterpret_cast<float4*>(p.part_o + (slot * S::ROWS + x) * D + c) = v;
+                    if (c == 0) p.part_ml[slot * S::ROWS + x] = s;
+                }
+            }
+            __syncthreads();
+            for (unsigned left = again; left; left &= left - 1) {   // (the same for all threads)
+                const int x = __ffs(left) - 1;
+                const UnitRow r = unit_row(p, w, x);
+                if (ml[0][x].y < 0.0f) continue;
+                float m, l, acc[256 / S::THREADS];
+                row_again<T, S::THREADS>(p, w, r, begun * S::KEYS, (w.tile + 1) * S::KEYS, m, l, acc);
+#pragma unroll
+                for (int i = 0; i < 256 / S::THREADS; i++) {
+                    const int c = t + i * S::THREADS;
+                    if (c >= D) continue;
+                    if (whole) p.out.data[r.row * p.out.row + r.head * p.out.head + c] = from_f<T>(acc[i] / l);
+                    else if (slot < p.slots) p.part_o[(slot * S::ROWS + x) * D + c] = acc[i];
+                }
+                if (t == 0) {
+                    if (whole) { if (p.lse) p.lse[r.row * p.q_heads + r.head] = lse_of(m, l); }
+                    else if (slot < p.slots) p.part_ml[slot * S::ROWS + x] = make_float2(m, l);
+                }
+            }
+        }
+        w.tile++;
+        start = last;
+    }
+    copy_wait<0>();
+}
+
+// ---- joining parts ---------------------------------------------------------------------------------------------------------------------------
+// WARPS warps a row and head, their lanes its columns in fours: each takes every WARPS-th part with a running (m, l, o), and they meet in shared memory.  8 where
+// rows are few and may have many parts, 1 otherwise (then a CTA has 8 rows or heads).
+template <typename T, int WARPS>
+__global__ void __launch_bounds__(256) join_kernel(const __grid_constant__ AttnParams<T> p) {
+    constexpr int ITEMS = 8 / WARPS;
+    __shared__ float2 ml[8];
+    __shared__ float4 sums[8][64];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, quads = p.head_size / 4, mine = warp % WARPS;
+    grid_wait();
+    const int64_t items = p.batch.n_rows * p.q_heads;
+    for (int64_t i0 = (int64_t)blockIdx.x * ITEMS; i0 < items; i0 += (int64_t)gridDim.x * ITEMS) {
+        const int64_t item = i0 + warp / WARPS;
+        bool out = item < items;
+        const int64_t r = out ? item / p.q_heads : 0;
+        const int head = (int)(item - r * p.q_heads), b = seq_of_row_warp(p.batch, r);
+        out = out && b >= 0;
+        float m = -INFINITY, l = 0.0f;
+        float4 o[2] = {};
+        bool any = false;
+        const int g = head / p.group, gi = head - g * p.group;
+        if (out) {
+            const Span s = span_of(p.batch, b);
+            const int i = (int)(r - s.first), x = i * p.group + gi, row_tile = x / p.tile_rows, tiles = unit_tiles(p, s, row_tile);
+            const int64_t index = (int64_t)s.len - s.count + i;
+            // the parts of its own unit: numbers c0 .. c1 (none: c1 < c0)
+            int64_t before = 0;
+            for (int t = lane; t < row_tile; t += 32) before += unit_tiles(p, s, t);
+            for (int d = 16; d; d >>= 1) before += __shfl_xor_sync(~0u, before, d);
+            const Plan plan = p.plan[b];
+            const int64_t total = p.plan[p.batch.seqs].tiles;
+            const int64_t tile0 = plan.tiles + before * p.kv_heads + (int64_t)g * tiles, unit = plan.units + (int64_t)row_tile * p.kv_heads + g;
+            const int c0 = tiles ? cta_of(total, p.ctas, tile0) : 0, c1 = tiles ? cta_of(total, p.ctas, tile0 + tiles - 1) : -1;
+            // and of the prefix'
+            int f0 = 0, f1 = -1;
+            const int64_t y = r * p.group + gi, f_unit = y / p.tile_rows * p.kv_heads + g;
+            if (p.front_tiles && index >= 0) {
+                f0 = cta_of(total, p.ctas, f_unit * p.front_tiles);
+                f1 = cta_of(total, p.ctas, (f_unit + 1) * p.front_tiles - 1);
+            }
+            out = p.front_tiles || c0 != c1;   // (else it was finished where it was computed)
+            if (out) {
+                const int n = (f1 - f0 + 1) + (c1 - c0 + 1);
+                for (int k = mine; k < n; k += WARPS) {
+                    const bool front = k <= f1 - f0;
+                    const int64_t slot = front ? f_unit + f0 + k : unit + c0 + (k - (f1 - f0 + 1));
+                    if (slot >= p.slots) continue;
+                    const int64_t row = slot * p.tile_rows + (front ? y % p.tile_rows : x % p.tile_rows);
+                    const float2 part = p.part_ml[row];
+                    if (part.y < 0.0f) continue;
+                    const float4* from = reinterpret_cast<const float4*>(p.part_o + row * p.head_size);
+                    float4 v[2];
+#pragma unroll
+                    for (int c = 0; c < 2; c++)
+                        if (lane + 32 * c < quads) v[c] = from[lane + 32 * c];
+                    const float now = fmaxf(m, part.x), base = now == -INFINITY ? 0.0f : now, f = ex2(m - base), w = ex2(part.x - base);
+                    m = now;
+                    l = l * f + part.y * w;
+                    any = true;
+#pragma unroll
+                    for (int c = 0; c < 2; c++)
+                        if (lane + 32 * c < quads) {
+                            o[c].x = fmaf(o[c].x, f, v[c].x * w); o[c].y = fmaf(o[c].y, f, v[c].y * w);
+                            o[c].z = fmaf(o[c].z, f, v[c].z * w); o[c].w = fmaf(o[c].w, f, v[c].w * w);
+                        }
+                }
+            }
+        }
+        if (WARPS > 1) {   // (one item a CTA: the same branch for all)
+            __syncthreads();
+            if (lane == 0) ml[warp] = make_float2(m, any ? l : -1.0f);
+#pragma unroll
+            for (int c = 0; c < 2; c++)
+                if (lane + 32 * c < quads) sums[warp][lane + 32 * c] = o[c];
+            __syncthreads();
+            if (warp) continue;
+            for (int i = 1; i < WARPS; i++) {
+                const float2 part = ml[i];
+                if (part.y < 0.0f) continue;
+                const float now = fmaxf(m, part.x), base = now == -INFINITY ? 0.0f : now, f = ex2(m - base), w = ex2(part.x - base);
+                m = now;
+                l = l * f + part.y * w;
+                any = true;
+#pragma unroll
+                for (int c = 0; c < 2; c++)
+                    if (lane + 32 * c < quads) {
+                        const float4 v = sums[i][lane + 32 * c];
+                        o[c].x = fmaf(o[c].x, f, v.x * w); o[c].y = fmaf(o[c].y, f, v.y * w);
+                        o[c].z = fmaf(o[c].z, f, v.z * w); o[c].w = fmaf(o[c].w, f, v.w * w);
+                    }
+            }
+        }
+        if (!out) continue;
+        const UnitRow row = {r, head, 0};
+#pragma unroll
+        for (int c = 0; c < 2; c++)
+            if (lane + 32 * c < quads)
+                store_row(p, row, 4 * (lane + 32 * c), any ? make_float4(o[c].x / l, o[c].y / l, o[c].z / l, o[c].w / l) : make_float4(0.0f, 0.0f, 0.0f, 0.0f));
+        if (lane == 0 && p.lse) p.lse[r * p.q_heads + head] = any ? lse_of(m, l) : -INFINITY;
+    }
 }
 
 }  // namespace paged
