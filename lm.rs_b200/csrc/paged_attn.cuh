@@ -325,11 +325,10 @@ template <typename T, int DP> struct WarpTile {
     uint32_t q[DP / 16][4];
     float o[DP / 8][4], m[2], l[2];   // rows lane / 4 and lane / 4 + 8
     bool seen[2];
-    PG_DEVINL void begin(uint32_t q_at, int head_size) {
+    PG_DEVINL void begin(uint32_t q_at) {
         const int lane = threadIdx.x & 31;
 #pragma unroll
-        for (int k = 0; k < DP / 16; k++)
-            if (16 * k < head_size) ldmatrix4(q[k], q_at + piece_at(lane & 15, 2 * k + (lane >> 4), S::ROW));
+        for (int k = 0; k < DP / 16; k++) ldmatrix4(q[k], q_at + piece_at(lane & 15, 2 * k + (lane >> 4), S::ROW));
 #pragma unroll
         for (int n = 0; n < DP / 8; n++) o[n][0] = o[n][1] = o[n][2] = o[n][3] = 0.0f;
         m[0] = m[1] = -INFINITY;
@@ -339,34 +338,59 @@ template <typename T, int DP> struct WarpTile {
     // there: bit j: key j of the warp's is there; first: number of its first key; row_keys: how many keys each row sees
     PG_DEVINL void tile(const AttnParams<T>& p, uint32_t, uint32_t k_at, uint32_t v_at, uint32_t there, int first, const int* row_keys, int, float*) {
         const int lane = threadIdx.x & 31, key0 = 16 * (threadIdx.x >> 5);
-        const int limit[2] = {row_keys[lane / 4] - first, row_keys[lane / 4 + 8] - first};
         float s[2][4] = {};
+        const uint32_t k_row = k_at + (uint32_t)(key0 + (lane & 7) + ((lane >> 4) << 3)) * S::ROW, k_turn = (uint32_t)(((lane >> 3) & 1) ^ (lane & 7)) << 4;
 #pragma unroll
-        for (int k = 0; k < DP / 16; k++)
-            if (16 * k < p.head_size) {
-                uint32_t b[4];
-                ldmatrix4(b, k_at + piece_at(key0 + (lane & 7) + ((lane >> 4) << 3), 2 * k + ((lane >> 3) & 1), S::ROW));
-                mma16816(s[0], q[k], b[0], b[1], T());
-                mma16816(s[1], q[k], b[2], b[3], T());
+        for (int k = 0; k < DP / 16; k++) {
+            uint32_t b[4];
+            ldmatrix4(b, k_row + (k_turn ^ (32 * k)));   // (piece 2k or 2k + 1, rotated by the row)
+            mma16816(s[0], q[k], b[0], b[1], T());
+            mma16816(s[1], q[k], b[2], b[3], T());
+        }
+        if (p.softcap > 0.0f) {
+#pragma unroll
+            for (int i = 0; i < 8; i++) s[i >> 2][i & 3] = score2(p, s[i >> 2][i & 3]);
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; i++) s[i >> 2][i & 3] *= p.scale2;
+        }
+        const int limit[2] = {row_keys[lane / 4] - first, row_keys[lane / 4 + 8] - first};
+        if (!__all_sync(~0u, there == 0xffffu && limit[0] >= 16 && limit[1] >= 16)) {
+#pragma unroll
+            for (int i = 0; i < 2; i++) {
+                const uint32_t sees = there & (limit[i] >= 16 ? 0xffffu : limit[i] <= 0 ? 0u : (1u << limit[i]) - 1);
+                seen[i] = seen[i] || sees;
+#pragma unroll
+                for (int h = 0; h < 2; h++)
+#pragma unroll
+                    for (int c = 0; c < 2; c++)
+                        if (!(sees >> (8 * h + 2 * (lane & 3) + c) & 1)) s[h][2 * i + c] = -INFINITY;
             }
-        const bool all = there == 0xffffu && limit[0] >= 16 && limit[1] >= 16;
+        } else {
+            seen[0] = seen[1] = true;
+        }
+        float now[2];
 #pragma unroll
-        for (int h = 0; h < 2; h++)
+        for (int i = 0; i < 2; i++) now[i] = fmaxf(fmaxf(s[0][2 * i], s[0][2 * i + 1]), fmaxf(s[1][2 * i], s[1][2 * i + 1]));
 #pragma unroll
-            for (int c = 0; c < 4; c++) {
-                const int j = 8 * h + 2 * (lane & 3) + (c & 1);
-                float a = score2(p, s[h][c]);
-                s[h][c] = all || ((there >> j & 1) && j < limit[c >> 1]) ? a : -INFINITY;
+        for (int d = 1; d < 4; d *= 2)
+#pragma unroll
+            for (int i = 0; i < 2; i++) now[i] = fmaxf(now[i], __shfl_xor_sync(~0u, now[i], d));
+        const bool grows = now[0] - WEIGHT_SHIFT<T> > m[0] || now[1] - WEIGHT_SHIFT<T> > m[1];
+        if (__any_sync(~0u, grows)) {
+#pragma unroll
+            for (int i = 0; i < 2; i++) {
+                const float top = fmaxf(m[i], now[i] - WEIGHT_SHIFT<T>), corr = ex2(m[i] - (top == -INFINITY ? 0.0f : top));
+                m[i] = top;
+                l[i] *= corr;
+#pragma unroll
+                for (int n = 0; n < DP / 8; n++) { o[n][2 * i] *= corr; o[n][2 * i + 1] *= corr; }
             }
+        }
         uint32_t a[4];
 #pragma unroll
         for (int i = 0; i < 2; i++) {
-            float top = fmaxf(fmaxf(s[0][2 * i], s[0][2 * i + 1]), fmaxf(s[1][2 * i], s[1][2 * i + 1]));
-            top = fmaxf(top, __shfl_xor_sync(~0u, top, 1));
-            top = fmaxf(top, __shfl_xor_sync(~0u, top, 2));
-            const float now = fmaxf(m[i], top - WEIGHT_SHIFT<T>), base = now == -INFINITY ? 0.0f : now, corr = ex2(m[i] - base);
-            m[i] = now;
-            seen[i] = seen[i] || all || (there & (limit[i] >= 16 ? 0xffffu : limit[i] <= 0 ? 0u : (1u << limit[i]) - 1)) != 0;
+            const float base = m[i] == -INFINITY ? 0.0f : m[i];
             float w[4];
 #pragma unroll
             for (int h = 0; h < 2; h++) {
@@ -374,20 +398,16 @@ template <typename T, int DP> struct WarpTile {
                 w[2 * h + 1] = ex2(s[h][2 * i + 1] - base);
                 a[2 * h + i] = close_word(make_float2(w[2 * h], w[2 * h + 1]), T());
             }
-            l[i] = l[i] * corr + ((w[0] + w[1]) + (w[2] + w[3]));   // (of this lane's keys: the four lanes of a row meet at the end)
-            if (__any_sync(~0u, corr != 1.0f)) {
-#pragma unroll
-                for (int n = 0; n < DP / 8; n++) { o[n][2 * i] *= corr; o[n][2 * i + 1] *= corr; }
-            }
+            l[i] += (w[0] + w[1]) + (w[2] + w[3]);   // (of this lane's keys: the four lanes of a row meet at the end)
         }
+        const uint32_t v_row = v_at + (uint32_t)(key0 + (lane & 15)) * S::ROW, v_turn = (uint32_t)((lane >> 4) ^ (lane & 7)) << 4;
 #pragma unroll
-        for (int n = 0; n < DP / 16; n++)
-            if (16 * n < p.head_size) {
-                uint32_t b[4];
-                ldmatrix4t(b, v_at + piece_at(key0 + (lane & 15), 2 * n + (lane >> 4), S::ROW));
-                mma16816(o[2 * n], a, b[0], b[1], T());
-                mma16816(o[2 * n + 1], a, b[2], b[3], T());
-            }
+        for (int n = 0; n < DP / 16; n++) {
+            uint32_t b[4];
+            ldmatrix4t(b, v_row + (v_turn ^ (32 * n)));
+            mma16816(o[2 * n], a, b[0], b[1], T());
+            mma16816(o[2 * n + 1], a, b[2], b[3], T());
+        }
     }
     PG_DEVINL void put_ml(float2* ml) {   // [16]
         const int lane = threadIdx.x & 31;
@@ -417,7 +437,7 @@ template <int DP> struct WarpTile<float, DP> {
     static constexpr int KEYS = S::WARP_KEYS, TEAMS = 32 / KEYS, SHARE = 16 / TEAMS, COLS = DP / 32;   // lanes KEYS * i .. are team i: rows i, i + TEAMS, ...
     float o[16][COLS], m[SHARE], l[SHARE];
     bool seen[SHARE];
-    PG_DEVINL void begin(uint32_t, int) {
+    PG_DEVINL void begin(uint32_t) {
 #pragma unroll
         for (int r = 0; r < 16; r++)
 #pragma unroll
@@ -547,45 +567,47 @@ __global__ void __launch_bounds__(TileShape<T, DP>::THREADS, TileShape<T, DP>::C
     grid_launch();
     if (from >= to) return;
 
-    // copies of a thread: keys t / 4 (and t / 4 + 32) of the tile, every fourth 16 bytes
+    // copies of a thread: keys t / 4 (and t / 4 + 32) of the tile, every fourth 16 bytes; past the end of a head zeros, so that the products need not know where it is
     Place place[S::COPY_KEYS];
-    int64_t line = from, unit_no = 0;   // the tile that `ahead` stands at, and which unit of this CTA that is
+    const int n_tiles = (int)(to - from), whole = D * (int)sizeof(T) / 16;
+    int copied = 0, stage_to = 0, set_to = 0;   // tiles copied, the stage and the unit's set that the next goes to
     bool first = true;
     auto look = [&]() {
 #pragma unroll
         for (int i = 0; i < S::COPY_KEYS; i++) place[i] = unit_place(p, ahead, ahead.tile * S::KEYS + t / 4 + 32 * i);
     };
-    auto copy_tile = [&]() {   // the tile at `line`, whose places are known; then on to the next one
-        if (line < to) {
-            const int stage = (int)((line - from) % S::STAGES);
-            const uint32_t k_at = kv + stage * 2 * S::KV, v_at = k_at + S::KV;
-            const int pieces = 2 * ((D * (int)sizeof(T) + 31) / 32), whole = D * (int)sizeof(T) / 16;   // (an odd last piece is paired with zeros)
+    auto copy_tile = [&]() {   // the tile that `ahead` stands at, whose places are known; then on to the next one
+        if (copied < n_tiles) {
+            const uint32_t k_at = kv + stage_to * 2 * S::KV + (t / 4) * S::ROW, turn = (uint32_t)((t & 3) ^ (t / 4 & 7)) << 4;
 #pragma unroll
             for (int i = 0; i < S::COPY_KEYS; i++) {
                 const bool is = place[i].page >= 0;
-                const int row = t / 4 + 32 * i;
-                const T* k = p.k + (is ? place[i].page * p.k_page + place[i].place * p.k_slot + ahead.head * p.k_head : 0);
-                const T* v = p.v + (is ? place[i].page * p.v_page + place[i].place * p.v_slot + ahead.head * p.v_head : 0);
+                const int page = is ? place[i].page : 0;
+                const char* k = reinterpret_cast<const char*>(p.k + page * p.k_page + place[i].place * p.k_slot + ahead.head * p.k_head) + 16 * (t & 3);
+                const char* v = reinterpret_cast<const char*>(p.v + page * p.v_page + place[i].place * p.v_slot + ahead.head * p.v_head) + 16 * (t & 3);
+                if (whole == S::PIECES) {
 #pragma unroll
-                for (int c0 = 0; c0 < S::PIECES; c0 += 4) {
-                    const int c = c0 + (t & 3);
-                    if (c < pieces) {
-                        const bool in = is && c < whole;
-                        copy16(k_at + piece_at(row, c, S::ROW), in ? k + c * (16 / sizeof(T)) : p.k, in);
-                        copy16(v_at + piece_at(row, c, S::ROW), in ? v + c * (16 / sizeof(T)) : p.v, in);
+                    for (int c = 0; c < S::PIECES; c += 4) {
+                        copy16(k_at + 32 * i * S::ROW + (turn ^ (16 * c)), k + 16 * c, is);
+                        copy16(k_at + S::KV + 32 * i * S::ROW + (turn ^ (16 * c)), v + 16 * c, is);
+                    }
+                } else {
+#pragma unroll
+                    for (int c = 0; c < S::PIECES; c += 4) {
+                        const bool in = is && c + (t & 3) < whole;
+                        copy16(k_at + 32 * i * S::ROW + (turn ^ (16 * c)), in ? k + 16 * c : reinterpret_cast<const char*>(p.k), in);
+                        copy16(k_at + S::KV + 32 * i * S::ROW + (turn ^ (16 * c)), in ? v + 16 * c : reinterpret_cast<const char*>(p.v), in);
                     }
                 }
                 const unsigned bits = __ballot_sync(~0u, __shfl_sync(~0u, is, (4 * lane) & 31)) & 0xff;
-                if (lane == 0) there[stage][warp + 4 * i] = (uint8_t)bits;
+                if (lane == 0) there[stage_to][warp + 4 * i] = (uint8_t)bits;
             }
             if (first) {
-                const int set = (int)(unit_no % S::STAGES);
-                if (t == 0) walks[set] = ahead;
-                if (t < S::ROWS) row_keys[set][t] = unit_row(p, ahead, t).keys;
-                const uint32_t q_at = queries + set * S::Q;
+                if (t == 0) walks[set_to] = ahead;
+                if (t < S::ROWS) row_keys[set_to][t] = unit_row(p, ahead, t).keys;
+                const uint32_t q_at = queries + set_to * S::Q;
                 for (int e = t; e < S::ROWS * S::PIECES; e += S::THREADS) {
                     const int x = e / S::PIECES, c = e % S::PIECES;
-                    if (c >= pieces) continue;
                     const UnitRow r = unit_row(p, ahead, x);
                     const bool in = r.row >= 0 && c < whole;
                     const T* q = in ? p.q.data + r.row * p.q.row + r.head * p.q.head + c * (16 / sizeof(T)) : p.q.data;
@@ -601,11 +623,11 @@ __global__ void __launch_bounds__(TileShape<T, DP>::THREADS, TileShape<T, DP>::C
                 }
                 first = false;
             }
-            line++;
-            if (line < to) {
+            stage_to = stage_to + 1 == S::STAGES ? 0 : stage_to + 1;
+            if (++copied < n_tiles) {
                 if (++ahead.tile == ahead.tiles) {
                     walk_next_unit(p, ahead);
-                    unit_no++;
+                    set_to = set_to + 1 == S::STAGES ? 0 : set_to + 1;
                     first = true;
                 }
                 look();
@@ -614,31 +636,32 @@ __global__ void __launch_bounds__(TileShape<T, DP>::THREADS, TileShape<T, DP>::C
         copy_commit();
     };
     look();
-#pragma unroll
+#pragma unroll 1
     for (int i = 0; i < S::STAGES - 1; i++) copy_tile();
 
     WarpTile<T, DP> tile;
     Walk w;
-    int set = S::STAGES - 1, begun = 0, used = 0;
+    int set = S::STAGES - 1, stage = S::STAGES - 1, begun = 0, used = 0;
     bool start = true;
-    for (int64_t at = from; at < to; at++) {
+#pragma unroll 1
+    for (int at = 0; at < n_tiles; at++) {
         copy_wait<S::STAGES - 2>();
         __syncthreads();   // the tile has landed for all threads, and the one before has been worked on by all
         copy_tile();
-        const int stage = (int)((at - from) % S::STAGES);
+        stage = stage + 1 == S::STAGES ? 0 : stage + 1;
         const uint32_t k_at = kv + stage * 2 * S::KV, v_at = k_at + S::KV;
         if (start) {
             set = set + 1 == S::STAGES ? 0 : set + 1;
             w = walks[set];
             begun = w.tile;
-            tile.begin(queries + set * S::Q, D);
+            tile.begin(queries + set * S::Q);
             used = w.b < 0 ? (int)min((int64_t)S::ROWS, p.batch.n_rows * p.group - (int64_t)w.row_tile * S::ROWS) : min(S::ROWS, w.s.count * p.group - w.row_tile * S::ROWS);
             start = false;
         }
         const uint32_t bits = S::WARP_KEYS == 16 ? *reinterpret_cast<const uint16_t*>(&there[stage][2 * warp]) : there[stage][warp];
         tile.tile(p, queries + set * S::Q, k_at, v_at, bits, w.tile * S::KEYS + warp * S::WARP_KEYS, row_keys[set], used, weights[sizeof(T) == 4 ? warp : 0]);
         const bool last = w.tile + 1 == w.tiles;
-        if (last || at + 1 == to) {   // the part ends: the warps' rows meet in the tile's place
+        if (last || at + 1 == n_tiles) {   // the part ends: the warps' rows meet in the tile's place
             tile.put_ml(ml[warp]);
             if (t == 0) again = 0;
             __syncthreads();
