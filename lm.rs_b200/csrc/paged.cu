@@ -9,6 +9,7 @@
 
 #include "paged_attn.cuh"
 #include "paged_rows.cuh"
+#include "paged_tensor.cuh"
 
 using namespace lmrs;
 using namespace lmrs::paged;
@@ -243,24 +244,41 @@ namespace {
 // How a call is cut, from what the host knows of it.  The number of CTAs counts a B200's SMs: it is part of the cut, and the workspace's size goes by it
 constexpr int SMS = 148;
 struct Cutting {
-    int tile_rows, tile_keys, ctas, front_tiles;
-    int64_t front_units, slots;
-    size_t plan_at, ml_at, o_at, bytes;
+    Line own, front;   // the kernel's that takes the sequences' units, and that takes the prefix' (the same where one takes both)
+    bool own_tensor, front_tensor;
+    size_t bytes;
 };
-template <typename T, int DP> Cutting cutting(const lmrs_b200_pages_t* pages, const lmrs_b200_batch_t* batch, int64_t n_rows, int q_heads) {
-    using S = TileShape<T, DP>;
-    const int64_t rows = n_rows * (q_heads / pages->kv_heads);
+// places in the workspace, counted from `base` (null: only their sizes matter)
+void place_line(Line& l, int64_t rows, const lmrs_b200_pages_t* pages, char* base, size_t& bytes) {
+    auto take = [&](size_t n) { char* at = base + bytes; bytes += (n + 255) / 256 * 256; return at; };
+    l.slots = l.front_units + l.ctas + (l.seqs ? (rows / l.tile_rows + l.seqs) * pages->kv_heads : 0);   // (a sequence's last unit may be a part of one)
+    l.plan = (Plan*)take(sizeof(Plan) * ((size_t)l.seqs + 1));
+    l.ml = (float2*)take(sizeof(float2) * (size_t)l.slots * l.tile_rows);
+    l.o = (float*)take(sizeof(float) * (size_t)l.slots * l.tile_rows * pages->head_size);
+}
+// Which kernel takes what.  16-bit types: rows128_kernel takes the prefix from TENSOR_ROWS rows a KV head on, and a call with more than that many in one
+// sequence altogether; rows16_kernel the rest, and everything in float32.
+constexpr int TENSOR_ROWS = 32;
+template <typename T, int DP> Cutting cutting(const lmrs_b200_pages_t* pages, const lmrs_b200_batch_t* batch, int64_t n_rows, int q_heads, char* base) {
+    const int64_t group = q_heads / pages->kv_heads, rows = n_rows * group;
     Cutting c = {};
-    c.tile_rows = S::ROWS;
-    c.tile_keys = S::KEYS;
-    c.ctas = SMS * S::CTAS;
-    c.front_tiles = (int)(((int64_t)batch->prefix_len + S::KEYS - 1) / S::KEYS);
-    c.front_units = c.front_tiles ? (rows + S::ROWS - 1) / S::ROWS * pages->kv_heads : 0;
-    c.slots = c.front_units + (rows / S::ROWS + batch->seqs) * pages->kv_heads + c.ctas;   // (a sequence's last unit may be a part of one)
-    auto take = [&](size_t n) { const size_t at = c.bytes; c.bytes += (n + 255) / 256 * 256; return at; };
-    c.plan_at = take(sizeof(Plan) * ((size_t)batch->seqs + 1));
-    c.ml_at = take(sizeof(float2) * (size_t)c.slots * S::ROWS);
-    c.o_at = take(sizeof(float) * (size_t)c.slots * S::ROWS * pages->head_size);
+    auto line = [&](Line& l, bool tensor, bool own, bool front) {
+        int tile_rows = TileShape<T, DP>::ROWS, tile_keys = TileShape<T, DP>::KEYS, ctas = SMS * TileShape<T, DP>::CTAS;
+        if constexpr (sizeof(T) == 2)
+            if (tensor) { tile_rows = TensorShape<T, DP>::ROWS; tile_keys = TensorShape<T, DP>::KEYS; ctas = SMS; }
+        l.tile_rows = tile_rows;
+        l.tile_keys = tile_keys;
+        l.ctas = ctas;
+        l.seqs = own ? batch->seqs : 0;
+        l.front_tiles = front ? (int)(((int64_t)batch->prefix_len + tile_keys - 1) / tile_keys) : 0;
+        l.front_units = l.front_tiles ? (rows + tile_rows - 1) / tile_rows * pages->kv_heads : 0;
+        place_line(l, rows, pages, base, c.bytes);
+    };
+    c.own_tensor = sizeof(T) == 2 && std::min<int64_t>(batch->max_rows, n_rows) * group >= TENSOR_ROWS;
+    c.front_tensor = c.own_tensor || (sizeof(T) == 2 && rows >= TENSOR_ROWS && batch->prefix_len > 0);
+    line(c.own, c.own_tensor, true, c.own_tensor == c.front_tensor);
+    if (c.own_tensor == c.front_tensor) c.front = c.own;
+    else line(c.front, true, false, true);
     return c;
 }
 template <typename F> int by_shape(const lmrs_b200_pages_t* pages, F f) {
@@ -278,7 +296,7 @@ template <typename K> cudaError_t allow_smem(K kernel, int device, int bytes, st
     return e;
 }
 // a kernel that may be set up while the one before it still runs, and waits for its results by itself
-template <typename K, typename P> cudaError_t launch_after(K kernel, unsigned grid, unsigned threads, size_t smem, cudaStream_t stream, const P& p) {
+template <typename K, typename... P> cudaError_t launch_after(K kernel, unsigned grid, unsigned threads, size_t smem, cudaStream_t stream, const P&... p) {
     cudaLaunchConfig_t c = {};
     c.gridDim = dim3(grid);
     c.blockDim = dim3(threads);
@@ -289,7 +307,7 @@ template <typename K, typename P> cudaError_t launch_after(K kernel, unsigned gr
     a.val.programmaticStreamSerializationAllowed = 1;
     c.attrs = &a;
     c.numAttrs = 1;
-    return cudaLaunchKernelEx(&c, kernel, p);
+    return cudaLaunchKernelEx(&c, kernel, p...);
 }
 
 }  // namespace
@@ -303,7 +321,7 @@ extern "C" int lmrs_b200_paged_attention_workspace(const lmrs_b200_pages_t* page
         *bytes = 0;
         if (n_rows == 0 || batch->seqs == 0) return 0;
         return by_shape(pages, [&](auto t, auto d) {
-            *bytes = cutting<decltype(t), decltype(d)::value>(pages, batch, n_rows, q_heads).bytes;
+            *bytes = cutting<decltype(t), decltype(d)::value>(pages, batch, n_rows, q_heads, nullptr).bytes;
             return 0;
         });
     });
@@ -331,7 +349,7 @@ extern "C" int lmrs_b200_paged_attention(const lmrs_b200_pages_t* pages, const l
         return by_shape(pages, [&](auto t, auto d) {
             using T = decltype(t);
             using S = TileShape<T, decltype(d)::value>;
-            const Cutting c = cutting<T, decltype(d)::value>(pages, batch, n_rows, q_heads);
+            const Cutting c = cutting<T, decltype(d)::value>(pages, batch, n_rows, q_heads, (char*)workspace);
             if (workspace_bytes < c.bytes) return refuse(me, "workspace has " + std::to_string(workspace_bytes) + " bytes, the call needs " + std::to_string(c.bytes));
             AttnParams<T> p = {};
             p.batch = batch_as(batch, pages, n_rows);
@@ -344,21 +362,29 @@ extern "C" int lmrs_b200_paged_attention(const lmrs_b200_pages_t* pages, const l
             p.scale2 = scale * LOG2E; p.softcap = softcap; p.cap_in = softcap > 0.0f ? scale / softcap : 0.0f; p.lse = lse;
             p.q_wide = vectors(q, dtype);
             p.out_wide = aligned(out->data, 4 * sizeof(T)) && out->row % 4 == 0 && out->head % 4 == 0;
-            p.tile_rows = c.tile_rows; p.tile_keys = c.tile_keys; p.ctas = c.ctas; p.front_units = c.front_units; p.front_tiles = c.front_tiles;
-            p.plan = (Plan*)((char*)workspace + c.plan_at);
-            p.part_ml = (float2*)((char*)workspace + c.ml_at);
-            p.part_o = (float*)((char*)workspace + c.o_at);
-            p.slots = c.slots;
-            static std::atomic<uint64_t> allowed{0};
-            auto kernel = rows16_kernel<T, decltype(d)::value>;
-            cudaError_t e = allow_smem(kernel, device, S::SMEM, allowed);
-            if (e != cudaSuccess) return refuse(me, cudaGetErrorString(e));
-            kernel<<<(unsigned)c.ctas, S::THREADS, S::SMEM, (cudaStream_t)stream>>>(p);
-            if (launched(me)) return 1;
+            p.whole = batch->prefix_len == 0;
+            static std::atomic<uint64_t> allowed{0}, allowed_tensor{0};
+            cudaError_t e = cudaSuccess;
+            if constexpr (sizeof(T) == 2)
+                if (c.front_tensor) {
+                    auto kernel = rows128_kernel<T, decltype(d)::value>;
+                    using X = TensorShape<T, decltype(d)::value>;
+                    if ((e = allow_smem(kernel, device, X::SMEM, allowed_tensor)) != cudaSuccess) return refuse(me, cudaGetErrorString(e));
+                    kernel<<<(unsigned)c.front.ctas, X::THREADS, X::SMEM, (cudaStream_t)stream>>>(p, c.front);
+                    if (launched(me)) return 1;
+                }
+            if (!c.own_tensor) {
+                auto kernel = rows16_kernel<T, decltype(d)::value>;
+                if ((e = allow_smem(kernel, device, S::SMEM, allowed)) != cudaSuccess) return refuse(me, cudaGetErrorString(e));
+                if (c.front_tensor) e = launch_after(kernel, (unsigned)c.own.ctas, S::THREADS, S::SMEM, (cudaStream_t)stream, p, c.own);
+                else kernel<<<(unsigned)c.own.ctas, S::THREADS, S::SMEM, (cudaStream_t)stream>>>(p, c.own);
+                if (e != cudaSuccess) return refuse(me, std::string("launch failed: ") + cudaGetErrorString(e));
+                if (launched(me)) return 1;
+            }
             // a warp a row and head, or 8 while that leaves warps on the GPU idle
             const int64_t items = n_rows * q_heads;
-            e = items <= SMS * 16 ? launch_after(join_kernel<T, 8>, (unsigned)items, 256, 0, (cudaStream_t)stream, p)
-                                  : launch_after(join_kernel<T, 1>, (unsigned)std::min<int64_t>((items + 7) / 8, SMS * 16), 256, 0, (cudaStream_t)stream, p);
+            e = items <= SMS * 16 ? launch_after(join_kernel<T, 8>, (unsigned)items, 256, 0, (cudaStream_t)stream, p, c.front, c.own)
+                                  : launch_after(join_kernel<T, 1>, (unsigned)std::min<int64_t>((items + 7) / 8, SMS * 16), 256, 0, (cudaStream_t)stream, p, c.front, c.own);
             return e == cudaSuccess ? 0 : refuse(me, std::string("launch failed: ") + cudaGetErrorString(e));
         });
     });

@@ -44,16 +44,20 @@ template <typename T> struct AttnParams {
     float scale2, softcap, cap_in;             // scores: scale2 = scale * log2 e; or softcap * log2 e * tanh(dot * cap_in), cap_in = scale / softcap
     float* lse;
     bool q_wide, out_wide;                     // rows on 16-byte boundaries
-    // the line: units of the prefix stand before those of the sequences
+    bool whole;                                // no prefix: a unit that one CTA takes is finished there
+};
+// What one kernel goes through: units of the prefix (if it takes them), then those of the sequences (if it takes them)
+struct Line {
     int tile_rows, tile_keys, ctas;
+    int seqs, front_tiles;                     // 0: not this kernel's; front_tiles: tiles of every unit of the prefix
     int64_t front_units;                       // kv_heads * tiles of rows
-    int front_tiles;                           // of each
     // workspace
     Plan* plan;        // [seqs + 1]
-    float2* part_ml;   // [slots][tile_rows]
-    float* part_o;     // [slots][tile_rows][head_size]
+    float2* ml;        // [slots][tile_rows]
+    float* o;          // [slots][head_size / 8][tile_rows][8]: whole sectors for kernels whose threads hold rows, and for those whose lanes lie along them
     int64_t slots;     // part of unit u by CTA c: u + c (each step along the line goes on to another unit, another CTA or both)
 };
+PG_DEVINL float* part_at(const Line& l, int head_size, int64_t slot, int row, int c) { return l.o + ((slot * (head_size >> 3) + (c >> 3)) * l.tile_rows + row) * 8 + (c & 7); }
 
 // (no more CTAs than tiles, so that each that takes part has some, and the parts of a unit are those of neighbours)
 PG_DEVINL int64_t cta_begin(int64_t total, int ctas, int i) {
@@ -69,14 +73,14 @@ template <typename T> PG_DEVINL int keys_upto(const AttnParams<T>& p, int64_t in
     const int64_t most = (int64_t)p.batch.table_len * p.batch.page_size, n = index + 1;
     return n <= 0 ? 0 : (int)(n < most ? n : most);
 }
-template <typename T> PG_DEVINL int unit_keys(const AttnParams<T>& p, const Span& s, int tile) {
-    const int last = min(s.count * p.group, (tile + 1) * p.tile_rows) - 1;
+template <typename T> PG_DEVINL int unit_keys(const AttnParams<T>& p, const Line& l, const Span& s, int tile) {
+    const int last = min(s.count * p.group, (tile + 1) * l.tile_rows) - 1;
     return keys_upto(p, (int64_t)s.len - s.count + last / p.group);
 }
-template <typename T> PG_DEVINL int unit_tiles(const AttnParams<T>& p, const Span& s, int tile) { return (unit_keys(p, s, tile) + p.tile_keys - 1) / p.tile_keys; }
-template <typename T> PG_DEVINL int64_t seq_tiles(const AttnParams<T>& p, const Span& s) {
+template <typename T> PG_DEVINL int unit_tiles(const AttnParams<T>& p, const Line& l, const Span& s, int tile) { return (unit_keys(p, l, s, tile) + l.tile_keys - 1) / l.tile_keys; }
+template <typename T> PG_DEVINL int64_t seq_tiles(const AttnParams<T>& p, const Line& l, const Span& s) {
     int64_t n = 0;
-    for (int t = unit_rows(s, p.group, p.tile_rows) - 1; t >= 0; t--) n += unit_tiles(p, s, t);
+    for (int t = unit_rows(s, p.group, l.tile_rows) - 1; t >= 0; t--) n += unit_tiles(p, l, s, t);
     return n * p.kv_heads;
 }
 
@@ -87,40 +91,40 @@ struct Walk {
     int tile, tiles, keys;     // tile of keys, how many the unit has, its keys
     Span s;
 };
-template <typename T> PG_DEVINL void walk_unit(const AttnParams<T>& p, Walk& w) {   // fills in the keys of the unit that b, head and row_tile name
-    w.keys = w.b < 0 ? p.batch.prefix_len : unit_keys(p, w.s, w.row_tile);
-    w.tiles = (w.keys + p.tile_keys - 1) / p.tile_keys;
+template <typename T> PG_DEVINL void walk_unit(const AttnParams<T>& p, const Line& l, Walk& w) {   // fills in the keys of the unit that b, head and row_tile name
+    w.keys = w.b < 0 ? p.batch.prefix_len : unit_keys(p, l, w.s, w.row_tile);
+    w.tiles = (w.keys + l.tile_keys - 1) / l.tile_keys;
 }
 // the next unit that has tiles; KV heads lie innermost
-template <typename T> PG_DEVINL void walk_next_unit(const AttnParams<T>& p, Walk& w) {
+template <typename T> PG_DEVINL void walk_next_unit(const AttnParams<T>& p, const Line& l, Walk& w) {
     do {
         w.unit++;
         if (++w.head == p.kv_heads) {
             w.head = 0;
             w.row_tile++;
-            if (w.b < 0 ? w.unit >= p.front_units : w.row_tile >= unit_rows(w.s, p.group, p.tile_rows)) {
+            if (w.b < 0 ? w.unit >= l.front_units : w.row_tile >= unit_rows(w.s, p.group, l.tile_rows)) {
                 w.row_tile = 0;
                 do {
                     w.b++;
-                    if (w.b >= p.batch.seqs) { w.tiles = w.keys = 0; return; }   // the end of the line
+                    if (w.b >= l.seqs) { w.tiles = w.keys = 0; return; }   // the end of the line
                     w.s = span_of(p.batch, w.b);
                 } while (w.s.count == 0);
             }
         }
-        walk_unit(p, w);
+        walk_unit(p, l, w);
     } while (w.tiles == 0);
     w.tile = 0;
 }
 // All threads: the whole line's length, and the CTA's place where it begins (`from` is that tile's number).  CTA 0 leaves the plan for join_kernel
 template <typename T, int THREADS>
-PG_DEVINL int64_t walk_begin(const AttnParams<T>& p, Walk& w, int64_t& from, int64_t& to) {
+PG_DEVINL int64_t walk_begin(const AttnParams<T>& p, const Line& l, Walk& w, int64_t& from, int64_t& to) {
     __shared__ int64_t warp_tiles[THREADS / 32], warp_units[THREADS / 32], found[3];
-    const int t = threadIdx.x, lane = t & 31, each = (p.batch.seqs + THREADS - 1) / THREADS, b0 = min(p.batch.seqs, t * each), b1 = min(p.batch.seqs, b0 + each);
+    const int t = threadIdx.x, lane = t & 31, each = (l.seqs + THREADS - 1) / THREADS, b0 = min(l.seqs, t * each), b1 = min(l.seqs, b0 + each);
     int64_t tiles = 0, units = 0;
     for (int b = b0; b < b1; b++) {
         const Span s = span_of(p.batch, b);
-        tiles += seq_tiles(p, s);
-        units += (int64_t)unit_rows(s, p.group, p.tile_rows) * p.kv_heads;
+        tiles += seq_tiles(p, l, s);
+        units += (int64_t)unit_rows(s, p.group, l.tile_rows) * p.kv_heads;
     }
     int64_t tiles_to = tiles, units_to = units;   // up to and with this thread's
     for (int o = 1; o < 32; o <<= 1) {
@@ -130,31 +134,31 @@ PG_DEVINL int64_t walk_begin(const AttnParams<T>& p, Walk& w, int64_t& from, int
     if (lane == 31) { warp_tiles[t >> 5] = tiles_to; warp_units[t >> 5] = units_to; }
     if (t == 0) found[0] = found[1] = found[2] = 0;
     __syncthreads();
-    const int64_t front = p.front_units * p.front_tiles;
+    const int64_t front = l.front_units * l.front_tiles;
     int64_t total = front;
     tiles_to += front;
-    units_to += p.front_units;
+    units_to += l.front_units;
     for (int i = 0; i < THREADS / 32; i++) {
         if (i < t >> 5) { tiles_to += warp_tiles[i]; units_to += warp_units[i]; }
         total += warp_tiles[i];
     }
-    from = cta_begin(total, p.ctas, blockIdx.x);
-    to = cta_begin(total, p.ctas, blockIdx.x + 1);
+    from = cta_begin(total, l.ctas, blockIdx.x);
+    to = cta_begin(total, l.ctas, blockIdx.x + 1);
     if (blockIdx.x == 0) {
         int64_t at = tiles_to - tiles, u = units_to - units;
         for (int b = b0; b < b1; b++) {
             const Span s = span_of(p.batch, b);
-            p.plan[b] = Plan{at, u};
-            at += seq_tiles(p, s);
-            u += (int64_t)unit_rows(s, p.group, p.tile_rows) * p.kv_heads;
+            l.plan[b] = Plan{at, u};
+            at += seq_tiles(p, l, s);
+            u += (int64_t)unit_rows(s, p.group, l.tile_rows) * p.kv_heads;
         }
-        if (t == 0) p.plan[p.batch.seqs] = Plan{total, 0};
+        if (t == 0) l.plan[l.seqs] = Plan{total, 0};
     }
     if (from >= front && from < to && tiles_to - tiles <= from && from < tiles_to) {   // one thread's sequences hold it
         int64_t at = tiles_to - tiles, u = units_to - units;
         for (int b = b0; b < b1; b++) {
             const Span s = span_of(p.batch, b);
-            const int64_t n = seq_tiles(p, s);
+            const int64_t n = seq_tiles(p, l, s);
             if (from < at + n) {
                 found[0] = b;
                 found[1] = at;
@@ -162,37 +166,37 @@ PG_DEVINL int64_t walk_begin(const AttnParams<T>& p, Walk& w, int64_t& from, int
                 break;
             }
             at += n;
-            u += (int64_t)unit_rows(s, p.group, p.tile_rows) * p.kv_heads;
+            u += (int64_t)unit_rows(s, p.group, l.tile_rows) * p.kv_heads;
         }
     }
     __syncthreads();
     if (from >= to) return total;
     if (from < front) {
-        w.unit = from / p.front_tiles;
+        w.unit = from / l.front_tiles;
         w.b = -1;
         w.row_tile = (int)(w.unit / p.kv_heads);
         w.head = (int)(w.unit - (int64_t)w.row_tile * p.kv_heads);
-        w.tile = (int)(from - w.unit * p.front_tiles);
+        w.tile = (int)(from - w.unit * l.front_tiles);
     } else {
         w.b = (int)found[0];
         w.s = span_of(p.batch, w.b);
         int64_t left = from - found[1];
-        int n = unit_tiles(p, w.s, 0);
+        int n = unit_tiles(p, l, w.s, 0);
         w.row_tile = 0;
-        for (const int rows = unit_rows(w.s, p.group, p.tile_rows); w.row_tile + 1 < rows && left >= (int64_t)n * p.kv_heads; n = unit_tiles(p, w.s, ++w.row_tile)) left -= (int64_t)n * p.kv_heads;
+        for (const int rows = unit_rows(w.s, p.group, l.tile_rows); w.row_tile + 1 < rows && left >= (int64_t)n * p.kv_heads; n = unit_tiles(p, l, w.s, ++w.row_tile)) left -= (int64_t)n * p.kv_heads;
         n = max(n, 1);   // (it is; lengths that change under the kernel may make it otherwise)
         w.head = min((int)(left / n), p.kv_heads - 1);
         w.tile = (int)(left - (int64_t)w.head * n);
         w.unit = found[2] + (int64_t)w.row_tile * p.kv_heads + w.head;
     }
-    walk_unit(p, w);
+    walk_unit(p, l, w);
     return total;
 }
 
 // What row `x` of a unit is: its row of the call's arrays (-1: none), its query head, and how many of the unit's keys it sees
 struct UnitRow { int64_t row; int head, keys; };
-template <typename T> PG_DEVINL UnitRow unit_row(const AttnParams<T>& p, const Walk& w, int x) {
-    const int i = w.row_tile * p.tile_rows + x, token = i / p.group;
+template <typename T> PG_DEVINL UnitRow unit_row(const AttnParams<T>& p, const Line& l, const Walk& w, int x) {
+    const int i = w.row_tile * l.tile_rows + x, token = i / p.group;
     UnitRow r = {-1, w.head * p.group + (i - token * p.group), w.keys};   // (rows that are not there see all, so that they need no mask)
     if (w.b < 0) {
         if (token < p.batch.n_rows) r.row = token;
@@ -228,21 +232,22 @@ template <typename T> PG_DEVINL void store_row(const AttnParams<T>& p, const Uni
     }
 }
 
-// A row of a unit once more, keys `from` to `to` - 1 of the unit, by all threads of the CTA: only keys that the row sees are touched.  In the matrix products a
-// value that is not finite spoils, through its weight 0, also the rows of the tile that do not see it.  acc[i]: column threadIdx.x + i * THREADS, unnormalised.
+// A row of a unit once more, keys `from` to `to` - 1 of the unit, by 128 threads that share a named barrier: only keys that the row sees are touched.  In the matrix products a
+// value that is not finite spoils, through its weight 0, also the rows of the tile that do not see it.  acc[i]: column threadIdx.x % 128 + 128 i, unnormalised.
 // Rows that come out finite never come here.
-template <typename T, int THREADS>
-static __device__ __noinline__ void row_again(const AttnParams<T>& p, const Walk& w, const UnitRow& r, int from, int to, float& m, float& l, float (&acc)[256 / THREADS]) {
-    __shared__ float weight[THREADS], most[THREADS / 32];
-    __shared__ int64_t at[THREADS];
-    const int t = threadIdx.x, D = p.head_size;
+constexpr int AGAIN = 128;
+struct AgainScratch { float weight[AGAIN], most[AGAIN / 32]; int64_t at[AGAIN]; };
+PG_DEVINL void again_sync(int barrier) { asm volatile("bar.sync %0, %1;" ::"r"(barrier), "n"(AGAIN) : "memory"); }
+template <typename T>
+static __device__ __noinline__ void row_again(const AttnParams<T>& p, const Walk& w, const UnitRow& r, int from, int to, AgainScratch& sc, int barrier, float& m, float& l, float (&acc)[2]) {
+    const int t = threadIdx.x & (AGAIN - 1), D = p.head_size;
     const T* q = p.q.data + r.row * p.q.row + r.head * p.q.head;
     m = -INFINITY;
     l = 0.0f;
 #pragma unroll
-    for (int i = 0; i < 256 / THREADS; i++) acc[i] = 0.0f;
+    for (int i = 0; i < 2; i++) acc[i] = 0.0f;
     to = min(to, r.keys);
-    for (int x0 = from; x0 < to; x0 += THREADS) {
+    for (int x0 = from; x0 < to; x0 += AGAIN) {
         Place at_x = {-1, 0};
         if (x0 + t < to) at_x = unit_place(p, w, x0 + t);
         const bool there = at_x.page >= 0;
@@ -255,32 +260,32 @@ static __device__ __noinline__ void row_again(const AttnParams<T>& p, const Walk
         }
         float top = a;
         for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(~0u, top, o));
-        __syncthreads();
-        at[t] = there ? at_x.page * p.v_page + at_x.place * p.v_slot + w.head * p.v_head : -1;
-        if ((t & 31) == 0) most[t >> 5] = top;
-        __syncthreads();
+        again_sync(barrier);
+        sc.at[t] = there ? at_x.page * p.v_page + at_x.place * p.v_slot + w.head * p.v_head : -1;
+        if ((t & 31) == 0) sc.most[t >> 5] = top;
+        again_sync(barrier);
         float now = m;
-        for (int i = 0; i < THREADS / 32; i++) now = fmaxf(now, most[i]);
+        for (int i = 0; i < AGAIN / 32; i++) now = fmaxf(now, sc.most[i]);
         const float base = now == -INFINITY ? 0.0f : now, corr = ex2(m - base);
-        weight[t] = there ? ex2(a - base) : 0.0f;
+        sc.weight[t] = there ? ex2(a - base) : 0.0f;
         m = now;
-        __syncthreads();
+        again_sync(barrier);
         l *= corr;
-        for (int i = 0; i < THREADS; i++) l += weight[i];
+        for (int i = 0; i < AGAIN; i++) l += sc.weight[i];
 #pragma unroll
-        for (int c = 0; c < 256 / THREADS; c++)
-            if (t + c * THREADS < D) {
+        for (int c = 0; c < 2; c++)
+            if (t + c * AGAIN < D) {
                 acc[c] *= corr;
-                for (int i = 0; i < THREADS; i++)
-                    if (at[i] >= 0) acc[c] = fmaf(weight[i], to_f(p.v[at[i] + t + c * THREADS]), acc[c]);
+                for (int i = 0; i < AGAIN; i++)
+                    if (sc.at[i] >= 0) acc[c] = fmaf(sc.weight[i], to_f(p.v[sc.at[i] + t + c * AGAIN]), acc[c]);
             }
     }
-    __syncthreads();
+    again_sync(barrier);
 }
 
 // A part's row leaves as (m, l) and o in the workspace, or as a result.  l = -1: the part holds no key that the row sees
 PG_DEVINL float lse_of(float m, float l) { return ((m == -INFINITY ? 0.0f : m) + log2f(l)) * LN2; }
-template <typename T> PG_DEVINL bool whole_unit(const AttnParams<T>& p, const Walk& w, int first, int last) { return w.b >= 0 && p.front_tiles == 0 && first == 0 && last == w.tiles - 1; }
+template <typename T> PG_DEVINL bool whole_unit(const AttnParams<T>& p, const Walk& w, int first, int last) { return w.b >= 0 && p.whole && first == 0 && last == w.tiles - 1; }
 
 // ---- 16 rows a unit ------------------------------------------------------------------------------------------------------------------------
 // CTA = 4 warps that share a tile's keys, each with the running (m, l, o) of all 16 rows over its keys; they meet when a part ends.  What bounds it is the
@@ -549,7 +554,7 @@ template <int DP> struct WarpTile<float, DP> {
 
 // (the f32 sums' 128 registers for heads of 256 leave no room for more than one CTA anyway)
 template <typename T, int DP>
-__global__ void __launch_bounds__(TileShape<T, DP>::THREADS, TileShape<T, DP>::CTAS) rows16_kernel(const __grid_constant__ AttnParams<T> p) {
+__global__ void __launch_bounds__(TileShape<T, DP>::THREADS, TileShape<T, DP>::CTAS) rows16_kernel(const __grid_constant__ AttnParams<T> p, const __grid_constant__ Line l) {
     using S = TileShape<T, DP>;
     extern __shared__ __align__(1024) uint8_t smem[];
     __shared__ Walk walks[S::STAGES];             // of the units that copies have got to, by their number in this CTA modulo STAGES
@@ -558,14 +563,15 @@ __global__ void __launch_bounds__(TileShape<T, DP>::THREADS, TileShape<T, DP>::C
     __shared__ float2 ml[4][S::ROWS];
     __shared__ __align__(16) float factor[4][S::ROWS], weights[sizeof(T) == 4 ? 4 : 1][sizeof(T) == 4 ? (S::WARP_KEYS + 1) * 16 : 1];
     __shared__ unsigned again;
+    __shared__ AgainScratch scratch;
     const int t = threadIdx.x, lane = t & 31, warp = t >> 5, D = p.head_size;
     const uint32_t kv = smem_at(smem), queries = kv + S::STAGES * 2 * S::KV;
 
     Walk ahead;   // where copies are
     int64_t from, to;
-    walk_begin<T, S::THREADS>(p, ahead, from, to);
+    walk_begin<T, S::THREADS>(p, l, ahead, from, to);
     grid_launch();
-    if (from >= to) return;
+    if (from >= to) { grid_wait(); return; }   // (the kernel before may still run: whoever waits for this one waits for both)
 
     // copies of a thread: keys t / 4 (and t / 4 + 32) of the tile, every fourth 16 bytes; past the end of a head zeros, so that the products need not know where it is
     Place place[S::COPY_KEYS];
@@ -604,11 +610,11 @@ __global__ void __launch_bounds__(TileShape<T, DP>::THREADS, TileShape<T, DP>::C
             }
             if (first) {
                 if (t == 0) walks[set_to] = ahead;
-                if (t < S::ROWS) row_keys[set_to][t] = unit_row(p, ahead, t).keys;
+                if (t < S::ROWS) row_keys[set_to][t] = unit_row(p, l, ahead, t).keys;
                 const uint32_t q_at = queries + set_to * S::Q;
                 for (int e = t; e < S::ROWS * S::PIECES; e += S::THREADS) {
                     const int x = e / S::PIECES, c = e % S::PIECES;
-                    const UnitRow r = unit_row(p, ahead, x);
+                    const UnitRow r = unit_row(p, l, ahead, x);
                     const bool in = r.row >= 0 && c < whole;
                     const T* q = in ? p.q.data + r.row * p.q.row + r.head * p.q.head + c * (16 / sizeof(T)) : p.q.data;
                     const uint32_t at = q_at + piece_at(x, c, S::ROW);
@@ -626,7 +632,7 @@ __global__ void __launch_bounds__(TileShape<T, DP>::THREADS, TileShape<T, DP>::C
             stage_to = stage_to + 1 == S::STAGES ? 0 : stage_to + 1;
             if (++copied < n_tiles) {
                 if (++ahead.tile == ahead.tiles) {
-                    walk_next_unit(p, ahead);
+                    walk_next_unit(p, l, ahead);
                     set_to = set_to + 1 == S::STAGES ? 0 : set_to + 1;
                     first = true;
                 }
@@ -666,7 +672,7 @@ __global__ void __launch_bounds__(TileShape<T, DP>::THREADS, TileShape<T, DP>::C
             if (t == 0) again = 0;
             __syncthreads();
             if (t < S::ROWS) {
-                float m = -INFINITY, l = 0.0f;
+                float m = -INFINITY, sum = 0.0f;
                 bool any = false;
                 for (int i = 0; i < 4; i++)
                     if (ml[i][t].y >= 0.0f || ml[i][t].y != ml[i][t].y) { m = fmaxf(m, ml[i][t].x); any = true; }
@@ -674,9 +680,9 @@ __global__ void __launch_bounds__(TileShape<T, DP>::THREADS, TileShape<T, DP>::C
                 for (int i = 0; i < 4; i++) {
                     const bool has = !(ml[i][t].y < 0.0f);
                     factor[i][t] = has ? ex2(ml[i][t].x - base) : 0.0f;
-                    if (has) l += ml[i][t].y * factor[i][t];
+                    if (has) sum += ml[i][t].y * factor[i][t];
                 }
-                ml[0][t] = make_float2(m, any ? l : -1.0f);
+                ml[0][t] = make_float2(m, any ? sum : -1.0f);
             }
             __syncthreads();
             float* rows = reinterpret_cast<float*>(smem + stage * 2 * S::KV);
@@ -698,32 +704,32 @@ __global__ void __launch_bounds__(TileShape<T, DP>::THREADS, TileShape<T, DP>::C
                 }
                 if (!isfinite(v.x + v.y + v.z + v.w) && w.b >= 0 && w.s.count > 1) atomicOr(&again, 1u << x);
                 if (whole) {
-                    const UnitRow r = unit_row(p, w, x);
+                    const UnitRow r = unit_row(p, l, w, x);
                     if (!(s.y < 0.0f)) { v.x /= s.y; v.y /= s.y; v.z /= s.y; v.w /= s.y; }
                     store_row(p, r, c, v);
                     if (c == 0 && p.lse) p.lse[r.row * p.q_heads + r.head] = s.y < 0.0f ? -INFINITY : lse_of(s.x, s.y);
-                } else if (slot < p.slots) {
-                    *reinterpret_cast<float4*>(p.part_o + (slot * S::ROWS + x) * D + c) = v;
-                    if (c == 0) p.part_ml[slot * S::ROWS + x] = s;
+                } else if (slot < l.slots) {
+                    *reinterpret_cast<float4*>(part_at(l, D, slot, x, c)) = v;
+                    if (c == 0) l.ml[slot * S::ROWS + x] = s;
                 }
             }
             __syncthreads();
             for (unsigned left = again; left; left &= left - 1) {   // (the same for all threads)
                 const int x = __ffs(left) - 1;
-                const UnitRow r = unit_row(p, w, x);
+                const UnitRow r = unit_row(p, l, w, x);
                 if (ml[0][x].y < 0.0f) continue;
-                float m, l, acc[256 / S::THREADS];
-                row_again<T, S::THREADS>(p, w, r, begun * S::KEYS, (w.tile + 1) * S::KEYS, m, l, acc);
+                float m, sum, acc[2];
+                row_again(p, w, r, begun * S::KEYS, (w.tile + 1) * S::KEYS, scratch, 0, m, sum, acc);
 #pragma unroll
-                for (int i = 0; i < 256 / S::THREADS; i++) {
-                    const int c = t + i * S::THREADS;
+                for (int i = 0; i < 2; i++) {
+                    const int c = t + AGAIN * i;
                     if (c >= D) continue;
-                    if (whole) p.out.data[r.row * p.out.row + r.head * p.out.head + c] = from_f<T>(acc[i] / l);
-                    else if (slot < p.slots) p.part_o[(slot * S::ROWS + x) * D + c] = acc[i];
+                    if (whole) p.out.data[r.row * p.out.row + r.head * p.out.head + c] = from_f<T>(acc[i] / sum);
+                    else if (slot < l.slots) *part_at(l, D, slot, x, c) = acc[i];
                 }
                 if (t == 0) {
-                    if (whole) { if (p.lse) p.lse[r.row * p.q_heads + r.head] = lse_of(m, l); }
-                    else if (slot < p.slots) p.part_ml[slot * S::ROWS + x] = make_float2(m, l);
+                    if (whole) { if (p.lse) p.lse[r.row * p.q_heads + r.head] = lse_of(m, sum); }
+                    else if (slot < l.slots) l.ml[slot * S::ROWS + x] = make_float2(m, sum);
                 }
             }
         }
@@ -731,13 +737,14 @@ __global__ void __launch_bounds__(TileShape<T, DP>::THREADS, TileShape<T, DP>::C
         start = last;
     }
     copy_wait<0>();
+    grid_wait();
 }
 
 // ---- joining parts ---------------------------------------------------------------------------------------------------------------------------
 // WARPS warps a row and head, their lanes its columns in fours: each takes every WARPS-th part with a running (m, l, o), and they meet in shared memory.  8 where
 // rows are few and may have many parts, 1 otherwise (then a CTA has 8 rows or heads).
 template <typename T, int WARPS>
-__global__ void __launch_bounds__(256) join_kernel(const __grid_constant__ AttnParams<T> p) {
+__global__ void __launch_bounds__(256) join_kernel(const __grid_constant__ AttnParams<T> p, const __grid_constant__ Line lf, const __grid_constant__ Line lo) {
     constexpr int ITEMS = 8 / WARPS;
     __shared__ float2 ml[8];
     __shared__ float4 sums[8][64];
@@ -756,38 +763,37 @@ __global__ void __launch_bounds__(256) join_kernel(const __grid_constant__ AttnP
         const int g = head / p.group, gi = head - g * p.group;
         if (out) {
             const Span s = span_of(p.batch, b);
-            const int i = (int)(r - s.first), x = i * p.group + gi, row_tile = x / p.tile_rows, tiles = unit_tiles(p, s, row_tile);
+            const int i = (int)(r - s.first), x = i * p.group + gi, row_tile = x / lo.tile_rows, tiles = unit_tiles(p, lo, s, row_tile);
             const int64_t index = (int64_t)s.len - s.count + i;
-            // the parts of its own unit: numbers c0 .. c1 (none: c1 < c0)
+            // the parts of its own unit: those of CTAs c0 .. c1 (none: c1 < c0)
             int64_t before = 0;
-            for (int t = lane; t < row_tile; t += 32) before += unit_tiles(p, s, t);
+            for (int t = lane; t < row_tile; t += 32) before += unit_tiles(p, lo, s, t);
             for (int d = 16; d; d >>= 1) before += __shfl_xor_sync(~0u, before, d);
-            const Plan plan = p.plan[b];
-            const int64_t total = p.plan[p.batch.seqs].tiles;
-            const int64_t tile0 = plan.tiles + before * p.kv_heads + (int64_t)g * tiles, unit = plan.units + (int64_t)row_tile * p.kv_heads + g;
-            const int c0 = tiles ? cta_of(total, p.ctas, tile0) : 0, c1 = tiles ? cta_of(total, p.ctas, tile0 + tiles - 1) : -1;
+            const Plan plan = lo.plan[b];
+            const int64_t total = lo.plan[lo.seqs].tiles, tile0 = plan.tiles + before * p.kv_heads + (int64_t)g * tiles, unit = plan.units + (int64_t)row_tile * p.kv_heads + g;
+            const int c0 = tiles ? cta_of(total, lo.ctas, tile0) : 0, c1 = tiles ? cta_of(total, lo.ctas, tile0 + tiles - 1) : -1;
             // and of the prefix'
             int f0 = 0, f1 = -1;
-            const int64_t y = r * p.group + gi, f_unit = y / p.tile_rows * p.kv_heads + g;
-            if (p.front_tiles && index >= 0) {
-                f0 = cta_of(total, p.ctas, f_unit * p.front_tiles);
-                f1 = cta_of(total, p.ctas, (f_unit + 1) * p.front_tiles - 1);
+            const int64_t y = r * p.group + gi, f_unit = y / lf.tile_rows * p.kv_heads + g;
+            if (lf.front_tiles && index >= 0) {
+                const int64_t all = lf.seqs ? lf.plan[lf.seqs].tiles : lf.front_units * lf.front_tiles;
+                f0 = cta_of(all, lf.ctas, f_unit * lf.front_tiles);
+                f1 = cta_of(all, lf.ctas, (f_unit + 1) * lf.front_tiles - 1);
             }
-            out = p.front_tiles || c0 != c1;   // (else it was finished where it was computed)
+            out = !p.whole || c0 != c1;   // (else it was finished where it was computed)
             if (out) {
-                const int n = (f1 - f0 + 1) + (c1 - c0 + 1);
+                const int n_front = f1 - f0 + 1, n = n_front + (c1 - c0 + 1);
                 for (int k = mine; k < n; k += WARPS) {
-                    const bool front = k <= f1 - f0;
-                    const int64_t slot = front ? f_unit + f0 + k : unit + c0 + (k - (f1 - f0 + 1));
-                    if (slot >= p.slots) continue;
-                    const int64_t row = slot * p.tile_rows + (front ? y % p.tile_rows : x % p.tile_rows);
-                    const float2 part = p.part_ml[row];
+                    const Line& l2 = k < n_front ? lf : lo;
+                    const int64_t slot = k < n_front ? f_unit + f0 + k : unit + c0 + (k - n_front);
+                    const int row = (int)(k < n_front ? y % lf.tile_rows : x % lo.tile_rows);
+                    if (slot >= l2.slots) continue;
+                    const float2 part = l2.ml[slot * l2.tile_rows + row];
                     if (part.y < 0.0f) continue;
-                    const float4* from = reinterpret_cast<const float4*>(p.part_o + row * p.head_size);
                     float4 v[2];
 #pragma unroll
                     for (int c = 0; c < 2; c++)
-                        if (lane + 32 * c < quads) v[c] = from[lane + 32 * c];
+                        if (lane + 32 * c < quads) v[c] = *reinterpret_cast<const float4*>(part_at(l2, p.head_size, slot, row, 4 * (lane + 32 * c)));
                     const float now = fmaxf(m, part.x), base = now == -INFINITY ? 0.0f : now, f = ex2(m - base), w = ex2(part.x - base);
                     m = now;
                     l = l * f + part.y * w;
