@@ -232,7 +232,7 @@ static std::string bad_attention(const lmrs_b200_pages_t* pages, const lmrs_b200
     const int64_t vec = 16 / (int64_t)size_of(pages->dtype);
     if (pages->head_size % 8) return "head_size must be a multiple of 8";
     if (q_heads < 1 || q_heads > MAX_HEADS || q_heads % pages->kv_heads) return "q_heads must be a positive multiple of kv_heads, at most 65535";
-    if (n_rows * (q_heads / pages->kv_heads) > 0x7fffffff) return "n_rows * q_heads / kv_heads is beyond 2^31 - 1";
+    if (n_rows * q_heads > 0x7fffffff) return "n_rows * q_heads is beyond 2^31 - 1";
     if (!aligned(pages->k, 16) || !aligned(pages->v, 16) || pages->k_page % vec || pages->k_slot % vec || pages->k_head % vec || pages->v_page % vec || pages->v_slot % vec ||
         pages->v_head % vec)
         return "the pages' rows must lie on 16-byte boundaries";
@@ -363,6 +363,9 @@ extern "C" int lmrs_b200_paged_attention(const lmrs_b200_pages_t* pages, const l
             p.q_wide = vectors(q, dtype);
             p.out_wide = aligned(out->data, 4 * sizeof(T)) && out->row % 4 == 0 && out->head % 4 == 0;
             p.whole = batch->prefix_len == 0;
+            p.page_shift = -1;
+            for (int i = 0; i < 31; i++)
+                if (pages->page_size == 1 << i) p.page_shift = i;
             static std::atomic<uint64_t> allowed{0}, allowed_tensor{0};
             cudaError_t e = cudaSuccess;
             if constexpr (sizeof(T) == 2)
@@ -381,10 +384,11 @@ extern "C" int lmrs_b200_paged_attention(const lmrs_b200_pages_t* pages, const l
                 if (e != cudaSuccess) return refuse(me, std::string("launch failed: ") + cudaGetErrorString(e));
                 if (launched(me)) return 1;
             }
-            // a warp a row and head, or 8 while that leaves warps on the GPU idle
+            // a warp a row and head, or 8 where that leaves most of the GPU's warps idle: there the parts may be many
             const int64_t items = n_rows * q_heads;
-            e = items <= SMS * 16 ? launch_after(join_kernel<T, 8>, (unsigned)items, 256, 0, (cudaStream_t)stream, p, c.front, c.own)
-                                  : launch_after(join_kernel<T, 1>, (unsigned)std::min<int64_t>((items + 7) / 8, SMS * 16), 256, 0, (cudaStream_t)stream, p, c.front, c.own);
+            constexpr int COLS = decltype(d)::value <= 128 ? 1 : 2;
+            e = items <= SMS * 4 ? launch_after(join_kernel<T, 8, COLS>, (unsigned)items, 256, 0, (cudaStream_t)stream, p, c.front, c.own)
+                                 : launch_after(join_kernel<T, 1, COLS>, (unsigned)std::min<int64_t>((items + 7) / 8, SMS * 16), 256, 0, (cudaStream_t)stream, p, c.front, c.own);
             return e == cudaSuccess ? 0 : refuse(me, std::string("launch failed: ") + cudaGetErrorString(e));
         });
     });

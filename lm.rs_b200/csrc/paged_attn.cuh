@@ -19,9 +19,9 @@ namespace paged {
 
 PG_DEVINL uint32_t smem_at(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
 PG_DEVINL float ex2(float v) { float r; asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v)); return r; }
-// 16 bytes to shared memory, zeros where there is nothing to copy
+// 16 bytes to shared memory, zeros where there is nothing to copy.  (No memory clobber: commits and waits have it, and what computes the next address may move ahead)
 PG_DEVINL void copy16(uint32_t to, const void* from, bool there) {
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(there ? 16 : 0) : "memory");
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(there ? 16 : 0));
 }
 PG_DEVINL void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N> PG_DEVINL void copy_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
@@ -44,6 +44,7 @@ template <typename T> struct AttnParams {
     float scale2, softcap, cap_in;             // scores: scale2 = scale * log2 e; or softcap * log2 e * tanh(dot * cap_in), cap_in = scale / softcap
     float* lse;
     bool q_wide, out_wide;                     // rows on 16-byte boundaries
+    int page_shift;                            // log2 of page_size, -1 if it is no power of two
     bool whole;                                // no prefix: a unit that one CTA takes is finished there
 };
 // What one kernel goes through: units of the prefix (if it takes them), then those of the sequences (if it takes them)
@@ -64,7 +65,10 @@ PG_DEVINL int64_t cta_begin(int64_t total, int ctas, int i) {
     const int64_t n = min((int64_t)ctas, total);
     return i < n ? total * i / n : total;
 }
-PG_DEVINL int cta_of(int64_t total, int ctas, int64_t tile) { return (int)((min((int64_t)ctas, total) * (tile + 1) + total - 1) / total) - 1; }
+PG_DEVINL int cta_of(int64_t total, int ctas, int64_t tile) {
+    const int64_t over = min((int64_t)ctas, total) * (tile + 1) + total - 1;
+    return (over >> 32 ? (int)(over / total) : (int)((uint32_t)over / (uint32_t)total)) - 1;   // (a 64-bit division takes a hundred instructions)
+}
 
 // rows of a sequence's unit and the keys it goes through
 // (a call's rows times the group stay below 2^31)
@@ -211,14 +215,49 @@ struct Place { int page, place; };
 template <typename T> PG_DEVINL Place unit_place(const AttnParams<T>& p, const Walk& w, int x) {
     Place r = {-1, 0};
     if (x < w.keys) {   // (so the table reaches it)
-        const int i = x / p.batch.page_size, page = (w.b < 0 ? p.batch.prefix : p.batch.tables + w.b * p.batch.table_stride)[i];
+        const int i = p.page_shift >= 0 ? x >> p.page_shift : x / p.batch.page_size, page = (w.b < 0 ? p.batch.prefix : p.batch.tables + w.b * p.batch.table_stride)[i];
         r.page = page < 0 || page >= p.batch.pages ? -1 : page;
         r.place = x - i * p.batch.page_size;
     }
     return r;
 }
-template <typename T> PG_DEVINL float score2(const AttnParams<T>& p, float dot) {   // in powers of two
-    return p.softcap > 0.0f ? p.softcap * LOG2E * tanhf(dot * p.cap_in) : dot * p.scale2;
+// A dot product as a score, in powers of two.  With a cap c: c tanh(x), x = dot scale / c.  What a weight is off by goes with the score's absolute error: from |x| = 1/2 on
+// 1 - 2 / (e^2x + 1) (two units of the last place of 1), below it the Taylor series up to x^13 (its next term is 4.4e-8 at 1/2), which leaves the special-function units alone.
+PG_DEVINL float tanh_far(float x) {
+    float r;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(ex2(x * (2.0f * LOG2E)) + 1.0f));   // (of infinity: 0)
+    return fmaf(-2.0f, r, 1.0f);
+}
+PG_DEVINL float tanh_near(float x) {
+    const float y = x * x;
+    float s = fmaf(y, 21844.0f / 6081075.0f, -1382.0f / 155925.0f);
+    s = fmaf(y, s, 62.0f / 2835.0f);
+    s = fmaf(y, s, -17.0f / 315.0f);
+    s = fmaf(y, s, 2.0f / 15.0f);
+    s = fmaf(y, s, -1.0f / 3.0f);
+    return fmaf(y * s, x, x);
+}
+template <typename T> PG_DEVINL float score2(const AttnParams<T>& p, float dot) {
+    if (!(p.softcap > 0.0f)) return dot * p.scale2;
+    const float x = dot * p.cap_in;
+    return p.softcap * LOG2E * (fabsf(x) <= 0.5f ? tanh_near(x) : tanh_far(x));
+}
+// N dots of a lane, capped (all lanes of the warp: the near form where it serves all of them)
+template <typename T, int N> PG_DEVINL void cap_scores(const AttnParams<T>& p, float (&s)[N]) {
+    const float cap2 = p.softcap * LOG2E;
+    float far = 0.0f;
+#pragma unroll
+    for (int i = 0; i < N; i++) {
+        s[i] *= p.cap_in;
+        far = fmaxf(far, fabsf(s[i]));
+    }
+    if (__all_sync(~0u, far <= 0.5f)) {   // (NaN comes out as NaN either way)
+#pragma unroll
+        for (int i = 0; i < N; i++) s[i] = cap2 * tanh_near(s[i]);
+    } else {
+#pragma unroll
+        for (int i = 0; i < N; i++) s[i] = cap2 * (fabsf(s[i]) <= 0.5f ? tanh_near(s[i]) : tanh_far(s[i]));
+    }
 }
 
 template <typename T> PG_DEVINL void store_row(const AttnParams<T>& p, const UnitRow& r, int e, float4 v) {   // 4 elements of a result
@@ -237,7 +276,7 @@ template <typename T> PG_DEVINL void store_row(const AttnParams<T>& p, const Uni
 // Rows that come out finite never come here.
 constexpr int AGAIN = 128;
 struct AgainScratch { float weight[AGAIN], most[AGAIN / 32]; int64_t at[AGAIN]; };
-PG_DEVINL void again_sync(int barrier) { asm volatile("bar.sync %0, %1;" ::"r"(barrier), "n"(AGAIN) : "memory"); }
+PG_DEVINL void again_sync(int barrier) { __syncwarp(); asm volatile("bar.sync %0, %1;" ::"r"(barrier), "n"(AGAIN) : "memory"); }
 template <typename T>
 static __device__ __noinline__ void row_again(const AttnParams<T>& p, const Walk& w, const UnitRow& r, int from, int to, AgainScratch& sc, int barrier, float& m, float& l, float (&acc)[2]) {
     const int t = threadIdx.x & (AGAIN - 1), D = p.head_size;
@@ -332,6 +371,7 @@ template <typename T, int DP> struct WarpTile {
     bool seen[2];
     PG_DEVINL void begin(uint32_t q_at) {
         const int lane = threadIdx.x & 31;
+        __syncwarp();
 #pragma unroll
         for (int k = 0; k < DP / 16; k++) ldmatrix4(q[k], q_at + piece_at(lane & 15, 2 * k + (lane >> 4), S::ROW));
 #pragma unroll
@@ -344,6 +384,7 @@ template <typename T, int DP> struct WarpTile {
     PG_DEVINL void tile(const AttnParams<T>& p, uint32_t, uint32_t k_at, uint32_t v_at, uint32_t there, int first, const int* row_keys, int, float*) {
         const int lane = threadIdx.x & 31, key0 = 16 * (threadIdx.x >> 5);
         float s[2][4] = {};
+        __syncwarp();   // (ldmatrix and mma are for a warp in step)
         const uint32_t k_row = k_at + (uint32_t)(key0 + (lane & 7) + ((lane >> 4) << 3)) * S::ROW, k_turn = (uint32_t)(((lane >> 3) & 1) ^ (lane & 7)) << 4;
 #pragma unroll
         for (int k = 0; k < DP / 16; k++) {
@@ -353,8 +394,12 @@ template <typename T, int DP> struct WarpTile {
             mma16816(s[1], q[k], b[2], b[3], T());
         }
         if (p.softcap > 0.0f) {
+            float flat[8];
 #pragma unroll
-            for (int i = 0; i < 8; i++) s[i >> 2][i & 3] = score2(p, s[i >> 2][i & 3]);
+            for (int i = 0; i < 8; i++) flat[i] = s[i >> 2][i & 3];
+            cap_scores(p, flat);
+#pragma unroll
+            for (int i = 0; i < 8; i++) s[i >> 2][i & 3] = flat[i];
         } else {
 #pragma unroll
             for (int i = 0; i < 8; i++) s[i >> 2][i & 3] *= p.scale2;
@@ -741,24 +786,24 @@ __global__ void __launch_bounds__(TileShape<T, DP>::THREADS, TileShape<T, DP>::C
 }
 
 // ---- joining parts ---------------------------------------------------------------------------------------------------------------------------
-// WARPS warps a row and head, their lanes its columns in fours: each takes every WARPS-th part with a running (m, l, o), and they meet in shared memory.  8 where
+// WARPS warps a row and head, their lanes its columns in fours: they take parts in turn, each with a running (m, l, o), and they meet in shared memory.  8 where
 // rows are few and may have many parts, 1 otherwise (then a CTA has 8 rows or heads).
-template <typename T, int WARPS>
-__global__ void __launch_bounds__(256) join_kernel(const __grid_constant__ AttnParams<T> p, const __grid_constant__ Line lf, const __grid_constant__ Line lo) {
-    constexpr int ITEMS = 8 / WARPS;
+template <typename T, int WARPS, int COLS>   // COLS: 128 columns each
+__global__ void __launch_bounds__(256, COLS == 1 ? 4 : 3) join_kernel(const __grid_constant__ AttnParams<T> p, const __grid_constant__ Line lf, const __grid_constant__ Line lo) {
+    constexpr int ITEMS = 8 / WARPS, EACH = WARPS == 1 ? 32 : 4;   // parts a warp takes at a time
     __shared__ float2 ml[8];
     __shared__ float4 sums[8][64];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, quads = p.head_size / 4, mine = warp % WARPS;
     grid_wait();
-    const int64_t items = p.batch.n_rows * p.q_heads;
+    const int items = (int)p.batch.n_rows * p.q_heads;   // (below 2^31)
     for (int64_t i0 = (int64_t)blockIdx.x * ITEMS; i0 < items; i0 += (int64_t)gridDim.x * ITEMS) {
-        const int64_t item = i0 + warp / WARPS;
+        const int item = (int)min(i0 + warp / WARPS, (int64_t)items);
         bool out = item < items;
-        const int64_t r = out ? item / p.q_heads : 0;
-        const int head = (int)(item - r * p.q_heads), b = seq_of_row_warp(p.batch, r);
+        const int r = out ? item / p.q_heads : 0;
+        const int head = item - r * p.q_heads, b = seq_of_row_warp(p.batch, r);
         out = out && b >= 0;
         float m = -INFINITY, l = 0.0f;
-        float4 o[2] = {};
+        float4 o[COLS] = {};
         bool any = false;
         const int g = head / p.group, gi = head - g * p.group;
         if (out) {
@@ -774,7 +819,8 @@ __global__ void __launch_bounds__(256) join_kernel(const __grid_constant__ AttnP
             const int c0 = tiles ? cta_of(total, lo.ctas, tile0) : 0, c1 = tiles ? cta_of(total, lo.ctas, tile0 + tiles - 1) : -1;
             // and of the prefix'
             int f0 = 0, f1 = -1;
-            const int64_t y = r * p.group + gi, f_unit = y / lf.tile_rows * p.kv_heads + g;
+            const int y = r * p.group + gi;
+            const int64_t f_unit = (int64_t)(y / lf.tile_rows) * p.kv_heads + g;
             if (lf.front_tiles && index >= 0) {
                 const int64_t all = lf.seqs ? lf.plan[lf.seqs].tiles : lf.front_units * lf.front_tiles;
                 f0 = cta_of(all, lf.ctas, f_unit * lf.front_tiles);
@@ -782,28 +828,53 @@ __global__ void __launch_bounds__(256) join_kernel(const __grid_constant__ AttnP
             }
             out = !p.whole || c0 != c1;   // (else it was finished where it was computed)
             if (out) {
-                const int n_front = f1 - f0 + 1, n = n_front + (c1 - c0 + 1);
-                for (int k = mine; k < n; k += WARPS) {
-                    const Line& l2 = k < n_front ? lf : lo;
-                    const int64_t slot = k < n_front ? f_unit + f0 + k : unit + c0 + (k - n_front);
-                    const int row = (int)(k < n_front ? y % lf.tile_rows : x % lo.tile_rows);
-                    if (slot >= l2.slots) continue;
-                    const float2 part = l2.ml[slot * l2.tile_rows + row];
-                    if (part.y < 0.0f) continue;
-                    float4 v[2];
-#pragma unroll
-                    for (int c = 0; c < 2; c++)
-                        if (lane + 32 * c < quads) v[c] = *reinterpret_cast<const float4*>(part_at(l2, p.head_size, slot, row, 4 * (lane + 32 * c)));
-                    const float now = fmaxf(m, part.x), base = now == -INFINITY ? 0.0f : now, f = ex2(m - base), w = ex2(part.x - base);
+                // EACH parts at a time: a lane reads the (m, l) of one, then all lanes sum the columns, four parts' loads ahead of their use
+                const int n_front = f1 - f0 + 1, n = n_front + (c1 - c0 + 1), y_row = y % lf.tile_rows, x_row = x % lo.tile_rows;
+                for (int k0 = EACH * mine; k0 < n; k0 += EACH * WARPS) {
+                    const int k = lane < EACH ? k0 + lane : n;
+                    const bool front = k < n_front;
+                    const int64_t slot = front ? f_unit + f0 + k : unit + c0 + (k - n_front);
+                    float2 part = make_float2(-INFINITY, -1.0f);
+                    if (k < n && slot >= 0 && slot < (front ? lf.slots : lo.slots)) part = front ? lf.ml[slot * lf.tile_rows + y_row] : lo.ml[slot * lo.tile_rows + x_row];
+                    const float* from = front ? part_at(lf, p.head_size, slot, y_row, 0) : part_at(lo, p.head_size, slot, x_row, 0);
+                    const bool has = !(part.y < 0.0f);
+                    unsigned left = __ballot_sync(~0u, has);
+                    if (!left) continue;
+                    float now = has ? part.x : -INFINITY;
+                    for (int d = 16; d; d >>= 1) now = fmaxf(now, __shfl_xor_sync(~0u, now, d));
+                    now = fmaxf(m, now);
+                    const float base = now == -INFINITY ? 0.0f : now, f = ex2(m - base), w = has ? ex2(part.x - base) : 0.0f;
+                    float sum = has ? part.y * w : 0.0f;
+                    for (int d = 16; d; d >>= 1) sum += __shfl_xor_sync(~0u, sum, d);
                     m = now;
-                    l = l * f + part.y * w;
+                    l = l * f + sum;
                     any = true;
 #pragma unroll
-                    for (int c = 0; c < 2; c++)
-                        if (lane + 32 * c < quads) {
-                            o[c].x = fmaf(o[c].x, f, v[c].x * w); o[c].y = fmaf(o[c].y, f, v[c].y * w);
-                            o[c].z = fmaf(o[c].z, f, v[c].z * w); o[c].w = fmaf(o[c].w, f, v[c].w * w);
+                    for (int c = 0; c < COLS; c++) { o[c].x *= f; o[c].y *= f; o[c].z *= f; o[c].w *= f; }
+                    while (left) {
+                        float4 v[4][COLS];
+                        float wk[4];
+#pragma unroll
+                        for (int u = 0; u < 4; u++) {
+                            const int i = left ? __ffs(left) - 1 : 0;
+                            wk[u] = left ? __shfl_sync(~0u, w, i) : 0.0f;
+                            const bool in_front = k0 + i < n_front;
+                            const float* at = reinterpret_cast<const float*>(__shfl_sync(~0u, reinterpret_cast<unsigned long long>(from), i));
+                            const int64_t step = (int64_t)(in_front ? lf.tile_rows : lo.tile_rows) * 8;   // from 8 columns to the next
+#pragma unroll
+                            for (int c = 0; c < COLS; c++)
+                                if (lane + 32 * c < quads) v[u][c] = left ? *reinterpret_cast<const float4*>(at + (lane + 32 * c >> 1) * step + 4 * (lane & 1)) : make_float4(0, 0, 0, 0);
+                            left &= left - 1;
                         }
+#pragma unroll
+                        for (int u = 0; u < 4; u++)
+#pragma unroll
+                            for (int c = 0; c < COLS; c++)
+                                if (lane + 32 * c < quads) {
+                                    o[c].x = fmaf(v[u][c].x, wk[u], o[c].x); o[c].y = fmaf(v[u][c].y, wk[u], o[c].y);
+                                    o[c].z = fmaf(v[u][c].z, wk[u], o[c].z); o[c].w = fmaf(v[u][c].w, wk[u], o[c].w);
+                                }
+                    }
                 }
             }
         }
@@ -811,7 +882,7 @@ __global__ void __launch_bounds__(256) join_kernel(const __grid_constant__ AttnP
             __syncthreads();
             if (lane == 0) ml[warp] = make_float2(m, any ? l : -1.0f);
 #pragma unroll
-            for (int c = 0; c < 2; c++)
+            for (int c = 0; c < COLS; c++)
                 if (lane + 32 * c < quads) sums[warp][lane + 32 * c] = o[c];
             __syncthreads();
             if (warp) continue;
@@ -823,7 +894,7 @@ __global__ void __launch_bounds__(256) join_kernel(const __grid_constant__ AttnP
                 l = l * f + part.y * w;
                 any = true;
 #pragma unroll
-                for (int c = 0; c < 2; c++)
+                for (int c = 0; c < COLS; c++)
                     if (lane + 32 * c < quads) {
                         const float4 v = sums[i][lane + 32 * c];
                         o[c].x = fmaf(o[c].x, f, v.x * w); o[c].y = fmaf(o[c].y, f, v.y * w);
@@ -832,12 +903,12 @@ __global__ void __launch_bounds__(256) join_kernel(const __grid_constant__ AttnP
             }
         }
         if (!out) continue;
-        const UnitRow row = {r, head, 0};
+        const UnitRow row = {(int64_t)r, head, 0};
 #pragma unroll
-        for (int c = 0; c < 2; c++)
+        for (int c = 0; c < COLS; c++)
             if (lane + 32 * c < quads)
                 store_row(p, row, 4 * (lane + 32 * c), any ? make_float4(o[c].x / l, o[c].y / l, o[c].z / l, o[c].w / l) : make_float4(0.0f, 0.0f, 0.0f, 0.0f));
-        if (lane == 0 && p.lse) p.lse[r * p.q_heads + head] = any ? lse_of(m, l) : -INFINITY;
+        if (lane == 0 && p.lse) p.lse[item] = any ? lse_of(m, l) : -INFINITY;
     }
 }
 

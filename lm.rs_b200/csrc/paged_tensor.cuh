@@ -32,22 +32,55 @@ template <typename T, int DP> struct TensorShape {
 constexpr float RESCALE_AT = 8.0f;
 constexpr int PAGED_WAIT = 5 << 8;   // (what a wait was for is not reported: any number that is not 0)
 
-PG_DEVINL bool wait_for(uint64_t* bar, int count, volatile int* gave_up) {   // until phase number `count` of the barrier has ended
-    return dense::mbar_wait_bounded(bar, (uint32_t)count & 1, gave_up, PAGED_WAIT);
+// A warp waits until phase number `count` of the barrier has ended (false: gave up).  One lane looks (9 warps of 32 looking lanes each filled the queue that copies to shared memory
+// go through, and every one of those took ten times as long), under a predicate and not in a branch of its own: what follows a wait - accesses to TMEM, products,
+// operands in uniform registers - is for a warp in step, and lanes that part here need not have met again by then.
+PG_DEVINL bool wait_warp(uint64_t* bar, int count, volatile int* gave_up) {
+    const uint32_t looks = (threadIdx.x & 31) == 0, at = smem_at(bar), parity = (uint32_t)count & 1;
+    uint32_t from = 0;
+    for (uint32_t i = 0;; i++) {
+        uint32_t state;   // 1: ended, 2: give up
+        asm volatile(
+            "{\n\t.reg .pred p, l;\n\t"
+            "setp.ne.b32 l, %3, 0;\n\t"
+            "mov.u32 %0, 0;\n\t"
+            "@l mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+            "@l selp.u32 %0, 1, 0, p;\n\t}"
+            : "=&r"(state)
+            : "r"(at), "r"(parity), "r"(looks)
+            : "memory");
+        const uint32_t now = dense::now_ns();
+        if (i < dense::TG_LEAST_TRIES) from = now;
+        if (state == 0 && (*gave_up || now - from > dense::TG_WAIT_NS)) state = 2;
+        state = __shfl_sync(~0u, state, 0);
+        if (state == 2) *gave_up = PAGED_WAIT;
+        if (state) {
+            __syncwarp();
+            return state == 1;
+        }
+    }
 }
-PG_DEVINL bool wait_warp(uint64_t* bar, int count, volatile int* gave_up) { return __all_sync(~0u, wait_for(bar, count, gave_up)); }
 PG_DEVINL void arrive(uint64_t* bar) { asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_at(bar)) : "memory"); }
 PG_DEVINL void tmem_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 PG_DEVINL void tmem_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
-PG_DEVINL void tmem_loaded(uint32_t (&v)[32]) {   // waits for the loads; the values pass through, so that nothing computed from them moves ahead
-    asm volatile("tcgen05.wait::ld.sync.aligned;"
-                 : "+r"(v[0]), "+r"(v[1]), "+r"(v[2]), "+r"(v[3]), "+r"(v[4]), "+r"(v[5]), "+r"(v[6]), "+r"(v[7]), "+r"(v[8]), "+r"(v[9]), "+r"(v[10]), "+r"(v[11]), "+r"(v[12]),
-                   "+r"(v[13]), "+r"(v[14]), "+r"(v[15]), "+r"(v[16]), "+r"(v[17]), "+r"(v[18]), "+r"(v[19]), "+r"(v[20]), "+r"(v[21]), "+r"(v[22]), "+r"(v[23]), "+r"(v[24]),
-                   "+r"(v[25]), "+r"(v[26]), "+r"(v[27]), "+r"(v[28]), "+r"(v[29]), "+r"(v[30]), "+r"(v[31])
-                 :
-                 : "memory");
+// Loads and stores of TMEM are for a whole warp in step: where lanes may have gone different ways before (rows that are not there store nothing), they meet first.
+// Loads are waited for in the same statement, so that no copy or spill of a register can come between.
+PG_DEVINL void tmem_load32(uint32_t at, uint32_t (&v)[32]) {
+    __syncwarp();
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {"
+        "%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+        "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];\n\t"
+        "tcgen05.wait::ld.sync.aligned;"
+        : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]), "=r"(v[9]),
+          "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15]), "=r"(v[16]), "=r"(v[17]), "=r"(v[18]), "=r"(v[19]),
+          "=r"(v[20]), "=r"(v[21]), "=r"(v[22]), "=r"(v[23]), "=r"(v[24]), "=r"(v[25]), "=r"(v[26]), "=r"(v[27]), "=r"(v[28]), "=r"(v[29]),
+          "=r"(v[30]), "=r"(v[31])
+        : "r"(at)
+        : "memory");
 }
 PG_DEVINL void tmem_store32(uint32_t at, const uint32_t (&v)[32]) {
+    __syncwarp();
     asm volatile(
         "tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], "
         "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
@@ -57,11 +90,12 @@ PG_DEVINL void tmem_store32(uint32_t at, const uint32_t (&v)[32]) {
         : "memory");
 }
 PG_DEVINL void tmem_store16(uint32_t at, const uint32_t (&v)[16]) {
+    __syncwarp();
     asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15};" ::"r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]),
                  "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]), "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15]), "r"(at)
                  : "memory");
 }
-PG_DEVINL void tmem_stored() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+PG_DEVINL void tmem_stored() { __syncwarp(); asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
 // shared memory besides the operands
 template <typename T, int DP> struct TensorShared {
@@ -70,10 +104,11 @@ template <typename T, int DP> struct TensorShared {
     uint64_t known[S::RING];                    // which of a tile's keys are there is written
     uint64_t scores[2], weights[2];             // sets of scores: written by the products, replaced by weights
     uint64_t summed[2], read[2];                // o of a block: the last product has ended; the part's o has been read
+    uint64_t queries;                           // the part's queries are there
     uint64_t queries_read;                      // the last product that reads the part's queries has ended
     uint64_t parted;                            // both groups have ended the part (neither runs ahead: phases are told apart by their parity alone)
     uint32_t there[S::RING][S::KEYS / 32];
-    int64_t k_from[2][S::KEYS], v_from[S::RING][S::KEYS];   // where the keys' rows begin (elements; -1: nowhere)
+    int64_t starts[4][S::KEYS];                 // a copying warp's: where the keys' rows begin (elements; -1: nowhere)
     uint32_t tmem;
     int gave_up;
     AgainScratch again[2];
@@ -90,9 +125,10 @@ __global__ void __launch_bounds__(512, 1) rows128_kernel(const __grid_constant__
     volatile int* gave_up = &sh.gave_up;
 
     if (threadIdx.x == 0) {
-        for (int i = 0; i < S::SLOTS; i++) { mbar_init(&sh.full[i], 128); mbar_init(&sh.empty[i], 1); }
-        for (int i = 0; i < S::RING; i++) mbar_init(&sh.known[i], 128);
+        for (int i = 0; i < S::SLOTS; i++) { mbar_init(&sh.full[i], 1); mbar_init(&sh.empty[i], 1); }
+        for (int i = 0; i < S::RING; i++) mbar_init(&sh.known[i], 1);
         for (int i = 0; i < 2; i++) { mbar_init(&sh.scores[i], 1); mbar_init(&sh.weights[i], 128); mbar_init(&sh.summed[i], 1); mbar_init(&sh.read[i], 128); }
+        mbar_init(&sh.queries, 128);
         mbar_init(&sh.queries_read, 1);
         mbar_init(&sh.parted, 256);
         sh.gave_up = 0;
@@ -103,6 +139,7 @@ __global__ void __launch_bounds__(512, 1) rows128_kernel(const __grid_constant__
     walk_begin<T, S::THREADS>(p, l, w, from, to);   // (synchronises the CTA)
     if (from >= to) { grid_launch(); return; }
     if (warp == 12) {
+        __syncwarp();
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_at(&sh.tmem)), "n"(512) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
@@ -125,84 +162,107 @@ __global__ void __launch_bounds__(512, 1) rows128_kernel(const __grid_constant__
         if (w.tiles == 0) { left = 0; return false; }   // (the line ended early: lengths changed under the kernel)
         return true;
     };
-    // registers: 512 x 128 at launch = 256 x 192 for the rows + 256 x 64
+    // (Every thread keeps its 128 registers.  Moved from the copying warps to the rows by setmaxnreg they were not safe: the compiler gave code of the copying warps
+    // more than was left to them)
     if (warp >= 8) {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
         if (warp < 12) {
-            // ---- copies ----
-            const int t = threadIdx.x - 256, pieces = (D + 15) / 16 * 2, whole = D / 8;
-            uint32_t n = 0, done = 0;   // operand tiles asked for, reported
-            int looked = 0;             // tiles looked up
+            // ---- copies: operand tile n is warp n % 4's, which waits for its slot, copies, and reports it when it has landed; the other warps are at theirs ----
+            const int mine = warp - 8, t = threadIdx.x - 256, pieces = (D + 15) / 16 * 2, whole = D / 8;
+            int64_t* starts = sh.starts[mine];
+            uint32_t n = 0;       // operand tiles of the CTA so far
+            int looked = 0, part = 0;
             bool ok = true;
-            auto report = [&](uint32_t upto) {   // (their copies have landed)
+            bool asked = false;   // queries are on their way
+            auto landed = [&]() {
+                copy_wait<0>();
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-                for (; done < upto; done++) arrive(&sh.full[done % S::SLOTS]);
+                if (asked) arrive(&sh.queries);
+                asked = false;
             };
-            auto copy_operand = [&](const T* base, const int64_t* starts) {
-                const uint32_t slot = n % S::SLOTS;
-                ok = ok && wait_warp(&sh.empty[slot], (int)(n / S::SLOTS) + 1, gave_up);
+            auto operand = [&](const T* base, bool values, int j) {   // tile j of the part; looked: its number in the CTA
+                const uint32_t slot = n % S::SLOTS, round = n / S::SLOTS;
+                if ((n++ & 3) != (uint32_t)mine || !ok) return;
+                // the places of its keys, four a lane
+                const int set = looked % S::RING;
+                __syncwarp();
+#pragma unroll
+                for (int i = 0; i < S::KEYS / 32; i++) {
+                    const Place at = unit_place(p, w, (w.tile + j) * S::KEYS + 32 * i + lane);
+                    starts[32 * i + lane] = at.page < 0 ? -1
+                                            : values    ? at.page * p.v_page + at.place * p.v_slot + w.head * p.v_head
+                                                        : at.page * p.k_page + at.place * p.k_slot + w.head * p.k_head;
+                    if (!values) {
+                        const unsigned bits = __ballot_sync(~0u, at.page >= 0);
+                        if (lane == 0) sh.there[set][i] = bits;
+                    }
+                }
+                __syncwarp();
+                if (!values && lane == 0) arrive(&sh.known[set]);
+                ok = wait_warp(&sh.empty[slot], (int)round + 1, gave_up);
                 if (!ok) return;
                 const uint32_t at = smem_at(ring) + slot * S::SLOT;
-                const int c = t & 7;
-#pragma unroll 4
-                for (int r = t >> 3; r < S::KEYS; r += 16) {
-                    const int64_t start = starts[r];
-                    const T* row = base + (start < 0 ? 0 : start);
-                    const uint32_t to_row = at + r * 128 + ((c ^ (r & 7)) << 4);
+                const int c = lane & 7;
+#pragma unroll 1
+                for (int r0 = lane >> 3; r0 < S::KEYS; r0 += 16) {   // (four rows' places are read before their copies are asked for)
+                    const T* row[4];
 #pragma unroll
-                    for (int b = 0; b < S::BOXES; b++)
-                        if (8 * b + c < pieces) {
-                            const bool in = start >= 0 && 8 * b + c < whole;
-                            copy16(to_row + b * S::KEYS * 128, in ? row + (8 * b + c) * 8 : base, in);
-                        }
+                    for (int i = 0; i < 4; i++) {
+                        const int64_t start = starts[r0 + 4 * i];
+                        row[i] = start < 0 ? nullptr : base + start + 8 * c;
+                    }
+#pragma unroll
+                    for (int i = 0; i < 4; i++) {
+                        const int r = r0 + 4 * i;
+                        const uint32_t to_row = at + r * 128 + ((c ^ (r & 7)) << 4);
+#pragma unroll
+                        for (int b = 0; b < S::BOXES; b++)
+                            if (8 * b + c < pieces) {
+                                const bool in = row[i] && 8 * b + c < whole;
+                                copy16(to_row + b * S::KEYS * 128, in ? row[i] + 64 * b : base, in);
+                            }
+                    }
                 }
                 copy_commit();
-                n++;
-                copy_wait<S::SLOTS - 2>();
-                if (n > S::SLOTS - 2) report(n - (S::SLOTS - 2));
+                landed();
+                __syncwarp();
+                if (lane == 0) arrive(&sh.full[slot]);
             };
-            int part = 0;
-            do {   // (the four warps meet at barrier 3 for every tile, whether or not one has given up)
+            do {
                 enter();
                 if (part > 0) ok = ok && wait_warp(&sh.queries_read, part - 1, gave_up);
-                for (int e = t; ok && e < blocks * S::BLOCK * pieces; e += 128) {   // the queries go with the first keys
-                    const int x = e / pieces, c = e - x * pieces;
-                    const UnitRow r = unit_row(p, l, w, x);
-                    const bool in = r.row >= 0 && x < used && c < whole;
-                    const T* q = in ? p.q.data + r.row * p.q.row + r.head * p.q.head + 8 * c : p.q.data;
-                    uint8_t* to_q = queries + (x >> 7) * S::Q_BLOCK + (c >> 3) * (S::BLOCK * 128) + (x & 127) * 128 + (((c & 7) ^ (x & 7)) << 4);
-                    if (p.q_wide) {
-                        copy16(smem_at(to_q), q, in);
-                    } else {
-                        Piece<T, 8> v;
+                if (ok) {   // the queries: eight threads a row; they are reported with the operand tile that follows
+                    const int c = t & 7;
+#pragma unroll 2
+                    for (int x = t >> 3; x < blocks * S::BLOCK; x += 16) {
+                        const UnitRow r = unit_row(p, l, w, x);
+                        const T* q = r.row >= 0 ? p.q.data + r.row * p.q.row + r.head * p.q.head + 8 * c : p.q.data;
+                        uint8_t* to_q = queries + (x >> 7) * S::Q_BLOCK + (x & 127) * 128 + ((c ^ (x & 7)) << 4);
 #pragma unroll
-                        for (int i = 0; i < 8; i++) v.v[i] = in ? q[i] : from_f<T>(0.0f);
-                        *reinterpret_cast<Piece<T, 8>*>(to_q) = v;
+                        for (int b = 0; b < S::BOXES; b++) {
+                            if (8 * b + c >= pieces) continue;
+                            const bool in = r.row >= 0 && 8 * b + c < whole;
+                            if (p.q_wide) {
+                                copy16(smem_at(to_q + b * (S::BLOCK * 128)), in ? q + 64 * b : p.q.data, in);
+                            } else {
+                                Piece<T, 8> v;
+#pragma unroll
+                                for (int i = 0; i < 8; i++) v.v[i] = in ? q[64 * b + i] : from_f<T>(0.0f);
+                                *reinterpret_cast<Piece<T, 8>*>(to_q + b * (S::BLOCK * 128)) = v;
+                            }
+                        }
                     }
+                    copy_commit();
+                    asked = true;
                 }
-                auto keys = [&](int j) {   // tile j of the part: where its keys lie, then the keys
-                    const int set = looked % S::RING;
-                    asm volatile("bar.sync 3, 128;" ::: "memory");   // (all have read the places that these replace)
-                    if (t < S::KEYS) {
-                        const Place at = unit_place(p, w, (w.tile + j) * S::KEYS + t);
-                        sh.k_from[looked & 1][t] = at.page < 0 ? -1 : at.page * p.k_page + at.place * p.k_slot + w.head * p.k_head;
-                        sh.v_from[set][t] = at.page < 0 ? -1 : at.page * p.v_page + at.place * p.v_slot + w.head * p.v_head;
-                        const unsigned bits = __ballot_sync(~0u, at.page >= 0);
-                        if (lane == 0) sh.there[set][t >> 5] = bits;
-                    }
-                    asm volatile("bar.sync 3, 128;" ::: "memory");
-                    if (ok) arrive(&sh.known[set]);
-                    copy_operand(p.k, sh.k_from[looked & 1]);
-                    looked++;
-                };
                 const int first = looked;
+                auto keys = [&](int j) { looked = first + j; operand(p.k, false, j); };
                 keys(0);
                 for (int j = 0; j < tiles; j++) {
                     if (j + 1 < tiles) keys(j + 1);
-                    copy_operand(p.v, sh.v_from[(first + j) % S::RING]);
+                    operand(p.v, true, j);
                 }
-                copy_wait<0>();   // (the next part waits for the queries' last reader, which needs all of this one)
-                report(n);
+                looked = first + tiles;
+                if (asked) landed();   // (a warp that no operand tile fell to)
                 part++;
             } while (leave());
         } else if (warp == 12) {
@@ -212,77 +272,90 @@ __global__ void __launch_bounds__(512, 1) rows128_kernel(const __grid_constant__
             const uint32_t score_form = form | ((uint32_t)(S::KEYS >> 3) << 17), sum_form = form | (1u << 16) | ((uint32_t)((D + 15) / 16 * 2) << 17);   // (values are MN-major)
             const uint32_t ring_lo = (uint32_t)dense::tg_desc_sw128(ring), q_lo = (uint32_t)dense::tg_desc_sw128(queries);
             const int steps = (D + 15) / 16;
-            uint32_t n = 0;                      // operand tiles taken
+            uint32_t n = 0, round = 0;           // slot of the next operand tile, rounds of the ring before it
             int w_count[2] = {0, 0}, part = 0;   // sets of weights taken
             bool ok = true;
-            do {
-                enter();
-                const int items = tiles * blocks;
-                uint32_t k_slot[2] = {0, 0}, v_slot = 0;   // of the tile whose keys, whose values are next
-                auto take = [&]() {
-                    ok = ok && wait_for(&sh.full[n % S::SLOTS], (int)(n / S::SLOTS), gave_up);
-                    tmem_after();
-                    return n++ % S::SLOTS;
-                };
-                auto scores = [&](int i) {
-                    const int block = blocks == 2 ? i & 1 : 0;
-                    if (blocks == 1 || block == 0) k_slot[0] = take();
-                    if (!ok) return;
-                    const uint32_t d = tmem + (uint32_t)(i & 1) * S::S_WIDTH, a = q_lo + (uint32_t)block * (S::Q_BLOCK >> 4), b = ring_lo + k_slot[0] * (S::SLOT >> 4);
-                    for (int k = 0; k < steps; k++)
+            auto take = [&]() {
+                ok = ok && wait_warp(&sh.full[n], (int)round, gave_up);
+                tmem_after();
+                const uint32_t slot = n;
+                if (++n == S::SLOTS) { n = 0; round++; }
+                return slot;
+            };
+            // (unrolled, so that descriptors are sums of constants in uniform registers: as a loop over k an issue took 96 cycles, three times the product)
+            auto scores = [&](int block, int set, uint32_t slot) {
+                const uint32_t d = tmem + (uint32_t)set * S::S_WIDTH, a = q_lo + (uint32_t)block * (S::Q_BLOCK >> 4), b = ring_lo + slot * (S::SLOT >> 4);
+#pragma unroll
+                for (int k = 0; k < DP / 16; k++)
+                    if (k < steps)
                         dense::tg_mma_ss1(one, d, a + (uint32_t)(k >> 2) * (S::BLOCK * 128 >> 4) + (k & 3) * 2, b + (uint32_t)(k >> 2) * (S::KEYS * 128 >> 4) + (k & 3) * 2, score_form, k > 0);
-                    if (blocks == 1 || block == 1) dense::tg_commit1(one, &sh.empty[k_slot[0]]);
-                    dense::tg_commit1(one, &sh.scores[i & 1]);
-                    if (i == items - 1) dense::tg_commit1(one, &sh.queries_read);
-                };
-                auto sums = [&](int i) {
-                    const int block = blocks == 2 ? i & 1 : 0, j = blocks == 2 ? i >> 1 : i;
-                    if (block == 0) v_slot = take();
-                    if (j == 0 && part > 0) ok = ok && wait_for(&sh.read[block], part - 1, gave_up);
-                    ok = ok && wait_for(&sh.weights[i & 1], w_count[i & 1]++, gave_up);
-                    if (!ok) return;
-                    tmem_after();
-                    const uint32_t d = tmem + S::O_AT + (uint32_t)block * DP, a = tmem + (uint32_t)(i & 1) * S::S_WIDTH;
-                    // 16 keys a step: two groups of 8 rows of 128 bytes; from 64 columns to the next: a box
-                    const uint32_t b = (ring_lo & 0xffffu) + v_slot * (S::SLOT >> 4) + ((uint32_t)(S::KEYS * 128 >> 4) << 16);
-                    for (int k = 0; k < S::KEYS / 16; k++) dense::tg_mma_ts1(one, d, a + k * 8, b + k * (2048 >> 4), sum_form, j > 0 || k > 0);
-                    if (blocks == 1 || block == 1) dense::tg_commit1(one, &sh.empty[v_slot]);
-                    dense::tg_commit1(one, &sh.summed[block]);
-                };
-                // operand tiles come as K0 K1 V0 K2 V1 ...: with two blocks, K1 is waited for before V0 is used
-                if (blocks == 1) {
-                    scores(0);
-                    if (ok && items > 1) scores(1);
-                    for (int i = 0; i < items && ok; i++) {
-                        sums(i);
-                        if (ok && i + 2 < items) scores(i + 2);
-                    }
-                } else {
-                    scores(0);
-                    if (ok) scores(1);
-                    for (int j = 0; j < tiles && ok; j++) {
-                        const uint32_t next = j + 1 < tiles ? take() : 0;
-                        for (int block = 0; block < 2 && ok; block++) {
-                            sums(2 * j + block);
-                            if (ok && j + 1 < tiles) {
-                                const uint32_t d = tmem + (uint32_t)block * S::S_WIDTH, a = q_lo + (uint32_t)block * (S::Q_BLOCK >> 4), b = ring_lo + next * (S::SLOT >> 4);
-                                for (int k = 0; k < steps; k++)
-                                    dense::tg_mma_ss1(one, d, a + (uint32_t)(k >> 2) * (S::BLOCK * 128 >> 4) + (k & 3) * 2, b + (uint32_t)(k >> 2) * (S::KEYS * 128 >> 4) + (k & 3) * 2, score_form, k > 0);
-                                if (block == 1) dense::tg_commit1(one, &sh.empty[next]);
-                                dense::tg_commit1(one, &sh.scores[block]);
-                                if (block == 1 && j + 2 == tiles) dense::tg_commit1(one, &sh.queries_read);
+                dense::tg_commit1(one, &sh.scores[set]);
+            };
+            auto sums = [&](int block, int set, int j, uint32_t slot) {
+                if (j == 0 && part > 0) ok = ok && wait_warp(&sh.read[block], part - 1, gave_up);
+                ok = ok && wait_warp(&sh.weights[set], w_count[set]++, gave_up);
+                if (!ok) return;
+                tmem_after();
+                // 16 keys a step: two groups of 8 rows of 128 bytes; from 64 columns to the next: a box
+                const uint32_t d = tmem + S::O_AT + (uint32_t)block * DP, a = tmem + (uint32_t)set * S::S_WIDTH;
+                const uint32_t b = (ring_lo & 0xffffu) + slot * (S::SLOT >> 4) + ((uint32_t)(S::KEYS * 128 >> 4) << 16), more = j > 0;
+#pragma unroll
+                for (int k = 0; k < S::KEYS / 16; k++) dense::tg_mma_ts1(one, d, a + k * 8, b + k * (2048 >> 4), sum_form, k > 0 ? 1u : more);
+                dense::tg_commit1(one, &sh.summed[block]);
+            };
+            do {   // operand tiles come as K0 K1 V0 K2 V1 ...
+                enter();
+                ok = ok && wait_warp(&sh.queries, part, gave_up);
+                uint32_t slot = take();
+                if (ok) {
+                    scores(0, 0, slot);
+                    if (blocks == 2) scores(1, 1, slot);
+                    dense::tg_commit1(one, &sh.empty[slot]);
+                }
+                uint32_t next = tiles > 1 ? take() : 0;
+                if (ok && blocks == 1 && tiles > 1) {
+                    scores(0, 1, next);
+                    dense::tg_commit1(one, &sh.empty[next]);
+                }
+                if (ok && (tiles == 1 || (blocks == 1 && tiles == 2))) dense::tg_commit1(one, &sh.queries_read);
+                for (int j = 0; j < tiles && ok; j++) {
+                    // one block: sums of tile j, then the scores of tile j + 2 into the same set; two: sums of a block, then its scores of tile j + 1
+                    const uint32_t values = take();
+                    if (!ok) break;
+                    if (blocks == 1) {
+                        sums(0, j & 1, j, values);
+                        if (ok) dense::tg_commit1(one, &sh.empty[values]);
+                        if (j + 2 < tiles) {
+                            next = take();
+                            if (ok) {
+                                scores(0, j & 1, next);
+                                dense::tg_commit1(one, &sh.empty[next]);
+                                if (j + 3 == tiles) dense::tg_commit1(one, &sh.queries_read);
                             }
                         }
+                    } else {
+                        sums(0, 0, j, values);
+                        if (ok && j + 1 < tiles) scores(0, 0, next);
+                        sums(1, 1, j, values);
+                        if (!ok) break;
+                        dense::tg_commit1(one, &sh.empty[values]);
+                        if (j + 1 < tiles) {
+                            scores(1, 1, next);
+                            dense::tg_commit1(one, &sh.empty[next]);
+                            if (j + 2 == tiles) dense::tg_commit1(one, &sh.queries_read);
+                        }
+                        if (j + 2 < tiles) next = take();
                     }
                 }
                 part++;
             } while (ok && leave());
+            // the last commit is that of the last values' slot: none may arrive after the CTA has ended
+            if (ok) ok = wait_warp(&sh.empty[n == 0 ? S::SLOTS - 1 : n - 1], (int)(n == 0 ? round - 1 : round), gave_up);
             if (!ok)   // gave up: products already issued may still run; they get a millisecond to end before shared memory and TMEM go away
                 for (int i = 0; i < 1000; i++) __nanosleep(1000);
         }
         __syncwarp();
     } else {
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 192;");
         // ---- rows ----
         const int group = warp >> 2, row = threadIdx.x & 127;
         const uint32_t lanes = (uint32_t)(warp & 3) << 21;   // this warp's 32 TMEM lanes
@@ -302,44 +375,38 @@ __global__ void __launch_bounds__(512, 1) rows128_kernel(const __grid_constant__
                     ok = wait_warp(&sh.known[known], (k_count + j) / S::RING, gave_up) && wait_warp(&sh.scores[set], s_count[set] + (blocks == 2 ? j : j >> 1), gave_up);
                     if (!ok) break;
                     tmem_after();
-                    uint32_t v[S::KEYS / 32][32];
                     const uint32_t at = tmem + lanes + (uint32_t)set * S::S_WIDTH;
-#pragma unroll
-                    for (int c = 0; c < S::KEYS / 32; c++) dense::tg_tmem_ld32(at + 32 * c, v[c]);
-#pragma unroll
-                    for (int c = 0; c < S::KEYS / 32; c++) tmem_loaded(v[c]);
                     bool all = key0 + S::KEYS <= least;
 #pragma unroll
                     for (int c = 0; c < S::KEYS / 32; c++) all = all && sh.there[known][c] == ~0u;
-                    if (p.softcap > 0.0f) {
+                    auto sees = [&](int c) {   // bit i: the row sees key 32 c + i of the tile
+                        const int limit = r.keys - key0 - 32 * c;
+                        return sh.there[known][c] & (limit >= 32 ? ~0u : limit <= 0 ? 0u : (1u << limit) - 1);
+                    };
+                    // The scores are read twice, for the largest and for the weights: 128 of them in registers leave no room for anything else (700 bytes of spills).  A score
+                    // rises with its dot (falls, with a negative factor): the largest dot makes the largest score
+                    float tops[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-                        for (int c = 0; c < S::KEYS / 32; c++)
+                    for (int c = 0; c < S::KEYS / 32; c++) {
+                        uint32_t v[32];
+                        tmem_load32(at + 32 * c, v);
+                        if (p.scale2 < 0.0f) {
 #pragma unroll
-                            for (int i = 0; i < 32; i++) v[c][i] = __float_as_uint(score2(p, __uint_as_float(v[c][i])));
-                    } else {
-#pragma unroll
-                        for (int c = 0; c < S::KEYS / 32; c++)
-#pragma unroll
-                            for (int i = 0; i < 32; i++) v[c][i] = __float_as_uint(__uint_as_float(v[c][i]) * p.scale2);
-                    }
-                    if (!all) {
-#pragma unroll
-                        for (int c = 0; c < S::KEYS / 32; c++) {
-                            const int limit = r.keys - key0 - 32 * c;
-                            const uint32_t sees = sh.there[known][c] & (limit >= 32 ? ~0u : limit <= 0 ? 0u : (1u << limit) - 1);
-                            seen = seen || sees;
+                            for (int i = 0; i < 32; i++) v[i] ^= 0x80000000u;
+                        }
+                        if (!all) {
+                            const uint32_t mask = sees(c);
+                            seen = seen || mask;
 #pragma unroll
                             for (int i = 0; i < 32; i++)
-                                if (!(sees >> i & 1)) v[c][i] = 0xff800000u;
+                                if (!(mask >> i & 1)) v[i] = 0xff800000u;
                         }
-                    } else {
-                        seen = true;
+#pragma unroll
+                        for (int i = 0; i < 32; i += 2) tops[i >> 1 & 3] = fmaxf(fmaxf(tops[i >> 1 & 3], __uint_as_float(v[i])), __uint_as_float(v[i + 1]));
                     }
-                    float top = -INFINITY;
-#pragma unroll
-                    for (int c = 0; c < S::KEYS / 32; c++)
-#pragma unroll
-                        for (int i = 0; i < 32; i++) top = fmaxf(top, __uint_as_float(v[c][i]));
+                    seen = seen || all;
+                    float top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
+                    if (top != -INFINITY) top = score2(p, p.scale2 < 0.0f ? -top : top);
                     top -= WEIGHT_SHIFT<T>;
                     if (__any_sync(~0u, top > m + RESCALE_AT || (m == -INFINITY && top > m))) {
                         const float now = fmaxf(m, top), corr = ex2(m - (now == -INFINITY ? 0.0f : now));
@@ -351,8 +418,7 @@ __global__ void __launch_bounds__(512, 1) rows128_kernel(const __grid_constant__
                             for (int c = 0; c < D; c += 32) {
                                 uint32_t o[32];
                                 const uint32_t o_at = tmem + lanes + S::O_AT + (uint32_t)group * DP + c;
-                                dense::tg_tmem_ld32(o_at, o);
-                                tmem_loaded(o);
+                                tmem_load32(o_at, o);
 #pragma unroll
                                 for (int i = 0; i < 32; i++) o[i] = __float_as_uint(__uint_as_float(o[i]) * corr);
                                 tmem_store32(o_at, o);
@@ -363,20 +429,37 @@ __global__ void __launch_bounds__(512, 1) rows128_kernel(const __grid_constant__
                         m = now;
                     }
                     const float base = m == -INFINITY ? 0.0f : m;
-                    float s0 = 0.0f, s1 = 0.0f;
+                    float2 part_sums[2] = {};
 #pragma unroll
                     for (int c = 0; c < S::KEYS / 32; c++) {
-                        uint32_t a[16];
+                        uint32_t v[32], a[16];
+                        tmem_load32(at + 32 * c, v);
+                        float e[32];
+                        if (p.softcap > 0.0f) {
+#pragma unroll
+                            for (int i = 0; i < 32; i++) e[i] = __uint_as_float(v[i]);
+                            cap_scores(p, e);
+#pragma unroll
+                            for (int i = 0; i < 32; i++) e[i] = ex2(e[i] - base);
+                        } else {
+#pragma unroll
+                            for (int i = 0; i < 32; i++) e[i] = ex2(fmaf(__uint_as_float(v[i]), p.scale2, -base));
+                        }
+                        if (!all) {
+                            const uint32_t mask = sees(c);
+#pragma unroll
+                            for (int i = 0; i < 32; i++)
+                                if (!(mask >> i & 1)) e[i] = 0.0f;
+                        }
 #pragma unroll
                         for (int i = 0; i < 16; i++) {
-                            const float2 e = make_float2(ex2(__uint_as_float(v[c][2 * i]) - base), ex2(__uint_as_float(v[c][2 * i + 1]) - base));
-                            s0 += e.x;
-                            s1 += e.y;
-                            a[i] = close_word(e, T());
+                            part_sums[i & 1].x += e[2 * i];
+                            part_sums[i & 1].y += e[2 * i + 1];
+                            a[i] = close_word(make_float2(e[2 * i], e[2 * i + 1]), T());
                         }
-                        tmem_store16(at + 16 * c, a);   // (over scores that have been read)
+                        tmem_store16(at + 16 * c, a);   // (over scores that have been read: these 16 columns hold those of tile columns below 32 c + 32)
                     }
-                    sum += s0 + s1;
+                    sum += (part_sums[0].x + part_sums[0].y) + (part_sums[1].x + part_sums[1].y);
                     tmem_stored();
                     tmem_before();
                     arrive(&sh.weights[set]);
@@ -393,8 +476,7 @@ __global__ void __launch_bounds__(512, 1) rows128_kernel(const __grid_constant__
 #pragma unroll 1
                     for (int c = 0; c < D; c += 32) {
                         uint32_t o[32];
-                        dense::tg_tmem_ld32(tmem + lanes + S::O_AT + (uint32_t)group * DP + c, o);
-                        tmem_loaded(o);
+                        tmem_load32(tmem + lanes + S::O_AT + (uint32_t)group * DP + c, o);
                         if (!seen) {
 #pragma unroll
                             for (int i = 0; i < 32; i++) o[i] = 0;
@@ -470,6 +552,7 @@ __global__ void __launch_bounds__(512, 1) rows128_kernel(const __grid_constant__
     tmem_before();
     __syncthreads();
     if (warp == 12) {
+        __syncwarp();
         tmem_after();
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "n"(512) : "memory");
     }
