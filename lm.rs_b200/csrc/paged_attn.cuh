@@ -63,11 +63,13 @@ PG_DEVINL float* part_at(const Line& l, int head_size, int64_t slot, int row, in
 // (no more CTAs than tiles, so that each that takes part has some, and the parts of a unit are those of neighbours)
 PG_DEVINL int64_t cta_begin(int64_t total, int ctas, int i) {
     const int64_t n = min((int64_t)ctas, total);
-    return i < n ? total * i / n : total;
+    if (i >= n) return total;
+    const int64_t over = total * i;
+    return over >> 32 ? over / n : (int64_t)((uint32_t)over / (uint32_t)n);   // (a 64-bit division takes a hundred instructions)
 }
 PG_DEVINL int cta_of(int64_t total, int ctas, int64_t tile) {
     const int64_t over = min((int64_t)ctas, total) * (tile + 1) + total - 1;
-    return (over >> 32 ? (int)(over / total) : (int)((uint32_t)over / (uint32_t)total)) - 1;   // (a 64-bit division takes a hundred instructions)
+    return (over >> 32 ? (int)(over / total) : (int)((uint32_t)over / (uint32_t)total)) - 1;
 }
 
 // rows of a sequence's unit and the keys it goes through

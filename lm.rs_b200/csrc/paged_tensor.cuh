@@ -1,15 +1,15 @@
 // paged_tensor.cuh -- the same attention for many rows that see the same keys (the prefix, which all rows of a call share; portions of prompts), on the 5th-generation
 // tensor cores.  16-bit types; the line, its units and the parts are those of paged_attn.cuh, with 128 or 256 rows a unit.
 //
-// CTA = 16 warps, one CTA an SM.  The rows of a unit are one or two blocks of 128, a TMEM lane each; a step of the work is one block against one tile of keys:
+// CTA = 12 warps of 168 registers, one CTA an SM.  The rows of a unit are one or two blocks of 128, a TMEM lane each; a step of the work is one block against one tile of keys:
 //     scores = Q . K^T            tcgen05.mma, both operands in shared memory, 128 x KEYS sums in TMEM (two sets, taken in turn)
 //     weights = 2^(scores - m)    a thread a row: the scores from TMEM, the weights rounded to the type and back to TMEM over the scores
 //     o += weights . V            tcgen05.mma, the weights from TMEM, the values in shared memory as they lie in the pages (keys x columns: MN-major)
 //   warps 0-3, 4-7   the rows.  Two blocks: a group each, steps in turn, so that one's exponentials run under the other's products.  One block: the first group, and the
 //                    scores of the next tile are computed meanwhile.
-//   warps 8-11       copies of keys and values (16 bytes a thread, zeros for what is not there) into a ring of slots, one operand tile each, in the order K0 K1 V0 K2 V1 ...
+//   warps 8-9        copies of keys and values (16 bytes a thread, zeros for what is not there) into a ring of slots, one operand tile each, in the order K0 K1 V0 K2 V1 ...
 //                    The places of a tile's keys are looked up by a thread each; pages of any size and order cost the same.
-//   warp 12          the products
+//   warp 10          the products
 // o stays in TMEM for a whole part.  m is the largest score when it was last set; it is set anew, and o rescaled, only when a row's largest score has grown by
 // more than 2^8 (weights stay below 2^8 and sums are f32, so that nothing is lost), which is rare after the first tile.
 // Every wait on an mbarrier is bounded in time, as in dense_gemm.cuh.  Of a CTA that gives up, the rows that it still had to do come out as NaN.
@@ -21,7 +21,7 @@ namespace lmrs {
 namespace paged {
 
 template <typename T, int DP> struct TensorShape {
-    static constexpr int THREADS = 512, BLOCK = 128, BLOCKS = DP <= 128 ? 2 : 1, ROWS = BLOCK * BLOCKS, KEYS = DP <= 128 ? 128 : 64;
+    static constexpr int THREADS = 384, COPIERS = 2, BLOCK = 128, BLOCKS = DP <= 128 ? 2 : 1, ROWS = BLOCK * BLOCKS, KEYS = DP <= 128 ? 128 : 64;
     static constexpr int BOXES = DP / 64;                                   // 64 columns of an operand: rows of 128 bytes, their 16-byte pieces rotated (SWIZZLE_128B)
     static constexpr int SLOT = BOXES * KEYS * 128, SLOTS = DP <= 64 ? 6 : 4, Q_BLOCK = BOXES * BLOCK * 128;
     static constexpr int RING = 8;                                          // tiles whose keys' places are known
@@ -32,34 +32,15 @@ template <typename T, int DP> struct TensorShape {
 constexpr float RESCALE_AT = 8.0f;
 constexpr int PAGED_WAIT = 5 << 8;   // (what a wait was for is not reported: any number that is not 0)
 
-// A warp waits until phase number `count` of the barrier has ended (false: gave up).  One lane looks (9 warps of 32 looking lanes each filled the queue that copies to shared memory
-// go through, and every one of those took ten times as long), under a predicate and not in a branch of its own: what follows a wait - accesses to TMEM, products,
-// operands in uniform registers - is for a warp in step, and lanes that part here need not have met again by then.
+// A warp waits until phase number `count` of the barrier has ended (false: gave up).  All lanes look: a look suspends whoever looks, so that a lane which looks for the
+// others parts from them, and what follows a wait - accesses to TMEM, products, operands in uniform registers - is for a warp in step.
 PG_DEVINL bool wait_warp(uint64_t* bar, int count, volatile int* gave_up) {
-    const uint32_t looks = (threadIdx.x & 31) == 0, at = smem_at(bar), parity = (uint32_t)count & 1;
-    uint32_t from = 0;
-    for (uint32_t i = 0;; i++) {
-        uint32_t state;   // 1: ended, 2: give up
-        asm volatile(
-            "{\n\t.reg .pred p, l;\n\t"
-            "setp.ne.b32 l, %3, 0;\n\t"
-            "mov.u32 %0, 0;\n\t"
-            "@l mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
-            "@l selp.u32 %0, 1, 0, p;\n\t}"
-            : "=&r"(state)
-            : "r"(at), "r"(parity), "r"(looks)
-            : "memory");
-        const uint32_t now = dense::now_ns();
-        if (i < dense::TG_LEAST_TRIES) from = now;
-        if (state == 0 && (*gave_up || now - from > dense::TG_WAIT_NS)) state = 2;
-        state = __shfl_sync(~0u, state, 0);
-        if (state == 2) *gave_up = PAGED_WAIT;
-        if (state) {
-            __syncwarp();
-            return state == 1;
-        }
-    }
+    const bool ok = __all_sync(~0u, dense::mbar_wait_bounded(bar, (uint32_t)count & 1, gave_up, PAGED_WAIT));
+    __syncwarp();
+    return ok;
 }
+// has the phase ended?
+PG_DEVINL bool looks_free(uint64_t* bar, int count) { return __all_sync(~0u, dense::mbar_test(bar, (uint32_t)count & 1)); }
 PG_DEVINL void arrive(uint64_t* bar) { asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_at(bar)) : "memory"); }
 PG_DEVINL void tmem_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 PG_DEVINL void tmem_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
@@ -79,6 +60,26 @@ PG_DEVINL void tmem_load32(uint32_t at, uint32_t (&v)[32]) {
         : "r"(at)
         : "memory");
 }
+PG_DEVINL void tmem_load64(uint32_t at, uint32_t (&v)[64]) {
+    __syncwarp();
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {"
+        "%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+        "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%64];\n\t"
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {"
+        "%32, %33, %34, %35, %36, %37, %38, %39, %40, %41, %42, %43, %44, %45, %46, %47, "
+        "%48, %49, %50, %51, %52, %53, %54, %55, %56, %57, %58, %59, %60, %61, %62, %63}, [%65];\n\t"
+        "tcgen05.wait::ld.sync.aligned;"
+        : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]), "=r"(v[9]),
+          "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15]), "=r"(v[16]), "=r"(v[17]), "=r"(v[18]), "=r"(v[19]),
+          "=r"(v[20]), "=r"(v[21]), "=r"(v[22]), "=r"(v[23]), "=r"(v[24]), "=r"(v[25]), "=r"(v[26]), "=r"(v[27]), "=r"(v[28]), "=r"(v[29]),
+          "=r"(v[30]), "=r"(v[31]), "=r"(v[32]), "=r"(v[33]), "=r"(v[34]), "=r"(v[35]), "=r"(v[36]), "=r"(v[37]), "=r"(v[38]), "=r"(v[39]),
+          "=r"(v[40]), "=r"(v[41]), "=r"(v[42]), "=r"(v[43]), "=r"(v[44]), "=r"(v[45]), "=r"(v[46]), "=r"(v[47]), "=r"(v[48]), "=r"(v[49]),
+          "=r"(v[50]), "=r"(v[51]), "=r"(v[52]), "=r"(v[53]), "=r"(v[54]), "=r"(v[55]), "=r"(v[56]), "=r"(v[57]), "=r"(v[58]), "=r"(v[59]),
+          "=r"(v[60]), "=r"(v[61]), "=r"(v[62]), "=r"(v[63])
+        : "r"(at), "r"(at + 32)
+        : "memory");
+}
 PG_DEVINL void tmem_store32(uint32_t at, const uint32_t (&v)[32]) {
     __syncwarp();
     asm volatile(
@@ -88,12 +89,6 @@ PG_DEVINL void tmem_store32(uint32_t at, const uint32_t (&v)[32]) {
         "r"(v[8]), "r"(v[9]), "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15]), "r"(v[16]), "r"(v[17]), "r"(v[18]), "r"(v[19]), "r"(v[20]), "r"(v[21]), "r"(v[22]),
         "r"(v[23]), "r"(v[24]), "r"(v[25]), "r"(v[26]), "r"(v[27]), "r"(v[28]), "r"(v[29]), "r"(v[30]), "r"(v[31]), "r"(at)
         : "memory");
-}
-PG_DEVINL void tmem_store16(uint32_t at, const uint32_t (&v)[16]) {
-    __syncwarp();
-    asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15};" ::"r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]),
-                 "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]), "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15]), "r"(at)
-                 : "memory");
 }
 PG_DEVINL void tmem_stored() { __syncwarp(); asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
@@ -108,27 +103,28 @@ template <typename T, int DP> struct TensorShared {
     uint64_t queries_read;                      // the last product that reads the part's queries has ended
     uint64_t parted;                            // both groups have ended the part (neither runs ahead: phases are told apart by their parity alone)
     uint32_t there[S::RING][S::KEYS / 32];
-    int64_t starts[4][S::KEYS];                 // a copying warp's: where the keys' rows begin (elements; -1: nowhere)
+    int64_t starts[S::COPIERS][S::KEYS / S::COPIERS];             // a copying warp's: where the rows that it copies begin (bytes; -1: nowhere)
     uint32_t tmem;
     int gave_up;
     AgainScratch again[2];
 };
 
 template <typename T, int DP>
-__global__ void __launch_bounds__(512, 1) rows128_kernel(const __grid_constant__ AttnParams<T> p, const __grid_constant__ Line l) {
+__global__ void __launch_bounds__(384, 1) rows128_kernel(const __grid_constant__ AttnParams<T> p, const __grid_constant__ Line l) {
     using S = TensorShape<T, DP>;
     extern __shared__ uint8_t raw[];
     __shared__ TensorShared<T, DP> sh;
     uint8_t* ring = raw + (((smem_at(raw) + 1023u) & ~1023u) - smem_at(raw));   // (values of heads of up to 64 lie in one box: the next one's stride is never used)
     uint8_t* queries = ring + S::SLOTS * S::SLOT;
     const int warp = __shfl_sync(~0u, (int)threadIdx.x >> 5, 0), lane = threadIdx.x & 31, D = p.head_size;
+    constexpr int PRODUCTS = 8 + S::COPIERS;   // the warp that issues them
     volatile int* gave_up = &sh.gave_up;
 
     if (threadIdx.x == 0) {
-        for (int i = 0; i < S::SLOTS; i++) { mbar_init(&sh.full[i], 1); mbar_init(&sh.empty[i], 1); }
-        for (int i = 0; i < S::RING; i++) mbar_init(&sh.known[i], 1);
+        for (int i = 0; i < S::SLOTS; i++) { mbar_init(&sh.full[i], S::COPIERS); mbar_init(&sh.empty[i], 1); }
+        for (int i = 0; i < S::RING; i++) mbar_init(&sh.known[i], S::COPIERS);
         for (int i = 0; i < 2; i++) { mbar_init(&sh.scores[i], 1); mbar_init(&sh.weights[i], 128); mbar_init(&sh.summed[i], 1); mbar_init(&sh.read[i], 128); }
-        mbar_init(&sh.queries, 128);
+        mbar_init(&sh.queries, 32 * S::COPIERS);
         mbar_init(&sh.queries_read, 1);
         mbar_init(&sh.parted, 256);
         sh.gave_up = 0;
@@ -138,7 +134,7 @@ __global__ void __launch_bounds__(512, 1) rows128_kernel(const __grid_constant__
     int64_t from, to;
     walk_begin<T, S::THREADS>(p, l, w, from, to);   // (synchronises the CTA)
     if (from >= to) { grid_launch(); return; }
-    if (warp == 12) {
+    if (warp == PRODUCTS) {
         __syncwarp();
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_at(&sh.tmem)), "n"(512) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
@@ -162,85 +158,87 @@ __global__ void __launch_bounds__(512, 1) rows128_kernel(const __grid_constant__
         if (w.tiles == 0) { left = 0; return false; }   // (the line ended early: lengths changed under the kernel)
         return true;
     };
-    // (Every thread keeps its 128 registers.  Moved from the copying warps to the rows by setmaxnreg they were not safe: the compiler gave code of the copying warps
+    // (Every thread keeps its registers.  Moved from the copying warps to the rows by setmaxnreg they were not safe: the compiler gave code of the copying warps
     // more than was left to them)
     if (warp >= 8) {
-        if (warp < 12) {
-            // ---- copies: operand tile n is warp n % 4's, which waits for its slot, copies, and reports it when it has landed; the other warps are at theirs ----
-            const int mine = warp - 8, t = threadIdx.x - 256, pieces = (D + 15) / 16 * 2, whole = D / 8;
+        if (warp < 8 + S::COPIERS) {
+            // ---- copies: each of the two warps half of every operand tile's rows; up to two are on their way while the next is asked for ----
+            constexpr int SHARE = S::KEYS / S::COPIERS, EACH = SHARE / 32;   // rows a warp copies, a lane looks up
+            const int mine = warp - 8, t = threadIdx.x - 256, pieces = (D + 15) / 16 * 2, whole = D / 8, c = lane & 7;
             int64_t* starts = sh.starts[mine];
-            uint32_t n = 0;       // operand tiles of the CTA so far
+            uint32_t n = 0, slot = 0, round = 0, reported = 0, report_slot = 0;   // operand tiles asked for, the next one's slot and round of the ring; those reported
             int looked = 0, part = 0;
-            bool ok = true;
-            bool asked = false;   // queries are on their way
-            auto landed = [&]() {
-                copy_wait<0>();
+            bool ok = true, asked = false;   // asked: queries are on their way
+            auto report = [&](uint32_t upto) {   // (they have landed)
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-                if (asked) arrive(&sh.queries);
-                asked = false;
-            };
-            auto operand = [&](const T* base, bool values, int j) {   // tile j of the part; looked: its number in the CTA
-                const uint32_t slot = n % S::SLOTS, round = n / S::SLOTS;
-                if ((n++ & 3) != (uint32_t)mine || !ok) return;
-                // the places of its keys, four a lane
-                const int set = looked % S::RING;
+                if (asked && upto > reported) { arrive(&sh.queries); asked = false; }
                 __syncwarp();
-#pragma unroll
-                for (int i = 0; i < S::KEYS / 32; i++) {
-                    const Place at = unit_place(p, w, (w.tile + j) * S::KEYS + 32 * i + lane);
-                    starts[32 * i + lane] = at.page < 0 ? -1
-                                            : values    ? at.page * p.v_page + at.place * p.v_slot + w.head * p.v_head
-                                                        : at.page * p.k_page + at.place * p.k_slot + w.head * p.k_head;
-                    if (!values) {
-                        const unsigned bits = __ballot_sync(~0u, at.page >= 0);
-                        if (lane == 0) sh.there[set][i] = bits;
-                    }
+                for (; reported < upto; reported++) {
+                    if (lane == 0) arrive(&sh.full[report_slot]);
+                    report_slot = report_slot + 1 == S::SLOTS ? 0 : report_slot + 1;
+                }
+            };
+            auto operand = [&](const T* base, const int64_t (&start)[EACH]) {   // start: where rows lane, lane + 32 of the warp's begin, in bytes; -1: nowhere
+                if (!ok) return;
+                if (!looks_free(&sh.empty[slot], (int)round + 1)) {   // (nothing that has landed waits for a slot to come free)
+                    copy_wait<0>();
+                    report(n);
+                    ok = wait_warp(&sh.empty[slot], (int)round + 1, gave_up);
+                    if (!ok) return;
                 }
                 __syncwarp();
-                if (!values && lane == 0) arrive(&sh.known[set]);
-                ok = wait_warp(&sh.empty[slot], (int)round + 1, gave_up);
-                if (!ok) return;
-                const uint32_t at = smem_at(ring) + slot * S::SLOT;
-                const int c = lane & 7;
+#pragma unroll
+                for (int i = 0; i < EACH; i++) starts[32 * i + lane] = start[i];
+                __syncwarp();
+                const uint32_t at = smem_at(ring) + slot * S::SLOT + (mine * SHARE + (lane >> 3)) * 128;
+                const char* from = reinterpret_cast<const char*>(base) + 16 * c;
 #pragma unroll 1
-                for (int r0 = lane >> 3; r0 < S::KEYS; r0 += 16) {   // (four rows' places are read before their copies are asked for)
-                    const T* row[4];
+                for (int i0 = 0; i0 < SHARE / 4; i0 += 8) {   // (eight rows a lane: their places are read before their copies are asked for)
+                    int64_t rows[8];
 #pragma unroll
-                    for (int i = 0; i < 4; i++) {
-                        const int64_t start = starts[r0 + 4 * i];
-                        row[i] = start < 0 ? nullptr : base + start + 8 * c;
-                    }
+                    for (int i = 0; i < 8; i++) rows[i] = starts[4 * (i0 + i) + (lane >> 3)];
 #pragma unroll
-                    for (int i = 0; i < 4; i++) {
-                        const int r = r0 + 4 * i;
-                        const uint32_t to_row = at + r * 128 + ((c ^ (r & 7)) << 4);
+                    for (int i = 0; i < 8; i++) {
+                        const uint32_t to_row = at + (i0 + i) * 512 + ((c ^ ((4 * i + (lane >> 3)) & 7)) << 4);
+                        if (whole == DP / 8) {
+                            const char* row = from + (rows[i] < 0 ? 0 : rows[i]);
 #pragma unroll
-                        for (int b = 0; b < S::BOXES; b++)
-                            if (8 * b + c < pieces) {
-                                const bool in = row[i] && 8 * b + c < whole;
-                                copy16(to_row + b * S::KEYS * 128, in ? row[i] + 64 * b : base, in);
-                            }
+                            for (int b = 0; b < S::BOXES; b++) copy16(to_row + b * S::KEYS * 128, row + 128 * b, rows[i] >= 0);
+                        } else {
+#pragma unroll
+                            for (int b = 0; b < S::BOXES; b++)
+                                if (8 * b + c < pieces) {
+                                    const bool in = rows[i] >= 0 && 8 * b + c < whole;
+                                    copy16(to_row + b * S::KEYS * 128, in ? from + rows[i] + 128 * b : reinterpret_cast<const char*>(base), in);
+                                }
+                        }
                     }
                 }
                 copy_commit();
-                landed();
-                __syncwarp();
-                if (lane == 0) arrive(&sh.full[slot]);
+                n++;
+                if (++slot == S::SLOTS) { slot = 0; round++; }
+                copy_wait<2>();
+                if (n > 2) report(n - 2);
             };
             do {
                 enter();
                 if (part > 0) ok = ok && wait_warp(&sh.queries_read, part - 1, gave_up);
                 if (ok) {   // the queries: eight threads a row; they are reported with the operand tile that follows
-                    const int c = t & 7;
-#pragma unroll 2
-                    for (int x = t >> 3; x < blocks * S::BLOCK; x += 16) {
-                        const UnitRow r = unit_row(p, l, w, x);
-                        const T* q = r.row >= 0 ? p.q.data + r.row * p.q.row + r.head * p.q.head + 8 * c : p.q.data;
+                    constexpr int AT_ONCE = 4 * S::COPIERS;
+                    const int x0 = t >> 3, i0 = w.row_tile * S::ROWS + x0, step = AT_ONCE / p.group, more = AT_ONCE - step * p.group;
+                    int token = i0 / p.group, g = i0 - token * p.group;
+#pragma unroll 4
+                    for (int x = x0; x < blocks * S::BLOCK; x += AT_ONCE) {
+                        const bool is = x < used;
+                        const T* q = is ? p.q.data + ((w.b < 0 ? 0 : w.s.first) + token) * p.q.row + (w.head * p.group + g) * p.q.head + 8 * c : p.q.data;
+                        token += step;
+                        g += more;
+                        if (g >= p.group) { g -= p.group; token++; }
                         uint8_t* to_q = queries + (x >> 7) * S::Q_BLOCK + (x & 127) * 128 + ((c ^ (x & 7)) << 4);
 #pragma unroll
                         for (int b = 0; b < S::BOXES; b++) {
                             if (8 * b + c >= pieces) continue;
-                            const bool in = r.row >= 0 && 8 * b + c < whole;
+                            const bool in = is && 8 * b + c < whole;
                             if (p.q_wide) {
                                 copy16(smem_at(to_q + b * (S::BLOCK * 128)), in ? q + 64 * b : p.q.data, in);
                             } else {
@@ -251,21 +249,43 @@ __global__ void __launch_bounds__(512, 1) rows128_kernel(const __grid_constant__
                             }
                         }
                     }
-                    copy_commit();
+                    __syncwarp();
                     asked = true;
                 }
-                const int first = looked;
-                auto keys = [&](int j) { looked = first + j; operand(p.k, false, j); };
+                int64_t values[EACH], next_values[EACH];   // where the values of tiles j and j + 1 begin
+                auto keys = [&](int j) {   // tile j of the part: where its keys and values lie, and which are there; then the keys
+                    const int set = looked++ % S::RING;
+                    int64_t start[EACH];
+#pragma unroll
+                    for (int i = 0; i < EACH; i++) {
+                        const Place at = unit_place(p, w, (w.tile + j) * S::KEYS + mine * SHARE + 32 * i + lane);
+                        const bool is = at.page >= 0;
+                        values[i] = next_values[i];
+                        next_values[i] = is ? (at.page * p.v_page + at.place * p.v_slot + w.head * p.v_head) * (int64_t)sizeof(T) : -1;
+                        start[i] = is ? (at.page * p.k_page + at.place * p.k_slot + w.head * p.k_head) * (int64_t)sizeof(T) : -1;
+                        const unsigned bits = __ballot_sync(~0u, is);
+                        if (lane == 0) sh.there[set][mine * EACH + i] = bits;
+                    }
+                    if (lane == 0 && ok) arrive(&sh.known[set]);
+                    operand(p.k, start);
+                };
+#pragma unroll
+                for (int i = 0; i < EACH; i++) next_values[i] = -1;
                 keys(0);
                 for (int j = 0; j < tiles; j++) {
-                    if (j + 1 < tiles) keys(j + 1);
-                    operand(p.v, true, j);
+                    if (j + 1 < tiles) {
+                        keys(j + 1);
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < EACH; i++) values[i] = next_values[i];
+                    }
+                    operand(p.v, values);
                 }
-                looked = first + tiles;
-                if (asked) landed();   // (a warp that no operand tile fell to)
+                copy_wait<0>();   // (the next part waits for the queries' last reader, which needs all of this one)
+                report(n);
                 part++;
             } while (leave());
-        } else if (warp == 12) {
+        } else if (warp == PRODUCTS) {
             // ---- products ----
             const uint32_t one = dense::elect_one(), type = sizeof(T) == 2 && std::is_same<T, __nv_bfloat16>::value ? 1u : 0u;
             const uint32_t form = (1u << 4) | (type << 7) | (type << 10) | ((uint32_t)(S::BLOCK >> 4) << 24);   // f32 += T x T, 128 rows
@@ -300,7 +320,7 @@ __global__ void __launch_bounds__(512, 1) rows128_kernel(const __grid_constant__
                 const uint32_t d = tmem + S::O_AT + (uint32_t)block * DP, a = tmem + (uint32_t)set * S::S_WIDTH;
                 const uint32_t b = (ring_lo & 0xffffu) + slot * (S::SLOT >> 4) + ((uint32_t)(S::KEYS * 128 >> 4) << 16), more = j > 0;
 #pragma unroll
-                for (int k = 0; k < S::KEYS / 16; k++) dense::tg_mma_ts1(one, d, a + k * 8, b + k * (2048 >> 4), sum_form, k > 0 ? 1u : more);
+                for (int k = 0; k < S::KEYS / 16; k++) dense::tg_mma_ts1(one, d, a + (k < 4 ? k * 8 : 64 + (k - 4) * 8), b + k * (2048 >> 4), sum_form, k > 0 ? 1u : more);   // (weights of 64 keys over the first half of their scores)
                 dense::tg_commit1(one, &sh.summed[block]);
             };
             do {   // operand tiles come as K0 K1 V0 K2 V1 ...
@@ -383,27 +403,25 @@ __global__ void __launch_bounds__(512, 1) rows128_kernel(const __grid_constant__
                         const int limit = r.keys - key0 - 32 * c;
                         return sh.there[known][c] & (limit >= 32 ? ~0u : limit <= 0 ? 0u : (1u << limit) - 1);
                     };
-                    // The scores are read twice, for the largest and for the weights: 128 of them in registers leave no room for anything else (700 bytes of spills).  A score
-                    // rises with its dot (falls, with a negative factor): the largest dot makes the largest score
+                    // A score rises with its dot (falls, with a negative factor): the largest dot makes the largest score.  64 scores stay in registers; of 128, the
+                    // first half is read again for its weights (all of them in registers leave no room for anything else)
+                    uint32_t v[64];
                     float tops[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+                    auto largest = [&](int half) {
+                        tmem_load64(at + 64 * half, v);
+                        if (all && !(p.scale2 < 0.0f)) {
 #pragma unroll
-                    for (int c = 0; c < S::KEYS / 32; c++) {
-                        uint32_t v[32];
-                        tmem_load32(at + 32 * c, v);
-                        if (p.scale2 < 0.0f) {
-#pragma unroll
-                            for (int i = 0; i < 32; i++) v[i] ^= 0x80000000u;
+                            for (int i = 0; i < 64; i += 2) tops[i >> 1 & 3] = fmaxf(fmaxf(tops[i >> 1 & 3], __uint_as_float(v[i])), __uint_as_float(v[i + 1]));
+                            return;
                         }
-                        if (!all) {
-                            const uint32_t mask = sees(c);
-                            seen = seen || mask;
+                        const uint32_t sign = p.scale2 < 0.0f ? 0x80000000u : 0u, mask[2] = {sees(2 * half), sees(2 * half + 1)};
+                        seen = seen || mask[0] || mask[1];
 #pragma unroll
-                            for (int i = 0; i < 32; i++)
-                                if (!(mask >> i & 1)) v[i] = 0xff800000u;
-                        }
-#pragma unroll
-                        for (int i = 0; i < 32; i += 2) tops[i >> 1 & 3] = fmaxf(fmaxf(tops[i >> 1 & 3], __uint_as_float(v[i])), __uint_as_float(v[i + 1]));
-                    }
+                        for (int i = 0; i < 64; i++)
+                            if (mask[i >> 5] >> (i & 31) & 1) tops[i & 3] = fmaxf(tops[i & 3], __uint_as_float(v[i] ^ sign));
+                    };
+                    largest(0);
+                    if constexpr (S::KEYS == 128) largest(1);
                     seen = seen || all;
                     float top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
                     if (top != -INFINITY) top = score2(p, p.scale2 < 0.0f ? -top : top);
@@ -429,37 +447,44 @@ __global__ void __launch_bounds__(512, 1) rows128_kernel(const __grid_constant__
                         m = now;
                     }
                     const float base = m == -INFINITY ? 0.0f : m;
-                    float2 part_sums[2] = {};
-#pragma unroll
-                    for (int c = 0; c < S::KEYS / 32; c++) {
-                        uint32_t v[32], a[16];
-                        tmem_load32(at + 32 * c, v);
-                        float e[32];
+                    float sums4[4] = {};
+                    auto weigh = [&](int half) {   // the scores in v become weights
                         if (p.softcap > 0.0f) {
 #pragma unroll
-                            for (int i = 0; i < 32; i++) e[i] = __uint_as_float(v[i]);
-                            cap_scores(p, e);
+                            for (int k = 0; k < 64; k += 16) {
+                                float e[16];
 #pragma unroll
-                            for (int i = 0; i < 32; i++) e[i] = ex2(e[i] - base);
+                                for (int i = 0; i < 16; i++) e[i] = __uint_as_float(v[k + i]);
+                                cap_scores(p, e);
+#pragma unroll
+                                for (int i = 0; i < 16; i++) v[k + i] = __float_as_uint(ex2(e[i] - base));
+                            }
                         } else {
 #pragma unroll
-                            for (int i = 0; i < 32; i++) e[i] = ex2(fmaf(__uint_as_float(v[i]), p.scale2, -base));
+                            for (int i = 0; i < 64; i++) v[i] = __float_as_uint(ex2(fmaf(__uint_as_float(v[i]), p.scale2, -base)));
                         }
                         if (!all) {
-                            const uint32_t mask = sees(c);
+                            const uint32_t mask[2] = {sees(2 * half), sees(2 * half + 1)};
 #pragma unroll
-                            for (int i = 0; i < 32; i++)
-                                if (!(mask >> i & 1)) e[i] = 0.0f;
+                            for (int i = 0; i < 64; i++)
+                                if (!(mask[i >> 5] >> (i & 31) & 1)) v[i] = 0;
                         }
+                        uint32_t a[32];
 #pragma unroll
-                        for (int i = 0; i < 16; i++) {
-                            part_sums[i & 1].x += e[2 * i];
-                            part_sums[i & 1].y += e[2 * i + 1];
-                            a[i] = close_word(make_float2(e[2 * i], e[2 * i + 1]), T());
+                        for (int i = 0; i < 32; i++) {
+                            const float2 e = make_float2(__uint_as_float(v[2 * i]), __uint_as_float(v[2 * i + 1]));
+                            sums4[2 * i & 3] += e.x;
+                            sums4[(2 * i + 1) & 3] += e.y;
+                            a[i] = close_word(e, T());
                         }
-                        tmem_store16(at + 16 * c, a);   // (over scores that have been read: these 16 columns hold those of tile columns below 32 c + 32)
+                        tmem_store32(at + 64 * half, a);   // (over scores that have been read)
+                    };
+                    if constexpr (S::KEYS == 128) {
+                        weigh(1);
+                        tmem_load64(at, v);
                     }
-                    sum += (part_sums[0].x + part_sums[0].y) + (part_sums[1].x + part_sums[1].y);
+                    weigh(0);
+                    sum += (sums4[0] + sums4[1]) + (sums4[2] + sums4[3]);
                     tmem_stored();
                     tmem_before();
                     arrive(&sh.weights[set]);
@@ -472,7 +497,10 @@ __global__ void __launch_bounds__(512, 1) rows128_kernel(const __grid_constant__
                 if (ok) {
                     tmem_after();
                     if (!seen) sum = -1.0f;
-                    bool finite = true;
+                    float odd = 0.0f;   // becomes NaN if a sum is not finite
+                    float* to = whole ? nullptr : part_at(l, D, slot, x, 0);
+                    const bool store = is && (whole || slot < l.slots);
+                    const float by = seen ? 1.0f / sum : 1.0f;   // (0: 1 / 0 * 0 is NaN, as 0 / 0 is)
 #pragma unroll 1
                     for (int c = 0; c < D; c += 32) {
                         uint32_t o[32];
@@ -482,19 +510,26 @@ __global__ void __launch_bounds__(512, 1) rows128_kernel(const __grid_constant__
                             for (int i = 0; i < 32; i++) o[i] = 0;
                         }
 #pragma unroll
-                        for (int i = 0; i < 32; i += 4) {
-                            if (c + i >= D) continue;
+                        for (int i = 0; i < 32; i += 8) {
+                            if (c + i >= D) break;   // (D is a multiple of 8)
                             float4 f = make_float4(__uint_as_float(o[i]), __uint_as_float(o[i + 1]), __uint_as_float(o[i + 2]), __uint_as_float(o[i + 3]));
-                            finite = finite && isfinite(f.x + f.y + f.z + f.w);
-                            if (!is) continue;
+                            float4 g = make_float4(__uint_as_float(o[i + 4]), __uint_as_float(o[i + 5]), __uint_as_float(o[i + 6]), __uint_as_float(o[i + 7]));
+                            odd = fmaf(f.x, 0.0f, fmaf(f.y, 0.0f, fmaf(f.z, 0.0f, fmaf(f.w, 0.0f, odd))));
+                            odd = fmaf(g.x, 0.0f, fmaf(g.y, 0.0f, fmaf(g.z, 0.0f, fmaf(g.w, 0.0f, odd))));
+                            if (!store) continue;
                             if (whole) {
-                                if (seen) { f.x /= sum; f.y /= sum; f.z /= sum; f.w /= sum; }
+                                f.x *= by; f.y *= by; f.z *= by; f.w *= by;
+                                g.x *= by; g.y *= by; g.z *= by; g.w *= by;
                                 store_row(p, r, c + i, f);
-                            } else if (slot < l.slots) {
-                                *reinterpret_cast<float4*>(part_at(l, D, slot, x, c + i)) = f;
+                                store_row(p, r, c + i + 4, g);
+                            } else {
+                                float4* at8 = reinterpret_cast<float4*>(to + (int64_t)((c + i) >> 3) * (S::ROWS * 8));
+                                at8[0] = f;
+                                at8[1] = g;
                             }
                         }
                     }
+                    const bool finite = odd == 0.0f;
                     if (is) {
                         if (whole) { if (p.lse) p.lse[r.row * p.q_heads + r.head] = seen ? lse_of(m, sum) : -INFINITY; }
                         else if (slot < l.slots) l.ml[slot * S::ROWS + x] = make_float2(m, sum);
@@ -551,7 +586,7 @@ __global__ void __launch_bounds__(512, 1) rows128_kernel(const __grid_constant__
     }
     tmem_before();
     __syncthreads();
-    if (warp == 12) {
+    if (warp == PRODUCTS) {
         __syncwarp();
         tmem_after();
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "n"(512) : "memory");
