@@ -334,10 +334,10 @@ template <typename T> PG_DEVINL bool whole_unit(const AttnParams<T>& p, const Wa
 // the units that follow, with the places of the keys one tile further ahead; rows are 16-byte pieces rotated by the row's number, which keeps all reads
 // free of bank conflicts.  A page may end anywhere in a tile.
 template <typename T, int DP> struct TileShape {
-    static constexpr int ROWS = 16, THREADS = 128, ROW = DP * (int)sizeof(T), PIECES = ROW / 16, KEYS = ROW > 512 ? 32 : 64, STAGES = ROW > 512 ? 2 : 3;
+    static constexpr int ROWS = 16, THREADS = 128, ROW = DP * (int)sizeof(T), PIECES = ROW / 16, KEYS = sizeof(T) == 4 && DP > 64 ? 32 : 64, STAGES = sizeof(T) == 4 ? 2 : 3;
     static constexpr int WARP_KEYS = KEYS / 4, COPY_KEYS = KEYS / 32;   // keys a warp works on; keys a thread copies a quarter of
     static constexpr int KV = KEYS * ROW, Q = ROWS * ROW, SMEM = STAGES * (2 * KV + Q);   // (queries: one set for each unit that copies can have got to)
-    static constexpr int CTAS = ROW <= 128 ? 3 : ROW <= 256 ? 2 : 1;
+    static constexpr int CTAS = ROW <= 128 ? 3 : ROW <= (sizeof(T) == 4 ? 512 : 256) ? 2 : 1;
     static_assert(4 * ROWS * DP * 4 <= 2 * KV, "the four warps' rows fit where a tile's keys and values were");
 };
 PG_DEVINL uint32_t piece_at(int row, int piece, int row_bytes) { return (uint32_t)(row * row_bytes + ((piece ^ (row & 7)) << 4)); }
@@ -509,68 +509,86 @@ template <int DP> struct WarpTile<float, DP> {
     }
     // scratch: the warp's own [KEYS + 1][16] floats: weights, and what the rows' sums are rescaled by
     PG_DEVINL void tile(const AttnParams<float>& p, uint32_t q_at, uint32_t k_at, uint32_t v_at, uint32_t there, int first, const int* row_keys, int used, float* scratch) {
+        if (used <= 4) rows<4>(p, q_at, k_at, v_at, there, first, row_keys, scratch);
+        else if (used <= 8) rows<8>(p, q_at, k_at, v_at, there, first, row_keys, scratch);
+        else rows<16>(p, q_at, k_at, v_at, there, first, row_keys, scratch);
+    }
+    template <int ROWS> PG_DEVINL void rows(const AttnParams<float>& p, uint32_t q_at, uint32_t k_at, uint32_t v_at, uint32_t there, int first, const int* row_keys, float* scratch) {
+        constexpr int MINE = ROWS / TEAMS;
         const int lane = threadIdx.x & 31, key0 = KEYS * (threadIdx.x >> 5), key = lane % KEYS, team = lane / KEYS;
-        float s[SHARE] = {};
-#pragma unroll 4
-        for (int c = 0; c < p.head_size / 4; c++) {
-            const float4 k = load4(k_at + piece_at(key0 + key, c, S::ROW));
+        float s[MINE] = {};
+        const uint32_t k_row = k_at + (key0 + key) * S::ROW, k_turn = (uint32_t)(key & 7) << 4;
 #pragma unroll
-            for (int i = 0; i < SHARE; i++)
-                if (i * TEAMS < used) {
-                    const float4 q = load4(q_at + piece_at(i * TEAMS + team, c, S::ROW));
-                    s[i] = fmaf(q.x, k.x, fmaf(q.y, k.y, fmaf(q.z, k.z, fmaf(q.w, k.w, s[i]))));
-                }
+        for (int c = 0; c < DP / 4; c++) {   // (past the end of a head there are zeros)
+            const float4 k = load4(k_row + (k_turn ^ (16 * c)));
+#pragma unroll
+            for (int i = 0; i < MINE; i++) {
+                const float4 q = load4(q_at + piece_at(i * TEAMS + team, c, S::ROW));
+                s[i] = fmaf(q.x, k.x, fmaf(q.y, k.y, fmaf(q.z, k.z, fmaf(q.w, k.w, s[i]))));
+            }
         }
         __syncwarp();   // (the weights of the tile before have been read)
+        float now[MINE];
+        bool sees[MINE];
 #pragma unroll
-        for (int i = 0; i < SHARE; i++)
-            if (i * TEAMS < used) {
-                const int row = i * TEAMS + team;
-                const bool sees = (there >> key & 1) && first + key < row_keys[row];
-                const float a = sees ? score2(p, s[i]) : -INFINITY;
-                float top = a;
+        for (int i = 0; i < MINE; i++) {
+            sees[i] = (there >> key & 1) && first + key < row_keys[i * TEAMS + team];
+            s[i] = now[i] = sees[i] ? score2(p, s[i]) : -INFINITY;
+        }
 #pragma unroll
-                for (int d = KEYS / 2; d; d >>= 1) top = fmaxf(top, __shfl_xor_sync(~0u, top, d));
-                const float now = fmaxf(m[i], top), base = now == -INFINITY ? 0.0f : now, corr = ex2(m[i] - base), w = ex2(a - base);
-                m[i] = now;
-                l[i] = l[i] * corr + w;   // (this lane's keys)
-                seen[i] = seen[i] || sees;
-                scratch[key * 16 + row] = w;
-                if (key == 0) scratch[KEYS * 16 + row] = corr;
+        for (int d = KEYS / 2; d; d >>= 1)
+#pragma unroll
+            for (int i = 0; i < MINE; i++) now[i] = fmaxf(now[i], __shfl_xor_sync(~0u, now[i], d));
+        bool grows = false;
+#pragma unroll
+        for (int i = 0; i < MINE; i++) grows = grows || now[i] > m[i];
+        const bool rescale = __any_sync(~0u, grows);
+#pragma unroll
+        for (int i = 0; i < MINE; i++) {
+            const float top = fmaxf(m[i], now[i]), base = top == -INFINITY ? 0.0f : top, corr = ex2(m[i] - base), w = ex2(s[i] - base);
+            if (rescale) {
+                m[i] = top;
+                l[i] *= corr;
+                if (key == 0) scratch[KEYS * 16 + i * TEAMS + team] = corr;
             }
+            l[i] += w;   // (this lane's keys)
+            seen[i] = seen[i] || sees[i];
+            scratch[key * 16 + i * TEAMS + team] = w;
+        }
         __syncwarp();
+        if (rescale) {
 #pragma unroll
-        for (int r = 0; r < 16; r++)
-            if ((r & ~3) < used) {
+            for (int r = 0; r < ROWS; r++) {
                 const float corr = scratch[KEYS * 16 + r];
 #pragma unroll
                 for (int c = 0; c < COLS; c++) o[r][c] *= corr;
             }
-#pragma unroll 2
+        }
+        const uint32_t v_row = v_at + key0 * S::ROW;
+#pragma unroll
         for (int j = 0; j < KEYS; j++) {
             float v[COLS];
             if constexpr (COLS == 2) {
-                const float2 x = load2(v_at + piece_at(key0 + j, lane >> 1, S::ROW) + 8 * (lane & 1));
+                const float2 x = load2(v_row + piece_at(j, lane >> 1, S::ROW) + 8 * (lane & 1));
                 v[0] = x.x; v[1] = x.y;
             } else {
 #pragma unroll
                 for (int c = 0; c < COLS; c += 4) {
-                    const float4 x = load4(v_at + piece_at(key0 + j, lane + 8 * c, S::ROW));
+                    const float4 x = load4(v_row + piece_at(j, lane + 8 * c, S::ROW));
                     v[c] = x.x; v[c + 1] = x.y; v[c + 2] = x.z; v[c + 3] = x.w;
                 }
             }
 #pragma unroll
-            for (int r = 0; r < 16; r += 4)
-                if (r < used) {
-                    const float4 w = *reinterpret_cast<const float4*>(scratch + j * 16 + r);
+            for (int r = 0; r < ROWS; r += 4) {
+                const float4 w = *reinterpret_cast<const float4*>(scratch + j * 16 + r);
 #pragma unroll
-                    for (int c = 0; c < COLS; c++) {
-                        o[r][c] = fmaf(w.x, v[c], o[r][c]);
-                        o[r + 1][c] = fmaf(w.y, v[c], o[r + 1][c]);
-                        o[r + 2][c] = fmaf(w.z, v[c], o[r + 2][c]);
-                        o[r + 3][c] = fmaf(w.w, v[c], o[r + 3][c]);
-                    }
+                for (int c = 0; c < COLS; c++) {
+                    o[r][c] = fmaf(w.x, v[c], o[r][c]);
+                    o[r + 1][c] = fmaf(w.y, v[c], o[r + 1][c]);
+                    o[r + 2][c] = fmaf(w.z, v[c], o[r + 2][c]);
+                    o[r + 3][c] = fmaf(w.w, v[c], o[r + 3][c]);
                 }
+            }
         }
     }
     PG_DEVINL void put_ml(float2* ml) {
@@ -599,7 +617,6 @@ template <int DP> struct WarpTile<float, DP> {
     }
 };
 
-// (the f32 sums' 128 registers for heads of 256 leave no room for more than one CTA anyway)
 template <typename T, int DP>
 __global__ void __launch_bounds__(TileShape<T, DP>::THREADS, TileShape<T, DP>::CTAS) rows16_kernel(const __grid_constant__ AttnParams<T> p, const __grid_constant__ Line l) {
     using S = TileShape<T, DP>;

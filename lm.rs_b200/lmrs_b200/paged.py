@@ -8,7 +8,6 @@ the host, and calls can be captured into CUDA graphs.
     q     = append(pages, batch, k_new, v_new, rope=rope, q=q)
     out   = attention(pages, batch, q)
 """
-import contextlib
 import ctypes as C
 
 import torch
@@ -86,22 +85,16 @@ def _ints(t, name, device):
 
 def _positions(pos, axes, rows, device):
     _ints(pos, "pos", device)
-    if pos.dim() == 1 and axes == 1 and pos.shape[0] == rows:
+    shape = pos.shape
+    if len(shape) == 2 and shape[0] >= axes and shape[1] == rows:
+        return _Positions(pos.data_ptr(), *pos.stride())
+    if len(shape) == 1 and axes == 1 and shape[0] == rows:
         return _Positions(pos.data_ptr(), 0, pos.stride(0))
-    if pos.dim() != 2 or pos.shape[0] < axes or pos.shape[1] != rows:
-        raise LmrsError(f"pos must be [{axes}, {rows}], not {list(pos.shape)}")
-    return _Positions(pos.data_ptr(), *pos.stride())
-
-
-def _on(device):
-    return _HERE if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+    raise LmrsError(f"pos must be [{axes}, {rows}], not {list(shape)}")
 
 
 def _stream(device):
     return torch._C._cuda_getCurrentRawStream(device.index)   # torch.cuda.current_stream(device).cuda_stream without the objects (2 us of a call's 10)
-
-
-_HERE = contextlib.nullcontext()
 
 
 class RopeAxes:
@@ -182,6 +175,7 @@ class Batch:
         self._c = _Batch(lens.data_ptr(), 0 if rows is None else rows.data_ptr(), tables.data_ptr(), 0 if not self.prefix_len else prefix.data_ptr(), tables.stride(0), self.seqs,
                          tables.shape[1], self.max_rows, self.prefix_len)
         self._ref = C.byref(self._c)
+        self._bytes = {}   # workspaces' sizes
 
     def _for(self, pages, n_rows):
         if not isinstance(pages, KVPages):
@@ -202,13 +196,15 @@ def rope_axes(x, pos, rope, out=None):
         raise LmrsError("x must be a [rows, heads, head_size] tensor of bfloat16, float16 or float32")
     n, heads, size = x.shape
     device, dtype = x.device, x.dtype
+    if x.is_cuda and device.index != torch.cuda.current_device():
+        with torch.cuda.device(device):
+            return rope_axes(x, pos, rope, out)
     xr = _heads(x, "x", device, dtype, n, heads, size)
     p = _positions(pos, rope.axes, n, device)
-    with _on(device):
-        if out is None:
-            out = torch.empty_like(x)
-        o = _heads(out, "out", device, dtype, n, heads, size, out=True)
-        check(lib().lmrs_b200_rope_axes(rope._ref, _DTYPES[dtype], C.byref(xr), C.byref(o), n, heads, size, C.byref(p), _stream(device)))
+    if out is None:
+        out = torch.empty_like(x)
+    o = _heads(out, "out", device, dtype, n, heads, size, out=True)
+    check(lib().lmrs_b200_rope_axes(rope._ref, _DTYPES[dtype], C.byref(xr), C.byref(o), n, heads, size, C.byref(p), _stream(device)))
     return out
 
 
@@ -222,6 +218,9 @@ def append(pages, batch, k, v, rope=None, pos=None, q=None, q_out=None):
     n = k.shape[0]
     batch._for(pages, n)
     device, dtype, size = pages.device, pages.dtype, pages.head_size
+    if device.index != torch.cuda.current_device():
+        with torch.cuda.device(device):
+            return append(pages, batch, k, v, rope, pos, q, q_out)
     kr = _heads(k, "k", device, dtype, n, pages.kv_heads, size)
     vr = _heads(v, "v", device, dtype, n, pages.kv_heads, size)
     if rope is None:
@@ -230,20 +229,19 @@ def append(pages, batch, k, v, rope=None, pos=None, q=None, q_out=None):
     elif not isinstance(rope, RopeAxes):
         raise LmrsError("rope must be RopeAxes")
     p = None if pos is None else C.byref(_positions(pos, rope.axes, n, device))
-    with _on(device):
-        qr = qo = None
-        heads = 0
-        if q is not None:
-            if not isinstance(q, torch.Tensor) or q.dim() != 3:
-                raise LmrsError("q must be a [rows, heads, head_size] tensor")
-            heads = q.shape[1]
-            qr = C.byref(_heads(q, "q", device, dtype, n, heads, size))
-            if q_out is None:
-                q_out = torch.empty_like(q)
-            qo = C.byref(_heads(q_out, "q_out", device, dtype, n, heads, size, out=True))
-        elif q_out is not None:
-            raise LmrsError("q_out without q")
-        check(lib().lmrs_b200_paged_append(pages._ref, batch._ref, n, C.byref(kr), C.byref(vr), None if rope is None else rope._ref, p, qr, qo, heads, _stream(device)))
+    qr = qo = None
+    heads = 0
+    if q is not None:
+        if not isinstance(q, torch.Tensor) or q.dim() != 3:
+            raise LmrsError("q must be a [rows, heads, head_size] tensor")
+        heads = q.shape[1]
+        qr = C.byref(_heads(q, "q", device, dtype, n, heads, size))
+        if q_out is None:
+            q_out = torch.empty_like(q)
+        qo = C.byref(_heads(q_out, "q_out", device, dtype, n, heads, size, out=True))
+    elif q_out is not None:
+        raise LmrsError("q_out without q")
+    check(lib().lmrs_b200_paged_append(pages._ref, batch._ref, n, C.byref(kr), C.byref(vr), None if rope is None else rope._ref, p, qr, qo, heads, _stream(device)))
     return q_out
 
 
@@ -258,16 +256,24 @@ def attention(pages, batch, q, out=None, scale=None, softcap=0.0, return_lse=Fal
     n, heads, size = q.shape
     batch._for(pages, n)
     device, dtype = pages.device, pages.dtype
+    if device.index != torch.cuda.current_device():
+        with torch.cuda.device(device):
+            return attention(pages, batch, q, out, scale, softcap, return_lse)
     qr = _heads(q, "q", device, dtype, n, heads, pages.head_size)
-    with _on(device):
-        if out is None:
-            out = torch.empty_like(q)
-        o = _heads(out, "out", device, dtype, n, heads, size, out=True)
-        lse = torch.empty((n, heads), dtype=torch.float32, device=device) if return_lse else None
-        L, need = lib(), C.c_size_t()
-        check(L.lmrs_b200_paged_attention_workspace(pages._ref, batch._ref, n, heads, C.byref(need)))
-        bytes = need.value
-        work = torch.empty(bytes, dtype=torch.uint8, device=device) if bytes else None
-        check(L.lmrs_b200_paged_attention(pages._ref, batch._ref, n, C.byref(qr), C.byref(o), heads, size ** -0.5 if scale is None else scale, softcap,
-                                          lse.data_ptr() if return_lse and n and heads else None, work.data_ptr() if bytes else None, bytes, _stream(device)))
+    if out is None:
+        out = torch.empty_like(q)
+    o = _heads(out, "out", device, dtype, n, heads, size, out=True)
+    lse = torch.empty(n, heads, dtype=torch.float32, device=device) if return_lse else None
+    L = lib()
+    key = (n, heads, pages.kv_heads, size, pages.page_size, dtype)
+    need = batch._bytes.get(key)
+    if need is None:   # (it goes by the numbers of the call alone)
+        got = C.c_size_t()
+        check(L.lmrs_b200_paged_attention_workspace(pages._ref, batch._ref, n, heads, C.byref(got)))
+        if len(batch._bytes) > 64:
+            batch._bytes.clear()
+        need = batch._bytes[key] = got.value
+    work = torch.empty(need, dtype=torch.uint8, device=device) if need else None
+    check(L.lmrs_b200_paged_attention(pages._ref, batch._ref, n, C.byref(qr), C.byref(o), heads, size ** -0.5 if scale is None else scale, softcap,
+                                      lse.data_ptr() if return_lse and n and heads else None, work.data_ptr() if need else None, need, _stream(device)))
     return (out, lse) if return_lse else out
