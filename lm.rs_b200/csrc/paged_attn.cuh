@@ -470,12 +470,12 @@ template <typename T, int DP> struct WarpTile {
             if ((lane & 3) == 0) ml[lane / 4 + 8 * i] = make_float2(m[i], seen[i] ? l[i] : -1.0f);
         }
     }
-    PG_DEVINL void put_o(float* to, const float* factor) {   // [16][DP] as sum_at has them, times the rows' factors
+    PG_DEVINL void put_o(float* to, float factor) {   // [16][DP] as sum_at has them, times the rows' factors (lane r has row r's)
         const int lane = threadIdx.x & 31;
 #pragma unroll
         for (int i = 0; i < 2; i++) {
             const int r = lane / 4 + 8 * i;
-            const float f = factor[r];
+            const float f = __shfl_sync(~0u, factor, r);
 #pragma unroll
             for (int n = 0; n < DP / 8; n++) *reinterpret_cast<float2*>(to + sum_at<DP>(r, 8 * n + 2 * (lane & 3))) = make_float2(o[n][2 * i] * f, o[n][2 * i + 1] * f);
         }
@@ -601,11 +601,11 @@ template <int DP> struct WarpTile<float, DP> {
             if (lane % KEYS == 0) ml[i * TEAMS + team] = make_float2(m[i], any >> (KEYS * team) & (KEYS == 16 ? 0xffffu : 0xffu) ? l[i] : -1.0f);
         }
     }
-    PG_DEVINL void put_o(float* to, const float* factor) {
+    PG_DEVINL void put_o(float* to, float factor) {
         const int lane = threadIdx.x & 31;
 #pragma unroll
         for (int r = 0; r < 16; r++) {
-            const float f = factor[r];
+            const float f = __shfl_sync(~0u, factor, r);
             if constexpr (COLS == 2) {
                 *reinterpret_cast<float2*>(to + sum_at<DP>(r, 2 * lane)) = make_float2(o[r][0] * f, o[r][1] * f);
             } else {
@@ -625,7 +625,8 @@ __global__ void __launch_bounds__(TileShape<T, DP>::THREADS, TileShape<T, DP>::C
     __shared__ int row_keys[S::STAGES][S::ROWS];
     __shared__ __align__(8) uint8_t there[S::STAGES][S::KEYS / 8];
     __shared__ float2 ml[4][S::ROWS];
-    __shared__ __align__(16) float factor[4][S::ROWS], weights[sizeof(T) == 4 ? 4 : 1][sizeof(T) == 4 ? (S::WARP_KEYS + 1) * 16 : 1];
+    __shared__ float2 joined[S::ROWS];
+    __shared__ __align__(16) float weights[sizeof(T) == 4 ? 4 : 1][sizeof(T) == 4 ? (S::WARP_KEYS + 1) * 16 : 1];
     __shared__ unsigned again;
     __shared__ AgainScratch scratch;
     const int t = threadIdx.x, lane = t & 31, warp = t >> 5, D = p.head_size;
@@ -732,32 +733,37 @@ __global__ void __launch_bounds__(TileShape<T, DP>::THREADS, TileShape<T, DP>::C
         tile.tile(p, queries + set * S::Q, k_at, v_at, bits, w.tile * S::KEYS + warp * S::WARP_KEYS, row_keys[set], used, weights[sizeof(T) == 4 ? warp : 0]);
         const bool last = w.tile + 1 == w.tiles;
         if (last || at + 1 == n_tiles) {   // the part ends: the warps' rows meet in the tile's place
+            const bool mixed = w.b >= 0 && w.s.count > 1;   // (rows that see different keys)
             tile.put_ml(ml[warp]);
             if (t == 0) again = 0;
             __syncthreads();
-            if (t < S::ROWS) {
-                float m = -INFINITY, sum = 0.0f;
+            {   // lane r: row r's largest score, what this warp's sums are multiplied by, the sum of the weights
+                float m = -INFINITY, sum = 0.0f, mine = 0.0f;
                 bool any = false;
+                const int r = lane & 15;
+#pragma unroll
                 for (int i = 0; i < 4; i++)
-                    if (ml[i][t].y >= 0.0f || ml[i][t].y != ml[i][t].y) { m = fmaxf(m, ml[i][t].x); any = true; }
+                    if (!(ml[i][r].y < 0.0f)) { m = fmaxf(m, ml[i][r].x); any = true; }
                 const float base = m == -INFINITY ? 0.0f : m;
+#pragma unroll
                 for (int i = 0; i < 4; i++) {
-                    const bool has = !(ml[i][t].y < 0.0f);
-                    factor[i][t] = has ? ex2(ml[i][t].x - base) : 0.0f;
-                    if (has) sum += ml[i][t].y * factor[i][t];
+                    const bool has = !(ml[i][r].y < 0.0f);
+                    const float f = has ? ex2(ml[i][r].x - base) : 0.0f;
+                    if (has) sum += ml[i][r].y * f;
+                    if (i == warp) mine = f;
                 }
-                ml[0][t] = make_float2(m, any ? sum : -1.0f);
+                if (t < S::ROWS) joined[t] = make_float2(m, any ? sum : -1.0f);
+                __syncwarp();
+                tile.put_o(reinterpret_cast<float*>(smem + stage * 2 * S::KV) + warp * S::ROWS * DP, mine);
             }
             __syncthreads();
             float* rows = reinterpret_cast<float*>(smem + stage * 2 * S::KV);
-            tile.put_o(rows + warp * S::ROWS * DP, factor[warp]);
-            __syncthreads();
             const bool whole = whole_unit(p, w, begun, w.tile);
             const int64_t slot = w.unit + blockIdx.x;
             const int quads = D / 4;
             for (int e = t; e < used * quads; e += S::THREADS) {
                 const int x = e / quads, c = 4 * (e - x * quads);
-                const float2 s = ml[0][x];
+                const float2 s = joined[x];
                 float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
                 if (!(s.y < 0.0f)) {
 #pragma unroll
@@ -766,7 +772,7 @@ __global__ void __launch_bounds__(TileShape<T, DP>::THREADS, TileShape<T, DP>::C
                         v.x += a.x; v.y += a.y; v.z += a.z; v.w += a.w;
                     }
                 }
-                if (!isfinite(v.x + v.y + v.z + v.w) && w.b >= 0 && w.s.count > 1) atomicOr(&again, 1u << x);
+                if (mixed && !isfinite(v.x + v.y + v.z + v.w)) atomicOr(&again, 1u << x);
                 if (whole) {
                     const UnitRow r = unit_row(p, l, w, x);
                     if (!(s.y < 0.0f)) { v.x /= s.y; v.y /= s.y; v.z /= s.y; v.w /= s.y; }
@@ -777,11 +783,11 @@ __global__ void __launch_bounds__(TileShape<T, DP>::THREADS, TileShape<T, DP>::C
                     if (c == 0) l.ml[slot * S::ROWS + x] = s;
                 }
             }
-            __syncthreads();
-            for (unsigned left = again; left; left &= left - 1) {   // (the same for all threads)
+            if (mixed) __syncthreads();
+            for (unsigned left = mixed ? again : 0; left; left &= left - 1) {   // (the same for all threads)
                 const int x = __ffs(left) - 1;
                 const UnitRow r = unit_row(p, l, w, x);
-                if (ml[0][x].y < 0.0f) continue;
+                if (joined[x].y < 0.0f) continue;
                 float m, sum, acc[2];
                 row_again(p, w, r, begun * S::KEYS, (w.tile + 1) * S::KEYS, scratch, 0, m, sum, acc);
 #pragma unroll
