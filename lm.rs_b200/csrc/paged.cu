@@ -295,6 +295,38 @@ template <typename K> cudaError_t allow_smem(K kernel, int device, int bytes, st
     if (e == cudaSuccess && device < 64) done.fetch_or(bit, std::memory_order_release);
     return e;
 }
+// Tensor maps of the pages for tiles of TensorShape X, if there are any (boxes.rows stays 0 otherwise): rows of a box are the most that divide a page and a copying warp's share
+template <typename X> void box_maps(const lmrs_b200_pages_t* pages, Boxes& boxes) {
+    typedef CUresult (*Encode)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
+                               CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+    static const Encode encode = [] {
+        void* f = nullptr;
+        cudaDriverEntryPointQueryResult q;
+        return cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &f, cudaEnableDefault, &q) == cudaSuccess && q == cudaDriverEntryPointSuccess ? (Encode)f : nullptr;
+    }();
+    int rows = X::KEYS / X::COPIERS;
+    while (rows >= 8 && pages->page_size % rows) rows /= 2;
+    if (!encode || rows < 8) return;
+    auto map = [&](CUtensorMap* m, void* base, int64_t page, int64_t slot, int64_t head, int& place_at, int& head_at) {
+        struct { int64_t stride; cuuint64_t n; cuuint32_t box; int what; } d[3] = {{slot, (cuuint64_t)pages->page_size, (cuuint32_t)rows, 0}, {head, (cuuint64_t)pages->kv_heads, 1, 1},
+                                                                              {page, (cuuint64_t)pages->pages, 1, 2}};
+        std::sort(d, d + 3, [](const auto& a, const auto& b) { return a.stride < b.stride; });
+        const size_t size = size_of(pages->dtype);
+        const cuuint64_t dims[4] = {pages->head_size * size, d[0].n, d[1].n, d[2].n};
+        const cuuint64_t strides[3] = {d[0].stride * size, d[1].stride * size, d[2].stride * size};
+        const cuuint32_t box[4] = {128, d[0].box, d[1].box, d[2].box}, step[4] = {1, 1, 1, 1};
+        for (int i = 0; i < 3; i++) {
+            if (d[i].what == 0) place_at = i;
+            if (d[i].what == 1) head_at = i;
+            if (strides[i] == 0 || strides[i] % 16 || strides[i] >= (1ull << 40)) return false;
+        }
+        return encode(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 4, base, dims, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                      CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+    };
+    if (map(&boxes.k, pages->k, pages->k_page, pages->k_slot, pages->k_head, boxes.k_place, boxes.k_head) &&
+        map(&boxes.v, pages->v, pages->v_page, pages->v_slot, pages->v_head, boxes.v_place, boxes.v_head))
+        boxes.rows = rows;
+}
 // a kernel that may be set up while the one before it still runs, and waits for its results by itself
 template <typename K, typename... P> cudaError_t launch_after(K kernel, unsigned grid, unsigned threads, size_t smem, cudaStream_t stream, const P&... p) {
     cudaLaunchConfig_t c = {};
@@ -373,7 +405,9 @@ extern "C" int lmrs_b200_paged_attention(const lmrs_b200_pages_t* pages, const l
                     auto kernel = rows128_kernel<T, decltype(d)::value>;
                     using X = TensorShape<T, decltype(d)::value>;
                     if ((e = allow_smem(kernel, device, X::SMEM, allowed_tensor)) != cudaSuccess) return refuse(me, cudaGetErrorString(e));
-                    kernel<<<(unsigned)c.front.ctas, X::THREADS, X::SMEM, (cudaStream_t)stream>>>(p, c.front);
+                    Boxes boxes = {};
+                    box_maps<X>(pages, boxes);
+                    kernel<<<(unsigned)c.front.ctas, X::THREADS, X::SMEM, (cudaStream_t)stream>>>(p, c.front, boxes);
                     if (launched(me)) return 1;
                 }
             if (!c.own_tensor) {

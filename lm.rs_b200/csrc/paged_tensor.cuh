@@ -7,8 +7,8 @@
 //     o += weights . V            tcgen05.mma, the weights from TMEM, the values in shared memory as they lie in the pages (keys x columns: MN-major)
 //   warps 0-3, 4-7   the rows.  Two blocks: a group each, steps in turn, so that one's exponentials run under the other's products.  One block: the first group, and the
 //                    scores of the next tile are computed meanwhile.
-//   warps 8-9        copies of keys and values (16 bytes a thread, zeros for what is not there) into a ring of slots, one operand tile each, in the order K0 K1 V0 K2 V1 ...
-//                    The places of a tile's keys are looked up by a thread each; pages of any size and order cost the same.
+//   warps 8-9        copies of keys and values into a ring of slots, one operand tile each, in the order K0 K1 V0 K2 V1 ...  By TMA, a piece of a page at a time; a unit's last tile, and all
+//                    where pages have odd sizes, 16 bytes a thread with zeros for what is not there.  The places of a tile's keys are looked up by a thread each.
 //   warp 10          the products
 // o stays in TMEM for a whole part.  m is the largest score when it was last set; it is set anew, and o rescaled, only when a row's largest score has grown by
 // more than 2^8 (weights stay below 2^8 and sums are f32, so that nothing is lost), which is rare after the first tile.
@@ -109,8 +109,21 @@ template <typename T, int DP> struct TensorShared {
     AgainScratch again[2];
 };
 
+// How the copies of whole tiles go: `rows` keys of a page at a time by TMA (0: never; pages of odd sizes, or strides that no tensor map takes).  The maps' dimensions are a
+// row's bytes and then, by falling nearness in memory, places, heads and pages: which of the three is which
+struct Boxes {
+    CUtensorMap k, v;
+    int rows, k_place, k_head, v_place, v_head;   // dimension (0, 1, 2) of the place and the head; the page has the third
+};
+PG_DEVINL void tma_box(uint32_t to, const CUtensorMap* map, int x, int place, int head, int page, int place_at, int head_at, uint64_t* bar) {
+    const int a = place_at == 0 ? place : head_at == 0 ? head : page, b = place_at == 1 ? place : head_at == 1 ? head : page, c = place_at == 2 ? place : head_at == 2 ? head : page;
+    asm volatile("cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(to), "l"(map), "r"(x), "r"(a), "r"(b), "r"(c),
+                 "r"(smem_at(bar))
+                 : "memory");
+}
+
 template <typename T, int DP>
-__global__ void __launch_bounds__(384, 1) rows128_kernel(const __grid_constant__ AttnParams<T> p, const __grid_constant__ Line l) {
+__global__ void __launch_bounds__(384, 1) rows128_kernel(const __grid_constant__ AttnParams<T> p, const __grid_constant__ Line l, const __grid_constant__ Boxes boxes) {
     using S = TensorShape<T, DP>;
     extern __shared__ uint8_t raw[];
     __shared__ TensorShared<T, DP> sh;
@@ -166,7 +179,7 @@ __global__ void __launch_bounds__(384, 1) rows128_kernel(const __grid_constant__
             constexpr int SHARE = S::KEYS / S::COPIERS, EACH = SHARE / 32;   // rows a warp copies, a lane looks up
             const int mine = warp - 8, t = threadIdx.x - 256, pieces = (D + 15) / 16 * 2, whole = D / 8, c = lane & 7;
             int64_t* starts = sh.starts[mine];
-            uint32_t n = 0, slot = 0, round = 0, reported = 0, report_slot = 0;   // operand tiles asked for, the next one's slot and round of the ring; those reported
+            uint32_t n = 0, slot = 0, round = 0, reported = 0, report_slot = 0;   // operand tiles asked for, the next one's slot and round of the ring; those reported, and the next of these
             int looked = 0, part = 0;
             bool ok = true, asked = false;   // asked: queries are on their way
             auto report = [&](uint32_t upto) {   // (they have landed)
@@ -178,7 +191,12 @@ __global__ void __launch_bounds__(384, 1) rows128_kernel(const __grid_constant__
                     report_slot = report_slot + 1 == S::SLOTS ? 0 : report_slot + 1;
                 }
             };
-            auto operand = [&](const T* base, const int64_t (&start)[EACH]) {   // start: where rows lane, lane + 32 of the warp's begin, in bytes; -1: nowhere
+            auto next_slot = [&]() {
+                n++;
+                if (++slot == S::SLOTS) { slot = 0; round++; }
+            };
+            // an operand tile: lane's rows lane, lane + 32 of the warp's lie at `place`.  boxed: all of the tile's keys are within the unit's
+            auto operand = [&](bool values, const Place (&place)[EACH], bool boxed) {
                 if (!ok) return;
                 if (!looks_free(&sh.empty[slot], (int)round + 1)) {   // (nothing that has landed waits for a slot to come free)
                     copy_wait<0>();
@@ -186,6 +204,41 @@ __global__ void __launch_bounds__(384, 1) rows128_kernel(const __grid_constant__
                     ok = wait_warp(&sh.empty[slot], (int)round + 1, gave_up);
                     if (!ok) return;
                 }
+                if (boxed) {
+                    report(n);   // (tiles by TMA report themselves; none before this one is on its way otherwise)
+                    if (lane == 0) mbar_expect_tx(&sh.full[slot], (uint32_t)(SHARE * 128 * ((D + 63) / 64)));
+                    const uint32_t to = smem_at(ring) + slot * S::SLOT + mine * SHARE * 128;
+                    for (int row = 0; row < SHARE; row += boxes.rows) {
+                        int page = __shfl_sync(~0u, place[0].page, row & 31), at_place = __shfl_sync(~0u, place[0].place, row & 31);
+                        if constexpr (EACH == 2) {
+                            const int page2 = __shfl_sync(~0u, place[1].page, row & 31), place2 = __shfl_sync(~0u, place[1].place, row & 31);
+                            if (row >= 32) { page = page2; at_place = place2; }
+                        }
+                        if (page < 0) { page = p.batch.pages; at_place = 0; }   // (outside the map: zeros)
+                        if (lane == 0)
+                            for (int b = 0; 64 * b < D; b++)
+                                tma_box(to + b * S::KEYS * 128 + row * 128, values ? &boxes.v : &boxes.k, 128 * b, at_place, w.head, page, values ? boxes.v_place : boxes.k_place,
+                                        values ? boxes.v_head : boxes.k_head, &sh.full[slot]);
+                    }
+                    __syncwarp();
+                    next_slot();
+                    reported = n;
+                    report_slot = slot;
+                    if (asked) {   // (the queries' copies are the only ones of the other kind)
+                        copy_wait<0>();
+                        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                        arrive(&sh.queries);
+                        asked = false;
+                    }
+                    return;
+                }
+                const T* base = values ? p.v : p.k;
+                int64_t start[EACH];
+#pragma unroll
+                for (int i = 0; i < EACH; i++)
+                    start[i] = place[i].page < 0 ? -1
+                                                 : (values ? place[i].page * p.v_page + place[i].place * p.v_slot + w.head * p.v_head
+                                                           : place[i].page * p.k_page + place[i].place * p.k_slot + w.head * p.k_head) * (int64_t)sizeof(T);
                 __syncwarp();
 #pragma unroll
                 for (int i = 0; i < EACH; i++) starts[32 * i + lane] = start[i];
@@ -215,10 +268,14 @@ __global__ void __launch_bounds__(384, 1) rows128_kernel(const __grid_constant__
                     }
                 }
                 copy_commit();
-                n++;
-                if (++slot == S::SLOTS) { slot = 0; round++; }
-                copy_wait<2>();
-                if (n > 2) report(n - 2);
+                next_slot();
+                if (boxes.rows) {   // (a unit's last tile)
+                    copy_wait<0>();
+                    report(n);
+                } else {
+                    copy_wait<2>();
+                    if (n > 2) report(n - 2);
+                }
             };
             do {
                 enter();
@@ -252,39 +309,32 @@ __global__ void __launch_bounds__(384, 1) rows128_kernel(const __grid_constant__
                     __syncwarp();
                     asked = true;
                 }
-                int64_t values[EACH], next_values[EACH];   // where the values of tiles j and j + 1 begin
+                Place at[EACH], next[EACH];   // of the keys of tiles j and j + 1
+                auto whole_tile = [&](int j) { return boxes.rows > 0 && (w.tile + j + 1) * S::KEYS <= w.keys; };
                 auto keys = [&](int j) {   // tile j of the part: where its keys and values lie, and which are there; then the keys
                     const int set = looked++ % S::RING;
-                    int64_t start[EACH];
 #pragma unroll
                     for (int i = 0; i < EACH; i++) {
-                        const Place at = unit_place(p, w, (w.tile + j) * S::KEYS + mine * SHARE + 32 * i + lane);
-                        const bool is = at.page >= 0;
-                        values[i] = next_values[i];
-                        next_values[i] = is ? (at.page * p.v_page + at.place * p.v_slot + w.head * p.v_head) * (int64_t)sizeof(T) : -1;
-                        start[i] = is ? (at.page * p.k_page + at.place * p.k_slot + w.head * p.k_head) * (int64_t)sizeof(T) : -1;
-                        const unsigned bits = __ballot_sync(~0u, is);
+                        next[i] = unit_place(p, w, (w.tile + j) * S::KEYS + mine * SHARE + 32 * i + lane);
+                        const unsigned bits = __ballot_sync(~0u, next[i].page >= 0);
                         if (lane == 0) sh.there[set][mine * EACH + i] = bits;
                     }
                     if (lane == 0 && ok) arrive(&sh.known[set]);
-                    operand(p.k, start);
+                    operand(false, next, whole_tile(j));
                 };
-#pragma unroll
-                for (int i = 0; i < EACH; i++) next_values[i] = -1;
                 keys(0);
                 for (int j = 0; j < tiles; j++) {
-                    if (j + 1 < tiles) {
-                        keys(j + 1);
-                    } else {
 #pragma unroll
-                        for (int i = 0; i < EACH; i++) values[i] = next_values[i];
-                    }
-                    operand(p.v, values);
+                    for (int i = 0; i < EACH; i++) at[i] = next[i];
+                    if (j + 1 < tiles) keys(j + 1);
+                    operand(true, at, whole_tile(j));
                 }
                 copy_wait<0>();   // (the next part waits for the queries' last reader, which needs all of this one)
                 report(n);
                 part++;
             } while (leave());
+            if (!ok)   // gave up: what TMA was asked for lands before shared memory goes away
+                for (uint32_t i = n > S::SLOTS ? n - S::SLOTS : 0; i < n; i++) dense::mbar_wait_for(&sh.full[i % S::SLOTS], (i / S::SLOTS) & 1, nullptr);
         } else if (warp == PRODUCTS) {
             // ---- products ----
             const uint32_t one = dense::elect_one(), type = sizeof(T) == 2 && std::is_same<T, __nv_bfloat16>::value ? 1u : 0u;
