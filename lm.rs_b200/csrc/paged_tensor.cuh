@@ -2,11 +2,10 @@
 // tensor cores.  16-bit types; the line, its units and the parts are those of paged_attn.cuh, with 128 or 256 rows a unit.
 //
 // CTA = 12 warps of 168 registers, one CTA an SM.  The rows of a unit are one or two blocks of 128, a TMEM lane each; a step of the work is one block against one tile of keys:
-//     scores = Q . K^T            tcgen05.mma, both operands in shared memory, 128 x KEYS sums in TMEM (two sets, taken in turn)
+//     scores = Q . K^T            tcgen05.mma, both operands in shared memory, 128 x 64 sums in TMEM (two sets for each block, taken in turn)
 //     weights = 2^(scores - m)    a thread a row: the scores from TMEM, the weights rounded to the type and back to TMEM over the scores
 //     o += weights . V            tcgen05.mma, the weights from TMEM, the values in shared memory as they lie in the pages (keys x columns: MN-major)
-//   warps 0-3, 4-7   the rows.  Two blocks: a group each, steps in turn, so that one's exponentials run under the other's products.  One block: the first group, and the
-//                    scores of the next tile are computed meanwhile.
+//   warps 0-3, 4-7   the rows of the first and the second block.  The scores of the next tile are computed under the exponentials of this one.
 //   warps 8-9        copies of keys and values into a ring of slots, one operand tile each, in the order K0 K1 V0 K2 V1 ...  By TMA, a piece of a page at a time; a unit's last tile, and all
 //                    where pages have odd sizes, 16 bytes a thread with zeros for what is not there.  The places of a tile's keys are looked up by a thread each.
 //   warp 10          the products
@@ -21,13 +20,13 @@ namespace lmrs {
 namespace paged {
 
 template <typename T, int DP> struct TensorShape {
-    static constexpr int THREADS = 384, COPIERS = 2, BLOCK = 128, BLOCKS = DP <= 128 ? 2 : 1, ROWS = BLOCK * BLOCKS, KEYS = DP <= 128 ? 128 : 64;
+    static constexpr int THREADS = 384, COPIERS = 2, BLOCK = 128, BLOCKS = DP <= 128 ? 2 : 1, ROWS = BLOCK * BLOCKS, KEYS = 64;
     static constexpr int BOXES = DP / 64;                                   // 64 columns of an operand: rows of 128 bytes, their 16-byte pieces rotated (SWIZZLE_128B)
-    static constexpr int SLOT = BOXES * KEYS * 128, SLOTS = DP <= 64 ? 6 : 4, Q_BLOCK = BOXES * BLOCK * 128;
+    static constexpr int SLOT = BOXES * KEYS * 128, SLOTS = DP <= 128 ? 8 : 4, Q_BLOCK = BOXES * BLOCK * 128;
     static constexpr int RING = 8;                                          // tiles whose keys' places are known
-    static constexpr int O_AT = DP <= 128 ? 256 : 256, S_WIDTH = 128;       // TMEM columns: two sets of scores, then o of each block
+    static constexpr int O_AT = 256;                                        // TMEM columns: two sets of scores for each block, then o of each block
     static constexpr int SMEM = 1024 + SLOTS * SLOT + BLOCKS * Q_BLOCK;
-    static_assert(O_AT + BLOCKS * DP <= 512 && 2 * S_WIDTH <= O_AT, "TMEM");
+    static_assert(O_AT + BLOCKS * DP <= 512 && 2 * 2 * KEYS <= O_AT, "TMEM");
 };
 constexpr float RESCALE_AT = 8.0f;
 constexpr int PAGED_WAIT = 5 << 8;   // (what a wait was for is not reported: any number that is not 0)
@@ -80,6 +79,27 @@ PG_DEVINL void tmem_load64(uint32_t at, uint32_t (&v)[64]) {
         : "r"(at), "r"(at + 32)
         : "memory");
 }
+PG_DEVINL void tmem_load16(uint32_t at, uint32_t (&v)[16]) {
+    __syncwarp();
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];\n\t"
+        "tcgen05.wait::ld.sync.aligned;"
+        : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]), "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]),
+          "=r"(v[14]), "=r"(v[15])
+        : "r"(at)
+        : "memory");
+}
+PG_DEVINL void tmem_store8(uint32_t at, const uint32_t (&v)[8]) {
+    __syncwarp();
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%8], {%0, %1, %2, %3, %4, %5, %6, %7};" ::"r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]),
+                 "r"(v[7]), "r"(at)
+                 : "memory");
+}
+// two floats in one register pair
+PG_DEVINL uint64_t pair_of(uint32_t a, uint32_t b) { uint64_t r; asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "r"(a), "r"(b)); return r; }
+PG_DEVINL float2 pair_open(uint64_t v) { float2 r; asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v)); return r; }
+PG_DEVINL uint64_t fma_pair(uint64_t a, uint64_t b, uint64_t c) { uint64_t r; asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c)); return r; }
+PG_DEVINL uint64_t add_pair(uint64_t a, uint64_t b) { uint64_t r; asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b)); return r; }
 PG_DEVINL void tmem_store32(uint32_t at, const uint32_t (&v)[32]) {
     __syncwarp();
     asm volatile(
@@ -97,7 +117,7 @@ template <typename T, int DP> struct TensorShared {
     using S = TensorShape<T, DP>;
     uint64_t full[S::SLOTS], empty[S::SLOTS];   // slots
     uint64_t known[S::RING];                    // which of a tile's keys are there is written
-    uint64_t scores[2], weights[2];             // sets of scores: written by the products, replaced by weights
+    uint64_t scores[4], weights[4];             // sets of scores (two for each block): written by the products, replaced by weights
     uint64_t summed[2], read[2];                // o of a block: the last product has ended; the part's o has been read
     uint64_t queries;                           // the part's queries are there
     uint64_t queries_read;                      // the last product that reads the part's queries has ended
@@ -136,7 +156,8 @@ __global__ void __launch_bounds__(384, 1) rows128_kernel(const __grid_constant__
     if (threadIdx.x == 0) {
         for (int i = 0; i < S::SLOTS; i++) { mbar_init(&sh.full[i], S::COPIERS); mbar_init(&sh.empty[i], 1); }
         for (int i = 0; i < S::RING; i++) mbar_init(&sh.known[i], S::COPIERS);
-        for (int i = 0; i < 2; i++) { mbar_init(&sh.scores[i], 1); mbar_init(&sh.weights[i], 128); mbar_init(&sh.summed[i], 1); mbar_init(&sh.read[i], 128); }
+        for (int i = 0; i < 4; i++) { mbar_init(&sh.scores[i], 1); mbar_init(&sh.weights[i], 128); }
+        for (int i = 0; i < 2; i++) { mbar_init(&sh.summed[i], 1); mbar_init(&sh.read[i], 128); }
         mbar_init(&sh.queries, 32 * S::COPIERS);
         mbar_init(&sh.queries_read, 1);
         mbar_init(&sh.parted, 256);
@@ -343,7 +364,7 @@ __global__ void __launch_bounds__(384, 1) rows128_kernel(const __grid_constant__
             const uint32_t ring_lo = (uint32_t)dense::tg_desc_sw128(ring), q_lo = (uint32_t)dense::tg_desc_sw128(queries);
             const int steps = (D + 15) / 16;
             uint32_t n = 0, round = 0;           // slot of the next operand tile, rounds of the ring before it
-            int w_count[2] = {0, 0}, part = 0;   // sets of weights taken
+            int w_count[4] = {0, 0, 0, 0}, part = 0;   // sets of weights taken
             bool ok = true;
             auto take = [&]() {
                 ok = ok && wait_warp(&sh.full[n], (int)round, gave_up);
@@ -352,69 +373,53 @@ __global__ void __launch_bounds__(384, 1) rows128_kernel(const __grid_constant__
                 if (++n == S::SLOTS) { n = 0; round++; }
                 return slot;
             };
-            // (unrolled, so that descriptors are sums of constants in uniform registers: as a loop over k an issue took 96 cycles, three times the product)
-            auto scores = [&](int block, int set, uint32_t slot) {
-                const uint32_t d = tmem + (uint32_t)set * S::S_WIDTH, a = q_lo + (uint32_t)block * (S::Q_BLOCK >> 4), b = ring_lo + slot * (S::SLOT >> 4);
+            // (unrolled, so that descriptors are sums of constants in uniform registers)
+            auto scores = [&](int block, int j, uint32_t slot) {
+                const int set = 2 * block + (j & 1);
+                const uint32_t d = tmem + (uint32_t)set * S::KEYS, a = q_lo + (uint32_t)block * (S::Q_BLOCK >> 4), b = ring_lo + slot * (S::SLOT >> 4);
 #pragma unroll
                 for (int k = 0; k < DP / 16; k++)
                     if (k < steps)
                         dense::tg_mma_ss1(one, d, a + (uint32_t)(k >> 2) * (S::BLOCK * 128 >> 4) + (k & 3) * 2, b + (uint32_t)(k >> 2) * (S::KEYS * 128 >> 4) + (k & 3) * 2, score_form, k > 0);
                 dense::tg_commit1(one, &sh.scores[set]);
             };
-            auto sums = [&](int block, int set, int j, uint32_t slot) {
+            auto sums = [&](int block, int j, uint32_t slot) {
+                const int set = 2 * block + (j & 1);
                 if (j == 0 && part > 0) ok = ok && wait_warp(&sh.read[block], part - 1, gave_up);
                 ok = ok && wait_warp(&sh.weights[set], w_count[set]++, gave_up);
                 if (!ok) return;
                 tmem_after();
                 // 16 keys a step: two groups of 8 rows of 128 bytes; from 64 columns to the next: a box
-                const uint32_t d = tmem + S::O_AT + (uint32_t)block * DP, a = tmem + (uint32_t)set * S::S_WIDTH;
+                const uint32_t d = tmem + S::O_AT + (uint32_t)block * DP, a = tmem + (uint32_t)set * S::KEYS;
                 const uint32_t b = (ring_lo & 0xffffu) + slot * (S::SLOT >> 4) + ((uint32_t)(S::KEYS * 128 >> 4) << 16), more = j > 0;
 #pragma unroll
-                for (int k = 0; k < S::KEYS / 16; k++) dense::tg_mma_ts1(one, d, a + (k < 4 ? k * 8 : 64 + (k - 4) * 8), b + k * (2048 >> 4), sum_form, k > 0 ? 1u : more);   // (weights of 64 keys over the first half of their scores)
+                for (int k = 0; k < S::KEYS / 16; k++) dense::tg_mma_ts1(one, d, a + k * 8, b + k * (2048 >> 4), sum_form, k > 0 ? 1u : more);
                 dense::tg_commit1(one, &sh.summed[block]);
             };
-            do {   // operand tiles come as K0 K1 V0 K2 V1 ...
+            do {   // operand tiles come as K0 K1 V0 K2 V1 ...: the scores of tile j + 2 follow the sums of tile j into the same set
                 enter();
                 ok = ok && wait_warp(&sh.queries, part, gave_up);
-                uint32_t slot = take();
-                if (ok) {
-                    scores(0, 0, slot);
-                    if (blocks == 2) scores(1, 1, slot);
-                    dense::tg_commit1(one, &sh.empty[slot]);
-                }
-                uint32_t next = tiles > 1 ? take() : 0;
-                if (ok && blocks == 1 && tiles > 1) {
-                    scores(0, 1, next);
-                    dense::tg_commit1(one, &sh.empty[next]);
-                }
-                if (ok && (tiles == 1 || (blocks == 1 && tiles == 2))) dense::tg_commit1(one, &sh.queries_read);
-                for (int j = 0; j < tiles && ok; j++) {
-                    // one block: sums of tile j, then the scores of tile j + 2 into the same set; two: sums of a block, then its scores of tile j + 1
-                    const uint32_t values = take();
+                for (int j = 0; j < 2 && j < tiles; j++) {
+                    const uint32_t keys = take();
                     if (!ok) break;
-                    if (blocks == 1) {
-                        sums(0, j & 1, j, values);
-                        if (ok) dense::tg_commit1(one, &sh.empty[values]);
+                    for (int g = 0; g < blocks; g++) scores(g, j, keys);
+                    dense::tg_commit1(one, &sh.empty[keys]);
+                }
+                if (ok && tiles <= 2) dense::tg_commit1(one, &sh.queries_read);
+                for (int j = 0; j < tiles && ok; j++) {
+                    const uint32_t values = take();
+                    uint32_t keys = 0;
+                    for (int g = 0; g < blocks && ok; g++) {
+                        sums(g, j, values);
+                        if (ok && g == blocks - 1) dense::tg_commit1(one, &sh.empty[values]);
                         if (j + 2 < tiles) {
-                            next = take();
-                            if (ok) {
-                                scores(0, j & 1, next);
-                                dense::tg_commit1(one, &sh.empty[next]);
-                                if (j + 3 == tiles) dense::tg_commit1(one, &sh.queries_read);
-                            }
+                            if (g == 0) keys = take();
+                            if (ok) scores(g, j + 2, keys);
                         }
-                    } else {
-                        sums(0, 0, j, values);
-                        if (ok && j + 1 < tiles) scores(0, 0, next);
-                        sums(1, 1, j, values);
-                        if (!ok) break;
-                        dense::tg_commit1(one, &sh.empty[values]);
-                        if (j + 1 < tiles) {
-                            scores(1, 1, next);
-                            dense::tg_commit1(one, &sh.empty[next]);
-                            if (j + 2 == tiles) dense::tg_commit1(one, &sh.queries_read);
-                        }
-                        if (j + 2 < tiles) next = take();
+                    }
+                    if (ok && j + 2 < tiles) {
+                        dense::tg_commit1(one, &sh.empty[keys]);
+                        if (j + 3 == tiles) dense::tg_commit1(one, &sh.queries_read);
                     }
                 }
                 part++;
@@ -429,7 +434,7 @@ __global__ void __launch_bounds__(384, 1) rows128_kernel(const __grid_constant__
         // ---- rows ----
         const int group = warp >> 2, row = threadIdx.x & 127;
         const uint32_t lanes = (uint32_t)(warp & 3) << 21;   // this warp's 32 TMEM lanes
-        int s_count[2] = {0, 0}, k_count = 0, o_count = 0, part = 0;   // phases of earlier parts: sets of scores, tiles, sums of o, parts
+        int s_count[2] = {0, 0}, k_count = 0, o_count = 0, part = 0;   // phases of earlier parts: this group's sets of scores, tiles, sums of o, parts
         bool ok = true;
         do {
             enter();
@@ -441,11 +446,11 @@ __global__ void __launch_bounds__(384, 1) rows128_kernel(const __grid_constant__
                 bool seen = false;
                 const int least = w.b < 0 ? w.keys : unit_row(p, l, w, group * S::BLOCK).keys;   // (rows that come later see more)
                 for (int j = 0; j < tiles && ok; j++) {
-                    const int set = blocks == 2 ? group : j & 1, key0 = (w.tile + j) * S::KEYS, known = (k_count + j) % S::RING;
-                    ok = wait_warp(&sh.known[known], (k_count + j) / S::RING, gave_up) && wait_warp(&sh.scores[set], s_count[set] + (blocks == 2 ? j : j >> 1), gave_up);
+                    const int set = 2 * group + (j & 1), key0 = (w.tile + j) * S::KEYS, known = (k_count + j) % S::RING;
+                    ok = wait_warp(&sh.known[known], (k_count + j) / S::RING, gave_up) && wait_warp(&sh.scores[set], s_count[j & 1] + (j >> 1), gave_up);
                     if (!ok) break;
                     tmem_after();
-                    const uint32_t at = tmem + lanes + (uint32_t)set * S::S_WIDTH;
+                    const uint32_t at = tmem + lanes + (uint32_t)set * S::KEYS;
                     bool all = key0 + S::KEYS <= least;
 #pragma unroll
                     for (int c = 0; c < S::KEYS / 32; c++) all = all && sh.there[known][c] == ~0u;
@@ -453,25 +458,29 @@ __global__ void __launch_bounds__(384, 1) rows128_kernel(const __grid_constant__
                         const int limit = r.keys - key0 - 32 * c;
                         return sh.there[known][c] & (limit >= 32 ? ~0u : limit <= 0 ? 0u : (1u << limit) - 1);
                     };
-                    // A score rises with its dot (falls, with a negative factor): the largest dot makes the largest score.  64 scores stay in registers; of 128, the
-                    // first half is read again for its weights (all of them in registers leave no room for anything else)
+                    // A score rises with its dot (falls, with a negative factor): the largest dot makes the largest score.  Tiles that need no mask are straight-line code on 64 scores
+                    // in registers; the others, and capped weights, go 16 at a time, in loops, to keep that code small (with all forms unrolled the rows' warps waited for
+                    // instructions a fifth of their time)
                     uint32_t v[64];
                     float tops[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-                    auto largest = [&](int half) {
-                        tmem_load64(at + 64 * half, v);
-                        if (all && !(p.scale2 < 0.0f)) {
+                    const bool plain = all && p.scale2 > 0.0f;
+                    if (plain) {
+                        tmem_load64(at, v);
 #pragma unroll
-                            for (int i = 0; i < 64; i += 2) tops[i >> 1 & 3] = fmaxf(fmaxf(tops[i >> 1 & 3], __uint_as_float(v[i])), __uint_as_float(v[i + 1]));
-                            return;
+                        for (int i = 0; i < 64; i += 2) tops[i >> 1 & 3] = fmaxf(fmaxf(tops[i >> 1 & 3], __uint_as_float(v[i])), __uint_as_float(v[i + 1]));
+                    } else {
+                        const uint32_t sign = p.scale2 < 0.0f ? 0x80000000u : 0u;
+#pragma unroll 1
+                        for (int c = 0; c < 64; c += 16) {
+                            const uint32_t mask = sees(c >> 5) >> (c & 16);
+                            uint32_t u[16];
+                            tmem_load16(at + c, u);
+                            seen = seen || (mask & 0xffff);
+#pragma unroll
+                            for (int i = 0; i < 16; i++)
+                                if (mask >> i & 1) tops[i & 3] = fmaxf(tops[i & 3], __uint_as_float(u[i] ^ sign));
                         }
-                        const uint32_t sign = p.scale2 < 0.0f ? 0x80000000u : 0u, mask[2] = {sees(2 * half), sees(2 * half + 1)};
-                        seen = seen || mask[0] || mask[1];
-#pragma unroll
-                        for (int i = 0; i < 64; i++)
-                            if (mask[i >> 5] >> (i & 31) & 1) tops[i & 3] = fmaxf(tops[i & 3], __uint_as_float(v[i] ^ sign));
-                    };
-                    largest(0);
-                    if constexpr (S::KEYS == 128) largest(1);
+                    }
                     seen = seen || all;
                     float top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
                     if (top != -INFINITY) top = score2(p, p.scale2 < 0.0f ? -top : top);
@@ -497,44 +506,52 @@ __global__ void __launch_bounds__(384, 1) rows128_kernel(const __grid_constant__
                         m = now;
                     }
                     const float base = m == -INFINITY ? 0.0f : m;
-                    float sums4[4] = {};
-                    auto weigh = [&](int half) {   // the scores in v become weights
-                        if (p.softcap > 0.0f) {
-#pragma unroll
-                            for (int k = 0; k < 64; k += 16) {
-                                float e[16];
-#pragma unroll
-                                for (int i = 0; i < 16; i++) e[i] = __uint_as_float(v[k + i]);
-                                cap_scores(p, e);
-#pragma unroll
-                                for (int i = 0; i < 16; i++) v[k + i] = __float_as_uint(ex2(e[i] - base));
-                            }
-                        } else {
-#pragma unroll
-                            for (int i = 0; i < 64; i++) v[i] = __float_as_uint(ex2(fmaf(__uint_as_float(v[i]), p.scale2, -base)));
-                        }
-                        if (!all) {
-                            const uint32_t mask[2] = {sees(2 * half), sees(2 * half + 1)};
-#pragma unroll
-                            for (int i = 0; i < 64; i++)
-                                if (!(mask[i >> 5] >> (i & 31) & 1)) v[i] = 0;
-                        }
+                    if (plain && !(p.softcap > 0.0f)) {
+                        const uint64_t factor = pair_of(__float_as_uint(p.scale2), __float_as_uint(p.scale2)), less = pair_of(__float_as_uint(-base), __float_as_uint(-base));
+                        uint64_t total[2] = {0, 0};
                         uint32_t a[32];
 #pragma unroll
                         for (int i = 0; i < 32; i++) {
-                            const float2 e = make_float2(__uint_as_float(v[2 * i]), __uint_as_float(v[2 * i + 1]));
-                            sums4[2 * i & 3] += e.x;
-                            sums4[(2 * i + 1) & 3] += e.y;
+                            float2 e = pair_open(fma_pair(pair_of(v[2 * i], v[2 * i + 1]), factor, less));
+                            e.x = ex2(e.x);
+                            e.y = ex2(e.y);
+                            total[i & 1] = add_pair(total[i & 1], pair_of(__float_as_uint(e.x), __float_as_uint(e.y)));
                             a[i] = close_word(e, T());
                         }
-                        tmem_store32(at + 64 * half, a);   // (over scores that have been read)
-                    };
-                    if constexpr (S::KEYS == 128) {
-                        weigh(1);
-                        tmem_load64(at, v);
+                        const float2 t = pair_open(add_pair(total[0], total[1]));
+                        sum += t.x + t.y;
+                        tmem_store32(at, a);   // (over scores that have been read)
+                    } else {
+                        float t0 = 0.0f, t1 = 0.0f;
+#pragma unroll 1
+                        for (int c = 0; c < 64; c += 16) {
+                            const uint32_t mask = sees(c >> 5) >> (c & 16);
+                            uint32_t u[16], a[8];
+                            float e[16];
+                            tmem_load16(at + c, u);
+#pragma unroll
+                            for (int i = 0; i < 16; i++) e[i] = __uint_as_float(u[i]);
+                            if (p.softcap > 0.0f) {
+                                cap_scores(p, e);
+#pragma unroll
+                                for (int i = 0; i < 16; i++) e[i] = ex2(e[i] - base);
+                            } else {
+#pragma unroll
+                                for (int i = 0; i < 16; i++) e[i] = ex2(fmaf(e[i], p.scale2, -base));
+                            }
+#pragma unroll
+                            for (int i = 0; i < 16; i++)
+                                if (!(mask >> i & 1)) e[i] = 0.0f;
+#pragma unroll
+                            for (int i = 0; i < 8; i++) {
+                                t0 += e[2 * i];
+                                t1 += e[2 * i + 1];
+                                a[i] = close_word(make_float2(e[2 * i], e[2 * i + 1]), T());
+                            }
+                            tmem_store8(at + (c >> 1), a);   // (columns c / 2 .. c / 2 + 7, all of them below c + 16: read)
+                        }
+                        sum += t0 + t1;
                     }
-                    weigh(0);
-                    sum += (sums4[0] + sums4[1]) + (sums4[2] + sums4[3]);
                     tmem_stored();
                     tmem_before();
                     arrive(&sh.weights[set]);
@@ -624,12 +641,12 @@ __global__ void __launch_bounds__(384, 1) rows128_kernel(const __grid_constant__
                     }
                 }
                 o_count += tiles;
+                s_count[0] += (tiles + 1) >> 1;
+                s_count[1] += tiles >> 1;
             } else {
                 arrive(&sh.read[1]);   // (a part without a second block: its turn passes)
             }
             k_count += tiles;
-            s_count[0] += blocks == 2 ? tiles : (tiles + 1) >> 1;
-            s_count[1] += blocks == 2 ? tiles : tiles >> 1;
             arrive(&sh.parted);
             ok = ok && wait_warp(&sh.parted, part++, gave_up);
         } while (leave());
