@@ -296,7 +296,7 @@ template <typename K> cudaError_t allow_smem(K kernel, int device, int bytes, st
     return e;
 }
 // Tensor maps of the pages for tiles of TensorShape X, if there are any (boxes.rows stays 0 otherwise): rows of a box are the most that divide a page and a copying warp's share
-template <typename X> void box_maps(const lmrs_b200_pages_t* pages, Boxes& boxes) {
+template <typename X> void box_maps(const lmrs_b200_pages_t* pages, const lmrs_b200_rows_t* q, int64_t n_rows, int q_heads, bool q_wide, Boxes& boxes) {
     typedef CUresult (*Encode)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
                                CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
     static const Encode encode = [] {
@@ -304,14 +304,24 @@ template <typename X> void box_maps(const lmrs_b200_pages_t* pages, Boxes& boxes
         cudaDriverEntryPointQueryResult q;
         return cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &f, cudaEnableDefault, &q) == cudaSuccess && q == cudaDriverEntryPointSuccess ? (Encode)f : nullptr;
     }();
+    if (!encode) return;
+    const size_t size = size_of(pages->dtype);
+    const int group = q_heads / pages->kv_heads;
+    if (q_wide && X::BLOCK % group == 0 && q->row > 0 && q->head > 0) {
+        const cuuint64_t dims[3] = {pages->head_size * size, (cuuint64_t)q_heads, (cuuint64_t)n_rows}, strides[2] = {q->head * size, q->row * size};
+        const cuuint32_t box[3] = {128, (cuuint32_t)group, (cuuint32_t)(X::BLOCK / group)}, step[3] = {1, 1, 1};
+        if (strides[0] < (1ull << 40) && strides[1] < (1ull << 40) &&
+            encode(&boxes.q, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, q->data, dims, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                   CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS)
+            boxes.q_tokens = X::BLOCK / group;
+    }
     int rows = X::KEYS / X::COPIERS;
     while (rows >= 8 && pages->page_size % rows) rows /= 2;
-    if (!encode || rows < 8) return;
+    if (rows < 8) return;
     auto map = [&](CUtensorMap* m, void* base, int64_t page, int64_t slot, int64_t head, int& place_at, int& head_at) {
         struct { int64_t stride; cuuint64_t n; cuuint32_t box; int what; } d[3] = {{slot, (cuuint64_t)pages->page_size, (cuuint32_t)rows, 0}, {head, (cuuint64_t)pages->kv_heads, 1, 1},
                                                                               {page, (cuuint64_t)pages->pages, 1, 2}};
         std::sort(d, d + 3, [](const auto& a, const auto& b) { return a.stride < b.stride; });
-        const size_t size = size_of(pages->dtype);
         const cuuint64_t dims[4] = {pages->head_size * size, d[0].n, d[1].n, d[2].n};
         const cuuint64_t strides[3] = {d[0].stride * size, d[1].stride * size, d[2].stride * size};
         const cuuint32_t box[4] = {128, d[0].box, d[1].box, d[2].box}, step[4] = {1, 1, 1, 1};
@@ -406,7 +416,7 @@ extern "C" int lmrs_b200_paged_attention(const lmrs_b200_pages_t* pages, const l
                     using X = TensorShape<T, decltype(d)::value>;
                     if ((e = allow_smem(kernel, device, X::SMEM, allowed_tensor)) != cudaSuccess) return refuse(me, cudaGetErrorString(e));
                     Boxes boxes = {};
-                    box_maps<X>(pages, boxes);
+                    box_maps<X>(pages, q, n_rows, q_heads, p.q_wide, boxes);
                     kernel<<<(unsigned)c.front.ctas, X::THREADS, X::SMEM, (cudaStream_t)stream>>>(p, c.front, boxes);
                     if (launched(me)) return 1;
                 }

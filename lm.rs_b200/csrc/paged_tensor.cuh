@@ -132,8 +132,9 @@ template <typename T, int DP> struct TensorShared {
 // How the copies of whole tiles go: `rows` keys of a page at a time by TMA (0: never; pages of odd sizes, or strides that no tensor map takes).  The maps' dimensions are a
 // row's bytes and then, by falling nearness in memory, places, heads and pages: which of the three is which
 struct Boxes {
-    CUtensorMap k, v;
+    CUtensorMap k, v, q;
     int rows, k_place, k_head, v_place, v_head;   // dimension (0, 1, 2) of the place and the head; the page has the third
+    int q_tokens;                                 // the same for queries: tokens that make up a block's rows (0: the group of a KV head does not divide them)
 };
 PG_DEVINL void tma_box(uint32_t to, const CUtensorMap* map, int x, int place, int head, int page, int place_at, int head_at, uint64_t* bar) {
     const int a = place_at == 0 ? place : head_at == 0 ? head : page, b = place_at == 1 ? place : head_at == 1 ? head : page, c = place_at == 2 ? place : head_at == 2 ? head : page;
@@ -158,7 +159,7 @@ __global__ void __launch_bounds__(384, 1) rows128_kernel(const __grid_constant__
         for (int i = 0; i < S::RING; i++) mbar_init(&sh.known[i], S::COPIERS);
         for (int i = 0; i < 4; i++) { mbar_init(&sh.scores[i], 1); mbar_init(&sh.weights[i], 128); }
         for (int i = 0; i < 2; i++) { mbar_init(&sh.summed[i], 1); mbar_init(&sh.read[i], 128); }
-        mbar_init(&sh.queries, 32 * S::COPIERS);
+        mbar_init(&sh.queries, boxes.q_tokens ? 1 : 32 * S::COPIERS);
         mbar_init(&sh.queries_read, 1);
         mbar_init(&sh.parted, 256);
         sh.gave_up = 0;
@@ -204,6 +205,7 @@ __global__ void __launch_bounds__(384, 1) rows128_kernel(const __grid_constant__
             int looked = 0, part = 0;
             bool ok = true, asked = false;   // asked: queries are on their way
             auto report = [&](uint32_t upto) {   // (they have landed)
+                if (upto == reported) return;   // (a fence costs a thousand cycles)
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                 if (asked && upto > reported) { arrive(&sh.queries); asked = false; }
                 __syncwarp();
@@ -226,7 +228,7 @@ __global__ void __launch_bounds__(384, 1) rows128_kernel(const __grid_constant__
                     if (!ok) return;
                 }
                 if (boxed) {
-                    report(n);   // (tiles by TMA report themselves; none before this one is on its way otherwise)
+                    // (tiles by TMA report themselves; no other one is on its way)
                     if (lane == 0) mbar_expect_tx(&sh.full[slot], (uint32_t)(SHARE * 128 * ((D + 63) / 64)));
                     const uint32_t to = smem_at(ring) + slot * S::SLOT + mine * SHARE * 128;
                     for (int row = 0; row < SHARE; row += boxes.rows) {
@@ -301,7 +303,19 @@ __global__ void __launch_bounds__(384, 1) rows128_kernel(const __grid_constant__
             do {
                 enter();
                 if (part > 0) ok = ok && wait_warp(&sh.queries_read, part - 1, gave_up);
-                if (ok) {   // the queries: eight threads a row; they are reported with the operand tile that follows
+                if (ok && boxes.q_tokens) {   // the queries: rows are tokens x the heads of a group, which one box holds (rows behind the unit's own are some others', or zeros)
+                    if (mine == 0 && lane == 0) {
+                        const int token = (int)(w.b < 0 ? 0 : w.s.first) + w.row_tile * S::ROWS / p.group;
+                        mbar_expect_tx(&sh.queries, (uint32_t)(blocks * S::BLOCK * 128 * ((D + 63) / 64)));
+                        for (int block = 0; block < blocks; block++)
+                            for (int b = 0; 64 * b < D; b++)
+                                asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(
+                                                 smem_at(queries) + block * S::Q_BLOCK + b * (S::BLOCK * 128)),
+                                             "l"(&boxes.q), "r"(128 * b), "r"(w.head * p.group), "r"(token + block * boxes.q_tokens), "r"(smem_at(&sh.queries))
+                                             : "memory");
+                    }
+                    __syncwarp();
+                } else if (ok) {   // eight threads a row; they are reported with the operand tile that follows
                     constexpr int AT_ONCE = 4 * S::COPIERS;
                     const int x0 = t >> 3, i0 = w.row_tile * S::ROWS + x0, step = AT_ONCE / p.group, more = AT_ONCE - step * p.group;
                     int token = i0 / p.group, g = i0 - token * p.group;
@@ -354,6 +368,7 @@ __global__ void __launch_bounds__(384, 1) rows128_kernel(const __grid_constant__
                 report(n);
                 part++;
             } while (leave());
+            if (!ok && boxes.q_tokens) dense::mbar_wait_for(&sh.queries, (part - 1) & 1, nullptr);
             if (!ok)   // gave up: what TMA was asked for lands before shared memory goes away
                 for (uint32_t i = n > S::SLOTS ? n - S::SLOTS : 0; i < n; i++) dense::mbar_wait_for(&sh.full[i % S::SLOTS], (i / S::SLOTS) & 1, nullptr);
         } else if (warp == PRODUCTS) {
