@@ -64,17 +64,28 @@ def _gpu(t, name, device):
 # (these run in every call: messages are made only where one is raised)
 def _heads(t, name, device, dtype, rows, heads, size, out=False):
     """t as the library takes it, checked: [rows, heads, size]"""
-    _gpu(t, name, device)
+    if not isinstance(t, torch.Tensor) or not t.is_cuda or t.device != device:
+        _gpu(t, name, device)
     if t.dtype != dtype:
         raise LmrsError(f"{name} is {t.dtype}, other arrays of the call {dtype}")
     if t.shape != (rows, heads, size):
         raise LmrsError(f"{name} must be [{rows}, {heads}, {size}], not {list(t.shape)}")
-    stride = t.stride()
-    if stride[2] != 1 and size != 1:
+    row, head, one = t.stride()
+    if one != 1 and size != 1:
         raise LmrsError(f"the elements of a head of {name} must lie next to each other")
     if out and not t.is_contiguous() and not _disjoint(t):
         raise LmrsError(f"elements of {name} share their places")
-    return _Rows(t.data_ptr(), stride[0], stride[1])
+    return _Rows(t.data_ptr(), row, head)
+
+
+def _new(like):
+    """a result for a call, and the same as the library takes it"""
+    t = torch.empty_like(like)
+    row, head, one = t.stride()
+    if one != 1:   # (only where a head has one element)
+        t = torch.empty(like.shape, dtype=like.dtype, device=like.device)
+        row, head, one = t.stride()
+    return t, _Rows(t.data_ptr(), row, head)
 
 
 def _ints(t, name, device):
@@ -93,8 +104,8 @@ def _positions(pos, axes, rows, device):
     raise LmrsError(f"pos must be [{axes}, {rows}], not {list(shape)}")
 
 
-def _stream(device):
-    return torch._C._cuda_getCurrentRawStream(device.index)   # torch.cuda.current_stream(device).cuda_stream without the objects (2 us of a call's 10)
+_stream = torch._C._cuda_getCurrentRawStream   # torch.cuda.current_stream(device).cuda_stream without the objects (2 us of a call's 10)
+_byref = C.byref
 
 
 class RopeAxes:
@@ -202,9 +213,12 @@ def rope_axes(x, pos, rope, out=None):
     xr = _heads(x, "x", device, dtype, n, heads, size)
     p = _positions(pos, rope.axes, n, device)
     if out is None:
-        out = torch.empty_like(x)
-    o = _heads(out, "out", device, dtype, n, heads, size, out=True)
-    check(lib().lmrs_b200_rope_axes(rope._ref, _DTYPES[dtype], C.byref(xr), C.byref(o), n, heads, size, C.byref(p), _stream(device)))
+        out, o = _new(x)
+    else:
+        o = _heads(out, "out", device, dtype, n, heads, size, out=True)
+    rc = lib().lmrs_b200_rope_axes(rope._ref, _DTYPES[dtype], _byref(xr), _byref(o), n, heads, size, _byref(p), _stream(device.index))
+    if rc:
+        check(rc)
     return out
 
 
@@ -228,20 +242,24 @@ def append(pages, batch, k, v, rope=None, pos=None, q=None, q_out=None):
             raise LmrsError("pos and q go with rope")
     elif not isinstance(rope, RopeAxes):
         raise LmrsError("rope must be RopeAxes")
-    p = None if pos is None else C.byref(_positions(pos, rope.axes, n, device))
+    p = None if pos is None else _byref(_positions(pos, rope.axes, n, device))
     qr = qo = None
     heads = 0
     if q is not None:
         if not isinstance(q, torch.Tensor) or q.dim() != 3:
             raise LmrsError("q must be a [rows, heads, head_size] tensor")
         heads = q.shape[1]
-        qr = C.byref(_heads(q, "q", device, dtype, n, heads, size))
+        qr = _byref(_heads(q, "q", device, dtype, n, heads, size))
         if q_out is None:
-            q_out = torch.empty_like(q)
-        qo = C.byref(_heads(q_out, "q_out", device, dtype, n, heads, size, out=True))
+            q_out, qo = _new(q)
+        else:
+            qo = _heads(q_out, "q_out", device, dtype, n, heads, size, out=True)
+        qo = _byref(qo)
     elif q_out is not None:
         raise LmrsError("q_out without q")
-    check(lib().lmrs_b200_paged_append(pages._ref, batch._ref, n, C.byref(kr), C.byref(vr), None if rope is None else rope._ref, p, qr, qo, heads, _stream(device)))
+    rc = lib().lmrs_b200_paged_append(pages._ref, batch._ref, n, _byref(kr), _byref(vr), None if rope is None else rope._ref, p, qr, qo, heads, _stream(device.index))
+    if rc:
+        check(rc)
     return q_out
 
 
@@ -261,8 +279,9 @@ def attention(pages, batch, q, out=None, scale=None, softcap=0.0, return_lse=Fal
             return attention(pages, batch, q, out, scale, softcap, return_lse)
     qr = _heads(q, "q", device, dtype, n, heads, pages.head_size)
     if out is None:
-        out = torch.empty_like(q)
-    o = _heads(out, "out", device, dtype, n, heads, size, out=True)
+        out, o = _new(q)
+    else:
+        o = _heads(out, "out", device, dtype, n, heads, size, out=True)
     lse = torch.empty(n, heads, dtype=torch.float32, device=device) if return_lse else None
     L = lib()
     key = (n, heads, pages.kv_heads, size, pages.page_size, dtype)
@@ -274,6 +293,8 @@ def attention(pages, batch, q, out=None, scale=None, softcap=0.0, return_lse=Fal
             batch._bytes.clear()
         need = batch._bytes[key] = got.value
     work = torch.empty(need, dtype=torch.uint8, device=device) if need else None
-    check(L.lmrs_b200_paged_attention(pages._ref, batch._ref, n, C.byref(qr), C.byref(o), heads, size ** -0.5 if scale is None else scale, softcap,
-                                      lse.data_ptr() if return_lse and n and heads else None, work.data_ptr() if need else None, need, _stream(device)))
+    rc = L.lmrs_b200_paged_attention(pages._ref, batch._ref, n, _byref(qr), _byref(o), heads, size ** -0.5 if scale is None else scale, softcap,
+                                     lse.data_ptr() if return_lse and n and heads else None, work.data_ptr() if need else None, need, _stream(device.index))
+    if rc:
+        check(rc)
     return (out, lse) if return_lse else out
