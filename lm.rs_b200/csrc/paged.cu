@@ -268,6 +268,8 @@ template <typename T, int DP> Cutting cutting(const lmrs_b200_pages_t* pages, co
             if (tensor) { tile_rows = TensorShape<T, DP>::ROWS; tile_keys = TensorShape<T, DP>::KEYS; ctas = SMS; }
         l.tile_rows = tile_rows;
         l.tile_keys = tile_keys;
+        while (1 << l.row_shift < tile_rows) l.row_shift++;
+        while (1 << l.key_shift < tile_keys) l.key_shift++;
         l.ctas = ctas;
         l.seqs = own ? batch->seqs : 0;
         l.front_tiles = front ? (int)(((int64_t)batch->prefix_len + tile_keys - 1) / tile_keys) : 0;

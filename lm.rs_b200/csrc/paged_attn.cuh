@@ -49,7 +49,8 @@ template <typename T> struct AttnParams {
 };
 // What one kernel goes through: units of the prefix (if it takes them), then those of the sequences (if it takes them)
 struct Line {
-    int tile_rows, tile_keys, ctas;
+    int tile_rows, tile_keys, ctas;            // (tile_rows and tile_keys: powers of two)
+    int row_shift, key_shift;                  // their logarithms
     int seqs, front_tiles;                     // 0: not this kernel's; front_tiles: tiles of every unit of the prefix
     int64_t front_units;                       // kv_heads * tiles of rows
     // workspace
@@ -74,19 +75,19 @@ PG_DEVINL int cta_of(int64_t total, int ctas, int64_t tile) {
 
 // rows of a sequence's unit and the keys it goes through
 // (a call's rows times the group stay below 2^31)
-PG_DEVINL int unit_rows(const Span& s, int group, int tile_rows) { return (s.count * group + tile_rows - 1) / tile_rows; }
+PG_DEVINL int unit_rows(const Span& s, int group, const Line& l) { return (s.count * group + l.tile_rows - 1) >> l.row_shift; }
 template <typename T> PG_DEVINL int keys_upto(const AttnParams<T>& p, int64_t index) {   // keys of its own that a row of this index sees
     const int64_t most = (int64_t)p.batch.table_len * p.batch.page_size, n = index + 1;
     return n <= 0 ? 0 : (int)(n < most ? n : most);
 }
 template <typename T> PG_DEVINL int unit_keys(const AttnParams<T>& p, const Line& l, const Span& s, int tile) {
-    const int last = min(s.count * p.group, (tile + 1) * l.tile_rows) - 1;
-    return keys_upto(p, (int64_t)s.len - s.count + last / p.group);
+    const int rows = s.count * p.group, end = (tile + 1) << l.row_shift;
+    return keys_upto(p, rows <= end ? (int64_t)s.len - 1 : (int64_t)s.len - s.count + (end - 1) / p.group);   // (of the last row)
 }
-template <typename T> PG_DEVINL int unit_tiles(const AttnParams<T>& p, const Line& l, const Span& s, int tile) { return (unit_keys(p, l, s, tile) + l.tile_keys - 1) / l.tile_keys; }
+template <typename T> PG_DEVINL int unit_tiles(const AttnParams<T>& p, const Line& l, const Span& s, int tile) { return (unit_keys(p, l, s, tile) + l.tile_keys - 1) >> l.key_shift; }
 template <typename T> PG_DEVINL int64_t seq_tiles(const AttnParams<T>& p, const Line& l, const Span& s) {
     int64_t n = 0;
-    for (int t = unit_rows(s, p.group, l.tile_rows) - 1; t >= 0; t--) n += unit_tiles(p, l, s, t);
+    for (int t = unit_rows(s, p.group, l) - 1; t >= 0; t--) n += unit_tiles(p, l, s, t);
     return n * p.kv_heads;
 }
 
@@ -99,7 +100,7 @@ struct Walk {
 };
 template <typename T> PG_DEVINL void walk_unit(const AttnParams<T>& p, const Line& l, Walk& w) {   // fills in the keys of the unit that b, head and row_tile name
     w.keys = w.b < 0 ? p.batch.prefix_len : unit_keys(p, l, w.s, w.row_tile);
-    w.tiles = (w.keys + l.tile_keys - 1) / l.tile_keys;
+    w.tiles = (w.keys + l.tile_keys - 1) >> l.key_shift;
 }
 // the next unit that has tiles; KV heads lie innermost
 template <typename T> PG_DEVINL void walk_next_unit(const AttnParams<T>& p, const Line& l, Walk& w) {
@@ -108,7 +109,7 @@ template <typename T> PG_DEVINL void walk_next_unit(const AttnParams<T>& p, cons
         if (++w.head == p.kv_heads) {
             w.head = 0;
             w.row_tile++;
-            if (w.b < 0 ? w.unit >= l.front_units : w.row_tile >= unit_rows(w.s, p.group, l.tile_rows)) {
+            if (w.b < 0 ? w.unit >= l.front_units : w.row_tile >= unit_rows(w.s, p.group, l)) {
                 w.row_tile = 0;
                 do {
                     w.b++;
@@ -130,7 +131,7 @@ PG_DEVINL int64_t walk_begin(const AttnParams<T>& p, const Line& l, Walk& w, int
     for (int b = b0; b < b1; b++) {
         const Span s = span_of(p.batch, b);
         tiles += seq_tiles(p, l, s);
-        units += (int64_t)unit_rows(s, p.group, l.tile_rows) * p.kv_heads;
+        units += (int64_t)unit_rows(s, p.group, l) * p.kv_heads;
     }
     int64_t tiles_to = tiles, units_to = units;   // up to and with this thread's
     for (int o = 1; o < 32; o <<= 1) {
@@ -156,7 +157,7 @@ PG_DEVINL int64_t walk_begin(const AttnParams<T>& p, const Line& l, Walk& w, int
             const Span s = span_of(p.batch, b);
             l.plan[b] = Plan{at, u};
             at += seq_tiles(p, l, s);
-            u += (int64_t)unit_rows(s, p.group, l.tile_rows) * p.kv_heads;
+            u += (int64_t)unit_rows(s, p.group, l) * p.kv_heads;
         }
         if (t == 0) l.plan[l.seqs] = Plan{total, 0};
     }
@@ -172,7 +173,7 @@ PG_DEVINL int64_t walk_begin(const AttnParams<T>& p, const Line& l, Walk& w, int
                 break;
             }
             at += n;
-            u += (int64_t)unit_rows(s, p.group, l.tile_rows) * p.kv_heads;
+            u += (int64_t)unit_rows(s, p.group, l) * p.kv_heads;
         }
     }
     __syncthreads();
@@ -189,7 +190,7 @@ PG_DEVINL int64_t walk_begin(const AttnParams<T>& p, const Line& l, Walk& w, int
         int64_t left = from - found[1];
         int n = unit_tiles(p, l, w.s, 0);
         w.row_tile = 0;
-        for (const int rows = unit_rows(w.s, p.group, l.tile_rows); w.row_tile + 1 < rows && left >= (int64_t)n * p.kv_heads; n = unit_tiles(p, l, w.s, ++w.row_tile)) left -= (int64_t)n * p.kv_heads;
+        for (const int rows = unit_rows(w.s, p.group, l); w.row_tile + 1 < rows && left >= (int64_t)n * p.kv_heads; n = unit_tiles(p, l, w.s, ++w.row_tile)) left -= (int64_t)n * p.kv_heads;
         n = max(n, 1);   // (it is; lengths that change under the kernel may make it otherwise)
         w.head = min((int)(left / n), p.kv_heads - 1);
         w.tile = (int)(left - (int64_t)w.head * n);
@@ -833,7 +834,7 @@ __global__ void __launch_bounds__(256, COLS == 1 ? 4 : 3) join_kernel(const __gr
         const int g = head / p.group, gi = head - g * p.group;
         if (out) {
             const Span s = span_of(p.batch, b);
-            const int i = (int)(r - s.first), x = i * p.group + gi, row_tile = x / lo.tile_rows, tiles = unit_tiles(p, lo, s, row_tile);
+            const int i = (int)(r - s.first), x = i * p.group + gi, row_tile = x >> lo.row_shift, tiles = unit_tiles(p, lo, s, row_tile);
             const int64_t index = (int64_t)s.len - s.count + i;
             // the parts of its own unit: those of CTAs c0 .. c1 (none: c1 < c0)
             int64_t before = 0;
@@ -845,7 +846,7 @@ __global__ void __launch_bounds__(256, COLS == 1 ? 4 : 3) join_kernel(const __gr
             // and of the prefix'
             int f0 = 0, f1 = -1;
             const int y = r * p.group + gi;
-            const int64_t f_unit = (int64_t)(y / lf.tile_rows) * p.kv_heads + g;
+            const int64_t f_unit = (int64_t)(y >> lf.row_shift) * p.kv_heads + g;
             if (lf.front_tiles && index >= 0) {
                 const int64_t all = lf.seqs ? lf.plan[lf.seqs].tiles : lf.front_units * lf.front_tiles;
                 f0 = cta_of(all, lf.ctas, f_unit * lf.front_tiles);
@@ -854,7 +855,7 @@ __global__ void __launch_bounds__(256, COLS == 1 ? 4 : 3) join_kernel(const __gr
             out = !p.whole || c0 != c1;   // (else it was finished where it was computed)
             if (out) {
                 // EACH parts at a time: a lane reads the (m, l) of one, then all lanes sum the columns, four parts' loads ahead of their use
-                const int n_front = f1 - f0 + 1, n = n_front + (c1 - c0 + 1), y_row = y % lf.tile_rows, x_row = x % lo.tile_rows;
+                const int n_front = f1 - f0 + 1, n = n_front + (c1 - c0 + 1), y_row = y & (lf.tile_rows - 1), x_row = x & (lo.tile_rows - 1);
                 for (int k0 = EACH * mine; k0 < n; k0 += EACH * WARPS) {
                     const int k = lane < EACH ? k0 + lane : n;
                     const bool front = k < n_front;
