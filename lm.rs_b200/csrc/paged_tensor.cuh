@@ -118,7 +118,9 @@ template <typename T, int DP> struct TensorShared {
     uint64_t full[S::SLOTS], empty[S::SLOTS];   // slots
     uint64_t known[S::RING];                    // which of a tile's keys are there is written
     uint64_t scores[4], weights[4];             // sets of scores (two for each block): written by the products, replaced by weights
-    uint64_t summed[2], read[2];                // o of a block: the last product has ended; the part's o has been read
+    uint64_t summed[4];                         // o of a block: the products of a tile have ended, even tiles and odd ones (rows may be two tiles ahead of the products, and a phase
+                                                // is told from the one before it only)
+    uint64_t read[2];                           // the part's o of a block has been read
     uint64_t queries;                           // the part's queries are there
     uint64_t queries_read;                      // the last product that reads the part's queries has ended
     uint64_t parted;                            // both groups have ended the part (neither runs ahead: phases are told apart by their parity alone)
@@ -157,8 +159,8 @@ __global__ void __launch_bounds__(384, 1) rows128_kernel(const __grid_constant__
     if (threadIdx.x == 0) {
         for (int i = 0; i < S::SLOTS; i++) { mbar_init(&sh.full[i], S::COPIERS); mbar_init(&sh.empty[i], 1); }
         for (int i = 0; i < S::RING; i++) mbar_init(&sh.known[i], S::COPIERS);
-        for (int i = 0; i < 4; i++) { mbar_init(&sh.scores[i], 1); mbar_init(&sh.weights[i], 128); }
-        for (int i = 0; i < 2; i++) { mbar_init(&sh.summed[i], 1); mbar_init(&sh.read[i], 128); }
+        for (int i = 0; i < 4; i++) { mbar_init(&sh.scores[i], 1); mbar_init(&sh.weights[i], 128); mbar_init(&sh.summed[i], 1); }
+        for (int i = 0; i < 2; i++) mbar_init(&sh.read[i], 128);
         mbar_init(&sh.queries, boxes.q_tokens ? 1 : 32 * S::COPIERS);
         mbar_init(&sh.queries_read, 1);
         mbar_init(&sh.parted, 256);
@@ -201,6 +203,10 @@ __global__ void __launch_bounds__(384, 1) rows128_kernel(const __grid_constant__
             constexpr int SHARE = S::KEYS / S::COPIERS, EACH = SHARE / 32;   // rows a warp copies, a lane looks up
             const int mine = warp - 8, t = threadIdx.x - 256, pieces = (D + 15) / 16 * 2, whole = D / 8, c = lane & 7;
             int64_t* starts = sh.starts[mine];
+            // a box a lane: piece of a page x 64 columns (one lane for all of them, with the places passed to it: 189 us instead of 176 for 128 sequences behind 32768 tokens)
+            static_assert(EACH == 1, "a lane has the place of its row");
+            const int wide = (D + 63) / 64, box_row = boxes.rows ? lane / wide * boxes.rows : SHARE, box_col = lane % wide;
+            const uint32_t box_to = smem_at(ring) + mine * SHARE * 128 + box_col * S::KEYS * 128 + box_row * 128;
             uint32_t n = 0, slot = 0, round = 0, reported = 0, report_slot = 0;   // operand tiles asked for, the next one's slot and round of the ring; those reported, and the next of these
             int looked = 0, part = 0;
             bool ok = true, asked = false;   // asked: queries are on their way
@@ -230,19 +236,11 @@ __global__ void __launch_bounds__(384, 1) rows128_kernel(const __grid_constant__
                 if (boxed) {
                     // (tiles by TMA report themselves; no other one is on its way)
                     if (lane == 0) mbar_expect_tx(&sh.full[slot], (uint32_t)(SHARE * 128 * ((D + 63) / 64)));
-                    const uint32_t to = smem_at(ring) + slot * S::SLOT + mine * SHARE * 128;
-                    for (int row = 0; row < SHARE; row += boxes.rows) {
-                        int page = __shfl_sync(~0u, place[0].page, row & 31), at_place = __shfl_sync(~0u, place[0].place, row & 31);
-                        if constexpr (EACH == 2) {
-                            const int page2 = __shfl_sync(~0u, place[1].page, row & 31), place2 = __shfl_sync(~0u, place[1].place, row & 31);
-                            if (row >= 32) { page = page2; at_place = place2; }
-                        }
-                        if (page < 0) { page = p.batch.pages; at_place = 0; }   // (outside the map: zeros)
-                        if (lane == 0)
-                            for (int b = 0; 64 * b < D; b++)
-                                tma_box(to + b * S::KEYS * 128 + row * 128, values ? &boxes.v : &boxes.k, 128 * b, at_place, w.head, page, values ? boxes.v_place : boxes.k_place,
-                                        values ? boxes.v_head : boxes.k_head, &sh.full[slot]);
-                    }
+                    int page = __shfl_sync(~0u, place[0].page, box_row & 31), at_place = __shfl_sync(~0u, place[0].place, box_row & 31);
+                    if (page < 0) { page = p.batch.pages; at_place = 0; }   // (outside the map: zeros)
+                    if (box_row < SHARE)
+                        tma_box(box_to + slot * S::SLOT, values ? &boxes.v : &boxes.k, 128 * box_col, at_place, w.head, page, values ? boxes.v_place : boxes.k_place,
+                                values ? boxes.v_head : boxes.k_head, &sh.full[slot]);
                     __syncwarp();
                     next_slot();
                     reported = n;
@@ -409,7 +407,7 @@ __global__ void __launch_bounds__(384, 1) rows128_kernel(const __grid_constant__
                 const uint32_t b = (ring_lo & 0xffffu) + slot * (S::SLOT >> 4) + ((uint32_t)(S::KEYS * 128 >> 4) << 16), more = j > 0;
 #pragma unroll
                 for (int k = 0; k < S::KEYS / 16; k++) dense::tg_mma_ts1(one, d, a + k * 8, b + k * (2048 >> 4), sum_form, k > 0 ? 1u : more);
-                dense::tg_commit1(one, &sh.summed[block]);
+                dense::tg_commit1(one, &sh.summed[set]);
             };
             do {   // operand tiles come as K0 K1 V0 K2 V1 ...: the scores of tile j + 2 follow the sums of tile j into the same set
                 enter();
@@ -449,7 +447,7 @@ __global__ void __launch_bounds__(384, 1) rows128_kernel(const __grid_constant__
         // ---- rows ----
         const int group = warp >> 2, row = threadIdx.x & 127;
         const uint32_t lanes = (uint32_t)(warp & 3) << 21;   // this warp's 32 TMEM lanes
-        int s_count[2] = {0, 0}, k_count = 0, o_count = 0, part = 0;   // phases of earlier parts: this group's sets of scores, tiles, sums of o, parts
+        int s_count[2] = {0, 0}, k_count = 0, part = 0;   // phases of earlier parts: this group's even and odd tiles, all tiles, parts
         bool ok = true;
         do {
             enter();
@@ -503,7 +501,7 @@ __global__ void __launch_bounds__(384, 1) rows128_kernel(const __grid_constant__
                     if (__any_sync(~0u, top > m + RESCALE_AT || (m == -INFINITY && top > m))) {
                         const float now = fmaxf(m, top), corr = ex2(m - (now == -INFINITY ? 0.0f : now));
                         if (j > 0) {
-                            ok = wait_warp(&sh.summed[group], o_count + j - 1, gave_up);
+                            ok = wait_warp(&sh.summed[2 * group + ((j - 1) & 1)], s_count[(j - 1) & 1] + ((j - 1) >> 1), gave_up);
                             if (!ok) break;
                             tmem_after();
 #pragma unroll 1
@@ -574,7 +572,7 @@ __global__ void __launch_bounds__(384, 1) rows128_kernel(const __grid_constant__
                 // the part's rows
                 const int64_t slot = w.unit + blockIdx.x;
                 const bool whole = whole_unit(p, w, w.tile, w.tile + tiles - 1), is = x < used;
-                ok = ok && wait_warp(&sh.summed[group], o_count + tiles - 1, gave_up);
+                ok = ok && wait_warp(&sh.summed[2 * group + ((tiles - 1) & 1)], s_count[(tiles - 1) & 1] + ((tiles - 1) >> 1), gave_up);
                 bool again = false;
                 if (ok) {
                     tmem_after();
@@ -655,7 +653,6 @@ __global__ void __launch_bounds__(384, 1) rows128_kernel(const __grid_constant__
                         }
                     }
                 }
-                o_count += tiles;
                 s_count[0] += (tiles + 1) >> 1;
                 s_count[1] += tiles >> 1;
             } else {

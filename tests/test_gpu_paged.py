@@ -364,6 +364,81 @@ def test_places_beyond_2_to_the_31(paged):
     assert ((out[0] - want).abs() <= A * (2.0 ** -8 + 2 * n * 2.0 ** -24 + 2.0 ** -14) + want.abs() * 2.0 ** -8).all()
 
 
+def exact_on_gpu(k, v, lens, tables, counts, prefix, prefix_len, q, scale, cap):
+    """the formula in 64 bits, a sequence and a KV head at a time on the GPU; out, lse and the sums of weighted sizes that bound what rounding does"""
+    G, D = k.shape[2:]
+    H, ps = q.shape[1], k.shape[1]
+    out = torch.zeros(q.shape, dtype=torch.float64, device="cuda")
+    lse, size = torch.full(q.shape[:2], -math.inf, dtype=torch.float64, device="cuda"), torch.zeros_like(out)
+    first = 0
+    for b, (have, c) in enumerate(zip(lens, counts)):
+        x = torch.arange(have, device="cuda")
+        pages = [prefix.long()[torch.arange(prefix_len, device="cuda") // ps] * ps + torch.arange(prefix_len, device="cuda") % ps] if prefix_len else []
+        at = torch.cat(pages + [tables[b].long()[x // ps] * ps + x % ps])
+        keys, values = k.reshape(-1, G, D)[at].double(), v.reshape(-1, G, D)[at].double()
+        last = prefix_len + have - c + torch.arange(c, device="cuda")
+        for g in range(G):
+            heads = slice(g * (H // G), (g + 1) * (H // G))
+            s = torch.einsum("rhd,kd->rhk", q[first:first + c, heads].double(), keys[:, g]) * scale
+            s = cap * torch.tanh(s / cap) if cap else s
+            s = s.masked_fill(torch.arange(at.numel(), device="cuda") > last[:, None, None], -math.inf)
+            w = torch.softmax(s, -1)
+            out[first:first + c, heads], size[first:first + c, heads] = w @ values[:, g], w @ values[:, g].abs()
+            lse[first:first + c, heads] = torch.logsumexp(s, -1)
+        first += c
+    return out, lse, size
+
+
+LONG = [  # sequences, rows of the longest, tokens before, prefix, page, kv heads, group, size, cap: CTAs that take many tiles, and parts of several units
+    (16, 1, 40, 5120, 16, 8, 4, 128, 0.0), (64, 1, 40, 5120, 16, 8, 4, 128, 0.0), (64, 1, 300, 20000, 64, 8, 4, 64, 0.0), (70, 1, 100, 9001, 7, 4, 8, 128, 0.0), (32, 1, 77, 8200, 32, 8, 4, 256, 0.0),
+    (100, 1, 500, 3001, 48, 4, 5, 96, 30.0), (12, 200, 900, 2050, 32, 8, 2, 128, 0.0), (12, 200, 900, 0, 32, 8, 2, 128, 50.0), (2, 1500, 4000, 0, 16, 4, 4, 64, 0.0), (5, 300, 700, 1000, 8, 2, 3, 256, 20.0), (3, 5, 30000, 0, 16, 2, 4, 128, 0.0),
+    (40, 1, 3000, 0, 16, 8, 4, 128, 0.0), (2, 1, 50000, 0, 1, 2, 8, 64, 0.0),
+]
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16, F32], ids=str)
+@pytest.mark.parametrize("case", LONG, ids=lambda c: "x".join(map(str, c)))
+def test_attention_of_many_tiles(paged, case, dtype):
+    seqs, most, past, prefix, page, kv, group, size, cap = case
+    r = random.Random(seqs + prefix)
+    counts = [most] + [r.randint(max(1, most // 3), most) for _ in range(seqs - 1)]
+    lens = [past + most] + [r.randint(past // 4, past) + c for c in counts[1:]]
+    held, shared = [-(-n // page) for n in lens], -(-prefix // page)
+    g = torch.Generator("cuda")
+    g.manual_seed(seqs)
+    pages = sum(held) + shared
+    k, v = (torch.randn(pages, page, kv, size, generator=g, device="cuda").to(dtype) for _ in range(2))
+    order = torch.randperm(pages, generator=g, device="cuda").to(torch.int32)
+    tables = torch.full((seqs, max(held)), -1, dtype=torch.int32, device="cuda")
+    at = shared
+    for b, h in enumerate(held):
+        tables[b, :h] = order[at:at + h]
+        if lens[b] % page:   # what lies behind a sequence's last token is not read
+            k[order[at + h - 1].item(), lens[b] % page:] = math.nan
+            v[order[at + h - 1].item(), lens[b] % page:] = math.nan
+        at += h
+    if prefix % page:
+        k[order[shared - 1].item(), prefix % page:] = math.nan
+        v[order[shared - 1].item(), prefix % page:] = math.nan
+    starts = [0]
+    for c in counts:
+        starts.append(starts[-1] + c)
+    q = (1.5 * torch.randn(starts[-1], kv * group, size, generator=g, device="cuda")).to(dtype)
+    rows = torch.tensor(starts, dtype=torch.int32, device="cuda") if most > 1 else None
+    batch = paged.Batch(torch.tensor(lens, dtype=torch.int32, device="cuda"), tables, rows=rows, max_rows=most, prefix=order[:shared].contiguous() if prefix else None, prefix_len=prefix)
+    scale = size ** -0.5
+    out, lse = paged.attention(paged.KVPages(k, v), batch, q, softcap=cap, return_lse=True)
+    want, want_lse, sizes = exact_on_gpu(k, v, lens, tables, counts, order[:shared], prefix, q, scale, cap)
+    # as in paged_oracle.attention: a dot product's error D u of the sum of sizes (at most |q| |k|: here 1.5 D E|x|^2 scale with room), the exponential, the weights' rounding, and
+    # sums of n terms, which in 16-bit types run in accumulators that may truncate
+    n, u = prefix + max(lens), 2.0 ** -24
+    off = (size + 4) * u * 2.5 * size * scale + 8 * u * cap
+    rel = 2 * (off + 4 * u * 64 + 2.0 ** -21) + (2 * n + 64) * u
+    eps = torch.finfo(dtype).eps / 2
+    assert ((out.double() - want).abs() <= sizes * (rel + P_EPS[dtype]) * (1 + eps) + want.abs() * eps + torch.finfo(dtype).tiny).all()
+    assert ((lse.double() - want_lse).abs() <= rel + 4 * u * want_lse.abs()).all()
+
+
 # ---- together, captured, on other streams -------------------------------------------------------------------------------------------------------
 @pytest.mark.parametrize("dtype", [BF16, F32], ids=str)
 def test_a_chat_of_many_steps(paged, dtype):
