@@ -112,7 +112,8 @@ bool vectors(const void* p, int64_t row, int64_t head, int dtype) {
     return aligned(p, 16) && row % vec == 0 && head % vec == 0;
 }
 bool vectors(const lmrs_b200_rows_t* r, int dtype) { return vectors(r->data, r->row, r->head, dtype); }
-// Warps for a row's pieces: one, or more where the rows alone would not give every SM's schedulers a few each; a warp keeps at least one piece a lane
+// Warps for a row's pieces: one, or more where the rows alone would not give every SM's schedulers a few each; a warp keeps at least one piece a lane.
+// One warp a row / this rule, us a call: one row of 40 heads 3.6 / 2.5, keys of one row 6.4 / 4.3, of 64 rows 9.9 / 4.7; from a few thousand rows on it is one in both
 int parts_of(int64_t n_rows, int64_t pieces, int sms) {
     const int64_t want = ((int64_t)sms * 16 + n_rows - 1) / n_rows, most = (pieces + 31) / 32;
     return (int)std::max<int64_t>(1, std::min(want, most));
@@ -256,9 +257,22 @@ void place_line(Line& l, int64_t rows, const lmrs_b200_pages_t* pages, char* bas
     l.ml = (float2*)take(sizeof(float2) * (size_t)l.slots * l.tile_rows);
     l.o = (float*)take(sizeof(float) * (size_t)l.slots * l.tile_rows * pages->head_size);
 }
-// Which kernel takes what.  16-bit types: rows128_kernel takes the prefix from TENSOR_ROWS rows a KV head on, and a call with more than that many in one
-// sequence altogether; rows16_kernel the rest, and everything in float32.
-constexpr int TENSOR_ROWS = 32;
+// Which kernel takes what.  float32: rows16_kernel.  16-bit types: it depends on how often the keys would be read again.  rows16_kernel reads them once per 16
+// rows of a KV head and, with little to do, starts some 8 us sooner; rows128_kernel reads them once per 128 or 256 rows.  Measured on a B200 with rows16_kernel / rows128_kernel,
+// us a call, 8 KV heads:
+//   a sequence's own keys, 16 sequences behind 4000 keys, rows of a sequence and KV head:
+//     head 64:  32: 45 / 64   64: 80 / 76   128: 139 / 79      128:  32: 71 / 72   64: 130 / 84   128: 239 / 87      256:  8: 143 / 93   16: 148 / 96   32: 243 / 97
+//     (one sequence alone: 64: 22 / 23 at head 64, 28 / 26 at 128;  16: 31 / 32 and 8: 27 / 31 at 256)
+//   the prefix, rows of all sequences and a KV head behind a prefix of 512, 2048, 8192, 32768 keys:
+//     head 64:   16: 11 / 18, 13 / 23, 20 / 27, 39 / 47   32: 11 / 18, 16 / 23, 24 / 28, 63 / 47   128: 17 / 23, 28 / 27, 67 / 32, 220 / 53
+//     head 128:  16: 12 / 19, 16 / 24, 25 / 30, 56 / 60   32: 13 / 19, 18 / 25, 35 / 31, 96 / 60   128: 21 / 27, 36 / 33, 102 / 34, 359 / 65
+//     head 256:   8: 15 / 21, 23 / 30, 60 / 38, 162 / 83  32: 25 / 22, 35 / 31, 106 / 39, 385 / 83 128: 46 / 39, 114 / 42, 399 / 61, 1503 / 100
+// So the own keys by the rows, and the prefix by the rows times keys times KV heads that rows16_kernel would have to go through; with 16 rows or fewer it reads the keys once
+// and loses nothing, but for heads of 256, where only one of its CTAs fits an SM and the bytes in flight do not fill the memory.
+template <int DP> struct TensorRule {
+    static constexpr int OWN_ROWS = DP <= 128 ? 64 : 16, FRONT_ROWS = DP <= 128 ? 17 : 1;
+    static constexpr int64_t FRONT_WORK = DP <= 128 ? 1 << 21 : 1 << 19;
+};
 template <typename T, int DP> Cutting cutting(const lmrs_b200_pages_t* pages, const lmrs_b200_batch_t* batch, int64_t n_rows, int q_heads, char* base) {
     const int64_t group = q_heads / pages->kv_heads, rows = n_rows * group;
     Cutting c = {};
@@ -276,8 +290,9 @@ template <typename T, int DP> Cutting cutting(const lmrs_b200_pages_t* pages, co
         l.front_units = l.front_tiles ? (rows + tile_rows - 1) / tile_rows * pages->kv_heads : 0;
         place_line(l, rows, pages, base, c.bytes);
     };
-    c.own_tensor = sizeof(T) == 2 && std::min<int64_t>(batch->max_rows, n_rows) * group >= TENSOR_ROWS;
-    c.front_tensor = c.own_tensor || (sizeof(T) == 2 && rows >= TENSOR_ROWS && batch->prefix_len > 0);
+    using R = TensorRule<DP>;
+    c.own_tensor = sizeof(T) == 2 && std::min<int64_t>(batch->max_rows, n_rows) * group >= R::OWN_ROWS;
+    c.front_tensor = c.own_tensor || (sizeof(T) == 2 && rows >= R::FRONT_ROWS && rows * pages->kv_heads * batch->prefix_len >= R::FRONT_WORK);
     line(c.own, c.own_tensor, true, c.own_tensor == c.front_tensor);
     if (c.own_tensor == c.front_tensor) c.front = c.own;
     else line(c.front, true, false, true);
@@ -430,7 +445,8 @@ extern "C" int lmrs_b200_paged_attention(const lmrs_b200_pages_t* pages, const l
                 if (e != cudaSuccess) return refuse(me, std::string("launch failed: ") + cudaGetErrorString(e));
                 if (launched(me)) return 1;
             }
-            // a warp a row and head, or 8 where that leaves most of the GPU's warps idle: there the parts may be many
+            // A warp a row and head, or 8 where that leaves most of the GPU's warps idle, since there the parts are many.  One warp / 8, us a call: 32 rows and heads behind
+            // 30000 keys 46 / 39; behind 4000 keys 128: 22.4 / 19.7, 512: 46.0 / 45.1, 640: 54.2 / 56.3, 1024: 77.5 / 80.6; behind 200 keys 512: 13.2 / 12.4, 1024: 19.6 / 22.0
             const int64_t items = n_rows * q_heads;
             constexpr int COLS = decltype(d)::value <= 128 ? 1 : 2;
             e = items <= SMS * 4 ? launch_after(join_kernel<T, 8, COLS>, (unsigned)items, 256, 0, (cudaStream_t)stream, p, c.front, c.own)

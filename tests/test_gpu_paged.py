@@ -393,6 +393,7 @@ LONG = [  # sequences, rows of the longest, tokens before, prefix, page, kv head
     (16, 1, 40, 5120, 16, 8, 4, 128, 0.0), (64, 1, 40, 5120, 16, 8, 4, 128, 0.0), (64, 1, 300, 20000, 64, 8, 4, 64, 0.0), (70, 1, 100, 9001, 7, 4, 8, 128, 0.0), (32, 1, 77, 8200, 32, 8, 4, 256, 0.0),
     (100, 1, 500, 3001, 48, 4, 5, 96, 30.0), (12, 200, 900, 2050, 32, 8, 2, 128, 0.0), (12, 200, 900, 0, 32, 8, 2, 128, 50.0), (2, 1500, 4000, 0, 16, 4, 4, 64, 0.0), (5, 300, 700, 1000, 8, 2, 3, 256, 20.0), (3, 5, 30000, 0, 16, 2, 4, 128, 0.0),
     (40, 1, 3000, 0, 16, 8, 4, 128, 0.0), (2, 1, 50000, 0, 1, 2, 8, 64, 0.0),
+    (9, 2, 50, 1111, 16, 8, 4, 256, 0.0), (17, 5, 900, 60, 16, 2, 4, 256, 0.0), (6, 17, 500, 130, 32, 2, 4, 64, 30.0), (33, 1, 20, 70000, 128, 1, 1, 80, 0.0),
 ]
 
 
