@@ -284,10 +284,18 @@ template <typename T, int DP> Cutting cutting(const lmrs_b200_pages_t* pages, co
         l.tile_keys = tile_keys;
         while (1 << l.row_shift < tile_rows) l.row_shift++;
         while (1 << l.key_shift < tile_keys) l.key_shift++;
-        l.ctas = ctas;
         l.seqs = own ? batch->seqs : 0;
         l.front_tiles = front ? (int)(((int64_t)batch->prefix_len + tile_keys - 1) / tile_keys) : 0;
         l.front_units = l.front_tiles ? (rows + tile_rows - 1) / tile_rows * pages->kv_heads : 0;
+        // The prefix by itself: as many CTAs for each unit, where that leaves few SMs out, so that none has a part of two units (rows16_kernel's first CTAs take the SMs left out).
+        // 148 / 144 CTAs, 8 or 16 units, with the own keys: 64 sequences behind 8200 keys 71 / 67 us, 128 behind 32768 175 / 171, behind 8192 113 / 109, 32 behind 32768 79 / 77, 100
+        // behind 4096 59 / 54.  (Fewer still, so that the own keys' reads overlap the prefix' products, are better or worse by the lengths, which the host does not know: 96 CTAs
+        // 66, 156, 114, 71, 53; 64 CTAs 61, 208, 110, 93, 45.)
+        if (tensor && !own && l.front_units > 0 && l.front_units <= SMS) {
+            const int even = SMS / (int)l.front_units * (int)l.front_units;
+            if (even * 16 >= SMS * 15) ctas = even;
+        }
+        l.ctas = ctas;
         place_line(l, rows, pages, base, c.bytes);
     };
     using R = TensorRule<DP>;

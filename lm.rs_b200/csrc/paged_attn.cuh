@@ -637,7 +637,9 @@ __global__ void __launch_bounds__(TileShape<T, DP>::THREADS, TileShape<T, DP>::C
     int64_t from, to;
     walk_begin<T, S::THREADS>(p, l, ahead, from, to);
     grid_launch();
-    if (from >= to) { grid_wait(); return; }   // (the kernel before may still run: whoever waits for this one waits for both)
+    // The kernel before may still run.  The last CTA ends after it, so that whoever waits for this kernel waits for both; the others leave their SM to the next ones
+    const bool last_cta = blockIdx.x == gridDim.x - 1;
+    if (from >= to) { if (last_cta) grid_wait(); return; }
 
     // copies of a thread: keys t / 4 (and t / 4 + 32) of the tile, every fourth 16 bytes; past the end of a head zeros, so that the products need not know where it is
     Place place[S::COPY_KEYS];
@@ -808,7 +810,7 @@ __global__ void __launch_bounds__(TileShape<T, DP>::THREADS, TileShape<T, DP>::C
         start = last;
     }
     copy_wait<0>();
-    grid_wait();
+    if (last_cta) grid_wait();
 }
 
 // ---- joining parts ---------------------------------------------------------------------------------------------------------------------------
