@@ -230,7 +230,7 @@ typedef struct lmrs_b200_pages {
  * The prefix_len tokens of the pages that `prefix` lists come before every sequence's own (prefix NULL: none).
  * lens, rows, tables and prefix are int32 in device memory and read by the kernels, so a captured call follows what is written there.  An entry of
  * tables or prefix outside 0 .. pages - 1 is no page: what would lie there is neither written nor seen, nor is what lies beyond table_len pages.
- * max_rows: most rows of one sequence (it chooses the kernels, no result depends on it). */
+ * max_rows: most rows of one sequence (it chooses the kernels; a wrong number costs time, and results differ by the kernels' roundings only). */
 typedef struct lmrs_b200_batch {
     const int32_t *lens, *rows, *tables, *prefix;
     int64_t table_stride;
@@ -246,7 +246,7 @@ int lmrs_b200_paged_append(const lmrs_b200_pages_t* pages, const lmrs_b200_batch
  * of the exponentials.  A row that sees nothing (padding rows see no prefix either): out 0, lse -infinity.  head_size: a multiple of 8, at most 256;
  * k, v and their strides on 16-byte boundaries.  workspace: device memory of the size that paged_attention_workspace gives for
  * the same pages, batch (its host fields), n_rows and q_heads, on a 256-byte boundary; its contents do not matter before the call and mean nothing after it.  Calls
- * that may run at the same time need one each. */
+ * that may run at the same time need one each.  Heads: up to 65535; n_rows * q_heads: up to 2^30. */
 int lmrs_b200_paged_attention_workspace(const lmrs_b200_pages_t* pages, const lmrs_b200_batch_t* batch, int64_t n_rows, int q_heads, size_t* bytes);
 int lmrs_b200_paged_attention(const lmrs_b200_pages_t* pages, const lmrs_b200_batch_t* batch, int64_t n_rows, const lmrs_b200_rows_t* q, const lmrs_b200_rows_t* out,
                               int q_heads, float scale, float softcap, float* lse, void* workspace, size_t workspace_bytes, void* stream);
