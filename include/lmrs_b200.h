@@ -243,7 +243,7 @@ int lmrs_b200_paged_append(const lmrs_b200_pages_t* pages, const lmrs_b200_batch
                            const lmrs_b200_rope_t* rope, const lmrs_b200_positions_t* pos, const lmrs_b200_rows_t* q, const lmrs_b200_rows_t* q_out, int q_heads, void* stream);
 /* out = softmax(scale * q . keys) . values for every row: the prefix, and the row's own sequence up to the row's index.  q head h reads KV head
  * h / (q_heads / kv_heads).  softcap > 0: scores become softcap * tanh(score / softcap).  lse (NULL, or f32 [n_rows][q_heads]): the logarithm of the sum
- * of the exponentials.  A row that sees nothing (padding rows see no prefix either): out 0, lse -infinity.  head_size: a multiple of 8, at most 256;
+ * of the exponentials.  A row that sees nothing (padding rows see no prefix either): out 0, lse -infinity.  out may not overlap q.  head_size: a multiple of 8, at most 256;
  * k, v and their strides on 16-byte boundaries.  workspace: device memory of the size that paged_attention_workspace gives for
  * the same pages, batch (its host fields), n_rows and q_heads, on a 256-byte boundary; its contents do not matter before the call and mean nothing after it.  Calls
  * that may run at the same time need one each.  Heads: up to 65535; n_rows * q_heads: up to 2^30. */

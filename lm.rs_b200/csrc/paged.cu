@@ -409,6 +409,7 @@ extern "C" int lmrs_b200_paged_attention(const lmrs_b200_pages_t* pages, const l
         why = bad_batch_memory(batch, device);
         if (why.empty()) why = bad_rows(q, "q", dtype, device);
         if (why.empty()) why = bad_rows(out, "out", dtype, device);
+        if (why.empty() && out->data == q->data) why = "out lies where q does, which is read until the call has ended";
         if (why.empty() && lse && (!aligned(lse, 4) || !on_device(lse, device))) why = "lse is not memory of the current device";
         if (why.empty() && (!on_device(pages->k, device) || !on_device(pages->v, device))) why = "the pages are not memory of the current device";
         if (why.empty() && (!workspace || !aligned(workspace, 256) || !on_device(workspace, device))) why = "workspace is not memory of the current device on a 256-byte boundary";

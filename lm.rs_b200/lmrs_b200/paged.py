@@ -266,7 +266,8 @@ def append(pages, batch, k, v, rope=None, pos=None, q=None, q_out=None):
 def attention(pages, batch, q, out=None, scale=None, softcap=0.0, return_lse=False):
     """softmax(scale * q . keys) . values for q [rows, heads, head_size]: every row over the prefix and over its own sequence up to its own place.
     heads: a multiple of kv_heads, neighbours share one.  scale None: head_size ** -0.5.  softcap > 0: scores s become softcap * tanh(s / softcap).  A row
-    that sees nothing is 0.  return_lse: also the logarithms of the sums of exponentials, float32 [rows, heads] (-inf for a row that sees nothing)."""
+    that sees nothing is 0.  return_lse: also the logarithms of the sums of exponentials, float32 [rows, heads] (-inf for a row that sees nothing).
+    out may not overlap q."""
     if not isinstance(batch, Batch):
         raise LmrsError("batch must be a Batch")
     if not isinstance(q, torch.Tensor) or q.dim() != 3:

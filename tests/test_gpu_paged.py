@@ -394,6 +394,7 @@ LONG = [  # sequences, rows of the longest, tokens before, prefix, page, kv head
     (100, 1, 500, 3001, 48, 4, 5, 96, 30.0), (12, 200, 900, 2050, 32, 8, 2, 128, 0.0), (12, 200, 900, 0, 32, 8, 2, 128, 50.0), (2, 1500, 4000, 0, 16, 4, 4, 64, 0.0), (5, 300, 700, 1000, 8, 2, 3, 256, 20.0), (3, 5, 30000, 0, 16, 2, 4, 128, 0.0),
     (40, 1, 3000, 0, 16, 8, 4, 128, 0.0), (2, 1, 50000, 0, 1, 2, 8, 64, 0.0),
     (9, 2, 50, 1111, 16, 8, 4, 256, 0.0), (17, 5, 900, 60, 16, 2, 4, 256, 0.0), (6, 17, 500, 130, 32, 2, 4, 64, 30.0), (33, 1, 20, 70000, 128, 1, 1, 80, 0.0),
+    (8, 1, 3000, 200, 16, 1, 16, 256, 0.0), (5, 1, 700, 0, 16, 1, 64, 128, 0.0), (4, 3, 500, 300, 16, 1, 48, 64, 0.0), (3, 2, 400, 1500, 24, 1, 128, 128, 20.0),
 ]
 
 
@@ -593,3 +594,12 @@ def test_calls_of_no_rows(paged):
     out = torch.full_like(q, 7.0)
     paged.attention(pages, idle, q, out=out)   # sequences without rows, rows without a sequence
     assert (out == 7.0).all()
+
+
+def test_attention_into_its_queries_is_refused(paged):
+    m = Made(paged, 1, BF16, [40, 50], [1, 1], 16, 2, 2, 64, 20, one_each=True)
+    pages, batch = m.on_gpu()
+    q = m.q.cuda()
+    with pytest.raises(paged.LmrsError, match="lies where q does"):
+        paged.attention(pages, batch, q, out=q)
+    m.check(*paged.attention(pages, batch, q, return_lse=True))
