@@ -345,6 +345,7 @@ __global__ void __launch_bounds__(384, 1) rows128_kernel(const __grid_constant__
                             }
                         }
                     }
+                    copy_commit();   // a group of their own: the wait for them may come before any operand tile by cp.async has made one
                     __syncwarp();
                     asked = true;
                 }

@@ -603,3 +603,79 @@ def test_attention_into_its_queries_is_refused(paged):
     with pytest.raises(paged.LmrsError, match="lies where q does"):
         paged.attention(pages, batch, q, out=q)
     m.check(*paged.attention(pages, batch, q, return_lse=True))
+
+
+# ---- batches made on the GPU ------------------------------------------------------------------------------------------------------------------------
+class MadeThere:
+    """sequences of given lengths and rows over pages in random order, values made on the GPU; what lies behind a list's last token holds NaN"""
+
+    def __init__(self, paged, seed, dtype, lens, counts, page, kv, group, size, prefix=0):
+        self.paged, self.dtype, self.lens, self.counts, self.prefix_len, self.size = paged, dtype, list(lens), list(counts), prefix, size
+        g = torch.Generator("cuda")
+        g.manual_seed(seed)
+        held, shared = [-(-n // page) for n in lens], -(-prefix // page)
+        pages = sum(held) + shared
+        self.k, self.v = (torch.randn(pages, page, kv, size, generator=g, device="cuda").to(dtype) for _ in range(2))
+        order = torch.randperm(pages, generator=g, device="cuda").to(torch.int32)
+        self.tables = torch.full((len(lens), max(held)), -1, dtype=torch.int32, device="cuda")
+        self.prefix = order[:shared].contiguous()
+        at, ends = shared, [(self.prefix, prefix)]
+        for b, h in enumerate(held):
+            self.tables[b, :h] = order[at:at + h]
+            at += h
+            ends.append((self.tables[b, :h], lens[b]))
+        for table, n in ends:
+            if n % page:
+                self.k[table[-1].item(), n % page:] = math.nan
+                self.v[table[-1].item(), n % page:] = math.nan
+        starts = [0]
+        for c in counts:
+            starts.append(starts[-1] + c)
+        self.q = (1.5 * torch.randn(starts[-1], kv * group, size, generator=g, device="cuda")).to(dtype)
+        one = max(counts) == min(counts) == 1
+        self.rows = None if one else torch.tensor(starts, dtype=torch.int32, device="cuda")
+        self.pages = paged.KVPages(self.k, self.v)
+        self.batch = self.batch_of()
+
+    def batch_of(self, max_rows=None):
+        return self.paged.Batch(torch.tensor(self.lens, dtype=torch.int32, device="cuda"), self.tables, rows=self.rows, max_rows=max_rows or max(self.counts),
+                                prefix=self.prefix if self.prefix_len else None, prefix_len=self.prefix_len)
+
+    def exact(self, cap=0.0):
+        """out, lse, and what a call may be off in either (as in test_attention_of_many_tiles)"""
+        scale = self.size ** -0.5
+        want, want_lse, sizes = exact_on_gpu(self.k, self.v, self.lens, self.tables, self.counts, self.prefix, self.prefix_len, self.q, scale, cap)
+        n, u, eps = self.prefix_len + max(self.lens), 2.0 ** -24, torch.finfo(self.dtype).eps / 2
+        off = (self.size + 4) * u * 2.5 * self.size * scale + 8 * u * cap
+        rel = 2 * (off + 4 * u * 64 + 2.0 ** -21) + (2 * n + 64) * u
+        return want, want_lse, sizes * (rel + P_EPS[self.dtype]) * (1 + eps) + want.abs() * eps + torch.finfo(self.dtype).tiny, rel + 4 * u * want_lse.abs()
+
+
+def holds(got, exact):
+    (out, lse), (want, want_lse, tol, tol_lse) = got, exact
+    assert ((out.double() - want).abs() <= tol).all(), float(((out.double() - want).abs() - tol).max())
+    assert ((lse.double() - want_lse).abs() <= tol_lse).all(), float(((lse.double() - want_lse).abs() - tol_lse).max())
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16], ids=str)
+@pytest.mark.parametrize("group, size", [(3, 64), (6, 128), (7, 256), (5, 96), (12, 40)], ids=str)
+@pytest.mark.parametrize("prefix", [0, 320], ids=["own", "prefix"])
+def test_groups_that_do_not_divide_a_block(paged, group, size, prefix, dtype):
+    """Tensor-core units whose queries no TMA box holds, several short ones a CTA, keys by TMA: the queries come from far away (the cache holds other things), the keys from near, and every call gives
+    the same bits as the first."""
+    if prefix:
+        rows = (60 if size <= 128 else 15) // group   # (below the own keys' rule, so that the prefix is a line by itself)
+        n = 300 * (256 if size <= 128 else 128) // (8 * group * rows)   # some 300 units of the prefix, 5 tiles each
+        m = MadeThere(paged, group, dtype, [rows + 3] * n, [rows] * n, 16, 8, group, size, prefix)
+    else:
+        rows = -(-64 // group)
+        m = MadeThere(paged, group, dtype, [rows + 70] * 60, [rows] * 60, 16, 8, group, size)   # 480 units, 2 or 3 tiles each
+    exact = m.exact()
+    first = paged.attention(m.pages, m.batch, m.q, return_lse=True)
+    holds(first, exact)
+    other = torch.empty(512 << 20, dtype=torch.uint8, device="cuda")
+    for i in range(8):
+        other.fill_(i)
+        m.k.sum(), m.v.sum()
+        out, lse = paged.attention(m.pages, m.batch, m.q, return_lse=True)
+        assert torch.equal(out, first[0]) and torch.equal(lse, first[1])

@@ -142,3 +142,17 @@ def test_every_refusal_without_a_gpu_says_so(paged, gpu_lib):
     assert L.lmrs_b200_paged_attention(C.byref(pg), C.byref(bt), 3, r, r, 4, 0.125, 0.0, None, P, 1 << 30, None) and b"no CUDA device" in L.lmrs_b200_last_error()
     assert L.lmrs_b200_paged_append(C.byref(pg), C.byref(bt), 3, r, r, C.byref(rope), None, None, None, 0, None) and b"no CUDA device" in L.lmrs_b200_last_error()
     assert L.lmrs_b200_rope_axes(C.byref(rope), 0, r, r, 3, 4, 64, C.byref(pos), None) and b"no CUDA device" in L.lmrs_b200_last_error()
+
+
+def test_every_asynchronous_copy_belongs_to_a_group():
+    """A wait for groups waits for committed copies only.  In the tensor-core kernel, whatever asks for copies by threads (queries, operand tiles without TMA) commits them before it says that they are on
+    their way: read from the source, since a copy that is late shows itself by chance only."""
+    import os
+    import re
+    src = open(os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "lm.rs_b200", "csrc", "paged_tensor.cuh")).read()
+    asked = [m.start() for m in re.finditer(r"copy16\(", src)]
+    handed_on = [m.start() for m in re.finditer(r"asked = true;|next_slot\(\);", src)]
+    assert len(asked) == 3 and "asked = true;" in src
+    for at in asked:
+        end = min(p for p in handed_on if p > at)
+        assert "copy_commit();" in src[at:end], src[at:at + 80]
