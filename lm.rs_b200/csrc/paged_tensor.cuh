@@ -134,6 +134,9 @@ template <typename T, int DP> struct TensorShared {
     int64_t starts[S::COPIERS][S::KEYS / S::COPIERS];             // a copying warp's: where the rows that it copies begin (bytes; -1: nowhere)
     uint32_t tmem;
     int gave_up;
+    bool spoiled;                               // some row of some part is not finite where other rows' keys may be why
+    Walk start;                                 // where the CTA begins, and how many tiles it has
+    int tiles;
     AgainScratch again[2];
 };
 
@@ -171,12 +174,14 @@ __global__ void __launch_bounds__(384, 1) rows128_kernel(const __grid_constant__
         mbar_init(&sh.queries_read, 1);
         mbar_init(&sh.parted, 256);
         sh.gave_up = 0;
+        sh.spoiled = false;
         fence_barrier_init();
     }
     Walk w;
     int64_t from, to;
     walk_begin<T, S::THREADS>(p, l, w, from, to);   // (synchronises the CTA)
     if (from >= to) { grid_launch(); return; }
+    if (threadIdx.x == 0) { sh.start = w; sh.tiles = (int)(to - from); }
     if (warp == PRODUCTS) {
         __syncwarp();
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_at(&sh.tmem)), "n"(512) : "memory");
@@ -580,7 +585,6 @@ __global__ void __launch_bounds__(384, 1) rows128_kernel(const __grid_constant__
                 const int64_t slot = w.unit + blockIdx.x;
                 const bool whole = whole_unit(p, w, w.tile, w.tile + tiles - 1), is = x < used;
                 ok = ok && wait_warp(&sh.summed[2 * group + ((tiles - 1) & 1)], s_count[(tiles - 1) & 1] + ((tiles - 1) >> 1), gave_up);
-                bool again = false;
                 if (ok) {
                     tmem_after();
                     if (!seen) sum = -1.0f;
@@ -623,41 +627,13 @@ __global__ void __launch_bounds__(384, 1) rows128_kernel(const __grid_constant__
                     }
                     tmem_before();
                     arrive(&sh.read[group]);
-                    again = is && seen && !finite && w.b >= 0 && w.s.count > 1;   // other rows' keys may have spoiled it
+                    if (is && seen && !finite && w.b >= 0 && w.s.count > 1) sh.spoiled = true;   // other rows' keys may have spoiled it
                 } else if (is) {   // gave up: NaN
                     if (whole) {
                         for (int c = 0; c < D; c++) p.out.data[r.row * p.out.row + r.head * p.out.head + c] = from_f<T>(NAN);
                         if (p.lse) p.lse[r.row * p.q_heads + r.head] = NAN;
                     } else if (slot < l.slots) {
                         l.ml[slot * S::ROWS + x] = make_float2(NAN, NAN);
-                    }
-                }
-                int* flags = reinterpret_cast<int*>(sh.again[group].weight);
-                again_sync(1 + group);
-                flags[row] = again;
-                again_sync(1 + group);
-                unsigned todo[4], any = 0;
-#pragma unroll
-                for (int i = 0; i < 4; i++) any |= todo[i] = __ballot_sync(~0u, flags[32 * i + lane]);
-                if (any) {
-                    again_sync(1 + group);   // (the flags' place is used below)
-#pragma unroll 1
-                    for (int i = 0; i < S::BLOCK; i++) {
-                        if (!((i < 32 ? todo[0] : i < 64 ? todo[1] : i < 96 ? todo[2] : todo[3]) >> (i & 31) & 1)) continue;
-                        const UnitRow r2 = unit_row(p, l, w, group * S::BLOCK + i);
-                        float m2, l2, acc[2];
-                        row_again(p, w, r2, w.tile * S::KEYS, (w.tile + tiles) * S::KEYS, sh.again[group], 1 + group, m2, l2, acc);
-#pragma unroll
-                        for (int k = 0; k < 2; k++) {
-                            const int c = row + AGAIN * k;
-                            if (c >= D) continue;
-                            if (whole) p.out.data[r2.row * p.out.row + r2.head * p.out.head + c] = from_f<T>(acc[k] / l2);
-                            else if (slot < l.slots) *part_at(l, D, slot, group * S::BLOCK + i, c) = acc[k];
-                        }
-                        if (row == 0) {
-                            if (whole) { if (p.lse) p.lse[r2.row * p.q_heads + r2.head] = lse_of(m2, l2); }
-                            else if (slot < l.slots) l.ml[slot * S::ROWS + group * S::BLOCK + i] = make_float2(m2, l2);
-                        }
                     }
                 }
                 s_count[0] += (tiles + 1) >> 1;
@@ -677,6 +653,56 @@ __global__ void __launch_bounds__(384, 1) rows128_kernel(const __grid_constant__
         tmem_after();
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "n"(512) : "memory");
     }
+    // Rows to be summed again, all parts once more: behind the last wait of the CTA, since this takes as long as it takes (128 rows of 64 columns over 150 thousand keys: seconds)
+    if (warp >= 8 || !sh.spoiled || *gave_up) return;
+    const int group = warp >> 2, row = threadIdx.x & 127;
+    int* flags = reinterpret_cast<int*>(sh.again[group].weight);
+    w = sh.start;
+    left = sh.tiles;
+    do {
+        enter();
+        if (w.b < 0 || w.s.count <= 1 || group >= blocks) continue;
+        const int64_t slot = w.unit + blockIdx.x;
+        const bool whole = whole_unit(p, w, w.tile, w.tile + tiles - 1);
+        if (!whole && slot >= l.slots) continue;
+        const int x = group * S::BLOCK + row;
+        bool again = false;
+        if (x < used) {   // (what this thread has stored)
+            const UnitRow r = unit_row(p, l, w, x);
+            float odd = 0.0f;   // becomes NaN if the row is not finite
+            if (whole)
+                for (int c = 0; c < D; c++) odd = fmaf(to_f(p.out.data[r.row * p.out.row + r.head * p.out.head + c]), 0.0f, odd);
+            else if (!(l.ml[slot * S::ROWS + x].y < 0.0f))
+                for (int c = 0; c < D; c++) odd = fmaf(*part_at(l, D, slot, x, c), 0.0f, odd);
+            again = odd != 0.0f;
+        }
+        again_sync(1 + group);
+        flags[row] = again;
+        again_sync(1 + group);
+        unsigned todo[4], any = 0;
+#pragma unroll
+        for (int i = 0; i < 4; i++) any |= todo[i] = __ballot_sync(~0u, flags[32 * i + lane]);
+        if (!any) continue;
+        again_sync(1 + group);   // (the flags' place is used below)
+#pragma unroll 1
+        for (int i = 0; i < S::BLOCK; i++) {
+            if (!((i < 32 ? todo[0] : i < 64 ? todo[1] : i < 96 ? todo[2] : todo[3]) >> (i & 31) & 1)) continue;
+            const UnitRow r = unit_row(p, l, w, group * S::BLOCK + i);
+            float m, sum, acc[2];
+            row_again(p, w, r, w.tile * S::KEYS, (w.tile + tiles) * S::KEYS, sh.again[group], 1 + group, m, sum, acc);
+#pragma unroll
+            for (int k = 0; k < 2; k++) {
+                const int c = row + AGAIN * k;
+                if (c >= D) continue;
+                if (whole) p.out.data[r.row * p.out.row + r.head * p.out.head + c] = from_f<T>(acc[k] / sum);
+                else *part_at(l, D, slot, group * S::BLOCK + i, c) = acc[k];
+            }
+            if (row == 0) {
+                if (whole) { if (p.lse) p.lse[r.row * p.q_heads + r.head] = lse_of(m, sum); }
+                else l.ml[slot * S::ROWS + group * S::BLOCK + i] = make_float2(m, sum);
+            }
+        }
+    } while (leave());
 }
 
 }  // namespace paged

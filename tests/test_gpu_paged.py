@@ -679,3 +679,54 @@ def test_groups_that_do_not_divide_a_block(paged, group, size, prefix, dtype):
         m.k.sum(), m.v.sum()
         out, lse = paged.attention(m.pages, m.batch, m.q, return_lse=True)
         assert torch.equal(out, first[0]) and torch.equal(lse, first[1])
+
+
+def exact_of_repeats(k, v, times, n, kv, group, q, cap=0.0):
+    """out, lse and sums of sizes in 64 bits for n rows at the end of `times` copies of the first page and one of the second: keys of the first count that often"""
+    page, size = k.shape[1], k.shape[3]
+    out, sizes = torch.empty(q.shape, dtype=torch.float64, device="cuda"), torch.empty(q.shape, dtype=torch.float64, device="cuda")
+    lse = torch.empty(q.shape[:2], dtype=torch.float64, device="cuda")
+    for h in range(kv):
+        heads = slice(h * group, (h + 1) * group)
+        s = torch.einsum("rgd,kd->rgk", q[:, heads].double(), k[:, :, h].reshape(-1, size).double()) * size ** -0.5
+        s = cap * torch.tanh(s / cap) if cap else s
+        s[..., :page] += math.log(times)
+        s.masked_fill_(torch.arange(2 * page, device="cuda") > (2 * page - n + torch.arange(n, device="cuda"))[:, None, None], -math.inf)
+        values, w = v[:, :, h].reshape(-1, size).double(), torch.softmax(s, -1)
+        out[:, heads], sizes[:, heads], lse[:, heads] = w @ values, w @ values.abs(), torch.logsumexp(s, -1)
+    return out, lse, sizes
+
+
+def repeats(paged, seed, kv, group, size, page, times, n):
+    """one sequence whose table names one page `times` times and then another, and its last n tokens' queries"""
+    g = torch.Generator("cuda")
+    g.manual_seed(seed)
+    k, v = (torch.randn(2, page, kv, size, generator=g, device="cuda").to(BF16) for _ in range(2))
+    q = (1.5 * torch.randn(n, kv * group, size, generator=g, device="cuda")).to(BF16)
+    batch = paged.Batch(torch.tensor([(times + 1) * page], dtype=torch.int32, device="cuda"), torch.tensor([[0] * times + [1]], dtype=torch.int32, device="cuda"),
+                        rows=torch.tensor([0, n], dtype=torch.int32, device="cuda"), max_rows=n)
+    return k, v, q, batch
+
+
+def repeats_tolerance(want, want_lse, sizes, have, size, cap=0.0):
+    """as in test_attention_of_many_tiles, but for the sums: 64 weights of a tile are added up before they join the running sum, and the tensor cores add 16 products at a time, in accumulators that
+    may truncate (2 u); on CUDA cores 128 terms at a time"""
+    eps, u = 2.0 ** -8, 2.0 ** -24
+    rel = 2 * ((size + 4) * u * 2.5 * size * size ** -0.5 + 8 * u * cap + 4 * u * 64 + 2.0 ** -21) + (have // 64 + 2 * (have // 16) + 2 * 128 + 64) * u
+    return sizes * (rel + eps) * (1 + eps) + want.abs() * eps + torch.finfo(BF16).tiny, rel + 4 * u * want_lse.abs()
+
+
+def test_rows_summed_again_while_others_wait(paged):
+    """An infinity in the last value of one KV head, behind 150 thousand keys, where 63 tokens x 4 heads do not see it: summing them again takes seconds, and what the same CTA has yet to do
+    (the next head's keys) is as it would be otherwise."""
+    kv, group, size, n, head = 75, 4, 64, 128, 1   # 150 units of 256 rows for 148 CTAs: one has the end of this head's second unit, then the begin of the next head's
+    k, v, q, batch = repeats(paged, 5, kv, group, size, 1024, 146, n)
+    v[1, -1, head, 7] = math.inf
+    out, lse = paged.attention(paged.KVPages(k, v), batch, q, return_lse=True)
+    seers = out.view(n, kv, group, size)[n - 1, head, :, 7]
+    assert torch.isposinf(seers).all()
+    v[1, -1, head, 7] = 0.0   # (for the comparison: a place that its seers' column alone has)
+    want, want_lse, sizes = exact_of_repeats(k, v, 146, n, kv, group, q)
+    tol, tol_lse = repeats_tolerance(want, want_lse, sizes, 147 * 1024, size)
+    seers.copy_(want.view(n, kv, group, size)[n - 1, head, :, 7])
+    holds((out, lse), (want, want_lse, tol, tol_lse))
