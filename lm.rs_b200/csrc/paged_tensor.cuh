@@ -44,6 +44,25 @@ PG_DEVINL bool wait_warp(uint64_t* bar, int count, volatile int* gave_up) {
     __syncwarp();
     return ok;
 }
+// The same for what comes once a part, however long the part is: the limit begins anew whenever `flips`, a barrier that goes on with the part's tiles, is seen in another phase
+PG_DEVINL bool wait_part_lane(uint64_t* bar, uint32_t parity, uint64_t* flips, volatile int* gave_up) {
+    uint32_t from = dense::now_ns();
+    bool phase = dense::mbar_test(flips, 0);
+    for (uint32_t i = 0;; i++) {   // (each try suspends for a while)
+        if (mbar_try_wait(bar, parity)) return true;
+        if (*gave_up) return false;
+        const bool now = dense::mbar_test(flips, 0);
+        if (now != phase) { phase = now; from = dense::now_ns(); i = 0; }
+        else if (i >= dense::TG_LEAST_TRIES && dense::now_ns() - from >= dense::TG_WAIT_NS) break;
+    }
+    if (!*gave_up) *gave_up = PAGED_WAIT;
+    return false;
+}
+PG_DEVINL bool wait_part(uint64_t* bar, int count, uint64_t* flips, volatile int* gave_up) {
+    const bool ok = __all_sync(~0u, wait_part_lane(bar, (uint32_t)count & 1, flips, gave_up));
+    __syncwarp();
+    return ok;
+}
 // has the phase ended?
 PG_DEVINL bool looks_free(uint64_t* bar, int count) { return __all_sync(~0u, dense::mbar_test(bar, (uint32_t)count & 1)); }
 PG_DEVINL void arrive(uint64_t* bar) { asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_at(bar)) : "memory"); }
@@ -643,7 +662,7 @@ __global__ void __launch_bounds__(384, 1) rows128_kernel(const __grid_constant__
             }
             k_count += tiles;
             arrive(&sh.parted);
-            ok = ok && wait_warp(&sh.parted, part++, gave_up);
+            ok = ok && wait_part(&sh.parted, part++, &sh.known[0], gave_up);
         } while (leave());
     }
     tmem_before();

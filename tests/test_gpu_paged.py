@@ -730,3 +730,12 @@ def test_rows_summed_again_while_others_wait(paged):
     tol, tol_lse = repeats_tolerance(want, want_lse, sizes, 147 * 1024, size)
     seers.copy_(want.view(n, kv, group, size)[n - 1, head, :, 7])
     holds((out, lse), (want, want_lse, tol, tol_lse))
+
+
+def test_a_part_of_seconds(paged):
+    """heads of 256, whose units have one block of rows: the CTA's second group waits for the end of the part, which here takes more than two seconds: 120 million keys (a page that the table names 234375 times)"""
+    kv, size, n = 148, 256, 128
+    k, v, q, batch = repeats(paged, 6, kv, 1, size, 512, 234375, n)
+    out, lse = paged.attention(paged.KVPages(k, v), batch, q, softcap=30.0, return_lse=True)
+    want, want_lse, sizes = exact_of_repeats(k, v, 234375, n, kv, 1, q, 30.0)
+    holds((out, lse), (want, want_lse, *repeats_tolerance(want, want_lse, sizes, 234376 * 512, size, 30.0)))
