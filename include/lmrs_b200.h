@@ -190,7 +190,7 @@ void lmrs_b200_weights_free(lmrs_b200_weights_t* w);
  * Keys and values of any number of sequences in pages of one pool, rows of a call appended to them with their rotary positions (one axis or
  * several: time, height, width of image and video rows) applied on the way, and attention over them in which a prefix that all sequences share is
  * read and computed once for all.  DEVICE pointers, on the caller's stream (a cudaStream_t; NULL: the legacy default stream) and the current
- * device; nothing is allocated, kept or synchronised, so calls on several streams, and calls captured into CUDA graphs, do not meet anywhere but in the
+ * device; nothing is allocated (but for one word of host memory in a process' first call of paged_attention with many rows), kept or synchronised, so calls on several streams, and calls captured into CUDA graphs, do not meet anywhere but in the
  * caller's own arrays.  dtype: 0 bfloat16, 1 float32, 2 float16, the same for all arrays of a call; angles, scores, softmax and sums are 32-bit or
  * wider.  Strides count elements; the elements of a head lie next to each other.
  *
@@ -246,7 +246,8 @@ int lmrs_b200_paged_append(const lmrs_b200_pages_t* pages, const lmrs_b200_batch
  * of the exponentials.  A row that sees nothing (padding rows see no prefix either): out 0, lse -infinity.  out may not overlap q.  head_size: a multiple of 8, at most 256;
  * k, v and their strides on 16-byte boundaries.  workspace: device memory of the size that paged_attention_workspace gives for
  * the same pages, batch (its host fields), n_rows and q_heads, on a 256-byte boundary; its contents do not matter before the call and mean nothing after it.  Calls
- * that may run at the same time need one each.  Heads: up to 65535; n_rows * q_heads: up to 2^30. */
+ * that may run at the same time need one each.  Heads: up to 65535; n_rows * q_heads: up to 2^30.  A kernel whose waits run out (two seconds in which nothing moves) leaves NaN in the
+ * rows that it still had to do; the process' next call of paged_attention then launches nothing and says which wait it was, once. */
 int lmrs_b200_paged_attention_workspace(const lmrs_b200_pages_t* pages, const lmrs_b200_batch_t* batch, int64_t n_rows, int q_heads, size_t* bytes);
 int lmrs_b200_paged_attention(const lmrs_b200_pages_t* pages, const lmrs_b200_batch_t* batch, int64_t n_rows, const lmrs_b200_rows_t* q, const lmrs_b200_rows_t* out,
                               int q_heads, float scale, float softcap, float* lse, void* workspace, size_t workspace_bytes, void* stream);

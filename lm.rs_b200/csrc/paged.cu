@@ -99,6 +99,7 @@ std::string bad_batch_memory(const lmrs_b200_batch_t* b, int device) {
 Batch batch_as(const lmrs_b200_batch_t* b, const lmrs_b200_pages_t* p, int64_t n_rows) {
     return Batch{b->lens, b->rows, b->tables, b->prefix, b->table_stride, b->seqs, b->table_len, b->prefix_len, p->pages, p->page_size, n_rows};
 }
+GaveUpWord gave_up_word;
 template <typename F> int guarded(const char* where, F f) {   // no exception leaves a C entry point
     try {
         return f();
@@ -414,6 +415,7 @@ extern "C" int lmrs_b200_paged_attention(const lmrs_b200_pages_t* pages, const l
         if (why.empty() && (!on_device(pages->k, device) || !on_device(pages->v, device))) why = "the pages are not memory of the current device";
         if (why.empty() && (!workspace || !aligned(workspace, 256) || !on_device(workspace, device))) why = "workspace is not memory of the current device on a 256-byte boundary";
         if (!why.empty()) return refuse(me, why);
+        if (const int status = gave_up_word.take()) return refuse(me, "results of an earlier call are NaN: " + dense::tg_gave_up(status));
         return by_shape(pages, [&](auto t, auto d) {
             using T = decltype(t);
             using S = TileShape<T, decltype(d)::value>;
@@ -441,6 +443,7 @@ extern "C" int lmrs_b200_paged_attention(const lmrs_b200_pages_t* pages, const l
                     auto kernel = rows128_kernel<T, decltype(d)::value>;
                     using X = TensorShape<T, decltype(d)::value>;
                     if ((e = allow_smem(kernel, device, X::SMEM, allowed_tensor)) != cudaSuccess) return refuse(me, cudaGetErrorString(e));
+                    if (!(p.err = gave_up_word.get())) return refuse(me, "out of host memory");
                     Boxes boxes = {};
                     box_maps<X>(pages, q, n_rows, q_heads, p.q_wide, boxes);
                     kernel<<<(unsigned)c.front.ctas, X::THREADS, X::SMEM, (cudaStream_t)stream>>>(p, c.front, boxes);

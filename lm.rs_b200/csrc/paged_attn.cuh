@@ -46,6 +46,7 @@ template <typename T> struct AttnParams {
     bool q_wide, out_wide;                     // rows on 16-byte boundaries
     int page_shift;                            // log2 of page_size, -1 if it is no power of two
     bool whole;                                // no prefix: a unit that one CTA takes is finished there
+    int* err;                                  // mapped host word: set when a kernel gave up
 };
 // What one kernel goes through: units of the prefix (if it takes them), then those of the sequences (if it takes them)
 struct Line {

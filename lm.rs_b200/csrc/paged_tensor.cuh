@@ -17,8 +17,11 @@
 // 64 keys a tile with two sets of scores: the scores of the next tile under the powers of this one.  (128 keys with one set / this, when it was changed:
 // 215 / 213 for 128 sequences behind 32768 with their own keys, 538 / 431 for the capped prompts.)
 // Keys by TMA boxes and by cp.async: 174 / 292, 67 / 87 and 312 / 515 for the three with their own keys.
-// Every wait on an mbarrier is bounded in time, as in dense_gemm.cuh.  Of a CTA that gives up, the rows that it still had to do come out as NaN.
+// Every wait on an mbarrier is bounded in time, as in dense_gemm.cuh.  Of a CTA that gives up, the rows that it still had to do come out as NaN, and the next call says so (GaveUpWord).
 #pragma once
+#include <atomic>
+#include <mutex>
+
 #include "dense_gemm.cuh"
 #include "paged_attn.cuh"
 
@@ -35,12 +38,11 @@ template <typename T, int DP> struct TensorShape {
     static_assert(O_AT + BLOCKS * DP <= 512 && 2 * 2 * KEYS <= O_AT, "TMEM");
 };
 constexpr float RESCALE_AT = 8.0f;
-constexpr int PAGED_WAIT = 5 << 8;   // (what a wait was for is not reported: any number that is not 0)
 
 // A warp waits until phase number `count` of the barrier has ended (false: gave up).  All lanes look: a look suspends whoever looks, so that a lane which looks for the
 // others parts from them, and what follows a wait - accesses to TMEM, products, operands in uniform registers - is for a warp in step.
-PG_DEVINL bool wait_warp(uint64_t* bar, int count, volatile int* gave_up) {
-    const bool ok = __all_sync(~0u, dense::mbar_wait_bounded(bar, (uint32_t)count & 1, gave_up, PAGED_WAIT));
+PG_DEVINL bool wait_warp(uint64_t* bar, int count, volatile int* gave_up, int what) {
+    const bool ok = __all_sync(~0u, dense::mbar_wait_bounded(bar, (uint32_t)count & 1, gave_up, dense::TG_PAGED + what));
     __syncwarp();
     return ok;
 }
@@ -55,7 +57,7 @@ PG_DEVINL bool wait_part_lane(uint64_t* bar, uint32_t parity, uint64_t* flips, v
         if (now != phase) { phase = now; from = dense::now_ns(); i = 0; }
         else if (i >= dense::TG_LEAST_TRIES && dense::now_ns() - from >= dense::TG_WAIT_NS) break;
     }
-    if (!*gave_up) *gave_up = PAGED_WAIT;
+    if (!*gave_up) *gave_up = dense::TG_PAGED + dense::TG_PART;
     return false;
 }
 PG_DEVINL bool wait_part(uint64_t* bar, int count, uint64_t* flips, volatile int* gave_up) {
@@ -136,6 +138,30 @@ PG_DEVINL void tmem_store32(uint32_t at, const uint32_t (&v)[32]) {
         : "memory");
 }
 PG_DEVINL void tmem_stored() { __syncwarp(); asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+// Where a kernel that gave up says so: a word of the process in mapped host memory, which the next call reads
+struct GaveUpWord {
+    std::atomic<int*> at{nullptr};
+    std::mutex making;
+    int* get() {   // null: there is no memory for it
+        if (int* p = at.load(std::memory_order_acquire)) return p;
+        std::lock_guard<std::mutex> hold(making);
+        if (int* p = at.load(std::memory_order_acquire)) return p;
+        void* p = nullptr;
+        cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;   // (the call may be captured; this is not part of it)
+        cudaThreadExchangeStreamCaptureMode(&mode);
+        const cudaError_t e = cudaHostAlloc(&p, sizeof(int), cudaHostAllocPortable | cudaHostAllocMapped);   // (the same address on every device)
+        cudaThreadExchangeStreamCaptureMode(&mode);
+        if (e != cudaSuccess) { cudaGetLastError(); return nullptr; }
+        *(int*)p = 0;
+        at.store((int*)p, std::memory_order_release);
+        return (int*)p;
+    }
+    int take() {   // what a kernel has written, once
+        int* p = at.load(std::memory_order_acquire);
+        return p && *(volatile int*)p ? __atomic_exchange_n(p, 0, __ATOMIC_ACQ_REL) : 0;
+    }
+};
 
 // shared memory besides the operands
 template <typename T, int DP> struct TensorShared {
@@ -260,7 +286,7 @@ __global__ void __launch_bounds__(384, 1) rows128_kernel(const __grid_constant__
                 if (!looks_free(&sh.empty[slot], (int)round + 1)) {   // (nothing that has landed waits for a slot to come free)
                     copy_wait<0>();
                     report(n);
-                    ok = wait_warp(&sh.empty[slot], (int)round + 1, gave_up);
+                    ok = wait_warp(&sh.empty[slot], (int)round + 1, gave_up, dense::TG_FREE);
                     if (!ok) return;
                 }
                 if (boxed) {
@@ -330,7 +356,7 @@ __global__ void __launch_bounds__(384, 1) rows128_kernel(const __grid_constant__
             };
             do {
                 enter();
-                if (part > 0) ok = ok && wait_warp(&sh.queries_read, part - 1, gave_up);
+                if (part > 0) ok = ok && wait_warp(&sh.queries_read, part - 1, gave_up, dense::TG_QUERIES_READ);
                 if (ok && boxes.q_tokens) {   // the queries: rows are tokens x the heads of a group, which one box holds (rows behind the unit's own are some others', or zeros)
                     if (mine == 0 && lane == 0) {
                         const int token = (int)(w.b < 0 ? 0 : w.s.first) + w.row_tile * S::ROWS / p.group;
@@ -411,7 +437,7 @@ __global__ void __launch_bounds__(384, 1) rows128_kernel(const __grid_constant__
             int w_count[4] = {0, 0, 0, 0}, part = 0;   // sets of weights taken
             bool ok = true;
             auto take = [&]() {
-                ok = ok && wait_warp(&sh.full[n], (int)round, gave_up);
+                ok = ok && wait_warp(&sh.full[n], (int)round, gave_up, dense::TG_FULL);
                 tmem_after();
                 const uint32_t slot = n;
                 if (++n == S::SLOTS) { n = 0; round++; }
@@ -429,8 +455,8 @@ __global__ void __launch_bounds__(384, 1) rows128_kernel(const __grid_constant__
             };
             auto sums = [&](int block, int j, uint32_t slot) {
                 const int set = 2 * block + (j & 1);
-                if (j == 0 && part > 0) ok = ok && wait_warp(&sh.read[block], part - 1, gave_up);
-                ok = ok && wait_warp(&sh.weights[set], w_count[set]++, gave_up);
+                if (j == 0 && part > 0) ok = ok && wait_warp(&sh.read[block], part - 1, gave_up, dense::TG_VALUES_READ);
+                ok = ok && wait_warp(&sh.weights[set], w_count[set]++, gave_up, dense::TG_WEIGHTS);
                 if (!ok) return;
                 tmem_after();
                 // 16 keys a step: two groups of 8 rows of 128 bytes; from 64 columns to the next: a box
@@ -442,7 +468,7 @@ __global__ void __launch_bounds__(384, 1) rows128_kernel(const __grid_constant__
             };
             do {   // operand tiles come as K0 K1 V0 K2 V1 ...: the scores of tile j + 2 follow the sums of tile j into the same set
                 enter();
-                ok = ok && wait_warp(&sh.queries, part, gave_up);
+                ok = ok && wait_warp(&sh.queries, part, gave_up, dense::TG_QUERIES);
                 for (int j = 0; j < 2 && j < tiles; j++) {
                     const uint32_t keys = take();
                     if (!ok) break;
@@ -469,7 +495,7 @@ __global__ void __launch_bounds__(384, 1) rows128_kernel(const __grid_constant__
                 part++;
             } while (ok && leave());
             // the last commit is that of the last values' slot: none may arrive after the CTA has ended
-            if (ok) ok = wait_warp(&sh.empty[n == 0 ? S::SLOTS - 1 : n - 1], (int)(n == 0 ? round - 1 : round), gave_up);
+            if (ok) ok = wait_warp(&sh.empty[n == 0 ? S::SLOTS - 1 : n - 1], (int)(n == 0 ? round - 1 : round), gave_up, dense::TG_FREE);
             if (!ok)   // gave up: products already issued may still run; they get a millisecond to end before shared memory and TMEM go away
                 for (int i = 0; i < 1000; i++) __nanosleep(1000);
         }
@@ -491,7 +517,7 @@ __global__ void __launch_bounds__(384, 1) rows128_kernel(const __grid_constant__
                 const int least = w.b < 0 ? w.keys : unit_row(p, l, w, group * S::BLOCK).keys;   // (rows that come later see more)
                 for (int j = 0; j < tiles && ok; j++) {
                     const int set = 2 * group + (j & 1), key0 = (w.tile + j) * S::KEYS, known = (k_count + j) % S::RING;
-                    ok = wait_warp(&sh.known[known], (k_count + j) / S::RING, gave_up) && wait_warp(&sh.scores[set], s_count[j & 1] + (j >> 1), gave_up);
+                    ok = wait_warp(&sh.known[known], (k_count + j) / S::RING, gave_up, dense::TG_PLACES) && wait_warp(&sh.scores[set], s_count[j & 1] + (j >> 1), gave_up, dense::TG_SCORES);
                     if (!ok) break;
                     tmem_after();
                     const uint32_t at = tmem + lanes + (uint32_t)set * S::KEYS;
@@ -532,7 +558,7 @@ __global__ void __launch_bounds__(384, 1) rows128_kernel(const __grid_constant__
                     if (__any_sync(~0u, top > m + RESCALE_AT || (m == -INFINITY && top > m))) {
                         const float now = fmaxf(m, top), corr = ex2(m - (now == -INFINITY ? 0.0f : now));
                         if (j > 0) {
-                            ok = wait_warp(&sh.summed[2 * group + ((j - 1) & 1)], s_count[(j - 1) & 1] + ((j - 1) >> 1), gave_up);
+                            ok = wait_warp(&sh.summed[2 * group + ((j - 1) & 1)], s_count[(j - 1) & 1] + ((j - 1) >> 1), gave_up, dense::TG_VALUES);
                             if (!ok) break;
                             tmem_after();
 #pragma unroll 1
@@ -603,7 +629,7 @@ __global__ void __launch_bounds__(384, 1) rows128_kernel(const __grid_constant__
                 // the part's rows
                 const int64_t slot = w.unit + blockIdx.x;
                 const bool whole = whole_unit(p, w, w.tile, w.tile + tiles - 1), is = x < used;
-                ok = ok && wait_warp(&sh.summed[2 * group + ((tiles - 1) & 1)], s_count[(tiles - 1) & 1] + ((tiles - 1) >> 1), gave_up);
+                ok = ok && wait_warp(&sh.summed[2 * group + ((tiles - 1) & 1)], s_count[(tiles - 1) & 1] + ((tiles - 1) >> 1), gave_up, dense::TG_VALUES);
                 if (ok) {
                     tmem_after();
                     if (!seen) sum = -1.0f;
@@ -672,6 +698,7 @@ __global__ void __launch_bounds__(384, 1) rows128_kernel(const __grid_constant__
         tmem_after();
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "n"(512) : "memory");
     }
+    if (threadIdx.x == 0 && *gave_up && p.err) *p.err = *gave_up;
     // Rows to be summed again, all parts once more: behind the last wait of the CTA, since this takes as long as it takes (128 rows of 64 columns over 150 thousand keys: seconds)
     if (warp >= 8 || !sh.spoiled || *gave_up) return;
     const int group = warp >> 2, row = threadIdx.x & 127;
