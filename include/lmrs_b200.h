@@ -214,7 +214,8 @@ typedef struct lmrs_b200_positions {
     const int32_t* data;
     int64_t axis, row;
 } lmrs_b200_positions_t;
-/* out = x turned by its rows' positions; out may be x itself */
+/* out = x turned by its rows' positions; out may be x itself (the same data and strides) and not lie over a part of it.  Arrays that interleave, as parts of one projection do, need equal
+ * strides to be told from arrays that lie over one another: here and below */
 int lmrs_b200_rope_axes(const lmrs_b200_rope_t* rope, int dtype, const lmrs_b200_rows_t* x, const lmrs_b200_rows_t* out, int64_t n_rows, int heads, int head_size,
                         const lmrs_b200_positions_t* pos, void* stream);
 
@@ -237,7 +238,7 @@ typedef struct lmrs_b200_batch {
     int32_t seqs, table_len, max_rows, prefix_len;
 } lmrs_b200_batch_t;
 /* Writes the rows k and v [n_rows][kv_heads][head_size] to their places in the pages, k turned; with q, also q_out = q turned ([n_rows][q_heads]
- * [head_size]; q_out may be q).  rope NULL: nothing is turned (then q is refused).  pos NULL: the position of a row is prefix_len + its index on every axis.
+ * [head_size]; q_out may be q itself, and lies over neither k nor v).  rope NULL: nothing is turned (then q is refused).  pos NULL: the position of a row is prefix_len + its index on every axis.
  * Padding rows are turned in q_out and written nowhere else.  Two rows with one place: either's elements. */
 int lmrs_b200_paged_append(const lmrs_b200_pages_t* pages, const lmrs_b200_batch_t* batch, int64_t n_rows, const lmrs_b200_rows_t* k, const lmrs_b200_rows_t* v,
                            const lmrs_b200_rope_t* rope, const lmrs_b200_positions_t* pos, const lmrs_b200_rows_t* q, const lmrs_b200_rows_t* q_out, int q_heads, void* stream);

@@ -61,6 +61,33 @@ std::string bad_rows(const lmrs_b200_rows_t* r, const char* name, int dtype, int
     if (!on_device(r->data, device)) return std::string(name) + " is not memory of the current device";
     return "";
 }
+// Do two arrays of a call share bytes?  Exact for equal strides (also where they interleave, as parts of one projection do): the second is the first moved by d elements, so they meet if
+// d + i row + j head comes within a head's size of 0 for distances i, j that rows and heads can have.  With other strides, arrays whose extents meet count as meeting.
+bool meet(const lmrs_b200_rows_t* a, int64_t a_heads, const lmrs_b200_rows_t* b, int64_t b_heads, int64_t n_rows, int64_t head_size, int dtype) {
+    if (n_rows < 1 || a_heads < 1 || b_heads < 1) return false;
+    const int64_t size = (int64_t)size_of(dtype);
+    int64_t a_row = a->row, a_head = a->head, b_row = b->row, b_head = b->head;
+    if (n_rows == 1) a_row = b_row = 0;   // (strides that nothing is reached by)
+    if (a_heads == 1) a_head = b_heads == 1 ? 0 : b_head;
+    if (b_heads == 1) b_head = a_head;
+    typedef __int128 wide;
+    const wide a0 = (wide)(uintptr_t)a->data, b0 = (wide)(uintptr_t)b->data;
+    if (a0 + ((wide)(n_rows - 1) * a_row + (wide)(a_heads - 1) * a_head + head_size) * size <= b0 || b0 + ((wide)(n_rows - 1) * b_row + (wide)(b_heads - 1) * b_head + head_size) * size <= a0) return false;
+    if (a_row != b_row || a_head != b_head || (a_row == 0 && n_rows > 1)) return true;
+    const wide d = b0 - a0, row = (wide)a_row * size, near = (wide)head_size * size;   // in bytes: the arrays may lie any number of them apart
+    for (int64_t j = -(a_heads - 1); j < b_heads; j++) {
+        const wide at = d + (wide)j * a_head * size;   // + i row for i in -(n_rows - 1) .. n_rows - 1: the nearest to 0 from either side
+        wide i = row ? -at / row : 0;
+        for (wide k = i - 1; k <= i + 1; k++) {
+            const wide t = at + (k < 1 - (wide)n_rows ? 1 - (wide)n_rows : k > (wide)n_rows - 1 ? (wide)n_rows - 1 : k) * row;
+            if (t < near && -t < near) return true;
+        }
+    }
+    return false;
+}
+bool same(const lmrs_b200_rows_t* a, const lmrs_b200_rows_t* b, int64_t n_rows, int64_t heads) {   // the same elements in the same places
+    return a->data == b->data && (n_rows < 2 || a->row == b->row) && (heads < 2 || a->head == b->head);
+}
 std::string bad_ints(const int32_t* p, const char* name, int device) {
     if (!aligned(p, 4)) return std::string(name) + " does not lie on a boundary of its elements";
     return on_device(p, device) ? "" : std::string(name) + " is not memory of the current device";
@@ -154,6 +181,7 @@ extern "C" int lmrs_b200_rope_axes(const lmrs_b200_rope_t* rope, int dtype, cons
         if (n_rows < 0 || n_rows > 0x7fffffff || heads < 0 || heads > MAX_HEADS || head_size < 1 || head_size > 256)
             return refuse(me, "n_rows must be 0 .. 2^31 - 1, heads 0 .. 65535, head_size 1 .. 256");
         why = bad_rope(rope, head_size);
+        if (why.empty() && !same(x, out, n_rows, heads) && meet(x, heads, out, heads, n_rows, head_size, dtype)) why = "out lies over x without being x itself";
         if (!why.empty()) return refuse(me, why);
         int device = 0;
         const int sms = device_sms(me, &device);
@@ -187,6 +215,9 @@ extern "C" int lmrs_b200_paged_append(const lmrs_b200_pages_t* pages, const lmrs
         if (why.empty() && q && !rope) why = "q without rope";
         if (why.empty() && q && (q_heads < 1 || q_heads > MAX_HEADS)) why = "q_heads must be 1 .. 65535";
         if (why.empty() && rope) why = bad_rope(rope, pages->head_size);
+        if (why.empty() && q && !same(q, q_out, n_rows, q_heads) && meet(q, q_heads, q_out, q_heads, n_rows, pages->head_size, pages->dtype)) why = "q_out lies over q without being q itself";
+        if (why.empty() && q && k && v && (meet(k, pages->kv_heads, q_out, q_heads, n_rows, pages->head_size, pages->dtype) || meet(v, pages->kv_heads, q_out, q_heads, n_rows, pages->head_size, pages->dtype)))
+            why = "q_out lies over k or v";
         if (!why.empty()) return refuse(me, why);
         int device = 0;
         const int sms = device_sms(me, &device);
@@ -403,14 +434,15 @@ extern "C" int lmrs_b200_paged_attention(const lmrs_b200_pages_t* pages, const l
         if (why.empty() && !isfinite(scale)) why = "scale is not finite";
         if (why.empty() && !(softcap >= 0.0f && isfinite(softcap))) why = "softcap must be 0 (none) or positive";
         if (!why.empty()) return refuse(me, why);
+        const bool over = q && out && meet(q, q_heads, out, q_heads, n_rows, pages->head_size, pages->dtype);
         int device = 0;
-        if (!device_sms(me, &device)) return 1;
+        if (!(over && q->data != out->data) && !device_sms(me, &device)) return 1;   // (a call without a device says so, before it says that it is one in place)
+        if (over) return refuse(me, "out lies where q does, which is read until the call has ended");
         if (n_rows == 0 || batch->seqs == 0) return 0;
         const int dtype = pages->dtype;
         why = bad_batch_memory(batch, device);
         if (why.empty()) why = bad_rows(q, "q", dtype, device);
         if (why.empty()) why = bad_rows(out, "out", dtype, device);
-        if (why.empty() && out->data == q->data) why = "out lies where q does, which is read until the call has ended";
         if (why.empty() && lse && (!aligned(lse, 4) || !on_device(lse, device))) why = "lse is not memory of the current device";
         if (why.empty() && (!on_device(pages->k, device) || !on_device(pages->v, device))) why = "the pages are not memory of the current device";
         if (why.empty() && (!workspace || !aligned(workspace, 256) || !on_device(workspace, device))) why = "workspace is not memory of the current device on a 256-byte boundary";

@@ -200,7 +200,7 @@ class Batch:
 
 
 def rope_axes(x, pos, rope, out=None):
-    """x [rows, heads, head_size] turned by pos [axes, rows] (or [rows] for one axis); out may be x."""
+    """x [rows, heads, head_size] turned by pos [axes, rows] (or [rows] for one axis); out may be x, and not lie over a part of it."""
     if not isinstance(rope, RopeAxes):
         raise LmrsError("rope must be RopeAxes")
     if not isinstance(x, torch.Tensor) or x.dim() != 3 or x.dtype not in _DTYPES:

@@ -739,3 +739,26 @@ def test_a_part_of_seconds(paged):
     out, lse = paged.attention(paged.KVPages(k, v), batch, q, softcap=30.0, return_lse=True)
     want, want_lse, sizes = exact_of_repeats(k, v, 234375, n, kv, 1, q, 30.0)
     holds((out, lse), (want, want_lse, *repeats_tolerance(want, want_lse, sizes, 234376 * 512, size, 30.0)))
+
+
+def test_results_over_what_is_read(paged):
+    """a result shifted against its input is refused; one that interleaves with it (a projection's queries, turned in place, and a place for the results beside them) is not"""
+    m = Made(paged, 1, BF16, [40, 50, 3], [1, 1, 1], 16, 2, 2, 64, 20, one_each=True)
+    pages, batch = m.on_gpu()
+    buf = torch.zeros(4, 4, 64, dtype=BF16, device="cuda")
+    buf[:3] = m.q.cuda()
+    rope = paged.RopeAxes.sections(64, 1e4)
+    pos, k = torch.tensor([3, 5, 7], dtype=torch.int32, device="cuda"), torch.zeros(3, 2, 64, dtype=BF16, device="cuda")
+    for call in (lambda: paged.attention(pages, batch, buf[:3], out=buf[1:]), lambda: paged.rope_axes(buf[:3], pos, rope, out=buf[1:]), lambda: paged.append(pages, batch, k, k, rope=rope, q=buf[:3], q_out=buf[1:]),
+                 lambda: paged.append(pages, batch, buf[:3, 1:3], k, rope=rope, q=m.q.cuda(), q_out=buf[:3])):
+        with pytest.raises(paged.LmrsError, match="lies"):
+            call()
+    assert torch.equal(buf[:3], m.q.cuda())
+    wide = torch.randn(3, 12, 64, generator=gen(2)).to(BF16).cuda()   # 4 heads of q, 2 of k, 2 of v, 4 of results
+    q, kk, v, out = wide[:, :4], wide[:, 4:6], wide[:, 6:8], wide[:, 8:]
+    want = paged.rope_axes(q.contiguous(), pos, rope)
+    rest = wide[:, 4:8].clone()
+    assert paged.append(pages, batch, kk, v, rope=rope, pos=pos, q=q, q_out=q) is q
+    assert torch.equal(q, want) and torch.equal(wide[:, 4:8], rest)
+    paged.attention(pages, batch, q, out=out)
+    assert torch.equal(out, paged.attention(pages, batch, want)) and torch.equal(q, want)

@@ -156,3 +156,53 @@ def test_every_asynchronous_copy_belongs_to_a_group():
     for at in asked:
         end = min(p for p in handed_on if p > at)
         assert "copy_commit();" in src[at:end], src[at:at + 80]
+
+
+# q (or x, k) and a result: data in elements from one place, row and head strides, n_rows, heads; is it refused?
+LIE = [
+    ((0, 256, 64), (0, 256, 64), 3, 4, "itself"), ((0, 256, 64), (256, 256, 64), 3, 4, True), ((0, 256, 64), (768, 256, 64), 3, 4, False), ((768, 256, 64), (0, 256, 64), 3, 4, False),
+    ((0, 256, 64), (8, 256, 64), 3, 4, True), ((767, 256, 64), (0, 256, 64), 3, 4, True), ((0, 512, 64), (256, 512, 64), 3, 4, False), ((0, 512, 64), (255, 512, 64), 3, 4, True), ((256, 512, 64), (0, 512, 64), 3, 4, False),
+    ((0, 512, 128), (64, 512, 128), 3, 4, False), ((0, 512, 128), (63, 512, 128), 3, 4, True), ((0, 64, 64 * 9), (64 * 3, 64, 64 * 9), 3, 4, False), ((0, 64, 64 * 9), (64 * 2, 64, 64 * 9), 3, 4, True),
+    ((0, 256, 64), (0, 64, 192), 3, 4, True), ((0, 256, 64), (0, 7, 64), 1, 4, "itself"), ((0, 999, 64), (256, 1, 64), 1, 4, False), ((0, 999, 64), (192, 1, 64), 1, 4, True), ((0, 64, 5), (0, 64, 7), 3, 1, "itself"),
+    ((0, 128, 5), (64, 128, 7), 3, 1, False), ((0, 128, 5), (32, 128, 7), 3, 1, True), ((0, 0, 64), (512, 256, 64), 3, 4, False), ((0, 0, 64), (128, 256, 64), 3, 4, True), ((0, 300, 64), (60 * 300, 300, 64), 60, 4, False),
+    ((0, 300, 64), (59 * 300, 300, 64), 60, 4, True), ((0, 2 ** 40, 2 ** 35), (2 ** 20, 2 ** 40, 2 ** 35), 60, 4, False),
+]
+
+
+@pytest.mark.parametrize("a, b, n, heads, lies", LIE, ids=str)
+def test_results_that_lie_over_what_is_read(paged, gpu_lib, a, b, n, heads, lies):
+    """a shifted result is refused, an interleaved one is not, wherever rows and heads lie (held against the elements themselves where they are few)"""
+    L = gpu_lib.lib()
+    base = 1 << 44
+    x, y = (paged._Rows(base + 2 * t[0], t[1], t[2]) for t in (a, b))
+    if max(a + b) < 10 ** 6:
+        places = [{t[0] + r * t[1] + h * t[2] + e for r in range(n) for h in range(heads) for e in range(64)} for t in (a, b)]
+        meet = bool(places[0] & places[1])
+        assert meet == bool(lies)
+    rope, pos = paged.RopeAxes([1.0] * 32)._c, paged._Positions(P, n, 1)
+    L.lmrs_b200_rope_axes(C.byref(rope), 0, C.byref(x), C.byref(y), n, heads, 64, C.byref(pos), None)
+    assert (b"lies over x" in L.lmrs_b200_last_error()) == (lies is True)
+    pg, bt = _pages(paged, kv_heads=1), _batch(paged, seqs=n)
+    far = paged._Rows(1 << 50, 64, 64)
+    L.lmrs_b200_paged_attention(C.byref(pg), C.byref(bt), n, C.byref(x), C.byref(y), heads, 0.125, 0.0, None, P, 1 << 30, None)
+    if a[0] != b[0] or torch.cuda.is_available():   # (in one place: asked for behind the device)
+        assert (b"lies where q does" in L.lmrs_b200_last_error()) == bool(lies)
+    L.lmrs_b200_paged_append(C.byref(pg), C.byref(bt), n, C.byref(far), C.byref(far), C.byref(rope), None, C.byref(x), C.byref(y), heads, None)
+    assert (b"lies over q" in L.lmrs_b200_last_error()) == (lies is True)
+    if heads > 1:
+        pg = _pages(paged, kv_heads=heads)
+        for k, v in ((x, far), (far, x)):
+            L.lmrs_b200_paged_append(C.byref(pg), C.byref(bt), n, C.byref(k), C.byref(v), C.byref(rope), None, C.byref(y), C.byref(y), heads, None)
+            assert (b"lies over k or v" in L.lmrs_b200_last_error()) == bool(lies)
+
+
+def test_one_projection_of_queries_keys_and_values(paged, gpu_lib):
+    """q, k and v beside one another in the rows of one array, queries turned in place"""
+    L = gpu_lib.lib()
+    base, n = 1 << 44, 5
+    for heads, kv in ((8, 2), (4, 4), (6, 1), (1, 1)):
+        width = (heads + 2 * kv) * 64
+        q, k, v = (paged._Rows(base + 2 * 64 * at, width, 64) for at in (0, heads, heads + kv))
+        pg, bt, rope = _pages(paged, kv_heads=kv), _batch(paged, seqs=n), paged.RopeAxes([1.0] * 32)._c
+        L.lmrs_b200_paged_append(C.byref(pg), C.byref(bt), n, C.byref(k), C.byref(v), C.byref(rope), None, C.byref(q), C.byref(q), heads, None)
+        assert b"lies" not in L.lmrs_b200_last_error()
