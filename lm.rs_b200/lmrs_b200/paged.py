@@ -104,7 +104,8 @@ def _positions(pos, axes, rows, device):
     raise LmrsError(f"pos must be [{axes}, {rows}], not {list(shape)}")
 
 
-_stream = torch._C._cuda_getCurrentRawStream   # torch.cuda.current_stream(device).cuda_stream without the objects (2 us of a call's 10)
+# torch.cuda.current_stream(device).cuda_stream without the objects (2 us of a call's 10), where torch has it: a build without CUDA imports this and is refused by the calls
+_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda index: torch.cuda.current_stream(index).cuda_stream)
 _byref = C.byref
 
 

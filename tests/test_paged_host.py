@@ -206,3 +206,18 @@ def test_one_projection_of_queries_keys_and_values(paged, gpu_lib):
         pg, bt, rope = _pages(paged, kv_heads=kv), _batch(paged, seqs=n), paged.RopeAxes([1.0] * 32)._c
         L.lmrs_b200_paged_append(C.byref(pg), C.byref(bt), n, C.byref(k), C.byref(v), C.byref(rope), None, C.byref(q), C.byref(q), heads, None)
         assert b"lies" not in L.lmrs_b200_last_error()
+
+
+def test_a_torch_without_cuda_imports(paged):
+    """(it has no name for the raw stream; what needs a GPU says so)"""
+    import os
+    import subprocess
+    import sys
+    code = ("import sys, torch; sys.path.insert(0, sys.argv[1])\n"
+            "if hasattr(torch._C, '_cuda_getCurrentRawStream'): del torch._C._cuda_getCurrentRawStream\n"
+            "from lmrs_b200 import paged\n"
+            "try: paged.rope_axes(torch.zeros(2, 3, 8), torch.zeros(2, dtype=torch.int32), paged.RopeAxes([1.0]))\n"
+            "except paged.LmrsError as e: print(e)\n")
+    lib = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "lm.rs_b200")
+    r = subprocess.run([sys.executable, "-c", code, lib], capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0 and "must be a tensor on a GPU" in r.stdout, r.stderr[-500:]
