@@ -1,6 +1,6 @@
 """Many sequences at once: rotary positions with several axes, keys and values in pages, and attention over the pages with a prefix that all
 sequences share (include/lmrs_b200.h, "many sequences at once").  Torch tensors on a GPU, the current stream of their device; nothing is copied to
-the host, and calls can be captured into CUDA graphs.
+the host, and calls can be captured into CUDA graphs.  Nothing here has a backward pass: tensors that require gradients are refused while torch records them.
 
     rope  = RopeAxes(freq, axis)                        # which axis' position turns which pair, and how fast
     pages = KVPages(k, v)                               # [pages, page_size, kv_heads, head_size] each
@@ -61,11 +61,19 @@ def _gpu(t, name, device):
         raise LmrsError(f"{name} lies on {t.device}, other arrays of the call on {device}")
 
 
+def _no_gradients(t, name):
+    """nothing here has a backward pass: a history that a call would drop is refused"""
+    if torch.is_grad_enabled():
+        raise LmrsError(f"{name} requires a gradient, and nothing here has a backward pass: call under torch.no_grad(), or pass {name}.detach()")
+
+
 # (these run in every call: messages are made only where one is raised)
 def _heads(t, name, device, dtype, rows, heads, size, out=False):
     """t as the library takes it, checked: [rows, heads, size]"""
     if not isinstance(t, torch.Tensor) or not t.is_cuda or t.device != device:
         _gpu(t, name, device)
+    if t.requires_grad:
+        _no_gradients(t, name)
     if t.dtype != dtype:
         raise LmrsError(f"{name} is {t.dtype}, other arrays of the call {dtype}")
     if t.shape != (rows, heads, size):
@@ -153,6 +161,8 @@ class KVPages:
         _need(k.dim() == 4 and k.shape == v.shape, f"k and v must be [pages, page_size, kv_heads, head_size] alike, not {list(k.shape)} and {list(v.shape)}")
         _need(k.dtype in _DTYPES and k.dtype == v.dtype, f"k and v must both be bfloat16, float16 or float32, not {k.dtype} and {v.dtype}")
         for t, name in ((k, "k"), (v, "v")):
+            if t.requires_grad:
+                _no_gradients(t, name)
             _need(t.stride(3) == 1 or t.shape[3] == 1, f"the elements of a head of {name} must lie next to each other")
             _need(_disjoint(t), f"elements of {name} share their places")
         self.k, self.v, self.device, self.dtype = k, v, k.device, k.dtype

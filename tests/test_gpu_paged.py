@@ -762,3 +762,23 @@ def test_results_over_what_is_read(paged):
     assert torch.equal(q, want) and torch.equal(wide[:, 4:8], rest)
     paged.attention(pages, batch, q, out=out)
     assert torch.equal(out, paged.attention(pages, batch, want)) and torch.equal(q, want)
+
+
+def test_gradients_are_refused_not_dropped(paged):
+    m = Made(paged, 1, F32, [40, 50], [1, 1], 16, 2, 2, 64, 20, one_each=True)
+    pages, batch = m.on_gpu()
+    q, k = m.q.cuda(), torch.randn(2, 2, 64, generator=gen(1)).cuda()
+    rope, pos = paged.RopeAxes.sections(64, 1e4), torch.zeros(2, dtype=torch.int32, device="cuda")
+    p, kp = q.clone().requires_grad_(), k.clone().requires_grad_()
+    calls = (lambda t, u: paged.rope_axes(t, pos, rope), lambda t, u: paged.attention(pages, batch, t), lambda t, u: paged.append(pages, batch, u, k, rope=rope, q=q), lambda t, u: paged.append(pages, batch, k, u),
+             lambda t, u: paged.append(pages, batch, k, k, rope=rope, q=t), lambda t, u: paged.KVPages(u[:, None], u[:, None]), lambda t, u: paged.rope_axes(t * 2.0, pos, rope))
+    for call in calls:
+        with pytest.raises(paged.LmrsError, match="gradient"):
+            call(p, kp)
+        with torch.no_grad():
+            got = call(p, kp)
+        want = call(q, k)
+        assert not isinstance(want, torch.Tensor) or (torch.equal(got, want) and not got.requires_grad)
+        call(p.detach(), kp.detach())
+    with pytest.raises(paged.LmrsError, match="out requires a gradient"):
+        paged.rope_axes(q, pos, rope, out=torch.zeros_like(q).requires_grad_())
