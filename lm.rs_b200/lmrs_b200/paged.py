@@ -165,6 +165,7 @@ class KVPages:
                 _no_gradients(t, name)
             _need(t.stride(3) == 1 or t.shape[3] == 1, f"the elements of a head of {name} must lie next to each other")
             _need(_disjoint(t), f"elements of {name} share their places")
+        _need(max(k.shape) < 1 << 31, f"a dimension of {list(k.shape)} is beyond 2^31 - 1")   # (ctypes would keep its lower 32 bits)
         self.k, self.v, self.device, self.dtype = k, v, k.device, k.dtype
         self.pages, self.page_size, self.kv_heads, self.head_size = k.shape
         self._c = _Pages(k.data_ptr(), v.data_ptr(), k.stride(0), k.stride(1), k.stride(2), v.stride(0), v.stride(1), v.stride(2), *k.shape, _DTYPES[k.dtype])
@@ -189,6 +190,7 @@ class Batch:
             _need(rows.dim() == 1 and rows.shape[0] == lens.shape[0] + 1 and (rows.stride(0) == 1 or rows.numel() < 2), f"rows must be [{lens.shape[0] + 1}], its elements next to each other")
         _need(int(max_rows) >= 1 and (rows is not None or int(max_rows) == 1), "max_rows must be positive, and 1 without rows")
         _need(prefix_len >= 0 and (prefix is not None or prefix_len == 0), "prefix_len without prefix")
+        _need(max(*tables.shape, int(max_rows), int(prefix_len)) < 1 << 31, "seqs, pages of a sequence, max_rows or prefix_len beyond 2^31 - 1")
         if prefix is not None:
             _ints(prefix, "prefix", device)
             _need(prefix.dim() == 1 and (prefix.stride(0) == 1 or prefix.numel() < 2), "prefix must be [pages], its elements next to each other")
@@ -217,6 +219,8 @@ def rope_axes(x, pos, rope, out=None):
     if not isinstance(x, torch.Tensor) or x.dim() != 3 or x.dtype not in _DTYPES:
         raise LmrsError("x must be a [rows, heads, head_size] tensor of bfloat16, float16 or float32")
     n, heads, size = x.shape
+    if heads > 65535:
+        raise LmrsError(f"{heads} heads: at most 65535")
     device, dtype = x.device, x.dtype
     if x.is_cuda and device.index != torch.cuda.current_device():
         with torch.cuda.device(device):
@@ -260,6 +264,8 @@ def append(pages, batch, k, v, rope=None, pos=None, q=None, q_out=None):
         if not isinstance(q, torch.Tensor) or q.dim() != 3:
             raise LmrsError("q must be a [rows, heads, head_size] tensor")
         heads = q.shape[1]
+        if heads > 65535:
+            raise LmrsError(f"{heads} heads: at most 65535")
         qr = _byref(_heads(q, "q", device, dtype, n, heads, size))
         if q_out is None:
             q_out, qo = _new(q)
@@ -284,6 +290,8 @@ def attention(pages, batch, q, out=None, scale=None, softcap=0.0, return_lse=Fal
     if not isinstance(q, torch.Tensor) or q.dim() != 3:
         raise LmrsError("q must be a [rows, heads, head_size] tensor")
     n, heads, size = q.shape
+    if heads > 65535:
+        raise LmrsError(f"{heads} heads: at most 65535")
     batch._for(pages, n)
     device, dtype = pages.device, pages.dtype
     if device.index != torch.cuda.current_device():

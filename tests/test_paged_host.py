@@ -221,3 +221,20 @@ def test_a_torch_without_cuda_imports(paged):
     lib = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "lm.rs_b200")
     r = subprocess.run([sys.executable, "-c", code, lib], capture_output=True, text=True, timeout=300)
     assert r.returncode == 0 and "must be a tensor on a GPU" in r.stdout, r.stderr[-500:]
+
+
+def test_numbers_that_32_bits_do_not_hold(paged, monkeypatch):
+    """refused, and not taken for their lower 32 bits (tensors without memory stand for those of a GPU)"""
+    monkeypatch.setattr(paged, "_gpu", lambda t, name, device: None)
+    i32 = dict(dtype=torch.int32)
+    lens, tables, prefix = torch.zeros(2, **i32), torch.zeros(2, 3, **i32), torch.zeros(4, **i32)
+    paged.Batch(lens, tables, rows=torch.zeros(3, **i32), max_rows=2 ** 31 - 1, prefix=prefix, prefix_len=2 ** 31 - 1)
+    for kw in (dict(max_rows=2 ** 32 + 1), dict(max_rows=2 ** 31), dict(prefix_len=2 ** 32 + 5), dict(tables=torch.empty(2, 2 ** 32 + 1, dtype=torch.int32, device="meta"))):
+        with pytest.raises(paged.LmrsError, match="2\\^31"):
+            paged.Batch(lens, **{"tables": tables, "rows": torch.zeros(3, **i32), "prefix": prefix, **kw})
+    for shape in ((2 ** 32 + 5, 1, 1, 1), (1, 2 ** 31, 1, 8)):
+        big = torch.empty(shape, dtype=torch.bfloat16, device="meta")
+        with pytest.raises(paged.LmrsError, match="2\\^31"):
+            paged.KVPages(big, big)
+    with pytest.raises(paged.LmrsError, match="heads"):
+        paged.rope_axes(torch.empty(1, 2 ** 32 + 4, 1, dtype=torch.bfloat16, device="meta"), torch.zeros(1, **i32), paged.RopeAxes([1.0]))
