@@ -264,6 +264,7 @@ static std::string bad_attention(const lmrs_b200_pages_t* pages, const lmrs_b200
     if (!why.empty()) return why;
     const int64_t vec = 16 / (int64_t)size_of(pages->dtype);
     if (pages->head_size % 8) return "head_size must be a multiple of 8";
+    if ((int64_t)batch->table_len * pages->page_size + batch->prefix_len > 0x7fffffff - AGAIN) return "prefix_len + table_len * page_size is beyond 2^31 - 129";   // (numbers of keys go up to the end of a tile)
     if (q_heads < 1 || q_heads > MAX_HEADS || q_heads % pages->kv_heads) return "q_heads must be a positive multiple of kv_heads, at most 65535";
     if (n_rows * q_heads > 0x40000000) return "n_rows * q_heads is beyond 2^30";
     if (!aligned(pages->k, 16) || !aligned(pages->v, 16) || pages->k_page % vec || pages->k_slot % vec || pages->k_head % vec || pages->v_page % vec || pages->v_slot % vec ||

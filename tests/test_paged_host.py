@@ -238,3 +238,12 @@ def test_numbers_that_32_bits_do_not_hold(paged, monkeypatch):
             paged.KVPages(big, big)
     with pytest.raises(paged.LmrsError, match="heads"):
         paged.rope_axes(torch.empty(1, 2 ** 32 + 4, 1, dtype=torch.bfloat16, device="meta"), torch.zeros(1, **i32), paged.RopeAxes([1.0]))
+
+
+def test_keys_up_to_the_end_of_32_bits(paged, gpu_lib):
+    """a tile's end is a number of 32 bits, too"""
+    L, size = gpu_lib.lib(), C.c_size_t()
+    most = 2 ** 31 - 129
+    for page, table, prefix, ok in ((most, 1, 0, True), (most + 1, 1, 0, False), (2 ** 31 - 1, 1, 0, False), (16, 4, most - 64, True), (16, 4, most - 63, False), (16, 4, 2 ** 31 - 1 - 64, False)):
+        pg, bt = _pages(paged, page_size=page), _batch(paged, table_len=table, prefix=P, prefix_len=prefix)
+        assert (L.lmrs_b200_paged_attention_workspace(C.byref(pg), C.byref(bt), 3, 4, C.byref(size)) == 0) == ok, (page, table, prefix)
