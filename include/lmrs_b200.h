@@ -231,7 +231,7 @@ typedef struct lmrs_b200_pages {
  * The prefix_len tokens of the pages that `prefix` lists come before every sequence's own (prefix NULL: none).
  * lens, rows, tables and prefix are int32 in device memory and read by the kernels, so a captured call follows what is written there.  An entry of
  * tables or prefix outside 0 .. pages - 1 is no page: what would lie there is neither written nor seen, nor is what lies beyond table_len pages.
- * max_rows: most rows of one sequence (it chooses the kernels; a wrong number costs time, and results differ by the kernels' roundings only). */
+ * seqs: up to 2^30.  max_rows: most rows of one sequence (it chooses the kernels; a wrong number costs time, and results differ by the kernels' roundings only). */
 typedef struct lmrs_b200_batch {
     const int32_t *lens, *rows, *tables, *prefix;
     int64_t table_stride;

@@ -107,7 +107,7 @@ std::string bad_pages(const lmrs_b200_pages_t* p) {
 }
 std::string bad_batch(const lmrs_b200_batch_t* b, int64_t n_rows, int page_size) {
     if (!b) return "null batch";
-    if (b->seqs < 0 || n_rows < 0 || n_rows > 0x7fffffff) return "seqs and n_rows must be 0 .. 2^31 - 1";
+    if (b->seqs < 0 || b->seqs > 1 << 30 || n_rows < 0 || n_rows > 0x7fffffff) return "seqs must be 0 .. 2^30, n_rows 0 .. 2^31 - 1";   // (sequences are looked at in strides of up to 384 threads)
     if (b->table_len < 0 || b->table_stride < 0) return "negative table_len or table_stride";
     if (b->prefix_len < 0 || (b->prefix_len > 0 && !b->prefix)) return "prefix_len without prefix";
     if ((int64_t)b->table_len * page_size + b->prefix_len > 0x7fffffff) return "prefix_len + table_len * page_size is beyond 2^31 - 1";

@@ -247,3 +247,10 @@ def test_keys_up_to_the_end_of_32_bits(paged, gpu_lib):
     for page, table, prefix, ok in ((most, 1, 0, True), (most + 1, 1, 0, False), (2 ** 31 - 1, 1, 0, False), (16, 4, most - 64, True), (16, 4, most - 63, False), (16, 4, 2 ** 31 - 1 - 64, False)):
         pg, bt = _pages(paged, page_size=page), _batch(paged, table_len=table, prefix=P, prefix_len=prefix)
         assert (L.lmrs_b200_paged_attention_workspace(C.byref(pg), C.byref(bt), 3, 4, C.byref(size)) == 0) == ok, (page, table, prefix)
+
+
+def test_sequences_up_to_2_to_the_30(paged, gpu_lib):
+    L, size, pg = gpu_lib.lib(), C.c_size_t(), _pages(paged)
+    for seqs, ok in ((1 << 30, True), ((1 << 30) + 1, False), (2 ** 31 - 1, False)):
+        bt = _batch(paged, seqs=seqs, rows=P)
+        assert (L.lmrs_b200_paged_attention_workspace(C.byref(pg), C.byref(bt), 3, 4, C.byref(size)) == 0) == ok
