@@ -1,5 +1,6 @@
 // paged.cu -- entry points of include/lmrs_b200.h for many sequences at once: checks of the arguments, choice of the kernels, launches.
 // Device pointers, the caller's stream; nothing here allocates, synchronises or remembers anything from one call to the next.
+#include <float.h>
 #include <math.h>
 
 #include <algorithm>
@@ -462,7 +463,9 @@ extern "C" int lmrs_b200_paged_attention(const lmrs_b200_pages_t* pages, const l
             p.k_page = pages->k_page; p.k_slot = pages->k_slot; p.k_head = pages->k_head;
             p.v_page = pages->v_page; p.v_slot = pages->v_slot; p.v_head = pages->v_head;
             p.kv_heads = pages->kv_heads; p.q_heads = q_heads; p.head_size = pages->head_size; p.group = q_heads / pages->kv_heads;
-            p.scale2 = scale * LOG2E; p.softcap = softcap; p.cap_in = softcap > 0.0f ? scale / softcap : 0.0f; p.lse = lse;
+            // At the ends of float32: a cap beyond 2^100 is one of 2^100 (scores of up to 2^88 are not moved by either, and its product with log2 e is finite), and no score is 0 times infinity
+            const float cap = std::min(softcap, 0x1p100f);
+            p.scale2 = std::max(-FLT_MAX, std::min(FLT_MAX, scale * LOG2E)); p.softcap = cap; p.cap_in = cap > 0.0f ? std::max(-FLT_MAX, std::min(FLT_MAX, scale / cap)) : 0.0f; p.lse = lse;
             p.q_wide = vectors(q, dtype);
             p.out_wide = aligned(out->data, 4 * sizeof(T)) && out->row % 4 == 0 && out->head % 4 == 0;
             p.whole = batch->prefix_len == 0;

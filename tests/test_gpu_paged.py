@@ -782,3 +782,19 @@ def test_gradients_are_refused_not_dropped(paged):
         call(p.detach(), kp.detach())
     with pytest.raises(paged.LmrsError, match="out requires a gradient"):
         paged.rope_axes(q, pos, rope, out=torch.zeros_like(q).requires_grad_())
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16, F32], ids=str)
+def test_caps_and_scales_at_the_ends_of_float32(paged, dtype):
+    """a cap so small that every score is 0, one so large that none is capped, a scale at the end: keys of zeros among the others, and queries of zeros"""
+    m = Made(paged, 9, dtype, [70, 90, 1], [1, 40, 1], 16, 2, 2, 64, 50)
+    for b, x in ((0, 3), (0, 69), (1, 5), (1, 60)):
+        m.k[oracle.place(m.tables[b], len(m.k), 16, x)] = 0.0
+    m.q[[0, 7]] = 0.0
+    pages, batch = m.on_gpu()
+    q = m.q.cuda()
+    for cap in (1e-45, 1e-40, 3e38):
+        out, lse = paged.attention(pages, batch, q, softcap=cap, return_lse=True)
+        m.check(out, lse, cap=cap if cap < 1 else 0.0)
+    rows = (q == 0).flatten(1).all(1)   # whatever the scale, a row of zeros weighs all keys alike
+    assert torch.equal(paged.attention(pages, batch, q, scale=3e38)[rows], paged.attention(pages, batch, q)[rows])
