@@ -149,6 +149,28 @@ int parts_of(int64_t n_rows, int64_t pieces, int sms) {
 }
 unsigned warps_grid(int64_t warps, int sms) { return (unsigned)std::min<int64_t>((warps + ROW_WARPS - 1) / ROW_WARPS, (int64_t)sms * ROW_CTAS); }
 
+// freq / 2 pi modulo 1, in 2^-64, to the nearest: off by at most 1/2 + |freq| 2^-65 of that.  freq = m 2^e with 53 bits in m, times 1 / 2 pi in 2^-128 (rounded; arctangents of 1/5 and
+// 1/239 give its digits, as the tests do), is a whole number of 192 bits in 2^(e - 128); what is wanted are its 64 bits below the point.
+uint64_t turns_of(double freq) {
+    constexpr uint64_t HIGH = 0x28be60db9391054aull, LOW = 0x7f09d5f47d4d3770ull;
+    int e = 0;
+    const uint64_t m = (uint64_t)ldexp(frexp(fabs(freq), &e), 53);
+    e -= 53;
+    const unsigned __int128 low = (unsigned __int128)m * LOW, high = (unsigned __int128)m * HIGH + (uint64_t)(low >> 64);
+    const uint64_t words[3] = {(uint64_t)low, (uint64_t)high, (uint64_t)(high >> 64)};
+    auto bits = [&](int from) {   // 64 bits of the product from bit `from` on
+        uint64_t r = 0;
+        for (int i = 0; i < 3; i++) {
+            const int at = 64 * i - from;
+            if (at > -64 && at < 64) r |= at < 0 ? words[i] >> -at : words[i] << at;
+        }
+        return r;
+    };
+    const int from = 64 - e;
+    const uint64_t t = bits(from) + (from > 0 ? bits(from - 1) & 1 : 0);   // (a whole turn is none)
+    return freq < 0 ? 0 - t : t;
+}
+
 }  // namespace
 
 extern "C" int lmrs_b200_rope_init(lmrs_b200_rope_t* out, const double* freq, const uint8_t* axis, int pairs, int layout) {
@@ -161,9 +183,7 @@ extern "C" int lmrs_b200_rope_init(lmrs_b200_rope_t* out, const double* freq, co
         r.layout = layout;
         for (int j = 0; j < pairs; j++) {
             if (!isfinite(freq[j])) return refuse("rope_init", "a frequency is not finite");
-            const long double turns = (long double)freq[j] / 6.283185307179586476925286766559005768L, part = turns - floorl(turns);
-            const long double scaled = floorl(ldexpl(part, 64) + 0.5L);
-            r.turns[j] = scaled >= ldexpl(1.0L, 64) ? 0 : (uint64_t)scaled;   // (a whole turn is none)
+            r.turns[j] = turns_of(freq[j]);
             r.axis[j] = axis ? axis[j] : 0;
             if (r.axis[j] >= r.axes) r.axes = r.axis[j] + 1;
         }

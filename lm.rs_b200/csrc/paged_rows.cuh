@@ -2,7 +2,8 @@
 //
 // Pair j of a head turns by t = position[axis j] * freq j.  An angle is wanted modulo a turn, and position * freq in f32 has lost it at
 // positions of some thousands; here freq / 2 pi is a 64-bit fraction of a turn (made once on the host) and the product wraps modulo 2^64, which is
-// modulo a turn, exactly: the angle is off by at most position * 2^-65 turns.  What is left after taking quarter turns off goes through f32.
+// modulo a turn, exactly: the angle is off by at most position * (2^-65 + |freq| 2^-129) turns, which is what the host rounds (turns_of).  What is left after taking quarter turns off goes
+// through f32.
 //
 // Both kernels are bound by the bytes of the rows (an angle serves every head of its row), or by one launch's latency where there are few.  A warp takes a row, or
 // some of its heads where rows are few: its lanes compute the row's cosines and sines once into the warp's part of shared memory, then walk the row in pieces.

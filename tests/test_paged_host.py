@@ -254,3 +254,28 @@ def test_sequences_up_to_2_to_the_30(paged, gpu_lib):
     for seqs, ok in ((1 << 30, True), ((1 << 30) + 1, False), (2 ** 31 - 1, False)):
         bt = _batch(paged, seqs=seqs, rows=P)
         assert (L.lmrs_b200_paged_attention_workspace(C.byref(pg), C.byref(bt), 3, 4, C.byref(size)) == 0) == ok
+
+
+def test_turns_to_the_last_bit(paged):
+    """against pi in whole numbers (Machin's formula): half a step of 2^-64, and what the 128 bits of 1 / 2 pi leave of large frequencies"""
+    import random
+    from fractions import Fraction
+    one = 1 << 1300
+
+    def arctan(x):
+        total, term, n = 0, one // x, 1
+        while term:
+            total += term // n if n % 4 == 1 else -(term // n)
+            term, n = term // (x * x), n + 2
+        return total
+
+    two_pi = Fraction(8 * (4 * arctan(5) - arctan(239)), one)
+    r = random.Random(1)
+    freq = [1.0, 0.5, 7.0, -0.25, 2 * math.pi, -2 * math.pi, 1e-6, 5e-324, 1e-300, 0.0, -0.0, 1e6, 1e15, 2.0 ** 60, 2.0 ** 64 + 2.0 ** 12, -3e17, 1e300, -1e300, 2.0 ** 128]
+    freq += [10000.0 ** (-2.0 * j / 128) for j in range(64)] + [math.ldexp(r.uniform(-1, 1), r.randint(-70, 70)) for _ in range(40)]
+    for at in range(0, len(freq), 100):
+        part = freq[at:at + 100]
+        c = paged.RopeAxes(part)._c
+        for j, f in enumerate(part):
+            off = (Fraction(int(c.turns[j]), 2 ** 64) - Fraction(f) / two_pi) % 1
+            assert min(off, 1 - off) * 2 ** 64 <= Fraction(1, 2) + Fraction(abs(f)) / 2 ** 65 + Fraction(1, 10 ** 6), f
