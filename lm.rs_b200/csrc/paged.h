@@ -56,18 +56,6 @@ PG_DEVINL int64_t slot_of(const int* table, int table_len, int page_size, int pa
     const int page = table[p];
     return page < 0 || page >= pages ? -1 : (int64_t)page * page_size + (x - p * page_size);
 }
-// the sequence of row r, found by all threads of a CTA (-1: behind the last one).  `found` in shared memory
-PG_DEVINL int seq_of_row(const Batch& s, int64_t r, int* found) {
-    if (!s.rows) return r < s.seqs ? (int)r : -1;
-    if (threadIdx.x == 0) *found = 0x7fffffff;
-    __syncthreads();
-    for (int b = threadIdx.x; b < s.seqs; b += blockDim.x)
-        if (s.rows[b] <= r && r < s.rows[b + 1]) atomicMin(found, b);   // (rows ascend, so that there is one)
-    __syncthreads();
-    const int b = *found;
-    __syncthreads();
-    return b == 0x7fffffff ? -1 : b;
-}
 
 }  // namespace paged
 }  // namespace lmrs
