@@ -314,7 +314,7 @@ void place_line(Line& l, int64_t rows, const lmrs_b200_pages_t* pages, char* bas
 // Which kernel takes what.  float32: rows16_kernel.  16-bit types: it depends on how often the keys would be read again.  rows16_kernel reads them once per 16
 // rows of a KV head and, with little to do, starts some 8 us sooner; rows128_kernel reads them once per 128 or 256 rows.  Measured on a B200 with rows16_kernel / rows128_kernel,
 // us a call, 8 KV heads:
-//   a sequence's own keys, 16 sequences behind 4000 keys, rows of a sequence and KV head:
+//   a sequence's own keys, 16 sequences behind up to 4000 keys (the others behind 1000 or more, with a third of the rows or more), rows of the longest sequence and a KV head:
 //     head 64:  32: 45 / 64   64: 80 / 76   128: 139 / 79      128:  32: 71 / 72   64: 130 / 84   128: 239 / 87      256:  8: 143 / 93   16: 148 / 96   32: 243 / 97
 //     (one sequence alone: 64: 22 / 23 at head 64, 28 / 26 at 128;  16: 31 / 32 and 8: 27 / 31 at 256)
 //   the prefix, rows of all sequences and a KV head behind a prefix of 512, 2048, 8192, 32768 keys:

@@ -364,9 +364,10 @@ PG_DEVINL void mma16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint
     asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
                  : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
-// Weights are rounded to the type of the values for the products (half a step of a weight that is at most 1 to 2^-9 of the row's sum, of either sign; the sums that
-// they are divided by are of the unrounded ones).  float16 keeps fewer small numbers: its weights are 2^7 times as large (m is 7 less), so that what a
-// weight loses below 2^-14 is 2^-32 of the largest at most.
+// Weights are rounded to the type of the values for the products, since the tensor cores take one type for both: each by half a step at most, 2^-8 of it in bf16 and 2^-11 in fp16, either way, so
+// that a result is off by that fraction of its weighted sizes where all of them go one way (measured against 64 bits: 0.0023 of a bf16 result, where rounding the result alone makes 0.0017). The sums that
+// they are divided by are of the unrounded ones. Here weights are at most 1; rows128_kernel, whose m may lag by RESCALE_AT, has up to 2^8. float16 keeps fewer small numbers: its weights are 2^7 times
+// as large (m is 7 less; up to 2^7 here, 2^15 there), so that what a weight loses below 2^-14 is 2^-32 of the largest at most.
 template <typename T> constexpr float WEIGHT_SHIFT = 0.0f;
 template <> constexpr float WEIGHT_SHIFT<__half> = 7.0f;
 

@@ -10,7 +10,7 @@
 //                    where pages have odd sizes, 16 bytes a thread with zeros for what is not there.  The places of a tile's keys are looked up by a thread each.
 //   warp 10          the products
 // o stays in TMEM for a whole part.  m is the largest score when it was last set; it is set anew, and o rescaled, only when a row's largest score has grown by
-// more than 2^8 (weights stay below 2^8 and sums are f32, so that nothing is lost), which is rare after the first tile.
+// more than 2^8 (weights stay below 2^8, fp16's below 2^15, and sums are f32, so that nothing is lost), which is rare after the first tile.
 // Measured on a B200, us: 512 rows of a KV head behind 32768 keys, 8 KV heads of 128, bf16: 110 (620 TFLOP/s; a library product reaches 1690).  256 rows behind
 // 8200, heads of 64: 28.  Rows of 12 prompts behind 2050, heads of 256, capped: 270 (the cap's tanh and one block of rows only).  What bounds it: no unit is half busy (tensor
 // cores 39 %, powers of two 29 %, issue slots 28 %, DRAM 16 %); it is the chain scores - TMEM - maximum - powers - TMEM - sums of a tile, two tiles of each block under way.
@@ -251,8 +251,8 @@ __global__ void __launch_bounds__(384, 1) rows128_kernel(const __grid_constant__
         if (w.tiles == 0) { left = 0; return false; }   // (the line ended early: lengths changed under the kernel)
         return true;
     };
-    // (Every thread keeps its registers.  Moved from the copying warps to the rows by setmaxnreg they were not safe: the compiler gave code of the copying warps
-    // more than was left to them)
+    // (Every thread keeps its registers.  Versions that moved some from the copying warps to the rows by setmaxnreg faulted, and had other faults as well; nothing shows that the compiler keeps code
+    // that follows below the number that is left, so it stays out)
     if (warp >= 8) {
         if (warp < 8 + S::COPIERS) {
             // ---- copies: each of the two warps half of every operand tile's rows, as far ahead as slots are free ----
