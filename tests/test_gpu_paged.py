@@ -798,3 +798,95 @@ def test_caps_and_scales_at_the_ends_of_float32(paged, dtype):
         m.check(out, lse, cap=cap if cap < 1 else 0.0)
     rows = (q == 0).flatten(1).all(1)   # whatever the scale, a row of zeros weighs all keys alike
     assert torch.equal(paged.attention(pages, batch, q, scale=3e38)[rows], paged.attention(pages, batch, q)[rows])
+
+
+def longer_and_shorter(m, seed):
+    """other lengths (none longer than its pages), the pages of two sequences of one length exchanged"""
+    r = random.Random(seed)
+    m.lens = [max(c, n - r.randrange(0, n // 2 + 1)) for n, c in zip(m.lens, m.counts)]
+    return torch.tensor(m.lens, dtype=torch.int32, device="cuda"), m.tables[torch.randperm(len(m.lens), generator=gen(seed))]
+
+
+@pytest.mark.parametrize("what", ["prefix", "own"])
+def test_tensor_core_calls_on_two_streams_and_two_graphs(paged, what):
+    """a prefix on the tensor cores, then the own keys on others, then the join, each launched before the one in front of it has ended; or own keys of many rows on the tensor cores, then the join.
+    Two batches at the same time, eager and as graphs that are replayed together, lengths and pages changed between replays: each what it is alone, which is held against 64 bits"""
+    if what == "prefix":
+        made = [MadeThere(paged, s, BF16, [300] * 64, [1] * 64, 16, 8, 4, 64, 5120 + 100 * s) for s in (1, 2)]
+    else:
+        made = [MadeThere(paged, s, F16, [300] * 16, [20] * 16, 16, 8, 4, 128) for s in (3, 4)]
+    for m in made:   # (pages change hands: every length fits every row of the table)
+        m.k.nan_to_num_(0.5), m.v.nan_to_num_(0.5)
+    lens, tables = [m.batch.lens for m in made], [m.tables for m in made]
+
+    def call(i):
+        return paged.attention(made[i].pages, made[i].batch, made[i].q, return_lse=True)
+
+    streams, graphs, outs = [torch.cuda.Stream() for _ in made], [], []
+    for i in range(2):
+        call(i)
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            outs.append(call(i))
+        graphs.append(graph)
+    for step in range(6):
+        if step:
+            for i, m in enumerate(made):
+                new_lens, new_tables = longer_and_shorter(m, 10 * step + i)
+                lens[i].copy_(new_lens)
+                tables[i].copy_(new_tables.clone())
+        alone = [[t.clone() for t in call(i)] for i in range(2)]
+        for i, m in enumerate(made):
+            holds(alone[i], m.exact())
+        torch.cuda.synchronize()
+        got = [[], []]
+        for _ in range(10):
+            for i in range(2):
+                with torch.cuda.stream(streams[i]):
+                    got[i].append(call(i))
+        torch.cuda.synchronize()
+        assert all(torch.equal(g[j], alone[i][j]) for i in range(2) for g in got[i] for j in range(2))
+        for _ in range(10):
+            for o, l in outs:
+                o.fill_(9.0), l.fill_(9.0)
+            torch.cuda.synchronize()
+            for i in range(2):
+                with torch.cuda.stream(streams[i]):
+                    graphs[i].replay()
+            torch.cuda.synchronize()
+            assert all(torch.equal(outs[i][j], alone[i][j]) for i in range(2) for j in range(2))
+
+
+ROWS_AND_HEADS = [  # tokens before, rows of each sequence, page, kv heads, group, size, prefix, cap
+    (60, [40, 17], 16, 2, 4, 24, 300, 0.0), (100, [70] * 3, 32, 3, 2, 40, 0, 0.0), (200, [33] * 4, 8, 2, 2, 8, 90, 0.0), (90, [64, 100], 16, 2, 8, 56, 700, 20.0), (30, [130], 64, 1, 1, 16, 0, 0.0),
+    (500, [200] + [1] * 40, 16, 4, 4, 64, 0, 0.0), (500, [200] + [1] * 40, 16, 2, 4, 128, 600, 0.0), (300, [1, 1, 60, 1, 2, 90], 32, 2, 3, 96, 100, 0.0), (700, [512] + [1] * 20, 16, 2, 4, 64, 0, 0.0),
+    (100, [128, 100, 300], 16, 8, 4, 64, 0, 0.0), (100, [128, 100, 300], 16, 4, 1, 96, 0, 0.0), (100, [128, 100, 300], 16, 2, 4, 128, 0, 0.0), (64, [16] * 9, 16, 2, 1, 256, 200, 0.0),
+]
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16, F32], ids=str)
+@pytest.mark.parametrize("case", ROWS_AND_HEADS, ids=lambda c: f"past{c[0]}-rows{'+'.join(map(str, sorted(set(c[1]))))}-page{c[2]}-{c[3]}x{c[4]}x{c[5]}-prefix{c[6]}")
+def test_portions_beside_single_tokens_and_narrow_heads(paged, case, dtype):
+    """prompts' portions by themselves and with single tokens of other sequences in the same call, heads that fill a part of a box; and the same with a max_rows that is wrong in either direction"""
+    past, counts, page, kv, group, size, prefix, cap = case
+    m = MadeThere(paged, size + page, dtype, [past + c for c in counts], counts, page, kv, group, size, prefix)
+    exact = m.exact(cap)
+    for max_rows in (None, 1, 7, 100000):
+        holds(paged.attention(m.pages, m.batch_of(max_rows), m.q, softcap=cap, return_lse=True), exact)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16, F32], ids=str)
+@pytest.mark.parametrize("counts, group, prefix", [([7, 2, 1], 2, 70), ([7, 2, 1], 2, 0), ([3, 15, 1], 1, 0), ([15, 8, 3], 4, 33)], ids=str)
+def test_values_that_are_not_finite_in_few_rows(paged, dtype, counts, group, prefix):
+    """as test_values_that_are_not_finite, in units of up to 16 rows: some rows of a sequence see the value, those before it do not"""
+    m = Made(paged, 12, dtype, [130, 80, 50], counts, 16, 2, group, 64, prefix)
+    for b, head, column, value, keys in ((0, 1, 3, math.inf, False), (0, 0, 5, math.nan, True), (1, 0, 63, math.nan, False), (1, 1, 0, -math.inf, False)):
+        x = m.lens[b] - max(1, counts[b] // 2)   # (seen by the last half of the rows)
+        (m.k if keys else m.v)[oracle.place(m.tables[b], len(m.k), 16, x)][head, column] = value
+    out, lse = paged.attention(*m.on_gpu(), m.q.cuda(), return_lse=True)
+    out, lse = out.cpu(), lse.cpu()
+    want, want_lse, tol, _ = oracle.attention(m.k, m.v, m.lens, m.tables, m.rows, m.prefix, prefix, m.q, 0.125, 0.0, P_EPS[dtype])
+    assert torch.equal(torch.isnan(out), torch.isnan(want)) and torch.equal(torch.isinf(out), torch.isinf(want)) and torch.equal(torch.isnan(lse), torch.isnan(want_lse))
+    fine = torch.isfinite(want)
+    assert fine.sum() > 0.5 * fine.numel() and ((out.double() - want).abs() <= tol)[fine].all()
