@@ -890,3 +890,21 @@ def test_values_that_are_not_finite_in_few_rows(paged, dtype, counts, group, pre
     assert torch.equal(torch.isnan(out), torch.isnan(want)) and torch.equal(torch.isinf(out), torch.isinf(want)) and torch.equal(torch.isnan(lse), torch.isnan(want_lse))
     fine = torch.isfinite(want)
     assert fine.sum() > 0.5 * fine.numel() and ((out.double() - want).abs() <= tol)[fine].all()
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16, F32], ids=str)
+@pytest.mark.parametrize("rows, prefix", [([1] * 20, 600), ([40, 17, 1], 0)], ids=str)
+def test_strides_that_are_no_multiples_of_one_another(paged, dtype, rows, prefix):
+    """keys and values in one array, page by page, with gaps that no other stride divides; queries and results with odd gaps between tokens: the same bits as packed"""
+    m = MadeThere(paged, 3, dtype, [90 + c for c in rows], rows, 16, 8, 4, 64, prefix)
+    want = paged.attention(m.pages, m.batch, m.q, return_lse=True)
+    holds(want, m.exact())
+    n, both = len(m.k), 16 * 8 * 64
+    buf = torch.full((n * (2 * both + 24) + 8,), math.nan, dtype=dtype, device="cuda")
+    k, v = (buf.as_strided(m.k.shape, (2 * both + 24, 8 * 64, 64, 1), at) for at in (0, both + 8))
+    k.copy_(m.k), v.copy_(m.v)
+    q, out = (torch.full((m.q.shape[0] * (32 * 72 + gap),), math.nan, dtype=dtype, device="cuda").as_strided(m.q.shape, (32 * 72 + gap, 72, 1)) for gap in (8, 16))
+    q.copy_(m.q)
+    got = paged.attention(paged.KVPages(k, v), m.batch, q, out=out, return_lse=True)
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+    assert torch.isnan(buf.as_strided((n, 8), (2 * both + 24, 1), both)).all()
