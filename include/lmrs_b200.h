@@ -247,9 +247,13 @@ int lmrs_b200_paged_append(const lmrs_b200_pages_t* pages, const lmrs_b200_batch
  * of the exponentials.  A row that sees nothing (padding rows see no prefix either): out 0, lse -infinity.  out may not overlap q.  head_size: a multiple of 8, at most 256;
  * k, v and their strides on 16-byte boundaries.  workspace: device memory of the size that paged_attention_workspace gives for
  * the same pages, batch (its host fields), n_rows and q_heads, on a 256-byte boundary; its contents do not matter before the call and mean nothing after it.  Calls
- * that may run at the same time need one each.  Heads: up to 65535; n_rows * q_heads: up to 2^30;
- * prefix_len + table_len * page_size: up to 2^31 - 129.  A kernel whose waits run out (two seconds in which nothing moves) leaves NaN in the
- * rows that it still had to do; the process' next call of paged_attention then launches nothing and says which wait it was, once. */
+ * that may run at the same time need one each.  Heads: up to 65535; n_rows * q_heads: up to 2^30; prefix_len + table_len * page_size: up to 2^31 - 129.
+ * 16-bit types: the softmax' weights are rounded to the type before the product with the values (by 2^-8 of a weight at most in bfloat16, 2^-11 in float16), their sum is not.  Sums
+ * run over weights of up to 2^8 (float16: 2^15) and are divided at the end, so |values| times keys times that stay below 2^128; a result within half a step of float16's largest number
+ * may come out infinite.  A key or value that is not finite reaches the rows that see it and no others; rows of a sequence's portion that it spoiled on the way are summed again one by one,
+ * which takes seconds behind some 100 thousand keys.
+ * A kernel whose waits run out (two seconds in which nothing moves) leaves NaN in the rows that it still had to do; the process' next call of paged_attention then launches nothing and
+ * says which wait it was, once. */
 int lmrs_b200_paged_attention_workspace(const lmrs_b200_pages_t* pages, const lmrs_b200_batch_t* batch, int64_t n_rows, int q_heads, size_t* bytes);
 int lmrs_b200_paged_attention(const lmrs_b200_pages_t* pages, const lmrs_b200_batch_t* batch, int64_t n_rows, const lmrs_b200_rows_t* q, const lmrs_b200_rows_t* out,
                               int q_heads, float scale, float softcap, float* lse, void* workspace, size_t workspace_bytes, void* stream);
