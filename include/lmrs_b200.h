@@ -214,8 +214,8 @@ typedef struct lmrs_b200_positions {
     const int32_t* data;
     int64_t axis, row;
 } lmrs_b200_positions_t;
-/* out = x turned by its rows' positions; out may be x itself (the same data and strides) and not lie over a part of it.  Arrays that interleave, as parts of one projection do, need equal
- * strides to be told from arrays that lie over one another: here and below */
+/* out = x turned by its rows' positions; out may be x itself (the same data and strides), and not lie over a part of it.  Here and below, arrays whose extents meet are told from arrays that lie
+ * over one another where rows have one stride and each array its own part of them (q, k and v of one projection), or where both strides are equal; others are refused */
 int lmrs_b200_rope_axes(const lmrs_b200_rope_t* rope, int dtype, const lmrs_b200_rows_t* x, const lmrs_b200_rows_t* out, int64_t n_rows, int heads, int head_size,
                         const lmrs_b200_positions_t* pos, void* stream);
 

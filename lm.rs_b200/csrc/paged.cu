@@ -62,8 +62,8 @@ std::string bad_rows(const lmrs_b200_rows_t* r, const char* name, int dtype, int
     if (!on_device(r->data, device)) return std::string(name) + " is not memory of the current device";
     return "";
 }
-// Do two arrays of a call share bytes?  Exact for equal strides (also where they interleave, as parts of one projection do): the second is the first moved by d elements, so they meet if
-// d + i row + j head comes within a head's size of 0 for distances i, j that rows and heads can have.  With other strides, arrays whose extents meet count as meeting.
+// Do two arrays of a call share bytes?  Exact for equal strides (also where they interleave, as parts of one projection do): the second is the first moved by d, so they meet if
+// d + i row + j head comes within a head's size of 0 for distances i, j that rows and heads can have.  With other strides, arrays whose extents meet count as meeting, but for parts of one array's rows.
 bool meet(const lmrs_b200_rows_t* a, int64_t a_heads, const lmrs_b200_rows_t* b, int64_t b_heads, int64_t n_rows, int64_t head_size, int dtype) {
     if (n_rows < 1 || a_heads < 1 || b_heads < 1) return false;
     const int64_t size = (int64_t)size_of(dtype);
@@ -71,11 +71,15 @@ bool meet(const lmrs_b200_rows_t* a, int64_t a_heads, const lmrs_b200_rows_t* b,
     if (n_rows == 1) a_row = b_row = 0;   // (strides that nothing is reached by)
     if (a_heads == 1) a_head = b_heads == 1 ? 0 : b_head;
     if (b_heads == 1) b_head = a_head;
-    typedef __int128 wide;
-    const wide a0 = (wide)(uintptr_t)a->data, b0 = (wide)(uintptr_t)b->data;
-    if (a0 + ((wide)(n_rows - 1) * a_row + (wide)(a_heads - 1) * a_head + head_size) * size <= b0 || b0 + ((wide)(n_rows - 1) * b_row + (wide)(b_heads - 1) * b_head + head_size) * size <= a0) return false;
+    typedef __int128 wide;   // in bytes: the arrays may lie any number of them apart
+    const wide a0 = (wide)(uintptr_t)a->data, b0 = (wide)(uintptr_t)b->data, d = b0 - a0, row = (wide)a_row * size, near = (wide)head_size * size;
+    const wide a_span = (wide)(a_heads - 1) * a_head * size + near, b_span = (wide)(b_heads - 1) * b_head * size + near;
+    if (a0 + (wide)(n_rows - 1) * a_row * size + a_span <= b0 || b0 + (wide)(n_rows - 1) * b_row * size + b_span <= a0) return false;
+    if (a_row == b_row && row > 0) {   // parts of one array's rows, whatever their heads: a's begin at 0 of a row, b's behind them
+        const wide at = (d % row + row) % row;
+        if (at >= a_span && at + b_span <= row) return false;
+    }
     if (a_row != b_row || a_head != b_head || (a_row == 0 && n_rows > 1)) return true;
-    const wide d = b0 - a0, row = (wide)a_row * size, near = (wide)head_size * size;   // in bytes: the arrays may lie any number of them apart
     for (int64_t j = -(a_heads - 1); j < b_heads; j++) {
         const wide at = d + (wide)j * a_head * size;   // + i row for i in -(n_rows - 1) .. n_rows - 1: the nearest to 0 from either side
         wide i = row ? -at / row : 0;

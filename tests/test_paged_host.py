@@ -166,6 +166,7 @@ LIE = [
     ((0, 256, 64), (0, 64, 192), 3, 4, True), ((0, 256, 64), (0, 7, 64), 1, 4, "itself"), ((0, 999, 64), (256, 1, 64), 1, 4, False), ((0, 999, 64), (192, 1, 64), 1, 4, True), ((0, 64, 5), (0, 64, 7), 3, 1, "itself"),
     ((0, 128, 5), (64, 128, 7), 3, 1, False), ((0, 128, 5), (32, 128, 7), 3, 1, True), ((0, 0, 64), (512, 256, 64), 3, 4, False), ((0, 0, 64), (128, 256, 64), 3, 4, True), ((0, 300, 64), (60 * 300, 300, 64), 60, 4, False),
     ((0, 300, 64), (59 * 300, 300, 64), 60, 4, True), ((0, 2 ** 40, 2 ** 35), (2 ** 20, 2 ** 40, 2 ** 35), 60, 4, False),
+    ((0, 600, 64), (256, 600, 70), 5, 4, False), ((256, 600, 70), (0, 600, 64), 5, 4, False), ((0, 600, 64), (255, 600, 70), 5, 4, True), ((0, 600, 64), (326, 600, 70), 5, 4, False), ((0, 600, 64), (327, 600, 70), 5, 4, True),
 ]
 
 
