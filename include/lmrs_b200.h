@@ -258,6 +258,44 @@ int lmrs_b200_paged_attention_workspace(const lmrs_b200_pages_t* pages, const lm
 int lmrs_b200_paged_attention(const lmrs_b200_pages_t* pages, const lmrs_b200_batch_t* batch, int64_t n_rows, const lmrs_b200_rows_t* q, const lmrs_b200_rows_t* out,
                               int q_heads, float scale, float softcap, float* lse, void* workspace, size_t workspace_bytes, void* stream);
 
+/* out = x / sqrt(mean of a head's x^2 + eps) * weight (NULL: none; head h's at weight + h * weight_head), then turned by its rows' positions (rope and pos NULL: not turned); float32 inside, rounded once.
+ * weight: f32.  The rest as in rope_axes. */
+int lmrs_b200_norm_rope(const lmrs_b200_rope_t* rope, int dtype, const lmrs_b200_rows_t* x, const lmrs_b200_rows_t* out, int64_t n_rows, int heads, int head_size, const float* weight,
+                        int64_t weight_head, float eps, const lmrs_b200_positions_t* pos, void* stream);
+
+/* ---- the same pool in 8 bits -----------------------------------------------------------------------------------------------------------------
+ * Codes k[page][slot][head][head_size] and v, a byte each, form 0: int8 (-127 .. 127), 1: e4m3 (a sign, 4 bits of exponent, 3 of mantissa, up to 448), and f32 scales
+ * k_scale[page][block of slots][head] and v_scale, one for `block` neighbouring slots of a page (block divides page_size): a code stands for code * scale.  Strides in elements.
+ * dtype, in the calls: the type of the arrays of rows. */
+typedef struct lmrs_b200_pages8 {
+    void *  k, *v;
+    float * k_scale, *v_scale;
+    int64_t k_page, k_slot, k_head, v_page, v_slot, v_head, ks_page, ks_block, ks_head, vs_page, vs_block, vs_head;
+    int32_t pages, page_size, kv_heads, head_size, block, form;
+} lmrs_b200_pages8_t;
+/* f32 weights of the norms of keys and queries, k_head and q_head elements from one head's to the next's (0: all heads share them); NULL: no norm */
+typedef struct lmrs_b200_norms {
+    const float *k, *q;
+    int64_t k_head, q_head;
+    float eps;
+} lmrs_b200_norms_t;
+/* paged_append to 8-bit pages: k normed and turned, v as it is, both quantised; with q (goes with rope or its norm), q_out = q normed and turned.  norms NULL: none.
+ * A block of slots that the call begins gets the scale a / Q, a the largest size of its new elements and Q 127 or 448, between 2^-60 and 2^60; where it held tokens of the sequence before, the larger of
+ * that and the scale that it had, and the codes that it held become the nearest ones of the same values under the new scale.  A code is the nearest one of element / scale, ties to even (what
+ * k's norm and rotation give is kept in 64 bits until then), elements beyond the largest code's that one.  An element that is not finite makes its block's scale NaN: all of the block reads as NaN.  Two rows with one
+ * place, or sequences that append to the same block: their codes are either's.  No part of the pages may be an input. */
+int lmrs_b200_paged8_append(const lmrs_b200_pages8_t* pages, const lmrs_b200_batch_t* batch, int dtype, int64_t n_rows, const lmrs_b200_rows_t* k, const lmrs_b200_rows_t* v,
+                            const lmrs_b200_rope_t* rope, const lmrs_b200_positions_t* pos, const lmrs_b200_rows_t* q, const lmrs_b200_rows_t* q_out, int q_heads,
+                            const lmrs_b200_norms_t* norms, void* stream);
+/* What the places of the batch's rows hold, k and v [n_rows][kv_heads][head_size]: code * scale in float32, rounded to the type.  Padding rows and rows whose page is none: 0.  Rows from rows[seqs] on
+ * are not touched.  (A batch whose rows are all that its sequences hold, rows[b + 1] - rows[b] = lens[b], reads them whole; prefix pages are read as those of a sequence.) */
+int lmrs_b200_paged8_read(const lmrs_b200_pages8_t* pages, const lmrs_b200_batch_t* batch, int dtype, int64_t n_rows, const lmrs_b200_rows_t* k, const lmrs_b200_rows_t* v, void* stream);
+/* paged_attention over 8-bit pages; dtype is that of q and out.  head_size: a multiple of 16, at most 256; codes and their strides on 16-byte boundaries.  Scales of values count as the nearest number between 2^-60 and 2^60.  The rest as
+ * there. */
+int lmrs_b200_paged8_attention_workspace(const lmrs_b200_pages8_t* pages, const lmrs_b200_batch_t* batch, int dtype, int64_t n_rows, int q_heads, size_t* bytes);
+int lmrs_b200_paged8_attention(const lmrs_b200_pages8_t* pages, const lmrs_b200_batch_t* batch, int dtype, int64_t n_rows, const lmrs_b200_rows_t* q, const lmrs_b200_rows_t* out,
+                               int q_heads, float scale, float softcap, float* lse, void* workspace, size_t workspace_bytes, void* stream);
+
 const char* lmrs_b200_last_error(void);
 /* "lmrs_b200 <version> sm_100a" */
 const char* lmrs_b200_version(void);

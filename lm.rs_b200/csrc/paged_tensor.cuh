@@ -162,6 +162,7 @@ struct GaveUpWord {
         return p && *(volatile int*)p ? __atomic_exchange_n(p, 0, __ATOMIC_ACQ_REL) : 0;
     }
 };
+inline GaveUpWord gave_up_word;   // (one for the process)
 
 // shared memory besides the operands
 template <typename T, int DP> struct TensorShared {

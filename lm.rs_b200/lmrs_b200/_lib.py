@@ -18,6 +18,7 @@ ABI_SYMBOLS = [
     "lmrs_b200_weights_upload", "lmrs_b200_matmul_w", "lmrs_b200_weights_free",
     "lmrs_b200_open", "lmrs_b200_forward_tokens", "lmrs_b200_set_option",
     "lmrs_b200_rope_init", "lmrs_b200_rope_axes", "lmrs_b200_paged_append", "lmrs_b200_paged_attention", "lmrs_b200_paged_attention_workspace",
+    "lmrs_b200_norm_rope", "lmrs_b200_paged8_append", "lmrs_b200_paged8_read", "lmrs_b200_paged8_attention", "lmrs_b200_paged8_attention_workspace",
     "lmrs_b200_last_error", "lmrs_b200_version",
 ]
 
@@ -94,6 +95,11 @@ def lib():
     L.lmrs_b200_paged_append.argtypes = [vp, vp, i64] + [vp] * 6 + [i, vp]
     L.lmrs_b200_paged_attention_workspace.argtypes = [vp, vp, i64, i, C.POINTER(sz)]
     L.lmrs_b200_paged_attention.argtypes = [vp, vp, i64, vp, vp, i, C.c_float, C.c_float, vp, vp, sz, vp]
+    L.lmrs_b200_norm_rope.argtypes = [vp, i, vp, vp, i64, i, i, vp, i64, C.c_float, vp, vp]
+    L.lmrs_b200_paged8_append.argtypes = [vp, vp, i, i64] + [vp] * 6 + [i, vp, vp]
+    L.lmrs_b200_paged8_read.argtypes = [vp, vp, i, i64, vp, vp, vp]
+    L.lmrs_b200_paged8_attention_workspace.argtypes = [vp, vp, i, i64, i, C.POINTER(sz)]
+    L.lmrs_b200_paged8_attention.argtypes = [vp, vp, i, i64, vp, vp, i, C.c_float, C.c_float, vp, vp, sz, vp]
     L.lmrs_b200_open.argtypes = [C.c_char_p, i, i, u32, C.POINTER(vp)]
     L.lmrs_b200_forward_tokens.argtypes = [vp, vp, sz, u32, vp, sz, vp]
     L.lmrs_b200_set_option.argtypes = [vp, C.c_char_p, i]

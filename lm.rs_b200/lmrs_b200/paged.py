@@ -7,6 +7,14 @@ the host, and calls can be captured into CUDA graphs.  Nothing here has a backwa
     batch = Batch(lens, tables, prefix=..., prefix_len=...)
     q     = append(pages, batch, k_new, v_new, rope=rope, q=q)
     out   = attention(pages, batch, q)
+
+The same with the pool in 8 bits, which takes half the room and half the time to read; keys and queries normed on the way where a model does that:
+
+    pages = QuantPages(k, v, k_scale, v_scale)          # int8 or float8_e4m3fn, a float32 scale for each block of tokens and head
+    q     = append(pages, batch, k_new, v_new, rope=rope, q=q, k_norm=wk, q_norm=wq)
+    out   = attention(pages, batch, q)
+    k, v  = read(pages, batch)                          # what the places of the batch's rows hold
+    x     = norm_rope(x, weight, pos, rope)             # the norm and the rotation by themselves
 """
 import ctypes as C
 
@@ -15,6 +23,7 @@ import torch
 from ._lib import LmrsError, check, lib
 
 _DTYPES = {torch.bfloat16: 0, torch.float32: 1, torch.float16: 2}
+_FORMS = {torch.int8: 0, torch.float8_e4m3fn: 1}
 
 
 class _Rope(C.Structure):
@@ -32,6 +41,16 @@ class _Positions(C.Structure):
 class _Pages(C.Structure):
     _fields_ = [("k", C.c_void_p), ("v", C.c_void_p)] + [(n, C.c_int64) for n in ("k_page", "k_slot", "k_head", "v_page", "v_slot", "v_head")] + \
                [(n, C.c_int32) for n in ("pages", "page_size", "kv_heads", "head_size", "dtype")]
+
+
+class _Pages8(C.Structure):
+    _fields_ = [(n, C.c_void_p) for n in ("k", "v", "k_scale", "v_scale")] + \
+               [(n, C.c_int64) for n in ("k_page", "k_slot", "k_head", "v_page", "v_slot", "v_head", "ks_page", "ks_block", "ks_head", "vs_page", "vs_block", "vs_head")] + \
+               [(n, C.c_int32) for n in ("pages", "page_size", "kv_heads", "head_size", "block", "form")]
+
+
+class _Norms(C.Structure):
+    _fields_ = [("k", C.c_void_p), ("q", C.c_void_p), ("k_head", C.c_int64), ("q_head", C.c_int64), ("eps", C.c_float)]
 
 
 class _Batch(C.Structure):
@@ -100,6 +119,21 @@ def _ints(t, name, device):
     _gpu(t, name, device)
     if t.dtype != torch.int32:
         raise LmrsError(f"{name} must be int32, not {t.dtype}")
+
+
+def _weight(w, name, heads, size, device):
+    """float32 weights of a norm, [size] or [heads, size]: their place, and from one head's to the next's"""
+    if not isinstance(w, torch.Tensor) or not w.is_cuda or w.device != device:
+        _gpu(w, name, device)
+    if w.requires_grad:
+        _no_gradients(w, name)
+    if w.dtype != torch.float32:
+        raise LmrsError(f"{name} must be float32, not {w.dtype}")
+    if w.shape != (size,) and w.shape != (heads, size):
+        raise LmrsError(f"{name} must be [{size}] or [{heads}, {size}], not {list(w.shape)}")
+    if w.stride(-1) != 1 and size != 1:
+        raise LmrsError(f"the elements of a head of {name} must lie next to each other")
+    return w.data_ptr(), w.stride(0) if w.dim() == 2 else 0
 
 
 def _positions(pos, axes, rows, device):
@@ -172,6 +206,33 @@ class KVPages:
         self._ref = C.byref(self._c)
 
 
+class QuantPages:
+    """The pool in 8 bits: codes of keys and values [pages, page_size, kv_heads, head_size], int8 or float8_e4m3fn, and float32 scales [pages, page_size / block, kv_heads], each in any order of the first
+    three dimensions.  A code stands for code * scale; `block` neighbouring tokens of a page share a head's scale.  Goes where KVPages goes; the rows of a call may be of any of the three types."""
+
+    def __init__(self, k, v, k_scale, v_scale):
+        _gpu(k, "k", k.device if isinstance(k, torch.Tensor) else None)
+        for t, name in ((v, "v"), (k_scale, "k_scale"), (v_scale, "v_scale")):
+            _gpu(t, name, k.device)
+        _need(k.dim() == 4 and k.shape == v.shape, f"k and v must be [pages, page_size, kv_heads, head_size] alike, not {list(k.shape)} and {list(v.shape)}")
+        _need(k.dtype in _FORMS and k.dtype == v.dtype, f"k and v must both be int8 or float8_e4m3fn, not {k.dtype} and {v.dtype}")
+        _need(k_scale.dtype == torch.float32 and v_scale.dtype == torch.float32, f"k_scale and v_scale must be float32, not {k_scale.dtype} and {v_scale.dtype}")
+        pages, page_size, kv_heads, _ = k.shape
+        _need(k_scale.dim() == 3 and k_scale.shape == v_scale.shape and k_scale.shape[0] == pages and k_scale.shape[2] == kv_heads and k_scale.shape[1] > 0 and page_size % k_scale.shape[1] == 0,
+              f"k_scale and v_scale must be [{pages}, blocks, {kv_heads}] alike, blocks a divisor of {page_size}, not {list(k_scale.shape)} and {list(v_scale.shape)}")
+        for t, name in ((k, "k"), (v, "v"), (k_scale, "k_scale"), (v_scale, "v_scale")):
+            if t.requires_grad:
+                _no_gradients(t, name)
+            _need(t.dim() == 3 or t.stride(3) == 1 or t.shape[3] == 1, f"the elements of a head of {name} must lie next to each other")
+            _need(_disjoint(t), f"elements of {name} share their places")
+        _need(max(k.shape) < 1 << 31, f"a dimension of {list(k.shape)} is beyond 2^31 - 1")   # (ctypes would keep its lower 32 bits)
+        self.k, self.v, self.k_scale, self.v_scale, self.device, self.form = k, v, k_scale, v_scale, k.device, k.dtype
+        self.pages, self.page_size, self.kv_heads, self.head_size = k.shape
+        self.block = page_size // k_scale.shape[1]
+        self._c = _Pages8(k.data_ptr(), v.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), *k.stride()[:3], *v.stride()[:3], *k_scale.stride(), *v_scale.stride(), *k.shape, self.block, _FORMS[k.dtype])
+        self._ref = C.byref(self._c)
+
+
 class Batch:
     """The sequences of a call.  lens [seqs]: tokens that each holds, those of the call included (which are its last).  tables [seqs, n]: the pages of
     each, in order.  rows [seqs + 1]: the first row of each in the call's arrays (None: one row each); max_rows: most rows of one sequence.  A
@@ -202,8 +263,8 @@ class Batch:
         self._bytes = {}   # workspaces' sizes
 
     def _for(self, pages, n_rows):
-        if not isinstance(pages, KVPages):
-            raise LmrsError("pages must be KVPages")
+        if not isinstance(pages, (KVPages, QuantPages)):
+            raise LmrsError("pages must be KVPages or QuantPages")
         if self.device != pages.device:
             raise LmrsError(f"the batch lies on {self.device}, the pages on {pages.device}")
         if self.prefix_len and self.prefix.shape[0] * pages.page_size < self.prefix_len:
@@ -237,23 +298,71 @@ def rope_axes(x, pos, rope, out=None):
     return out
 
 
-def append(pages, batch, k, v, rope=None, pos=None, q=None, q_out=None):
+def norm_rope(x, weight=None, pos=None, rope=None, eps=1e-6, out=None):
+    """x [rows, heads, head_size], every head divided by the root of its mean square (plus eps) and multiplied by weight, float32 [head_size] or [heads, head_size] (None: 1), then turned by pos as in
+    rope_axes (rope None: not turned); out may be x, and not lie over a part of it."""
+    if not isinstance(x, torch.Tensor) or x.dim() != 3 or x.dtype not in _DTYPES:
+        raise LmrsError("x must be a [rows, heads, head_size] tensor of bfloat16, float16 or float32")
+    if rope is not None and not isinstance(rope, RopeAxes):
+        raise LmrsError("rope must be RopeAxes")
+    if (rope is None) != (pos is None):
+        raise LmrsError("rope and pos come together")
+    n, heads, size = x.shape
+    if heads > 65535:
+        raise LmrsError(f"{heads} heads: at most 65535")
+    device, dtype = x.device, x.dtype
+    if x.is_cuda and device.index != torch.cuda.current_device():
+        with torch.cuda.device(device):
+            return norm_rope(x, weight, pos, rope, eps, out)
+    xr = _heads(x, "x", device, dtype, n, heads, size)
+    w, w_head = (None, 0) if weight is None else _weight(weight, "weight", heads, size, device)
+    p = None if rope is None else _byref(_positions(pos, rope.axes, n, device))
+    if out is None:
+        out, o = _new(x)
+    else:
+        o = _heads(out, "out", device, dtype, n, heads, size, out=True)
+    rc = lib().lmrs_b200_norm_rope(None if rope is None else rope._ref, _DTYPES[dtype], _byref(xr), _byref(o), n, heads, size, w, w_head, eps, p, _stream(device.index))
+    if rc:
+        check(rc)
+    return out
+
+
+def append(pages, batch, k, v, rope=None, pos=None, q=None, q_out=None, k_norm=None, q_norm=None, eps=1e-6):
     """Writes k and v [rows, kv_heads, head_size] to the places in the pages that the batch gives their rows, k turned by pos [axes, rows] (None: by its
-    place, the prefix included, on every axis); rope None: k as it is.  Returns q [rows, heads, head_size] turned alike (q_out may be q), or None."""
+    place, the prefix included, on every axis); rope None: k as it is.  Returns q [rows, heads, head_size] turned alike (q_out may be q), or None.
+    Into QuantPages (which the next lines are about; for KVPages, norm_rope comes before): k_norm and q_norm, float32 [head_size] or one row a head, norm the heads of k and q first (None: not).  A block of
+    tokens that the call begins gets the scale a / Q, a its largest size and Q the format's largest number, within 2^-60 .. 2^60; a block that held tokens before the larger of that and its old
+    scale, to which its codes are rounded again.  Codes are the nearest ones, ties to even; an element that is not finite makes its block read as NaN."""
     if not isinstance(batch, Batch):
         raise LmrsError("batch must be a Batch")
     if not isinstance(k, torch.Tensor) or k.dim() != 3:
         raise LmrsError("k must be a [rows, kv_heads, head_size] tensor")
     n = k.shape[0]
     batch._for(pages, n)
-    device, dtype, size = pages.device, pages.dtype, pages.head_size
+    quant = isinstance(pages, QuantPages)
+    device, dtype, size = pages.device, k.dtype if quant else pages.dtype, pages.head_size
     if device.index != torch.cuda.current_device():
         with torch.cuda.device(device):
-            return append(pages, batch, k, v, rope, pos, q, q_out)
+            return append(pages, batch, k, v, rope, pos, q, q_out, k_norm, q_norm, eps)
+    norms = None
+    if quant:
+        if dtype not in _DTYPES:
+            raise LmrsError(f"k must be bfloat16, float16 or float32, not {dtype}")
+        if k_norm is not None or q_norm is not None:
+            if q_norm is not None and q is None:
+                raise LmrsError("q_norm without q")
+            norms = _Norms(eps=eps)
+            if k_norm is not None:
+                norms.k, norms.k_head = _weight(k_norm, "k_norm", pages.kv_heads, size, device)
+            if q_norm is not None:
+                norms.q, norms.q_head = _weight(q_norm, "q_norm", q.shape[1] if isinstance(q, torch.Tensor) and q.dim() == 3 else 0, size, device)
+            norms = _byref(norms)
+    elif k_norm is not None or q_norm is not None:
+        raise LmrsError("k_norm and q_norm go with QuantPages: call norm_rope before")
     kr = _heads(k, "k", device, dtype, n, pages.kv_heads, size)
     vr = _heads(v, "v", device, dtype, n, pages.kv_heads, size)
     if rope is None:
-        if pos is not None or q is not None or q_out is not None:
+        if pos is not None or ((q is not None or q_out is not None) and q_norm is None):
             raise LmrsError("pos and q go with rope")
     elif not isinstance(rope, RopeAxes):
         raise LmrsError("rope must be RopeAxes")
@@ -274,17 +383,52 @@ def append(pages, batch, k, v, rope=None, pos=None, q=None, q_out=None):
         qo = _byref(qo)
     elif q_out is not None:
         raise LmrsError("q_out without q")
-    rc = lib().lmrs_b200_paged_append(pages._ref, batch._ref, n, _byref(kr), _byref(vr), None if rope is None else rope._ref, p, qr, qo, heads, _stream(device.index))
+    turn = None if rope is None else rope._ref
+    if quant:
+        rc = lib().lmrs_b200_paged8_append(pages._ref, batch._ref, _DTYPES[dtype], n, _byref(kr), _byref(vr), turn, p, qr, qo, heads, norms, _stream(device.index))
+    else:
+        rc = lib().lmrs_b200_paged_append(pages._ref, batch._ref, n, _byref(kr), _byref(vr), turn, p, qr, qo, heads, _stream(device.index))
     if rc:
         check(rc)
     return q_out
+
+
+def read(pages, batch, rows=None, dtype=torch.bfloat16, k=None, v=None):
+    """What the places of the batch's rows in QuantPages hold: keys and values [rows, kv_heads, head_size] of the dtype (or of k and v, which are written then), code * scale rounded to it.  rows: how many rows
+    the batch has (None: one each).  Rows without a place (padding, entries of a table that are no pages) are 0; rows behind the last sequence are not touched.  A batch whose rows are all that its
+    sequences hold reads them whole."""
+    if not isinstance(batch, Batch):
+        raise LmrsError("batch must be a Batch")
+    if not isinstance(pages, QuantPages):
+        raise LmrsError("pages must be QuantPages")
+    n = batch.seqs if rows is None else int(rows)
+    if not 0 <= n < 1 << 31:
+        raise LmrsError("rows must be 0 .. 2^31 - 1")
+    if (k is None) != (v is None):
+        raise LmrsError("k and v come together")
+    batch._for(pages, n)
+    device, shape = pages.device, (n, pages.kv_heads, pages.head_size)
+    if device.index != torch.cuda.current_device():
+        with torch.cuda.device(device):
+            return read(pages, batch, rows, dtype, k, v)
+    if k is None:
+        if dtype not in _DTYPES:
+            raise LmrsError(f"dtype must be bfloat16, float16 or float32, not {dtype}")
+        k, v = torch.empty(shape, dtype=dtype, device=device), torch.empty(shape, dtype=dtype, device=device)
+    elif not isinstance(k, torch.Tensor) or k.dtype not in _DTYPES:
+        raise LmrsError("k must be a tensor of bfloat16, float16 or float32")
+    kr, vr = _heads(k, "k", device, k.dtype, *shape, out=True), _heads(v, "v", device, k.dtype, *shape, out=True)
+    rc = lib().lmrs_b200_paged8_read(pages._ref, batch._ref, _DTYPES[k.dtype], n, _byref(kr), _byref(vr), _stream(device.index))
+    if rc:
+        check(rc)
+    return k, v
 
 
 def attention(pages, batch, q, out=None, scale=None, softcap=0.0, return_lse=False):
     """softmax(scale * q . keys) . values for q [rows, heads, head_size]: every row over the prefix and over its own sequence up to its own place.
     heads: a multiple of kv_heads, neighbours share one.  scale None: head_size ** -0.5.  softcap > 0: scores s become softcap * tanh(s / softcap).  A row
     that sees nothing is 0.  return_lse: also the logarithms of the sums of exponentials, float32 [rows, heads] (-inf for a row that sees nothing).
-    out may not overlap q.  16-bit types: the softmax' weights are rounded to the type before the product with the values, their sum is not."""
+    out may not overlap q.  16-bit types: the softmax' weights are rounded to the type before the product with the values, their sum is not.  QuantPages: q is of any type, and head_size a multiple of 16."""
     if not isinstance(batch, Batch):
         raise LmrsError("batch must be a Batch")
     if not isinstance(q, torch.Tensor) or q.dim() != 3:
@@ -293,7 +437,10 @@ def attention(pages, batch, q, out=None, scale=None, softcap=0.0, return_lse=Fal
     if heads > 65535:
         raise LmrsError(f"{heads} heads: at most 65535")
     batch._for(pages, n)
-    device, dtype = pages.device, pages.dtype
+    quant = isinstance(pages, QuantPages)
+    device, dtype = pages.device, q.dtype if quant else pages.dtype
+    if dtype not in _DTYPES:
+        raise LmrsError(f"q must be bfloat16, float16 or float32, not {dtype}")
     if device.index != torch.cuda.current_device():
         with torch.cuda.device(device):
             return attention(pages, batch, q, out, scale, softcap, return_lse)
@@ -304,17 +451,24 @@ def attention(pages, batch, q, out=None, scale=None, softcap=0.0, return_lse=Fal
         o = _heads(out, "out", device, dtype, n, heads, size, out=True)
     lse = torch.empty(n, heads, dtype=torch.float32, device=device) if return_lse else None
     L = lib()
-    key = (n, heads, pages.kv_heads, size, pages.page_size, dtype)
+    key = (n, heads, pages.kv_heads, size, pages.page_size, dtype, quant)
     need = batch._bytes.get(key)
     if need is None:   # (it goes by the numbers of the call alone)
         got = C.c_size_t()
-        check(L.lmrs_b200_paged_attention_workspace(pages._ref, batch._ref, n, heads, C.byref(got)))
+        if quant:
+            check(L.lmrs_b200_paged8_attention_workspace(pages._ref, batch._ref, _DTYPES[dtype], n, heads, C.byref(got)))
+        else:
+            check(L.lmrs_b200_paged_attention_workspace(pages._ref, batch._ref, n, heads, C.byref(got)))
         if len(batch._bytes) > 64:
             batch._bytes.clear()
         need = batch._bytes[key] = got.value
     work = torch.empty(need, dtype=torch.uint8, device=device) if need else None
-    rc = L.lmrs_b200_paged_attention(pages._ref, batch._ref, n, _byref(qr), _byref(o), heads, size ** -0.5 if scale is None else scale, softcap,
-                                     lse.data_ptr() if return_lse and n and heads else None, work.data_ptr() if need else None, need, _stream(device.index))
+    scale = size ** -0.5 if scale is None else scale
+    lse_at, work_at = lse.data_ptr() if return_lse and n and heads else None, work.data_ptr() if need else None
+    if quant:
+        rc = L.lmrs_b200_paged8_attention(pages._ref, batch._ref, _DTYPES[dtype], n, _byref(qr), _byref(o), heads, scale, softcap, lse_at, work_at, need, _stream(device.index))
+    else:
+        rc = L.lmrs_b200_paged_attention(pages._ref, batch._ref, n, _byref(qr), _byref(o), heads, scale, softcap, lse_at, work_at, need, _stream(device.index))
     if rc:
         check(rc)
     return (out, lse) if return_lse else out
