@@ -170,14 +170,6 @@ struct Cutting {
     bool own_tensor, front_tensor;
     size_t bytes;
 };
-// places in the workspace, counted from `base` (null: only their sizes matter)
-void place_line(Line& l, int64_t rows, const lmrs_b200_pages_t* pages, char* base, size_t& bytes) {
-    auto take = [&](size_t n) { char* at = base + bytes; bytes += (n + 255) / 256 * 256; return at; };
-    l.slots = l.front_units + l.ctas + (l.seqs ? (rows / l.tile_rows + l.seqs) * pages->kv_heads : 0);   // (a sequence's last unit may be a part of one)
-    l.plan = (Plan*)take(sizeof(Plan) * ((size_t)l.seqs + 1));
-    l.ml = (float2*)take(sizeof(float2) * (size_t)l.slots * l.tile_rows);
-    l.o = (float*)take(sizeof(float) * (size_t)l.slots * l.tile_rows * pages->head_size);
-}
 // Which kernel takes what.  float32: rows16_kernel.  16-bit types: it depends on how often the keys would be read again.  rows16_kernel reads them once per 16
 // rows of a KV head and, with little to do, starts some 8 us sooner; rows128_kernel reads them once per 128 or 256 rows.  Measured on a B200 with rows16_kernel / rows128_kernel,
 // us a call, 8 KV heads:
@@ -217,7 +209,7 @@ template <typename T, int DP> Cutting cutting(const lmrs_b200_pages_t* pages, co
             if (even * 16 >= SMS * 15) ctas = even;
         }
         l.ctas = ctas;
-        place_line(l, rows, pages, base, c.bytes);
+        place_line(l, rows, pages->kv_heads, pages->head_size, base, c.bytes);
     };
     using R = TensorRule<DP>;
     c.own_tensor = sizeof(T) == 2 && std::min<int64_t>(batch->max_rows, n_rows) * group >= R::OWN_ROWS;

@@ -237,6 +237,44 @@ static std::string bad_attention8(const lmrs_b200_pages8_t* pages, const lmrs_b2
     return "";
 }
 
+namespace {
+
+// How a call is cut, from what the host knows of it (as in paged.cu)
+struct Cutting8 {
+    Line own, front;   // the kernel's that takes the sequences' units, and that takes the prefix' (the same where one takes both)
+    size_t bytes;
+};
+template <typename T, int DP> Cutting8 cutting8(const lmrs_b200_pages8_t* pages, const lmrs_b200_batch_t* batch, int64_t n_rows, int q_heads, char* base) {
+    using S = TileShape8<T, DP>;
+    const int64_t group = q_heads / pages->kv_heads, rows = n_rows * group;
+    Cutting8 c = {};
+    auto line = [&](Line& l, bool own, bool front) {
+        l.tile_rows = S::ROWS;
+        l.tile_keys = S::KEYS;
+        l.ctas = SMS * S::CTAS;
+        while (1 << l.row_shift < l.tile_rows) l.row_shift++;
+        while (1 << l.key_shift < l.tile_keys) l.key_shift++;
+        l.seqs = own ? batch->seqs : 0;
+        l.front_tiles = front ? (int)(((int64_t)batch->prefix_len + l.tile_keys - 1) / l.tile_keys) : 0;
+        l.front_units = l.front_tiles ? (rows + l.tile_rows - 1) / l.tile_rows * pages->kv_heads : 0;
+        place_line(l, rows, pages->kv_heads, pages->head_size, base, c.bytes);
+    };
+    line(c.own, true, true);
+    c.front = c.own;
+    return c;
+}
+template <typename F> int by_shape8(const lmrs_b200_pages8_t* pages, int dtype, F f) {
+    return by_type(dtype, [&](auto t) {
+        return by_form(pages->form, [&](auto form) {
+            using T = decltype(t);
+            using FORM = decltype(form);
+            return pages->head_size <= 64 ? f(T(), FORM(), std::integral_constant<int, 64>()) : pages->head_size <= 128 ? f(T(), FORM(), std::integral_constant<int, 128>()) : f(T(), FORM(), std::integral_constant<int, 256>());
+        });
+    });
+}
+
+}  // namespace
+
 extern "C" int lmrs_b200_paged8_attention_workspace(const lmrs_b200_pages8_t* pages, const lmrs_b200_batch_t* batch, int dtype, int64_t n_rows, int q_heads, size_t* bytes) {
     static const char* me = "paged8_attention_workspace";
     return guarded(me, [&]() -> int {
@@ -244,7 +282,11 @@ extern "C" int lmrs_b200_paged8_attention_workspace(const lmrs_b200_pages8_t* pa
         const std::string why = bad_attention8(pages, batch, dtype, n_rows, q_heads);
         if (!why.empty()) return refuse(me, why);
         *bytes = 0;
-        return 0;
+        if (n_rows == 0 || batch->seqs == 0) return 0;
+        return by_shape8(pages, dtype, [&](auto t, auto, auto d) {
+            *bytes = cutting8<decltype(t), decltype(d)::value>(pages, batch, n_rows, q_heads, nullptr).bytes;
+            return 0;
+        });
     });
 }
 
@@ -265,25 +307,44 @@ extern "C" int lmrs_b200_paged8_attention(const lmrs_b200_pages8_t* pages, const
         if (why.empty()) why = bad_rows(out, "out", dtype, device);
         if (why.empty() && lse && (!aligned(lse, 4) || !on_device(lse, device))) why = "lse is not memory of the current device";
         if (why.empty()) why = bad_pages8_memory(pages, device);
+        if (why.empty() && (!workspace || !aligned(workspace, 256) || !on_device(workspace, device))) why = "workspace is not memory of the current device on a 256-byte boundary";
         if (!why.empty()) return refuse(me, why);
-        return by_type(dtype, [&](auto t) {
+        return by_shape8(pages, dtype, [&](auto t, auto form, auto d) {
             using T = decltype(t);
-            return by_form(pages->form, [&](auto form) {
-                Attn8Params<T> p = {};
-                p.batch = batch8_as(batch, pages, n_rows);
-                p.q = rows_as<const T>(q);
-                p.out = rows_as<T>(out);
-                p.c = pages8_as(pages);
-                p.kv_heads = pages->kv_heads; p.q_heads = q_heads; p.head_size = pages->head_size; p.group = q_heads / pages->kv_heads;
-                // At the ends of float32: a cap beyond 2^100 is one of 2^100 (scores of up to 2^88 are not moved by either, and its product with log2 e is finite), and no score is 0 times infinity
-                const float cap = std::min(softcap, 0x1p100f);
-                p.scale2 = std::max(-FLT_MAX, std::min(FLT_MAX, scale * LOG2E)); p.softcap = cap; p.cap_in = cap > 0.0f ? std::max(-FLT_MAX, std::min(FLT_MAX, scale / cap)) : 0.0f; p.lse = lse;
-                p.page_shift = -1;
-                for (int i = 0; i < 31; i++)
-                    if (pages->page_size == 1 << i) p.page_shift = i;
-                row8_kernel<T, decltype(form)::value><<<(unsigned)(n_rows * q_heads), 128, 0, (cudaStream_t)stream>>>(p);
-                return launched(me);
-            });
+            constexpr int FORM = decltype(form)::value, DP = decltype(d)::value;
+            using S = TileShape8<T, DP>;
+            const Cutting8 c = cutting8<T, DP>(pages, batch, n_rows, q_heads, (char*)workspace);
+            if (workspace_bytes < c.bytes) return refuse(me, "workspace has " + std::to_string(workspace_bytes) + " bytes, the call needs " + std::to_string(c.bytes));
+            Attn8Params<T> p = {};
+            p.batch = batch8_as(batch, pages, n_rows);
+            p.q = rows_as<const T>(q);
+            p.out = rows_as<T>(out);
+            p.c = pages8_as(pages);
+            p.kv_heads = pages->kv_heads; p.q_heads = q_heads; p.head_size = pages->head_size; p.group = q_heads / pages->kv_heads;
+            // At the ends of float32: a cap beyond 2^100 is one of 2^100 (scores of up to 2^88 are not moved by either, and its product with log2 e is finite), and no score is 0 times infinity
+            const float cap = std::min(softcap, 0x1p100f);
+            p.scale2 = std::max(-FLT_MAX, std::min(FLT_MAX, scale * LOG2E)); p.softcap = cap; p.cap_in = cap > 0.0f ? std::max(-FLT_MAX, std::min(FLT_MAX, scale / cap)) : 0.0f; p.lse = lse;
+            p.q_wide = vectors(q, dtype);
+            p.out_wide = aligned(out->data, 4 * sizeof(T)) && out->row % 4 == 0 && out->head % 4 == 0;
+            p.whole = batch->prefix_len == 0;
+            p.page_shift = p.block_shift = -1;
+            for (int i = 0; i < 31; i++) {
+                if (pages->page_size == 1 << i) p.page_shift = i;
+                if (pages->block == 1 << i) p.block_shift = i;
+            }
+            static std::atomic<uint64_t> allowed{0};
+            auto kernel = rows16_codes_kernel<T, FORM, DP>;
+            cudaError_t e = allow_smem(kernel, device, S::SMEM, allowed);
+            if (e != cudaSuccess) return refuse(me, cudaGetErrorString(e));
+            kernel<<<(unsigned)c.own.ctas, S::THREADS, S::SMEM, (cudaStream_t)stream>>>(p, c.own);
+            if (launched(me)) return 1;
+            // (which join, as in paged.cu)
+            const int64_t items = n_rows * q_heads;
+            constexpr int COLS = DP <= 128 ? 1 : 2;
+            const AttnParams<T>& rows = p;
+            e = items <= SMS * 4 ? launch_after(join_kernel<T, 8, COLS>, (unsigned)items, 256, 0, (cudaStream_t)stream, rows, c.front, c.own)
+                                 : launch_after(join_kernel<T, 1, COLS>, (unsigned)std::min<int64_t>((items + 7) / 8, SMS * 16), 256, 0, (cudaStream_t)stream, rows, c.front, c.own);
+            return e == cudaSuccess ? 0 : refuse(me, std::string("launch failed: ") + cudaGetErrorString(e));
         });
     });
 }

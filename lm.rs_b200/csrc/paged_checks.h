@@ -7,7 +7,7 @@
 #include <atomic>
 #include <string>
 
-#include "paged.h"
+#include "paged_attn.cuh"
 #include "paged_rows.cuh"
 
 namespace lmrs {
@@ -150,6 +150,14 @@ inline unsigned warps_grid(int64_t warps, int sms) { return (unsigned)std::min<i
 
 // The number of CTAs that share a call's work counts a B200's SMs: it is part of how a call is cut, and a workspace's size goes by it
 constexpr int SMS = 148;
+// a line's places in the workspace, counted from `base` (null: only their sizes matter)
+inline void place_line(Line& l, int64_t rows, int kv_heads, int head_size, char* base, size_t& bytes) {
+    auto take = [&](size_t n) { char* at = base + bytes; bytes += (n + 255) / 256 * 256; return at; };
+    l.slots = l.front_units + l.ctas + (l.seqs ? (rows / l.tile_rows + l.seqs) * kv_heads : 0);   // (a sequence's last unit may be a part of one)
+    l.plan = (Plan*)take(sizeof(Plan) * ((size_t)l.seqs + 1));
+    l.ml = (float2*)take(sizeof(float2) * (size_t)l.slots * l.tile_rows);
+    l.o = (float*)take(sizeof(float) * (size_t)l.slots * l.tile_rows * head_size);
+}
 // lets a kernel use more than 48 KB of shared memory: once a device
 template <typename K> cudaError_t allow_smem(K kernel, int device, int bytes, std::atomic<uint64_t>& done) {
     const uint64_t bit = 1ull << (device & 63);
