@@ -244,8 +244,8 @@ struct Cutting8 {
     Line own, front;   // the kernel's that takes the sequences' units, and that takes the prefix' (the same where one takes both)
     size_t bytes;
 };
-template <typename T, int DP> Cutting8 cutting8(const lmrs_b200_pages8_t* pages, const lmrs_b200_batch_t* batch, int64_t n_rows, int q_heads, char* base) {
-    using S = TileShape8<T, DP>;
+template <typename T, int DP, int ROW_TILES> Cutting8 cutting8(const lmrs_b200_pages8_t* pages, const lmrs_b200_batch_t* batch, int64_t n_rows, int q_heads, char* base) {
+    using S = TileShape8<T, DP, ROW_TILES>;
     const int64_t group = q_heads / pages->kv_heads, rows = n_rows * group;
     Cutting8 c = {};
     auto line = [&](Line& l, bool own, bool front) {
@@ -263,12 +263,47 @@ template <typename T, int DP> Cutting8 cutting8(const lmrs_b200_pages8_t* pages,
     c.front = c.own;
     return c;
 }
-template <typename F> int by_shape8(const lmrs_b200_pages8_t* pages, int dtype, F f) {
+// Tensor maps of the codes for boxes of S::BOX columns, if there are any (boxes.rows stays 0 otherwise): rows of a box are the most that divide a page and a warp's keys
+template <typename S> void box_maps8(const lmrs_b200_pages8_t* pages, Boxes8& boxes) {
+    typedef CUresult (*Encode)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
+                               CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+    static const Encode encode = [] {
+        void* f = nullptr;
+        cudaDriverEntryPointQueryResult q;
+        return cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &f, cudaEnableDefault, &q) == cudaSuccess && q == cudaDriverEntryPointSuccess ? (Encode)f : nullptr;
+    }();
+    int rows = S::WARP_KEYS;
+    while (rows > 1 && pages->page_size % rows) rows /= 2;
+    if (!encode || 2 * (S::WARP_KEYS / rows) * (S::KV / S::WARP_KEYS / S::BOX) > 32) return;   // (a box a lane)
+    auto map = [&](CUtensorMap* m, void* base, int64_t page, int64_t slot, int64_t head, int& place_at, int& head_at) {
+        struct { int64_t stride; cuuint64_t n; cuuint32_t box; int what; } d[3] = {{slot, (cuuint64_t)pages->page_size, (cuuint32_t)rows, 0}, {head, (cuuint64_t)pages->kv_heads, 1, 1},
+                                                                              {page, (cuuint64_t)pages->pages, 1, 2}};
+        std::sort(d, d + 3, [](const auto& a, const auto& b) { return a.stride < b.stride; });
+        const cuuint64_t dims[4] = {(cuuint64_t)pages->head_size, d[0].n, d[1].n, d[2].n};
+        const cuuint64_t strides[3] = {(cuuint64_t)d[0].stride, (cuuint64_t)d[1].stride, (cuuint64_t)d[2].stride};
+        const cuuint32_t box[4] = {(cuuint32_t)S::BOX, d[0].box, d[1].box, d[2].box}, step[4] = {1, 1, 1, 1};
+        for (int i = 0; i < 3; i++) {
+            if (d[i].what == 0) place_at = i;
+            if (d[i].what == 1) head_at = i;
+            if (strides[i] == 0 || strides[i] % 16 || strides[i] >= (1ull << 40)) return false;
+        }
+        return encode(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 4, base, dims, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE, S::BOX == 64 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B,
+                      CU_TENSOR_MAP_L2_PROMOTION_NONE, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+    };
+    if (map(&boxes.k, pages->k, pages->k_page, pages->k_slot, pages->k_head, boxes.k_place, boxes.k_head) &&
+        map(&boxes.v, pages->v, pages->v_page, pages->v_slot, pages->v_head, boxes.v_place, boxes.v_head))
+        boxes.rows = rows;
+}
+// rows of a unit in eights: one where no unit has more
+int row_tiles(const lmrs_b200_pages8_t* pages, const lmrs_b200_batch_t* batch, int64_t n_rows, int q_heads) {
+    const int64_t group = q_heads / pages->kv_heads;
+    return (batch->prefix_len ? n_rows : std::min<int64_t>(batch->max_rows, n_rows)) * group <= 8 ? 1 : 2;
+}
+template <typename F> int by_shape8(const lmrs_b200_pages8_t* pages, int dtype, int tiles, F f) {
     return by_type(dtype, [&](auto t) {
         return by_form(pages->form, [&](auto form) {
-            using T = decltype(t);
-            using FORM = decltype(form);
-            return pages->head_size <= 64 ? f(T(), FORM(), std::integral_constant<int, 64>()) : pages->head_size <= 128 ? f(T(), FORM(), std::integral_constant<int, 128>()) : f(T(), FORM(), std::integral_constant<int, 256>());
+            auto by_tiles = [&](auto d) { return tiles == 1 ? f(t, form, d, std::integral_constant<int, 1>()) : f(t, form, d, std::integral_constant<int, 2>()); };
+            return pages->head_size <= 64 ? by_tiles(std::integral_constant<int, 64>()) : pages->head_size <= 128 ? by_tiles(std::integral_constant<int, 128>()) : by_tiles(std::integral_constant<int, 256>());
         });
     });
 }
@@ -283,8 +318,8 @@ extern "C" int lmrs_b200_paged8_attention_workspace(const lmrs_b200_pages8_t* pa
         if (!why.empty()) return refuse(me, why);
         *bytes = 0;
         if (n_rows == 0 || batch->seqs == 0) return 0;
-        return by_shape8(pages, dtype, [&](auto t, auto, auto d) {
-            *bytes = cutting8<decltype(t), decltype(d)::value>(pages, batch, n_rows, q_heads, nullptr).bytes;
+        return by_shape8(pages, dtype, row_tiles(pages, batch, n_rows, q_heads), [&](auto t, auto, auto d, auto tiles) {
+            *bytes = cutting8<decltype(t), decltype(d)::value, decltype(tiles)::value>(pages, batch, n_rows, q_heads, nullptr).bytes;
             return 0;
         });
     });
@@ -309,11 +344,13 @@ extern "C" int lmrs_b200_paged8_attention(const lmrs_b200_pages8_t* pages, const
         if (why.empty()) why = bad_pages8_memory(pages, device);
         if (why.empty() && (!workspace || !aligned(workspace, 256) || !on_device(workspace, device))) why = "workspace is not memory of the current device on a 256-byte boundary";
         if (!why.empty()) return refuse(me, why);
-        return by_shape8(pages, dtype, [&](auto t, auto form, auto d) {
+        if (const int status = gave_up_word.take())
+            return refuse(me, "results of an earlier call are NaN: " + (status >> 8 == TG_ROWS8 >> 8 ? "rows8_kernel gave up waiting for a slot's copies (device status " + std::to_string(status) + ")" : dense::tg_gave_up(status)));
+        return by_shape8(pages, dtype, row_tiles(pages, batch, n_rows, q_heads), [&](auto t, auto form, auto d, auto tiles) {
             using T = decltype(t);
-            constexpr int FORM = decltype(form)::value, DP = decltype(d)::value;
-            using S = TileShape8<T, DP>;
-            const Cutting8 c = cutting8<T, DP>(pages, batch, n_rows, q_heads, (char*)workspace);
+            constexpr int FORM = decltype(form)::value, DP = decltype(d)::value, ROW_TILES = decltype(tiles)::value;
+            using S = TileShape8<T, DP, ROW_TILES>;
+            const Cutting8 c = cutting8<T, DP, ROW_TILES>(pages, batch, n_rows, q_heads, (char*)workspace);
             if (workspace_bytes < c.bytes) return refuse(me, "workspace has " + std::to_string(workspace_bytes) + " bytes, the call needs " + std::to_string(c.bytes));
             Attn8Params<T> p = {};
             p.batch = batch8_as(batch, pages, n_rows);
@@ -333,10 +370,13 @@ extern "C" int lmrs_b200_paged8_attention(const lmrs_b200_pages8_t* pages, const
                 if (pages->block == 1 << i) p.block_shift = i;
             }
             static std::atomic<uint64_t> allowed{0};
-            auto kernel = rows16_codes_kernel<T, FORM, DP>;
+            auto kernel = rows8_kernel<T, FORM, DP, ROW_TILES>;
             cudaError_t e = allow_smem(kernel, device, S::SMEM, allowed);
             if (e != cudaSuccess) return refuse(me, cudaGetErrorString(e));
-            kernel<<<(unsigned)c.own.ctas, S::THREADS, S::SMEM, (cudaStream_t)stream>>>(p, c.own);
+            if (!(p.err = gave_up_word.get())) return refuse(me, "out of host memory");
+            Boxes8 boxes = {};
+            box_maps8<S>(pages, boxes);
+            kernel<<<(unsigned)c.own.ctas, S::THREADS, S::SMEM, (cudaStream_t)stream>>>(p, c.own, boxes);
             if (launched(me)) return 1;
             // (which join, as in paged.cu)
             const int64_t items = n_rows * q_heads;

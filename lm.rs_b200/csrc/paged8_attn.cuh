@@ -8,8 +8,11 @@
 // The queries' types: float16 as it is; bfloat16, whose 8 bits of mantissa float16 has, times a power of two for each row that brings its largest element to 2^14 (what is below 2^-38 of that loses
 // bits: 2^-40 of the largest element at most); float32 the same way in three pieces of 11 bits each.  Weights in float16: up to 2^7, rounded by 2^-11 of each and 2^-32 of the largest; float32: in three pieces.
 #pragma once
+#include <float.h>
+
 #include "paged8.h"
 #include "paged_attn.cuh"
+#include "paged_tensor.cuh"
 
 namespace lmrs {
 namespace paged {
@@ -57,7 +60,8 @@ PG_DEVINL float2 row_factor(float most) {
     const int e = min(253, 268 - (int)(__float_as_uint(most) >> 23));
     return make_float2(__uint_as_float((uint32_t)e << 23), __uint_as_float((uint32_t)(254 - e) << 23));
 }
-constexpr float SHIFT8 = 7.0f;   // m is so much less than the largest exponent
+constexpr float SHIFT8 = 7.0f;   // m is so much less than the largest exponent when it is set
+constexpr int TG_ROWS8 = 6 << 8;   // (a kernel that gave up: after those of dense_gemm.cuh)
 // the exponent and the reciprocal of a scale of values (a scale that is NaN leaves a finite reciprocal: it reaches whoever has the weight)
 PG_DEVINL float2 value_terms(float v) {
     const float c = fminf(fmaxf(v, SCALE_LEAST), SCALE_MOST);
@@ -67,27 +71,50 @@ PG_DEVINL float2 value_terms(float v) {
     return make_float2(v == v ? lg : v, by);
 }
 
-// CTA = 4 warps that share a tile's keys, as in rows16_kernel.  What bounds it is the bytes of the pages, and next to them the conversions: 16 codes a lane take 4 to 6 instructions for each 4.
-template <typename T, int DP> struct TileShape8 {
+// CTA = 4 warps that share a tile's keys: a warp copies its own WARP_KEYS of them to its own slots, a tile or two ahead, and works on them by itself; the warps meet only where parts begin and end.  Codes
+// come by TMA, a piece of a page at a time, where all of a warp's keys are within the unit's (else, and where strides or pages take no tensor map, 16 bytes a lane, zeros for what is not there); scales 4 bytes a lane.
+template <typename T, int DP, int ROW_TILES> struct TileShape8 {
     static constexpr int PIECES = sizeof(T) == 4 ? 3 : 1;   // of queries and weights
-    static constexpr int ROWS = 16, THREADS = 128, ROW = DP, CHUNKS = DP / 16, KEYS = DP <= 128 ? 128 : 64, STAGES = DP > 128 || (sizeof(T) == 4 && DP > 64) ? 2 : 3;
-    static constexpr int WARP_KEYS = KEYS / 4, COPY_KEYS = KEYS / 32, TILES = WARP_KEYS / 8;   // keys a warp works on; keys a thread copies a quarter of; 8 keys' scores
-    static constexpr int Q_ROW = DP * (int)sizeof(T), Q = ROWS * Q_ROW, KV = KEYS * ROW, STAGE = 2 * KV + 8 * KEYS, SMEM = STAGES * (STAGE + Q);
-    static constexpr int CTAS = DP <= 64 ? 3 : 2;
+    static constexpr int ROWS = 8 * ROW_TILES, WARPS = 4, THREADS = 32 * WARPS, CHUNKS = DP / 16, WARP_KEYS = DP <= 128 ? 32 : 16, KEYS = WARPS * WARP_KEYS, STAGES = 2;
+    static constexpr int KEY_TILES = WARP_KEYS / 16;        // products take 16 keys and 8 rows
+    static constexpr int BOX = DP < 128 ? DP : 128;         // columns of a box: the bytes of a row of codes in shared memory
+    static constexpr int KV = WARP_KEYS * DP, SLOT = 2 * KV, Q_ROW = DP * (int)sizeof(T), Q = ROWS * Q_ROW;
+    static constexpr int SCALES = 2 * WARP_KEYS;            // floats of a slot: the keys', the values' (their logarithms, later); and a warp's WARP_KEYS reciprocals of values'
+    static constexpr int SMEM = 1024 + WARPS * STAGES * SLOT + Q + WARPS * (STAGES * SCALES + WARP_KEYS) * 4;
+    static constexpr int CTAS = ROW_TILES == 1 ? (DP <= 64 ? 4 : sizeof(T) == 4 && DP > 64 ? 2 : 3) : sizeof(T) == 4 ? (DP <= 64 ? 3 : 2) : DP <= 64 ? 4 : DP <= 128 ? 3 : 2;
     static constexpr int COLS = DP < 128 ? DP : 128;        // columns at a time where the warps' rows meet
-    static_assert(4 * ROWS * COLS * 4 <= 2 * KV, "the four warps' rows fit where a tile's keys and values were");
+    static_assert(ROWS * COLS * 4 <= SLOT, "a warp's rows fit where its keys and values were");
+    static_assert(CTAS * (SMEM + 2560) <= 233472, "they fit an SM");
 };
-// rows of 64 bytes: two of them make a line of the banks
-template <int ROW> PG_DEVINL uint32_t code_at(int row, int piece) { return (uint32_t)(row * ROW + ((piece ^ (ROW == 64 ? row >> 1 & 3 : row & 7)) << 4)); }
-template <int COLS> PG_DEVINL int sum8_at(int r, int c) { return r * COLS + (c ^ ((r & 1) << 4)); }
+// a row's 16-byte pieces, rotated as TMA does (SWIZZLE_128B, and SWIZZLE_64B for rows of 64 bytes)
+template <typename S> PG_DEVINL uint32_t code_at(int row, int piece) {
+    if constexpr (S::BOX == 64) return (uint32_t)(row * 64 + ((piece ^ (row >> 1 & 3)) << 4));
+    else return (uint32_t)((piece >> 3) * (S::WARP_KEYS * 128) + row * 128 + (((piece & 7) ^ (row & 7)) << 4));
+}
+template <int COLS> PG_DEVINL int sum8_at(int r, int c) { return r * COLS + (c ^ ((r >> 1 & 3) << 3)); }
 
-template <typename T, int FORM, int DP> struct WarpTile8 {
-    using S = TileShape8<T, DP>;
+// How codes come by TMA: `rows` keys of a page at a time (0: never); the maps' dimensions as in paged_tensor.cuh
+struct Boxes8 {
+    CUtensorMap k, v;
+    int rows, k_place, k_head, v_place, v_head;
+};
+
+PG_DEVINL uint32_t transpose8(uint32_t v) {   // 8 x 8 elements of 16 bits, a row four lanes
+    uint32_t r;
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+    return r;
+}
+
+// The products of one warp: mma.sync with 16 keys as the first operand's rows, 16 columns, and 8 rows of the unit as the second operand's columns: what there is to do for a row - scores, weights, sums - takes no
+// more registers and instructions than the unit's rows, and codes are converted once.  lane = 4 g + t
+template <typename T, int FORM, int DP, int ROW_TILES> struct WarpTile8 {
+    using S = TileShape8<T, DP, ROW_TILES>;
     static constexpr int N = S::PIECES;
-    uint32_t q[N == 1 ? S::CHUNKS : 1][4];   // (float32: cut into pieces again for each tile, since they do not fit the registers)
-    float o[S::CHUNKS][2][4];                // columns 16c + 4t + {0, 2} and {1, 3} of rows lane / 4 and lane / 4 + 8, t = lane % 4
-    float m[2], l[2], up[2], down[2];        // up: what the queries are multiplied by
-    bool seen[2];
+    uint32_t q[N == 1 ? S::CHUNKS : 1][ROW_TILES][2];   // columns 16c + 4t .. of row 8n + g (float32: cut into pieces again for each tile, since they do not fit the registers)
+    float o[S::CHUNKS][ROW_TILES][4];                   // columns 16c + 2g of rows 8n + 2t and 8n + 2t + 1, then 16c + 2g + 1
+    float m[ROW_TILES][2], l[ROW_TILES][2], up[ROW_TILES], down[ROW_TILES][2];   // of rows 2t, 2t + 1, but up: what row g's queries are multiplied by; down: the dot products (times the scale, where there is no cap)
+    int limit[ROW_TILES][2];                            // keys of the unit that the rows see
+    bool seen[ROW_TILES][2];
     // four elements of row r, columns 16c + 4t ..
     PG_DEVINL static float4 load_q(uint32_t q_at, int r, int c) {
         const int t = threadIdx.x & 3;
@@ -102,293 +129,331 @@ template <typename T, int FORM, int DP> struct WarpTile8 {
             return make_float4(x.x, x.y, y.x, y.y);
         }
     }
-    PG_DEVINL void begin(uint32_t q_at) {
-        const int g = (threadIdx.x & 31) >> 2;
+    PG_DEVINL void begin(const Attn8Params<T>& p, uint32_t q_at) {
+        const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
         __syncwarp();
 #pragma unroll
-        for (int i = 0; i < 2; i++) {
-            float most = 0.0f;
+        for (int n = 0; n < ROW_TILES; n++) {
+            float2 f = make_float2(1.0f, 1.0f);
             if constexpr (!std::is_same<T, __half>::value) {
+                float most = 0.0f;
 #pragma unroll
                 for (int c = 0; c < S::CHUNKS; c++) {
-                    const float4 v = load_q(q_at, g + 8 * i, c);
+                    const float4 v = load_q(q_at, 8 * n + g, c);
                     most = fmaxf(fmaxf(fmaxf(most, fabsf(v.x)), fmaxf(fabsf(v.y), fabsf(v.z))), fabsf(v.w));
                 }
                 most = fmaxf(most, __shfl_xor_sync(~0u, most, 1));
                 most = fmaxf(most, __shfl_xor_sync(~0u, most, 2));
-                const float2 f = row_factor(most);
-                up[i] = f.x;
-                down[i] = f.y;
-            } else {
-                up[i] = down[i] = 1.0f;
+                f = row_factor(most);
             }
+            up[n] = f.x;
             if constexpr (N == 1) {
 #pragma unroll
                 for (int c = 0; c < S::CHUNKS; c++) {
-                    const float4 v = load_q(q_at, g + 8 * i, c);
-                    q[c][i] = to_halves(v.x * up[i], v.y * up[i]);
-                    q[c][2 + i] = to_halves(v.z * up[i], v.w * up[i]);
+                    const float4 v = load_q(q_at, 8 * n + g, c);
+                    q[c][n][0] = to_halves(v.x * f.x, v.y * f.x);
+                    q[c][n][1] = to_halves(v.z * f.x, v.w * f.x);
                 }
             }
-            m[i] = -INFINITY;
-            l[i] = 0.0f;
-            seen[i] = false;
+            if (!(p.softcap > 0.0f)) f.y = fminf(fmaxf(f.y * p.scale2, -FLT_MAX), FLT_MAX);
+#pragma unroll
+            for (int i = 0; i < 2; i++) {
+                down[n][i] = __shfl_sync(~0u, f.y, 8 * t + 4 * i);
+                m[n][i] = -INFINITY;
+                l[n][i] = 0.0f;
+                seen[n][i] = false;
+            }
         }
 #pragma unroll
         for (int c = 0; c < S::CHUNKS; c++)
 #pragma unroll
-            for (int k = 0; k < 4; k++) o[c][0][k] = o[c][1][k] = 0.0f;
+            for (int n = 0; n < ROW_TILES; n++)
+#pragma unroll
+                for (int k = 0; k < 4; k++) o[c][n][k] = 0.0f;
     }
-    // there: bit j: key j of the warp's is there; first: number of its first key; row_keys: how many keys each row sees; ks, vs: the warp's keys' scales in shared memory, by: room for as many floats
-    PG_DEVINL void tile(const Attn8Params<T>& p, uint32_t q_at, uint32_t k_at, uint32_t v_at, uint32_t there, int first, const int* row_keys, float* ks, float* vs, float* by) {
-        const int lane = threadIdx.x & 31, t = lane & 3, key0 = S::WARP_KEYS * (threadIdx.x >> 5);
-        float s[S::TILES][4] = {};
+    // there: bit j: key j of the warp's is there; first: number of its first key; scales: of the warp's keys and values in shared memory; by: room for the values' reciprocals
+    PG_DEVINL void tile(const Attn8Params<T>& p, uint32_t q_at, uint32_t k_at, uint32_t v_at, uint32_t there, int first, float* scales, float* by) {
+        const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+        float *ks = scales, *vs = scales + S::WARP_KEYS;
+        float s[S::KEY_TILES][ROW_TILES][4] = {};   // keys 16j + g of rows 2t and 2t + 1, then keys 16j + g + 8
         if (lane < S::WARP_KEYS) {   // (in their places)
             const float2 v = value_terms(vs[lane]);
             vs[lane] = v.x;
             by[lane] = v.y;
         }
         __syncwarp();   // (ldmatrix and mma are for a warp in step)
-        // keys: a matrix is 8 keys of 16 columns; a lane gets columns 4t .. 4t + 3 of key lane / 4, which stand for rows 2t, 2t + 1, 2t + 8 and 2t + 9 of the product's second operand, as the queries' do for
-        // columns of the first
+        // keys: a matrix is 8 keys of 16 columns; a lane gets columns 4t .. 4t + 3 of key g, which stand for columns 2t, 2t + 1, 2t + 8 and 2t + 9 of the product, as the queries' do
 #pragma unroll
-        for (int c = 0; c < S::CHUNKS; c += 4 / S::TILES) {
+        for (int c = 0; c < S::CHUNKS; c += 2 / S::KEY_TILES) {
             uint32_t w[4];
-            if constexpr (S::TILES == 4) ldmatrix4(w, k_at + code_at<S::ROW>(key0 + lane, c));
-            else ldmatrix4(w, k_at + code_at<S::ROW>(key0 + (lane & 15), c + (lane >> 4)));
+            if constexpr (S::KEY_TILES == 2) ldmatrix4(w, k_at + code_at<S>(lane, c));
+            else ldmatrix4(w, k_at + code_at<S>(lane & 15, c + (lane >> 4)));
 #pragma unroll
-            for (int d = 0; d < 4 / S::TILES; d++) {
-                uint32_t a[N][4];
-                if constexpr (N == 1) {
+            for (int d = 0; d < 2 / S::KEY_TILES; d++) {
+                uint32_t b[N][ROW_TILES][2];
 #pragma unroll
-                    for (int k = 0; k < 4; k++) a[0][k] = q[c + d][k];
-                } else {
-#pragma unroll
-                    for (int i = 0; i < 2; i++) {
-                        const float4 v = load_q(q_at, lane / 4 + 8 * i, c + d);
+                for (int n = 0; n < ROW_TILES; n++) {
+                    if constexpr (N == 1) {
+                        b[0][n][0] = q[c + d][n][0];
+                        b[0][n][1] = q[c + d][n][1];
+                    } else {
+                        const float4 v = load_q(q_at, 8 * n + g, c + d);
                         uint32_t x[N], y[N];
-                        split_halves<N>(v.x * up[i], v.y * up[i], x);
-                        split_halves<N>(v.z * up[i], v.w * up[i], y);
+                        split_halves<N>(v.x * up[n], v.y * up[n], x);
+                        split_halves<N>(v.z * up[n], v.w * up[n], y);
 #pragma unroll
-                        for (int k = 0; k < N; k++) { a[k][i] = x[k]; a[k][2 + i] = y[k]; }
+                        for (int k = 0; k < N; k++) { b[k][n][0] = x[k]; b[k][n][1] = y[k]; }
                     }
                 }
 #pragma unroll
-                for (int n = 0; n < S::TILES; n++) {
-                    uint32_t b0, b1;
-                    codes_to_halves<FORM, 0>(w[S::TILES * d + n], b0, b1);
+                for (int j = 0; j < S::KEY_TILES; j++) {
+                    uint32_t a[4];
+                    codes_to_halves<FORM, 0>(w[2 * (S::KEY_TILES * d + j)], a[0], a[2]);
+                    codes_to_halves<FORM, 0>(w[2 * (S::KEY_TILES * d + j) + 1], a[1], a[3]);
 #pragma unroll
-                    for (int k = N - 1; k >= 0; k--) mma16816(s[n], a[k], b0, b1, __half());
+                    for (int n = 0; n < ROW_TILES; n++)
+#pragma unroll
+                        for (int k = N - 1; k >= 0; k--) mma16816(s[j][n], a, b[k][n][0], b[k][n][1], __half());
                 }
             }
         }
-        // scores
+        // scores, in powers of two, and the values' scales
 #pragma unroll
-        for (int n = 0; n < S::TILES; n++) {
-            const float2 k = *reinterpret_cast<const float2*>(ks + 8 * n + 2 * t);
+        for (int j = 0; j < S::KEY_TILES; j++) {
+            const float k[2] = {ks[16 * j + g], ks[16 * j + g + 8]}, v[2] = {vs[16 * j + g], vs[16 * j + g + 8]};
+            if (p.softcap > 0.0f) {
+                float flat[4 * ROW_TILES];
 #pragma unroll
-            for (int i = 0; i < 2; i++) {
-                s[n][2 * i] *= down[i] * k.x;
-                s[n][2 * i + 1] *= down[i] * k.y;
-            }
-        }
-        if (p.softcap > 0.0f) {
-            float flat[4 * S::TILES];
+                for (int i = 0; i < 4 * ROW_TILES; i++) flat[i] = s[j][i >> 2][i & 3] * down[i >> 2][i & 1] * k[i >> 1 & 1];
+                cap_scores(p, flat);
 #pragma unroll
-            for (int i = 0; i < 4 * S::TILES; i++) flat[i] = s[i >> 2][i & 3];
-            cap_scores(p, flat);
+                for (int i = 0; i < 4 * ROW_TILES; i++) s[j][i >> 2][i & 3] = flat[i] + v[i >> 1 & 1];
+            } else {
 #pragma unroll
-            for (int i = 0; i < 4 * S::TILES; i++) s[i >> 2][i & 3] = flat[i];
-        } else {
-#pragma unroll
-            for (int i = 0; i < 4 * S::TILES; i++) s[i >> 2][i & 3] *= p.scale2;
-        }
-#pragma unroll
-        for (int n = 0; n < S::TILES; n++) {
-            const float2 v = *reinterpret_cast<const float2*>(vs + 8 * n + 2 * t);
-#pragma unroll
-            for (int i = 0; i < 2; i++) {
-                s[n][2 * i] += v.x;
-                s[n][2 * i + 1] += v.y;
+                for (int i = 0; i < 4 * ROW_TILES; i++) s[j][i >> 2][i & 3] = fmaf(s[j][i >> 2][i & 3] * k[i >> 1 & 1], down[i >> 2][i & 1], v[i >> 1 & 1]);
             }
         }
         constexpr uint32_t ALL = S::WARP_KEYS == 32 ? ~0u : (1u << S::WARP_KEYS % 32) - 1;
-        const int limit[2] = {row_keys[lane / 4] - first, row_keys[lane / 4 + 8] - first};
-        if (!__all_sync(~0u, there == ALL && limit[0] >= S::WARP_KEYS && limit[1] >= S::WARP_KEYS)) {
+        int least = limit[0][0];
 #pragma unroll
-            for (int i = 0; i < 2; i++) {
-                const uint32_t sees = there & (limit[i] >= S::WARP_KEYS ? ALL : limit[i] <= 0 ? 0u : (1u << limit[i]) - 1);
-                seen[i] = seen[i] || sees;
+        for (int i = 1; i < 2 * ROW_TILES; i++) least = min(least, limit[i >> 1][i & 1]);
+        if (!__all_sync(~0u, there == ALL && least - first >= S::WARP_KEYS)) {
 #pragma unroll
-                for (int n = 0; n < S::TILES; n++)
+            for (int n = 0; n < ROW_TILES; n++)
 #pragma unroll
-                    for (int c = 0; c < 2; c++)
-                        if (!(sees >> (8 * n + 2 * t + c) & 1)) s[n][2 * i + c] = -INFINITY;
-            }
+                for (int i = 0; i < 2; i++) {
+                    const int left = limit[n][i] - first;
+                    const uint32_t sees = there & (left >= S::WARP_KEYS ? ALL : left <= 0 ? 0u : (1u << left) - 1);
+                    seen[n][i] = seen[n][i] || sees;
+#pragma unroll
+                    for (int k = 0; k < 2 * S::KEY_TILES; k++)
+                        if (!(sees >> (8 * k + g) & 1)) s[k >> 1][n][2 * (k & 1) + i] = -INFINITY;
+                }
         } else {
-            seen[0] = seen[1] = true;
+#pragma unroll
+            for (int n = 0; n < ROW_TILES; n++) seen[n][0] = seen[n][1] = true;
         }
-        float now[2] = {-INFINITY, -INFINITY};
+        float now[ROW_TILES][2];
+        bool grows = false;
 #pragma unroll
-        for (int i = 0; i < 2; i++)
-#pragma unroll
-            for (int n = 0; n < S::TILES; n++) now[i] = fmaxf(now[i], fmaxf(s[n][2 * i], s[n][2 * i + 1]));
-#pragma unroll
-        for (int d = 1; d < 4; d *= 2)
-#pragma unroll
-            for (int i = 0; i < 2; i++) now[i] = fmaxf(now[i], __shfl_xor_sync(~0u, now[i], d));
-        if (__any_sync(~0u, now[0] - SHIFT8 > m[0] || now[1] - SHIFT8 > m[1])) {
+        for (int n = 0; n < ROW_TILES; n++)
 #pragma unroll
             for (int i = 0; i < 2; i++) {
-                const float top = fmaxf(m[i], now[i] - SHIFT8), corr = ex2(m[i] - (top == -INFINITY ? 0.0f : top));
-                m[i] = top;
-                l[i] *= corr;
-#pragma unroll
-                for (int c = 0; c < S::CHUNKS; c++)
-#pragma unroll
-                    for (int h = 0; h < 2; h++) { o[c][h][2 * i] *= corr; o[c][h][2 * i + 1] *= corr; }
+                now[n][i] = fmaxf(s[0][n][i], s[0][n][2 + i]);
+                if (S::KEY_TILES == 2) now[n][i] = fmaxf(now[n][i], fmaxf(s[S::KEY_TILES - 1][n][i], s[S::KEY_TILES - 1][n][2 + i]));
+                grows = grows || now[n][i] > m[n][i] + (SHIFT8 + 8.0f);
             }
+        // m is raised when an exponent is 8 above it, which is rare after the first tiles: weights stay below 2^15
+        if (__any_sync(~0u, grows)) {
+#pragma unroll
+            for (int n = 0; n < ROW_TILES; n++)
+#pragma unroll
+                for (int i = 0; i < 2; i++) {
+#pragma unroll
+                    for (int d = 4; d < 32; d *= 2) now[n][i] = fmaxf(now[n][i], __shfl_xor_sync(~0u, now[n][i], d));
+                    const float top = fmaxf(m[n][i], now[n][i] - SHIFT8), corr = ex2(m[n][i] - (top == -INFINITY ? 0.0f : top));
+                    m[n][i] = top;
+                    l[n][i] *= corr;
+#pragma unroll
+                    for (int c = 0; c < S::CHUNKS; c++) { o[c][n][i] *= corr; o[c][n][2 + i] *= corr; }
+                }
         }
-        // weights, as the first operand: 16 keys a step
-        uint32_t a[S::TILES / 2][N][4];
-        const float base[2] = {m[0] == -INFINITY ? 0.0f : m[0], m[1] == -INFINITY ? 0.0f : m[1]};
+        // weights, as the second operand: 16 keys a step
+        uint32_t b[S::KEY_TILES][N][ROW_TILES][2];
 #pragma unroll
-        for (int n = 0; n < S::TILES; n++) {
-            const float2 f = *reinterpret_cast<const float2*>(by + 8 * n + 2 * t);
+        for (int n = 0; n < ROW_TILES; n++) {
+            const float base[2] = {m[n][0] == -INFINITY ? 0.0f : m[n][0], m[n][1] == -INFINITY ? 0.0f : m[n][1]};
 #pragma unroll
-            for (int i = 0; i < 2; i++) {
-                const float x = ex2(s[n][2 * i] - base[i]), y = ex2(s[n][2 * i + 1] - base[i]);
-                l[i] = fmaf(x, f.x, fmaf(y, f.y, l[i]));   // (of this lane's keys: the four lanes of a row meet at the end)
+            for (int k = 0; k < 2 * S::KEY_TILES; k++) {
+                const float f = by[8 * k + g], x = ex2(s[k >> 1][n][2 * (k & 1)] - base[0]), y = ex2(s[k >> 1][n][2 * (k & 1) + 1] - base[1]);
+                l[n][0] = fmaf(x, f, l[n][0]);   // (of this lane's keys: the eight lanes of a row meet at the end)
+                l[n][1] = fmaf(y, f, l[n][1]);
                 uint32_t w[N];
                 split_halves<N>(x, y, w);
 #pragma unroll
-                for (int k = 0; k < N; k++) a[n >> 1][k][2 * (n & 1) + i] = w[k];
+                for (int i = 0; i < N; i++) b[k >> 1][i][n][k & 1] = transpose8(w[i]);
             }
         }
-        // values: a matrix is 8 keys of 16 columns, transposed in pairs of columns: a lane gets columns 2 (lane / 4) and the next of keys 2t and 2t + 1, so even and odd columns are products of their own
+        // values: a matrix is 8 keys of 16 columns, transposed in pairs of columns: a lane gets columns 2g and 2g + 1 of keys 2t and 2t + 1; rows g and g + 8 of the product stand for them
 #pragma unroll
-        for (int c = 0; c < S::CHUNKS; c += 4 / S::TILES) {
+        for (int c = 0; c < S::CHUNKS; c += 2 / S::KEY_TILES) {
             uint32_t w[4];
-            if constexpr (S::TILES == 4) ldmatrix4t(w, v_at + code_at<S::ROW>(key0 + lane, c));
-            else ldmatrix4t(w, v_at + code_at<S::ROW>(key0 + (lane & 15), c + (lane >> 4)));
+            if constexpr (S::KEY_TILES == 2) ldmatrix4t(w, v_at + code_at<S>(lane, c));
+            else ldmatrix4t(w, v_at + code_at<S>(lane & 15, c + (lane >> 4)));
 #pragma unroll
-            for (int d = 0; d < 4 / S::TILES; d++)
+            for (int d = 0; d < 2 / S::KEY_TILES; d++)
 #pragma unroll
-                for (int j = 0; j < S::TILES / 2; j++) {
-                    uint32_t even[2], odd[2];
-                    codes_to_halves<FORM, 1>(w[S::TILES * d + 2 * j], even[0], odd[0]);
-                    codes_to_halves<FORM, 1>(w[S::TILES * d + 2 * j + 1], even[1], odd[1]);
+                for (int j = 0; j < S::KEY_TILES; j++) {
+                    uint32_t a[4];
+                    codes_to_halves<FORM, 1>(w[2 * (S::KEY_TILES * d + j)], a[0], a[1]);
+                    codes_to_halves<FORM, 1>(w[2 * (S::KEY_TILES * d + j) + 1], a[2], a[3]);
 #pragma unroll
-                    for (int k = N - 1; k >= 0; k--) {
-                        mma16816(o[c + d][0], a[j][k], even[0], even[1], __half());
-                        mma16816(o[c + d][1], a[j][k], odd[0], odd[1], __half());
-                    }
+                    for (int n = 0; n < ROW_TILES; n++)
+#pragma unroll
+                        for (int k = N - 1; k >= 0; k--) mma16816(o[c + d][n], a, b[j][k][n][0], b[j][k][n][1], __half());
                 }
         }
     }
-    PG_DEVINL void put_ml(float2* ml) {   // [16]
+    PG_DEVINL void put_ml(float2* ml) {   // [ROWS]
         const int lane = threadIdx.x & 31;
 #pragma unroll
-        for (int i = 0; i < 2; i++) {
-            l[i] += __shfl_xor_sync(~0u, l[i], 1);
-            l[i] += __shfl_xor_sync(~0u, l[i], 2);
-            if ((lane & 3) == 0) ml[lane / 4 + 8 * i] = make_float2(m[i], seen[i] ? l[i] : -1.0f);
-        }
+        for (int n = 0; n < ROW_TILES; n++)
+#pragma unroll
+            for (int i = 0; i < 2; i++) {
+                const bool any = __shfl_sync(~0u, (int)seen[n][i], lane & 3);   // (the same for the lanes of a row)
+#pragma unroll
+                for (int d = 4; d < 32; d *= 2) l[n][i] += __shfl_xor_sync(~0u, l[n][i], d);
+                if (lane < 4) ml[8 * n + 2 * lane + i] = make_float2(m[n][i], any ? l[n][i] : -1.0f);
+            }
     }
-    // [16][COLS] as sum8_at has them, columns from COLS * pass on, times the rows' factors (lane r has row r's)
+    // [ROWS][COLS] as sum8_at has them, columns from COLS * pass on, times the rows' factors (lane r has row r's)
     PG_DEVINL void put_o(float* to, float factor, int pass) {
-        const int lane = threadIdx.x & 31, t = lane & 3;
+        const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
 #pragma unroll
-        for (int i = 0; i < 2; i++) {
-            const int r = lane / 4 + 8 * i;
-            const float f = __shfl_sync(~0u, factor, r);
+        for (int n = 0; n < ROW_TILES; n++)
 #pragma unroll
-            for (int c = 0; c < S::CHUNKS; c++)
-                if (c / (S::COLS / 16) == pass)
-                    *reinterpret_cast<float4*>(to + sum8_at<S::COLS>(r, 16 * (c % (S::COLS / 16)) + 4 * t)) =
-                        make_float4(o[c][0][2 * i] * f, o[c][1][2 * i] * f, o[c][0][2 * i + 1] * f, o[c][1][2 * i + 1] * f);
-        }
+            for (int i = 0; i < 2; i++) {
+                const int r = 8 * n + 2 * t + i;
+                const float f = __shfl_sync(~0u, factor, r);
+#pragma unroll
+                for (int c = 0; c < S::CHUNKS; c++)
+                    if (c / (S::COLS / 16) == pass)
+                        *reinterpret_cast<float2*>(to + sum8_at<S::COLS>(r, 16 * (c % (S::COLS / 16)) + 2 * g)) = make_float2(o[c][n][i] * f, o[c][n][2 + i] * f);
+            }
     }
 };
 
-template <typename T, int FORM, int DP>
-__global__ void __launch_bounds__(TileShape8<T, DP>::THREADS, TileShape8<T, DP>::CTAS) rows16_codes_kernel(const __grid_constant__ Attn8Params<T> p, const __grid_constant__ Line l) {
-    using S = TileShape8<T, DP>;
-    extern __shared__ __align__(1024) uint8_t smem[];
-    __shared__ Walk walks[S::STAGES];             // of the units that copies have got to, by their number in this CTA modulo STAGES
-    __shared__ int row_keys[S::STAGES][S::ROWS];
-    __shared__ __align__(16) uint8_t there[S::STAGES][S::KEYS / 8];
-    __shared__ float2 ml[4][S::ROWS];
-    __shared__ float2 joined[S::ROWS];
-    __shared__ __align__(16) float by[S::KEYS];
-    const int t = threadIdx.x, lane = t & 31, warp = t >> 5, D = p.head_size;
-    const uint32_t kv = smem_at(smem), queries = kv + S::STAGES * S::STAGE;
+template <typename T, int FORM, int DP, int ROW_TILES>
+__global__ void __launch_bounds__(TileShape8<T, DP, ROW_TILES>::THREADS, TileShape8<T, DP, ROW_TILES>::CTAS) rows8_kernel(const __grid_constant__ Attn8Params<T> p, const __grid_constant__ Line l, const __grid_constant__ Boxes8 boxes) {
+    using S = TileShape8<T, DP, ROW_TILES>;
+    extern __shared__ uint8_t raw[];
+    __shared__ Walk walks[S::WARPS][S::STAGES];   // a warp's: of the units that its copies have got to, by their number in this CTA modulo STAGES
+    __shared__ uint64_t full[S::WARPS][S::STAGES];
+    __shared__ float2 ml[S::WARPS][S::ROWS];
+    __shared__ int gave_up_at;
+    const int t = threadIdx.x, lane = t & 31, warp = __shfl_sync(~0u, t >> 5, 0), D = p.head_size;
+    uint8_t* smem = raw + (((smem_at(raw) + 1023u) & ~1023u) - smem_at(raw));
+    uint8_t *slots = smem + warp * (S::STAGES * S::SLOT), *queries = smem + S::WARPS * S::STAGES * S::SLOT;
+    float* scales = reinterpret_cast<float*>(queries + S::Q) + warp * (S::STAGES * S::SCALES + S::WARP_KEYS);
+    volatile int* gave_up = &gave_up_at;
+    if (t < S::WARPS * S::STAGES) mbar_init(&full[0][0] + t, 1);
+    if (t == 0) gave_up_at = 0;
+    fence_barrier_init();
 
     Walk ahead;   // where copies are
     int64_t from, to;
-    walk_begin<T, S::THREADS>(p, l, ahead, from, to);
+    walk_begin<T, S::THREADS>(p, l, ahead, from, to);   // (synchronises the CTA)
     grid_launch();
     // The kernel before may still run.  The last CTA ends after it, so that whoever waits for this kernel waits for both; the others leave their SM to the next ones
     const bool last_cta = blockIdx.x == gridDim.x - 1;
     if (from >= to) { if (last_cta) grid_wait(); return; }
 
-    // copies of a thread: keys t / 4, t / 4 + 32, ... of the tile, every fourth 16 bytes; past the end of a head zeros, so that the products need not know where it is; the first and second of four
-    // neighbours also copy the keys' and the values' scales
-    Place place[S::COPY_KEYS];
     const int n_tiles = (int)(to - from), whole = D / 16;
-    int copied = 0, stage_to = 0, set_to = 0;   // tiles copied, the stage and the unit's set that the next goes to
-    bool first = true;
-    auto look = [&]() {
+    int copied = 0, slot_to = 0, set_to = 0;    // tiles copied, the slot and the unit's set that the next goes to
+    bool first = true, ok = true;
+    uint32_t there[S::STAGES], by_tma = 0, written = 0, rounds = 0;   // a bit a slot: a tile is on its way by TMA, its bytes were last written otherwise, the phase that its barrier is in
+    int page = -1, at_page = 0;   // of this lane's key in the tile that is copied next: what its table says (looked at when the copies are asked for, so that nothing waits for it), and its place there
+    auto copy_queries = [&](const Walk& w) {   // by all threads
+        constexpr int PIECES = S::Q_ROW / 16, VEC = 16 / sizeof(T);
+        for (int e = t; e < S::ROWS * PIECES; e += S::THREADS) {
+            const int x = e / PIECES, c = e % PIECES;
+            const UnitRow r = unit_row(p, l, w, x);
+            const bool in = r.row >= 0 && c * VEC < D;
+            const T* q = in ? p.q.data + r.row * p.q.row + r.head * p.q.head + c * VEC : p.q.data;
+            uint8_t* to_q = queries + piece_at(x, c, S::Q_ROW);
+            if (p.q_wide) {
+                copy16(smem_at(to_q), q, in);
+            } else {
+                Piece<T, VEC> v;
 #pragma unroll
-        for (int i = 0; i < S::COPY_KEYS; i++) place[i] = unit_place(p, ahead, ahead.tile * S::KEYS + t / 4 + 32 * i);
-    };
-    auto copy_tile = [&]() {   // the tile that `ahead` stands at, whose places are known; then on to the next one
-        if (copied < n_tiles) {
-            const uint32_t stage = kv + stage_to * S::STAGE;
-#pragma unroll
-            for (int i = 0; i < S::COPY_KEYS; i++) {
-                const bool is = place[i].page >= 0;
-                const int page = is ? place[i].page : 0, row = t / 4 + 32 * i;
-                const uint8_t* k = p.c.k + page * p.c.k_page + place[i].place * p.c.k_slot + ahead.head * p.c.k_head;
-                const uint8_t* v = p.c.v + page * p.c.v_page + place[i].place * p.c.v_slot + ahead.head * p.c.v_head;
-#pragma unroll
-                for (int c = 0; c < S::CHUNKS; c += 4) {
-                    const int piece = c + (t & 3);
-                    const bool in = is && (S::CHUNKS == whole || piece < whole);
-                    copy16(stage + code_at<S::ROW>(row, piece), in ? k + 16 * piece : p.c.k, in);
-                    copy16(stage + S::KV + code_at<S::ROW>(row, piece), in ? v + 16 * piece : p.c.v, in);
-                }
-                if ((t & 3) < 2) {
-                    const int block = p.block_shift >= 0 ? place[i].place >> p.block_shift : place[i].place / p.c.block;
-                    const float* scale = (t & 3) ? p.c.vs + page * p.c.vs_page + block * p.c.vs_block + ahead.head * p.c.vs_head : p.c.ks + page * p.c.ks_page + block * p.c.ks_block + ahead.head * p.c.ks_head;
-                    copy4(stage + 2 * S::KV + 4 * (row + (t & 3) * S::KEYS), is ? scale : p.c.ks, is);
-                }
-                const unsigned bits = __ballot_sync(~0u, __shfl_sync(~0u, is, (4 * lane) & 31)) & 0xff;
-                if (lane == 0) there[stage_to][warp + 4 * i] = (uint8_t)bits;
+                for (int i = 0; i < VEC; i++) v.v[i] = in ? q[i] : from_f<T>(0.0f);
+                *reinterpret_cast<Piece<T, VEC>*>(to_q) = v;
             }
-            if (first) {
-                if (t == 0) walks[set_to] = ahead;
-                if (t < S::ROWS) row_keys[set_to][t] = unit_row(p, l, ahead, t).keys;
-                const uint32_t q_at = queries + set_to * S::Q;
-                constexpr int PIECES = S::Q_ROW / 16, VEC = 16 / sizeof(T);
-                for (int e = t; e < S::ROWS * PIECES; e += S::THREADS) {
-                    const int x = e / PIECES, c = e % PIECES;
-                    const UnitRow r = unit_row(p, l, ahead, x);
-                    const bool in = r.row >= 0 && c * VEC < D;
-                    const T* q = in ? p.q.data + r.row * p.q.row + r.head * p.q.head + c * VEC : p.q.data;
-                    const uint32_t at = q_at + piece_at(x, c, S::Q_ROW);
-                    if (p.q_wide) {
-                        copy16(at, q, in);
-                    } else {
-                        Piece<T, VEC> v;
+        }
+        copy_commit();
+    };
+    auto look = [&]() {   // (as unit_place)
+        const int x = ahead.tile * S::KEYS + warp * S::WARP_KEYS + (lane & (S::WARP_KEYS - 1));
+        page = -1;
+        if (x < ahead.keys) {
+            const int i = p.page_shift >= 0 ? x >> p.page_shift : x / p.batch.page_size;
+            page = (ahead.b < 0 ? p.batch.prefix : p.batch.tables + ahead.b * p.batch.table_stride)[i];
+            at_page = x - i * p.batch.page_size;
+        }
+    };
+    // boxes of a lane: keys or values, rows, columns
+    constexpr int COL_BOXES = DP / S::BOX;
+    const int box_rows = boxes.rows, groups = box_rows ? S::WARP_KEYS / box_rows : 0, box = lane % max(1, 2 * COL_BOXES * groups), box_value = box & 1, box_col = (box >> 1) % COL_BOXES, box_group = (box >> 1) / COL_BOXES;
+    auto copy_tile = [&]() {   // the warp's part of the tile that `ahead` stands at, whose places are known; then on to the next one
+        if (copied < n_tiles) {
+            const bool is = page >= 0 && page < p.batch.pages;
+            const uint32_t to_codes = smem_at(slots) + slot_to * S::SLOT, bits = __ballot_sync(~0u, is) & (S::WARP_KEYS == 32 ? ~0u : (1u << S::WARP_KEYS % 32) - 1);
 #pragma unroll
-                        for (int i = 0; i < VEC; i++) v.v[i] = in ? q[i] : from_f<T>(0.0f);
-                        *reinterpret_cast<Piece<T, VEC>*>(smem + (at - kv)) = v;
+            for (int i = 0; i < S::STAGES; i++)
+                if (i == slot_to) there[i] = bits;
+            const int page_or_0 = is ? page : 0, at = is ? at_page : 0;
+            if (box_rows && ahead.tile * S::KEYS + (warp + 1) * S::WARP_KEYS <= ahead.keys) {
+                if (written >> slot_to & 1) asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                __syncwarp();
+                if (lane == 0) mbar_expect_tx(&full[warp][slot_to], S::SLOT);
+                int of = __shfl_sync(~0u, is ? page : -1, box_group * box_rows & 31), from_row = __shfl_sync(~0u, at, box_group * box_rows & 31);
+                if (of < 0) { of = p.batch.pages; from_row = 0; }   // (outside the map: zeros)
+                __syncwarp();
+                if (lane < 2 * COL_BOXES * groups)
+                    tma_box(to_codes + box_value * S::KV + box_col * (S::WARP_KEYS * S::BOX) + box_group * box_rows * S::BOX, box_value ? &boxes.v : &boxes.k, S::BOX * box_col, from_row, ahead.head, of,
+                            box_value ? boxes.v_place : boxes.k_place, box_value ? boxes.v_head : boxes.k_head, &full[warp][slot_to]);
+                __syncwarp();
+                by_tma |= 1u << slot_to;
+                written &= ~(1u << slot_to);
+            } else {
+                by_tma &= ~(1u << slot_to);
+                written |= 1u << slot_to;
+                const int64_t k_from = is ? page_or_0 * p.c.k_page + at * p.c.k_slot + ahead.head * p.c.k_head : -1, v_from = is ? page_or_0 * p.c.v_page + at * p.c.v_slot + ahead.head * p.c.v_head : -1;
+                constexpr int LANES = S::CHUNKS < 8 ? S::CHUNKS : 8, AT_ONCE = 32 / LANES;   // lanes a row, rows at a time
+#pragma unroll 2
+                for (int r0 = 0; r0 < S::WARP_KEYS; r0 += AT_ONCE) {
+                    const int row = r0 + lane / LANES;
+                    const int64_t k = __shfl_sync(~0u, k_from, row), v = __shfl_sync(~0u, v_from, row);
+#pragma unroll
+                    for (int c = 0; c < S::CHUNKS; c += LANES) {
+                        const int piece = c + lane % LANES;
+                        const bool in = k >= 0 && piece < whole;
+                        copy16(to_codes + code_at<S>(row, piece), in ? p.c.k + k + 16 * piece : p.c.k, in);
+                        copy16(to_codes + S::KV + code_at<S>(row, piece), in ? p.c.v + v + 16 * piece : p.c.v, in);
                     }
                 }
+            }
+            if (lane < S::WARP_KEYS) {
+                const int block = p.block_shift >= 0 ? at >> p.block_shift : at / p.c.block;
+                const uint32_t to_scale = smem_at(scales + slot_to * S::SCALES) + 4 * lane;
+                copy4(to_scale, p.c.ks + page_or_0 * p.c.ks_page + block * p.c.ks_block + ahead.head * p.c.ks_head, is);
+                copy4(to_scale + 4 * S::WARP_KEYS, p.c.vs + page_or_0 * p.c.vs_page + block * p.c.vs_block + ahead.head * p.c.vs_head, is);
+            }
+            if (first) {
+                if (lane == 0) walks[warp][set_to] = ahead;
                 first = false;
             }
-            stage_to = stage_to + 1 == S::STAGES ? 0 : stage_to + 1;
+            slot_to = slot_to + 1 == S::STAGES ? 0 : slot_to + 1;
             if (++copied < n_tiles) {
                 if (++ahead.tile == ahead.tiles) {
                     walk_next_unit(p, l, ahead);
@@ -404,84 +469,118 @@ __global__ void __launch_bounds__(TileShape8<T, DP>::THREADS, TileShape8<T, DP>:
 #pragma unroll 1
     for (int i = 0; i < S::STAGES - 1; i++) copy_tile();
 
-    WarpTile8<T, FORM, DP> tile;
-    Walk w;
-    int set = S::STAGES - 1, stage = S::STAGES - 1, begun = 0, used = 0;
+    WarpTile8<T, FORM, DP, ROW_TILES> tile;
+    int set = S::STAGES - 1, slot = S::STAGES - 1, begun = 0, now = 0, tiles = 0;   // now: the tile of the unit that is worked on
     bool start = true;
 #pragma unroll 1
     for (int at = 0; at < n_tiles; at++) {
-        copy_wait<S::STAGES - 2>();
-        __syncthreads();   // the tile has landed for all threads, and the one before has been worked on by all
-        copy_tile();
-        stage = stage + 1 == S::STAGES ? 0 : stage + 1;
-        const uint32_t k_at = kv + stage * S::STAGE, v_at = k_at + S::KV;
+        slot = slot + 1 == S::STAGES ? 0 : slot + 1;
         if (start) {
             set = set + 1 == S::STAGES ? 0 : set + 1;
-            w = walks[set];
-            begun = w.tile;
-            tile.begin(queries + set * S::Q);
-            used = w.b < 0 ? (int)min((int64_t)S::ROWS, p.batch.n_rows * p.group - (int64_t)w.row_tile * S::ROWS) : min(S::ROWS, w.s.count * p.group - w.row_tile * S::ROWS);
+            __syncwarp();
+            copy_queries(walks[warp][set]);
+            copy_wait<0>();
+            __syncthreads();          // the other warps' parts of them
+            tile.begin(p, smem_at(queries));
+            const Walk& w = walks[0][set];   // (one for all warps, which meet as often as it says: lengths that change under the kernel may part the others)
+            begun = now = w.tile;
+            tiles = w.tiles;
+#pragma unroll
+            for (int i = 0; i < 2 * ROW_TILES; i++) tile.limit[i >> 1][i & 1] = unit_row(p, l, w, 8 * (i >> 1) + 2 * (lane & 3) + (i & 1)).keys;
             start = false;
+        } else {
+            copy_wait<S::STAGES - 2>();   // (of the scales, and what does not come by TMA)
         }
-        const uint32_t bits = S::WARP_KEYS == 32 ? *reinterpret_cast<const uint32_t*>(&there[stage][4 * warp]) : *reinterpret_cast<const uint16_t*>(&there[stage][2 * warp]);
-        float* scales = reinterpret_cast<float*>(smem + stage * S::STAGE + 2 * S::KV) + S::WARP_KEYS * warp;
-        tile.tile(p, queries + set * S::Q, k_at, v_at, bits, w.tile * S::KEYS + warp * S::WARP_KEYS, row_keys[set], scales, scales + S::KEYS, by + S::WARP_KEYS * warp);
-        const bool last = w.tile + 1 == w.tiles;
-        if (last || at + 1 == n_tiles) {   // the part ends: the warps' rows meet in the tile's place
+        __syncwarp();
+        if (ok) copy_tile();          // (into the slot of the tile before, which this warp has worked on)
+        if (ok && (by_tma >> slot & 1)) {
+            ok = __all_sync(~0u, dense::mbar_wait_bounded(&full[warp][slot], rounds >> slot & 1, gave_up, TG_ROWS8 + dense::TG_FULL));
+            if (ok) {
+                rounds ^= 1u << slot;
+                by_tma &= ~(1u << slot);
+            }
+        }
+        __syncwarp();
+        if (ok) {
+            uint32_t bits = there[0];
+#pragma unroll
+            for (int i = 1; i < S::STAGES; i++)
+                if (i == slot) bits = there[i];
+            tile.tile(p, smem_at(queries), smem_at(slots) + slot * S::SLOT, smem_at(slots) + slot * S::SLOT + S::KV, bits, now * S::KEYS + warp * S::WARP_KEYS, scales + slot * S::SCALES, scales + S::STAGES * S::SCALES);
+        } else {   // gave up: what this warp still had to do comes out as NaN
+#pragma unroll
+            for (int i = 0; i < 2 * ROW_TILES; i++) {
+                tile.l[i >> 1][i & 1] = NAN;
+                tile.seen[i >> 1][i & 1] = true;
+            }
+        }
+        now++;
+        if (now == tiles || at + 1 == n_tiles) {   // the part ends: the warps' rows meet in their slots
+            const Walk& w = walks[0][set];
             tile.put_ml(ml[warp]);
             __syncthreads();
             // lane r: row r's largest exponent, what this warp's sums are multiplied by, the sum of the weights
             float m = -INFINITY, sum = 0.0f, mine = 0.0f;
             bool any = false;
 #pragma unroll
-            for (int i = 0; i < 4; i++)
-                if (!(ml[i][lane & 15].y < 0.0f)) { m = fmaxf(m, ml[i][lane & 15].x); any = true; }
+            for (int i = 0; i < S::WARPS; i++)
+                if (!(ml[i][lane & (S::ROWS - 1)].y < 0.0f)) { m = fmaxf(m, ml[i][lane & (S::ROWS - 1)].x); any = true; }
             const float base = m == -INFINITY ? 0.0f : m;
 #pragma unroll
-            for (int i = 0; i < 4; i++) {
-                const bool has = !(ml[i][lane & 15].y < 0.0f);
-                const float f = has ? ex2(ml[i][lane & 15].x - base) : 0.0f;
-                if (has) sum += ml[i][lane & 15].y * f;
+            for (int i = 0; i < S::WARPS; i++) {
+                const bool has = !(ml[i][lane & (S::ROWS - 1)].y < 0.0f);
+                const float f = has ? ex2(ml[i][lane & (S::ROWS - 1)].x - base) : 0.0f;
+                if (has) sum += ml[i][lane & (S::ROWS - 1)].y * f;
                 if (i == warp) mine = f;
             }
-            if (t < S::ROWS) joined[t] = make_float2(m, any ? sum : -1.0f);
-            float* rows = reinterpret_cast<float*>(smem + stage * S::STAGE);
-            const bool whole_part = whole_unit(p, w, begun, w.tile);
-            const int64_t slot = w.unit + blockIdx.x;
+            if (!any) sum = -1.0f;
+            const int used = w.b < 0 ? (int)min((int64_t)S::ROWS, p.batch.n_rows * p.group - (int64_t)w.row_tile * S::ROWS) : min(S::ROWS, w.s.count * p.group - w.row_tile * S::ROWS);
+            const float* rows = reinterpret_cast<const float*>(smem + slot * S::SLOT);
+            const bool whole_part = whole_unit(p, w, begun, now - 1);
+            const int64_t slot_of_part = w.unit + blockIdx.x;
 #pragma unroll
             for (int pass = 0; pass < DP / S::COLS; pass++) {
                 if (pass) __syncthreads();
                 __syncwarp();
-                tile.put_o(rows + warp * S::ROWS * S::COLS, mine, pass);
+                tile.put_o(reinterpret_cast<float*>(slots + slot * S::SLOT), mine, pass);
                 __syncthreads();
                 const int quads = min(S::COLS, D - pass * S::COLS) / 4;
-                for (int e = t; e < used * quads; e += S::THREADS) {
-                    const int x = e / quads, c = 4 * (e - x * quads), column = pass * S::COLS + c;
-                    const float2 sums = joined[x];
-                    float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-                    if (!(sums.y < 0.0f)) {
+                for (int x = warp; x < used; x += S::WARPS) {   // a warp a row, a lane four columns
+                    const float row_m = __shfl_sync(~0u, m, x), row_sum = __shfl_sync(~0u, sum, x);
+                    if (lane < quads) {
+                        const int c = 4 * lane, column = pass * S::COLS + c;
+                        float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                        if (!(row_sum < 0.0f)) {
 #pragma unroll
-                        for (int i = 0; i < 4; i++) {
-                            const float4 a = *reinterpret_cast<const float4*>(rows + i * S::ROWS * S::COLS + sum8_at<S::COLS>(x, c));
-                            v.x += a.x; v.y += a.y; v.z += a.z; v.w += a.w;
+                            for (int i = 0; i < S::WARPS; i++) {
+                                const float4 a = *reinterpret_cast<const float4*>(rows + i * (S::STAGES * S::SLOT / 4) + sum8_at<S::COLS>(x, c));
+                                v.x += a.x; v.y += a.y; v.z += a.z; v.w += a.w;
+                            }
+                        }
+                        if (whole_part) {
+                            const UnitRow r = unit_row(p, l, w, x);
+                            if (!(row_sum < 0.0f)) { v.x /= row_sum; v.y /= row_sum; v.z /= row_sum; v.w /= row_sum; }
+                            store_row(p, r, column, v);
+                            if (column == 0 && p.lse) p.lse[r.row * p.q_heads + r.head] = row_sum < 0.0f ? -INFINITY : lse_of(row_m, row_sum);
+                        } else if (slot_of_part < l.slots) {
+                            *reinterpret_cast<float4*>(part_at(l, D, slot_of_part, x, column)) = v;
+                            if (column == 0) l.ml[slot_of_part * S::ROWS + x] = make_float2(row_m, row_sum);
                         }
                     }
-                    if (whole_part) {
-                        const UnitRow r = unit_row(p, l, w, x);
-                        if (!(sums.y < 0.0f)) { v.x /= sums.y; v.y /= sums.y; v.z /= sums.y; v.w /= sums.y; }
-                        store_row(p, r, column, v);
-                        if (column == 0 && p.lse) p.lse[r.row * p.q_heads + r.head] = sums.y < 0.0f ? -INFINITY : lse_of(sums.x, sums.y);
-                    } else if (slot < l.slots) {
-                        *reinterpret_cast<float4*>(part_at(l, D, slot, x, column)) = v;
-                        if (column == 0) l.ml[slot * S::ROWS + x] = sums;
-                    }
+                    __syncwarp();
                 }
             }
+            written |= 1u << slot;
+            start = true;
+            __syncthreads();   // (before the slots are copied to again)
         }
-        w.tile++;
-        start = last;
     }
     copy_wait<0>();
+    if (!ok) {   // what TMA was asked for lands before shared memory goes away
+        for (int i = 0; i < S::STAGES; i++)
+            if (by_tma >> i & 1) dense::mbar_wait_for(&full[warp][i], rounds >> i & 1, nullptr);
+        if (lane == 0 && p.err) *p.err = *gave_up;
+    }
     if (last_cta) grid_wait();
 }
 
