@@ -9,6 +9,7 @@
 
 #include "paged8_attn.cuh"
 #include "paged8_rows.cuh"
+#include "paged8_tensor.cuh"
 #include "paged_checks.h"
 
 using namespace lmrs;
@@ -242,25 +243,48 @@ namespace {
 // How a call is cut, from what the host knows of it (as in paged.cu)
 struct Cutting8 {
     Line own, front;   // the kernel's that takes the sequences' units, and that takes the prefix' (the same where one takes both)
+    bool own_tensor, front_tensor;
     size_t bytes;
 };
-template <typename T, int DP, int ROW_TILES> Cutting8 cutting8(const lmrs_b200_pages8_t* pages, const lmrs_b200_batch_t* batch, int64_t n_rows, int q_heads, char* base) {
-    using S = TileShape8<T, DP, ROW_TILES>;
+// Which kernel takes what: float32 rows8_kernel; 16-bit types by how often the keys would be read again (as in paged.cu)
+struct Which8 { bool own_tensor, front_tensor; int row_tiles; };   // row_tiles: rows of a unit of rows8_kernel, in eights
+template <int DP> struct TensorRule8 {
+    static constexpr int OWN_ROWS = DP <= 128 ? 64 : 16, FRONT_ROWS = DP <= 128 ? 17 : 1;
+    static constexpr int64_t FRONT_WORK = DP <= 128 ? 1 << 21 : 1 << 19;
+};
+template <int DP> Which8 which8(const lmrs_b200_pages8_t* pages, const lmrs_b200_batch_t* batch, int dtype, int64_t n_rows, int q_heads) {
+    using R = TensorRule8<DP>;
+    const int64_t group = q_heads / pages->kv_heads, rows = n_rows * group, most = std::min<int64_t>(batch->max_rows, n_rows) * group;
+    Which8 w = {};
+    w.own_tensor = dtype != 1 && most >= R::OWN_ROWS;
+    w.front_tensor = batch->prefix_len > 0 && (w.own_tensor || (dtype != 1 && rows >= R::FRONT_ROWS && rows * pages->kv_heads * batch->prefix_len >= R::FRONT_WORK));
+    w.row_tiles = (batch->prefix_len && !w.front_tensor ? rows : most) <= 8 ? 1 : 2;
+    return w;
+}
+template <typename T, int DP, int ROW_TILES> Cutting8 cutting8(const lmrs_b200_pages8_t* pages, const lmrs_b200_batch_t* batch, int64_t n_rows, int q_heads, const Which8& which, char* base) {
     const int64_t group = q_heads / pages->kv_heads, rows = n_rows * group;
     Cutting8 c = {};
-    auto line = [&](Line& l, bool own, bool front) {
-        l.tile_rows = S::ROWS;
-        l.tile_keys = S::KEYS;
-        l.ctas = SMS * S::CTAS;
+    auto line = [&](Line& l, bool tensor, bool own, bool front) {
+        using S = TileShape8<T, DP, ROW_TILES>;
+        using X = TensorShape8<DP>;
+        l.tile_rows = tensor ? X::ROWS : S::ROWS;
+        l.tile_keys = tensor ? X::KEYS : S::KEYS;
+        l.ctas = tensor ? SMS : SMS * S::CTAS;
         while (1 << l.row_shift < l.tile_rows) l.row_shift++;
         while (1 << l.key_shift < l.tile_keys) l.key_shift++;
         l.seqs = own ? batch->seqs : 0;
         l.front_tiles = front ? (int)(((int64_t)batch->prefix_len + l.tile_keys - 1) / l.tile_keys) : 0;
         l.front_units = l.front_tiles ? (rows + l.tile_rows - 1) / l.tile_rows * pages->kv_heads : 0;
+        if (tensor && !own && l.front_units > 0 && l.front_units <= SMS) {   // (as many CTAs for each unit, as in paged.cu)
+            const int even = SMS / (int)l.front_units * (int)l.front_units;
+            if (even * 16 >= SMS * 15) l.ctas = even;
+        }
         place_line(l, rows, pages->kv_heads, pages->head_size, base, c.bytes);
     };
-    line(c.own, true, true);
-    c.front = c.own;
+    const bool one = batch->prefix_len == 0 || which.own_tensor == which.front_tensor;
+    line(c.own, which.own_tensor, true, one);
+    if (one) c.front = c.own;
+    else line(c.front, true, false, true);
     return c;
 }
 // Tensor maps of the codes for boxes of S::BOX columns, if there are any (boxes.rows stays 0 otherwise): rows of a box are the most that divide a page and a warp's keys
@@ -294,15 +318,14 @@ template <typename S> void box_maps8(const lmrs_b200_pages8_t* pages, Boxes8& bo
         map(&boxes.v, pages->v, pages->v_page, pages->v_slot, pages->v_head, boxes.v_place, boxes.v_head))
         boxes.rows = rows;
 }
-// rows of a unit in eights: one where no unit has more
-int row_tiles(const lmrs_b200_pages8_t* pages, const lmrs_b200_batch_t* batch, int64_t n_rows, int q_heads) {
-    const int64_t group = q_heads / pages->kv_heads;
-    return (batch->prefix_len ? n_rows : std::min<int64_t>(batch->max_rows, n_rows)) * group <= 8 ? 1 : 2;
-}
-template <typename F> int by_shape8(const lmrs_b200_pages8_t* pages, int dtype, int tiles, F f) {
+// f(type, form, padded head size, rows of a unit in eights, which kernels)
+template <typename F> int by_shape8(const lmrs_b200_pages8_t* pages, const lmrs_b200_batch_t* batch, int dtype, int64_t n_rows, int q_heads, F f) {
     return by_type(dtype, [&](auto t) {
         return by_form(pages->form, [&](auto form) {
-            auto by_tiles = [&](auto d) { return tiles == 1 ? f(t, form, d, std::integral_constant<int, 1>()) : f(t, form, d, std::integral_constant<int, 2>()); };
+            auto by_tiles = [&](auto d) {
+                const Which8 w = which8<decltype(d)::value>(pages, batch, dtype, n_rows, q_heads);
+                return w.row_tiles == 1 ? f(t, form, d, std::integral_constant<int, 1>(), w) : f(t, form, d, std::integral_constant<int, 2>(), w);
+            };
             return pages->head_size <= 64 ? by_tiles(std::integral_constant<int, 64>()) : pages->head_size <= 128 ? by_tiles(std::integral_constant<int, 128>()) : by_tiles(std::integral_constant<int, 256>());
         });
     });
@@ -318,8 +341,8 @@ extern "C" int lmrs_b200_paged8_attention_workspace(const lmrs_b200_pages8_t* pa
         if (!why.empty()) return refuse(me, why);
         *bytes = 0;
         if (n_rows == 0 || batch->seqs == 0) return 0;
-        return by_shape8(pages, dtype, row_tiles(pages, batch, n_rows, q_heads), [&](auto t, auto, auto d, auto tiles) {
-            *bytes = cutting8<decltype(t), decltype(d)::value, decltype(tiles)::value>(pages, batch, n_rows, q_heads, nullptr).bytes;
+        return by_shape8(pages, batch, dtype, n_rows, q_heads, [&](auto t, auto, auto d, auto tiles, const Which8& which) {
+            *bytes = cutting8<decltype(t), decltype(d)::value, decltype(tiles)::value>(pages, batch, n_rows, q_heads, which, nullptr).bytes;
             return 0;
         });
     });
@@ -344,13 +367,15 @@ extern "C" int lmrs_b200_paged8_attention(const lmrs_b200_pages8_t* pages, const
         if (why.empty()) why = bad_pages8_memory(pages, device);
         if (why.empty() && (!workspace || !aligned(workspace, 256) || !on_device(workspace, device))) why = "workspace is not memory of the current device on a 256-byte boundary";
         if (!why.empty()) return refuse(me, why);
-        if (const int status = gave_up_word.take())
-            return refuse(me, "results of an earlier call are NaN: " + (status >> 8 == TG_ROWS8 >> 8 ? "rows8_kernel gave up waiting for a slot's copies (device status " + std::to_string(status) + ")" : dense::tg_gave_up(status)));
-        return by_shape8(pages, dtype, row_tiles(pages, batch, n_rows, q_heads), [&](auto t, auto form, auto d, auto tiles) {
+        if (const int status = gave_up_word.take()) {
+            const int kernel = status & ~255;
+            return refuse(me, "results of an earlier call are NaN: " + (kernel == TG_ROWS8 || kernel == TG_CODES128 ? (kernel == TG_ROWS8 ? "rows8_kernel: " : "codes128_kernel: ") : std::string()) + dense::tg_gave_up(status));
+        }
+        return by_shape8(pages, batch, dtype, n_rows, q_heads, [&](auto t, auto form, auto d, auto tiles, const Which8& which) {
             using T = decltype(t);
             constexpr int FORM = decltype(form)::value, DP = decltype(d)::value, ROW_TILES = decltype(tiles)::value;
             using S = TileShape8<T, DP, ROW_TILES>;
-            const Cutting8 c = cutting8<T, DP, ROW_TILES>(pages, batch, n_rows, q_heads, (char*)workspace);
+            const Cutting8 c = cutting8<T, DP, ROW_TILES>(pages, batch, n_rows, q_heads, which, (char*)workspace);
             if (workspace_bytes < c.bytes) return refuse(me, "workspace has " + std::to_string(workspace_bytes) + " bytes, the call needs " + std::to_string(c.bytes));
             Attn8Params<T> p = {};
             p.batch = batch8_as(batch, pages, n_rows);
@@ -369,15 +394,31 @@ extern "C" int lmrs_b200_paged8_attention(const lmrs_b200_pages8_t* pages, const
                 if (pages->page_size == 1 << i) p.page_shift = i;
                 if (pages->block == 1 << i) p.block_shift = i;
             }
-            static std::atomic<uint64_t> allowed{0};
-            auto kernel = rows8_kernel<T, FORM, DP, ROW_TILES>;
-            cudaError_t e = allow_smem(kernel, device, S::SMEM, allowed);
-            if (e != cudaSuccess) return refuse(me, cudaGetErrorString(e));
             if (!(p.err = gave_up_word.get())) return refuse(me, "out of host memory");
-            Boxes8 boxes = {};
-            box_maps8<S>(pages, boxes);
-            kernel<<<(unsigned)c.own.ctas, S::THREADS, S::SMEM, (cudaStream_t)stream>>>(p, c.own, boxes);
-            if (launched(me)) return 1;
+            static std::atomic<uint64_t> allowed{0}, allowed_tensor{0};
+            cudaError_t e = cudaSuccess;
+            const bool tensor = which.own_tensor || which.front_tensor;
+            if constexpr (sizeof(T) == 2)
+                if (tensor) {
+                    auto kernel = codes128_kernel<T, FORM, DP>;
+                    using X = TensorShape8<DP>;
+                    if ((e = allow_smem(kernel, device, X::SMEM, allowed_tensor)) != cudaSuccess) return refuse(me, cudaGetErrorString(e));
+                    Boxes8 boxes = {};
+                    box_maps8<X>(pages, boxes);
+                    const Line& line = which.own_tensor ? c.own : c.front;
+                    kernel<<<(unsigned)line.ctas, X::THREADS, X::SMEM, (cudaStream_t)stream>>>(p, line, boxes);
+                    if (launched(me)) return 1;
+                }
+            if (!which.own_tensor) {
+                auto kernel = rows8_kernel<T, FORM, DP, ROW_TILES>;
+                if ((e = allow_smem(kernel, device, S::SMEM, allowed)) != cudaSuccess) return refuse(me, cudaGetErrorString(e));
+                Boxes8 boxes = {};
+                box_maps8<S>(pages, boxes);
+                if (tensor) e = launch_after(kernel, (unsigned)c.own.ctas, S::THREADS, S::SMEM, (cudaStream_t)stream, p, c.own, boxes);
+                else kernel<<<(unsigned)c.own.ctas, S::THREADS, S::SMEM, (cudaStream_t)stream>>>(p, c.own, boxes);
+                if (e != cudaSuccess) return refuse(me, std::string("launch failed: ") + cudaGetErrorString(e));
+                if (launched(me)) return 1;
+            }
             // (which join, as in paged.cu)
             const int64_t items = n_rows * q_heads;
             constexpr int COLS = DP <= 128 ? 1 : 2;

@@ -130,7 +130,7 @@ template <typename T, int FORM, int DP, int ROW_TILES> struct WarpTile8 {
         }
     }
     PG_DEVINL void begin(const Attn8Params<T>& p, uint32_t q_at) {
-        const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+        const int g = (threadIdx.x & 31) >> 2, t = threadIdx.x & 3;
         __syncwarp();
 #pragma unroll
         for (int n = 0; n < ROW_TILES; n++) {

@@ -1,0 +1,556 @@
+// paged8_tensor.cuh -- attention over 8-bit pages for many rows that see the same keys (the prefix, portions of prompts), on the 5th-generation tensor cores.  Rows of 16-bit types.
+//
+// The line, its units and parts, the order of the work and TMEM are rows128_kernel's (paged_tensor.cuh), the mathematics that of paged8_attn.cuh: both products take float16, and codes are converted on
+// the way into the operands' ring:
+//   warps 0-3, 4-7   the rows of the first and the second block, a thread a row.  They also bring the queries in: float16, times a power of two for each row of bfloat16
+//   warps 8-9        keys and values, 32 keys of an operand tile each: codes by TMA (or 16 bytes a lane) into slots of their own, three operands ahead; from there, 16 codes a lane at a time, as float16 into the ring
+//   warp 10          the products
+// A thread's score of a key is its dot product times the key's scale; its weight carries the value's scale; both scales come from shared memory, four keys a load.
+#pragma once
+#include "paged8_attn.cuh"
+#include "paged_tensor.cuh"
+
+namespace lmrs {
+namespace paged {
+
+constexpr int TG_CODES128 = 7 << 8;   // (a kernel that gave up: after TG_ROWS8)
+
+template <int DP> struct TensorShape8 {
+    static constexpr int THREADS = 384, COPIERS = 2, BLOCK = 128, BLOCKS = DP <= 128 ? 2 : 1, ROWS = BLOCK * BLOCKS, KEYS = 64, WARP_KEYS = KEYS / COPIERS;
+    static constexpr int COL_BOXES = DP / 64;                               // 64 columns of an operand in float16: rows of 128 bytes, their 16-byte pieces rotated (SWIZZLE_128B)
+    static constexpr int SLOT = COL_BOXES * KEYS * 128, SLOTS = DP <= 64 ? 8 : DP <= 128 ? 6 : 3, Q_BLOCK = COL_BOXES * BLOCK * 128;
+    static constexpr int BOX = DP < 128 ? DP : 128, KV = WARP_KEYS * DP;    // codes of a copying warp: columns of a TMA box, bytes of an operand
+    static constexpr int STAGES = 3;                                        // its slots for them
+    static constexpr int RING = 16;                                         // tiles whose keys' places and scales are known
+    static constexpr int O_AT = 256;                                        // TMEM columns: two sets of scores for each block, then o of each block
+    static constexpr int SMEM = 1024 + SLOTS * SLOT + BLOCKS * Q_BLOCK + COPIERS * STAGES * KV;
+    static_assert(O_AT + BLOCKS * DP <= 512 && 2 * 2 * KEYS <= O_AT, "TMEM");
+};
+struct KeyAt { int page, place, head, boxed; };   // (page -1: nowhere)
+template <int DP> struct TensorShared8 {
+    using S = TensorShape8<DP>;
+    uint64_t full[S::SLOTS], empty[S::SLOTS];   // slots of the ring
+    uint64_t staged[S::COPIERS][S::STAGES];     // slots of codes, where they come by TMA
+    uint64_t known[S::RING];                    // which of a tile's keys are there, and their scales, are written
+    uint64_t scores[4], weights[4];             // sets of scores (two for each block): written by the products, replaced by weights
+    uint64_t summed[4];                         // o of a block: the products of a tile have ended, even tiles and odd ones
+    uint64_t read[2];                           // the part's o of a block has been read
+    uint64_t queries;                           // the part's queries are there
+    uint64_t parted;                            // both groups have ended the part
+    alignas(16) float key_scale[S::RING][S::KEYS], value_log[S::RING][S::KEYS], value_by[S::RING][S::KEYS];
+    KeyAt places[S::COPIERS][4][S::WARP_KEYS];  // of the last four tiles whose keys were asked for
+    int part_tiles[S::COPIERS][4];              // of the last four parts
+    uint32_t there[S::RING][S::COPIERS];
+    uint32_t tmem;
+    int gave_up;
+};
+PG_DEVINL uint64_t mul_pair(uint64_t a, uint64_t b) { uint64_t r; asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b)); return r; }
+PG_DEVINL uint64_t same_pair(float a) { return pair_of(__float_as_uint(a), __float_as_uint(a)); }
+
+template <typename T, int FORM, int DP>
+__global__ void __launch_bounds__(384, 1) codes128_kernel(const __grid_constant__ Attn8Params<T> p, const __grid_constant__ Line l, const __grid_constant__ Boxes8 boxes) {
+    using S = TensorShape8<DP>;
+    extern __shared__ uint8_t raw[];
+    __shared__ TensorShared8<DP> sh;
+    uint8_t* ring = raw + (((smem_at(raw) + 1023u) & ~1023u) - smem_at(raw));
+    uint8_t *queries = ring + S::SLOTS * S::SLOT, *codes = queries + S::BLOCKS * S::Q_BLOCK;
+    const int warp = __shfl_sync(~0u, (int)threadIdx.x >> 5, 0), lane = threadIdx.x & 31, D = p.head_size;
+    constexpr int PRODUCTS = 8 + S::COPIERS;   // the warp that issues them
+    volatile int* gave_up = &sh.gave_up;
+
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < S::SLOTS; i++) { mbar_init(&sh.full[i], S::COPIERS); mbar_init(&sh.empty[i], 1); }
+        for (int i = 0; i < S::COPIERS * S::STAGES; i++) mbar_init(&sh.staged[0][0] + i, 1);
+        for (int i = 0; i < S::RING; i++) mbar_init(&sh.known[i], S::COPIERS);
+        for (int i = 0; i < 4; i++) { mbar_init(&sh.scores[i], 1); mbar_init(&sh.weights[i], 128); mbar_init(&sh.summed[i], 1); }
+        for (int i = 0; i < 2; i++) mbar_init(&sh.read[i], 128);
+        mbar_init(&sh.queries, 256);
+        mbar_init(&sh.parted, 256);
+        sh.gave_up = 0;
+        fence_barrier_init();
+    }
+    Walk w;
+    int64_t from, to;
+    walk_begin<T, S::THREADS>(p, l, w, from, to);   // (synchronises the CTA)
+    if (from >= to) { grid_launch(); return; }
+    if (warp == PRODUCTS) {
+        __syncwarp();
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_at(&sh.tmem)), "n"(512) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    tmem_before();
+    __syncthreads();
+    tmem_after();
+    const uint32_t tmem = sh.tmem;
+    grid_launch();
+    // Parts of the CTA, one after the other: `tiles` of unit w from w.tile on, `blocks` of its rows.  Every role walks along by itself.
+    int left = (int)(to - from), tiles = 0, blocks = 0, used = 0;
+    auto enter = [&]() {
+        tiles = min(left, w.tiles - w.tile);
+        used = w.b < 0 ? (int)min((int64_t)S::ROWS, p.batch.n_rows * p.group - (int64_t)w.row_tile * S::ROWS) : min(S::ROWS, w.s.count * p.group - w.row_tile * S::ROWS);
+        blocks = used > S::BLOCK ? 2 : 1;
+    };
+    auto leave = [&]() {   // false: that was the last one
+        left -= tiles;
+        if (left <= 0) return false;
+        walk_next_unit(p, l, w);
+        if (w.tiles == 0) { left = 0; return false; }   // (the line ended early: lengths changed under the kernel)
+        return true;
+    };
+    if (warp >= 8) {
+        if (warp < 8 + S::COPIERS) {
+            // ---- keys and values: asked for as codes STAGES - 1 operands ahead, then converted.  Operands of a part come as K0 K1 V0 K2 V1 ... ----
+            const int mine = warp - 8, whole = D / 16;
+            uint8_t* stage = codes + mine * (S::STAGES * S::KV);
+            const int box_rows = boxes.rows, groups = box_rows ? S::WARP_KEYS / box_rows : 0;
+            constexpr int COL_BOXES = DP / S::BOX;
+            const int box_col = lane % COL_BOXES, box_group = lane / COL_BOXES;
+            // what is asked for next: tile `at` of part w (`asked` keys and `values` of the part's operands have been), whose places are on their way
+            int keys_asked = 0, values_asked = 0, key_tiles = 0, value_tiles = 0, parts = 0, asked = 0;   // of the part; of all parts; operands
+            int page = -1, place = 0, boxed = 0;
+            bool more = true, ok = true;
+            uint32_t by_tma = 0, written = 0, rounds = 0;   // a bit a slot: codes are on their way by TMA, its bytes were last written otherwise, the phase that its barrier is in
+            // w runs ahead: it goes on to the next part when the last keys of this one have been asked for
+            int ahead_tiles = 0;                            // of the part that w is in
+            auto look = [&](int j) {
+                const int first = (w.tile + j) * S::KEYS + mine * S::WARP_KEYS, x = first + lane;
+                page = -1;
+                boxed = box_rows && first + S::WARP_KEYS <= w.keys;
+                if (x < w.keys) {
+                    const int i = p.page_shift >= 0 ? x >> p.page_shift : x / p.batch.page_size;
+                    page = (w.b < 0 ? p.batch.prefix : p.batch.tables + w.b * p.batch.table_stride)[i];
+                    place = x - i * p.batch.page_size;
+                }
+            };
+            auto ask = [&]() {   // the next operand's codes, if there is one
+                if (more) {
+                    const bool values = !(keys_asked < tiles && keys_asked - values_asked < 2);
+                    const int slot = asked % S::STAGES;
+                    if (!values) {
+                        KeyAt k = {page >= 0 && page < p.batch.pages ? page : -1, place, w.head, boxed};
+                        sh.places[mine][key_tiles & 3][lane] = k;
+                        if (k.page < 0) k.page = k.place = 0;
+                        const bool is = page >= 0 && page < p.batch.pages;
+                        const int block = p.block_shift >= 0 ? k.place >> p.block_shift : k.place / p.c.block, set = key_tiles % S::RING, x = mine * S::WARP_KEYS + lane;
+                        copy4(smem_at(&sh.key_scale[set][x]), p.c.ks + k.page * p.c.ks_page + block * p.c.ks_block + k.head * p.c.ks_head, is);
+                        copy4(smem_at(&sh.value_log[set][x]), p.c.vs + k.page * p.c.vs_page + block * p.c.vs_block + k.head * p.c.vs_head, is);
+                        __syncwarp();
+                    }
+                    const KeyAt k = sh.places[mine][(values ? value_tiles : key_tiles) & 3][lane];
+                    const uint32_t to_codes = smem_at(stage) + slot * S::KV;
+                    if (k.boxed) {   // (the same for all lanes)
+                        if (written >> slot & 1) asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                        __syncwarp();
+                        if (lane == 0) mbar_expect_tx(&sh.staged[mine][slot], S::KV);
+                        int of = __shfl_sync(~0u, k.page, box_group * box_rows & 31), from_row = __shfl_sync(~0u, k.place, box_group * box_rows & 31);
+                        if (of < 0) { of = p.batch.pages; from_row = 0; }   // (outside the map: zeros)
+                        __syncwarp();
+                        if (box_group < groups)
+                            tma_box(to_codes + box_col * (S::WARP_KEYS * S::BOX) + box_group * box_rows * S::BOX, values ? &boxes.v : &boxes.k, S::BOX * box_col, from_row, k.head, of,
+                                    values ? boxes.v_place : boxes.k_place, values ? boxes.v_head : boxes.k_head, &sh.staged[mine][slot]);
+                        __syncwarp();
+                        by_tma |= 1u << slot;
+                        written &= ~(1u << slot);
+                    } else {
+                        written |= 1u << slot;
+                        const uint8_t* base = values ? p.c.v : p.c.k;
+                        const int64_t start = k.page < 0 ? -1 : values ? k.page * p.c.v_page + k.place * p.c.v_slot + k.head * p.c.v_head : k.page * p.c.k_page + k.place * p.c.k_slot + k.head * p.c.k_head;
+                        constexpr int CHUNKS = DP / 16, LANES = CHUNKS < 8 ? CHUNKS : 8, AT_ONCE = 32 / LANES;   // lanes a row, rows at a time
+#pragma unroll 2
+                        for (int r0 = 0; r0 < S::WARP_KEYS; r0 += AT_ONCE) {
+                            const int row = r0 + lane / LANES;
+                            const int64_t row_start = __shfl_sync(~0u, start, row);
+#pragma unroll
+                            for (int c = 0; c < CHUNKS; c += LANES) {
+                                const int piece = c + lane % LANES;
+                                const bool in = row_start >= 0 && piece < whole;
+                                copy16(to_codes + code_at<S>(row, piece), in ? base + row_start + 16 * piece : base, in);
+                            }
+                        }
+                    }
+                    asked++;
+                    if (values) {
+                        value_tiles++;
+                        if (++values_asked == tiles) {   // the part's last operand: w has gone on
+                            keys_asked = values_asked = 0;
+                            tiles = ahead_tiles;
+                            more = tiles > 0;
+                        }
+                    } else {
+                        key_tiles++;
+                        if (++keys_asked < tiles) look(keys_asked);
+                        else {
+                            left -= tiles;
+                            ahead_tiles = 0;
+                            if (left > 0) {
+                                walk_next_unit(p, l, w);
+                                if (w.tiles > 0) {
+                                    ahead_tiles = min(left, w.tiles - w.tile);
+                                    if (lane == 0) sh.part_tiles[mine][parts & 3] = ahead_tiles;
+                                    parts++;
+                                    look(0);
+                                }
+                            }
+                            if (!ahead_tiles) left = 0;
+                        }
+                    }
+                }
+                copy_commit();
+            };
+            enter();
+            if (lane == 0) sh.part_tiles[mine][0] = tiles;
+            parts = 1;
+            __syncwarp();
+            look(0);
+            for (int i = 0; i < S::STAGES - 1; i++) ask();
+            // conversion: keys and values of the part that is converted, and what has been in all
+            int part = 0, k_done = 0, v_done = 0, k_all = 0, slot = 0, round = 0, done = 0, part_has = tiles;
+            {
+                __syncwarp();
+                part_has = sh.part_tiles[mine][0];
+            }
+            while (ok && done < asked) {
+                ask();
+                copy_wait<S::STAGES - 1>();
+                const bool values = !(k_done < part_has && k_done - v_done < 2);
+                const int from_slot = done % S::STAGES;
+                if (by_tma >> from_slot & 1) {
+                    ok = __all_sync(~0u, dense::mbar_wait_bounded(&sh.staged[mine][from_slot], rounds >> from_slot & 1, gave_up, TG_CODES128 + dense::TG_FULL));
+                    if (!ok) break;
+                    rounds ^= 1u << from_slot;
+                    by_tma &= ~(1u << from_slot);
+                }
+                __syncwarp();
+                if (!values) {
+                    const int set = k_all % S::RING, x = mine * S::WARP_KEYS + lane;
+                    const float2 v = value_terms(sh.value_log[set][x]);
+                    sh.value_log[set][x] = v.x;
+                    sh.value_by[set][x] = v.y;
+                    const unsigned bits = __ballot_sync(~0u, sh.places[mine][k_all & 3][lane].page >= 0);
+                    if (lane == 0) {
+                        sh.there[set][mine] = bits;
+                    }
+                    __syncwarp();
+                    if (lane == 0) arrive(&sh.known[set]);
+                }
+                ok = wait_warp(&sh.empty[slot], round + 1, gave_up, TG_CODES128 + dense::TG_FREE - dense::TG_PAGED);
+                if (!ok) break;
+                const uint32_t code_row = smem_at(stage) + from_slot * S::KV, to_row = smem_at(ring) + slot * S::SLOT + (mine * S::WARP_KEYS + lane) * 128;
+#pragma unroll 4
+                for (int c = 0; c < DP / 16; c++) {
+                    if (c >= whole) break;
+                    uint32_t u[4], h[8];
+                    asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(u[0]), "=r"(u[1]), "=r"(u[2]), "=r"(u[3]) : "r"(code_row + code_at<S>(lane, c)));
+#pragma unroll
+                    for (int i = 0; i < 4; i++) codes_to_halves<FORM, 0>(u[i], h[2 * i], h[2 * i + 1]);
+                    const uint32_t at = to_row + (c >> 2) * (S::KEYS * 128);
+#pragma unroll
+                    for (int i = 0; i < 2; i++)
+                        asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(at + (((2 * (c & 3) + i) ^ (lane & 7)) << 4)), "r"(h[4 * i]), "r"(h[4 * i + 1]), "r"(h[4 * i + 2]), "r"(h[4 * i + 3]) : "memory");
+                }
+                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                __syncwarp();
+                if (lane == 0) arrive(&sh.full[slot]);
+                done++;
+                if (++slot == S::SLOTS) { slot = 0; round++; }
+                if (!values) {
+                    k_done++;
+                    k_all++;
+                } else if (++v_done == part_has) {
+                    k_done = v_done = 0;
+                    part++;
+                    if (part < parts) part_has = sh.part_tiles[mine][part & 3];
+                }
+            }
+            copy_wait<0>();
+            if (!ok)   // gave up: what TMA was asked for lands before shared memory goes away
+                for (int i = 0; i < S::STAGES; i++)
+                    if (by_tma >> i & 1) dense::mbar_wait_for(&sh.staged[mine][i], rounds >> i & 1, nullptr);
+        } else if (warp == PRODUCTS) {
+            // ---- products ----
+            constexpr int WHO = TG_CODES128 - dense::TG_PAGED;
+            const uint32_t one = dense::elect_one();
+            const uint32_t form = (1u << 4) | ((uint32_t)(S::BLOCK >> 4) << 24);   // f32 += f16 x f16, 128 rows
+            const uint32_t score_form = form | ((uint32_t)(S::KEYS >> 3) << 17), sum_form = form | (1u << 16) | ((uint32_t)(D >> 3) << 17);   // (values are MN-major)
+            const uint32_t ring_lo = (uint32_t)dense::tg_desc_sw128(ring), q_lo = (uint32_t)dense::tg_desc_sw128(queries);
+            const int steps = D / 16;
+            uint32_t n = 0, round = 0;           // slot of the next operand tile, rounds of the ring before it
+            int w_count[4] = {0, 0, 0, 0}, part = 0;   // sets of weights taken
+            bool ok = true;
+            auto take = [&]() {
+                ok = ok && wait_warp(&sh.full[n], (int)round, gave_up, WHO + dense::TG_FULL);
+                tmem_after();
+                const uint32_t slot = n;
+                if (++n == S::SLOTS) { n = 0; round++; }
+                return slot;
+            };
+            // (unrolled, so that descriptors are sums of constants in uniform registers)
+            auto scores = [&](int block, int j, uint32_t slot) {
+                const int set = 2 * block + (j & 1);
+                const uint32_t d = tmem + (uint32_t)set * S::KEYS, a = q_lo + (uint32_t)block * (S::Q_BLOCK >> 4), b = ring_lo + slot * (S::SLOT >> 4);
+#pragma unroll
+                for (int k = 0; k < DP / 16; k++)
+                    if (k < steps)
+                        dense::tg_mma_ss1(one, d, a + (uint32_t)(k >> 2) * (S::BLOCK * 128 >> 4) + (k & 3) * 2, b + (uint32_t)(k >> 2) * (S::KEYS * 128 >> 4) + (k & 3) * 2, score_form, k > 0);
+                dense::tg_commit1(one, &sh.scores[set]);
+            };
+            auto sums = [&](int block, int j, uint32_t slot) {
+                const int set = 2 * block + (j & 1);
+                if (j == 0 && part > 0) ok = ok && wait_warp(&sh.read[block], part - 1, gave_up, WHO + dense::TG_VALUES_READ);
+                ok = ok && wait_warp(&sh.weights[set], w_count[set]++, gave_up, WHO + dense::TG_WEIGHTS);
+                if (!ok) return;
+                tmem_after();
+                // 16 keys a step: two groups of 8 rows of 128 bytes; from 64 columns to the next: a box
+                const uint32_t d = tmem + S::O_AT + (uint32_t)block * DP, a = tmem + (uint32_t)set * S::KEYS;
+                const uint32_t b = (ring_lo & 0xffffu) + slot * (S::SLOT >> 4) + ((uint32_t)(S::KEYS * 128 >> 4) << 16), more = j > 0;
+#pragma unroll
+                for (int k = 0; k < S::KEYS / 16; k++) dense::tg_mma_ts1(one, d, a + k * 8, b + k * (2048 >> 4), sum_form, k > 0 ? 1u : more);
+                dense::tg_commit1(one, &sh.summed[set]);
+            };
+            do {   // the scores of tile j + 2 follow the sums of tile j into the same set
+                enter();
+                ok = ok && wait_warp(&sh.queries, part, gave_up, WHO + dense::TG_QUERIES);
+                tmem_after();
+                for (int j = 0; j < 2 && j < tiles; j++) {
+                    const uint32_t keys = take();
+                    if (!ok) break;
+                    for (int g = 0; g < blocks; g++) scores(g, j, keys);
+                    dense::tg_commit1(one, &sh.empty[keys]);
+                }
+                for (int j = 0; j < tiles && ok; j++) {
+                    const uint32_t values = take();
+                    uint32_t keys = 0;
+                    for (int g = 0; g < blocks && ok; g++) {
+                        sums(g, j, values);
+                        if (ok && g == blocks - 1) dense::tg_commit1(one, &sh.empty[values]);
+                        if (j + 2 < tiles) {
+                            if (g == 0) keys = take();
+                            if (ok) scores(g, j + 2, keys);
+                        }
+                    }
+                    if (ok && j + 2 < tiles) dense::tg_commit1(one, &sh.empty[keys]);
+                }
+                part++;
+            } while (ok && leave());
+            // the last commit is that of the last values' slot: none may arrive after the CTA has ended
+            if (ok) ok = wait_warp(&sh.empty[n == 0 ? S::SLOTS - 1 : n - 1], (int)(n == 0 ? round - 1 : round), gave_up, WHO + dense::TG_FREE);
+            if (!ok)   // gave up: products already issued may still run; they get a millisecond to end before shared memory and TMEM go away
+                for (int i = 0; i < 1000; i++) __nanosleep(1000);
+        }
+        __syncwarp();
+    } else {
+        // ---- rows ----
+        constexpr int WHO = TG_CODES128 - dense::TG_PAGED;
+        const int group = warp >> 2, row = threadIdx.x & 127;
+        const uint32_t lanes = (uint32_t)(warp & 3) << 21;   // this warp's 32 TMEM lanes
+        int s_count[2] = {0, 0}, k_count = 0, part = 0;   // phases of earlier parts: this group's even and odd tiles, all tiles, parts
+        bool ok = true;
+        do {
+            enter();
+            const bool mine = group < blocks;
+            const int x = group * S::BLOCK + row;
+            if (mine) {
+                const UnitRow r = unit_row(p, l, w, x);
+                // the row's query, as float16: all products that read the last one have ended, since their sums have been waited for
+                float2 factor = make_float2(1.0f, 1.0f);
+                {
+                    const bool is = x < used;
+                    const T* q = is ? p.q.data + r.row * p.q.row + r.head * p.q.head : p.q.data;
+                    auto piece = [&](int c) {   // 8 elements
+                        Piece<T, 8> v;
+                        if (is && p.q_wide) v = *reinterpret_cast<const Piece<T, 8>*>(q + 8 * c);
+                        else
+#pragma unroll
+                            for (int i = 0; i < 8; i++) v.v[i] = is ? q[8 * c + i] : from_f<T>(0.0f);
+                        return v;
+                    };
+                    if constexpr (!std::is_same<T, __half>::value) {
+                        float most = 0.0f;
+#pragma unroll 4
+                        for (int c = 0; c < D / 8; c++) {
+                            const Piece<T, 8> v = piece(c);
+#pragma unroll
+                            for (int i = 0; i < 8; i++) most = fmaxf(most, fabsf(to_f(v.v[i])));
+                        }
+                        factor = row_factor(most);
+                    }
+                    const uint32_t q_at = smem_at(queries) + group * S::Q_BLOCK + row * 128;
+#pragma unroll 4
+                    for (int c = 0; c < D / 8; c++) {
+                        const Piece<T, 8> v = piece(c);
+                        uint32_t h[4];
+#pragma unroll
+                        for (int i = 0; i < 4; i++) h[i] = to_halves(to_f(v.v[2 * i]) * factor.x, to_f(v.v[2 * i + 1]) * factor.x);
+                        asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(q_at + (c >> 3) * (S::BLOCK * 128) + (((c & 7) ^ (row & 7)) << 4)), "r"(h[0]), "r"(h[1]), "r"(h[2]), "r"(h[3]) : "memory");
+                    }
+                    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                    arrive(&sh.queries);
+                }
+                const float down = p.softcap > 0.0f ? factor.y : fminf(fmaxf(factor.y * p.scale2, -FLT_MAX), FLT_MAX);
+                float m = -INFINITY, sum = 0.0f;
+                bool seen = false;
+                const int least = w.b < 0 ? w.keys : unit_row(p, l, w, group * S::BLOCK).keys;   // (rows that come later see more)
+                for (int j = 0; j < tiles && ok; j++) {
+                    const int set = 2 * group + (j & 1), key0 = (w.tile + j) * S::KEYS, known = (k_count + j) % S::RING;
+                    ok = wait_warp(&sh.known[known], (k_count + j) / S::RING, gave_up, WHO + dense::TG_PLACES) && wait_warp(&sh.scores[set], s_count[j & 1] + (j >> 1), gave_up, WHO + dense::TG_SCORES);
+                    if (!ok) break;
+                    tmem_after();
+                    const uint32_t at = tmem + lanes + (uint32_t)set * S::KEYS;
+                    const bool all = key0 + S::KEYS <= least && sh.there[known][0] == ~0u && sh.there[known][1] == ~0u;
+                    const float *ks = sh.key_scale[known], *vl = sh.value_log[known], *vb = sh.value_by[known];
+                    // exponents, 64 of them in registers.  Tiles that need no mask are straight-line code
+                    uint32_t v[64];
+                    tmem_load64(at, v);
+                    float tops[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+                    if (!(p.softcap > 0.0f)) {
+                        const uint64_t by = same_pair(down);
+#pragma unroll
+                        for (int i = 0; i < 64; i += 4) {
+                            const ulonglong2 k = *reinterpret_cast<const ulonglong2*>(ks + i), a = *reinterpret_cast<const ulonglong2*>(vl + i);
+                            const float2 e = pair_open(fma_pair(mul_pair(pair_of(v[i], v[i + 1]), k.x), by, a.x)), f = pair_open(fma_pair(mul_pair(pair_of(v[i + 2], v[i + 3]), k.y), by, a.y));
+                            v[i] = __float_as_uint(e.x); v[i + 1] = __float_as_uint(e.y); v[i + 2] = __float_as_uint(f.x); v[i + 3] = __float_as_uint(f.y);
+                        }
+                    } else {
+#pragma unroll
+                        for (int c = 0; c < 64; c += 16) {
+                            float e[16];
+#pragma unroll
+                            for (int i = 0; i < 16; i++) e[i] = __uint_as_float(v[c + i]) * down * ks[c + i];
+                            cap_scores(p, e);
+#pragma unroll
+                            for (int i = 0; i < 16; i++) v[c + i] = __float_as_uint(e[i] + vl[c + i]);
+                        }
+                    }
+                    if (!all) {
+                        uint32_t any = 0;
+#pragma unroll
+                        for (int c = 0; c < 2; c++) {
+                            const int limit = r.keys - key0 - 32 * c;
+                            const uint32_t sees = sh.there[known][c] & (limit >= 32 ? ~0u : limit <= 0 ? 0u : (1u << limit) - 1);
+                            any |= sees;
+#pragma unroll
+                            for (int i = 0; i < 32; i++)
+                                if (!(sees >> i & 1)) v[32 * c + i] = 0xff800000u;
+                        }
+                        seen = seen || any;
+                    }
+                    seen = seen || all;
+#pragma unroll
+                    for (int i = 0; i < 64; i += 2) tops[i >> 1 & 3] = fmaxf(fmaxf(tops[i >> 1 & 3], __uint_as_float(v[i])), __uint_as_float(v[i + 1]));
+                    const float top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3])) - SHIFT8;
+                    if (__any_sync(~0u, top > m + RESCALE_AT || (m == -INFINITY && top > m))) {
+                        const float now = fmaxf(m, top), corr = ex2(m - (now == -INFINITY ? 0.0f : now));
+                        if (j > 0) {
+                            ok = wait_warp(&sh.summed[2 * group + ((j - 1) & 1)], s_count[(j - 1) & 1] + ((j - 1) >> 1), gave_up, WHO + dense::TG_VALUES);
+                            if (!ok) break;
+                            tmem_after();
+#pragma unroll 1
+                            for (int c = 0; c < D; c += 16) {
+                                uint32_t o[16];
+                                const uint32_t o_at = tmem + lanes + S::O_AT + (uint32_t)group * DP + c;
+                                tmem_load16(o_at, o);
+                                uint32_t a[8];
+#pragma unroll
+                                for (int h = 0; h < 16; h += 8) {
+#pragma unroll
+                                    for (int i = 0; i < 8; i++) a[i] = __float_as_uint(__uint_as_float(o[h + i]) * corr);
+                                    tmem_store8(o_at + h, a);
+                                }
+                            }
+                            tmem_stored();
+                        }
+                        sum *= corr;
+                        m = now;
+                    }
+                    const float base = m == -INFINITY ? 0.0f : m;
+                    {
+                        const uint64_t less = same_pair(-base);
+                        uint64_t total[2] = {0, 0};
+                        uint32_t a[32];
+#pragma unroll
+                        for (int i = 0; i < 64; i += 4) {
+                            const ulonglong2 by = *reinterpret_cast<const ulonglong2*>(vb + i);
+                            float2 e = pair_open(add_pair(pair_of(v[i], v[i + 1]), less)), f = pair_open(add_pair(pair_of(v[i + 2], v[i + 3]), less));
+                            e.x = ex2(e.x); e.y = ex2(e.y); f.x = ex2(f.x); f.y = ex2(f.y);
+                            total[0] = fma_pair(pair_of(__float_as_uint(e.x), __float_as_uint(e.y)), by.x, total[0]);
+                            total[1] = fma_pair(pair_of(__float_as_uint(f.x), __float_as_uint(f.y)), by.y, total[1]);
+                            a[i >> 1] = to_halves(e.x, e.y);
+                            a[(i >> 1) + 1] = to_halves(f.x, f.y);
+                        }
+                        const float2 t = pair_open(add_pair(total[0], total[1]));
+                        sum += t.x + t.y;
+                        tmem_store32(at, a);   // (over scores that have been read)
+                    }
+                    tmem_stored();
+                    tmem_before();
+                    arrive(&sh.weights[set]);
+                }
+                // the part's rows
+                const int64_t slot = w.unit + blockIdx.x;
+                const bool whole = whole_unit(p, w, w.tile, w.tile + tiles - 1), is = x < used;
+                ok = ok && wait_warp(&sh.summed[2 * group + ((tiles - 1) & 1)], s_count[(tiles - 1) & 1] + ((tiles - 1) >> 1), gave_up, WHO + dense::TG_VALUES);
+                if (ok) {
+                    tmem_after();
+                    if (!seen) sum = -1.0f;
+                    float* to_part = whole ? nullptr : part_at(l, D, slot, x, 0);
+                    const bool store = is && (whole || slot < l.slots);
+                    const float by = seen ? 1.0f / sum : 1.0f;
+#pragma unroll 1
+                    for (int c = 0; c < D; c += 16) {   // (D is a multiple of 16)
+                        uint32_t o[16];
+                        tmem_load16(tmem + lanes + S::O_AT + (uint32_t)group * DP + c, o);
+                        if (!store) continue;
+#pragma unroll
+                        for (int i = 0; i < 16; i += 8) {
+                            float4 f = make_float4(__uint_as_float(o[i]), __uint_as_float(o[i + 1]), __uint_as_float(o[i + 2]), __uint_as_float(o[i + 3]));
+                            float4 g = make_float4(__uint_as_float(o[i + 4]), __uint_as_float(o[i + 5]), __uint_as_float(o[i + 6]), __uint_as_float(o[i + 7]));
+                            if (!seen) f = g = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                            if (whole) {
+                                f.x *= by; f.y *= by; f.z *= by; f.w *= by;
+                                g.x *= by; g.y *= by; g.z *= by; g.w *= by;
+                                store_row(p, r, c + i, f);
+                                store_row(p, r, c + i + 4, g);
+                            } else {
+                                float4* at8 = reinterpret_cast<float4*>(to_part + (int64_t)((c + i) >> 3) * (S::ROWS * 8));
+                                at8[0] = f;
+                                at8[1] = g;
+                            }
+                        }
+                    }
+                    if (is) {
+                        if (whole) { if (p.lse) p.lse[r.row * p.q_heads + r.head] = seen ? lse_of(m, sum) : -INFINITY; }
+                        else if (slot < l.slots) l.ml[slot * S::ROWS + x] = make_float2(m, sum);
+                    }
+                    tmem_before();
+                    arrive(&sh.read[group]);
+                } else if (is) {   // gave up: NaN
+                    if (whole) {
+                        for (int c = 0; c < D; c++) p.out.data[r.row * p.out.row + r.head * p.out.head + c] = from_f<T>(NAN);
+                        if (p.lse) p.lse[r.row * p.q_heads + r.head] = NAN;
+                    } else if (slot < l.slots) {
+                        l.ml[slot * S::ROWS + x] = make_float2(NAN, NAN);
+                    }
+                }
+                s_count[0] += (tiles + 1) >> 1;
+                s_count[1] += tiles >> 1;
+            } else {   // a part without a second block: its turns pass
+                arrive(&sh.queries);
+                arrive(&sh.read[1]);
+            }
+            k_count += tiles;
+            arrive(&sh.parted);
+            ok = ok && wait_part(&sh.parted, part++, &sh.known[0], gave_up);
+        } while (leave());
+    }
+    tmem_before();
+    __syncthreads();
+    if (warp == PRODUCTS) {
+        __syncwarp();
+        tmem_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "n"(512) : "memory");
+    }
+    if (threadIdx.x == 0 && *gave_up && p.err) *p.err = *gave_up;
+}
+
+}  // namespace paged
+}  // namespace lmrs

@@ -379,6 +379,30 @@ def test_attention_of_several_rows(paged, case, form, dtype):
     assert (out[-2:] == 7.0).all()
 
 
+LARGE = [  # (many rows against the same keys: tensor-core products) tokens held, rows of the call or None, page, block, kv heads, group, size, prefix
+    ([40] * 29 + [0, 7], None, 16, 16, 2, 8, 128, 4500), ([200, 130], [200, 65], 32, 8, 2, 2, 64, 700), ([300], [257], 48, 12, 1, 2, 112, 0), ([90, 70, 5], [80, 64, 5], 7, 7, 1, 1, 128, 133),
+    ([10] * 9, None, 8, 8, 4, 4, 256, 3700), ([64, 129], [64, 128], 1, 1, 1, 4, 64, 65), ([150, 260], [33, 140], 64, 64, 2, 3, 208, 515), ([130] * 3, [70] * 3, 128, 128, 1, 5, 128, 1000),
+]
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16], ids=str)
+@pytest.mark.parametrize("form", [INT8, E4M3], ids=str)
+@pytest.mark.parametrize("case", LARGE, ids=lambda c: f"{len(c[0])}x{max(c[0])}-rows{max(c[1] or [1])}-page{c[2]}-block{c[3]}-{c[4]}x{c[5]}x{c[6]}-prefix{c[7]}")
+def test_attention_of_many_rows(paged, case, form, dtype):
+    lens, counts, page, block, kv, group, size, prefix = case
+    m = Made(paged, len(lens) + size, dtype, form, lens, counts or [1] * len(lens), page, block, kv, group, size, prefix, one_each=counts is None, tail=0 if counts is None else 2,
+             order="phsd" if page == 64 else "pshd", bad=[(-1, 3, -1)] if page == 32 else [(0, 0, 10 ** 6)] if page == 48 else [])
+    pages, batch = m.on_gpu()
+    for cap in (0.0, 30.0):
+        out = torch.full((m.n, m.heads, size), 7.0, dtype=dtype, device="cuda")
+        got, lse = paged.attention(pages, batch, m.q.cuda(), out=out, softcap=cap, return_lse=True)
+        m.check(out, lse, cap=cap)
+        assert counts is None or (out[-2:] == 7.0).all()
+        assert torch.equal(paged.attention(pages, batch, laid_out(m.q, "odd"), softcap=cap)[:m.n - 2], out[:m.n - 2])
+    out, lse = paged.attention(pages, batch, m.q.cuda(), scale=-0.3, return_lse=True)
+    m.check(out, lse, scale=-0.3)
+
+
 @pytest.mark.parametrize("dtype", [BF16, F16, F32], ids=str)
 @pytest.mark.parametrize("form", [INT8, E4M3], ids=str)
 def test_attention_scale_and_cap(paged, form, dtype):
