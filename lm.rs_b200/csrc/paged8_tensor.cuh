@@ -16,7 +16,10 @@ namespace paged {
 constexpr int TG_CODES128 = 7 << 8;   // (a kernel that gave up: after TG_ROWS8)
 
 template <int DP> struct TensorShape8 {
-    static constexpr int THREADS = 384, COPIERS = 2, BLOCK = 128, BLOCKS = DP <= 128 ? 2 : 1, ROWS = BLOCK * BLOCKS, KEYS = 64, WARP_KEYS = KEYS / COPIERS;
+    static constexpr int THREADS = 384, BLOCK = 128, BLOCKS = DP <= 128 ? 2 : 1, ROWS = BLOCK * BLOCKS, KEYS = 64;
+    // copying warps: for heads of up to 128 one for the keys and one for the values, all 64 of a tile; beyond that (one block of rows, so that warps 4-7 are free) four for both, 16 keys each
+    static constexpr bool SPLIT = DP <= 128;
+    static constexpr int COPIERS = SPLIT ? 2 : 4, COPIER = SPLIT ? 8 : 4, PRODUCTS = 10, WARP_KEYS = SPLIT ? 64 : 16, EACH = SPLIT ? 2 : 1;   // (their number, the first of them; keys of a lane)
     static constexpr int COL_BOXES = DP / 64;                               // 64 columns of an operand in float16: rows of 128 bytes, their 16-byte pieces rotated (SWIZZLE_128B)
     static constexpr int SLOT = COL_BOXES * KEYS * 128, SLOTS = DP <= 64 ? 8 : DP <= 128 ? 6 : 3, Q_BLOCK = COL_BOXES * BLOCK * 128;
     static constexpr int BOX = DP < 128 ? DP : 128, KV = WARP_KEYS * DP;    // codes of a copying warp: columns of a TMA box, bytes of an operand
@@ -38,9 +41,9 @@ template <int DP> struct TensorShared8 {
     uint64_t queries;                           // the part's queries are there
     uint64_t parted;                            // both groups have ended the part
     alignas(16) float key_scale[S::RING][S::KEYS], value_log[S::RING][S::KEYS], value_by[S::RING][S::KEYS];
-    KeyAt places[S::COPIERS][4][S::WARP_KEYS];  // of the last four tiles whose keys were asked for
+    KeyAt places[S::SPLIT ? 1 : S::COPIERS][4][16];   // (of warps that take both) of the last four tiles whose keys were asked for
     int part_tiles[S::COPIERS][4];              // of the last four parts
-    uint32_t there[S::RING][S::COPIERS];
+    uint32_t there[S::RING][2];
     uint32_t tmem;
     int gave_up;
 };
@@ -48,24 +51,23 @@ PG_DEVINL uint64_t mul_pair(uint64_t a, uint64_t b) { uint64_t r; asm("mul.rn.f3
 PG_DEVINL uint64_t same_pair(float a) { return pair_of(__float_as_uint(a), __float_as_uint(a)); }
 
 template <typename T, int FORM, int DP>
-__global__ void __launch_bounds__(384, 1) codes128_kernel(const __grid_constant__ Attn8Params<T> p, const __grid_constant__ Line l, const __grid_constant__ Boxes8 boxes) {
+__global__ void __launch_bounds__(TensorShape8<DP>::THREADS, 1) codes128_kernel(const __grid_constant__ Attn8Params<T> p, const __grid_constant__ Line l, const __grid_constant__ Boxes8 boxes) {
     using S = TensorShape8<DP>;
     extern __shared__ uint8_t raw[];
     __shared__ TensorShared8<DP> sh;
     uint8_t* ring = raw + (((smem_at(raw) + 1023u) & ~1023u) - smem_at(raw));
     uint8_t *queries = ring + S::SLOTS * S::SLOT, *codes = queries + S::BLOCKS * S::Q_BLOCK;
     const int warp = __shfl_sync(~0u, (int)threadIdx.x >> 5, 0), lane = threadIdx.x & 31, D = p.head_size;
-    constexpr int PRODUCTS = 8 + S::COPIERS;   // the warp that issues them
     volatile int* gave_up = &sh.gave_up;
 
     if (threadIdx.x == 0) {
-        for (int i = 0; i < S::SLOTS; i++) { mbar_init(&sh.full[i], S::COPIERS); mbar_init(&sh.empty[i], 1); }
+        for (int i = 0; i < S::SLOTS; i++) { mbar_init(&sh.full[i], S::KEYS / S::WARP_KEYS); mbar_init(&sh.empty[i], 1); }
         for (int i = 0; i < S::COPIERS * S::STAGES; i++) mbar_init(&sh.staged[0][0] + i, 1);
         for (int i = 0; i < S::RING; i++) mbar_init(&sh.known[i], S::COPIERS);
         for (int i = 0; i < 4; i++) { mbar_init(&sh.scores[i], 1); mbar_init(&sh.weights[i], 128); mbar_init(&sh.summed[i], 1); }
         for (int i = 0; i < 2; i++) mbar_init(&sh.read[i], 128);
-        mbar_init(&sh.queries, 256);
-        mbar_init(&sh.parted, 256);
+        mbar_init(&sh.queries, S::ROWS);
+        mbar_init(&sh.parted, S::ROWS);
         sh.gave_up = 0;
         fence_barrier_init();
     }
@@ -73,7 +75,7 @@ __global__ void __launch_bounds__(384, 1) codes128_kernel(const __grid_constant_
     int64_t from, to;
     walk_begin<T, S::THREADS>(p, l, w, from, to);   // (synchronises the CTA)
     if (from >= to) { grid_launch(); return; }
-    if (warp == PRODUCTS) {
+    if (warp == S::PRODUCTS) {
         __syncwarp();
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_at(&sh.tmem)), "n"(512) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
@@ -97,69 +99,102 @@ __global__ void __launch_bounds__(384, 1) codes128_kernel(const __grid_constant_
         if (w.tiles == 0) { left = 0; return false; }   // (the line ended early: lengths changed under the kernel)
         return true;
     };
-    if (warp >= 8) {
-        if (warp < 8 + S::COPIERS) {
-            // ---- keys and values: asked for as codes STAGES - 1 operands ahead, then converted.  Operands of a part come as K0 K1 V0 K2 V1 ... ----
-            const int mine = warp - 8, whole = D / 16;
-            uint8_t* stage = codes + mine * (S::STAGES * S::KV);
+    if (warp >= 4 * S::BLOCKS) {
+        if (const int copier = warp - S::COPIER; copier < S::COPIERS) {
+            // ---- keys and values: asked for as codes STAGES - 1 operands ahead, then converted.  Operands of a part lie in the ring as K0 K1 V0 K2 V1 ... ----
+            const bool takes_keys = !S::SPLIT || copier == 0, takes_values = !S::SPLIT || copier == 1;
+            const int mine = S::SPLIT ? 0 : copier, whole = D / 16, key = lane & (S::SPLIT ? 31 : S::WARP_KEYS - 1);   // (of 16 keys, two lanes each; of 64, a lane has this one and the one 32 on)
+            const bool first_lanes = S::SPLIT || lane < S::WARP_KEYS;
+            uint8_t* stage = codes + copier * (S::STAGES * S::KV);
+            uint64_t* staged = sh.staged[copier];
             const int box_rows = boxes.rows, groups = box_rows ? S::WARP_KEYS / box_rows : 0;
             constexpr int COL_BOXES = DP / S::BOX;
             const int box_col = lane % COL_BOXES, box_group = lane / COL_BOXES;
-            // what is asked for next: tile `at` of part w (`asked` keys and `values` of the part's operands have been), whose places are on their way
-            int keys_asked = 0, values_asked = 0, key_tiles = 0, value_tiles = 0, parts = 0, asked = 0;   // of the part; of all parts; operands
-            int page = -1, place = 0, boxed = 0;
+            // what is asked for next: of part w, whose places are looked up a tile ahead
+            int keys_asked = 0, values_asked = 0, key_tiles = 0, value_tiles = 0, parts = 0, asked = 0, ask_slot = 0;   // of the part; of all parts; operands
+            int page[S::EACH], place[S::EACH], boxed = 0, ahead_tiles = 0;   // ahead_tiles: of the part that w is in (w goes on to it when the last places of this one have been taken)
             bool more = true, ok = true;
             uint32_t by_tma = 0, written = 0, rounds = 0;   // a bit a slot: codes are on their way by TMA, its bytes were last written otherwise, the phase that its barrier is in
-            // w runs ahead: it goes on to the next part when the last keys of this one have been asked for
-            int ahead_tiles = 0;                            // of the part that w is in
+            uint32_t bits_of[3][S::EACH] = {};               // (of keys by themselves) which of a slot's are there
+            static_assert(S::STAGES == 3, "bits_of");
+            const int* table = nullptr;
             auto look = [&](int j) {
-                const int first = (w.tile + j) * S::KEYS + mine * S::WARP_KEYS, x = first + lane;
-                page = -1;
+                const int first = (w.tile + j) * S::KEYS + mine * S::WARP_KEYS;
+                if (j == 0) table = w.b < 0 ? p.batch.prefix : p.batch.tables + w.b * p.batch.table_stride;
                 boxed = box_rows && first + S::WARP_KEYS <= w.keys;
-                if (x < w.keys) {
-                    const int i = p.page_shift >= 0 ? x >> p.page_shift : x / p.batch.page_size;
-                    page = (w.b < 0 ? p.batch.prefix : p.batch.tables + w.b * p.batch.table_stride)[i];
-                    place = x - i * p.batch.page_size;
+#pragma unroll
+                for (int e = 0; e < S::EACH; e++) {
+                    const int x = first + key + 32 * e;
+                    page[e] = -1;
+                    place[e] = 0;
+                    if (x < w.keys) {
+                        const int i = p.page_shift >= 0 ? x >> p.page_shift : x / p.batch.page_size;
+                        page[e] = table[i];
+                        place[e] = x - i * p.batch.page_size;
+                    }
                 }
             };
             auto ask = [&]() {   // the next operand's codes, if there is one
                 if (more) {
-                    const bool values = !(keys_asked < tiles && keys_asked - values_asked < 2);
-                    const int slot = asked % S::STAGES;
-                    if (!values) {
-                        KeyAt k = {page >= 0 && page < p.batch.pages ? page : -1, place, w.head, boxed};
-                        sh.places[mine][key_tiles & 3][lane] = k;
-                        if (k.page < 0) k.page = k.place = 0;
-                        const bool is = page >= 0 && page < p.batch.pages;
-                        const int block = p.block_shift >= 0 ? k.place >> p.block_shift : k.place / p.c.block, set = key_tiles % S::RING, x = mine * S::WARP_KEYS + lane;
-                        copy4(smem_at(&sh.key_scale[set][x]), p.c.ks + k.page * p.c.ks_page + block * p.c.ks_block + k.head * p.c.ks_head, is);
-                        copy4(smem_at(&sh.value_log[set][x]), p.c.vs + k.page * p.c.vs_page + block * p.c.vs_block + k.head * p.c.vs_head, is);
-                        __syncwarp();
+                    const bool values = S::SPLIT ? takes_values : !(keys_asked < tiles && keys_asked - values_asked < 2);
+                    KeyAt k[S::EACH];
+                    if (S::SPLIT || !values) {   // whose places have been looked up
+#pragma unroll
+                        for (int e = 0; e < S::EACH; e++) {
+                            const bool is = page[e] >= 0 && page[e] < p.batch.pages;
+                            k[e] = KeyAt{is ? page[e] : -1, place[e], w.head, boxed};
+                            if (S::SPLIT) {
+                                const uint32_t bits = __ballot_sync(~0u, is);
+#pragma unroll
+                                for (int i = 0; i < 3; i++)
+                                    if (i == ask_slot) bits_of[i][e] = bits;
+                            }
+                            const int page_or_0 = is ? page[e] : 0, at = is ? place[e] : 0, block = p.block_shift >= 0 ? at >> p.block_shift : at / p.c.block;
+                            const int set = (takes_keys ? key_tiles : value_tiles) % S::RING, x = mine * S::WARP_KEYS + key + 32 * e;
+                            if (first_lanes) {
+                                if (takes_keys) copy4(smem_at(&sh.key_scale[set][x]), p.c.ks + page_or_0 * p.c.ks_page + block * p.c.ks_block + w.head * p.c.ks_head, is);
+                                if (takes_values) copy4(smem_at(&sh.value_log[set][x]), p.c.vs + page_or_0 * p.c.vs_page + block * p.c.vs_block + w.head * p.c.vs_head, is);
+                            }
+                        }
+                        if (!S::SPLIT && first_lanes) sh.places[mine][key_tiles & 3][key] = k[0];
+                    } else {
+                        k[0] = sh.places[mine][value_tiles & 3][key];
                     }
-                    const KeyAt k = sh.places[mine][(values ? value_tiles : key_tiles) & 3][lane];
-                    const uint32_t to_codes = smem_at(stage) + slot * S::KV;
-                    if (k.boxed) {   // (the same for all lanes)
-                        if (written >> slot & 1) asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-                        __syncwarp();
-                        if (lane == 0) mbar_expect_tx(&sh.staged[mine][slot], S::KV);
-                        int of = __shfl_sync(~0u, k.page, box_group * box_rows & 31), from_row = __shfl_sync(~0u, k.place, box_group * box_rows & 31);
+                    const uint32_t to_codes = smem_at(stage) + ask_slot * S::KV;
+                    __syncwarp();
+                    if (k[0].boxed) {   // (the same for all lanes)
+                        if (written >> ask_slot & 1) {
+                            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                            __syncwarp();
+                        }
+                        if (lane == 0) mbar_expect_tx(&staged[ask_slot], S::KV);
+                        const int of_key = box_group * box_rows & (S::WARP_KEYS - 1);
+                        int of = __shfl_sync(~0u, k[0].page, of_key & 31), from_row = __shfl_sync(~0u, k[0].place, of_key & 31);
+                        if (S::EACH == 2) {
+                            const int other = __shfl_sync(~0u, k[S::EACH - 1].page, of_key & 31), other_row = __shfl_sync(~0u, k[S::EACH - 1].place, of_key & 31);
+                            if (of_key >= 32) { of = other; from_row = other_row; }
+                        }
                         if (of < 0) { of = p.batch.pages; from_row = 0; }   // (outside the map: zeros)
                         __syncwarp();
                         if (box_group < groups)
-                            tma_box(to_codes + box_col * (S::WARP_KEYS * S::BOX) + box_group * box_rows * S::BOX, values ? &boxes.v : &boxes.k, S::BOX * box_col, from_row, k.head, of,
-                                    values ? boxes.v_place : boxes.k_place, values ? boxes.v_head : boxes.k_head, &sh.staged[mine][slot]);
+                            tma_box(to_codes + box_col * (S::WARP_KEYS * S::BOX) + box_group * box_rows * S::BOX, values ? &boxes.v : &boxes.k, S::BOX * box_col, from_row, k[0].head, of,
+                                    values ? boxes.v_place : boxes.k_place, values ? boxes.v_head : boxes.k_head, &staged[ask_slot]);
                         __syncwarp();
-                        by_tma |= 1u << slot;
-                        written &= ~(1u << slot);
+                        by_tma |= 1u << ask_slot;
+                        written &= ~(1u << ask_slot);
                     } else {
-                        written |= 1u << slot;
+                        written |= 1u << ask_slot;
                         const uint8_t* base = values ? p.c.v : p.c.k;
-                        const int64_t start = k.page < 0 ? -1 : values ? k.page * p.c.v_page + k.place * p.c.v_slot + k.head * p.c.v_head : k.page * p.c.k_page + k.place * p.c.k_slot + k.head * p.c.k_head;
+                        int64_t start[S::EACH];
+#pragma unroll
+                        for (int e = 0; e < S::EACH; e++)
+                            start[e] = k[e].page < 0 ? -1 : values ? k[e].page * p.c.v_page + k[e].place * p.c.v_slot + k[e].head * p.c.v_head : k[e].page * p.c.k_page + k[e].place * p.c.k_slot + k[e].head * p.c.k_head;
                         constexpr int CHUNKS = DP / 16, LANES = CHUNKS < 8 ? CHUNKS : 8, AT_ONCE = 32 / LANES;   // lanes a row, rows at a time
 #pragma unroll 2
                         for (int r0 = 0; r0 < S::WARP_KEYS; r0 += AT_ONCE) {
                             const int row = r0 + lane / LANES;
-                            const int64_t row_start = __shfl_sync(~0u, start, row);
+                            int64_t row_start = __shfl_sync(~0u, start[0], row & 31);
+                            if (S::EACH == 2 && r0 >= 32) row_start = __shfl_sync(~0u, start[S::EACH - 1], row & 31);
 #pragma unroll
                             for (int c = 0; c < CHUNKS; c += LANES) {
                                 const int piece = c + lane % LANES;
@@ -169,16 +204,12 @@ __global__ void __launch_bounds__(384, 1) codes128_kernel(const __grid_constant_
                         }
                     }
                     asked++;
-                    if (values) {
-                        value_tiles++;
-                        if (++values_asked == tiles) {   // the part's last operand: w has gone on
-                            keys_asked = values_asked = 0;
-                            tiles = ahead_tiles;
-                            more = tiles > 0;
-                        }
-                    } else {
-                        key_tiles++;
-                        if (++keys_asked < tiles) look(keys_asked);
+                    ask_slot = ask_slot + 1 == S::STAGES ? 0 : ask_slot + 1;
+                    if (values) { value_tiles++; values_asked++; }
+                    else { key_tiles++; keys_asked++; }
+                    if (S::SPLIT || !values) {   // its places are taken: look for the next ones
+                        const int taken = takes_keys ? keys_asked : values_asked;
+                        if (taken < tiles) look(taken);
                         else {
                             left -= tiles;
                             ahead_tiles = 0;
@@ -186,7 +217,7 @@ __global__ void __launch_bounds__(384, 1) codes128_kernel(const __grid_constant_
                                 walk_next_unit(p, l, w);
                                 if (w.tiles > 0) {
                                     ahead_tiles = min(left, w.tiles - w.tile);
-                                    if (lane == 0) sh.part_tiles[mine][parts & 3] = ahead_tiles;
+                                    if (lane == 0) sh.part_tiles[copier][parts & 3] = ahead_tiles;
                                     parts++;
                                     look(0);
                                 }
@@ -194,79 +225,104 @@ __global__ void __launch_bounds__(384, 1) codes128_kernel(const __grid_constant_
                             if (!ahead_tiles) left = 0;
                         }
                     }
+                    if ((takes_values ? values_asked : keys_asked) == tiles) {   // the part's last operand: w has gone on
+                        keys_asked = values_asked = 0;
+                        tiles = ahead_tiles;
+                        more = tiles > 0;
+                    }
                 }
                 copy_commit();
             };
             enter();
-            if (lane == 0) sh.part_tiles[mine][0] = tiles;
+            if (lane == 0) sh.part_tiles[copier][0] = tiles;
             parts = 1;
             __syncwarp();
             look(0);
             for (int i = 0; i < S::STAGES - 1; i++) ask();
-            // conversion: keys and values of the part that is converted, and what has been in all
-            int part = 0, k_done = 0, v_done = 0, k_all = 0, slot = 0, round = 0, done = 0, part_has = tiles;
-            {
-                __syncwarp();
-                part_has = sh.part_tiles[mine][0];
-            }
+            // conversion: keys and values of the part that is converted, its first place in the ring, and what has been in all
+            int part = 0, k_done = 0, v_done = 0, all = 0, base = 0, done = 0, from_slot = 0, part_has = tiles;
+            __syncwarp();
+            part_has = sh.part_tiles[copier][0];
             while (ok && done < asked) {
                 ask();
                 copy_wait<S::STAGES - 1>();
-                const bool values = !(k_done < part_has && k_done - v_done < 2);
-                const int from_slot = done % S::STAGES;
+                const bool values = S::SPLIT ? takes_values : !(k_done < part_has && k_done - v_done < 2);
+                const int at = base + (values ? (v_done + 1 < part_has ? 2 * v_done + 2 : 2 * part_has - 1) : k_done ? 2 * k_done - 1 : 0), slot = at % S::SLOTS;   // the operand's number in the ring
                 if (by_tma >> from_slot & 1) {
-                    ok = __all_sync(~0u, dense::mbar_wait_bounded(&sh.staged[mine][from_slot], rounds >> from_slot & 1, gave_up, TG_CODES128 + dense::TG_FULL));
+                    ok = __all_sync(~0u, dense::mbar_wait_bounded(&staged[from_slot], rounds >> from_slot & 1, gave_up, TG_CODES128 + dense::TG_FULL));
                     if (!ok) break;
                     rounds ^= 1u << from_slot;
                     by_tma &= ~(1u << from_slot);
                 }
                 __syncwarp();
-                if (!values) {
-                    const int set = k_all % S::RING, x = mine * S::WARP_KEYS + lane;
-                    const float2 v = value_terms(sh.value_log[set][x]);
-                    sh.value_log[set][x] = v.x;
-                    sh.value_by[set][x] = v.y;
-                    const unsigned bits = __ballot_sync(~0u, sh.places[mine][k_all & 3][lane].page >= 0);
-                    if (lane == 0) {
-                        sh.there[set][mine] = bits;
+                if (S::SPLIT || !values) {
+                    const int set = all % S::RING;
+                    if (takes_values && first_lanes) {
+#pragma unroll
+                        for (int e = 0; e < S::EACH; e++) {
+                            const int x = mine * S::WARP_KEYS + key + 32 * e;
+                            const float2 v = value_terms(sh.value_log[set][x]);
+                            sh.value_log[set][x] = v.x;
+                            sh.value_by[set][x] = v.y;
+                        }
+                    }
+                    if (takes_keys) {
+                        if (S::SPLIT) {
+#pragma unroll
+                            for (int e = 0; e < S::EACH; e++)
+                                if (lane == 0) sh.there[set][e] = from_slot == 0 ? bits_of[0][e] : from_slot == 1 ? bits_of[1][e] : bits_of[2][e];
+                        } else {
+                            const unsigned bits = __ballot_sync(~0u, sh.places[S::SPLIT ? 0 : mine][all & 3][key].page >= 0);
+                            if (lane == 0) reinterpret_cast<uint16_t*>(sh.there[set])[mine] = (uint16_t)bits;
+                        }
                     }
                     __syncwarp();
                     if (lane == 0) arrive(&sh.known[set]);
+                    all++;
                 }
-                ok = wait_warp(&sh.empty[slot], round + 1, gave_up, TG_CODES128 + dense::TG_FREE - dense::TG_PAGED);
+                ok = wait_warp(&sh.empty[slot], at / S::SLOTS + 1, gave_up, TG_CODES128 + dense::TG_FREE - dense::TG_PAGED);
                 if (!ok) break;
-                const uint32_t code_row = smem_at(stage) + from_slot * S::KV, to_row = smem_at(ring) + slot * S::SLOT + (mine * S::WARP_KEYS + lane) * 128;
-#pragma unroll 4
-                for (int c = 0; c < DP / 16; c++) {
-                    if (c >= whole) break;
-                    uint32_t u[4], h[8];
-                    asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(u[0]), "=r"(u[1]), "=r"(u[2]), "=r"(u[3]) : "r"(code_row + code_at<S>(lane, c)));
+                constexpr int BATCH = 4;
+#pragma unroll 1
+                for (int e = 0; e < S::EACH; e++) {
+                    const int row = key + 32 * e;
+                    uint8_t* to_row = ring + slot * S::SLOT + (mine * S::WARP_KEYS + row) * 128;
+#pragma unroll 1
+                    for (int c0 = S::SPLIT ? 0 : BATCH * (lane / S::WARP_KEYS); c0 < whole; c0 += S::SPLIT ? BATCH : 2 * BATCH) {   // (past the end of a head: zeros, or what an earlier tile left; the products do not read it)
+                        uint4 u[BATCH];
 #pragma unroll
-                    for (int i = 0; i < 4; i++) codes_to_halves<FORM, 0>(u[i], h[2 * i], h[2 * i + 1]);
-                    const uint32_t at = to_row + (c >> 2) * (S::KEYS * 128);
+                        for (int i = 0; i < BATCH; i++) u[i] = *reinterpret_cast<const uint4*>(stage + from_slot * S::KV + code_at<S>(row, c0 + i));
 #pragma unroll
-                    for (int i = 0; i < 2; i++)
-                        asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(at + (((2 * (c & 3) + i) ^ (lane & 7)) << 4)), "r"(h[4 * i]), "r"(h[4 * i + 1]), "r"(h[4 * i + 2]), "r"(h[4 * i + 3]) : "memory");
+                        for (int i = 0; i < BATCH; i++) {
+                            const uint32_t words[4] = {u[i].x, u[i].y, u[i].z, u[i].w};
+                            uint32_t h[8];
+#pragma unroll
+                            for (int k = 0; k < 4; k++) codes_to_halves<FORM, 0>(words[k], h[2 * k], h[2 * k + 1]);
+                            uint8_t* to = to_row + (c0 >> 2) * (S::KEYS * 128);
+                            *reinterpret_cast<uint4*>(to + ((2 * i ^ (row & 7)) << 4)) = make_uint4(h[0], h[1], h[2], h[3]);
+                            *reinterpret_cast<uint4*>(to + (((2 * i + 1) ^ (row & 7)) << 4)) = make_uint4(h[4], h[5], h[6], h[7]);
+                        }
+                    }
                 }
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                 __syncwarp();
                 if (lane == 0) arrive(&sh.full[slot]);
                 done++;
-                if (++slot == S::SLOTS) { slot = 0; round++; }
-                if (!values) {
-                    k_done++;
-                    k_all++;
-                } else if (++v_done == part_has) {
+                from_slot = from_slot + 1 == S::STAGES ? 0 : from_slot + 1;
+                if (values) v_done++;
+                else k_done++;
+                if ((takes_values ? v_done : k_done) == part_has) {
+                    base += 2 * part_has;
                     k_done = v_done = 0;
                     part++;
-                    if (part < parts) part_has = sh.part_tiles[mine][part & 3];
+                    if (part < parts) part_has = sh.part_tiles[copier][part & 3];
                 }
             }
             copy_wait<0>();
             if (!ok)   // gave up: what TMA was asked for lands before shared memory goes away
                 for (int i = 0; i < S::STAGES; i++)
-                    if (by_tma >> i & 1) dense::mbar_wait_for(&sh.staged[mine][i], rounds >> i & 1, nullptr);
-        } else if (warp == PRODUCTS) {
+                    if (by_tma >> i & 1) dense::mbar_wait_for(&staged[i], rounds >> i & 1, nullptr);
+        } else if (warp == S::PRODUCTS) {
             // ---- products ----
             constexpr int WHO = TG_CODES128 - dense::TG_PAGED;
             const uint32_t one = dense::elect_one();
@@ -351,37 +407,60 @@ __global__ void __launch_bounds__(384, 1) codes128_kernel(const __grid_constant_
             const int x = group * S::BLOCK + row;
             if (mine) {
                 const UnitRow r = unit_row(p, l, w, x);
-                // the row's query, as float16: all products that read the last one have ended, since their sums have been waited for
+                // The queries of the warp's rows, as float16: all products that read the last ones have ended, since their sums have been waited for.  Eight lanes a row, four rows at a time
                 float2 factor = make_float2(1.0f, 1.0f);
                 {
-                    const bool is = x < used;
-                    const T* q = is ? p.q.data + r.row * p.q.row + r.head * p.q.head : p.q.data;
-                    auto piece = [&](int c) {   // 8 elements
-                        Piece<T, 8> v;
-                        if (is && p.q_wide) v = *reinterpret_cast<const Piece<T, 8>*>(q + 8 * c);
-                        else
+                    const int c = lane & 7, whole = D / 8, row0 = (warp & 3) * 32;
+                    const uint32_t q_at = smem_at(queries) + group * S::Q_BLOCK;
+                    constexpr int AT_ONCE = DP <= 128 ? 4 : 2;   // fours of rows whose loads are under way together
+#pragma unroll 1
+                    for (int i0 = 0; i0 < 8; i0 += AT_ONCE) {
+                        Piece<T, 8> v[AT_ONCE][S::COL_BOXES];
 #pragma unroll
-                            for (int i = 0; i < 8; i++) v.v[i] = is ? q[8 * c + i] : from_f<T>(0.0f);
-                        return v;
-                    };
-                    if constexpr (!std::is_same<T, __half>::value) {
-                        float most = 0.0f;
-#pragma unroll 4
-                        for (int c = 0; c < D / 8; c++) {
-                            const Piece<T, 8> v = piece(c);
+                        for (int u = 0; u < AT_ONCE; u++) {
+                            const int at = group * S::BLOCK + row0 + 4 * (i0 + u) + (lane >> 3);
+                            const UnitRow of = unit_row(p, l, w, at);
+                            const bool is = at < used;
+                            const T* q = is ? p.q.data + of.row * p.q.row + of.head * p.q.head + 8 * c : p.q.data;
 #pragma unroll
-                            for (int i = 0; i < 8; i++) most = fmaxf(most, fabsf(to_f(v.v[i])));
+                            for (int k = 0; k < S::COL_BOXES; k++) {
+                                const bool in = is && 8 * k + c < whole;
+                                if (p.q_wide) {
+                                    if (in) v[u][k] = *reinterpret_cast<const Piece<T, 8>*>(q + 64 * k);
+                                } else {
+#pragma unroll
+                                    for (int e = 0; e < 8; e++)
+                                        if (in) v[u][k].v[e] = q[64 * k + e];
+                                }
+                                if (!in)
+#pragma unroll
+                                    for (int e = 0; e < 8; e++) v[u][k].v[e] = from_f<T>(0.0f);
+                            }
                         }
-                        factor = row_factor(most);
-                    }
-                    const uint32_t q_at = smem_at(queries) + group * S::Q_BLOCK + row * 128;
-#pragma unroll 4
-                    for (int c = 0; c < D / 8; c++) {
-                        const Piece<T, 8> v = piece(c);
-                        uint32_t h[4];
 #pragma unroll
-                        for (int i = 0; i < 4; i++) h[i] = to_halves(to_f(v.v[2 * i]) * factor.x, to_f(v.v[2 * i + 1]) * factor.x);
-                        asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(q_at + (c >> 3) * (S::BLOCK * 128) + (((c & 7) ^ (row & 7)) << 4)), "r"(h[0]), "r"(h[1]), "r"(h[2]), "r"(h[3]) : "memory");
+                        for (int u = 0; u < AT_ONCE; u++) {
+                            float2 f = make_float2(1.0f, 1.0f);
+                            if constexpr (!std::is_same<T, __half>::value) {
+                                float most = 0.0f;
+#pragma unroll
+                                for (int k = 0; k < S::COL_BOXES; k++)
+#pragma unroll
+                                    for (int e = 0; e < 8; e++) most = fmaxf(most, fabsf(to_f(v[u][k].v[e])));
+#pragma unroll
+                                for (int d = 1; d < 8; d *= 2) most = fmaxf(most, __shfl_xor_sync(~0u, most, d));
+                                f = row_factor(most);
+                                const float mine_up = __shfl_sync(~0u, f.x, 8 * (lane & 3)), mine_down = __shfl_sync(~0u, f.y, 8 * (lane & 3));
+                                if (lane >> 2 == i0 + u) factor = make_float2(mine_up, mine_down);
+                            }
+                            const int to = row0 + 4 * (i0 + u) + (lane >> 3);
+#pragma unroll
+                            for (int k = 0; k < S::COL_BOXES; k++) {
+                                uint32_t h[4];
+#pragma unroll
+                                for (int e = 0; e < 4; e++) h[e] = to_halves(to_f(v[u][k].v[2 * e]) * f.x, to_f(v[u][k].v[2 * e + 1]) * f.x);
+                                asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(q_at + k * (S::BLOCK * 128) + to * 128 + ((c ^ (to & 7)) << 4)), "r"(h[0]), "r"(h[1]), "r"(h[2]), "r"(h[3]) : "memory");
+                            }
+                        }
                     }
                     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                     arrive(&sh.queries);
@@ -496,12 +575,13 @@ __global__ void __launch_bounds__(384, 1) codes128_kernel(const __grid_constant_
                     const bool store = is && (whole || slot < l.slots);
                     const float by = seen ? 1.0f / sum : 1.0f;
 #pragma unroll 1
-                    for (int c = 0; c < D; c += 16) {   // (D is a multiple of 16)
-                        uint32_t o[16];
-                        tmem_load16(tmem + lanes + S::O_AT + (uint32_t)group * DP + c, o);
+                    for (int c = 0; c < D; c += 32) {
+                        uint32_t o[32];
+                        tmem_load32(tmem + lanes + S::O_AT + (uint32_t)group * DP + c, o);
                         if (!store) continue;
 #pragma unroll
-                        for (int i = 0; i < 16; i += 8) {
+                        for (int i = 0; i < 32; i += 8) {
+                            if (c + i >= D) break;   // (D is a multiple of 16)
                             float4 f = make_float4(__uint_as_float(o[i]), __uint_as_float(o[i + 1]), __uint_as_float(o[i + 2]), __uint_as_float(o[i + 3]));
                             float4 g = make_float4(__uint_as_float(o[i + 4]), __uint_as_float(o[i + 5]), __uint_as_float(o[i + 6]), __uint_as_float(o[i + 7]));
                             if (!seen) f = g = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
@@ -544,7 +624,7 @@ __global__ void __launch_bounds__(384, 1) codes128_kernel(const __grid_constant_
     }
     tmem_before();
     __syncthreads();
-    if (warp == PRODUCTS) {
+    if (warp == S::PRODUCTS) {
         __syncwarp();
         tmem_after();
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "n"(512) : "memory");
