@@ -50,6 +50,37 @@ template <int DP> struct TensorShared8 {
 PG_DEVINL uint64_t mul_pair(uint64_t a, uint64_t b) { uint64_t r; asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b)); return r; }
 PG_DEVINL uint64_t same_pair(float a) { return pair_of(__float_as_uint(a), __float_as_uint(a)); }
 
+// 16 dot products (times their keys' scales) of a lane, capped, as cap_scores does
+template <typename T> PG_DEVINL void cap_pairs(const AttnParams<T>& p, uint64_t (&s)[8]) {
+    const uint64_t in = same_pair(p.cap_in), out = same_pair(p.softcap * LOG2E);
+    float far = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+        s[i] = mul_pair(s[i], in);
+        const float2 x = pair_open(s[i]);
+        far = fmaxf(far, fmaxf(fabsf(x.x), fabsf(x.y)));
+    }
+    if (__all_sync(~0u, far <= 0.5f)) {   // (tanh_near, two at a time)
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+            const uint64_t y = mul_pair(s[i], s[i]);
+            uint64_t t = fma_pair(y, same_pair(21844.0f / 6081075.0f), same_pair(-1382.0f / 155925.0f));
+            t = fma_pair(y, t, same_pair(62.0f / 2835.0f));
+            t = fma_pair(y, t, same_pair(-17.0f / 315.0f));
+            t = fma_pair(y, t, same_pair(2.0f / 15.0f));
+            t = fma_pair(y, t, same_pair(-1.0f / 3.0f));
+            s[i] = mul_pair(fma_pair(mul_pair(y, t), s[i], s[i]), out);
+        }
+    } else {
+        const float cap2 = p.softcap * LOG2E;
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+            const float2 x = pair_open(s[i]);
+            s[i] = pair_of(__float_as_uint(cap2 * (fabsf(x.x) <= 0.5f ? tanh_near(x.x) : tanh_far(x.x))), __float_as_uint(cap2 * (fabsf(x.y) <= 0.5f ? tanh_near(x.y) : tanh_far(x.y))));
+        }
+    }
+}
+
 template <typename T, int FORM, int DP>
 __global__ void __launch_bounds__(TensorShape8<DP>::THREADS, 1) codes128_kernel(const __grid_constant__ Attn8Params<T> p, const __grid_constant__ Line l, const __grid_constant__ Boxes8 boxes) {
     using S = TensorShape8<DP>;
@@ -477,11 +508,17 @@ __global__ void __launch_bounds__(TensorShape8<DP>::THREADS, 1) codes128_kernel(
                     const uint32_t at = tmem + lanes + (uint32_t)set * S::KEYS;
                     const bool all = key0 + S::KEYS <= least && sh.there[known][0] == ~0u && sh.there[known][1] == ~0u;
                     const float *ks = sh.key_scale[known], *vl = sh.value_log[known], *vb = sh.value_by[known];
-                    // exponents, 64 of them in registers.  Tiles that need no mask are straight-line code
+                    // Exponents.  Tiles that need neither a mask nor a cap are straight-line code on 64 of them in registers; the others go 16 at a time, in loops, to keep that code small (the warps of all
+                    // roles wait for instructions otherwise), and leave the exponents where the scores were
                     uint32_t v[64];
-                    tmem_load64(at, v);
                     float tops[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-                    if (!(p.softcap > 0.0f)) {
+                    const bool plain = all && !(p.softcap > 0.0f);
+                    auto sees = [&](int c) {   // bit i: the row sees key 32 c + i of the tile
+                        const int limit = r.keys - key0 - 32 * c;
+                        return sh.there[known][c] & (limit >= 32 ? ~0u : limit <= 0 ? 0u : (1u << limit) - 1);
+                    };
+                    if (plain) {
+                        tmem_load64(at, v);
                         const uint64_t by = same_pair(down);
 #pragma unroll
                         for (int i = 0; i < 64; i += 4) {
@@ -489,33 +526,36 @@ __global__ void __launch_bounds__(TensorShape8<DP>::THREADS, 1) codes128_kernel(
                             const float2 e = pair_open(fma_pair(mul_pair(pair_of(v[i], v[i + 1]), k.x), by, a.x)), f = pair_open(fma_pair(mul_pair(pair_of(v[i + 2], v[i + 3]), k.y), by, a.y));
                             v[i] = __float_as_uint(e.x); v[i + 1] = __float_as_uint(e.y); v[i + 2] = __float_as_uint(f.x); v[i + 3] = __float_as_uint(f.y);
                         }
+#pragma unroll
+                        for (int i = 0; i < 64; i += 2) tops[i >> 1 & 3] = fmaxf(fmaxf(tops[i >> 1 & 3], __uint_as_float(v[i])), __uint_as_float(v[i + 1]));
+                        seen = true;
                     } else {
-#pragma unroll
+#pragma unroll 1
                         for (int c = 0; c < 64; c += 16) {
-                            float e[16];
+                            uint32_t u[16], half[8];
+                            tmem_load16(at + c, u);
+                            uint64_t e[8];
 #pragma unroll
-                            for (int i = 0; i < 16; i++) e[i] = __uint_as_float(v[c + i]) * down * ks[c + i];
-                            cap_scores(p, e);
+                            for (int i = 0; i < 8; i++) e[i] = mul_pair(mul_pair(pair_of(u[2 * i], u[2 * i + 1]), *reinterpret_cast<const uint64_t*>(ks + c + 2 * i)), same_pair(down));
+                            if (p.softcap > 0.0f) cap_pairs(p, e);
+                            const uint32_t mask = sees(c >> 5) >> (c & 16);
+                            seen = seen || (mask & 0xffff);
 #pragma unroll
-                            for (int i = 0; i < 16; i++) v[c + i] = __float_as_uint(e[i] + vl[c + i]);
+                            for (int h = 0; h < 8; h += 4) {
+#pragma unroll
+                                for (int i = 0; i < 4; i++) {
+                                    float2 x = pair_open(add_pair(e[h + i], *reinterpret_cast<const uint64_t*>(vl + c + 2 * (h + i))));
+                                    if (!(mask >> (2 * (h + i)) & 1)) x.x = -INFINITY;
+                                    if (!(mask >> (2 * (h + i) + 1) & 1)) x.y = -INFINITY;
+                                    tops[i] = fmaxf(tops[i], fmaxf(x.x, x.y));
+                                    half[2 * i] = __float_as_uint(x.x);
+                                    half[2 * i + 1] = __float_as_uint(x.y);
+                                }
+                                tmem_store8(at + c + 2 * h, half);
+                            }
                         }
+                        tmem_stored();
                     }
-                    if (!all) {
-                        uint32_t any = 0;
-#pragma unroll
-                        for (int c = 0; c < 2; c++) {
-                            const int limit = r.keys - key0 - 32 * c;
-                            const uint32_t sees = sh.there[known][c] & (limit >= 32 ? ~0u : limit <= 0 ? 0u : (1u << limit) - 1);
-                            any |= sees;
-#pragma unroll
-                            for (int i = 0; i < 32; i++)
-                                if (!(sees >> i & 1)) v[32 * c + i] = 0xff800000u;
-                        }
-                        seen = seen || any;
-                    }
-                    seen = seen || all;
-#pragma unroll
-                    for (int i = 0; i < 64; i += 2) tops[i >> 1 & 3] = fmaxf(fmaxf(tops[i >> 1 & 3], __uint_as_float(v[i])), __uint_as_float(v[i + 1]));
                     const float top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3])) - SHIFT8;
                     if (__any_sync(~0u, top > m + RESCALE_AT || (m == -INFINITY && top > m))) {
                         const float now = fmaxf(m, top), corr = ex2(m - (now == -INFINITY ? 0.0f : now));
@@ -542,24 +582,40 @@ __global__ void __launch_bounds__(TensorShape8<DP>::THREADS, 1) codes128_kernel(
                         m = now;
                     }
                     const float base = m == -INFINITY ? 0.0f : m;
-                    {
-                        const uint64_t less = same_pair(-base);
-                        uint64_t total[2] = {0, 0};
+                    const uint64_t less = same_pair(-base);
+                    uint64_t total[2] = {0, 0};
+                    auto weigh = [&](const uint32_t (&x)[4], const float* reciprocals, uint32_t& a, uint32_t& b) {   // four exponents to weights
+                        const ulonglong2 by = *reinterpret_cast<const ulonglong2*>(reciprocals);
+                        float2 e = pair_open(add_pair(pair_of(x[0], x[1]), less)), f = pair_open(add_pair(pair_of(x[2], x[3]), less));
+                        e.x = ex2(e.x); e.y = ex2(e.y); f.x = ex2(f.x); f.y = ex2(f.y);
+                        total[0] = fma_pair(pair_of(__float_as_uint(e.x), __float_as_uint(e.y)), by.x, total[0]);
+                        total[1] = fma_pair(pair_of(__float_as_uint(f.x), __float_as_uint(f.y)), by.y, total[1]);
+                        a = to_halves(e.x, e.y);
+                        b = to_halves(f.x, f.y);
+                    };
+                    if (plain) {
                         uint32_t a[32];
 #pragma unroll
                         for (int i = 0; i < 64; i += 4) {
-                            const ulonglong2 by = *reinterpret_cast<const ulonglong2*>(vb + i);
-                            float2 e = pair_open(add_pair(pair_of(v[i], v[i + 1]), less)), f = pair_open(add_pair(pair_of(v[i + 2], v[i + 3]), less));
-                            e.x = ex2(e.x); e.y = ex2(e.y); f.x = ex2(f.x); f.y = ex2(f.y);
-                            total[0] = fma_pair(pair_of(__float_as_uint(e.x), __float_as_uint(e.y)), by.x, total[0]);
-                            total[1] = fma_pair(pair_of(__float_as_uint(f.x), __float_as_uint(f.y)), by.y, total[1]);
-                            a[i >> 1] = to_halves(e.x, e.y);
-                            a[(i >> 1) + 1] = to_halves(f.x, f.y);
+                            const uint32_t x[4] = {v[i], v[i + 1], v[i + 2], v[i + 3]};
+                            weigh(x, vb + i, a[i >> 1], a[(i >> 1) + 1]);
                         }
-                        const float2 t = pair_open(add_pair(total[0], total[1]));
-                        sum += t.x + t.y;
                         tmem_store32(at, a);   // (over scores that have been read)
+                    } else {
+#pragma unroll 1
+                        for (int c = 0; c < 64; c += 16) {
+                            uint32_t u[16], a[8];
+                            tmem_load16(at + c, u);
+#pragma unroll
+                            for (int i = 0; i < 16; i += 4) {
+                                const uint32_t x[4] = {u[i], u[i + 1], u[i + 2], u[i + 3]};
+                                weigh(x, vb + c + i, a[i >> 1], a[(i >> 1) + 1]);
+                            }
+                            tmem_store8(at + (c >> 1), a);   // (columns c / 2 .. c / 2 + 7, all of them below c + 16: read)
+                        }
                     }
+                    const float2 both = pair_open(add_pair(total[0], total[1]));
+                    sum += both.x + both.y;
                     tmem_stored();
                     tmem_before();
                     arrive(&sh.weights[set]);
