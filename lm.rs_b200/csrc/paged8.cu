@@ -1,4 +1,4 @@
-// paged8.cu -- entry points of include/lmrs_b200.h for pages of 8-bit codes, and for norms with rotary positions: checks of the arguments, choice of the kernels, launches.
+// paged8.cu -- entry points of include/lmrs_b200.h for attention over pages of 8-bit codes: checks of the arguments, choice of the kernels, launches.
 // Device pointers, the caller's stream; nothing here allocates, synchronises or remembers anything from one call to the next.
 #include <float.h>
 #include <math.h>
@@ -8,223 +8,11 @@
 #include <type_traits>
 
 #include "paged8_attn.cuh"
-#include "paged8_rows.cuh"
 #include "paged8_tensor.cuh"
-#include "paged_checks.h"
+#include "paged8_checks.h"
 
 using namespace lmrs;
 using namespace lmrs::paged;
-
-namespace {
-
-// lanes of a warp that share a head of n pieces (their logarithm), and pieces of each
-int group_of(int n) {
-    int g = 0;
-    while (g < 5 && 1 << g < n) g++;
-    return g;
-}
-int rounds_of(int n) { return (n + 31) / 32; }
-template <int VEC, typename F> int by_rounds(int n, F f) {   // 16-byte pieces: 64 of a head at most; single elements: 256
-    if constexpr (VEC > 1) return rounds_of(n) <= 1 ? f(std::integral_constant<int, 1>()) : f(std::integral_constant<int, 2>());
-    else return f(std::integral_constant<int, 8>());
-}
-std::string bad_weight(const float* w, int64_t head, const char* name, int device) {
-    if (!w) return "";
-    if (!aligned(w, 4)) return std::string(name) + " does not lie on a boundary of its elements";
-    if (head < 0) return std::string("negative stride of ") + name;
-    return on_device(w, device) ? "" : std::string(name) + " is not memory of the current device";
-}
-bool wide_weight(const HeadNorm& n) { return !n.weight || (aligned(n.weight, 16) && n.head % 4 == 0); }
-// do the rows r lie over any of n bytes from p on?
-bool over(const lmrs_b200_rows_t* r, int64_t n_rows, int64_t heads, int64_t head_size, int dtype, const void* p, int64_t bytes) {
-    if (!p || !r || n_rows < 1 || heads < 1) return false;
-    typedef __int128 wide;
-    const wide a = (wide)(uintptr_t)r->data, b = (wide)(uintptr_t)p, end = a + ((wide)(n_rows - 1) * r->row + (wide)(heads - 1) * r->head + head_size) * (wide)size_of(dtype);
-    return a < b + bytes && b < end;
-}
-
-std::string bad_pages8(const lmrs_b200_pages8_t* p) {
-    if (!p || !p->k || !p->v || !p->k_scale || !p->v_scale) return "null pages";
-    if (p->form != FORM_INT8 && p->form != FORM_E4M3) return "form must be 0 (int8) or 1 (e4m3)";
-    if (p->pages < 1 || p->page_size < 1 || p->kv_heads < 1 || p->kv_heads > MAX_HEADS) return "pages, page_size and kv_heads must be positive, kv_heads at most 65535";
-    if (p->head_size < 1 || p->head_size > 256) return "head_size must be 1 .. 256";
-    if (p->block < 1 || p->page_size % p->block) return "block must divide page_size";
-    if (p->k_page < 0 || p->k_slot < 0 || p->k_head < 0 || p->v_page < 0 || p->v_slot < 0 || p->v_head < 0 || p->ks_page < 0 || p->ks_block < 0 || p->ks_head < 0 || p->vs_page < 0 || p->vs_block < 0 ||
-        p->vs_head < 0)
-        return "negative stride of pages";
-    if (!aligned(p->k_scale, 4) || !aligned(p->v_scale, 4)) return "the scales do not lie on a boundary of their elements";
-    return "";
-}
-std::string bad_pages8_memory(const lmrs_b200_pages8_t* p, int device) {
-    if (!on_device(p->k, device) || !on_device(p->v, device)) return "the pages are not memory of the current device";
-    return on_device(p->k_scale, device) && on_device(p->v_scale, device) ? "" : "the scales are not memory of the current device";
-}
-Pages8 pages8_as(const lmrs_b200_pages8_t* p) {
-    return Pages8{(uint8_t*)p->k, (uint8_t*)p->v, p->k_scale, p->v_scale, p->k_page, p->k_slot, p->k_head, p->v_page, p->v_slot, p->v_head,
-                  p->ks_page, p->ks_block, p->ks_head, p->vs_page, p->vs_block, p->vs_head, p->kv_heads, p->head_size, p->block};
-}
-Batch batch8_as(const lmrs_b200_batch_t* b, const lmrs_b200_pages8_t* p, int64_t n_rows) {
-    return Batch{b->lens, b->rows, b->tables, b->prefix, b->table_stride, b->seqs, b->table_len, b->prefix_len, p->pages, p->page_size, n_rows};
-}
-template <typename F> int by_form(int form, F f) { return form == FORM_INT8 ? f(std::integral_constant<int, FORM_INT8>()) : f(std::integral_constant<int, FORM_E4M3>()); }
-// do all codes that a head's begin with lie on 16-byte boundaries, and heads have whole pieces of 16?
-bool wide_codes(const lmrs_b200_pages8_t* p) {
-    return p->head_size % 16 == 0 && aligned(p->k, 16) && aligned(p->v, 16) && p->k_page % 16 == 0 && p->k_slot % 16 == 0 && p->k_head % 16 == 0 && p->v_page % 16 == 0 && p->v_slot % 16 == 0 &&
-           p->v_head % 16 == 0;
-}
-
-}  // namespace
-
-extern "C" int lmrs_b200_norm_rope(const lmrs_b200_rope_t* rope, int dtype, const lmrs_b200_rows_t* x, const lmrs_b200_rows_t* out, int64_t n_rows, int heads, int head_size, const float* weight,
-                                   int64_t weight_head, float eps, const lmrs_b200_positions_t* pos, void* stream) {
-    static const char* me = "norm_rope";
-    return guarded(me, [&]() -> int {
-        if (!x || !out) return refuse(me, "null argument");
-        std::string why = bad_dtype(dtype);
-        if (!why.empty()) return refuse(me, why);
-        if (n_rows < 0 || n_rows > 0x7fffffff || heads < 0 || heads > MAX_HEADS || head_size < 1 || head_size > 256)
-            return refuse(me, "n_rows must be 0 .. 2^31 - 1, heads 0 .. 65535, head_size 1 .. 256");
-        if (rope) why = bad_rope(rope, head_size);
-        if (why.empty() && (rope != nullptr) != (pos != nullptr)) why = "rope and positions come together";
-        if (why.empty() && !(eps >= 0.0f && isfinite(eps))) why = "eps must be 0 or positive";
-        if (why.empty() && !same(x, out, n_rows, heads) && meet(x, heads, out, heads, n_rows, head_size, dtype)) why = "out lies over x without being x itself";
-        if (why.empty() && over(out, n_rows, heads, head_size, dtype, weight, 4 * ((int64_t)(heads - 1) * std::max<int64_t>(weight_head, 0) + head_size))) why = "out lies over the weights";
-        if (!why.empty()) return refuse(me, why);
-        int device = 0;
-        const int sms = device_sms(me, &device);
-        if (!sms) return 1;
-        if (n_rows == 0 || heads == 0) return 0;
-        why = bad_rows(x, "x", dtype, device);
-        if (why.empty()) why = bad_rows(out, "out", dtype, device);
-        if (why.empty()) why = bad_weight(weight, weight_head, "weight", device);
-        if (why.empty() && pos) why = !pos->data ? "null positions" : bad_ints(pos->data, "positions", device);
-        if (!why.empty()) return refuse(me, why);
-        const HeadNorm norm = {weight, weight_head, eps, 1};
-        const lmrs_b200_rope_t none = {};
-        return by_type(dtype, [&](auto t) {
-            using T = decltype(t);
-            constexpr int VEC = 16 / sizeof(T);
-            const int pairs = rope ? rope->pairs : 0;
-            const bool wide = vectors(x, dtype) && vectors(out, dtype) && wide_weight(norm) && pairs % VEC == 0 && head_size % VEC == 0;
-            const Cut cut = cut_of(pairs, rope ? rope->layout : 0, head_size, wide ? VEC : 1);
-            const int n = cut.turning + cut.passing, group = group_of(n), at_once = 32 >> group;
-            const int64_t want = ((int64_t)sms * 16 + n_rows - 1) / n_rows;
-            const int parts = (int)std::max<int64_t>(1, std::min<int64_t>(want, (heads + at_once - 1) / at_once));
-            auto go = [&](auto vec) {
-                constexpr int V = decltype(vec)::value;
-                return by_rounds<V>(n, [&](auto rounds) {
-                    norm_rope_kernel<T, V, decltype(rounds)::value><<<warps_grid(n_rows * parts, sms), 32 * ROW_WARPS, 0, (cudaStream_t)stream>>>(
-                        rope ? *rope : none, rows_as<const T>(x), rows_as<T>(out), n_rows, heads, head_size, cut, norm, pos_as(pos), parts, group);
-                    return launched(me);
-                });
-            };
-            return wide ? go(std::integral_constant<int, VEC>()) : go(std::integral_constant<int, 1>());
-        });
-    });
-}
-
-extern "C" int lmrs_b200_paged8_append(const lmrs_b200_pages8_t* pages, const lmrs_b200_batch_t* batch, int dtype, int64_t n_rows, const lmrs_b200_rows_t* k, const lmrs_b200_rows_t* v,
-                                       const lmrs_b200_rope_t* rope, const lmrs_b200_positions_t* pos, const lmrs_b200_rows_t* q, const lmrs_b200_rows_t* q_out, int q_heads,
-                                       const lmrs_b200_norms_t* norms, void* stream) {
-    static const char* me = "paged8_append";
-    return guarded(me, [&]() -> int {
-        std::string why = bad_pages8(pages);
-        if (why.empty()) why = bad_dtype(dtype);
-        if (why.empty()) why = bad_batch(batch, n_rows, pages->page_size);
-        if (why.empty() && (q || q_out) && (!q || !q_out)) why = "q and q_out come together";
-        if (why.empty() && q && !rope && !(norms && norms->q)) why = "q without rope or a norm";
-        if (why.empty() && q && (q_heads < 1 || q_heads > MAX_HEADS)) why = "q_heads must be 1 .. 65535";
-        if (why.empty() && rope) why = bad_rope(rope, pages->head_size);
-        if (why.empty() && norms && !(norms->eps >= 0.0f && isfinite(norms->eps))) why = "eps must be 0 or positive";
-        const int size = why.empty() ? pages->head_size : 0;
-        if (why.empty() && q && !same(q, q_out, n_rows, q_heads) && meet(q, q_heads, q_out, q_heads, n_rows, size, dtype)) why = "q_out lies over q without being q itself";
-        if (why.empty() && q && k && v && (meet(k, pages->kv_heads, q_out, q_heads, n_rows, size, dtype) || meet(v, pages->kv_heads, q_out, q_heads, n_rows, size, dtype)))
-            why = "q_out lies over k or v";
-        if (why.empty() && q && norms && (over(q_out, n_rows, q_heads, size, dtype, norms->q, 4 * ((int64_t)(q_heads - 1) * std::max<int64_t>(norms->q_head, 0) + size)) ||
-                                          over(q_out, n_rows, q_heads, size, dtype, norms->k, 4 * ((int64_t)(pages->kv_heads - 1) * std::max<int64_t>(norms->k_head, 0) + size))))
-            why = "q_out lies over the weights";
-        if (!why.empty()) return refuse(me, why);
-        int device = 0;
-        const int sms = device_sms(me, &device);
-        if (!sms) return 1;
-        if (n_rows == 0 || batch->seqs == 0) return 0;
-        why = bad_batch_memory(batch, device);
-        if (why.empty()) why = bad_rows(k, "k", dtype, device);
-        if (why.empty()) why = bad_rows(v, "v", dtype, device);
-        if (why.empty() && q) why = bad_rows(q, "q", dtype, device);
-        if (why.empty() && q) why = bad_rows(q_out, "q_out", dtype, device);
-        if (why.empty() && pos) why = !pos->data ? "null positions" : bad_ints(pos->data, "positions", device);
-        if (why.empty() && norms) why = bad_weight(norms->k, norms->k_head, "the keys' weight", device);
-        if (why.empty() && norms) why = bad_weight(norms->q, norms->q_head, "the queries' weight", device);
-        if (why.empty()) why = bad_pages8_memory(pages, device);
-        if (!why.empty()) return refuse(me, why);
-        return by_type(dtype, [&](auto t) {
-            using T = decltype(t);
-            return by_form(pages->form, [&](auto form) {
-                PutParams<T> p = {};
-                if (rope) p.rope = *rope;
-                p.batch = batch8_as(batch, pages, n_rows);
-                p.pos = pos_as(rope ? pos : nullptr);
-                p.k = rows_as<const T>(k);
-                p.v = rows_as<const T>(v);
-                if (q) { p.q = rows_as<const T>(q); p.q_out = rows_as<T>(q_out); p.q_heads = q_heads; }
-                p.pages = pages8_as(pages);
-                if (norms) {
-                    p.k_norm = HeadNorm{norms->k, norms->k_head, norms->eps, norms->k != nullptr};
-                    p.q_norm = HeadNorm{norms->q, norms->q_head, norms->eps, norms->q != nullptr};
-                }
-                constexpr int VEC = 16 / sizeof(T);
-                const int pairs = rope ? rope->pairs : 0;
-                const bool wide = q && vectors(q, dtype) && vectors(q_out, dtype) && wide_weight(p.q_norm) && pairs % VEC == 0 && size % VEC == 0;
-                p.turn = cut_of(pairs, rope ? rope->layout : 0, size, wide ? VEC : 1);
-                const int n = p.turn.turning + p.turn.passing, at_once = 32 >> group_of(n);
-                p.group = group_of(n);
-                p.parts = (int)std::max<int64_t>(1, std::min<int64_t>(((int64_t)sms * 16 + n_rows - 1) / n_rows, (q_heads + at_once - 1) / at_once));
-                p.head_ctas = (pages->kv_heads + PUT_HEADS - 1) / PUT_HEADS;
-                p.put_ctas = (int)std::min<int64_t>(n_rows, (int64_t)sms * 64);
-                const int q_ctas = q ? (int)std::min<int64_t>((n_rows * p.parts + PUT_WARPS - 1) / PUT_WARPS, (int64_t)sms * 16) : 0;
-                auto go = [&](auto vec) {
-                    constexpr int V = decltype(vec)::value;
-                    return by_rounds<V>(n, [&](auto rounds) {
-                        paged8_append_kernel<T, decltype(form)::value, V, decltype(rounds)::value><<<(unsigned)(p.put_ctas * p.head_ctas + q_ctas), 32 * PUT_WARPS, 0, (cudaStream_t)stream>>>(p);
-                        return launched(me);
-                    });
-                };
-                return wide ? go(std::integral_constant<int, VEC>()) : go(std::integral_constant<int, 1>());
-            });
-        });
-    });
-}
-
-extern "C" int lmrs_b200_paged8_read(const lmrs_b200_pages8_t* pages, const lmrs_b200_batch_t* batch, int dtype, int64_t n_rows, const lmrs_b200_rows_t* k, const lmrs_b200_rows_t* v, void* stream) {
-    static const char* me = "paged8_read";
-    return guarded(me, [&]() -> int {
-        std::string why = bad_pages8(pages);
-        if (why.empty()) why = bad_dtype(dtype);
-        if (why.empty()) why = bad_batch(batch, n_rows, pages->page_size);
-        if (why.empty() && (!k || !v)) why = "null argument";
-        if (why.empty() && meet(k, pages->kv_heads, v, pages->kv_heads, n_rows, pages->head_size, dtype)) why = "k lies over v";
-        if (!why.empty()) return refuse(me, why);
-        int device = 0;
-        const int sms = device_sms(me, &device);
-        if (!sms) return 1;
-        if (n_rows == 0 || batch->seqs == 0) return 0;
-        why = bad_batch_memory(batch, device);
-        if (why.empty()) why = bad_rows(k, "k", dtype, device);
-        if (why.empty()) why = bad_rows(v, "v", dtype, device);
-        if (why.empty()) why = bad_pages8_memory(pages, device);
-        if (!why.empty()) return refuse(me, why);
-        return by_type(dtype, [&](auto t) {
-            using T = decltype(t);
-            return by_form(pages->form, [&](auto form) {
-                ReadParams<T> p = {batch8_as(batch, pages, n_rows), pages8_as(pages), rows_as<T>(k), rows_as<T>(v)};
-                const bool wide = wide_codes(pages) && vectors(k, dtype) && vectors(v, dtype);
-                (wide ? paged8_read_kernel<T, decltype(form)::value, 16> : paged8_read_kernel<T, decltype(form)::value, 1>)<<<warps_grid(n_rows, sms), 32 * ROW_WARPS, 0, (cudaStream_t)stream>>>(p);
-                return launched(me);
-            });
-        });
-    });
-}
 
 static std::string bad_attention8(const lmrs_b200_pages8_t* pages, const lmrs_b200_batch_t* batch, int dtype, int64_t n_rows, int q_heads) {
     std::string why = bad_pages8(pages);

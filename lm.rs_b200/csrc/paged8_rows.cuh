@@ -7,123 +7,210 @@ namespace lmrs {
 namespace paged {
 
 // ---- norms and rotation ----------------------------------------------------------------------------------------------------------------------
-// y = x / sqrt(mean x^2 + eps) * weight of a head, then its pairs turned; float32 inside, rounded once.  A head is taken by 2^group neighbouring lanes of a warp, each with ROUNDS of the pieces
-// that paged_rows.cuh cuts heads into, so that it is read once: the sum of its squares is done in the lanes' registers and a few exchanges.
+// y = x / sqrt(mean x^2 + eps) * weight of a head, then its pairs turned; float32 inside, rounded once.  A head is read once: it lies in the registers of neighbouring lanes of a warp, eight elements each, and
+// the sum of its squares takes a few exchanges.  Eight elements are four pairs that turn (two times four neighbours in halves, eight in pairs) or eight that do not, so that all lanes have the same to do.
+// Where arrays do not lie on the boundaries that this wants, or sizes are no multiples of eight, a general walk takes the elements of a head one at a time, 32 apart.
+// Two elements an instruction (f32x2) wherever there is one for it: instructions bound these kernels next to the bytes.
 struct HeadNorm {
     const float* weight;   // null: 1
     int64_t head;          // from one head's weights to the next's (0: all heads share them)
     float eps;
     int on;                // 0: no norm
 };
-template <int VEC> PG_DEVINL void load_weights(const float* w, float (&to)[VEC]) {
-    if constexpr (VEC >= 4) {
+PG_DEVINL uint64_t two(float a, float b) { uint64_t r; asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b)); return r; }
+PG_DEVINL float2 apart(uint64_t v) { float2 r; asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v)); return r; }
+PG_DEVINL uint64_t mul2(uint64_t a, uint64_t b) { uint64_t r; asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b)); return r; }
+PG_DEVINL uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) { uint64_t r; asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c)); return r; }
+
+// A row's angles as the fast walks read them: cosines and sines of 128 pairs, 1 and 0 from the last one on
+struct Turns { float c[128], s[128]; };
+// eight elements of a head, and where: lane c of its lanes has elements first .. first + 3 and second .. second + 3
+struct Eight { uint64_t v[4]; };
+struct EightAt {
+    int first, second;
+    bool zipped;   // a pair is neighbours (layout 1); else it is first + i and second + i
+    PG_DEVINL EightAt(int c, int pairs, int layout) {
+        const bool halves = layout == 0 && 4 * c < pairs;
+        first = halves ? 4 * c : 8 * c;
+        second = halves ? first + pairs : first + 4;
+        zipped = layout != 0;
+    }
+};
+template <typename T> struct Quad;   // four elements in memory
+template <> struct Quad<float> { typedef float4 type; };
+template <> struct Quad<__nv_bfloat16> { typedef uint2 type; };
+template <> struct Quad<__half> { typedef uint2 type; };
+PG_DEVINL void open_quad(float4 q, uint64_t& a, uint64_t& b, float) { a = two(q.x, q.y); b = two(q.z, q.w); }
+template <typename T> PG_DEVINL void open_quad(uint2 q, uint64_t& a, uint64_t& b, T) {
+    const float2 x = open_word(q.x, T()), y = open_word(q.y, T());
+    a = two(x.x, x.y);
+    b = two(y.x, y.y);
+}
+PG_DEVINL float4 close_quad(uint64_t a, uint64_t b, float) { const float2 x = apart(a), y = apart(b); return make_float4(x.x, x.y, y.x, y.y); }
+template <typename T> PG_DEVINL uint2 close_quad(uint64_t a, uint64_t b, T) { return make_uint2(close_word(apart(a), T()), close_word(apart(b), T())); }
+PG_DEVINL float squares8(const Eight& x) {
+    const float2 s = apart(fma2(x.v[0], x.v[0], fma2(x.v[1], x.v[1], fma2(x.v[2], x.v[2], mul2(x.v[3], x.v[3])))));
+    return s.x + s.y;
+}
+PG_DEVINL void scale8(Eight& x, float f) {
 #pragma unroll
-        for (int i = 0; i < VEC; i += 4) {
-            const float4 v = *reinterpret_cast<const float4*>(w + i);
-            to[i] = v.x; to[i + 1] = v.y; to[i + 2] = v.z; to[i + 3] = v.w;
-        }
+    for (int i = 0; i < 4; i++) x.v[i] = mul2(x.v[i], two(f, f));
+}
+PG_DEVINL void load_weights8(const float* w, const EightAt& at, Eight& to) {
+    const ulonglong2 a = *reinterpret_cast<const ulonglong2*>(w + at.first), b = *reinterpret_cast<const ulonglong2*>(w + at.second);
+    to.v[0] = a.x; to.v[1] = a.y; to.v[2] = b.x; to.v[3] = b.y;
+}
+PG_DEVINL void turn8(Eight& x, const Turns& t, int c, bool zipped) {
+    const ulonglong2 cs = *reinterpret_cast<const ulonglong2*>(t.c + 4 * c), sn = *reinterpret_cast<const ulonglong2*>(t.s + 4 * c);
+    const uint64_t minus = 0x8000000080000000ull;
+    if (zipped) {
+        const float2 p0 = apart(x.v[0]), p1 = apart(x.v[1]), p2 = apart(x.v[2]), p3 = apart(x.v[3]);
+        const uint64_t a0 = two(p0.x, p1.x), b0 = two(p0.y, p1.y), a1 = two(p2.x, p3.x), b1 = two(p2.y, p3.y);
+        const float2 y0 = apart(fma2(b0, sn.x ^ minus, mul2(a0, cs.x))), z0 = apart(fma2(b0, cs.x, mul2(a0, sn.x)));
+        const float2 y1 = apart(fma2(b1, sn.y ^ minus, mul2(a1, cs.y))), z1 = apart(fma2(b1, cs.y, mul2(a1, sn.y)));
+        x.v[0] = two(y0.x, z0.x); x.v[1] = two(y0.y, z0.y); x.v[2] = two(y1.x, z1.x); x.v[3] = two(y1.y, z1.y);
     } else {
-#pragma unroll
-        for (int i = 0; i < VEC; i++) to[i] = w[i];
+        const uint64_t a0 = x.v[0], a1 = x.v[1], b0 = x.v[2], b1 = x.v[3];
+        x.v[0] = fma2(b0, sn.x ^ minus, mul2(a0, cs.x));
+        x.v[1] = fma2(b1, sn.y ^ minus, mul2(a1, cs.y));
+        x.v[2] = fma2(b0, cs.x, mul2(a0, sn.x));
+        x.v[3] = fma2(b1, cs.y, mul2(a1, sn.y));
     }
 }
-// heads from .. to - 1 of a row, by a warp.  from and to may be the same array
-template <typename T, int VEC, int ROUNDS>
-PG_DEVINL void norm_row(const Cut& cut, const HeadNorm& norm, int group, int D, const T* x, int64_t x_head, T* out, int64_t out_head, int from, int to, const float2* angles) {
-    using P = Piece<T, VEC>;
-    const int lane = threadIdx.x & 31, width = 1 << group, mine = lane & (width - 1), n = cut.turning + cut.passing, step = cut.layout ? VEC : cut.pairs;
-    for (int h0 = from; h0 < to; h0 += 32 >> group) {
-        const int h = h0 + (lane >> group);
-        const bool is = h < to;
-        P a[ROUNDS], b[ROUNDS];
-        float sum = 0.0f;
+// the row's angles, by its warp
+PG_DEVINL void row_turns(const lmrs_b200_rope_t& rope, const Positions& pos, int64_t r, int same, Turns& t) {
+    const lmrs_b200_rope_t* at = &rope;   // (ordinary loads, as in row_angles)
+    asm("" : "+l"(at));
+    __syncwarp();
+    for (int j = threadIdx.x & 31; j < 128; j += 32) {
+        float c = 1.0f, s = 0.0f;
+        if (j < rope.pairs) cos_sin(pos.data ? pos.data[at->axis[j] * pos.axis + r * pos.row] : same, at->turns[j], c, s);
+        t.c[j] = c;
+        t.s[j] = s;
+    }
+    __syncwarp();
+}
+// heads from .. to - 1 of a row, by a warp, LANES lanes a head, NORM_AHEAD times as many heads loaded before the first is stored.  x and out may be the same array
+constexpr int NORM_AHEAD = 2;
+template <typename T, int LANES>
+PG_DEVINL void norm_row8(int pairs, int layout, const HeadNorm& norm, int D, const T* x, int64_t x_head, T* out, int64_t out_head, int from, int to, const Turns& turns) {
+    using Q = typename Quad<T>::type;
+    constexpr int HEADS = 32 / LANES;
+    const int lane = threadIdx.x & 31, c = lane & (LANES - 1);
+    const EightAt at(c, pairs, layout);
+    const bool mine = 8 * c < D;
+    const bool turns_here = pairs > 0;
+    Eight w;
+    if (norm.weight && norm.head == 0 && mine) load_weights8(norm.weight, at, w);
+    for (int h0 = from + lane / LANES; h0 < to + lane / LANES; h0 += HEADS * NORM_AHEAD) {   // (the same for all lanes)
+        Q a[NORM_AHEAD], b[NORM_AHEAD];
 #pragma unroll
-        for (int u = 0; u < ROUNDS; u++) {
-            const int c = mine + u * width;
-            if (!is || c >= n) continue;
-            const bool turns = c < cut.turning;
-            const T* p = x + h * x_head + (turns ? (cut.layout ? 2 * VEC : VEC) * c : 2 * cut.pairs + VEC * (c - cut.turning));
-            a[u] = *reinterpret_cast<const P*>(p);
-            if (turns) b[u] = *reinterpret_cast<const P*>(p + step);
+        for (int u = 0; u < NORM_AHEAD; u++) {
+            const int h = h0 + HEADS * u;
+            if (h >= to || !mine) { a[u] = Q{}; b[u] = Q{}; continue; }
+            const T* p = x + h * x_head;
+            a[u] = *reinterpret_cast<const Q*>(p + at.first);
+            b[u] = *reinterpret_cast<const Q*>(p + at.second);
+        }
 #pragma unroll
-            for (int i = 0; i < VEC; i++) {
-                const float f = to_f(a[u].v[i]), g = turns ? to_f(b[u].v[i]) : 0.0f;
-                sum = fmaf(f, f, fmaf(g, g, sum));
+        for (int u = 0; u < NORM_AHEAD; u++) {
+            const int h = h0 + HEADS * u;
+            Eight y;
+            open_quad(a[u], y.v[0], y.v[1], T());
+            open_quad(b[u], y.v[2], y.v[3], T());
+            if (norm.on) {
+                float sum = squares8(y);
+#pragma unroll
+                for (int d = LANES >> 1; d; d >>= 1) sum += __shfl_xor_sync(~0u, sum, d);
+                scale8(y, 1.0f / sqrtf(sum / (float)D + norm.eps));
             }
+            if (h >= to || !mine) continue;
+            if (norm.weight) {
+                if (norm.head) load_weights8(norm.weight + h * norm.head, at, w);
+#pragma unroll
+                for (int i = 0; i < 4; i++) y.v[i] = mul2(y.v[i], w.v[i]);
+            }
+            if (turns_here) turn8(y, turns, c, at.zipped);
+            T* p = out + h * out_head;
+            *reinterpret_cast<Q*>(p + at.first) = close_quad(y.v[0], y.v[1], T());
+            *reinterpret_cast<Q*>(p + at.second) = close_quad(y.v[2], y.v[3], T());
+        }
+    }
+}
+// the same for any size and place: a warp a head, elements first(s), second(s) of slots s = lane + 32 i; a slot is a pair that turns, or two neighbours that do not
+struct HeadSlots {
+    int pairs, layout, D;
+    PG_DEVINL int count() const { return (D + 1) / 2; }
+    PG_DEVINL int first(int s) const { return s < pairs ? (layout ? 2 * s : s) : 2 * s; }
+    PG_DEVINL int second(int s) const { return s < pairs ? (layout ? 2 * s + 1 : s + pairs) : 2 * s + 1; }   // (D: there is none)
+};
+template <typename T>
+PG_DEVINL void norm_row1(int pairs, int layout, const HeadNorm& norm, int D, const T* x, int64_t x_head, T* out, int64_t out_head, int from, int to, const Turns& turns) {
+    const HeadSlots at = {pairs, layout, D};
+    const int lane = threadIdx.x & 31;
+    for (int h = from; h < to; h++) {
+        float y[4][2], sum = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const int s = lane + 32 * i;
+            y[i][0] = s < at.count() ? to_f(x[h * x_head + at.first(s)]) : 0.0f;
+            y[i][1] = s < at.count() && at.second(s) < D ? to_f(x[h * x_head + at.second(s)]) : 0.0f;
+            sum = fmaf(y[i][0], y[i][0], fmaf(y[i][1], y[i][1], sum));
         }
         float by = 1.0f;
         if (norm.on) {
-            for (int d = width >> 1; d; d >>= 1) sum += __shfl_xor_sync(~0u, sum, d);
+            for (int d = 16; d; d >>= 1) sum += __shfl_xor_sync(~0u, sum, d);
             by = 1.0f / sqrtf(sum / (float)D + norm.eps);
         }
+        __syncwarp();   // (all of the head has been read)
 #pragma unroll
-        for (int u = 0; u < ROUNDS; u++) {
-            const int c = mine + u * width;
-            if (!is || c >= n) continue;
-            const bool turns = c < cut.turning;
-            const int e = turns ? (cut.layout ? 2 * VEC : VEC) * c : 2 * cut.pairs + VEC * (c - cut.turning);
-            float f[VEC], g[VEC];
-#pragma unroll
-            for (int i = 0; i < VEC; i++) { f[i] = to_f(a[u].v[i]) * by; g[i] = turns ? to_f(b[u].v[i]) * by : 0.0f; }
+        for (int i = 0; i < 4; i++) {
+            const int s = lane + 32 * i;
+            if (s >= at.count()) continue;
+            const int e = at.first(s), f = at.second(s);
+            float a = y[i][0] * by, b = y[i][1] * by;
             if (norm.weight) {
-                float w[VEC];
-                load_weights<VEC>(norm.weight + h * norm.head + e, w);
-#pragma unroll
-                for (int i = 0; i < VEC; i++) f[i] *= w[i];
-                if (turns) {
-                    load_weights<VEC>(norm.weight + h * norm.head + e + step, w);
-#pragma unroll
-                    for (int i = 0; i < VEC; i++) g[i] *= w[i];
-                }
+                a *= norm.weight[h * norm.head + e];
+                if (f < D) b *= norm.weight[h * norm.head + f];
             }
-            if (turns) {
-                const float2* t = angles + VEC * c;
-#pragma unroll
-                for (int i = 0; i < VEC; i++) {
-                    if (VEC > 1 && cut.layout) {   // neighbours: pairs 0 .. VEC / 2 - 1 of the piece are in f, the others in g
-                        if (i & 1) continue;
-                        turn_pair(f[i], f[i + 1 < VEC ? i + 1 : i], t[i / 2].x, t[i / 2].y);
-                        turn_pair(g[i], g[i + 1 < VEC ? i + 1 : i], t[VEC / 2 + i / 2].x, t[VEC / 2 + i / 2].y);
-                    } else {
-                        turn_pair(f[i], g[i], t[i].x, t[i].y);
-                    }
-                }
-            }
-            P o;
-            T* to_p = out + h * out_head + e;
-#pragma unroll
-            for (int i = 0; i < VEC; i++) o.v[i] = from_f<T>(f[i]);
-            *reinterpret_cast<P*>(to_p) = o;
-            if (turns) {
-#pragma unroll
-                for (int i = 0; i < VEC; i++) o.v[i] = from_f<T>(g[i]);
-                *reinterpret_cast<P*>(to_p + step) = o;
-            }
+            if (s < pairs) turn_pair(a, b, turns.c[s], turns.s[s]);
+            out[h * out_head + e] = from_f<T>(a);
+            if (f < D) out[h * out_head + f] = from_f<T>(b);
         }
     }
 }
+// LANES 0: the general walk
+template <typename T, int LANES>
+PG_DEVINL void norm_row(int pairs, int layout, const HeadNorm& norm, int D, const T* x, int64_t x_head, T* out, int64_t out_head, int from, int to, const Turns& turns) {
+    if constexpr (LANES == 0) norm_row1(pairs, layout, norm, D, x, x_head, out, out_head, from, to, turns);
+    else norm_row8<T, LANES>(pairs, layout, norm, D, x, x_head, out, out_head, from, to, turns);
+}
 
 // parts: how many warps share a row; rope.pairs 0: nothing turns
-template <typename T, int VEC, int ROUNDS>
-__global__ void __launch_bounds__(32 * ROW_WARPS) norm_rope_kernel(const __grid_constant__ lmrs_b200_rope_t rope, const Rows<const T> x, const Rows<T> out, int64_t n_rows, int heads, int D, const Cut cut,
-                                                                   const HeadNorm norm, const Positions pos, int parts, int group) {
-    __shared__ alignas(16) float2 angles[ROW_WARPS][128];
-    float2* mine = angles[threadIdx.x >> 5];
+template <typename T, int LANES>
+__global__ void __launch_bounds__(32 * ROW_WARPS) norm_rope_kernel(const __grid_constant__ lmrs_b200_rope_t rope, const Rows<const T> x, const Rows<T> out, int64_t n_rows, int heads, int D,
+                                                                   const HeadNorm norm, const Positions pos, int parts) {
+    __shared__ alignas(16) Turns turns[ROW_WARPS];
+    Turns& mine = turns[threadIdx.x >> 5];
     const int each = (heads + parts - 1) / parts;
     for (int64_t w = (int64_t)blockIdx.x * ROW_WARPS + (threadIdx.x >> 5); w < n_rows * parts; w += (int64_t)gridDim.x * ROW_WARPS) {
         const int64_t r = w / parts;
         const int from = (int)(w - r * parts) * each;
-        row_angles(rope, pos, r, 0, mine);
-        norm_row<T, VEC, ROUNDS>(cut, norm, group, D, x.data + r * x.row, x.head, out.data + r * out.row, out.head, from, min(heads, from + each), mine);
+        if (rope.pairs) row_turns(rope, pos, r, 0, mine);
+        norm_row<T, LANES>(rope.pairs, rope.layout, norm, D, x.data + r * x.row, x.head, out.data + r * out.row, out.head, from, min(heads, from + each), mine);
     }
 }
 
 // ---- appending -------------------------------------------------------------------------------------------------------------------------------
-// A CTA takes one block of tokens that share a scale: it is led by the row that is the call's first in the block, and CTAs of other rows leave at once.  First the largest size of every head
-// among the block's new tokens, then the scales (and the codes that the block held before, where its scale grows), then the new codes; keys are normed and turned again for
-// that, which is cheaper than keeping them.  All that a rounding to 8 bits depends on is computed in 64 bits, so that a code is the nearest one of the value that the formulas give, but for
-// values within some 2^-45 of a border: in 32 bits one of ten thousand codes would be its neighbour, by 1/127 of the block's largest value.
-constexpr int PUT_WARPS = 8, PUT_HEADS = 8, PUT_TOKENS = 16;   // heads a CTA takes, tokens whose angles it holds at a time
+// A warp takes one head of the keys or of the values for a block of tokens that share a scale: the largest size among the block's new tokens, the scale (and the codes that the block held before,
+// where its scale grows), the new codes.  Up to PUT_HOLD tokens stay in registers all the while; longer blocks go through the input twice.  A CTA's warps share the angles of a block's tokens.
+//
+// A code is the nearest one of the value that the formulas give, and a scale their largest value's, to within some 2^-45 of a border: in 32 bits alone one of ten thousand codes would be its neighbour, by 1/127 of
+// the block's largest value.  But 64 bits are needed where 32 cannot tell only.  With u = 2^-24, an element after its norm is off by 12 u of itself (squares: 13 u of their sum, halved by the root; mean, eps,
+// root, quotient, two products: u each), after its rotation by 17 u (|a| + |b|) of its pair (cosines 3 u, two products and a sum), which is 24 u of the turned pair's sizes; PUT_OFF is 32 u.  An element so near to a border between two codes is computed again in
+// 64 bits (head64; one head of eight has one), and so are the tokens whose largest element is within 2^-17 of the block's largest.  Inputs that 32 bits would overflow on go that way altogether.
+constexpr int PUT_WARPS = 8, PUT_TOKENS = 16;   // warps of a CTA, tokens whose angles it holds at a time
+constexpr float PUT_OFF = 0x1p-19f;
 
 template <typename T> struct PutParams {
     lmrs_b200_rope_t rope;   // pairs 0: nothing turns
@@ -133,8 +220,8 @@ template <typename T> struct PutParams {
     Rows<T> q_out;           // null data: no queries
     Pages8 pages;
     HeadNorm k_norm, q_norm;
-    Cut turn;                // of the queries
-    int q_heads, parts, group, put_ctas, head_ctas;   // CTAs that quantise: put_ctas rows times head_ctas groups of heads; the others take the queries
+    int q_heads, parts;
+    int window, windows, heads, head_ctas, put_ctas, ctas;   // CTAs that quantise: a window of rows (whose leaders they take) and `heads` heads each; the others take the queries
 };
 
 // cosine and sine of position * turns / 2^64 turns, in 64 bits
@@ -147,170 +234,459 @@ PG_DEVINL double2 cos_sin64(int position, uint64_t turns) {
     return make_double2((quarter + 1) & 2 ? -a : a, quarter & 2 ? -b : b);
 }
 
-// A head of one row in a warp's registers: lane's elements are first(i), second(i) of slots lane + 32 i; a slot is a pair that turns, or two neighbours that do not
-struct HeadSlots {
-    int pairs, layout, D;
-    PG_DEVINL int count() const { return (D + 1) / 2; }
-    PG_DEVINL int first(int s) const { return s < pairs ? (layout ? 2 * s : s) : 2 * s; }
-    PG_DEVINL int second(int s) const { return s < pairs ? (layout ? 2 * s + 1 : s + pairs) : 2 * s + 1; }   // (D: there is none)
-};
-constexpr int MOST_SLOTS = 4;   // 256 elements
-
-template <typename T> PG_DEVINL void load_head(const HeadSlots& at, const T* x, double (&y)[MOST_SLOTS][2]) {
-#pragma unroll
-    for (int i = 0; i < MOST_SLOTS; i++) {
-        const int s = (threadIdx.x & 31) + 32 * i;
-        y[i][0] = s < at.count() ? (double)to_f(x[at.first(s)]) : 0.0;
-        y[i][1] = s < at.count() && at.second(s) < at.D ? (double)to_f(x[at.second(s)]) : 0.0;
-    }
+template <typename T> PG_DEVINL int put_position(const PutParams<T>& p, int64_t row, int index, int j) {
+    return p.pos.data ? p.pos.data[p.rope.axis[j] * p.pos.axis + row * p.pos.row] : (int)(p.batch.prefix_len + index);
 }
-PG_DEVINL void norm_head(const HeadSlots& at, const HeadNorm& norm, int h, double (&y)[MOST_SLOTS][2]) {
-    if (!norm.on) return;
+// key head h of a row in 64 bits, by a warp: elements as HeadSlots has them
+template <typename T>
+static __device__ __noinline__ void head64(const PutParams<T>& p, int64_t row, int index, int h, double (&y)[4][2]) {
+    const HeadSlots at = {p.rope.pairs, p.rope.layout, p.pages.head_size};
+    const T* x = p.k.data + row * p.k.row + h * p.k.head;
+    const int lane = threadIdx.x & 31;
     double sum = 0.0;
 #pragma unroll
-    for (int i = 0; i < MOST_SLOTS; i++) sum = fma(y[i][0], y[i][0], fma(y[i][1], y[i][1], sum));
-    for (int d = 16; d; d >>= 1) sum += __shfl_xor_sync(~0u, sum, d);
-    const double by = 1.0 / sqrt(sum / at.D + (double)norm.eps);
+    for (int i = 0; i < 4; i++) {
+        const int s = lane + 32 * i;
+        y[i][0] = s < at.count() ? (double)to_f(x[at.first(s)]) : 0.0;
+        y[i][1] = s < at.count() && at.second(s) < at.D ? (double)to_f(x[at.second(s)]) : 0.0;
+        sum = fma(y[i][0], y[i][0], fma(y[i][1], y[i][1], sum));
+    }
+    if (p.k_norm.on) {
+        for (int d = 16; d; d >>= 1) sum += __shfl_xor_sync(~0u, sum, d);
+        const double by = 1.0 / sqrt(sum / at.D + (double)p.k_norm.eps);
+        const float* w = p.k_norm.weight + h * p.k_norm.head;
 #pragma unroll
-    for (int i = 0; i < MOST_SLOTS; i++) {
-        const int s = (threadIdx.x & 31) + 32 * i;
-        if (s >= at.count()) continue;
-        y[i][0] *= by;
-        y[i][1] *= by;
-        if (norm.weight) {
-            const float* w = norm.weight + h * norm.head;
-            y[i][0] *= (double)w[at.first(s)];
-            if (at.second(s) < at.D) y[i][1] *= (double)w[at.second(s)];
+        for (int i = 0; i < 4; i++) {
+            const int s = lane + 32 * i;
+            if (s >= at.count()) continue;
+            y[i][0] *= by * (double)w[at.first(s)];
+            if (at.second(s) < at.D) y[i][1] *= by * (double)w[at.second(s)];
         }
     }
-}
-PG_DEVINL void turn_head(const HeadSlots& at, const double2* angles, double (&y)[MOST_SLOTS][2]) {
-#pragma unroll
-    for (int i = 0; i < MOST_SLOTS; i++) {
-        const int s = (threadIdx.x & 31) + 32 * i;
+#pragma unroll 1
+    for (int i = 0; i < 4; i++) {
+        const int s = lane + 32 * i;
         if (s >= at.pairs) continue;
-        const double2 t = angles[s];
+        const double2 t = cos_sin64(put_position(p, row, index, s), p.rope.turns[s]);
         const double a = y[i][0], b = y[i][1];
         y[i][0] = a * t.x - b * t.y;
         y[i][1] = b * t.x + a * t.y;
     }
 }
-// the largest size of this lane's elements, as bits without the sign: they rise with the size, and NaN lies above all
-PG_DEVINL unsigned long long size_of_head(const double (&y)[MOST_SLOTS][2]) {
-    unsigned long long a = 0;
-#pragma unroll
-    for (int i = 0; i < MOST_SLOTS; i++)
-#pragma unroll
-        for (int k = 0; k < 2; k++) a = max(a, (unsigned long long)__double_as_longlong(y[i][k]) & 0x7fffffffffffffffull);
-    return a;
+PG_DEVINL unsigned long long size_bits(double a) { return (unsigned long long)__double_as_longlong(a) & 0x7fffffffffffffffull; }   // (rise with the size, and NaN lies above all)
+
+// y times by (1 / scale), off by `off` at most, as a code: its bits; unsure: a border lies too near
+template <int FORM> PG_DEVINL uint32_t quick_code(float y, float by, float off, bool& unsure) {
+    const float r = y * by;
+    const float slack = fmaf(fabsf(r), 0x1p-22f, off * fabsf(by));
+    if (FORM == FORM_INT8) {
+        const float n = rintf(r);
+        unsure = !(0.5f - fabsf(r - n) > slack);
+        return (uint32_t)(int)fminf(fmaxf(n, -127.0f), 127.0f) & 0xff;
+    }
+    const int e = max((int)(__float_as_uint(r) >> 23 & 0xff) - 127, -6) - 3;
+    const float up = __uint_as_float((uint32_t)(127 - e) << 23), t = r * up;   // (what lies above 448 is cut off: e is 125 at most)
+    unsure = !(0.5f - fabsf(t - rintf(t)) > slack * up);
+    uint16_t c;
+    asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %1;" : "=h"(c) : "f"(r));
+    return c & 0xff;
 }
 
-template <typename T, int FORM, int VEC, int ROUNDS>
-__global__ void __launch_bounds__(32 * PUT_WARPS) paged8_append_kernel(const __grid_constant__ PutParams<T> p) {
-    __shared__ alignas(16) double2 angles[PUT_TOKENS][128];
-    __shared__ unsigned long long most[2][PUT_HEADS];
-    __shared__ float scales[2][PUT_HEADS], before[2][PUT_HEADS];
+// PUT_HOLD: tokens in registers; SLOTS: slots of a lane
+template <int SLOTS> constexpr int PUT_HOLD = SLOTS == 4 ? 8 : 16;
+template <typename T, int SLOTS> struct HeldHeads {
+    float y[PUT_HOLD<SLOTS>][SLOTS][2];
+    unsigned slow;   // bit t: token t goes by 64 bits (the same for all lanes)
+};
+// n tokens (rows from `row` on) of a head
+template <typename T, int SLOTS>
+PG_DEVINL void hold_heads(const PutParams<T>& p, bool value, int64_t row, int h, int n, const Turns* turns, HeldHeads<T, SLOTS>& z) {
+    const HeadSlots at = value ? HeadSlots{0, 0, p.pages.head_size} : HeadSlots{p.rope.pairs, p.rope.layout, p.pages.head_size};
+    const Rows<const T>& from = value ? p.v : p.k;
+    const T* x = from.data + row * from.row + h * from.head;
+    const int lane = threadIdx.x & 31;
+    constexpr int HOLD = PUT_HOLD<SLOTS>;
+#pragma unroll
+    for (int t = 0; t < HOLD; t++)
+#pragma unroll
+        for (int i = 0; i < SLOTS; i++) {
+            const int s = lane + 32 * i;
+            z.y[t][i][0] = t < n && s < at.count() ? to_f(x[t * from.row + at.first(s)]) : 0.0f;
+            z.y[t][i][1] = t < n && s < at.count() && at.second(s) < at.D ? to_f(x[t * from.row + at.second(s)]) : 0.0f;
+        }
+    z.slow = 0;
+    if (value || (!p.k_norm.on && p.rope.pairs == 0)) return;   // (the inputs themselves)
+    unsigned odd = 0;
+    if (p.k_norm.on) {
+        float mine = 0.0f;   // lane t: the sum of token t's squares
+#pragma unroll
+        for (int t = 0; t < HOLD; t++) {
+            if (t >= n) break;
+            float sum = 0.0f;
+#pragma unroll
+            for (int i = 0; i < SLOTS; i++) sum = fmaf(z.y[t][i][0], z.y[t][i][0], fmaf(z.y[t][i][1], z.y[t][i][1], sum));
+            for (int d = 16; d; d >>= 1) sum += __shfl_xor_sync(~0u, sum, d);
+            if (lane == t) mine = sum;
+        }
+        const float mean = mine / (float)at.D + p.k_norm.eps, by = 1.0f / sqrtf(mean);
+        odd = lane < n && !(mean > 0x1p-100f && mean < 0x1p100f && mine < 0x1p100f) ? 1u << lane : 0;
+        const float* w = p.k_norm.weight + h * p.k_norm.head;
+        float weight[SLOTS][2];
+#pragma unroll
+        for (int i = 0; i < SLOTS; i++) {
+            const int s = lane + 32 * i;
+            weight[i][0] = s < at.count() ? w[at.first(s)] : 0.0f;
+            weight[i][1] = s < at.count() && at.second(s) < at.D ? w[at.second(s)] : 0.0f;
+        }
+#pragma unroll
+        for (int t = 0; t < HOLD; t++) {
+            const float f = __shfl_sync(~0u, by, t);
+#pragma unroll
+            for (int i = 0; i < SLOTS; i++) {
+                z.y[t][i][0] *= f * weight[i][0];
+                z.y[t][i][1] *= f * weight[i][1];
+            }
+        }
+    }
+#pragma unroll
+    for (int t = 0; t < HOLD; t++) {
+        if (t >= n) break;
+#pragma unroll
+        for (int i = 0; i < SLOTS; i++) {
+            if (!(fabsf(z.y[t][i][0]) + fabsf(z.y[t][i][1]) < 0x1p100f)) odd |= 1u << t;
+            const int s = lane + 32 * i;
+            if (s < at.pairs) {
+                turn_pair(z.y[t][i][0], z.y[t][i][1], turns[t].c[s], turns[t].s[s]);
+            }
+        }
+    }
+    z.slow = __reduce_or_sync(~0u, odd);
+}
+
+// What a warp does with a block's tokens is one of two, with the same steps: HeldHeads, elements one at a time, and HeldEights, eight a lane
+template <typename T, int FORM, int SLOTS> struct PutOne {
+    static constexpr int HOLD = PUT_HOLD<SLOTS>, LANES = 0;
+    HeldHeads<T, SLOTS> z;
+    PG_DEVINL void hold(const PutParams<T>& p, bool value, int64_t row, int h, int n, const Turns* turns) { hold_heads<T, SLOTS>(p, value, row, h, n, turns, z); }
+    PG_DEVINL uint32_t largest(int n) const {   // of this lane's elements of tokens that are not slow, as bits
+        uint32_t a = 0;
+#pragma unroll
+        for (int t = 0; t < HOLD; t++)
+#pragma unroll
+            for (int i = 0; i < SLOTS; i++)
+                if (t < n && !(z.slow >> t & 1)) a = max(a, max(__float_as_uint(z.y[t][i][0]) & 0x7fffffffu, __float_as_uint(z.y[t][i][1]) & 0x7fffffffu));
+        return a;
+    }
+    PG_DEVINL unsigned tokens_from(int n, float near) const {   // tokens that have an element of size `near` or more
+        unsigned with = 0;
+#pragma unroll
+        for (int t = 0; t < HOLD; t++)
+#pragma unroll
+            for (int i = 0; i < SLOTS; i++)
+                if (t < n && fmaxf(fabsf(z.y[t][i][0]), fabsf(z.y[t][i][1])) >= near) with |= 1u << t;
+        return with;
+    }
+    // stores the codes; returns the tokens that have unsure ones
+    PG_DEVINL unsigned close(const HeadSlots& at, bool plain, int n, float by, uint8_t* c, int64_t step) const {
+        const int lane = threadIdx.x & 31;
+        unsigned again = 0;
+#pragma unroll
+        for (int t = 0; t < HOLD; t++) {
+            if (t >= n) break;
+#pragma unroll
+            for (int i = 0; i < SLOTS; i++) {
+                const int sl = lane + 32 * i;
+                if (sl >= at.count()) continue;
+                const float off = plain ? 0.0f : (fabsf(z.y[t][i][0]) + fabsf(z.y[t][i][1])) * PUT_OFF;
+                bool unsure[2];
+                const uint32_t code[2] = {quick_code<FORM>(z.y[t][i][0], by, off, unsure[0]), quick_code<FORM>(z.y[t][i][1], by, off, unsure[1])};
+                if (unsure[0] || unsure[1]) again |= 1u << t;
+                c[t * step + at.first(sl)] = (uint8_t)code[0];
+                if (at.second(sl) < at.D) c[t * step + at.second(sl)] = (uint8_t)code[1];
+            }
+        }
+        return again;
+    }
+};
+
+// LANE lanes a token, 32 / LANE tokens at a time
+template <typename T, int FORM, int LANE> struct PutEight {
+    static constexpr int LANES = LANE, AT_ONCE = 32 / LANE, TIMES = LANE == 32 ? 8 : 16 / AT_ONCE, HOLD = AT_ONCE * TIMES;
+    Eight z[TIMES];
+    unsigned slow;
+    PG_DEVINL int token(int u) const { return u * AT_ONCE + (threadIdx.x & 31) / LANE; }
+    PG_DEVINL void hold(const PutParams<T>& p, bool value, int64_t row, int h, int n, const Turns* turns) {
+        using Q = typename Quad<T>::type;
+        const int lane = threadIdx.x & 31, c = lane & (LANE - 1), D = p.pages.head_size;
+        const EightAt at(c, value ? 0 : p.rope.pairs, value ? 0 : p.rope.layout);
+        const Rows<const T>& from = value ? p.v : p.k;
+        const T* x = from.data + row * from.row + h * from.head;
+        const bool mine = 8 * c < D;
+        Q a[TIMES], b[TIMES];
+#pragma unroll
+        for (int u = 0; u < TIMES; u++) {
+            const int t = token(u);
+            if (t >= n || !mine) { a[u] = Q{}; b[u] = Q{}; continue; }
+            a[u] = *reinterpret_cast<const Q*>(x + t * from.row + at.first);
+            b[u] = *reinterpret_cast<const Q*>(x + t * from.row + at.second);
+        }
+        const bool norm = !value && p.k_norm.on, turn = !value && p.rope.pairs;
+        Eight w = {};
+        if (norm && mine) load_weights8(p.k_norm.weight + h * p.k_norm.head, at, w);
+        unsigned odd = 0;
+#pragma unroll
+        for (int u = 0; u < TIMES; u++) {
+            Eight& y = z[u];
+            open_quad(a[u], y.v[0], y.v[1], T());
+            open_quad(b[u], y.v[2], y.v[3], T());
+            if (!norm && !turn) continue;
+            const int t = token(u);
+            float sum = squares8(y);
+            if (norm) {
+#pragma unroll
+                for (int d = LANE >> 1; d; d >>= 1) sum += __shfl_xor_sync(~0u, sum, d);
+                const float mean = sum / (float)D + p.k_norm.eps;
+                if (t < n && !(mean > 0x1p-100f && mean < 0x1p100f)) odd |= 1u << t;
+                scale8(y, 1.0f / sqrtf(mean));
+#pragma unroll
+                for (int i = 0; i < 4; i++) y.v[i] = mul2(y.v[i], w.v[i]);
+                sum = squares8(y);
+            }
+            if (t < n && !(sum < 0x1p120f)) odd |= 1u << t;   // (elements of this lane's pairs below 2^60, and none NaN)
+            if (turn) turn8(y, turns[t], c, at.zipped);
+        }
+        slow = __reduce_or_sync(~0u, odd);
+    }
+    PG_DEVINL static uint32_t size8(const Eight& y) {
+        uint32_t a = 0;
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const float2 f = apart(y.v[i]);
+            a = max(a, max(__float_as_uint(f.x) & 0x7fffffffu, __float_as_uint(f.y) & 0x7fffffffu));
+        }
+        return a;
+    }
+    PG_DEVINL uint32_t largest(int n) const {
+        uint32_t a = 0;
+#pragma unroll
+        for (int u = 0; u < TIMES; u++)
+            if (token(u) < n && !(slow >> token(u) & 1)) a = max(a, size8(z[u]));
+        return a;
+    }
+    PG_DEVINL unsigned tokens_from(int n, float near) const {
+        unsigned with = 0;
+#pragma unroll
+        for (int u = 0; u < TIMES; u++)
+            if (token(u) < n && __uint_as_float(size8(z[u])) >= near) with |= 1u << token(u);
+        return with;
+    }
+    PG_DEVINL unsigned close(const HeadSlots& slots, bool plain, int n, float by, uint8_t* codes, int64_t step) const {
+        const int c = threadIdx.x & (LANE - 1);
+        const EightAt at(c, slots.pairs, slots.layout);
+        if (8 * c >= slots.D) return 0;
+        unsigned again = 0;
+#pragma unroll
+        for (int u = 0; u < TIMES; u++) {
+            const int t = token(u);
+            if (t >= n) break;
+            const Eight& y = z[u];
+            // (an element's pair is among the lane's eight: twice the largest of them bounds its size)
+            const float off = plain ? 0.0f : 2.0f * __uint_as_float(size8(y)) * PUT_OFF * by;
+            uint32_t word[2];
+            bool unsure = false;
+            if (FORM == FORM_INT8) {
+                // y by + 1.5 2^23 has the nearest whole number in its lower bits; what is left tells how far the border is
+                const float limit = 0.5f - 127.0f * 0x1p-22f - off;
+                uint32_t n8[8];
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    const uint64_t b2 = two(by, by), r = fma2(y.v[i], b2, two(12582912.0f, 12582912.0f));
+                    const float2 rest = apart(fma2(y.v[i], b2, fma2(r, two(-1.0f, -1.0f), two(12582912.0f, 12582912.0f)))), whole = apart(r);
+                    unsure = unsure || !(fmaxf(fabsf(rest.x), fabsf(rest.y)) < limit);
+                    n8[2 * i] = __float_as_uint(whole.x);
+                    n8[2 * i + 1] = __float_as_uint(whole.y);
+                }
+#pragma unroll
+                for (int i = 0; i < 2; i++) word[i] = __byte_perm(__byte_perm(n8[4 * i], n8[4 * i + 1], 0x0040), __byte_perm(n8[4 * i + 2], n8[4 * i + 3], 0x0040), 0x5410);
+            } else {
+                uint16_t half[4];
+#pragma unroll
+                for (int i = 0; i < 4; i++) {   // what lies `slack` below and above goes to the same code
+                    const float2 r = apart(mul2(y.v[i], two(by, by)));
+                    const float sx = fmaf(fabsf(r.x), 0x1p-22f, off), sy = fmaf(fabsf(r.y), 0x1p-22f, off);
+                    uint16_t below, above;
+                    asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(below) : "f"(r.y - sy), "f"(r.x - sx));
+                    asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(above) : "f"(r.y + sy), "f"(r.x + sx));
+                    unsure = unsure || below != above;
+                    half[i] = below;
+                }
+                word[0] = half[0] | (uint32_t)half[1] << 16;
+                word[1] = half[2] | (uint32_t)half[3] << 16;
+            }
+            if (unsure) again |= 1u << t;
+            *reinterpret_cast<uint32_t*>(codes + t * step + at.first) = word[0];
+            *reinterpret_cast<uint32_t*>(codes + t * step + at.second) = word[1];
+        }
+        return again;
+    }
+};
+template <typename T, int FORM, int SLOTS> PG_DEVINL unsigned slow_tokens(const PutOne<T, FORM, SLOTS>& x) { return x.z.slow; }
+template <typename T, int FORM, int LANE> PG_DEVINL unsigned slow_tokens(const PutEight<T, FORM, LANE>& x) { return x.slow; }
+
+template <typename T, int FORM, typename Put>
+__global__ void __launch_bounds__(32 * PUT_WARPS, 2) paged8_append_kernel(const __grid_constant__ PutParams<T> p) {
+    __shared__ alignas(16) Turns turns[PUT_TOKENS];
+    constexpr int HOLD = Put::HOLD;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, D = p.pages.head_size;
-    const int puts = p.put_ctas * p.head_ctas;
-    if ((int)blockIdx.x >= puts) {   // the queries
-        float2* mine = reinterpret_cast<float2*>(angles) + 128 * warp;
+    // CTAs of both kinds take turns, so that an SM has the one's arithmetic beside the other's copies
+    const int put = (int)((int64_t)blockIdx.x * p.put_ctas / p.ctas);
+    if ((int)((int64_t)(blockIdx.x + 1) * p.put_ctas / p.ctas) == put) {   // the queries
+        const int q_ctas = p.ctas - p.put_ctas;
+        Turns& mine = turns[warp];
         const int each = (p.q_heads + p.parts - 1) / p.parts;
-        for (int64_t w = (int64_t)(blockIdx.x - puts) * PUT_WARPS + warp; w < p.batch.n_rows * p.parts; w += (int64_t)(gridDim.x - puts) * PUT_WARPS) {
+        for (int64_t w = (int64_t)(blockIdx.x - put) * PUT_WARPS + warp; w < p.batch.n_rows * p.parts; w += (int64_t)q_ctas * PUT_WARPS) {
             const int64_t r = w / p.parts;
             const int from = (int)(w - r * p.parts) * each, b = seq_of_row_warp(p.batch, r);
             if (b < 0) continue;
             const Span s = span_of(p.batch, b);
-            row_angles(p.rope, p.pos, r, (int)(p.batch.prefix_len + (int64_t)s.len - s.count + (r - s.first)), mine);
-            norm_row<T, VEC, ROUNDS>(p.turn, p.q_norm, p.group, D, p.q.data + r * p.q.row, p.q.head, p.q_out.data + r * p.q_out.row, p.q_out.head, from, min(p.q_heads, from + each), mine);
+            if (p.rope.pairs) row_turns(p.rope, p.pos, r, (int)(p.batch.prefix_len + (int64_t)s.len - s.count + (r - s.first)), mine);
+            norm_row<T, Put::LANES>(p.rope.pairs, p.rope.layout, p.q_norm, D, p.q.data + r * p.q.row, p.q.head, p.q_out.data + r * p.q_out.row, p.q_out.head, from, min(p.q_heads, from + each), mine);
         }
         return;
     }
-    const int head_cta = (int)blockIdx.x % p.head_ctas, head0 = head_cta * PUT_HEADS, heads = min(PUT_HEADS, p.pages.kv_heads - head0);
-    for (int64_t r = blockIdx.x / p.head_ctas; r < p.batch.n_rows; r += p.put_ctas) {
+    const lmrs_b200_rope_t* rope = &p.rope;   // (lanes read different entries: ordinary loads, as in row_turns)
+    asm("" : "+l"(rope));
+    const int window = put / p.head_ctas, head0 = (put - window * p.head_ctas) * p.heads, heads = min(p.heads, p.pages.kv_heads - head0);
+    int64_t r = (int64_t)window * p.window;
+    const int64_t r_end = min(r + p.window, p.batch.n_rows);
+    // Leaders of the window: rows that are their call's first in a block.  From a row on, the next one is the first of the next block or of the next sequence
+    while (r < r_end) {
         const int b = seq_of_row_warp(p.batch, r);
-        if (b < 0) continue;
+        if (b < 0) {   // (of no sequence: rows between two of them, or behind the last)
+            r++;
+            continue;
+        }
         const Span s = span_of(p.batch, b);
         const int64_t first_new = (int64_t)s.len - s.count, index64 = first_new + (r - s.first);
-        if (index64 < 0) continue;
+        if (index64 < 0) {   // padding
+            r = s.first + min((int64_t)s.count, -first_new);
+            continue;
+        }
         const int index = (int)index64, start = index / p.pages.block * p.pages.block;
-        if (index != start && r != s.first && index64 - 1 >= 0) continue;   // (the row before it leads)
+        const int tokens = (int)min((int64_t)(start + p.pages.block - index), (int64_t)s.len - index);
+        const int64_t row = r;
+        r += tokens;
+        if (index != start && row != s.first && index64 - 1 >= 0) continue;   // (the row before it leads)
         const int64_t slot = slot_of(p.batch.tables + b * p.batch.table_stride, p.batch.table_len, p.batch.page_size, p.batch.pages, index);
         if (slot < 0) continue;
         const int64_t page = slot / p.batch.page_size;
-        const int place = (int)(slot - page * p.batch.page_size), tokens = (int)min((int64_t)(start + p.pages.block - index), (int64_t)s.len - index), older = index - start;
+        const int place = (int)(slot - page * p.batch.page_size), older = index - start;
         const int64_t in_page = place / p.pages.block;
-        const HeadSlots key_at = {p.rope.pairs, p.rope.layout, D}, value_at = {0, 0, D};
-        __syncthreads();   // (the block before is done with)
-        if (threadIdx.x < 2 * PUT_HEADS) most[threadIdx.x / PUT_HEADS][threadIdx.x % PUT_HEADS] = 0;
-        double y[MOST_SLOTS][2];
-        int64_t kept = -1;   // the item that y holds
-        for (int pass = 0; pass < 2; pass++) {
-            for (int t0 = 0; t0 < tokens; t0 += PUT_TOKENS) {
-                const int now = min(PUT_TOKENS, tokens - t0);
-                if (pass == 0 || tokens > PUT_TOKENS) {
-                    __syncthreads();
-                    for (int i = threadIdx.x; i < now * p.rope.pairs; i += 32 * PUT_WARPS) {
-                        const int t = i / p.rope.pairs, j = i - t * p.rope.pairs;
-                        const int64_t row = r + t0 + t;
-                        const int position = p.pos.data ? p.pos.data[p.rope.axis[j] * p.pos.axis + row * p.pos.row] : (int)(p.batch.prefix_len + index + t0 + t);
-                        angles[t][j] = cos_sin64(position, p.rope.turns[j]);
-                    }
-                    __syncthreads();
-                }
-                for (int item = warp; item < 2 * heads * now; item += PUT_WARPS) {
-                    const int t = item / (2 * heads), which = (item - t * 2 * heads) / heads, h = item - t * 2 * heads - which * heads;
-                    const int64_t row = r + t0 + t, number = (int64_t)t0 * 2 * heads + item;
-                    const HeadSlots& at = which ? value_at : key_at;
-                    if (number != kept) {
-                        load_head(at, which ? p.v.data + row * p.v.row + (head0 + h) * p.v.head : p.k.data + row * p.k.row + (head0 + h) * p.k.head, y);
-                        if (!which) {
-                            norm_head(at, p.k_norm, head0 + h, y);
-                            turn_head(at, angles[t], y);
-                        }
-                        kept = number;
-                    }
-                    if (pass == 0) {
-                        unsigned long long a = size_of_head(y);
-                        for (int d = 16; d; d >>= 1) a = max(a, __shfl_xor_sync(~0u, a, d));
-                        if (lane == 0) atomicMax(&most[which][h], a);   // (a largest: the order does not matter)
-                    } else {
-                        const double scale = scales[which][h], by = 1.0 / scale;
-                        uint8_t* to = which ? p.pages.v + page * p.pages.v_page + (place + t0 + t) * p.pages.v_slot + (head0 + h) * p.pages.v_head
-                                            : p.pages.k + page * p.pages.k_page + (place + t0 + t) * p.pages.k_slot + (head0 + h) * p.pages.k_head;
+        auto share_turns = [&](int t0, int n) {
+            __syncthreads();
+            for (int i = threadIdx.x; i < n * 128; i += 32 * PUT_WARPS) {
+                const int t = i >> 7, j = i & 127;
+                float c = 1.0f, sn = 0.0f;
+                if (j < p.rope.pairs) cos_sin(p.pos.data ? p.pos.data[rope->axis[j] * p.pos.axis + (row + t0 + t) * p.pos.row] : (int)(p.batch.prefix_len + index + t0 + t), rope->turns[j], c, sn);
+                turns[t].c[j] = c;
+                turns[t].s[j] = sn;
+            }
+            __syncthreads();
+        };
+        const bool one_go = tokens <= HOLD;
+        // Tasks of the warp: heads of keys and of values.  Where a block takes several goes, all warps go through its tokens together, since they share the angles
+        for (int task0 = 0; task0 < 2 * heads; task0 += PUT_WARPS) {
+            const int task = task0 + warp, value = task >= heads, h = head0 + (value ? task - heads : task);
+            const bool is = task < 2 * heads;
+            Put z;
+            const HeadSlots at = value ? HeadSlots{0, 0, D} : HeadSlots{p.rope.pairs, p.rope.layout, D};
+            const bool plain = value || (!p.k_norm.on && p.rope.pairs == 0);   // (the inputs themselves)
+            float* scale_at = value ? p.pages.vs + page * p.pages.vs_page + in_page * p.pages.vs_block + h * p.pages.vs_head : p.pages.ks + page * p.pages.ks_page + in_page * p.pages.ks_block + h * p.pages.ks_head;
+            float old = 0.0f;
+            if (is && older) old = *scale_at;
+            unsigned long long most = 0;   // the largest size, as its bits
+            for (int t0 = 0; t0 < tokens; t0 += HOLD) {
+                const int n = min(HOLD, tokens - t0);
+                if (p.rope.pairs && (!one_go || task0 == 0)) share_turns(t0, n);
+                if (!is) continue;
+                z.hold(p, value, row + t0, h, n, turns);
+                const uint32_t a = __reduce_max_sync(~0u, z.largest(n));
+                if (plain) {
+                    most = max(most, size_bits((double)__uint_as_float(a)));
+                } else {
+                    const float near = fmaxf(__uint_as_float(a), (float)__longlong_as_double((long long)most)) * (1.0f - 0x1p-17f);
+                    unsigned long long top = 0;
+                    for (unsigned left = __reduce_or_sync(~0u, z.tokens_from(n, near)) | slow_tokens(z); left; left &= left - 1) {   // (one, mostly)
+                        const int t = __ffs(left) - 1;
+                        double y[4][2];
+                        head64(p, row + t0 + t, index + t0 + t, h, y);
 #pragma unroll
-                        for (int i = 0; i < MOST_SLOTS; i++) {
-                            const int sl = lane + 32 * i;
-                            if (sl >= at.count()) continue;
-                            to[at.first(sl)] = close_code<FORM>(y[i][0], scale, by);
-                            if (at.second(sl) < D) to[at.second(sl)] = close_code<FORM>(y[i][1], scale, by);
-                        }
+                        for (int i = 0; i < 4; i++) top = max(top, max(size_bits(y[i][0]), size_bits(y[i][1])));
                     }
+                    for (int d = 16; d; d >>= 1) top = max(top, __shfl_xor_sync(~0u, top, d));
+                    most = max(most, top);
                 }
             }
-            if (pass) break;
-            __syncthreads();
-            if (threadIdx.x < 2 * heads) {
-                const int which = threadIdx.x / heads, h = threadIdx.x - which * heads;
-                float* at = which ? p.pages.vs + page * p.pages.vs_page + in_page * p.pages.vs_block + (head0 + h) * p.pages.vs_head
-                                  : p.pages.ks + page * p.pages.ks_page + in_page * p.pages.ks_block + (head0 + h) * p.pages.ks_head;
-                float scale = scale_for<FORM>(__longlong_as_double((long long)most[which][h]));
-                const float old = older ? *at : scale;
+            float scale = 0.0f;
+            if (is) {
+                scale = scale_for<FORM>(__longlong_as_double((long long)most));
                 if (older && !(scale >= old)) scale = scale == scale ? old : scale;   // (NaN stays, old or new)
-                scales[which][h] = scale;
-                before[which][h] = old;
-                *at = scale;
+                if (lane == 0) *scale_at = scale;
+                // the codes that the block held, where its scale has grown
+                if (older && scale > old) {
+                    uint8_t* c = value ? p.pages.v + page * p.pages.v_page + (place - older) * p.pages.v_slot + h * p.pages.v_head : p.pages.k + page * p.pages.k_page + (place - older) * p.pages.k_slot + h * p.pages.k_head;
+                    const int64_t step = value ? p.pages.v_slot : p.pages.k_slot;
+                    const float by = 1.0f / scale;
+                    for (int t = 0; t < older; t++, c += step)
+                        for (int e = lane; e < D; e += 32) {
+                            const float x = open_code<FORM>(c[e]);
+                            bool unsure;   // (x old is off by u of itself)
+                            uint32_t code = quick_code<FORM>(x * old, by, fabsf(x * old) * 0x1p-23f, unsure);
+                            if (unsure) code = close_code<FORM>((double)x * old, scale, 1.0 / (double)scale);
+                            c[e] = (uint8_t)code;
+                        }
+                }
             }
-            __syncthreads();
-            // the codes that the block held, where its scale has grown
-            for (int item = warp; item < 2 * heads * older; item += PUT_WARPS) {
-                const int t = item / (2 * heads), which = (item - t * 2 * heads) / heads, h = item - t * 2 * heads - which * heads;
-                const double old = before[which][h], scale = scales[which][h], by = 1.0 / scale;
-                if (!(scale > old)) continue;
-                uint8_t* at = which ? p.pages.v + page * p.pages.v_page + (place - older + t) * p.pages.v_slot + (head0 + h) * p.pages.v_head
-                                    : p.pages.k + page * p.pages.k_page + (place - older + t) * p.pages.k_slot + (head0 + h) * p.pages.k_head;
-                for (int e = lane; e < D; e += 32) at[e] = close_code<FORM>((double)open_code<FORM>(at[e]) * old, scale, by);
+            // the new codes
+            for (int t0 = 0; t0 < tokens; t0 += HOLD) {
+                const int n = min(HOLD, tokens - t0);
+                if (!one_go) {
+                    if (p.rope.pairs) share_turns(t0, n);
+                    if (is) z.hold(p, value, row + t0, h, n, turns);
+                }
+                if (!is) continue;
+                uint8_t* c = value ? p.pages.v + page * p.pages.v_page + (place + t0) * p.pages.v_slot + h * p.pages.v_head : p.pages.k + page * p.pages.k_page + (place + t0) * p.pages.k_slot + h * p.pages.k_head;
+                const int64_t step = value ? p.pages.v_slot : p.pages.k_slot;
+                // (at the largest scale elements may lie beyond the largest code, and with one that is NaN they all are: both go by 64 bits)
+                const unsigned all = (1u << n) - 1;
+                const unsigned again = scale < SCALE_MOST ? __reduce_or_sync(~0u, z.close(at, plain, n, 1.0f / scale, c, step)) | slow_tokens(z) : all;
+                __syncwarp();   // (the lanes that write a head again are others)
+                for (unsigned left = again; left; left &= left - 1) {
+                    const int t = __ffs(left) - 1;
+                    double y[4][2];
+                    if (plain) {
+                        const Rows<const T>& from = value ? p.v : p.k;
+                        const T* x = from.data + (row + t0 + t) * from.row + h * from.head;
+#pragma unroll
+                        for (int i = 0; i < 4; i++) {
+                            const int sl = lane + 32 * i;
+                            y[i][0] = sl < at.count() ? (double)to_f(x[at.first(sl)]) : 0.0;
+                            y[i][1] = sl < at.count() && at.second(sl) < D ? (double)to_f(x[at.second(sl)]) : 0.0;
+                        }
+                    } else {
+                        head64(p, row + t0 + t, index + t0 + t, h, y);
+                    }
+#pragma unroll
+                    for (int i = 0; i < 4; i++) {
+                        const int sl = lane + 32 * i;
+                        if (sl >= at.count()) continue;
+                        c[t * step + at.first(sl)] = close_code<FORM>(y[i][0], scale, 1.0 / (double)scale);
+                        if (at.second(sl) < D) c[t * step + at.second(sl)] = close_code<FORM>(y[i][1], scale, 1.0 / (double)scale);
+                    }
+                }
             }
         }
+        if (p.rope.pairs) __syncthreads();   // (the angles are used by all until here)
     }
 }
 
