@@ -91,7 +91,9 @@ PG_DEVINL void row_turns(const lmrs_b200_rope_t& rope, const Positions& pos, int
     __syncwarp();
 }
 // heads from .. to - 1 of a row, by a warp, LANES lanes a head, NORM_AHEAD times as many heads loaded before the first is stored.  x and out may be the same array
-constexpr int NORM_AHEAD = 2;
+template <typename T> constexpr int NORM_AHEAD = sizeof(T) == 2 ? 4 : 2;
+// 1 / sqrt(sum / D + eps), off by 4 u (u = 2^-24) for the root's approximation and 2 u for what it is taken of
+PG_DEVINL float norm_factor(float sum, float over_D, float eps) { return rsqrtf(fmaf(sum, over_D, eps)); }
 template <typename T, int LANES>
 PG_DEVINL void norm_row8(int pairs, int layout, const HeadNorm& norm, int D, const T* x, int64_t x_head, T* out, int64_t out_head, int from, int to, const Turns& turns) {
     using Q = typename Quad<T>::type;
@@ -100,12 +102,14 @@ PG_DEVINL void norm_row8(int pairs, int layout, const HeadNorm& norm, int D, con
     const EightAt at(c, pairs, layout);
     const bool mine = 8 * c < D;
     const bool turns_here = pairs > 0;
+    constexpr int AHEAD = NORM_AHEAD<T>;
+    const float over_D = 1.0f / (float)D;
     Eight w;
     if (norm.weight && norm.head == 0 && mine) load_weights8(norm.weight, at, w);
-    for (int h0 = from + lane / LANES; h0 < to + lane / LANES; h0 += HEADS * NORM_AHEAD) {   // (the same for all lanes)
-        Q a[NORM_AHEAD], b[NORM_AHEAD];
+    for (int h0 = from + lane / LANES; h0 < to + lane / LANES; h0 += HEADS * AHEAD) {   // (the same for all lanes)
+        Q a[AHEAD], b[AHEAD];
 #pragma unroll
-        for (int u = 0; u < NORM_AHEAD; u++) {
+        for (int u = 0; u < AHEAD; u++) {
             const int h = h0 + HEADS * u;
             if (h >= to || !mine) { a[u] = Q{}; b[u] = Q{}; continue; }
             const T* p = x + h * x_head;
@@ -113,8 +117,11 @@ PG_DEVINL void norm_row8(int pairs, int layout, const HeadNorm& norm, int D, con
             b[u] = *reinterpret_cast<const Q*>(p + at.second);
         }
 #pragma unroll
-        for (int u = 0; u < NORM_AHEAD; u++) {
+        for (int u = 0; u < AHEAD; u++) {
             const int h = h0 + HEADS * u;
+            if (h0 - lane / LANES + HEADS * u >= to) break;   // (all lanes)
+            const bool is = h < to && mine;
+            if (norm.weight && norm.head && is) load_weights8(norm.weight + h * norm.head, at, w);
             Eight y;
             open_quad(a[u], y.v[0], y.v[1], T());
             open_quad(b[u], y.v[2], y.v[3], T());
@@ -122,11 +129,10 @@ PG_DEVINL void norm_row8(int pairs, int layout, const HeadNorm& norm, int D, con
                 float sum = squares8(y);
 #pragma unroll
                 for (int d = LANES >> 1; d; d >>= 1) sum += __shfl_xor_sync(~0u, sum, d);
-                scale8(y, 1.0f / sqrtf(sum / (float)D + norm.eps));
+                scale8(y, norm_factor(sum, over_D, norm.eps));
             }
-            if (h >= to || !mine) continue;
+            if (!is) continue;
             if (norm.weight) {
-                if (norm.head) load_weights8(norm.weight + h * norm.head, at, w);
 #pragma unroll
                 for (int i = 0; i < 4; i++) y.v[i] = mul2(y.v[i], w.v[i]);
             }
@@ -160,7 +166,7 @@ PG_DEVINL void norm_row1(int pairs, int layout, const HeadNorm& norm, int D, con
         float by = 1.0f;
         if (norm.on) {
             for (int d = 16; d; d >>= 1) sum += __shfl_xor_sync(~0u, sum, d);
-            by = 1.0f / sqrtf(sum / (float)D + norm.eps);
+            by = norm_factor(sum, 1.0f / (float)D, norm.eps);
         }
         __syncwarp();   // (all of the head has been read)
 #pragma unroll
@@ -206,8 +212,8 @@ __global__ void __launch_bounds__(32 * ROW_WARPS) norm_rope_kernel(const __grid_
 // where its scale grows), the new codes.  Up to PUT_HOLD tokens stay in registers all the while; longer blocks go through the input twice.  A CTA's warps share the angles of a block's tokens.
 //
 // A code is the nearest one of the value that the formulas give, and a scale their largest value's, to within some 2^-45 of a border: in 32 bits alone one of ten thousand codes would be its neighbour, by 1/127 of
-// the block's largest value.  But 64 bits are needed where 32 cannot tell only.  With u = 2^-24, an element after its norm is off by 12 u of itself (squares: 13 u of their sum, halved by the root; mean, eps,
-// root, quotient, two products: u each), after its rotation by 17 u (|a| + |b|) of its pair (cosines 3 u, two products and a sum), which is 24 u of the turned pair's sizes; PUT_OFF is 32 u.  An element so near to a border between two codes is computed again in
+// the block's largest value.  But 64 bits are needed where 32 cannot tell only.  With u = 2^-24, an element after its norm is off by 14 u of itself (squares: 13 u of their sum,
+// mean 2 u, halved by the root; the root's approximation 4 u; two products), after its rotation by 19 u (|a| + |b|) of its pair (cosines 3 u, two products and a sum), which is 27 u of the turned pair's sizes; PUT_OFF is 32 u.  An element so near to a border between two codes is computed again in
 // 64 bits (head64; one head of eight has one), and so are the tokens whose largest element is within 2^-17 of the block's largest.  Inputs that 32 bits would overflow on go that way altogether.
 constexpr int PUT_WARPS = 8, PUT_TOKENS = 16;   // warps of a CTA, tokens whose angles it holds at a time
 constexpr float PUT_OFF = 0x1p-19f;
@@ -328,7 +334,7 @@ PG_DEVINL void hold_heads(const PutParams<T>& p, bool value, int64_t row, int h,
             for (int d = 16; d; d >>= 1) sum += __shfl_xor_sync(~0u, sum, d);
             if (lane == t) mine = sum;
         }
-        const float mean = mine / (float)at.D + p.k_norm.eps, by = 1.0f / sqrtf(mean);
+        const float mean = fmaf(mine, 1.0f / (float)at.D, p.k_norm.eps), by = rsqrtf(mean);
         odd = lane < n && !(mean > 0x1p-100f && mean < 0x1p100f && mine < 0x1p100f) ? 1u << lane : 0;
         const float* w = p.k_norm.weight + h * p.k_norm.head;
         float weight[SLOTS][2];
@@ -431,6 +437,7 @@ template <typename T, int FORM, int LANE> struct PutEight {
             b[u] = *reinterpret_cast<const Q*>(x + t * from.row + at.second);
         }
         const bool norm = !value && p.k_norm.on, turn = !value && p.rope.pairs;
+        const float over_D = 1.0f / (float)D;
         Eight w = {};
         if (norm && mine) load_weights8(p.k_norm.weight + h * p.k_norm.head, at, w);
         unsigned odd = 0;
@@ -445,9 +452,9 @@ template <typename T, int FORM, int LANE> struct PutEight {
             if (norm) {
 #pragma unroll
                 for (int d = LANE >> 1; d; d >>= 1) sum += __shfl_xor_sync(~0u, sum, d);
-                const float mean = sum / (float)D + p.k_norm.eps;
+                const float mean = fmaf(sum, over_D, p.k_norm.eps);
                 if (t < n && !(mean > 0x1p-100f && mean < 0x1p100f)) odd |= 1u << t;
-                scale8(y, 1.0f / sqrtf(mean));
+                scale8(y, rsqrtf(mean));
 #pragma unroll
                 for (int i = 0; i < 4; i++) y.v[i] = mul2(y.v[i], w.v[i]);
                 sum = squares8(y);
