@@ -37,8 +37,8 @@ struct Cutting8 {
 // Which kernel takes what: float32 rows8_kernel; 16-bit types by how often the keys would be read again (as in paged.cu)
 struct Which8 { bool own_tensor, front_tensor; int row_tiles; };   // row_tiles: rows of a unit of rows8_kernel, in eights
 template <int DP> struct TensorRule8 {
-    static constexpr int OWN_ROWS = DP <= 128 ? 64 : 16, FRONT_ROWS = DP <= 128 ? 17 : 1;
-    static constexpr int64_t FRONT_WORK = DP <= 128 ? 1 << 21 : 1 << 19;
+    static constexpr int OWN_ROWS = DP <= 128 ? 64 : 16, FRONT_ROWS = DP <= 128 ? 17 : 9;
+    static constexpr int64_t FRONT_WORK = DP <= 128 ? 1 << 21 : 1 << 20;
 };
 template <int DP> Which8 which8(const lmrs_b200_pages8_t* pages, const lmrs_b200_batch_t* batch, int dtype, int64_t n_rows, int q_heads) {
     using R = TensorRule8<DP>;

@@ -147,14 +147,30 @@ extern "C" int lmrs_b200_paged8_append(const lmrs_b200_pages8_t* pages, const lm
                 p.head_ctas = (pages->kv_heads + p.heads - 1) / p.heads;
                 if ((int64_t)p.windows * p.head_ctas > 0x3fffffff) return refuse(me, "n_rows * kv_heads is too large");
                 p.put_ctas = p.windows * p.head_ctas;
-                const int q_ctas = q ? (int)std::min<int64_t>((n_rows * p.parts + PUT_WARPS - 1) / PUT_WARPS, (int64_t)sms * 16) : 0;
+                // Queries in the same kernel where there are few: a second launch takes longer than they do
+                const bool apart = q && n_rows * q_heads > 1 << 14;
+                const int q_ctas = q && !apart ? (int)std::min<int64_t>((n_rows * p.parts + PUT_WARPS - 1) / PUT_WARPS, (int64_t)sms * 16) : 0;
                 p.ctas = p.put_ctas + q_ctas;
                 constexpr int FORM = decltype(form)::value;
                 auto launch = [&](auto put) {
-                    paged8_append_kernel<T, FORM, typename decltype(put)::type><<<(unsigned)p.ctas, 32 * PUT_WARPS, 0, (cudaStream_t)stream>>>(p);
-                    return launched(me);
+                    using Put = typename decltype(put)::type;
+                    cudaError_t e = cudaSuccess;
+                    if (apart) {
+                        put_queries_kernel<T, Put::LANES><<<(unsigned)std::min<int64_t>((n_rows * p.parts + ROW_WARPS - 1) / ROW_WARPS, (int64_t)sms * QUERY_CTAS), 32 * ROW_WARPS, 0, (cudaStream_t)stream>>>(p);
+                        if (launched(me)) return 1;
+                        e = launch_after(paged8_append_kernel<T, FORM, Put>, (unsigned)p.ctas, 32 * PUT_WARPS, 0, (cudaStream_t)stream, p);
+                    } else {
+                        paged8_append_kernel<T, FORM, Put><<<(unsigned)p.ctas, 32 * PUT_WARPS, 0, (cudaStream_t)stream>>>(p);
+                        e = cudaGetLastError();
+                    }
+                    return e == cudaSuccess ? 0 : refuse(me, std::string("launch failed: ") + cudaGetErrorString(e));
                 };
-                if (wide) return by_lanes(size, [&](auto lanes) { return launch(Kind<PutEight<T, FORM, decltype(lanes)::value>>()); });
+                // Few tokens of a block in a call: as many as a warp's lanes take at once, with half the registers
+                const int64_t together = std::min<int64_t>(std::min<int64_t>(batch->max_rows, n_rows), pages->block);
+                if (wide) return by_lanes(size, [&](auto lanes) {
+                    constexpr int L = decltype(lanes)::value;
+                    return together <= 32 / L ? launch(Kind<PutEight<T, FORM, L, 1>>()) : launch(Kind<PutEight<T, FORM, L, L == 8 ? 4 : 8>>());
+                });
                 return size <= 64 ? launch(Kind<PutOne<T, FORM, 1>>()) : size <= 128 ? launch(Kind<PutOne<T, FORM, 2>>()) : launch(Kind<PutOne<T, FORM, 4>>());
             });
         });

@@ -298,6 +298,25 @@ template <int FORM> PG_DEVINL uint32_t quick_code(float y, float by, float off, 
     return c & 0xff;
 }
 
+// An input by itself, x / scale as the nearest code: exactly, in 32 bits, always.  (Half of all tokens of 16-bit rows have an element in the middle of two codes but for the scale's rounding, since it and the
+// largest have 8 or 11 bits.)  With n steps the nearest to x by, x - n step scale is off by nothing near the middle: it is a multiple of half the last place of scale, or of x's where that is more, and
+// no more than 2^24 of it; so it tells which side of the middle x lies on.
+template <int FORM> PG_DEVINL uint32_t settled_code(float x, float scale, float by) {
+    const float size = fabsf(x);
+    const float r = __fmul_rn(size, by);   // (not to be joined with the sum below, which two things are made of)
+    const uint32_t sign = __float_as_uint(x) >> 31, e = FORM == FORM_INT8 ? 130u << 23 : max(__float_as_uint(r) & 0x7f800000u, 121u << 23);   // (a step is 2^(e - 3): 1 for whole numbers)
+    const float far = __uint_as_float(e + (20u << 23) + 0x400000u), half_step = __uint_as_float(e - (4u << 23));
+    const float sum = __fadd_rn(r, far);   // (n in its lower bits)
+    const float rest = fmaf(__fsub_rn(far, sum), scale, size), half = __fmul_rn(half_step, scale);
+    uint32_t n = __float_as_uint(sum) & (FORM == FORM_INT8 ? 255 : 31);
+    if (fabsf(rest) > half || (fabsf(rest) == half && (n & 1))) n += rest > 0.0f ? 1 : -1;
+    if (FORM == FORM_INT8) {
+        n = min(n, 127u);
+        return (sign ? 0u - n : n) & 0xff;
+    }
+    return min(((e - (121u << 23)) >> 20) + n, 0x7eu) | sign << 7;
+}
+
 // PUT_HOLD: tokens in registers; SLOTS: slots of a lane
 template <int SLOTS> constexpr int PUT_HOLD = SLOTS == 4 ? 8 : 16;
 template <typename T, int SLOTS> struct HeldHeads {
@@ -371,7 +390,7 @@ PG_DEVINL void hold_heads(const PutParams<T>& p, bool value, int64_t row, int h,
 
 // What a warp does with a block's tokens is one of two, with the same steps: HeldHeads, elements one at a time, and HeldEights, eight a lane
 template <typename T, int FORM, int SLOTS> struct PutOne {
-    static constexpr int HOLD = PUT_HOLD<SLOTS>, LANES = 0;
+    static constexpr int HOLD = PUT_HOLD<SLOTS>, LANES = 0, CTAS = 2;
     HeldHeads<T, SLOTS> z;
     PG_DEVINL void hold(const PutParams<T>& p, bool value, int64_t row, int h, int n, const Turns* turns) { hold_heads<T, SLOTS>(p, value, row, h, n, turns, z); }
     PG_DEVINL uint32_t largest(int n) const {   // of this lane's elements of tokens that are not slow, as bits
@@ -393,7 +412,8 @@ template <typename T, int FORM, int SLOTS> struct PutOne {
         return with;
     }
     // stores the codes; returns the tokens that have unsure ones
-    PG_DEVINL unsigned close(const HeadSlots& at, bool plain, int n, float by, uint8_t* c, int64_t step) const {
+    PG_DEVINL unsigned close(const HeadSlots& at, bool plain, int n, float scale, uint8_t* c, int64_t step) const {
+        const float by = 1.0f / scale;
         const int lane = threadIdx.x & 31;
         unsigned again = 0;
 #pragma unroll
@@ -405,8 +425,13 @@ template <typename T, int FORM, int SLOTS> struct PutOne {
                 if (sl >= at.count()) continue;
                 const float off = plain ? 0.0f : (fabsf(z.y[t][i][0]) + fabsf(z.y[t][i][1])) * PUT_OFF;
                 bool unsure[2];
-                const uint32_t code[2] = {quick_code<FORM>(z.y[t][i][0], by, off, unsure[0]), quick_code<FORM>(z.y[t][i][1], by, off, unsure[1])};
-                if (unsure[0] || unsure[1]) again |= 1u << t;
+                uint32_t code[2] = {quick_code<FORM>(z.y[t][i][0], by, off, unsure[0]), quick_code<FORM>(z.y[t][i][1], by, off, unsure[1])};
+                if (plain) {
+                    if (unsure[0]) code[0] = settled_code<FORM>(z.y[t][i][0], scale, by);
+                    if (unsure[1]) code[1] = settled_code<FORM>(z.y[t][i][1], scale, by);
+                } else if (unsure[0] || unsure[1]) {
+                    again |= 1u << t;
+                }
                 c[t * step + at.first(sl)] = (uint8_t)code[0];
                 if (at.second(sl) < at.D) c[t * step + at.second(sl)] = (uint8_t)code[1];
             }
@@ -415,13 +440,25 @@ template <typename T, int FORM, int SLOTS> struct PutOne {
     }
 };
 
+// r, off by `off` and 2^-22 of itself, as a code.  Codes are n steps of 2^(e - 3), e the exponent of r or -6: r + 1.5 2^23 steps has n in its lower bits (conversions by cvt, two for two elements, were slower:
+// 10,900 rows of 8 heads as they are 131 us, and 74 in int8)
+PG_DEVINL uint32_t e4m3_code(float r, float off, bool& unsure) {
+    const float size = fabsf(r);
+    const uint32_t e = max(__float_as_uint(size) & 0x7f800000u, 121u << 23);
+    const float far = __uint_as_float(e + (20u << 23) + 0x400000u), sum = __fadd_rn(size, far);
+    const float rest = __fsub_rn(size, __fsub_rn(sum, far)), half_step = __uint_as_float(e - (4u << 23));
+    unsure = unsure || !(fabsf(rest) + fmaf(size, 0x1p-22f, off) < half_step);
+    return min(((e - (121u << 23)) >> 20) + (__float_as_uint(sum) & 31), 0x7eu) | (__float_as_uint(r) >> 24 & 0x80);
+}
+
 // LANE lanes a token, 32 / LANE tokens at a time
-template <typename T, int FORM, int LANE> struct PutEight {
-    static constexpr int LANES = LANE, AT_ONCE = 32 / LANE, TIMES = LANE == 32 ? 8 : 16 / AT_ONCE, HOLD = AT_ONCE * TIMES;
+template <typename T, int FORM, int LANE, int TIMES_> struct PutEight {
+    static constexpr int LANES = LANE, AT_ONCE = 32 / LANE, TIMES = TIMES_, HOLD = AT_ONCE * TIMES, CTAS = TIMES == 1 ? 4 : 2;   // CTAS: on an SM
     Eight z[TIMES];
     unsigned slow;
     PG_DEVINL int token(int u) const { return u * AT_ONCE + (threadIdx.x & 31) / LANE; }
-    PG_DEVINL void hold(const PutParams<T>& p, bool value, int64_t row, int h, int n, const Turns* turns) {
+    // FULL: n is HOLD, and nothing is asked for each token (with the questions, loads do not go ahead of one another: 10,900 rows of 8 heads in 141 us instead of 107)
+    template <bool FULL> PG_DEVINL void hold_as(const PutParams<T>& p, bool value, int64_t row, int h, int n, const Turns* turns) {
         using Q = typename Quad<T>::type;
         const int lane = threadIdx.x & 31, c = lane & (LANE - 1), D = p.pages.head_size;
         const EightAt at(c, value ? 0 : p.rope.pairs, value ? 0 : p.rope.layout);
@@ -432,7 +469,7 @@ template <typename T, int FORM, int LANE> struct PutEight {
 #pragma unroll
         for (int u = 0; u < TIMES; u++) {
             const int t = token(u);
-            if (t >= n || !mine) { a[u] = Q{}; b[u] = Q{}; continue; }
+            if ((!FULL && t >= n) || !mine) { a[u] = Q{}; b[u] = Q{}; continue; }
             a[u] = *reinterpret_cast<const Q*>(x + t * from.row + at.first);
             b[u] = *reinterpret_cast<const Q*>(x + t * from.row + at.second);
         }
@@ -443,6 +480,7 @@ template <typename T, int FORM, int LANE> struct PutEight {
         unsigned odd = 0;
 #pragma unroll
         for (int u = 0; u < TIMES; u++) {
+            if (!FULL && u * AT_ONCE >= n) break;
             Eight& y = z[u];
             open_quad(a[u], y.v[0], y.v[1], T());
             open_quad(b[u], y.v[2], y.v[3], T());
@@ -453,16 +491,20 @@ template <typename T, int FORM, int LANE> struct PutEight {
 #pragma unroll
                 for (int d = LANE >> 1; d; d >>= 1) sum += __shfl_xor_sync(~0u, sum, d);
                 const float mean = fmaf(sum, over_D, p.k_norm.eps);
-                if (t < n && !(mean > 0x1p-100f && mean < 0x1p100f)) odd |= 1u << t;
+                if ((FULL || t < n) && !(mean > 0x1p-100f && mean < 0x1p100f)) odd |= 1u << t;
                 scale8(y, rsqrtf(mean));
 #pragma unroll
                 for (int i = 0; i < 4; i++) y.v[i] = mul2(y.v[i], w.v[i]);
                 sum = squares8(y);
             }
-            if (t < n && !(sum < 0x1p120f)) odd |= 1u << t;   // (elements of this lane's pairs below 2^60, and none NaN)
+            if ((FULL || t < n) && !(sum < 0x1p120f)) odd |= 1u << t;   // (elements of this lane's pairs below 2^60, and none NaN)
             if (turn) turn8(y, turns[t], c, at.zipped);
         }
         slow = __reduce_or_sync(~0u, odd);
+    }
+    PG_DEVINL void hold(const PutParams<T>& p, bool value, int64_t row, int h, int n, const Turns* turns) {
+        if (n == HOLD) hold_as<true>(p, value, row, h, n, turns);
+        else hold_as<false>(p, value, row, h, n, turns);
     }
     PG_DEVINL static uint32_t size8(const Eight& y) {
         uint32_t a = 0;
@@ -487,7 +529,8 @@ template <typename T, int FORM, int LANE> struct PutEight {
             if (token(u) < n && __uint_as_float(size8(z[u])) >= near) with |= 1u << token(u);
         return with;
     }
-    PG_DEVINL unsigned close(const HeadSlots& slots, bool plain, int n, float by, uint8_t* codes, int64_t step) const {
+    template <bool FULL> PG_DEVINL unsigned close_as(const HeadSlots& slots, bool plain, int n, float scale, uint8_t* codes, int64_t step) const {
+        const float by = 1.0f / scale;
         const int c = threadIdx.x & (LANE - 1);
         const EightAt at(c, slots.pairs, slots.layout);
         if (8 * c >= slots.D) return 0;
@@ -495,16 +538,22 @@ template <typename T, int FORM, int LANE> struct PutEight {
 #pragma unroll
         for (int u = 0; u < TIMES; u++) {
             const int t = token(u);
-            if (t >= n) break;
+            if (!FULL && t >= n) break;
             const Eight& y = z[u];
             // (an element's pair is among the lane's eight: twice the largest of them bounds its size)
-            const float off = plain ? 0.0f : 2.0f * __uint_as_float(size8(y)) * PUT_OFF * by;
-            uint32_t word[2];
+            const float off = 2.0f * __uint_as_float(size8(y)) * PUT_OFF * by;
+            uint32_t n8[8];
             bool unsure = false;
-            if (FORM == FORM_INT8) {
+            if (plain) {
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    const float2 f = apart(y.v[i]);
+                    n8[2 * i] = settled_code<FORM>(f.x, scale, by);
+                    n8[2 * i + 1] = settled_code<FORM>(f.y, scale, by);
+                }
+            } else if (FORM == FORM_INT8) {
                 // y by + 1.5 2^23 has the nearest whole number in its lower bits; what is left tells how far the border is
                 const float limit = 0.5f - 127.0f * 0x1p-22f - off;
-                uint32_t n8[8];
 #pragma unroll
                 for (int i = 0; i < 4; i++) {
                     const uint64_t b2 = two(by, by), r = fma2(y.v[i], b2, two(12582912.0f, 12582912.0f));
@@ -513,52 +562,62 @@ template <typename T, int FORM, int LANE> struct PutEight {
                     n8[2 * i] = __float_as_uint(whole.x);
                     n8[2 * i + 1] = __float_as_uint(whole.y);
                 }
-#pragma unroll
-                for (int i = 0; i < 2; i++) word[i] = __byte_perm(__byte_perm(n8[4 * i], n8[4 * i + 1], 0x0040), __byte_perm(n8[4 * i + 2], n8[4 * i + 3], 0x0040), 0x5410);
             } else {
-                uint16_t half[4];
 #pragma unroll
-                for (int i = 0; i < 4; i++) {   // what lies `slack` below and above goes to the same code
+                for (int i = 0; i < 4; i++) {
                     const float2 r = apart(mul2(y.v[i], two(by, by)));
-                    const float sx = fmaf(fabsf(r.x), 0x1p-22f, off), sy = fmaf(fabsf(r.y), 0x1p-22f, off);
-                    uint16_t below, above;
-                    asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(below) : "f"(r.y - sy), "f"(r.x - sx));
-                    asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(above) : "f"(r.y + sy), "f"(r.x + sx));
-                    unsure = unsure || below != above;
-                    half[i] = below;
+                    n8[2 * i] = e4m3_code(r.x, off, unsure);
+                    n8[2 * i + 1] = e4m3_code(r.y, off, unsure);
                 }
-                word[0] = half[0] | (uint32_t)half[1] << 16;
-                word[1] = half[2] | (uint32_t)half[3] << 16;
             }
             if (unsure) again |= 1u << t;
+            uint32_t word[2];
+#pragma unroll
+            for (int i = 0; i < 2; i++) word[i] = __byte_perm(__byte_perm(n8[4 * i], n8[4 * i + 1], 0x0040), __byte_perm(n8[4 * i + 2], n8[4 * i + 3], 0x0040), 0x5410);
             *reinterpret_cast<uint32_t*>(codes + t * step + at.first) = word[0];
             *reinterpret_cast<uint32_t*>(codes + t * step + at.second) = word[1];
         }
         return again;
     }
+    PG_DEVINL unsigned close(const HeadSlots& slots, bool plain, int n, float scale, uint8_t* codes, int64_t step) const {
+        return n == HOLD ? close_as<true>(slots, plain, n, scale, codes, step) : close_as<false>(slots, plain, n, scale, codes, step);
+    }
 };
 template <typename T, int FORM, int SLOTS> PG_DEVINL unsigned slow_tokens(const PutOne<T, FORM, SLOTS>& x) { return x.z.slow; }
-template <typename T, int FORM, int LANE> PG_DEVINL unsigned slow_tokens(const PutEight<T, FORM, LANE>& x) { return x.slow; }
+template <typename T, int FORM, int LANE, int TIMES> PG_DEVINL unsigned slow_tokens(const PutEight<T, FORM, LANE, TIMES>& x) { return x.slow; }
+
+// the queries of a call, by warps w, w + step, ... of all
+template <typename T, int LANES> PG_DEVINL void put_queries(const PutParams<T>& p, int64_t w, int64_t step, Turns& turns) {
+    const int each = (p.q_heads + p.parts - 1) / p.parts;
+    for (; w < p.batch.n_rows * p.parts; w += step) {
+        const int64_t r = w / p.parts;
+        const int from = (int)(w - r * p.parts) * each, b = seq_of_row_warp(p.batch, r);
+        if (b < 0) continue;
+        const Span s = span_of(p.batch, b);
+        if (p.rope.pairs) row_turns(p.rope, p.pos, r, (int)(p.batch.prefix_len + (int64_t)s.len - s.count + (r - s.first)), turns);
+        norm_row<T, LANES>(p.rope.pairs, p.rope.layout, p.q_norm, p.pages.head_size, p.q.data + r * p.q.row, p.q.head, p.q_out.data + r * p.q_out.row, p.q_out.head, from, min(p.q_heads, from + each), turns);
+    }
+}
+// By themselves, launched before paged8_append_kernel, which may start while this runs and needs nothing of it: half the warps that fit an SM, so that the other kernel's arithmetic has room beside these copies
+constexpr int QUERY_CTAS = ROW_CTAS / 2;
+template <typename T, int LANES>
+__global__ void __launch_bounds__(32 * ROW_WARPS, ROW_CTAS) put_queries_kernel(const __grid_constant__ PutParams<T> p) {
+    __shared__ alignas(16) Turns turns[ROW_WARPS];
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    put_queries<T, LANES>(p, (int64_t)blockIdx.x * ROW_WARPS + (threadIdx.x >> 5), (int64_t)gridDim.x * ROW_WARPS, turns[threadIdx.x >> 5]);
+}
 
 template <typename T, int FORM, typename Put>
-__global__ void __launch_bounds__(32 * PUT_WARPS, 2) paged8_append_kernel(const __grid_constant__ PutParams<T> p) {
+__global__ void __launch_bounds__(32 * PUT_WARPS, Put::CTAS) paged8_append_kernel(const __grid_constant__ PutParams<T> p) {
     __shared__ alignas(16) Turns turns[PUT_TOKENS];
     constexpr int HOLD = Put::HOLD;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, D = p.pages.head_size;
-    // CTAs of both kinds take turns, so that an SM has the one's arithmetic beside the other's copies
+    const bool last_cta = blockIdx.x == gridDim.x - 1;   // (ends after put_queries_kernel, where there is one, so that whoever waits for this kernel waits for both)
+    // CTAs of both kinds take turns
     const int put = (int)((int64_t)blockIdx.x * p.put_ctas / p.ctas);
     if ((int)((int64_t)(blockIdx.x + 1) * p.put_ctas / p.ctas) == put) {   // the queries
-        const int q_ctas = p.ctas - p.put_ctas;
-        Turns& mine = turns[warp];
-        const int each = (p.q_heads + p.parts - 1) / p.parts;
-        for (int64_t w = (int64_t)(blockIdx.x - put) * PUT_WARPS + warp; w < p.batch.n_rows * p.parts; w += (int64_t)q_ctas * PUT_WARPS) {
-            const int64_t r = w / p.parts;
-            const int from = (int)(w - r * p.parts) * each, b = seq_of_row_warp(p.batch, r);
-            if (b < 0) continue;
-            const Span s = span_of(p.batch, b);
-            if (p.rope.pairs) row_turns(p.rope, p.pos, r, (int)(p.batch.prefix_len + (int64_t)s.len - s.count + (r - s.first)), mine);
-            norm_row<T, Put::LANES>(p.rope.pairs, p.rope.layout, p.q_norm, D, p.q.data + r * p.q.row, p.q.head, p.q_out.data + r * p.q_out.row, p.q_out.head, from, min(p.q_heads, from + each), mine);
-        }
+        put_queries<T, Put::LANES>(p, (int64_t)(blockIdx.x - put) * PUT_WARPS + warp, (int64_t)(p.ctas - p.put_ctas) * PUT_WARPS, turns[warp]);
+        if (last_cta) asm volatile("griddepcontrol.wait;" ::: "memory");
         return;
     }
     const lmrs_b200_rope_t* rope = &p.rope;   // (lanes read different entries: ordinary loads, as in row_turns)
@@ -666,7 +725,7 @@ __global__ void __launch_bounds__(32 * PUT_WARPS, 2) paged8_append_kernel(const 
                 const int64_t step = value ? p.pages.v_slot : p.pages.k_slot;
                 // (at the largest scale elements may lie beyond the largest code, and with one that is NaN they all are: both go by 64 bits)
                 const unsigned all = (1u << n) - 1;
-                const unsigned again = scale < SCALE_MOST ? __reduce_or_sync(~0u, z.close(at, plain, n, 1.0f / scale, c, step)) | slow_tokens(z) : all;
+                const unsigned again = scale < SCALE_MOST ? __reduce_or_sync(~0u, z.close(at, plain, n, scale, c, step)) | slow_tokens(z) : all;
                 __syncwarp();   // (the lanes that write a head again are others)
                 for (unsigned left = again; left; left &= left - 1) {
                     const int t = __ffs(left) - 1;
@@ -695,6 +754,7 @@ __global__ void __launch_bounds__(32 * PUT_WARPS, 2) paged8_append_kernel(const 
         }
         if (p.rope.pairs) __syncthreads();   // (the angles are used by all until here)
     }
+    if (last_cta) asm volatile("griddepcontrol.wait;" ::: "memory");
 }
 
 // ---- reading back ----------------------------------------------------------------------------------------------------------------------------

@@ -293,6 +293,27 @@ def test_ties_go_to_even(paged, form):
         assert torch.equal(t.cpu()[0].float().double(), oracle.nearest(x.double(), form))
 
 
+@pytest.mark.parametrize("dtype", [BF16, F16], ids=str)
+@pytest.mark.parametrize("how", ["packed", "odd"])
+@pytest.mark.parametrize("form", [INT8, E4M3], ids=str)
+def test_inputs_next_to_the_middle_of_two_codes(paged, form, how, dtype):
+    """all 8 bits of mantissa of elements against all of the largest: quotients that only the scale's rounding keeps from the middle"""
+    x = torch.zeros(128, 1, 256)
+    x[:, 0, :128] = torch.arange(128, 256)
+    x[:, 0, 128:255] = torch.arange(129, 256) / 64.0
+    x[:, 0, 255] = 256 + 2 * torch.arange(128)   # the largest of each token
+    x[1::2] *= -0.37109375   # (another 8 bits' worth of scales: rounded to the type)
+    x = x.to(dtype)
+    k = torch.zeros(8, 16, 1, 256).to(form).cuda()
+    pages = paged.QuantPages(k, k.clone(), torch.zeros(8, 16, 1, device="cuda"), torch.zeros(8, 16, 1, device="cuda"))
+    batch = paged.Batch(torch.tensor([128], dtype=torch.int32).cuda(), torch.arange(8, dtype=torch.int32).cuda()[None], rows=torch.tensor([0, 128], dtype=torch.int32).cuda(), max_rows=128)
+    paged.append(pages, batch, laid_out(x, how), laid_out(-x, how))
+    for t, s, sign in ((pages.k, pages.k_scale, 1.0), (pages.v, pages.v_scale, -1.0)):
+        scale = s.cpu().double().view(128, 1, 1)
+        assert ((scale[:, 0, 0] - x.double().abs().amax((1, 2)) / oracle.MOST[form]).abs() <= scale[:, 0, 0] * 2.0 ** -24).all()
+        assert torch.equal(t.cpu().float().double().view(128, 1, 256), oracle.nearest(sign * x.double() / scale, form))
+
+
 @pytest.mark.parametrize("dtype", [BF16, F32], ids=str)
 @pytest.mark.parametrize("form", [INT8, E4M3], ids=str)
 def test_what_is_not_finite_and_what_is_far_from_one(paged, form, dtype):
