@@ -213,10 +213,11 @@ __global__ void __launch_bounds__(32 * ROW_WARPS) norm_rope_kernel(const __grid_
 //
 // A code is the nearest one of the value that the formulas give, and a scale their largest value's, to within some 2^-45 of a border: in 32 bits alone one of ten thousand codes would be its neighbour, by 1/127 of
 // the block's largest value.  But 64 bits are needed where 32 cannot tell only.  With u = 2^-24, an element after its norm is off by 14 u of itself (squares: 13 u of their sum,
-// mean 2 u, halved by the root; the root's approximation 4 u; two products), after its rotation by 19 u (|a| + |b|) of its pair (cosines 3 u, two products and a sum), which is 27 u of the turned pair's sizes; PUT_OFF is 32 u.  An element so near to a border between two codes is computed again in
+// mean 2 u, halved by the root; the root's approximation 4 u; two products), after its rotation by 19 u (|a| + |b|) of its pair (cosines 3 u, two products and a sum), which is 27 u of the turned pair's sizes, and by 5 u (7 u) without a norm; PUT_OFF is 32 u, PUT_OFF_TURN
+// 10 u.  An element so near to a border between two codes is computed again in
 // 64 bits (head64; one head of eight has one), and so are the tokens whose largest element is within 2^-17 of the block's largest.  Inputs that 32 bits would overflow on go that way altogether.
 constexpr int PUT_WARPS = 8, PUT_TOKENS = 16;   // warps of a CTA, tokens whose angles it holds at a time
-constexpr float PUT_OFF = 0x1p-19f;
+constexpr float PUT_OFF = 0x1p-19f, PUT_OFF_TURN = 10.0f * 0x1p-24f;
 
 template <typename T> struct PutParams {
     lmrs_b200_rope_t rope;   // pairs 0: nothing turns
@@ -230,14 +231,38 @@ template <typename T> struct PutParams {
     int window, windows, heads, head_ctas, put_ctas, ctas;   // CTAs that quantise: a window of rows (whose leaders they take) and `heads` heads each; the others take the queries
 };
 
-// cosine and sine of position * turns / 2^64 turns, in 64 bits
+// Cosine and sine of position * turns / 2^64 turns, in 64 bits: quarter turns off, then the Taylor series on an eighth of a turn either way (their next terms are 2^-63 and 2^-66 there)
 PG_DEVINL double2 cos_sin64(int position, uint64_t turns) {
     const int64_t t = (int64_t)((uint64_t)(int64_t)position * turns);
     const int64_t quarter = (t >> 62) + ((t >> 61) & 1);
-    double s0, c0;
-    sincospi((double)(t - (int64_t)((uint64_t)quarter << 62)) * 0x1p-63, &s0, &c0);
+    const double x = (double)(t - (int64_t)((uint64_t)quarter << 62)) * (3.14159265358979323846 * 0x1p-63), y = x * x;
+    double s0 = 1.0 / 355687428096000.0, c0 = -1.0 / 6402373705728000.0;   // 1 / 17!, -1 / 18!
+    s0 = fma(y, s0, -1.0 / 1307674368000.0);  c0 = fma(y, c0, 1.0 / 20922789888000.0);
+    s0 = fma(y, s0, 1.0 / 6227020800.0);      c0 = fma(y, c0, -1.0 / 87178291200.0);
+    s0 = fma(y, s0, -1.0 / 39916800.0);       c0 = fma(y, c0, 1.0 / 479001600.0);
+    s0 = fma(y, s0, 1.0 / 362880.0);          c0 = fma(y, c0, -1.0 / 3628800.0);
+    s0 = fma(y, s0, -1.0 / 5040.0);           c0 = fma(y, c0, 1.0 / 40320.0);
+    s0 = fma(y, s0, 1.0 / 120.0);             c0 = fma(y, c0, -1.0 / 720.0);
+    s0 = fma(y, s0, -1.0 / 6.0);              c0 = fma(y, c0, 1.0 / 24.0);
+    s0 = fma(y * s0, x, x);                   c0 = fma(y, fma(y, c0, -0.5), 1.0);
     const double a = quarter & 1 ? s0 : c0, b = quarter & 1 ? c0 : s0;
     return make_double2((quarter + 1) & 2 ? -a : a, quarter & 2 ? -b : b);
+}
+// 1 / x and 1 / sqrt(x) by Newton's steps, off by some 2^-52 (x within float32's range; others by the functions)
+PG_DEVINL double over64(double x) {
+    const float f = (float)x;
+    if (!(fabsf(f) > 0x1p-100f && fabsf(f) < 0x1p100f)) return 1.0 / x;
+    double r = (double)(1.0f / f);
+    r = fma(fma(-x, r, 1.0), r, r);
+    return fma(fma(-x, r, 1.0), r, r);
+}
+PG_DEVINL double over_sqrt64(double x) {
+    const float f = (float)x;
+    if (!(f > 0x1p-100f && f < 0x1p100f)) return 1.0 / sqrt(x);
+    double r = (double)rsqrtf(f);
+    r = fma(fma(-x * r, r, 1.0), 0.5 * r, r);
+    r = fma(fma(-x * r, r, 1.0), 0.5 * r, r);
+    return fma(fma(-x * r, r, 1.0), 0.5 * r, r);
 }
 
 template <typename T> PG_DEVINL int put_position(const PutParams<T>& p, int64_t row, int index, int j) {
@@ -259,7 +284,7 @@ static __device__ __noinline__ void head64(const PutParams<T>& p, int64_t row, i
     }
     if (p.k_norm.on) {
         for (int d = 16; d; d >>= 1) sum += __shfl_xor_sync(~0u, sum, d);
-        const double by = 1.0 / sqrt(sum / at.D + (double)p.k_norm.eps);
+        const double by = over_sqrt64(fma(sum, over64(at.D), (double)p.k_norm.eps));
         const float* w = p.k_norm.weight + h * p.k_norm.head;
 #pragma unroll
         for (int i = 0; i < 4; i++) {
@@ -412,7 +437,7 @@ template <typename T, int FORM, int SLOTS> struct PutOne {
         return with;
     }
     // stores the codes; returns the tokens that have unsure ones
-    PG_DEVINL unsigned close(const HeadSlots& at, bool plain, int n, float scale, uint8_t* c, int64_t step) const {
+    PG_DEVINL unsigned close(const HeadSlots& at, bool plain, float off_by, int n, float scale, uint8_t* c, int64_t step) const {
         const float by = 1.0f / scale;
         const int lane = threadIdx.x & 31;
         unsigned again = 0;
@@ -423,7 +448,7 @@ template <typename T, int FORM, int SLOTS> struct PutOne {
             for (int i = 0; i < SLOTS; i++) {
                 const int sl = lane + 32 * i;
                 if (sl >= at.count()) continue;
-                const float off = plain ? 0.0f : (fabsf(z.y[t][i][0]) + fabsf(z.y[t][i][1])) * PUT_OFF;
+                const float off = plain ? 0.0f : (fabsf(z.y[t][i][0]) + fabsf(z.y[t][i][1])) * off_by;
                 bool unsure[2];
                 uint32_t code[2] = {quick_code<FORM>(z.y[t][i][0], by, off, unsure[0]), quick_code<FORM>(z.y[t][i][1], by, off, unsure[1])};
                 if (plain) {
@@ -529,7 +554,7 @@ template <typename T, int FORM, int LANE, int TIMES_> struct PutEight {
             if (token(u) < n && __uint_as_float(size8(z[u])) >= near) with |= 1u << token(u);
         return with;
     }
-    template <bool FULL> PG_DEVINL unsigned close_as(const HeadSlots& slots, bool plain, int n, float scale, uint8_t* codes, int64_t step) const {
+    template <bool FULL> PG_DEVINL unsigned close_as(const HeadSlots& slots, bool plain, float off_by, int n, float scale, uint8_t* codes, int64_t step) const {
         const float by = 1.0f / scale;
         const int c = threadIdx.x & (LANE - 1);
         const EightAt at(c, slots.pairs, slots.layout);
@@ -540,8 +565,11 @@ template <typename T, int FORM, int LANE, int TIMES_> struct PutEight {
             const int t = token(u);
             if (!FULL && t >= n) break;
             const Eight& y = z[u];
-            // (an element's pair is among the lane's eight: twice the largest of them bounds its size)
-            const float off = 2.0f * __uint_as_float(size8(y)) * PUT_OFF * by;
+            // sizes of pairs: (first + i, second + i), or neighbours
+            const float2 f0 = apart(y.v[0]), f1 = apart(y.v[1]), f2 = apart(y.v[2]), f3 = apart(y.v[3]);
+            const float each = off_by * by;
+            const float off[4] = {each * (at.zipped ? fabsf(f0.x) + fabsf(f0.y) : fabsf(f0.x) + fabsf(f2.x)), each * (at.zipped ? fabsf(f1.x) + fabsf(f1.y) : fabsf(f0.y) + fabsf(f2.y)),
+                                  each * (at.zipped ? fabsf(f2.x) + fabsf(f2.y) : fabsf(f1.x) + fabsf(f3.x)), each * (at.zipped ? fabsf(f3.x) + fabsf(f3.y) : fabsf(f1.y) + fabsf(f3.y))};
             uint32_t n8[8];
             bool unsure = false;
             if (plain) {
@@ -553,7 +581,7 @@ template <typename T, int FORM, int LANE, int TIMES_> struct PutEight {
                 }
             } else if (FORM == FORM_INT8) {
                 // y by + 1.5 2^23 has the nearest whole number in its lower bits; what is left tells how far the border is
-                const float limit = 0.5f - 127.0f * 0x1p-22f - off;
+                const float limit = 0.5f - 127.0f * 0x1p-22f - fmaxf(fmaxf(off[0], off[1]), fmaxf(off[2], off[3]));
 #pragma unroll
                 for (int i = 0; i < 4; i++) {
                     const uint64_t b2 = two(by, by), r = fma2(y.v[i], b2, two(12582912.0f, 12582912.0f));
@@ -566,8 +594,8 @@ template <typename T, int FORM, int LANE, int TIMES_> struct PutEight {
 #pragma unroll
                 for (int i = 0; i < 4; i++) {
                     const float2 r = apart(mul2(y.v[i], two(by, by)));
-                    n8[2 * i] = e4m3_code(r.x, off, unsure);
-                    n8[2 * i + 1] = e4m3_code(r.y, off, unsure);
+                    n8[2 * i] = e4m3_code(r.x, at.zipped ? off[i] : off[2 * (i & 1)], unsure);
+                    n8[2 * i + 1] = e4m3_code(r.y, at.zipped ? off[i] : off[2 * (i & 1) + 1], unsure);
                 }
             }
             if (unsure) again |= 1u << t;
@@ -579,8 +607,8 @@ template <typename T, int FORM, int LANE, int TIMES_> struct PutEight {
         }
         return again;
     }
-    PG_DEVINL unsigned close(const HeadSlots& slots, bool plain, int n, float scale, uint8_t* codes, int64_t step) const {
-        return n == HOLD ? close_as<true>(slots, plain, n, scale, codes, step) : close_as<false>(slots, plain, n, scale, codes, step);
+    PG_DEVINL unsigned close(const HeadSlots& slots, bool plain, float off_by, int n, float scale, uint8_t* codes, int64_t step) const {
+        return n == HOLD ? close_as<true>(slots, plain, off_by, n, scale, codes, step) : close_as<false>(slots, plain, off_by, n, scale, codes, step);
     }
 };
 template <typename T, int FORM, int SLOTS> PG_DEVINL unsigned slow_tokens(const PutOne<T, FORM, SLOTS>& x) { return x.z.slow; }
@@ -708,7 +736,7 @@ __global__ void __launch_bounds__(32 * PUT_WARPS, Put::CTAS) paged8_append_kerne
                             const float x = open_code<FORM>(c[e]);
                             bool unsure;   // (x old is off by u of itself)
                             uint32_t code = quick_code<FORM>(x * old, by, fabsf(x * old) * 0x1p-23f, unsure);
-                            if (unsure) code = close_code<FORM>((double)x * old, scale, 1.0 / (double)scale);
+                            if (unsure) code = close_code<FORM>((double)x * old, scale, over64((double)scale));
                             c[e] = (uint8_t)code;
                         }
                 }
@@ -725,7 +753,7 @@ __global__ void __launch_bounds__(32 * PUT_WARPS, Put::CTAS) paged8_append_kerne
                 const int64_t step = value ? p.pages.v_slot : p.pages.k_slot;
                 // (at the largest scale elements may lie beyond the largest code, and with one that is NaN they all are: both go by 64 bits)
                 const unsigned all = (1u << n) - 1;
-                const unsigned again = scale < SCALE_MOST ? __reduce_or_sync(~0u, z.close(at, plain, n, scale, c, step)) | slow_tokens(z) : all;
+                const unsigned again = scale < SCALE_MOST ? __reduce_or_sync(~0u, z.close(at, plain, p.k_norm.on ? PUT_OFF : PUT_OFF_TURN, n, scale, c, step)) | slow_tokens(z) : all;
                 __syncwarp();   // (the lanes that write a head again are others)
                 for (unsigned left = again; left; left &= left - 1) {
                     const int t = __ffs(left) - 1;
@@ -746,8 +774,8 @@ __global__ void __launch_bounds__(32 * PUT_WARPS, Put::CTAS) paged8_append_kerne
                     for (int i = 0; i < 4; i++) {
                         const int sl = lane + 32 * i;
                         if (sl >= at.count()) continue;
-                        c[t * step + at.first(sl)] = close_code<FORM>(y[i][0], scale, 1.0 / (double)scale);
-                        if (at.second(sl) < D) c[t * step + at.second(sl)] = close_code<FORM>(y[i][1], scale, 1.0 / (double)scale);
+                        c[t * step + at.first(sl)] = close_code<FORM>(y[i][0], scale, over64((double)scale));
+                        if (at.second(sl) < D) c[t * step + at.second(sl)] = close_code<FORM>(y[i][1], scale, over64((double)scale));
                     }
                 }
             }
