@@ -34,11 +34,19 @@ struct Cutting8 {
     bool own_tensor, front_tensor;
     size_t bytes;
 };
-// Which kernel takes what: float32 rows8_kernel; 16-bit types by how often the keys would be read again (as in paged.cu)
+// Which kernel takes what.  float32: rows8_kernel.  16-bit types: by how often the keys would be read, and converted, again, as in paged.cu: rows8_kernel does so for every 16 rows of a KV head (8 where no unit has more),
+// codes128_kernel for every 128 or 256, and starts some 10 us later.  Measured on a B200 with rows8_kernel / codes128_kernel, us a call, 8 KV heads, int8, a scale for 16 tokens:
+//   a sequence's own keys, 16 sequences behind up to 4000 keys, rows of the longest sequence and a KV head:
+//     head 64:  32: 41 / 81   64: 64 / 89   128: 106 / 94      128:  32: 68 / 104   64: 120 / 115   128: 206 / 126      256:  16: 80 / 140   32: 120 / 141   64: 220 / 158
+//     (one sequence alone, 64 rows: 22 / 27 at head 64, 32 / 31 at 128, 50 / 43 at 256)
+//   the prefix, rows of all sequences and a KV head behind a prefix of 512, 2048, 8192, 32768 keys:
+//     head 64:   16: 14 / 18, 14 / 25, 23 / 33, 35 / 62    32: 14 / 19, 16 / 26, 27 / 34, 55 / 64    64: 21 / 23, 23 / 27, 38 / 34, 91 / 65     128: 28 / 31, 33 / 36, 61 / 43, 172 / 74
+//     head 128:  16: 16 / 20, 17 / 28, 29 / 37, 53 / 74    32: 17 / 24, 25 / 29, 36 / 38, 90 / 76    64: 27 / 29, 34 / 34, 58 / 43, 166 / 80    128: 37 / 41, 53 / 53, 106 / 61, 322 / 100
+//     head 256:   8: 14 / 22, 18 / 33, 31 / 45, 71 / 101   16: 18 / 23, 26 / 33, 44 / 46, 129 / 116  32: 27 / 27, 34 / 36, 72 / 48, 238 / 118   128: 58 / 51, 97 / 67, 260 / 81, 906 / 155
 struct Which8 { bool own_tensor, front_tensor; int row_tiles; };   // row_tiles: rows of a unit of rows8_kernel, in eights
 template <int DP> struct TensorRule8 {
-    static constexpr int OWN_ROWS = DP <= 128 ? 64 : 16, FRONT_ROWS = DP <= 128 ? 17 : 9;
-    static constexpr int64_t FRONT_WORK = DP <= 128 ? 1 << 21 : 1 << 20;
+    static constexpr int OWN_ROWS = DP <= 64 ? 128 : DP <= 128 ? 64 : 48, FRONT_ROWS = DP <= 64 ? 33 : DP <= 128 ? 17 : 9;
+    static constexpr int64_t FRONT_WORK = DP <= 64 ? 1 << 22 : DP <= 128 ? 1 << 21 : 1 << 20;
 };
 template <int DP> Which8 which8(const lmrs_b200_pages8_t* pages, const lmrs_b200_batch_t* batch, int dtype, int64_t n_rows, int q_heads) {
     using R = TensorRule8<DP>;

@@ -351,12 +351,9 @@ def append(pages, batch, k, v, rope=None, pos=None, q=None, q_out=None, k_norm=N
         if k_norm is not None or q_norm is not None:
             if q_norm is not None and q is None:
                 raise LmrsError("q_norm without q")
-            norms = _Norms(eps=eps)
-            if k_norm is not None:
-                norms.k, norms.k_head = _weight(k_norm, "k_norm", pages.kv_heads, size, device)
-            if q_norm is not None:
-                norms.q, norms.q_head = _weight(q_norm, "q_norm", q.shape[1] if isinstance(q, torch.Tensor) and q.dim() == 3 else 0, size, device)
-            norms = _byref(norms)
+            wk, wk_head = (None, 0) if k_norm is None else _weight(k_norm, "k_norm", pages.kv_heads, size, device)
+            wq, wq_head = (None, 0) if q_norm is None else _weight(q_norm, "q_norm", q.shape[1] if isinstance(q, torch.Tensor) and q.dim() == 3 else 0, size, device)
+            norms = _byref(_Norms(wk, wq, wk_head, wq_head, eps))
     elif k_norm is not None or q_norm is not None:
         raise LmrsError("k_norm and q_norm go with QuantPages: call norm_rope before")
     kr = _heads(k, "k", device, dtype, n, pages.kv_heads, size)
@@ -415,10 +412,13 @@ def read(pages, batch, rows=None, dtype=torch.bfloat16, k=None, v=None):
         if dtype not in _DTYPES:
             raise LmrsError(f"dtype must be bfloat16, float16 or float32, not {dtype}")
         k, v = torch.empty(shape, dtype=dtype, device=device), torch.empty(shape, dtype=dtype, device=device)
+        kr, vr = _Rows(k.data_ptr(), shape[1] * shape[2], shape[2]), _Rows(v.data_ptr(), shape[1] * shape[2], shape[2])
     elif not isinstance(k, torch.Tensor) or k.dtype not in _DTYPES:
         raise LmrsError("k must be a tensor of bfloat16, float16 or float32")
-    kr, vr = _heads(k, "k", device, k.dtype, *shape, out=True), _heads(v, "v", device, k.dtype, *shape, out=True)
-    rc = lib().lmrs_b200_paged8_read(pages._ref, batch._ref, _DTYPES[k.dtype], n, _byref(kr), _byref(vr), _stream(device.index))
+    else:
+        dtype = k.dtype
+        kr, vr = _heads(k, "k", device, dtype, *shape, out=True), _heads(v, "v", device, dtype, *shape, out=True)
+    rc = lib().lmrs_b200_paged8_read(pages._ref, batch._ref, _DTYPES[dtype], n, _byref(kr), _byref(vr), _stream(device.index))
     if rc:
         check(rc)
     return k, v

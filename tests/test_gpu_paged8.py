@@ -402,7 +402,7 @@ def test_attention_of_several_rows(paged, case, form, dtype):
 
 LARGE = [  # (many rows against the same keys: tensor-core products) tokens held, rows of the call or None, page, block, kv heads, group, size, prefix
     ([40] * 29 + [0, 7], None, 16, 16, 2, 8, 128, 4500), ([200, 130], [200, 65], 32, 8, 2, 2, 64, 700), ([300], [257], 48, 12, 1, 2, 112, 0), ([90, 70, 5], [80, 64, 5], 7, 7, 1, 1, 128, 133),
-    ([10] * 9, None, 8, 8, 4, 4, 256, 3700), ([64, 129], [64, 128], 1, 1, 1, 4, 64, 65), ([150, 260], [33, 140], 64, 64, 2, 3, 208, 515), ([130] * 3, [70] * 3, 128, 128, 1, 5, 128, 1000),
+    ([10] * 9, None, 8, 8, 4, 4, 256, 3700), ([10] * 9, None, 8, 8, 4, 8, 256, 4000), ([3] * 40, None, 16, 4, 4, 4, 64, 6700), ([64, 129], [64, 128], 1, 1, 1, 4, 64, 65), ([150, 260], [33, 140], 64, 64, 2, 3, 208, 515), ([130] * 3, [70] * 3, 128, 128, 1, 5, 128, 1000),
 ]
 
 
