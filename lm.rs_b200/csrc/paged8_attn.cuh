@@ -71,6 +71,11 @@ PG_DEVINL float2 value_terms(float v) {
     return make_float2(v == v ? lg : v, by);
 }
 
+// What bounds it: where the keys are many, the bytes of the pages, and close behind them issue slots (a warp spends some 800 instructions on 32 keys of 128 in int8, a third of them on making float16 of
+// codes); where they are few, the chain length - table - codes - scores - join.  Measured (B200): four sequences of up to 100,000 keys (520 MB of codes, 32/8 heads of 128, float16 rows, int8, a scale for each
+// token) 112 us, 4620 GB/s, and 105 with a scale for 32 tokens; one sequence of 1000 keys, heads of 64: 10.8 us with the join; float32 rows, 15 sequences behind a prefix of 4096, heads of 64: 28 us.
+// Steps, us for the first: tiles of 128 keys copied by all threads 16 bytes at a time 184; a warp its own keys by TMA 167; 8 rows as the products' columns (16 as their rows before) 136; boxes that ask the L2 for
+// no more than their own 128 bytes of each 1024 (of 256 before: the heads' codes lie side by side) 112.
 // CTA = 4 warps that share a tile's keys: a warp copies its own WARP_KEYS of them to its own slots, a tile or two ahead, and works on them by itself; the warps meet only where parts begin and end.  Codes
 // come by TMA, a piece of a page at a time, where all of a warp's keys are within the unit's (else, and where strides or pages take no tensor map, 16 bytes a lane, zeros for what is not there); scales 4 bytes a lane.
 template <typename T, int DP, int ROW_TILES> struct TileShape8 {
@@ -173,7 +178,7 @@ template <typename T, int FORM, int DP, int ROW_TILES> struct WarpTile8 {
     }
     // there: bit j: key j of the warp's is there; first: number of its first key; scales: of the warp's keys and values in shared memory; by: room for the values' reciprocals
     PG_DEVINL void tile(const Attn8Params<T>& p, uint32_t q_at, uint32_t k_at, uint32_t v_at, uint32_t there, int first, float* scales, float* by) {
-        const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+        const int lane = threadIdx.x & 31, g = lane >> 2;
         float *ks = scales, *vs = scales + S::WARP_KEYS;
         float s[S::KEY_TILES][ROW_TILES][4] = {};   // keys 16j + g of rows 2t and 2t + 1, then keys 16j + g + 8
         if (lane < S::WARP_KEYS) {   // (in their places)

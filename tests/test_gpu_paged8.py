@@ -448,6 +448,35 @@ def test_attention_with_missing_pages(paged, dtype):
             assert (out[row] == 0).all() and (lse[row] == -math.inf).all()
 
 
+@pytest.mark.parametrize("dtype", [BF16, F32], ids=str)
+def test_attention_beyond_the_table_and_a_wrong_max_rows(paged, dtype):
+    """a length that the table does not reach: what it does reach counts.  max_rows chooses kernels, and nothing else"""
+    m = Made(paged, 4, dtype, INT8, [40, 70, 200], [1, 1, 1], 16, 8, 1, 2, 64, 20, one_each=True)
+    pages, batch = m.on_gpu()
+    m.tables = m.tables[:, :3]
+    short = paged.Batch(batch.lens, m.tables.cuda(), prefix=batch.prefix, prefix_len=20)   # 48 tokens at most
+    m.check(*paged.attention(pages, short, m.q.cuda(), return_lse=True))
+    batch.lens.copy_(torch.tensor([2 ** 31 - 1, -2 ** 31, 0], dtype=torch.int32))
+    out, lse = paged.attention(pages, short, m.q.cuda(), return_lse=True)
+    assert (out[1:] == 0).all() and (lse[1:] == -math.inf).all()   # (the first row sees all that the table has, scales of blocks that hold nothing among it)
+    empty = paged.Batch(batch.lens, m.tables[:, :0].cuda(), prefix=batch.prefix, prefix_len=20)
+    batch.lens.fill_(5)
+    m.lens, m.tables = [5, 5, 5], m.tables[:, :0]
+    m.check(*paged.attention(pages, empty, m.q.cuda(), return_lse=True))
+    m = Made(paged, 5, dtype, E4M3, [300, 90], [150, 70], 16, 8, 1, 2, 64, 90)
+    pages, batch = m.on_gpu()
+    for most in (1, 7, 10 ** 6):
+        batch = paged.Batch(batch.lens, batch.tables, rows=batch.rows, max_rows=most, prefix=batch.prefix, prefix_len=90)
+        m.check(*paged.attention(pages, batch, m.q.cuda(), return_lse=True))
+        x = torch.randn(m.n, 1, 64, generator=gen(most)).to(dtype).cuda()
+        paged.append(pages, batch, x, x)
+        k, v = paged.read(pages, batch, rows=m.n, dtype=dtype)
+        step = x.float().abs().amax() / 16   # (half a step of e4m3, and what the block's older scale makes of it)
+        assert ((k.float() - x.float()).abs() <= step + 448 * 2.0 ** -4 * pages.k_scale[~torch.isnan(pages.k_scale)].max()).all() and torch.isfinite(v).all()
+        m = Made(paged, 5, dtype, E4M3, [300, 90], [150, 70], 16, 8, 1, 2, 64, 90)
+        pages = m.on_gpu()[0]
+
+
 @pytest.mark.parametrize("dtype", [BF16, F16, F32], ids=str)
 @pytest.mark.parametrize("form", [INT8, E4M3], ids=str)
 def test_scales_that_are_not_finite(paged, form, dtype):
