@@ -190,7 +190,7 @@ void lmrs_b200_weights_free(lmrs_b200_weights_t* w);
  * Keys and values of any number of sequences in pages of one pool, rows of a call appended to them with their rotary positions (one axis or
  * several: time, height, width of image and video rows) applied on the way, and attention over them in which a prefix that all sequences share is
  * read and computed once for all.  DEVICE pointers, on the caller's stream (a cudaStream_t; NULL: the legacy default stream) and the current
- * device; nothing is allocated (but for one word of host memory in a process' first call of paged_attention with many rows), kept or synchronised, so calls on several streams, and calls captured into CUDA graphs, do not meet anywhere but in the
+ * device; nothing is allocated (but for one word of host memory in a process' first call of paged_attention with many rows or of paged8_attention), kept or synchronised, so calls on several streams, and calls captured into CUDA graphs, do not meet anywhere but in the
  * caller's own arrays.  dtype: 0 bfloat16, 1 float32, 2 float16, the same for all arrays of a call; angles, scores, softmax and sums are 32-bit or
  * wider.  Strides count elements; the elements of a head lie next to each other.
  *
@@ -290,8 +290,9 @@ int lmrs_b200_paged8_append(const lmrs_b200_pages8_t* pages, const lmrs_b200_bat
 /* What the places of the batch's rows hold, k and v [n_rows][kv_heads][head_size]: code * scale in float32, rounded to the type.  Padding rows and rows whose page is none: 0.  Rows from rows[seqs] on
  * are not touched.  (A batch whose rows are all that its sequences hold, rows[b + 1] - rows[b] = lens[b], reads them whole; prefix pages are read as those of a sequence.) */
 int lmrs_b200_paged8_read(const lmrs_b200_pages8_t* pages, const lmrs_b200_batch_t* batch, int dtype, int64_t n_rows, const lmrs_b200_rows_t* k, const lmrs_b200_rows_t* v, void* stream);
-/* paged_attention over 8-bit pages; dtype is that of q and out.  head_size: a multiple of 16, at most 256; codes and their strides on 16-byte boundaries.  Scales of values count as the nearest number between 2^-60 and 2^60.  The rest as
- * there. */
+/* paged_attention over 8-bit pages; dtype is that of q and out.  head_size: a multiple of 16, at most 256; codes and their strides on 16-byte boundaries.  Scales of values count as the nearest number between 2^-60 and 2^60.  16-bit
+ * types: the softmax' weights, times the values' scales, are rounded to float16 (by 2^-11 of each at most, and 2^-32 of the largest) before the product with the codes, their sum is not.  A scale that is NaN reaches the rows that
+ * see it and no others; e4m3's two codes of NaN, which nothing here writes, may reach other rows of the same portion.  The rest as there. */
 int lmrs_b200_paged8_attention_workspace(const lmrs_b200_pages8_t* pages, const lmrs_b200_batch_t* batch, int dtype, int64_t n_rows, int q_heads, size_t* bytes);
 int lmrs_b200_paged8_attention(const lmrs_b200_pages8_t* pages, const lmrs_b200_batch_t* batch, int dtype, int64_t n_rows, const lmrs_b200_rows_t* q, const lmrs_b200_rows_t* out,
                                int q_heads, float scale, float softcap, float* lse, void* workspace, size_t workspace_bytes, void* stream);

@@ -428,7 +428,8 @@ def attention(pages, batch, q, out=None, scale=None, softcap=0.0, return_lse=Fal
     """softmax(scale * q . keys) . values for q [rows, heads, head_size]: every row over the prefix and over its own sequence up to its own place.
     heads: a multiple of kv_heads, neighbours share one.  scale None: head_size ** -0.5.  softcap > 0: scores s become softcap * tanh(s / softcap).  A row
     that sees nothing is 0.  return_lse: also the logarithms of the sums of exponentials, float32 [rows, heads] (-inf for a row that sees nothing).
-    out may not overlap q.  16-bit types: the softmax' weights are rounded to the type before the product with the values, their sum is not.  QuantPages: q is of any type, and head_size a multiple of 16."""
+    out may not overlap q.  16-bit types: the softmax' weights are rounded to the type before the product with the values, their sum is not.  QuantPages: q is of any type, head_size a
+    multiple of 16, and 16-bit types round the weights to float16."""
     if not isinstance(batch, Batch):
         raise LmrsError("batch must be a Batch")
     if not isinstance(q, torch.Tensor) or q.dim() != 3:
