@@ -13,7 +13,7 @@ The same with the pool in 8 bits, which takes half the room and half the time to
     pages = QuantPages(k, v, k_scale, v_scale)          # int8 or float8_e4m3fn, a float32 scale for each block of tokens and head
     q     = append(pages, batch, k_new, v_new, rope=rope, q=q, k_norm=wk, q_norm=wq)
     out   = attention(pages, batch, q)
-    k, v  = read(pages, batch)                          # what the places of the batch's rows hold
+    k, v  = read(pages, batch, rows=n)                  # what the places of the batch's n rows hold
     x     = norm_rope(x, weight, pos, rope)             # the norm and the rotation by themselves
 """
 import ctypes as C
@@ -392,13 +392,20 @@ def append(pages, batch, k, v, rope=None, pos=None, q=None, q_out=None, k_norm=N
 
 def read(pages, batch, rows=None, dtype=torch.bfloat16, k=None, v=None):
     """What the places of the batch's rows in QuantPages hold: keys and values [rows, kv_heads, head_size] of the dtype (or of k and v, which are written then), code * scale rounded to it.  rows: how many rows
-    the batch has (None: one each).  Rows without a place (padding, entries of a table that are no pages) are 0; rows behind the last sequence are not touched.  A batch whose rows are all that its
+    the batch has, which lies on the GPU and is not asked for it (None: those of k and v, or one each; a batch that was given `rows` needs the one or the other).  Rows without a place (padding, entries of a table that are no pages) are 0; rows behind the last sequence are not touched.  A batch whose rows are all that its
     sequences hold reads them whole."""
     if not isinstance(batch, Batch):
         raise LmrsError("batch must be a Batch")
     if not isinstance(pages, QuantPages):
         raise LmrsError("pages must be QuantPages")
-    n = batch.seqs if rows is None else int(rows)
+    if rows is not None:
+        n = int(rows)
+    elif isinstance(k, torch.Tensor) and k.dim():
+        n = k.shape[0]
+    elif batch.rows is None:
+        n = batch.seqs
+    else:
+        raise LmrsError("rows: how many the batch has (its last entry of rows), since it has more or fewer than one a sequence")
     if not 0 <= n < 1 << 31:
         raise LmrsError("rows must be 0 .. 2^31 - 1")
     if (k is None) != (v is None):

@@ -334,6 +334,22 @@ def test_what_is_not_finite_and_what_is_far_from_one(paged, form, dtype):
         assert scale[1, 0].max() == 2.0 ** 60 and (got[4].abs() <= most * 2.0 ** 60).all() and torch.equal(got[5, 0], torch.full((64,), most * 2.0 ** 60, dtype=torch.float64))
 
 
+def test_reading_rows_that_are_not_counted(paged):
+    """the rows of k and v, or one a sequence; a batch with rows of its own is refused, since fewer of them would be other tokens"""
+    m = Made(paged, 7, BF16, INT8, [10, 40, 33], [4, 1, 9], 16, 4, 2, 1, 64)
+    pages, batch = m.on_gpu()
+    with pytest.raises(paged.LmrsError, match="rows"):
+        paged.read(pages, batch)
+    want = paged.read(pages, batch, rows=m.n)
+    k, v = (torch.full((m.n + 2, 2, 64), 5.0, dtype=BF16, device="cuda") for _ in range(2))
+    paged.read(pages, batch, k=k, v=v)
+    for got, w in ((k, want[0]), (v, want[1])):
+        assert torch.equal(got[:m.n], w) and (got[m.n:] == 5.0).all()
+    last = paged.read(pages, paged.Batch(batch.lens, batch.tables))
+    for got, w in zip(last, want):
+        assert torch.equal(got, w[[3, 4, 13]])
+
+
 def test_entries_that_are_no_pages_and_lengths_beyond_the_table(paged):
     m = Made(paged, 3, BF16, INT8, [40, 20, 64], [9, 20, 64], 16, 4, 2, 1, 64, bad=[(0, 2, -1), (1, 0, 2 ** 31 - 1), (2, 1, 1000), (2, 3, -2 ** 31)], empty=True)
     pages, batch = m.on_gpu()

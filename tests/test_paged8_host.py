@@ -123,3 +123,25 @@ def test_host_tensors_and_other_arguments_are_refused(paged):
                 lambda: paged.read(None, None), lambda: paged.norm_rope(x, rope=paged.RopeAxes([1.0])), lambda: paged.norm_rope(x, pos=x), lambda: paged.norm_rope(x, rope=3, pos=x)):
         with pytest.raises(paged.LmrsError):
             bad()
+
+
+def test_reading_without_the_number_of_rows(paged, monkeypatch):
+    """a batch with rows of its own does not say here how many they are: fewer would be other tokens"""
+    monkeypatch.setattr(paged, "_gpu", lambda t, name, device: None)
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: None)
+    asked = []
+    monkeypatch.setattr(paged, "lib", lambda: type("Lib", (), {"lmrs_b200_paged8_read": staticmethod(lambda pages, batch, dtype, n, k, v, stream: asked.append(n) or 0)}))
+    monkeypatch.setattr(paged, "_stream", lambda index: None)
+    monkeypatch.setattr(paged, "_heads", lambda t, name, device, dtype, *shape, out=False: paged._Rows(t.data_ptr(), *t.stride()[:2]) if t.shape == shape else paged._need(False, name))
+    ints = dict(dtype=torch.int32)
+    codes, scales = torch.zeros(3, 16, 2, 64, dtype=torch.int8), torch.zeros(3, 4, 2)
+    pages, lens, tables = paged.QuantPages(codes, codes, scales, scales), torch.tensor([10, 20], **ints), torch.zeros(2, 2, **ints)
+    each, several = paged.Batch(lens, tables), paged.Batch(lens, tables, rows=torch.tensor([0, 4, 9], **ints), max_rows=5)
+    with pytest.raises(paged.LmrsError, match="rows"):
+        paged.read(pages, several)
+    assert not asked
+    k, v = (torch.zeros(9, 2, 64) for _ in range(2))
+    assert paged.read(pages, each)[0].shape == (2, 2, 64) and paged.read(pages, several, rows=9)[0].shape == (9, 2, 64) and paged.read(pages, several, k=k, v=v)[0] is k
+    assert asked == [2, 9, 9]
+    with pytest.raises(paged.LmrsError):
+        paged.read(pages, several, rows=8, k=k, v=v)
