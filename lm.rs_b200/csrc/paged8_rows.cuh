@@ -30,11 +30,13 @@ struct Eight { uint64_t v[4]; };
 struct EightAt {
     int first, second;
     bool zipped;   // a pair is neighbours (layout 1); else it is first + i and second + i
+    bool turns;    // or the elements pass
     PG_DEVINL EightAt(int c, int pairs, int layout) {
         const bool halves = layout == 0 && 4 * c < pairs;
         first = halves ? 4 * c : 8 * c;
         second = halves ? first + pairs : first + 4;
         zipped = layout != 0;
+        turns = 4 * c < pairs;
     }
 };
 template <typename T> struct Quad;   // four elements in memory
@@ -61,6 +63,7 @@ PG_DEVINL void load_weights8(const float* w, const EightAt& at, Eight& to) {
     const ulonglong2 a = *reinterpret_cast<const ulonglong2*>(w + at.first), b = *reinterpret_cast<const ulonglong2*>(w + at.second);
     to.v[0] = a.x; to.v[1] = a.y; to.v[2] = b.x; to.v[3] = b.y;
 }
+// (of a lane that does not turn: times a cosine of 1 and a sine of 0, by which an infinity makes NaN of the element beside it)
 PG_DEVINL void turn8(Eight& x, const Turns& t, int c, bool zipped) {
     const ulonglong2 cs = *reinterpret_cast<const ulonglong2*>(t.c + 4 * c), sn = *reinterpret_cast<const ulonglong2*>(t.s + 4 * c);
     const uint64_t minus = 0x8000000080000000ull;
@@ -102,7 +105,6 @@ PG_DEVINL void norm_row8(int pairs, int layout, const HeadNorm& norm, int D, con
     const int lane = threadIdx.x & 31, c = lane & (LANES - 1);
     const EightAt at(c, pairs, layout);
     const bool mine = 8 * c < D;
-    const bool turns_here = pairs > 0;
     constexpr int AHEAD = NORM_AHEAD<T>;
     const float over_D = 1.0f / (float)D;
     Eight w;
@@ -137,7 +139,7 @@ PG_DEVINL void norm_row8(int pairs, int layout, const HeadNorm& norm, int D, con
 #pragma unroll
                 for (int i = 0; i < 4; i++) y.v[i] = mul2(y.v[i], w.v[i]);
             }
-            if (turns_here) turn8(y, turns, c, at.zipped);
+            if (at.turns) turn8(y, turns, c, at.zipped);
             T* p = out + h * out_head;
             *reinterpret_cast<Q*>(p + at.first) = close_quad(y.v[0], y.v[1], T());
             *reinterpret_cast<Q*>(p + at.second) = close_quad(y.v[2], y.v[3], T());
@@ -527,7 +529,7 @@ template <typename T, int FORM, int LANE, int TIMES_> struct PutEight {
                 sum = squares8(y);
             }
             if ((FULL || t < n) && !(sum < 0x1p120f)) odd |= 1u << t;   // (elements of this lane's pairs below 2^60, and none NaN)
-            if (turn) turn8(y, turns[t], c, at.zipped);
+            if (turn) turn8(y, turns[t], c, at.zipped);   // (lanes that do not turn as well: what is not finite makes its block's scale NaN in any case)
         }
         slow = __reduce_or_sync(~0u, odd);
     }

@@ -94,6 +94,34 @@ def test_norm_rope_of_nothing_and_of_what_is_not_finite(paged):
     assert torch.isfinite(got[~bad]).all() and torch.isnan(got[bad]).any(-1).all()
 
 
+@pytest.mark.parametrize("dtype", [BF16, F16, F32], ids=str)
+@pytest.mark.parametrize("layout", ["halves", "pairs"])
+def test_elements_that_do_not_turn_pass_unchanged(paged, layout, dtype):
+    """an infinity, a NaN or a zero's sign behind the pairs that turn: the elements beside it know nothing of it, wherever the rows lie"""
+    n, heads, size, rot = 12, 3, 64, 16
+    x = torch.randn(n, heads, size, generator=gen(1)).to(dtype)
+    for r, e in enumerate((16, 19, 23, 40, 63)):
+        x[r, 0, e], x[r + 5, 1, e] = math.inf, math.nan
+    x[10:] = -0.0
+    pos = torch.arange(5, 5 + n, dtype=torch.int32, device="cuda")
+    rope = paged.RopeAxes.sections(rot, 10000.0, layout=layout)
+    codes, scales = torch.zeros(n, 8, 1, size, dtype=INT8, device="cuda"), torch.ones(n, 1, 1, device="cuda")
+    pages = paged.QuantPages(codes, codes.clone(), scales, scales.clone())
+    batch = paged.Batch(torch.ones(n, dtype=torch.int32, device="cuda"), torch.arange(n, dtype=torch.int32, device="cuda")[:, None])
+    k = torch.ones(n, 1, size, dtype=dtype, device="cuda")
+    normed = []
+    for how in ("packed", "gaps", "odd"):
+        q = paged.append(pages, batch, k, k, rope=rope, pos=pos, q=laid_out(x, how)).cpu()
+        assert torch.equal(torch.isnan(q), torch.isnan(x)) and torch.equal(torch.isinf(q), torch.isinf(x))
+        bits = torch.int32 if dtype == F32 else torch.int16
+        assert torch.equal(torch.where(torch.isnan(x), 0, q.view(bits))[..., rot:], torch.where(torch.isnan(x), 0, x.view(bits))[..., rot:])
+        normed.append(paged.norm_rope(laid_out(x, how), None, pos, rope).cpu())
+        spoilt = torch.zeros(n, heads, size, dtype=torch.bool)
+        spoilt[torch.isinf(x)] = True                    # (an infinite element over an infinite root; the others of its head over it are 0)
+        spoilt[torch.isnan(x).any(-1)] = True            # (a NaN is in the root of the whole head)
+        assert torch.equal(torch.isnan(normed[-1]), spoilt)
+
+
 # ---- a batch: sequences of given lengths in a pool whose unused places hold NaN ------------------------------------------------------------------
 class Made:
     def __init__(self, paged, seed, dtype, form, lens, counts, page, block, kv_heads, group, size, prefix=0, one_each=False, order="pshd", tail=0, bad=(), empty=False):
