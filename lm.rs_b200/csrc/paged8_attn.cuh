@@ -409,50 +409,52 @@ __global__ void __launch_bounds__(TileShape8<T, DP, ROW_TILES>::THREADS, TileSha
     // boxes of a lane: keys or values, rows, columns
     constexpr int COL_BOXES = DP / S::BOX;
     const int box_rows = boxes.rows, groups = box_rows ? S::WARP_KEYS / box_rows : 0, box = lane % max(1, 2 * COL_BOXES * groups), box_value = box & 1, box_col = (box >> 1) % COL_BOXES, box_group = (box >> 1) / COL_BOXES;
-    auto copy_tile = [&]() {   // the warp's part of the tile that `ahead` stands at, whose places are known; then on to the next one
+    auto copy_tile = [&]() {   // the warp's part of the tile that `ahead` stands at, whose places are known; then on to the next one.  A warp that gave up copies nothing, but walks on: all warps go by the units that warp 0 writes down
         if (copied < n_tiles) {
-            const bool is = page >= 0 && page < p.batch.pages;
-            const uint32_t to_codes = smem_at(slots) + slot_to * S::SLOT, bits = __ballot_sync(~0u, is) & (S::WARP_KEYS == 32 ? ~0u : (1u << S::WARP_KEYS % 32) - 1);
+            if (ok) {
+                const bool is = page >= 0 && page < p.batch.pages;
+                const uint32_t to_codes = smem_at(slots) + slot_to * S::SLOT, bits = __ballot_sync(~0u, is) & (S::WARP_KEYS == 32 ? ~0u : (1u << S::WARP_KEYS % 32) - 1);
 #pragma unroll
-            for (int i = 0; i < S::STAGES; i++)
-                if (i == slot_to) there[i] = bits;
-            const int page_or_0 = is ? page : 0, at = is ? at_page : 0;
-            if (box_rows && ahead.tile * S::KEYS + (warp + 1) * S::WARP_KEYS <= ahead.keys) {
-                if (written >> slot_to & 1) asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-                __syncwarp();
-                if (lane == 0) mbar_expect_tx(&full[warp][slot_to], S::SLOT);
-                int of = __shfl_sync(~0u, is ? page : -1, box_group * box_rows & 31), from_row = __shfl_sync(~0u, at, box_group * box_rows & 31);
-                if (of < 0) { of = p.batch.pages; from_row = 0; }   // (outside the map: zeros)
-                __syncwarp();
-                if (lane < 2 * COL_BOXES * groups)
-                    tma_box(to_codes + box_value * S::KV + box_col * (S::WARP_KEYS * S::BOX) + box_group * box_rows * S::BOX, box_value ? &boxes.v : &boxes.k, S::BOX * box_col, from_row, ahead.head, of,
-                            box_value ? boxes.v_place : boxes.k_place, box_value ? boxes.v_head : boxes.k_head, &full[warp][slot_to]);
-                __syncwarp();
-                by_tma |= 1u << slot_to;
-                written &= ~(1u << slot_to);
-            } else {
-                by_tma &= ~(1u << slot_to);
-                written |= 1u << slot_to;
-                const int64_t k_from = is ? page_or_0 * p.c.k_page + at * p.c.k_slot + ahead.head * p.c.k_head : -1, v_from = is ? page_or_0 * p.c.v_page + at * p.c.v_slot + ahead.head * p.c.v_head : -1;
-                constexpr int LANES = S::CHUNKS < 8 ? S::CHUNKS : 8, AT_ONCE = 32 / LANES;   // lanes a row, rows at a time
+                for (int i = 0; i < S::STAGES; i++)
+                    if (i == slot_to) there[i] = bits;
+                const int page_or_0 = is ? page : 0, at = is ? at_page : 0;
+                if (box_rows && ahead.tile * S::KEYS + (warp + 1) * S::WARP_KEYS <= ahead.keys) {
+                    if (written >> slot_to & 1) asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                    __syncwarp();
+                    if (lane == 0) mbar_expect_tx(&full[warp][slot_to], S::SLOT);
+                    int of = __shfl_sync(~0u, is ? page : -1, box_group * box_rows & 31), from_row = __shfl_sync(~0u, at, box_group * box_rows & 31);
+                    if (of < 0) { of = p.batch.pages; from_row = 0; }   // (outside the map: zeros)
+                    __syncwarp();
+                    if (lane < 2 * COL_BOXES * groups)
+                        tma_box(to_codes + box_value * S::KV + box_col * (S::WARP_KEYS * S::BOX) + box_group * box_rows * S::BOX, box_value ? &boxes.v : &boxes.k, S::BOX * box_col, from_row, ahead.head, of,
+                                box_value ? boxes.v_place : boxes.k_place, box_value ? boxes.v_head : boxes.k_head, &full[warp][slot_to]);
+                    __syncwarp();
+                    by_tma |= 1u << slot_to;
+                    written &= ~(1u << slot_to);
+                } else {
+                    by_tma &= ~(1u << slot_to);
+                    written |= 1u << slot_to;
+                    const int64_t k_from = is ? page_or_0 * p.c.k_page + at * p.c.k_slot + ahead.head * p.c.k_head : -1, v_from = is ? page_or_0 * p.c.v_page + at * p.c.v_slot + ahead.head * p.c.v_head : -1;
+                    constexpr int LANES = S::CHUNKS < 8 ? S::CHUNKS : 8, AT_ONCE = 32 / LANES;   // lanes a row, rows at a time
 #pragma unroll 2
-                for (int r0 = 0; r0 < S::WARP_KEYS; r0 += AT_ONCE) {
-                    const int row = r0 + lane / LANES;
-                    const int64_t k = __shfl_sync(~0u, k_from, row), v = __shfl_sync(~0u, v_from, row);
+                    for (int r0 = 0; r0 < S::WARP_KEYS; r0 += AT_ONCE) {
+                        const int row = r0 + lane / LANES;
+                        const int64_t k = __shfl_sync(~0u, k_from, row), v = __shfl_sync(~0u, v_from, row);
 #pragma unroll
-                    for (int c = 0; c < S::CHUNKS; c += LANES) {
-                        const int piece = c + lane % LANES;
-                        const bool in = k >= 0 && piece < whole;
-                        copy16(to_codes + code_at<S>(row, piece), in ? p.c.k + k + 16 * piece : p.c.k, in);
-                        copy16(to_codes + S::KV + code_at<S>(row, piece), in ? p.c.v + v + 16 * piece : p.c.v, in);
+                        for (int c = 0; c < S::CHUNKS; c += LANES) {
+                            const int piece = c + lane % LANES;
+                            const bool in = k >= 0 && piece < whole;
+                            copy16(to_codes + code_at<S>(row, piece), in ? p.c.k + k + 16 * piece : p.c.k, in);
+                            copy16(to_codes + S::KV + code_at<S>(row, piece), in ? p.c.v + v + 16 * piece : p.c.v, in);
+                        }
                     }
                 }
-            }
-            if (lane < S::WARP_KEYS) {
-                const int block = p.block_shift >= 0 ? at >> p.block_shift : at / p.c.block;
-                const uint32_t to_scale = smem_at(scales + slot_to * S::SCALES) + 4 * lane;
-                copy4(to_scale, p.c.ks + page_or_0 * p.c.ks_page + block * p.c.ks_block + ahead.head * p.c.ks_head, is);
-                copy4(to_scale + 4 * S::WARP_KEYS, p.c.vs + page_or_0 * p.c.vs_page + block * p.c.vs_block + ahead.head * p.c.vs_head, is);
+                if (lane < S::WARP_KEYS) {
+                    const int block = p.block_shift >= 0 ? at >> p.block_shift : at / p.c.block;
+                    const uint32_t to_scale = smem_at(scales + slot_to * S::SCALES) + 4 * lane;
+                    copy4(to_scale, p.c.ks + page_or_0 * p.c.ks_page + block * p.c.ks_block + ahead.head * p.c.ks_head, is);
+                    copy4(to_scale + 4 * S::WARP_KEYS, p.c.vs + page_or_0 * p.c.vs_page + block * p.c.vs_block + ahead.head * p.c.vs_head, is);
+                }
             }
             if (first) {
                 if (lane == 0) walks[warp][set_to] = ahead;
@@ -497,7 +499,7 @@ __global__ void __launch_bounds__(TileShape8<T, DP, ROW_TILES>::THREADS, TileSha
             copy_wait<S::STAGES - 2>();   // (of the scales, and what does not come by TMA)
         }
         __syncwarp();
-        if (ok) copy_tile();          // (into the slot of the tile before, which this warp has worked on)
+        copy_tile();                  // (into the slot of the tile before, which this warp has worked on)
         if (ok && (by_tma >> slot & 1)) {
             ok = __all_sync(~0u, dense::mbar_wait_bounded(&full[warp][slot], rounds >> slot & 1, gave_up, TG_ROWS8 + dense::TG_FULL));
             if (ok) {
