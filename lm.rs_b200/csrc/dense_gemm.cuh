@@ -38,15 +38,15 @@ constexpr size_t TG_SMEM = 1024 + (size_t)TG_STAGES * TG_STAGE_BYTES + 256;
 constexpr uint32_t TG_WAIT_NS = 2000000000u;   // how long a wait may take ...
 constexpr uint32_t TG_LEAST_TRIES = 4096;      // ... after it has looked this often (a context that was switched out for a while may not have)
 // what a wait was for, in the status word: kernel * 256 + barrier
-enum { TG_ONE_CTA = 1 << 8, TG_PAIR = 2 << 8, TG_ATTENTION = 3 << 8, TG_F32 = 4 << 8, TG_PAGED = 5 << 8,
+enum { TG_ONE_CTA = 1 << 8, TG_PAIR = 2 << 8, TG_ATTENTION = 3 << 8, TG_F32 = 4 << 8, TG_PAGED = 5 << 8, TG_ROWS8 = 6 << 8, TG_CODES128 = 7 << 8,
        TG_FREE = 1, TG_FULL, TG_SUMS, TG_SUMS_READ, TG_ROWS_FREE, TG_ROWS_FULL, TG_SPLIT_FREE, TG_SPLIT_FULL, TG_QUERIES, TG_SCORES, TG_WEIGHTS, TG_VALUES, TG_VALUES_READ,
        TG_QUERIES_READ, TG_PLACES, TG_PART };
 inline std::string tg_gave_up(int status) {
-    static const char* kernels[] = {"a tensor-core kernel", "gemm_bf16_tc_kernel", "gemm_bf16_pair_kernel", "attn_tensor_kernel", "gemm_split_kernel", "rows128_kernel"};
+    static const char* kernels[] = {"a tensor-core kernel", "gemm_bf16_tc_kernel", "gemm_bf16_pair_kernel", "attn_tensor_kernel", "gemm_split_kernel", "rows128_kernel", "rows8_kernel", "codes128_kernel"};
     static const char* waits[] = {"one of its barriers", "a free stage", "a stage's copies", "the sums", "its sums to be read", "a free stage of rows", "a stage of rows",
                                   "room for split weights", "split weights", "the split queries", "scores", "softmax weights", "weighted values", "weighted values to be read", "its queries to be read", "the places of a tile's keys", "the other rows of a part"};
     const int k = status >> 8, w = status & 255;
-    return std::string(k >= 1 && k <= 5 ? kernels[k] : kernels[0]) + " gave up waiting for " + (w >= 1 && w <= 16 ? waits[w] : waits[0]) + " (device status " + std::to_string(status) + ")";
+    return std::string(k >= 1 && k <= 7 ? kernels[k] : kernels[0]) + " gave up waiting for " + (w >= 1 && w <= 16 ? waits[w] : waits[0]) + " (device status " + std::to_string(status) + ")";
 }
 
 struct TcGemmParams {

@@ -163,10 +163,7 @@ extern "C" int lmrs_b200_paged8_attention(const lmrs_b200_pages8_t* pages, const
         if (why.empty()) why = bad_pages8_memory(pages, device);
         if (why.empty() && (!workspace || !aligned(workspace, 256) || !on_device(workspace, device))) why = "workspace is not memory of the current device on a 256-byte boundary";
         if (!why.empty()) return refuse(me, why);
-        if (const int status = gave_up_word.take()) {
-            const int kernel = status & ~255;
-            return refuse(me, "results of an earlier call are NaN: " + (kernel == TG_ROWS8 || kernel == TG_CODES128 ? (kernel == TG_ROWS8 ? "rows8_kernel: " : "codes128_kernel: ") : std::string()) + dense::tg_gave_up(status));
-        }
+        if (const int status = gave_up_word.take()) return refuse(me, "results of an earlier call are NaN: " + dense::tg_gave_up(status));
         return by_shape8(pages, batch, dtype, n_rows, q_heads, [&](auto t, auto form, auto d, auto tiles, const Which8& which) {
             using T = decltype(t);
             constexpr int FORM = decltype(form)::value, DP = decltype(d)::value, ROW_TILES = decltype(tiles)::value;

@@ -61,7 +61,6 @@ PG_DEVINL float2 row_factor(float most) {
     return make_float2(__uint_as_float((uint32_t)e << 23), __uint_as_float((uint32_t)(254 - e) << 23));
 }
 constexpr float SHIFT8 = 7.0f;   // m is so much less than the largest exponent when it is set
-constexpr int TG_ROWS8 = 6 << 8;   // (a kernel that gave up: after those of dense_gemm.cuh)
 // the exponent and the reciprocal of a scale of values (a scale that is NaN leaves a finite reciprocal: it reaches whoever has the weight)
 PG_DEVINL float2 value_terms(float v) {
     const float c = fminf(fmaxf(v, SCALE_LEAST), SCALE_MOST);
@@ -501,7 +500,7 @@ __global__ void __launch_bounds__(TileShape8<T, DP, ROW_TILES>::THREADS, TileSha
         __syncwarp();
         copy_tile();                  // (into the slot of the tile before, which this warp has worked on)
         if (ok && (by_tma >> slot & 1)) {
-            ok = __all_sync(~0u, dense::mbar_wait_bounded(&full[warp][slot], rounds >> slot & 1, gave_up, TG_ROWS8 + dense::TG_FULL));
+            ok = __all_sync(~0u, dense::mbar_wait_bounded(&full[warp][slot], rounds >> slot & 1, gave_up, dense::TG_ROWS8 + dense::TG_FULL));
             if (ok) {
                 rounds ^= 1u << slot;
                 by_tma &= ~(1u << slot);

@@ -19,8 +19,6 @@
 namespace lmrs {
 namespace paged {
 
-constexpr int TG_CODES128 = 7 << 8;   // (a kernel that gave up: after TG_ROWS8)
-
 template <int DP> struct TensorShape8 {
     static constexpr int THREADS = 384, BLOCK = 128, BLOCKS = DP <= 128 ? 2 : 1, ROWS = BLOCK * BLOCKS, KEYS = 64;
     // copying warps: for heads of up to 128 one for the keys and one for the values, all 64 of a tile; beyond that (one block of rows, so that warps 4-7 are free) four for both, 16 keys each
@@ -286,7 +284,7 @@ __global__ void __launch_bounds__(TensorShape8<DP>::THREADS, 1) codes128_kernel(
                 const bool values = S::SPLIT ? takes_values : !(k_done < part_has && k_done - v_done < 2);
                 const int at = base + (values ? (v_done + 1 < part_has ? 2 * v_done + 2 : 2 * part_has - 1) : k_done ? 2 * k_done - 1 : 0), slot = at % S::SLOTS;   // the operand's number in the ring
                 if (by_tma >> from_slot & 1) {
-                    ok = __all_sync(~0u, dense::mbar_wait_bounded(&staged[from_slot], rounds >> from_slot & 1, gave_up, TG_CODES128 + dense::TG_FULL));
+                    ok = __all_sync(~0u, dense::mbar_wait_bounded(&staged[from_slot], rounds >> from_slot & 1, gave_up, dense::TG_CODES128 + dense::TG_FULL));
                     if (!ok) break;
                     rounds ^= 1u << from_slot;
                     by_tma &= ~(1u << from_slot);
@@ -317,7 +315,7 @@ __global__ void __launch_bounds__(TensorShape8<DP>::THREADS, 1) codes128_kernel(
                     if (lane == 0) arrive(&sh.known[set]);
                     all++;
                 }
-                ok = wait_warp(&sh.empty[slot], at / S::SLOTS + 1, gave_up, TG_CODES128 + dense::TG_FREE - dense::TG_PAGED);
+                ok = wait_warp(&sh.empty[slot], at / S::SLOTS + 1, gave_up, dense::TG_CODES128 + dense::TG_FREE - dense::TG_PAGED);
                 if (!ok) break;
                 constexpr int BATCH = 4;
 #pragma unroll 1
@@ -361,7 +359,7 @@ __global__ void __launch_bounds__(TensorShape8<DP>::THREADS, 1) codes128_kernel(
                     if (by_tma >> i & 1) dense::mbar_wait_for(&staged[i], rounds >> i & 1, nullptr);
         } else if (warp == S::PRODUCTS) {
             // ---- products ----
-            constexpr int WHO = TG_CODES128 - dense::TG_PAGED;
+            constexpr int WHO = dense::TG_CODES128 - dense::TG_PAGED;
             const uint32_t one = dense::elect_one();
             const uint32_t form = (1u << 4) | ((uint32_t)(S::BLOCK >> 4) << 24);   // f32 += f16 x f16, 128 rows
             const uint32_t score_form = form | ((uint32_t)(S::KEYS >> 3) << 17), sum_form = form | (1u << 16) | ((uint32_t)(D >> 3) << 17);   // (values are MN-major)
@@ -433,7 +431,7 @@ __global__ void __launch_bounds__(TensorShape8<DP>::THREADS, 1) codes128_kernel(
         __syncwarp();
     } else {
         // ---- rows ----
-        constexpr int WHO = TG_CODES128 - dense::TG_PAGED;
+        constexpr int WHO = dense::TG_CODES128 - dense::TG_PAGED;
         const int group = warp >> 2, row = threadIdx.x & 127;
         const uint32_t lanes = (uint32_t)(warp & 3) << 21;   // this warp's 32 TMEM lanes
         int s_count[2] = {0, 0}, k_count = 0, part = 0;   // phases of earlier parts: this group's even and odd tiles, all tiles, parts

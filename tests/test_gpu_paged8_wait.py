@@ -39,4 +39,5 @@ def test_a_wait_that_runs_out(program, case, waits):
         kernel = {ROWS8: "rows8_kernel", CODES128: "codes128_kernel"}[what & ~255]
         assert int(wrong) == 0 and 0 < int(nan) < int(rows), (case, what, nan, wrong)
         assert said == "1" and "results of an earlier call are NaN: " + kernel in words and words.endswith(f" gave up waiting for {WAITS[what & 255]} (device status {what})")
+        assert f"NaN: {kernel} gave up" in words   # (paged_attention, which reads the same word, says it in the same words)
         assert after == "0" and same == "1"   # (said once)
