@@ -258,8 +258,8 @@ int lmrs_b200_paged_attention_workspace(const lmrs_b200_pages_t* pages, const lm
 int lmrs_b200_paged_attention(const lmrs_b200_pages_t* pages, const lmrs_b200_batch_t* batch, int64_t n_rows, const lmrs_b200_rows_t* q, const lmrs_b200_rows_t* out,
                               int q_heads, float scale, float softcap, float* lse, void* workspace, size_t workspace_bytes, void* stream);
 
-/* out = x / sqrt(mean of a head's x^2 + eps) * weight (NULL: none; head h's at weight + h * weight_head), then turned by its rows' positions (rope and pos NULL: not turned); float32 inside, rounded once.
- * weight: f32.  The rest as in rope_axes. */
+/* out = x / sqrt(mean of a head's x^2 + eps) * weight (NULL: none; head h's at weight + h * weight_head), then turned by its rows' positions (rope and pos NULL: not turned); float32 inside, rounded once
+ * (elements from 2^60 on: the sum of their squares may be beyond float32, and the head 0; below 2^-60, with no eps to speak of, squares lose bits and vanish).  weight: f32.  The rest as in rope_axes. */
 int lmrs_b200_norm_rope(const lmrs_b200_rope_t* rope, int dtype, const lmrs_b200_rows_t* x, const lmrs_b200_rows_t* out, int64_t n_rows, int heads, int head_size, const float* weight,
                         int64_t weight_head, float eps, const lmrs_b200_positions_t* pos, void* stream);
 
@@ -279,7 +279,7 @@ typedef struct lmrs_b200_norms {
     int64_t k_head, q_head;
     float eps;
 } lmrs_b200_norms_t;
-/* paged_append to 8-bit pages: k normed and turned, v as it is, both quantised; with q (goes with rope or its norm), q_out = q normed and turned.  norms NULL: none.
+/* paged_append to 8-bit pages: k normed and turned, v as it is, both quantised; with q (goes with rope or its norm), q_out = q normed and turned as by norm_rope.  norms NULL: none.
  * A block of slots that the call begins gets the scale a / Q, a the largest size of its new elements and Q 127 or 448, between 2^-60 and 2^60; where it held tokens of the sequence before, the larger of
  * that and the scale that it had, and the codes that it held become the nearest ones of the same values under the new scale.  A code is the nearest one of element / scale, ties to even (what
  * k's norm and rotation give is kept in 64 bits until then), elements beyond the largest code's that one.  An element that is not finite makes its block's scale NaN: all of the block reads as NaN.  Two rows with one

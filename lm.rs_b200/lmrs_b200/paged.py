@@ -300,7 +300,7 @@ def rope_axes(x, pos, rope, out=None):
 
 def norm_rope(x, weight=None, pos=None, rope=None, eps=1e-6, out=None):
     """x [rows, heads, head_size], every head divided by the root of its mean square (plus eps) and multiplied by weight, float32 [head_size] or [heads, head_size] (None: 1), then turned by pos as in
-    rope_axes (rope None: not turned); out may be x, and not lie over a part of it."""
+    rope_axes (rope None: not turned); out may be x, and not lie over a part of it.  Squares and their sum are float32: elements are to be below 2^60, and from 2^-60 on where eps is 0."""
     if not isinstance(x, torch.Tensor) or x.dim() != 3 or x.dtype not in _DTYPES:
         raise LmrsError("x must be a [rows, heads, head_size] tensor of bfloat16, float16 or float32")
     if rope is not None and not isinstance(rope, RopeAxes):

@@ -94,6 +94,35 @@ def test_norm_rope_of_nothing_and_of_what_is_not_finite(paged):
     assert torch.isfinite(got[~bad]).all() and torch.isnan(got[bad]).any(-1).all()
 
 
+@pytest.mark.parametrize("dtype", [BF16, F32], ids=str)
+@pytest.mark.parametrize("size", [16, 64, 96, 200, 256, 33])
+def test_norms_of_heads_far_from_one(paged, size, dtype):
+    """squares up to the ends of float32 (elements of 2^59, or 2^-60 with no eps beside them), heads of all sizes in a row; without an eps and with one"""
+    n, heads = 7, 9
+    g = gen(size)
+    x = torch.randn(n, heads, size, generator=g)
+    for r, f in enumerate((57, 40, 20, -20, -40, -57)):
+        x[r, ::2 + r % 2] *= 2.0 ** f
+    x[2, 1, 1:], x[3, 1, :-1] = 0.0, 0.0   # (one element only)
+    x = x.to(dtype)
+    weight = torch.randn(heads, size, generator=g)
+    pos = torch.randint(0, 200, (1, n), generator=g).to(torch.int32)
+    rot = size // 8 * 4
+    rope = paged.RopeAxes.sections(rot, 10000.0)
+    freq = [10000.0 ** (-2.0 * j / rot) for j in range(rot // 2)]
+    codes, scales = torch.zeros(n, 8, 1, size, dtype=INT8, device="cuda"), torch.ones(n, 1, 1, device="cuda")
+    pages = paged.QuantPages(codes, codes.clone(), scales, scales.clone())
+    batch = paged.Batch(torch.ones(n, dtype=torch.int32, device="cuda"), torch.arange(n, dtype=torch.int32, device="cuda")[:, None])
+    k = torch.ones(n, 1, size, dtype=dtype, device="cuda")
+    for eps in (0.0, 1e-30, 1e-6, 1e30):
+        normed = oracle.norm(x, weight, eps)
+        want = oracle.turn(normed, pos, freq, [0] * len(freq), "halves")
+        tol = oracle.norm_tolerance(normed, want, freq, "halves", dtype) + normed.abs().amax(-1, keepdim=True) * 200 * 2.0 ** -51
+        for how in ("packed", "gaps", "odd"):
+            for got in (paged.norm_rope(laid_out(x, how), weight.cuda(), pos.cuda(), rope, eps), paged.append(pages, batch, k, k, rope=rope, pos=pos.cuda(), q=laid_out(x, how), q_norm=weight.cuda(), eps=eps)):
+                assert ((got.cpu().double() - want).abs() <= tol).all(), (eps, how, float(((got.cpu().double() - want).abs() - tol).max()))
+
+
 @pytest.mark.parametrize("dtype", [BF16, F16, F32], ids=str)
 @pytest.mark.parametrize("layout", ["halves", "pairs"])
 def test_elements_that_do_not_turn_pass_unchanged(paged, layout, dtype):
