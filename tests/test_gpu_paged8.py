@@ -309,6 +309,73 @@ def test_append_and_read(paged, case, how, form, dtype):
             assert torch.equal(new[1][first + i].cpu(), torch.zeros(kv, size) if p is None else got[1][p[0], p[1]].float() * got[3][p[0], p[1] // block][:, None])
 
 
+LONG = [  # (windows of several rows, queries in a kernel of their own) tokens held, rows, page, block, kv heads, group, size, rot, layout, prefix, weights of norms, entries that are no pages
+    ([900, 40, 0, 700, 333, 5, 500], [800, 60, 3, 700, 333, 5, 499], 32, 16, 2, 8, 64, 64, "halves", 20, "each", [(0, 20, -1)]), ([1200, 130], [1150, 77], 16, 4, 3, 2, 64, 24, "halves", 0, None, []),
+    ([2600, 77], [2433, 20], 64, 64, 1, 8, 128, 32, "pairs", 0, "all", []), ([1000] * 3, [990, 1000, 991], 48, 12, 2, 3, 96, 96, "halves", 7, "each", [(1, 0, 10 ** 6)]), ([1500, 9], [1400, 30], 8, 1, 2, 2, 33, 10, "halves", 0, "all", []),
+    ([3] * 500, [3, 2, 1, 5, 4] * 100, 16, 8, 4, 4, 128, 64, "halves", 0, "each", []), ([4000, 17], [3900, 17], 128, 128, 2, 2, 64, 16, "pairs", 0, None, []),
+]
+
+
+@pytest.mark.parametrize("form, dtype, how", [(INT8, BF16, "packed"), (E4M3, F16, "packed"), (E4M3, F32, "packed"), (INT8, F32, "odd")], ids=str)
+@pytest.mark.parametrize("case", LONG, ids=lambda c: f"{len(c[0])}x{sum(c[1])}-page{c[2]}-block{c[3]}-{c[4]}x{c[5]}x{c[6]}-rot{c[7]}{c[8]}")
+def test_append_of_many_rows(paged, case, how, form, dtype):
+    """blocks that begin before a window of rows and end behind it, starts inside a block, padding in front and rows behind; the attention that follows reads the same queries and codes as a later one"""
+    lens, counts, page, block, kv, group, size, rot, layout, prefix, norms, bad = case
+    m = Made(paged, len(lens) + size, dtype, form, lens, counts, page, block, kv, group, size, prefix, tail=5, empty=True, bad=bad)
+    g = gen(4)
+    k, v = ((torch.exp(torch.randn(m.n, kv, 1, generator=g)) * torch.randn(m.n, kv, size, generator=g)).to(dtype) for _ in range(2))
+    k_norm, q_norm = (None, None) if norms is None else (torch.randn(kv, size, generator=g), torch.randn(m.heads, size, generator=g)) if norms == "each" else (torch.randn(size, generator=g), torch.randn(size, generator=g))
+    rope = paged.RopeAxes.sections(rot, 10000.0, layout=layout)
+    freq, axis = [10000.0 ** (-2.0 * j / rot) for j in range(rot // 2)], [0] * (rot // 2)
+    (pages, batch), twin = m.on_gpu(), m.on_gpu()[0]
+    spans = oracle.spans(lens, m.rows, m.n)
+    where, index = [], torch.zeros(m.n, dtype=torch.int64)
+    for b, (first, c, have) in enumerate(spans):
+        index[first:first + c] = have - c + torch.arange(c)
+        where.append([None if p is None else (*p, have - c + i) for i in range(c) for p in [oracle.place(m.tables[b], len(m.k), page, have - c + i)]])
+    real, use = sum(c for _, c, _ in spans), (prefix + index).to(torch.int32)[None]
+    k_in, q_in = (oracle.norm(k, k_norm, 1e-5), oracle.norm(m.q, q_norm, 1e-5)) if norms else (k.double(), m.q.double())
+    k_want, q_want = oracle.turn(k_in, use, freq, axis, layout), oracle.turn(q_in, use, freq, axis, layout)
+    args = [laid_out(t, how) for t in (k, v, m.q)]
+    more = dict(k_norm=k_norm.cuda(), q_norm=q_norm.cuda(), eps=1e-5) if norms else {}
+    q_out = torch.full(m.q.shape, 7.0, dtype=dtype, device="cuda")
+    paged.append(pages, batch, args[0], args[1], rope=rope, q=args[2], q_out=q_out, **more)
+    attend = size % 16 == 0
+    at_once = paged.attention(pages, batch, q_out) if attend else None
+    torch.cuda.synchronize()
+    if attend:
+        assert torch.equal(paged.attention(pages, batch, q_out)[:real], at_once[:real])
+    got = [t.cpu() for t in (pages.k, pages.v, pages.k_scale, pages.v_scale)]
+    before = m.k.clone(), m.v.clone()
+    for codes, scales, x, off, left in ((m.k, m.ks, k_want, 2.0 ** -38, got[2]), (m.v, m.vs, v.double(), 0.0, got[3])):
+        for (first, c, _), w in zip(spans, where):
+            oracle.put(codes, scales, block, form, x[first:first + c], w, off, left)
+    if not norms:   # (keys' elements that pass are the inputs themselves: 24 bits over 24 bits, which 64 tell from the middle of two codes)
+        for (first, _, _), w in zip(spans, where):
+            for i, p in enumerate(w):
+                if p is not None:
+                    m.k[p[0], p[1], :, rot:] = oracle.nearest(k[first + i, :, rot:].double() / m.ks[p[0], p[1] // block][:, None], form)
+    for codes, left in ((m.k, got[0]), (m.v, got[1])):
+        left, sure = left.float().double(), ~torch.isnan(codes)
+        assert torch.equal(left[sure], codes[sure]), int((left != codes)[sure].sum())
+    assert sum(int((torch.isnan(codes) & ~torch.isnan(old)).sum()) for codes, old in zip((m.k, m.v), before)) <= 1
+    for scales, left in ((m.ks, got[2]), (m.vs, got[3])):
+        assert torch.equal(left.double().nan_to_num(-1.0), scales.nan_to_num(-1.0))
+    tol = oracle.norm_tolerance(q_in, q_want, freq, layout, dtype) + q_in.abs().amax(-1, keepdim=True) * 4100 * 2.0 ** -51
+    assert ((q_out.cpu().double() - q_want).abs() <= tol)[:real].all() and (q_out[real:] == 7.0).all()
+    # captured, over a pool as the first one was, with the queries in place: the same bits
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        paged.append(twin, batch, args[0], args[1], rope=rope, q=args[2], q_out=args[2], **more)
+        again = paged.attention(twin, batch, args[2]) if attend else None
+    graph.replay()
+    assert torch.equal(args[2][:real], q_out[:real])
+    for t, left in zip((twin.k, twin.v, twin.k_scale, twin.v_scale), got):
+        assert torch.equal(t.cpu().contiguous().view(torch.uint8), left.contiguous().view(torch.uint8))
+    if attend:
+        assert torch.equal(again[:real], at_once[:real])
+
+
 @pytest.mark.parametrize("form", [INT8, E4M3], ids=str)
 def test_token_by_token(paged, form):
     """a sequence that grows by single tokens: a block's scale is the largest so far, and codes follow it"""
