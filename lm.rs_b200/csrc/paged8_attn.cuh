@@ -5,8 +5,8 @@
 //     scores     are tensor-core products of the queries in float16 and the codes as they are, times k_j in float32
 //     weights    are w_j = 2^(s_j log2 e + log2 v_j - m): the values' scales go into the weights' exponents, m is the largest exponent (less 7), and the codes are multiplied as they are
 //     the sum    of e^(s_j) is that of w_j / v_j, in float32
-// The queries' types: float16 as it is; bfloat16, whose 8 bits of mantissa float16 has, times a power of two for each row that brings its largest element to 2^14 (what is below 2^-38 of that loses
-// bits: 2^-40 of the largest element at most); float32 the same way in three pieces of 11 bits each.  Weights in float16: up to 2^7, rounded by 2^-11 of each and 2^-32 of the largest; float32: in three pieces.
+// The queries' types: float16 as it is; bfloat16, whose 8 bits of mantissa float16 has, times a power of two for each row that brings its largest element to between 2^14 and 2^15 (float16's steps end at 2^-24: what
+// is below 2^-31 of that element loses bits, 2^-39 of it at most); float32 the same way in three pieces of 11 bits each (24 bits whole down to 2^-15 of the largest element, below that off by 2^-39 of it at most).  Weights in float16: up to 2^7, rounded by 2^-11 of each and 2^-32 of the largest; float32: in three pieces.
 #pragma once
 #include <float.h>
 
@@ -70,13 +70,13 @@ PG_DEVINL float2 value_terms(float v) {
     return make_float2(v == v ? lg : v, by);
 }
 
-// What bounds it: where the keys are many, the bytes of the pages, and close behind them issue slots (a warp spends some 800 instructions on 32 keys of 128 in int8, a third of them on making float16 of
-// codes); where they are few, the chain length - table - codes - scores - join.  Measured (B200): four sequences of up to 100,000 keys (520 MB of codes, 32/8 heads of 128, float16 rows, int8, a scale for each
+// What bounds it: where the keys are many, latency: 5.0 TB/s of 6.5 from memory and 2.0 instructions a cycle of 4 with 12 warps on an SM (a warp spends some 800 instructions on 32 keys of 128 in int8, a third of them
+// on making float16 of codes, and takes turns between waiting for the codes, 1.2 cycles an instruction, and for what it computes, 1.3); where they are few, the chain length - table - codes - scores - join.  Measured (B200): four sequences of up to 100,000 keys (520 MB of codes, 32/8 heads of 128, float16 rows, int8, a scale for each
 // token) 112 us, 4620 GB/s, and 105 with a scale for 32 tokens; one sequence of 1000 keys, heads of 64: 10.8 us with the join; float32 rows, 15 sequences behind a prefix of 4096, heads of 64: 28 us.
 // Steps, us for the first: tiles of 128 keys copied by all threads 16 bytes at a time 184; a warp its own keys by TMA 167; 8 rows as the products' columns (16 as their rows before) 136; boxes that ask the L2 for
 // no more than their own 128 bytes of each 1024 (of 256 before: the heads' codes lie side by side) 112.
 // CTA = 4 warps that share a tile's keys: a warp copies its own WARP_KEYS of them to its own slots, a tile or two ahead, and works on them by itself; the warps meet only where parts begin and end.  Codes
-// come by TMA, a piece of a page at a time, where all of a warp's keys are within the unit's (else, and where strides or pages take no tensor map, 16 bytes a lane, zeros for what is not there); scales 4 bytes a lane.
+// come by TMA, a piece of a page at a time (spills: with 16 rows 220 to 240 bytes a thread for 16-bit heads of 128, 150 to 165 for 256), where all of a warp's keys are within the unit's (else, and where strides or pages take no tensor map, 16 bytes a lane, zeros for what is not there); scales 4 bytes a lane.
 template <typename T, int DP, int ROW_TILES> struct TileShape8 {
     static constexpr int PIECES = sizeof(T) == 4 ? 3 : 1;   // of queries and weights
     static constexpr int ROWS = 8 * ROW_TILES, WARPS = 4, THREADS = 32 * WARPS, CHUNKS = DP / 16, WARP_KEYS = DP <= 128 ? 32 : 16, KEYS = WARPS * WARP_KEYS, STAGES = 2;

@@ -11,7 +11,8 @@ namespace paged {
 // the sum of its squares takes a few exchanges.  Eight elements are four pairs that turn (two times four neighbours in halves, eight in pairs) or eight that do not, so that all lanes have the same to do.
 // Where arrays do not lie on the boundaries that this wants, or sizes are no multiples of eight, a general walk takes the elements of a head one at a time, 32 apart.
 // Two elements an instruction (f32x2) wherever there is one for it: instructions bound these kernels next to the bytes.
-// Measured (B200): 4099 rows of 40 bf16 heads of 128 with weights of their own, 84 MB: 21.0 us, 4010 GB/s (by pieces of 16 bytes and with a root and a quotient 28.6; two heads ahead instead of four 26.3); one row 2.6 us.
+// Measured (B200): 4099 rows of 40 bf16 heads of 128 with weights of their own, 84 MB: 21.4 us, 3920 GB/s, 2.6 instructions a cycle of 4 (21.0 where
+// lanes that do not turn multiply all the same; by pieces of 16 bytes and with a root and a quotient 28.6; two heads ahead instead of four 26.3); one row 2.6 us.
 struct HeadNorm {
     const float* weight;   // null: 1
     int64_t head;          // from one head's weights to the next's (0: all heads share them)
@@ -219,9 +220,11 @@ __global__ void __launch_bounds__(32 * ROW_WARPS) norm_rope_kernel(const __grid_
 // mean 2 u, halved by the root; the root's approximation 4 u; two products), after its rotation by 19 u (|a| + |b|) of its pair (cosines 3 u, two products and a sum), which is 27 u of the turned pair's sizes, and by 5 u (7 u) without a norm; PUT_OFF is 32 u, PUT_OFF_TURN
 // 10 u.  An element so near to a border between two codes is computed again in
 // 64 bits (head64; one head of eight has one), and so are the tokens whose largest element is within 2^-17 of the block's largest.  Inputs that 32 bits would overflow on go that way altogether.
-// What bounds it: the chain row - sequence - length - table - input of a block, with 16 warps on an SM (128 registers: 16 tokens of a head), and the instructions of what is near a border.  Measured (B200): 11,805
-// rows of 24 prompts, 32 query and 8 KV heads of 128, norms, half the columns turned, a scale for 16 tokens, 290 MB with the queries: int8 178 us (keys and values alone 118, without norm and rotation 58), e4m3 214;
-// a scale for each token 341; one row 6.3 us, one of each of 61 sequences 10.2.  All of it in 64 bits, a warp a token and head: 391.
+// What bounds it: the chain row - sequence - length - table - input of a block, with 16 warps on an SM (128 registers: 16 tokens of a head), the instructions of what is near a border, and fetching them (of some 9 cycles
+// that a warp waits for an instruction, 3.7 go by until it has been fetched; 1.3 a cycle of 4).  Measured (B200): 11,805
+// rows of 24 prompts, 32 query and 8 KV heads of 128, norms, half the columns turned, a scale for 16 tokens, 290 MB with the queries: int8 185 us (keys and values alone 125, without norm and rotation 72), e4m3 213
+// (155, 81); a scale for each token 341; one row of 32 and 8 heads of 64 7.4 us, one of each of 64 sequences 10.  All of it in 64 bits, a warp a token and head: 391.
+// Spills: the kernels for few tokens, with 64 registers, put 148 to 268 bytes a thread away; those of longer blocks for heads beyond 64, with 128, 776 to 916 in float32 and 200 to 284 in 16 bits.
 constexpr int PUT_WARPS = 8, PUT_TOKENS = 16;   // warps of a CTA, tokens whose angles it holds at a time
 constexpr float PUT_OFF = 0x1p-19f, PUT_OFF_TURN = 10.0f * 0x1p-24f;
 
@@ -792,7 +795,9 @@ __global__ void __launch_bounds__(32 * PUT_WARPS, Put::CTAS) paged8_append_kerne
 }
 
 // ---- reading back ----------------------------------------------------------------------------------------------------------------------------
-// code * scale in float32 (exact to half a step), rounded to the type.  What bounds it is the bytes: 74,000 tokens of 8 heads of 128 in e4m3 to bf16, 560 MB, 115 us, 4830 GB/s (B200).  A warp a row; its lanes take 16 codes each (one, where something does not lie on 16-byte boundaries).
+// code * scale in float32 (exact to half a step), rounded to the type.  A warp a row; its lanes take 16 codes each (one, where something does not lie on 16-byte boundaries).
+// 74,000 tokens of 8 heads of 128 in e4m3 to bf16, 560 MB: 115 us, 4830 GB/s (B200).  What bounds it is latency: a lane has one piece on its way at a time, and of 11 cycles that a warp waits for an instruction 7.7 are for
+// memory (2.3 instructions a cycle of 4).
 template <typename T> struct ReadParams {
     Batch batch;
     Pages8 pages;
