@@ -2,6 +2,7 @@
 products all arrive, so they are compiled into a program whose waits can be told that they have waited long enough."""
 import os
 import subprocess
+import sys
 
 import pytest
 
@@ -41,3 +42,32 @@ def test_a_wait_that_runs_out(program, case, waits):
         assert said == "1" and "results of an earlier call are NaN: " + kernel in words and words.endswith(f" gave up waiting for {WAITS[what & 255]} (device status {what})")
         assert f"NaN: {kernel} gave up" in words   # (paged_attention, which reads the same word, says it in the same words)
         assert after == "0" and same == "1"   # (said once)
+
+
+FIRST = """
+import sys; sys.path.insert(0, sys.argv[1])
+import torch
+from lmrs_b200 import paged
+g = torch.Generator("cuda"); g.manual_seed(1)
+i32 = dict(dtype=torch.int32, device="cuda")
+rows = int(sys.argv[2])
+k, v, q = (torch.randn(rows, h, 64, generator=g, device="cuda").half() for h in (2, 2, 8))
+pool = torch.zeros(8, 64, 2, 64, dtype=torch.int8, device="cuda")
+pages = paged.QuantPages(pool, pool.clone(), torch.ones(8, 4, 2, device="cuda"), torch.ones(8, 4, 2, device="cuda"))
+batch = paged.Batch(torch.tensor([rows], **i32), torch.arange(8, **i32)[None], rows=torch.tensor([0, rows], **i32), max_rows=rows)
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    paged.append(pages, batch, k, v)
+    out = paged.attention(pages, batch, q)
+out.fill_(9.0)
+graph.replay()
+assert torch.equal(out, paged.attention(pages, batch, q)) and not (out == 9.0).all()
+print("ok")
+"""
+
+
+@pytest.mark.parametrize("rows", [3, 300])
+def test_a_process_whose_first_call_is_captured(rows):
+    """(either kernel needs the word that it may say something in)"""
+    lib = os.path.join(os.path.dirname(HERE), "lm.rs_b200")
+    assert subprocess.run([sys.executable, "-c", FIRST, lib, str(rows)], check=True, capture_output=True, text=True, timeout=200).stdout.strip() == "ok"
