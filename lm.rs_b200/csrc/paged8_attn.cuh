@@ -6,7 +6,7 @@
 //     weights    are w_j = 2^(s_j log2 e + log2 v_j - m): the values' scales go into the weights' exponents, m is the largest exponent (less 7), and the codes are multiplied as they are
 //     the sum    of e^(s_j) is that of w_j / v_j, in float32
 // The queries' types: float16 as it is; bfloat16, whose 8 bits of mantissa float16 has, times a power of two for each row that brings its largest element to between 2^14 and 2^15 (float16's steps end at 2^-24: what
-// is below 2^-31 of that element loses bits, 2^-39 of it at most); float32 the same way in three pieces of 11 bits each (24 bits whole down to 2^-15 of the largest element, below that off by 2^-39 of it at most).  Weights in float16: up to 2^7, rounded by 2^-11 of each and 2^-32 of the largest; float32: in three pieces.
+// is below 2^-31 of that element loses bits, 2^-39 of it at most); float32 the same way in three pieces of 11 bits each (24 bits whole down to 2^-15 of the largest element, below that off by 2^-39 of it at most).  Weights in float16: a row's largest 2^7 to 2^15, rounded by 2^-11 of each and 2^-32 of the largest; float32: in three pieces.
 #pragma once
 #include <float.h>
 

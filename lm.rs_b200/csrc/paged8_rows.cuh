@@ -64,7 +64,7 @@ PG_DEVINL void load_weights8(const float* w, const EightAt& at, Eight& to) {
     const ulonglong2 a = *reinterpret_cast<const ulonglong2*>(w + at.first), b = *reinterpret_cast<const ulonglong2*>(w + at.second);
     to.v[0] = a.x; to.v[1] = a.y; to.v[2] = b.x; to.v[3] = b.y;
 }
-// (of a lane that does not turn: times a cosine of 1 and a sine of 0, by which an infinity makes NaN of the element beside it)
+// (With the cosine of 1 and the sine of 0 that a lane has which does not turn, an infinity makes NaN of the element beside it)
 PG_DEVINL void turn8(Eight& x, const Turns& t, int c, bool zipped) {
     const ulonglong2 cs = *reinterpret_cast<const ulonglong2*>(t.c + 4 * c), sn = *reinterpret_cast<const ulonglong2*>(t.s + 4 * c);
     const uint64_t minus = 0x8000000080000000ull;

@@ -9,7 +9,7 @@
 // A thread's score of a key is its dot product times the key's scale; its weight carries the value's scale; both scales come from shared memory, four keys a load.
 // Measured on a B200, us: 244 rows of a KV head behind 8200 keys, 8 KV heads of 128, e4m3: 39 (and 80 with the own keys and the join); 12 prompts behind 2050, heads of 256, capped: 306, and 42 for the join.
 // What bounds it: of the 1.7 us that a tile of 64 keys and 256 rows takes, 1.05 go by between a copying warp's conversions (0.7 of them on places, scales and boxes of the next operand: dependent instructions of
-// one warp), 0.65 for one; the rows' warps need 0.95, the products 0.3 (the tensor pipe is active for 11 % of the first of these, 16 % of the second).  A part costs some 5 us besides: its queries, its first tile, its sums.
+// one warp), 0.65 for one; the rows' warps need 0.95, the products 0.3 (the tensor pipe is active for 11 % of the prefix' time, 16 % of the prompts').  A part costs some 5 us besides: its queries, its first tile, its sums.
 // Steps, us for the prompts without / with a cap: all rows' queries a row a thread 399 / 492; four copying warps for heads of 256 363 / 454; queries eight lanes a row 314 / 469; caps and masks in loops
 // (unrolled, their code pushes the other roles' out of the instruction cache) 314 / 348.  13 warps, so that keys and values have two each: 128 registers a thread, no faster; taken back.
 #pragma once
